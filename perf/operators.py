@@ -180,7 +180,7 @@ def prepare(case, seed):
         st["cache"] = KVCache(st["k_pages"], st["v_pages"])
         st["batch"] = KVBatch(st["kv_len"], st["table"], st["row_off"])
         if case["op"] == "decode":
-            st["space"] = _handle.attention_paged_workspace(st["cache"], n, heads)
+            st["space"] = _handle.attention_paged_workspace(st["cache"], heads)
     return st
 
 
