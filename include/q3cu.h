@@ -21,8 +21,8 @@
  *   - Every entry point returns a q3cu_status; none exits or throws.  The
  *     message of the last failure on the calling thread is available from
  *     q3cu_last_error_string().
- *   - Errors found on the device (an out-of-range token id, a wait that gave
- *     up) set bits in a per-context status word and skip the affected row;
+ *   - Errors found on the device (an out-of-range token or page id, a wait that
+ *     gave up) set bits in a per-context status word and skip the affected row;
  *     q3cu_device_status() synchronises the stream and returns and clears
  *     them.
  *   - Q8_0 tensors are two arrays, as QuantizedTensor in
@@ -49,7 +49,7 @@ typedef enum {
     Q3CU_ERR_ALIGN = 2,      /* a pointer or row is not aligned as required             */
     Q3CU_ERR_GROUP = 3,      /* a Q8_0 length is not a multiple of the group size (64)  */
     Q3CU_ERR_CUDA = 4,       /* a CUDA runtime call failed                              */
-    Q3CU_ERR_INDEX = 5,      /* device status: a token id was out of range              */
+    Q3CU_ERR_INDEX = 5,      /* device status: a token or page id was out of range      */
     Q3CU_ERR_TIMEOUT = 6,    /* device status: a bounded wait gave up                   */
     Q3CU_ERR_NOT_INIT = 7,   /* NULL or destroyed context                               */
     Q3CU_ERR_OOM = 8,        /* device or host allocation failed                        */
@@ -187,6 +187,89 @@ q3cu_status q3cu_matmul_q8(q3cu_ctx *ctx, const int8_t *xq, const float *xs, int
 q3cu_status q3cu_attention(q3cu_ctx *ctx, const float *q, const float *key_cache, const float *value_cache,
                            int pos, int n_heads, int kv_dim, int kv_mul, float *att, int att_stride, float *probs,
                            float *xb, q3cu_stream stream);
+
+/* ---- a paged key-value cache shared by many sequences ---------------------
+ * No counterpart in the reference, whose cache holds one sequence
+ * (qwen3_original.c:403-404).  A cache is a pool of pages; a page holds
+ * page_size consecutive positions of one sequence, and a table row per
+ * sequence says which page holds its positions i * page_size ... .  Three
+ * operators work on one layer's cache and one description of a batch:
+ * append the batch's new token rows, then attend to the cache from the rows of
+ * prompts, or from one new token per sequence. */
+typedef struct {
+    void *k, *v;             /* pages of [n_kv][page_size][head_dim], 16-byte aligned (device) */
+    int64_t page_stride;     /* elements between the starts of two pages, of k and of v: at least
+                                n_kv * page_size * head_dim, and a multiple of 8 */
+    int32_t n_pages, n_kv;
+    int32_t page_size;       /* 16, 32, 64, 128 or 256 */
+    int32_t head_dim;        /* 128 */
+    int32_t dtype;           /* q3cu_dtype of k and v */
+} q3cu_kv_cache;
+
+/* The packed token rows of n_seqs sequences.  Sequence s owns rows row_off[s]
+ * .. row_off[s+1]-1, the last of which is at position kv_len[s] - 1: kv_len
+ * counts the sequence's positions with the new rows.  Rows at or behind
+ * row_off[n_seqs] belong to no sequence and are left as they are.  A row whose
+ * position would be negative is padding: nothing is appended for it, and its
+ * attention is zero.  All three arrays are device memory, read when the
+ * kernels run.  pages[s][i] is the page of positions i * page_size ...;
+ * entries beyond the last position are not read. */
+typedef struct {
+    const int32_t *row_off;  /* [n_seqs + 1], rising from 0 (not read by q3cu_attention_paged) */
+    const int32_t *kv_len;   /* [n_seqs] */
+    const int32_t *pages;    /* [n_seqs][max_pages] */
+    int32_t n_seqs, max_pages;   /* max_pages * page_size < 2^31 */
+} q3cu_kv_batch;
+
+/* QK-RMSNorm and rotation of the packed rows, keys and values into the cache
+ * (the per-head operation of qwen3_original.c:361-393, for many rows).  q: [rows][n_heads][128] with q_stride elements
+ * between rows, k and v: [rows][n_kv][128] with kv_stride, all of `dtype`
+ * (one fused projection's output may hold all three).  q_norm, k_norm: [128]
+ * f32, or NULL for the rotation alone.  q_out: [rows][n_heads][128] of
+ * q_dtype; it may be q itself when the types agree and q_stride is
+ * n_heads * 128.  n_heads 0 (q, q_out NULL) appends keys and values only.
+ * The angle pos * theta^(-j/64) is formed in binary64: unlike
+ * q3cu_qk_norm_rope, which keeps the reference's binary32 product, it is exact
+ * at far positions.  Pointers 16-byte aligned, strides multiples of 16 bytes.
+ * A page id outside the cache, or a position beyond the table, sets
+ * Q3CU_DEV_BAD_INDEX and stores nothing for that row's keys and values. Two
+ * rows of a call must not fall on the same page slot. */
+q3cu_status q3cu_kv_append(q3cu_ctx *ctx, const q3cu_kv_cache *cache, const q3cu_kv_batch *batch, int64_t rows,
+                           const void *q, const void *k, const void *v, q3cu_dtype dtype, int64_t q_stride,
+                           int64_t kv_stride, int n_heads, const float *q_norm, const float *k_norm, float theta,
+                           float eps, void *q_out, q3cu_dtype q_dtype, q3cu_stream stream);
+
+/* Attention of one new token per sequence: row s of q ([n_seqs][n_heads][128]
+ * of `dtype`, q_stride elements between rows) over positions 0..kv_len[s]-1 of
+ * sequence s; query head h reads kv head h / (n_heads / n_kv), at most 16
+ * query heads to a kv head.  Scores are scaled by 1/sqrt(128); the softmax is
+ * the usual one (its maximum is the row's, where q3cu_softmax_rows' starts at
+ * 0).  out: [n_seqs][n_heads][128] of `dtype`, other memory than q; zeros where kv_len is 0.  Any
+ * mix of `dtype` and the cache's type; sums are binary32.  The caller's `work`
+ * (device, 16-byte aligned, q3cu_attention_paged_workspace bytes, contents
+ * irrelevant) holds partial results during the call: calls that may run at the
+ * same time need one each.  What a page holds beyond a sequence's last
+ * position is never used, NaN included.  A page id outside the cache sets
+ * Q3CU_DEV_BAD_INDEX and reads as zeros; a kv_len beyond the table sets it and
+ * is cut. */
+q3cu_status q3cu_attention_paged(q3cu_ctx *ctx, const q3cu_kv_cache *cache, const q3cu_kv_batch *batch,
+                                 const void *q, q3cu_dtype dtype, int64_t q_stride, int n_heads, void *work,
+                                 size_t work_bytes, void *out, q3cu_stream stream);
+/* Bytes of `work` for the head counts, any batch. */
+q3cu_status q3cu_attention_paged_workspace(q3cu_ctx *ctx, int n_heads, int n_kv, size_t *bytes);
+
+/* Causal attention of packed prompt rows over the cache, which holds their
+ * keys and values already (q3cu_kv_append): a row at position p over positions
+ * 0..p.  A whole prompt has kv_len equal to its rows; a chunk behind a cached
+ * prefix has more.  q: [rows][n_heads][128] with q_stride elements between
+ * rows; out: [rows][n_heads][128], other memory than q.  Both of the cache's type: bf16 runs on the tensor cores with
+ * probabilities rounded to bf16 (the sums binary32), f32 throughout in
+ * binary32.  Grouped heads, scale, softmax, empty rows, unused page space, bad
+ * pages and alignment as above.  Sequences with one row are allowed, but
+ * q3cu_attention_paged is made for them. */
+q3cu_status q3cu_attention_prompt(q3cu_ctx *ctx, const q3cu_kv_cache *cache, const q3cu_kv_batch *batch,
+                                  int64_t rows, const void *q, q3cu_dtype dtype, int64_t q_stride, int n_heads,
+                                  void *out, q3cu_stream stream);
 
 /* ---- a checkpoint on the device and its decode step --------------------- */
 typedef struct q3cu_model q3cu_model;

@@ -32,6 +32,8 @@ struct q3cu_ctx {
     void *d_scratch = nullptr;              // staging for the host-pointer wrappers
     size_t scratch_bytes = 0;
     std::map<std::pair<int, uint32_t>, q3::InvFreq> inv_freq;   // (head_dim, bits of theta)
+    float turn_theta = 0.0f;                                    // the theta turn_freq was made for (0: none)
+    q3::TurnFreq turn_freq{};
     bool alive = false;
 };
 
@@ -94,6 +96,14 @@ const q3::InvFreq &inv_freq_for(q3cu_ctx *ctx, int head_dim, float theta) {
     const int half = head_dim / 2;
     for (int j = 0; j < half && j < 64; ++j) f.v[j] = powf(theta, -(float)j / half);
     return ctx->inv_freq.emplace(key, f).first->second;
+}
+
+// theta^(-j/64) / (2 pi): a position times it is the rotation's angle in turns.
+const q3::TurnFreq &turn_freq_for(q3cu_ctx *ctx, float theta) {
+    if (ctx->turn_theta != theta)
+        for (int j = 0; j < 64; ++j) ctx->turn_freq.v[j] = std::pow(double(theta), -j / 64.0) / 6.283185307179586476925;
+    ctx->turn_theta = theta;
+    return ctx->turn_freq;
 }
 
 // The softmax kernel balances rows across SMs with a pair of device counters
@@ -268,7 +278,7 @@ q3cu_status q3cu_device_status(q3cu_ctx *ctx, q3cu_stream stream, uint32_t *flag
     if (e != cudaSuccess) return cuda_fail(e, "reading the device status word");
     if (flags) *flags = h;
     if (h & Q3CU_DEV_TIMEOUT) return fail(Q3CU_ERR_TIMEOUT, "a device-side wait gave up (status 0x%x)", h);
-    if (h & Q3CU_DEV_BAD_INDEX) return fail(Q3CU_ERR_INDEX, "a token id was out of range (status 0x%x)", h);
+    if (h & Q3CU_DEV_BAD_INDEX) return fail(Q3CU_ERR_INDEX, "a token or page id was out of range (status 0x%x)", h);
     return Q3CU_OK;
 }
 
@@ -470,6 +480,146 @@ q3cu_status q3cu_attention(q3cu_ctx *ctx, const float *q, const float *key_cache
     return launched(q3::launch_attention_rows(q, key_cache, value_cache, att, probs, xb, pos, n_heads, kv_dim, kv_mul,
                                               att_stride, static_cast<cudaStream_t>(stream), ctx->sms),
                     "attention launch");
+}
+
+// ---------------------------------------------------------------------------
+// the paged key-value cache
+// ---------------------------------------------------------------------------
+
+// Checks the descriptors and copies them into the kernels' form.
+static q3cu_status check_paged(const char *op, const q3cu_kv_cache *cache, const q3cu_kv_batch *batch, int n_heads,
+                               bool with_rows, q3::PagedKV &c, q3::PagedSeqs &b) {
+    if (!cache || !batch) return fail(Q3CU_ERR_INVALID, "%s: cache or batch is NULL", op);
+    if (q3cu_status st = check_dtype(q3cu_dtype(cache->dtype))) return st;
+    if (cache->head_dim != q3::PAGED_HD)
+        return fail(Q3CU_ERR_INVALID, "%s: head_dim %d: only 128 is supported", op, cache->head_dim);
+    int shift = 4;
+    while (shift < 8 && (1 << shift) != cache->page_size) ++shift;
+    if ((1 << shift) != cache->page_size)
+        return fail(Q3CU_ERR_INVALID, "%s: page_size %d is not 16, 32, 64, 128 or 256", op, cache->page_size);
+    if (cache->n_kv <= 0 || cache->n_pages <= 0 || batch->n_seqs < 0 || batch->max_pages < 0)
+        return fail(Q3CU_ERR_INVALID, "%s: n_kv=%d n_pages=%d n_seqs=%d max_pages=%d", op, cache->n_kv,
+                    cache->n_pages, batch->n_seqs, batch->max_pages);
+    if (n_heads < 0 || n_heads % cache->n_kv || n_heads / cache->n_kv > q3::PAGED_GROUP_MAX)
+        return fail(Q3CU_ERR_INVALID, "%s: n_heads %d is not a multiple of n_kv %d up to 16 times it", op, n_heads,
+                    cache->n_kv);
+    if (int64_t(batch->max_pages) * cache->page_size > INT32_MAX)
+        return fail(Q3CU_ERR_INVALID, "%s: max_pages %d * page_size %d does not fit 31 bits", op, batch->max_pages,
+                    cache->page_size);
+    const int64_t dense = int64_t(cache->n_kv) * cache->page_size * q3::PAGED_HD;
+    if (cache->page_stride < dense || cache->page_stride > (int64_t(1) << 36))
+        return fail(Q3CU_ERR_INVALID, "%s: page_stride %lld, a page has %lld elements", op,
+                    (long long)cache->page_stride, (long long)dense);
+    if (cache->page_stride % 8)
+        return fail(Q3CU_ERR_ALIGN, "%s: page_stride must be a multiple of 8 elements", op);
+    if (!cache->k || !cache->v) return fail(Q3CU_ERR_INVALID, "%s: cache pointer is NULL", op);
+    if (!aligned(cache->k, 16) || !aligned(cache->v, 16))
+        return fail(Q3CU_ERR_ALIGN, "%s: cache pages must be 16-byte aligned", op);
+    if (batch->n_seqs > 0 && ((with_rows && !batch->row_off) || !batch->kv_len || (batch->max_pages > 0 && !batch->pages)))
+        return fail(Q3CU_ERR_INVALID, "%s: batch pointer is NULL", op);
+    if (!aligned(batch->row_off, 4) || !aligned(batch->kv_len, 4) || !aligned(batch->pages, 4))
+        return fail(Q3CU_ERR_ALIGN, "%s: batch arrays must be 4-byte aligned", op);
+    c = {cache->k, cache->v, cache->page_stride, cache->n_pages, cache->n_kv, shift};
+    b = {batch->row_off, batch->kv_len, batch->pages, batch->n_seqs, batch->max_pages};
+    return Q3CU_OK;
+}
+
+// Rows of `heads` heads, `stride` elements apart.
+static q3cu_status check_rows(const char *op, const char *name, const void *p, q3cu_dtype dt, int64_t stride,
+                              int64_t heads) {
+    if (!p) return fail(Q3CU_ERR_INVALID, "%s: %s is NULL", op, name);
+    if (stride < heads * q3::PAGED_HD || stride > (int64_t(1) << 32))
+        return fail(Q3CU_ERR_INVALID, "%s: %s rows of %lld elements are %lld apart", op, name,
+                    (long long)(heads * q3::PAGED_HD), (long long)stride);
+    if (!aligned(p, 16) || (size_t(stride) * esize(dt)) % 16)
+        return fail(Q3CU_ERR_ALIGN, "%s: %s must be 16-byte aligned, its row stride a multiple of 16 bytes", op, name);
+    return Q3CU_OK;
+}
+
+q3cu_status q3cu_kv_append(q3cu_ctx *ctx, const q3cu_kv_cache *cache, const q3cu_kv_batch *batch, int64_t rows,
+                           const void *q, const void *k, const void *v, q3cu_dtype dtype, int64_t q_stride,
+                           int64_t kv_stride, int n_heads, const float *q_norm, const float *k_norm, float theta,
+                           float eps, void *q_out, q3cu_dtype q_dtype, q3cu_stream stream) {
+    CHECK_CTX(ctx);
+    q3::PagedKV c;
+    q3::PagedSeqs b;
+    if (q3cu_status st = check_paged("kv_append", cache, batch, n_heads, true, c, b)) return st;
+    if (q3cu_status st = check_dtype(dtype)) return st;
+    if (q3cu_status st = check_dtype(q_dtype)) return st;
+    if (rows < 0 || rows > INT32_MAX / (n_heads + 2 * int64_t(c.n_kv)))
+        return fail(Q3CU_ERR_INVALID, "kv_append: rows %lld", (long long)rows);
+    if (!(theta > 0.0f) || std::isinf(theta)) return fail(Q3CU_ERR_INVALID, "kv_append: theta must be positive");
+    if (rows == 0 || b.n_seqs == 0) return Q3CU_OK;
+    if (n_heads > 0) {
+        if (q3cu_status st = check_rows("kv_append", "q", q, dtype, q_stride, n_heads)) return st;
+        if (q3cu_status st = check_rows("kv_append", "q_out", q_out, q_dtype, int64_t(n_heads) * q3::PAGED_HD, n_heads))
+            return st;
+        if (q_out == q && (q_dtype != dtype || q_stride != int64_t(n_heads) * q3::PAGED_HD))
+            return fail(Q3CU_ERR_INVALID, "kv_append: q_out may be q only with its type and dense rows");
+    }
+    if (q3cu_status st = check_rows("kv_append", "k", k, dtype, kv_stride, c.n_kv)) return st;
+    if (q3cu_status st = check_rows("kv_append", "v", v, dtype, kv_stride, c.n_kv)) return st;
+    if (!aligned(q_norm, 16) || !aligned(k_norm, 16))
+        return fail(Q3CU_ERR_ALIGN, "kv_append: norm weights must be 16-byte aligned");
+    if (q3cu_status st = use_device(ctx)) return st;
+    return launched(q3::launch_kv_append(c, q3cu_dtype(cache->dtype), b, rows, q, k, v, dtype, q_stride, kv_stride,
+                                         n_heads, q_norm, k_norm, turn_freq_for(ctx, theta), eps, q_out, q_dtype,
+                                         ctx->d_status, static_cast<cudaStream_t>(stream)),
+                    "kv_append launch");
+}
+
+q3cu_status q3cu_attention_paged_workspace(q3cu_ctx *ctx, int n_heads, int n_kv, size_t *bytes) {
+    CHECK_CTX(ctx);
+    if (!bytes || n_kv <= 0 || n_heads <= 0 || n_heads % n_kv || n_heads / n_kv > q3::PAGED_GROUP_MAX)
+        return fail(Q3CU_ERR_INVALID, "attention_paged_workspace: n_heads %d, n_kv %d", n_heads, n_kv);
+    *bytes = q3::attention_paged_workspace(n_heads, n_kv, ctx->sms);
+    return Q3CU_OK;
+}
+
+q3cu_status q3cu_attention_paged(q3cu_ctx *ctx, const q3cu_kv_cache *cache, const q3cu_kv_batch *batch, const void *q,
+                                 q3cu_dtype dtype, int64_t q_stride, int n_heads, void *work, size_t work_bytes,
+                                 void *out, q3cu_stream stream) {
+    CHECK_CTX(ctx);
+    q3::PagedKV c;
+    q3::PagedSeqs b;
+    if (q3cu_status st = check_paged("attention_paged", cache, batch, n_heads, false, c, b)) return st;
+    if (q3cu_status st = check_dtype(dtype)) return st;
+    if (n_heads == 0) return fail(Q3CU_ERR_INVALID, "attention_paged: n_heads is 0");
+    if (b.n_seqs > INT32_MAX / n_heads) return fail(Q3CU_ERR_INVALID, "attention_paged: n_seqs %d", b.n_seqs);
+    if (b.n_seqs == 0) return Q3CU_OK;
+    if (q3cu_status st = check_rows("attention_paged", "q", q, dtype, q_stride, n_heads)) return st;
+    if (q3cu_status st = check_rows("attention_paged", "out", out, dtype, int64_t(n_heads) * q3::PAGED_HD, n_heads)) return st;
+    if (out == q) return fail(Q3CU_ERR_INVALID, "attention_paged: out must be other memory than q");
+    const size_t need = q3::attention_paged_workspace(n_heads, c.n_kv, ctx->sms);
+    if (!work || work_bytes < need)
+        return fail(Q3CU_ERR_INVALID, "attention_paged: work of %zu bytes, need %zu", work ? work_bytes : size_t(0), need);
+    if (!aligned(work, 16)) return fail(Q3CU_ERR_ALIGN, "attention_paged: work must be 16-byte aligned");
+    if (q3cu_status st = use_device(ctx)) return st;
+    return launched(q3::launch_attention_paged(c, q3cu_dtype(cache->dtype), b, q, dtype, q_stride, n_heads, work, out,
+                                               ctx->d_status, static_cast<cudaStream_t>(stream), ctx->sms),
+                    "attention_paged launch");
+}
+
+q3cu_status q3cu_attention_prompt(q3cu_ctx *ctx, const q3cu_kv_cache *cache, const q3cu_kv_batch *batch, int64_t rows,
+                                  const void *q, q3cu_dtype dtype, int64_t q_stride, int n_heads, void *out,
+                                  q3cu_stream stream) {
+    CHECK_CTX(ctx);
+    q3::PagedKV c;
+    q3::PagedSeqs b;
+    if (q3cu_status st = check_paged("attention_prompt", cache, batch, n_heads, true, c, b)) return st;
+    if (q3cu_status st = check_dtype(dtype)) return st;
+    if (cache->dtype != dtype) return fail(Q3CU_ERR_INVALID, "attention_prompt: q and the cache differ in type");
+    if (n_heads == 0) return fail(Q3CU_ERR_INVALID, "attention_prompt: n_heads is 0");
+    if (rows < 0 || rows > INT32_MAX / n_heads)
+        return fail(Q3CU_ERR_INVALID, "attention_prompt: rows %lld", (long long)rows);
+    if (rows == 0 || b.n_seqs == 0) return Q3CU_OK;
+    if (q3cu_status st = check_rows("attention_prompt", "q", q, dtype, q_stride, n_heads)) return st;
+    if (q3cu_status st = check_rows("attention_prompt", "out", out, dtype, int64_t(n_heads) * q3::PAGED_HD, n_heads)) return st;
+    if (out == q) return fail(Q3CU_ERR_INVALID, "attention_prompt: out must be other memory than q");
+    if (q3cu_status st = use_device(ctx)) return st;
+    return launched(q3::launch_attention_prompt(c, b, rows, q, dtype, q_stride, n_heads, out, ctx->d_status,
+                                                static_cast<cudaStream_t>(stream), ctx->sms),
+                    "attention_prompt launch");
 }
 
 // ---------------------------------------------------------------------------

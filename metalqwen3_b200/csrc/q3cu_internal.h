@@ -131,6 +131,33 @@ cudaError_t launch_attention_rows(const float *q, const float *kc, const float *
                                   int pos, int n_heads, int kv_dim, int kv_mul, int att_stride, cudaStream_t stream,
                                   int sms);
 
+// ---- the paged key-value cache (k_append.cu, k_paged.cu, k_prompt.cu) ----
+constexpr int PAGED_HD = 128;          // head_dim
+constexpr int PAGED_GROUP_MAX = 16;    // query heads to a kv head
+struct PagedKV {                       // q3cu_kv_cache, checked
+    void *k, *v;
+    int64_t page_stride;               // elements
+    int n_pages, n_kv, page_shift;     // page_size = 1 << page_shift
+};
+struct PagedSeqs {                     // q3cu_kv_batch
+    const int32_t *row_off, *kv_len, *pages;
+    int n_seqs, max_pages;
+};
+struct TurnFreq { double v[64]; };     // theta^(-j/64) / (2 pi)
+cudaError_t launch_kv_append(const PagedKV &c, q3cu_dtype cache_dt, const PagedSeqs &b, int64_t rows, const void *q,
+                             const void *k, const void *v, q3cu_dtype dt, int64_t q_stride, int64_t kv_stride,
+                             int n_heads, const float *q_norm, const float *k_norm, const TurnFreq &freq, float eps,
+                             void *q_out, q3cu_dtype q_dt, uint32_t *status, cudaStream_t stream);
+// One query row per sequence (row s of q: sequence s) over its kv_len keys.
+size_t attention_paged_workspace(int n_heads, int n_kv, int sms);
+cudaError_t launch_attention_paged(const PagedKV &c, q3cu_dtype cache_dt, const PagedSeqs &b, const void *q,
+                                   q3cu_dtype dt, int64_t q_stride, int n_heads, void *work, void *out,
+                                   uint32_t *status, cudaStream_t stream, int sms);
+// Packed query rows, causal: a row at position p over the keys 0..p.
+cudaError_t launch_attention_prompt(const PagedKV &c, const PagedSeqs &b, int64_t rows, const void *q, q3cu_dtype dt,
+                                    int64_t q_stride, int n_heads, void *out, uint32_t *status, cudaStream_t stream,
+                                    int sms);
+
 cudaError_t launch_swiglu(const void *hb, const void *hb2, q3cu_dtype dt, int64_t elems, void *out, int8_t *q,
                           float *s, uint32_t *status, cudaStream_t stream, int sms);
 

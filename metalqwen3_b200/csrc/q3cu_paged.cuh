@@ -1,0 +1,137 @@
+// q3cu_paged.cuh -- the paged key-value cache as the kernels see it: where a
+// position's row lies, and which sequence a packed token row belongs to.
+#pragma once
+
+#include "q3cu_device.cuh"
+#include "q3cu_internal.h"
+
+namespace q3 {
+
+constexpr int HD = PAGED_HD;
+
+template <typename T> struct Elem;
+template <> struct Elem<float> {
+    typedef float type;
+    static constexpr int BYTES = 4;
+};
+template <> struct Elem<bf16raw> {
+    typedef uint16_t type;
+    static constexpr int BYTES = 2;
+};
+
+// (Host and device: the index arithmetic is also checked on the CPU.)
+__host__ __device__ __forceinline__ void flag_bad_index(uint32_t *status) {
+    if (!status) return;
+#ifdef __CUDA_ARCH__
+    atomicOr(status, Q3CU_DEV_BAD_INDEX);
+#else
+    *status |= Q3CU_DEV_BAD_INDEX;
+#endif
+}
+
+// Keys a sequence holds: kv_len, no more than its table row has pages for (a
+// longer kv_len is flagged) and no fewer than none.
+__host__ __device__ __forceinline__ int paged_len(const PagedSeqs &b, const PagedKV &c, int s, uint32_t *status) {
+    const int64_t cap = int64_t(b.max_pages) << c.page_shift;
+    const int n = b.kv_len[s];
+    if (n > cap) {
+        flag_bad_index(status);
+        return int(cap);
+    }
+    return n < 0 ? 0 : n;
+}
+
+// Page of position t (t >= 0, below max_pages << page_shift) of sequence s; -1 and the status bit for an id
+// outside the cache.
+__host__ __device__ __forceinline__ int paged_page(const PagedSeqs &b, const PagedKV &c, int s, int t, uint32_t *status) {
+    const int page = b.pages[int64_t(s) * b.max_pages + (t >> c.page_shift)];
+    if (page >= 0 && page < c.n_pages) return page;
+    flag_bad_index(status);
+    return -1;
+}
+
+// Element offset of (page, kv head, slot): 64 bits, a cache is larger than 2^31 elements.
+__host__ __device__ __forceinline__ int64_t paged_at(const PagedKV &c, int page, int head, int t) {
+    const int slot = t & ((1 << c.page_shift) - 1);
+    return int64_t(page) * c.page_stride + ((int64_t(head) << c.page_shift) + slot) * HD;
+}
+
+// The sequence of packed row r: the last s with row_off[s] <= r, or -1 when r
+// lies in no sequence (behind the last one, or offsets that do not rise).
+__host__ __device__ __forceinline__ int paged_seq_of(const PagedSeqs &b, int64_t r) {
+    int lo = 0, hi = b.n_seqs;                               // row_off[lo] <= r < row_off[hi], if any does
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (b.row_off[mid] <= r) lo = mid;
+        else hi = mid;
+    }
+    return b.n_seqs > 0 && b.row_off[lo] <= r && r < b.row_off[lo + 1] ? lo : -1;
+}
+
+// Position of packed row r of sequence s (as paged_seq_of finds it): negative for padding before position 0, and,
+// flagged, beyond the table's pages.
+__host__ __device__ __forceinline__ int paged_pos(const PagedSeqs &b, const PagedKV &c, int s, int64_t r,
+                                                  uint32_t *status) {
+    const int64_t p = int64_t(b.kv_len[s]) - b.row_off[s + 1] + r;
+    if (p < 0) return -1;
+    if (p < int64_t(b.max_pages) << c.page_shift) return int(p);
+    flag_bad_index(status);
+    return -1;
+}
+
+// Keys that packed row r of sequence s attends to: the positions up to its own, as far as the sequence holds them
+// (`len` of paged_len).
+__host__ __device__ __forceinline__ int paged_seen(const PagedSeqs &b, int s, int64_t r, int len) {
+    const int64_t n = int64_t(b.kv_len[s]) - b.row_off[s + 1] + r + 1;
+    return n < 0 ? 0 : n < len ? int(n) : len;
+}
+
+// Four consecutive elements as floats, and a float4 stored as T.
+__device__ __forceinline__ float4 load_quad(const float *p) { return *reinterpret_cast<const float4 *>(p); }
+__device__ __forceinline__ float4 load_quad(const uint16_t *p) {
+    const uint2 u = *reinterpret_cast<const uint2 *>(p);
+    return make_float4(bf16_to_f32(u.x & 0xffffu), bf16_to_f32(u.x >> 16), bf16_to_f32(u.y & 0xffffu),
+                       bf16_to_f32(u.y >> 16));
+}
+__device__ __forceinline__ void store_quad(float *p, float4 v) { *reinterpret_cast<float4 *>(p) = v; }
+__device__ __forceinline__ void store_quad(uint16_t *p, float4 v) {
+    *reinterpret_cast<uint2 *>(p) = make_uint2(f32_to_bf16(v.x) | (f32_to_bf16(v.y) << 16),
+                                               f32_to_bf16(v.z) | (f32_to_bf16(v.w) << 16));
+}
+
+// Attention of one query row and head by one warp, straight from the formula:
+// lane l holds elements 4l .. 4l+3 of q (scaled by 1/sqrt(128)), of every key
+// and value and of the result.  The running maximum and sum of the softmax, one pass over
+// the keys 0 .. n-1 of sequence s.  Returns zeros for n = 0.
+template <typename TC>
+__device__ __forceinline__ float4 attend_row(const PagedKV &c, const PagedSeqs &b, int s, int head, int n, float4 q,
+                                             uint32_t *status) {
+    const typename Elem<TC>::type *kp = static_cast<const typename Elem<TC>::type *>(c.k);
+    const typename Elem<TC>::type *vp = static_cast<const typename Elem<TC>::type *>(c.v);
+    const int lane = threadIdx.x & 31;
+    float m = -INFINITY, sum = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int t = 0; t < n; ++t) {
+        const int page = paged_page(b, c, s, t, lane == 0 ? status : nullptr);
+        float4 k = make_float4(0.0f, 0.0f, 0.0f, 0.0f), v = k;
+        if (page >= 0) {
+            const int64_t at = paged_at(c, page, head, t) + 4 * lane;
+            k = load_quad(kp + at);
+            v = load_quad(vp + at);
+        }
+        float d = fmaf(q.x, k.x, fmaf(q.y, k.y, fmaf(q.z, k.z, q.w * k.w)));
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) d += __shfl_xor_sync(FULL, d, x);
+        const float nm = fmaxf(m, d), f = m == nm ? 1.0f : expf(m - nm), p = expf(d - nm);
+        m = nm;
+        sum = fmaf(sum, f, p);
+        o = make_float4(fmaf(o.x, f, p * v.x), fmaf(o.y, f, p * v.y), fmaf(o.z, f, p * v.z), fmaf(o.w, f, p * v.w));
+    }
+    if (n == 0) return o;
+    const float r = 1.0f / sum;
+    return make_float4(o.x * r, o.y * r, o.z * r, o.w * r);
+}
+
+constexpr float ATT_SCALE = 0.08838834764831845f;            // 1/sqrt(128)
+
+}  // namespace q3

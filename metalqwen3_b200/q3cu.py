@@ -31,6 +31,16 @@ class Q3Error(RuntimeError):
         self.status = status
 
 
+class _KVCache(C.Structure):             # q3cu_kv_cache
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("page_stride", C.c_int64), ("n_pages", C.c_int32),
+                ("n_kv", C.c_int32), ("page_size", C.c_int32), ("head_dim", C.c_int32), ("dtype", C.c_int32)]
+
+
+class _KVBatch(C.Structure):             # q3cu_kv_batch
+    _fields_ = [("row_off", C.c_void_p), ("kv_len", C.c_void_p), ("pages", C.c_void_p), ("n_seqs", C.c_int32),
+                ("max_pages", C.c_int32)]
+
+
 def header_functions(path: str = HEADER) -> list[str]:
     """Names of the entry points declared in include/q3cu.h."""
     text = open(path).read()
@@ -68,6 +78,13 @@ def load_library(path: str = LIB_PATH) -> C.CDLL:
                 "q3cu_matmul_q8": (st, [vp, vp, vp, i32, vp, vp, i32, i32, vp, vp]),
                 "q3cu_execute_quantized_matmul": (st, [vp, vp, vp, vp, vp, vp, i32, i32, i32]),
                 "q3cu_attention": (st, [vp, vp, vp, vp, i32, i32, i32, i32, vp, i32, vp, vp, vp]),
+                "q3cu_kv_append": (st, [vp, C.POINTER(_KVCache), C.POINTER(_KVBatch), i64, vp, vp, vp, i32, i64, i64,
+                                        i32, vp, vp, f32, f32, vp, i32, vp]),
+                "q3cu_attention_paged": (st, [vp, C.POINTER(_KVCache), C.POINTER(_KVBatch), vp, i32, i64, i32, vp,
+                                              C.c_size_t, vp, vp]),
+                "q3cu_attention_paged_workspace": (st, [vp, i32, i32, C.POINTER(C.c_size_t)]),
+                "q3cu_attention_prompt": (st, [vp, C.POINTER(_KVCache), C.POINTER(_KVBatch), i64, vp, i32, i64, i32,
+                                               vp, vp]),
                 "q3cu_execute_attention": (st, [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, C.c_uint64,
                                                 i32]),
                 "q3cu_model_load": (st, [vp, vp, C.c_size_t, i32, C.POINTER(vp)]),
@@ -105,6 +122,56 @@ def _dtype(t):
     if t.dtype == torch.bfloat16:
         return BF16
     raise TypeError(f"unsupported dtype {t.dtype}")
+
+
+def _tensor(t, what, dtype=None, shape=None, device=None):
+    """Checks a device tensor's type and shape (None: any)."""
+    if not t.is_cuda or (device is not None and t.get_device() != device):
+        raise ValueError(f"{what} must be on the context's GPU, it is on {t.device}")
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError(f"{what} must be {dtype}, it is {t.dtype}")
+    if shape is not None and (t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape))):
+        raise ValueError(f"{what} must be {list(shape)}, it is {list(t.shape)}")
+    return t
+
+
+def _rows(t, what):
+    """Row stride in elements of t [rows][heads][128], whose rows are dense."""
+    if t.numel() and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2])):
+        raise ValueError(f"{what}: the heads of a row must be contiguous, strides are {t.stride()}")
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1] * t.shape[2])
+
+
+class KVCache:
+    """One layer's paged key-value cache: k and v [n_pages][n_kv][page_size][128] of one type (f32 or bf16).
+    A page is dense; pages may lie further apart (the same stride in k and v)."""
+
+    def __init__(self, k, v):
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
+            raise ValueError("k and v must be [n_pages][n_kv][page_size][128] of one type on one GPU")
+        n_pages, n_kv, size, hd = k.shape
+        if k.stride()[1:] != (size * hd, hd, 1) or v.stride()[1:] != k.stride()[1:] or (
+                n_pages > 1 and k.stride(0) != v.stride(0)):
+            raise ValueError("a page must be contiguous, and k and v have one page stride")
+        _tensor(k, "k"), _tensor(v, "v")
+        self.k, self.v, self.n_kv = k, v, n_kv
+        self.c = _KVCache(k.data_ptr(), v.data_ptr(), k.stride(0) if n_pages > 1 else n_kv * size * hd, n_pages, n_kv,
+                          size, hd, _dtype(k))
+
+
+class KVBatch:
+    """The sequences of a call: kv_len [n_seqs], pages [n_seqs][max_pages] and, for packed rows, row_off
+    [n_seqs + 1], all int32 on the GPU (the meaning of each: q3cu_kv_batch in include/q3cu.h)."""
+
+    def __init__(self, kv_len, pages, row_off=None):
+        n = kv_len.numel()
+        i32 = kv_len.new_empty(0).int().dtype
+        for t, what, shape in ((kv_len, "kv_len", (n,)), (pages, "pages", (n, None)), (row_off, "row_off", (n + 1,))):
+            if t is not None and not _tensor(t, what, i32, shape).is_contiguous():
+                raise ValueError(f"{what} must be contiguous")
+        self.kv_len, self.pages, self.row_off = kv_len, pages, row_off
+        self.c = _KVBatch(None if row_off is None else row_off.data_ptr(), kv_len.data_ptr(), pages.data_ptr(), n,
+                          pages.shape[1])
 
 
 class Q3CU:
@@ -252,6 +319,72 @@ class Q3CU:
                                             kv_dim, kv_mul, _ptr(att), att.shape[-1], _ptr(probs), _ptr(xb),
                                             self._stream(stream)), "q3cu_attention")
         return xb, probs
+
+    # -- the paged key-value cache -----------------------------------------------
+    def kv_append(self, cache, batch, q, k, v, q_norm=None, k_norm=None, theta=1e6, eps=1e-6, q_out=None,
+                  out_dtype=None, stream=None):
+        """QK-norm (where weights are given) and rotation of the packed rows q [rows][n_heads][128] and
+        k [rows][n_kv][128] (q may be None); keys and values into the cache; returns the rotated queries
+        (out_dtype, the cache's type by default, or q_out).  q, k, v may be slices of one projection's rows."""
+        rows = k.shape[0]
+        _tensor(k, "k", None, (rows, cache.n_kv, 128), self.device)
+        _tensor(v, "v", k.dtype, (rows, cache.n_kv, 128), self.device)
+        for w, what in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+            if w is not None and not _tensor(w, what, self.torch.float32, (128,), self.device).is_contiguous():
+                raise ValueError(f"{what} must be contiguous")
+        kv_stride, q_stride, heads = _rows(k, "k"), 0, 0
+        if rows > 1 and _rows(v, "v") != kv_stride:
+            raise ValueError("k and v must have one row stride")
+        if q is not None:
+            heads = _tensor(q, "q", k.dtype, (rows, None, 128), self.device).shape[1]
+            q_stride = _rows(q, "q")
+            if q_out is None:
+                q_out = self.torch.empty((rows, heads, 128), dtype=out_dtype or cache.k.dtype, device=q.device)
+            if not _tensor(q_out, "q_out", out_dtype, (rows, heads, 128), self.device).is_contiguous():
+                raise ValueError("q_out must be contiguous")
+        self._check(self.lib.q3cu_kv_append(self.ctx, C.byref(cache.c), C.byref(batch.c), rows, _ptr(q), _ptr(k),
+                                            _ptr(v), _dtype(k), q_stride, kv_stride, heads, _ptr(q_norm),
+                                            _ptr(k_norm), theta, eps, _ptr(q_out) if q is not None else None,
+                                            _dtype(q_out) if q is not None else F32, self._stream(stream)),
+                    "q3cu_kv_append")
+        return q_out
+
+    def attention_paged_workspace(self, cache, n_heads):
+        """A workspace for attention_paged with these head counts, for any batch; calls that may run at
+        the same time (other streams, captured graphs replayed side by side) need one each."""
+        n = C.c_size_t(0)
+        self._check(self.lib.q3cu_attention_paged_workspace(self.ctx, n_heads, cache.n_kv, C.byref(n)),
+                    "q3cu_attention_paged_workspace")
+        return self.torch.empty(n.value, dtype=self.torch.uint8, device=cache.k.device)
+
+    def _query(self, q, out, rows):
+        _tensor(q, "q", None, (rows, None, 128), self.device)
+        out = self.torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
+        if not _tensor(out, "out", q.dtype, tuple(q.shape), self.device).is_contiguous():
+            raise ValueError("out must be contiguous")
+        return out
+
+    def attention_paged(self, cache, batch, q, out=None, work=None, stream=None):
+        """One new token per sequence: q [n_seqs][n_heads][128] over each sequence's kv_len positions."""
+        out = self._query(q, out, batch.c.n_seqs)
+        if work is None:
+            work = self.attention_paged_workspace(cache, q.shape[1])
+            if stream is not None:
+                work.record_stream(stream)      # its memory is not given out again before the call has run
+        self._check(self.lib.q3cu_attention_paged(self.ctx, C.byref(cache.c), C.byref(batch.c), _ptr(q), _dtype(q),
+                                                  _rows(q, "q"), q.shape[1], _ptr(work),
+                                                  work.numel() * work.element_size(), _ptr(out),
+                                                  self._stream(stream)), "q3cu_attention_paged")
+        return out
+
+    def attention_prompt(self, cache, batch, q, out=None, stream=None):
+        """Causal attention of the packed rows q [rows][n_heads][128] over the cache, which holds their
+        keys and values; rows behind the last sequence are not written."""
+        out = self._query(q, out, q.shape[0])
+        self._check(self.lib.q3cu_attention_prompt(self.ctx, C.byref(cache.c), C.byref(batch.c), q.shape[0], _ptr(q),
+                                                   _dtype(q), _rows(q, "q"), q.shape[1], _ptr(out),
+                                                   self._stream(stream)), "q3cu_attention_prompt")
+        return out
 
     # -- host-pointer drop-in (numpy arrays, synchronous) -----------------------
     def execute_attention(self, xb, q, att, key_cache, value_cache, pos, head_dim, n_heads, n_kv_heads, seq_len,
