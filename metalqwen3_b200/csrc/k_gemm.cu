@@ -44,6 +44,7 @@
 // Every wait is bounded; on a timeout the kernel records Q3CU_DEV_TIMEOUT,
 // waits (bounded) for its own copies and MMAs, frees tensor memory and returns.
 #include "q3cu_internal.h"
+#include "q3cu_tcgen05.cuh"
 #include "q3cu_tma.h"
 
 namespace q3 {
@@ -64,25 +65,12 @@ constexpr size_t TC_SMEM = size_t(TC_NS) * TC_STAGE_B + 1024 +
 // N = 128 (bits 17-22: N / 8), M = 128 (bits 24-28: M / 16).
 constexpr uint32_t TC_IDESC = (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(TC_BN / 8) << 17) | (uint32_t(TC_BM / 16) << 24);
 
-// Shared-memory matrix descriptor of a K-major, 128-byte-swizzled operand:
-// start address / 16, leading offset 1 (unused with the swizzle), stride 1024 B
-// between 8-row groups (/16), descriptor version 1, layout SWIZZLE_128B (2).
-__device__ __forceinline__ uint64_t tc_sdesc(uint32_t smem_addr) {
-    return uint64_t((smem_addr & 0x3FFFFu) >> 4) | (uint64_t(1) << 16) | (uint64_t(1024 >> 4) << 32) |
-           (uint64_t(1) << 46) | (uint64_t(2) << 61);
-}
 __device__ __forceinline__ void tc_mma(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t accumulate) {
     asm volatile(
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
         :: "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(TC_IDESC), "r"(accumulate) : "memory");
 }
-__device__ __forceinline__ void tc_commit(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
-                 :: "r"(smem_addr(bar)) : "memory");
-}
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t (&v)[16]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
@@ -90,7 +78,6 @@ __device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t (&v)[16]) {
           "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
         : "r"(taddr) : "memory");
 }
-__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 // The wait, with the loaded registers as operands: nothing that reads them can
 // be scheduled before it.
 __device__ __forceinline__ void tc_wait_ld16(uint32_t (&v)[16]) {

@@ -150,12 +150,12 @@ size_t up32(size_t b) { return (b + 31) & ~size_t(31); }
 
 namespace q3 {
 cudaError_t ensure_smem_attr(const void *kernel, size_t bytes, int slot) {
-    static std::atomic<uint32_t> done[64];
+    static std::atomic<uint64_t> done[64];
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
-    if (dev < 0 || dev >= 64 || slot < 0 || slot >= 32) return cudaErrorInvalidValue;
-    const uint32_t bit = 1u << slot;
+    if (dev < 0 || dev >= 64 || slot < 0 || slot >= 64) return cudaErrorInvalidValue;
+    const uint64_t bit = uint64_t(1) << slot;
     if (done[dev].load(std::memory_order_acquire) & bit) return cudaSuccess;
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
     if (e == cudaSuccess) done[dev].fetch_or(bit, std::memory_order_release);

@@ -17,7 +17,7 @@ int ctx_sms(const q3cu_ctx *ctx);
 uint32_t *ctx_status_word(const q3cu_ctx *ctx);               // the device status word (Q3CU_DEV_* bits)
 
 // Raises a kernel's dynamic shared-memory limit once per (device, slot):
-// `slot` (< 32) names the kernel instantiation.
+// `slot` (< 64) names the kernel instantiation.
 cudaError_t ensure_smem_attr(const void *kernel, size_t bytes, int slot);
 
 // Launches `kernel` as a programmatic dependent of the stream's previous

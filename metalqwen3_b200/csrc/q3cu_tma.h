@@ -41,6 +41,13 @@ bool encode_rows_2d_map(CUtensorMap *map, const void *base, uint64_t rows, uint6
 bool encode_f32_2d_map(CUtensorMap *map, const void *base, uint64_t rows, uint64_t cols, uint32_t box_cols,
                        uint32_t box_rows, bool swizzle128);
 
+// A bf16 tensor of `rank` (3 or 4) dimensions, innermost first and dense in dimension 0 (strides[i]: bytes between
+// neighbours in dimension i + 1, multiples of 16), read in boxes of 64 elements by box[1..]; a box lands as lines
+// of 128 B with the 128-byte swizzle (1024-byte aligned), elements outside the tensor as zeros.  Encoded anew by
+// every call (a fraction of a microsecond).
+bool encode_bf16_map(CUtensorMap *map, const void *base, int rank, const uint64_t *dims, const uint64_t *strides,
+                     const uint32_t *box);
+
 #if defined(__CUDACC__)
 __device__ __forceinline__ void tma_load_2d(void *dst, const CUtensorMap *map, int x, int y, uint64_t *bar) {
     asm volatile(
@@ -57,6 +64,15 @@ __device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, i
         "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
         :: "r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))), "l"(reinterpret_cast<uint64_t>(map)), "r"(x),
            "r"(y), "r"(z), "r"(static_cast<uint32_t>(__cvta_generic_to_shared(bar)))
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, int x, int y, int z, int w,
+                                            uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3, %4, %5}], [%6];"
+        :: "r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))), "l"(reinterpret_cast<uint64_t>(map)), "r"(x),
+           "r"(y), "r"(z), "r"(w), "r"(static_cast<uint32_t>(__cvta_generic_to_shared(bar)))
         : "memory");
 }
 // Tiled 2-D tensor store of the box at (x, y) from shared memory at src, in the
