@@ -1,40 +1,555 @@
 // k_paged.cu -- attention of one new token per sequence over the paged cache.
+//
+// Query head h of sequence s: o = sum_t softmax_t(q . k_t / sqrt(128)) v_t over
+// its kv_len positions, in one pass with the running maximum and sum of the
+// softmax.  Bound by memory: every key and value of the batch is read once, for
+// all the query heads of its kv head together.
+//
+// The split.  Lengths are ragged and known to the device only, so the unit of
+// work is a tile of positions of one (sequence, kv head): all tiles, in the
+// order sequence, head, position, are cut into one equal run per CTA, two CTAs
+// on each SM.  A run that covers all tiles of a (sequence, head) writes its
+// result; one that begins or ends inside leaves maximum, sum and unnormalised
+// result in the workspace (at most two per CTA), and a second kernel joins
+// those.  One long sequence spreads over the whole GPU just as a full batch does.
+//
+// A CTA is one fetching warp and four computing warps around a ring of three
+// 32 KB stages, filled page by page by TMA (128-byte swizzle).  A stage is K
+// and V of 64 positions in bf16 or 32 in f32; each computing warp takes a
+// quarter of them, with its own running maximum, sum and result, and the four
+// are joined when the run leaves the (sequence, head).
+//
+// The products run on mma.sync with the group's query heads as the 16 rows of
+// the tile: at one to sixteen query rows the tensor cores are mostly idle by
+// either path, and the operands come straight from registers.  Nothing is
+// rounded below 16 bits of mantissa on the way: an f32 query against a bf16
+// cache is two bf16 parts (the keys are exact), a probability is two bf16 parts,
+// and an f32 cache is multiplied as tf32 parts, high x high + high x low +
+// low x high, whose remainder is 2^-21 of the product.  Sums are binary32.
+//
+// Positions at and beyond the length score -inf, and their values are masked to
+// zero in registers: unused page space may hold anything.
 #include "q3cu_paged.cuh"
+#include "q3cu_tma.h"
 
 namespace q3 {
 
-template <typename T, typename TC>
-__global__ void __launch_bounds__(128) paged_rows_kernel(const PagedKV c, const PagedSeqs b,
-                                                         const typename Elem<T>::type *q, int64_t q_stride,
-                                                         int n_heads, typename Elem<T>::type *out, uint32_t *status) {
-    griddep_wait();
-    const int lane = threadIdx.x & 31;
-    const int64_t w = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5);
-    const int64_t s = w / n_heads;
-    const int h = int(w % n_heads);
-    if (s >= b.n_seqs) return;
-    const int n = paged_len(b, c, int(s), lane == 0 ? status : nullptr);
-    float4 x = load_quad(q + s * q_stride + int64_t(h) * HD + 4 * lane);
-    x = make_float4(x.x * ATT_SCALE, x.y * ATT_SCALE, x.z * ATT_SCALE, x.w * ATT_SCALE);
-    store_quad(out + w * HD + 4 * lane, attend_row<TC>(c, b, int(s), h / (n_heads / c.n_kv), n, x, status));
+constexpr int PD_WARPS = 4, PD_THREADS = (PD_WARPS + 1) * 32;
+constexpr int PD_NS = 3;                                     // stages
+constexpr uint32_t PD_SIDE = 16384, PD_STAGE = 2 * PD_SIDE;  // K or V of a stage; both
+constexpr int PD_SPARE = 16 * HD * 4;                        // queries (f32 cache), then the join of the warps
+constexpr size_t PD_SMEM = size_t(PD_NS) * PD_STAGE + PD_SPARE + 1024;
+constexpr float PD_LOG2 = ATT_SCALE * 1.44269504088896341f;  // scores to base-2 exponents
+constexpr int PD_PART = HD + 2;                              // floats of a row's partial result: 128, maximum, sum
+
+template <typename TC> __host__ __device__ constexpr int pd_tile() { return int(PD_SIDE) / (HD * Elem<TC>::BYTES); }   // positions of a stage
+
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_tf32(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ float4 lds4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+// Two floats as bf16 (hi) and what that leaves of them as bf16 (lo).
+__device__ __forceinline__ void split_bf16(float x, float y, uint32_t &hi, uint32_t &lo) {
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(y), "f"(x));
+    const float rx = x - __uint_as_float(hi << 16), ry = y - __uint_as_float(hi & 0xffff0000u);
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(ry), "f"(rx));
+}
+// A float's leading 11 bits (tf32) and the rest, exactly.
+__device__ __forceinline__ void split_tf32(float x, uint32_t &hi, uint32_t &lo) {
+    hi = __float_as_uint(x) & 0xffffe000u;
+    lo = __float_as_uint(x - __uint_as_float(hi));
 }
 
-size_t attention_paged_workspace(int n_heads, int n_kv, int sms) { return 16; }
+// A place in the batch's tiles: sequence, kv head, tile, and the sequence's length and tiles.
+struct PagedWalk {
+    int s, head, tile, len, tiles;
+};
+template <typename TC>
+__device__ __forceinline__ int64_t walk_total(const PagedSeqs &b, const PagedKV &c, uint32_t *status) {
+    int64_t n = 0;
+    for (int s = threadIdx.x & 31; s < b.n_seqs; s += 32) n += (paged_len(b, c, s, status) + pd_tile<TC>() - 1) / pd_tile<TC>();
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(FULL, n, o);
+    return n * c.n_kv;
+}
+// Tiles of the sequences before s (one warp).
+template <typename TC>
+__device__ __forceinline__ int64_t walk_before(const PagedSeqs &b, const PagedKV &c, int s) {
+    int64_t n = 0;
+    for (int i = threadIdx.x & 31; i < s; i += 32) n += (paged_len(b, c, i, nullptr) + pd_tile<TC>() - 1) / pd_tile<TC>();
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(FULL, n, o);
+    return n * c.n_kv;
+}
+// The place of tile u < total (one warp; every lane returns it).
+template <typename TC>
+__device__ __forceinline__ PagedWalk walk_to(const PagedSeqs &b, const PagedKV &c, int64_t u) {
+    PagedWalk w = {};
+    const int lane = threadIdx.x & 31;
+    for (int s0 = 0; s0 < b.n_seqs; s0 += 32) {
+        const int len = s0 + lane < b.n_seqs ? paged_len(b, c, s0 + lane, nullptr) : 0;
+        const int tiles = (len + pd_tile<TC>() - 1) / pd_tile<TC>();
+        int64_t end = int64_t(tiles) * c.n_kv;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t x = __shfl_up_sync(FULL, end, o);
+            if (lane >= o) end += x;
+        }
+        const unsigned hit = __ballot_sync(FULL, u < end);
+        if (hit) {
+            const int l = __ffs(hit) - 1;
+            w.s = s0 + l;
+            w.len = __shfl_sync(FULL, len, l);
+            w.tiles = __shfl_sync(FULL, tiles, l);
+            const int64_t at = u - (__shfl_sync(FULL, end, l) - int64_t(w.tiles) * c.n_kv);
+            w.head = int(at / w.tiles);
+            w.tile = int(at % w.tiles);
+            return w;
+        }
+        u -= __shfl_sync(FULL, end, 31);
+    }
+    return w;
+}
+// `n` tiles further, which lie in the same (sequence, head) or begin the next one that has any.
+template <typename TC>
+__device__ __forceinline__ void walk_on(const PagedSeqs &b, const PagedKV &c, PagedWalk &w, int n) {
+    w.tile += n;
+    if (w.tile < w.tiles) return;
+    w.tile = 0;
+    if (++w.head < c.n_kv) return;
+    w.head = 0;
+    do {
+        if (++w.s >= b.n_seqs) return;
+        w.len = paged_len(b, c, w.s, nullptr);
+    } while (w.len == 0);
+    w.tiles = (w.len + pd_tile<TC>() - 1) / pd_tile<TC>();
+}
+
+// One pair of result elements (row, dims at, at + step) as the output's type.
+__device__ __forceinline__ void put2(float *p, int step, float x, float y) { p[0] = x, p[step] = y; }
+__device__ __forceinline__ void put2(uint16_t *p, int step, float x, float y) {
+    if (step == 1) *reinterpret_cast<uint32_t *>(p) = f32_to_bf16(x) | (f32_to_bf16(y) << 16);
+    else p[0] = uint16_t(f32_to_bf16(x)), p[step] = uint16_t(f32_to_bf16(y));
+}
+
+// WIDE: more than 8 query heads to a kv head (rows 8-15 of the products are used).
+template <typename T, typename TC, bool WIDE>
+__global__ void __launch_bounds__(PD_THREADS, 2)
+paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, const PagedKV c,
+                   const PagedSeqs b, const typename Elem<T>::type *q, int64_t q_stride, int n_heads, int group,
+                   typename Elem<T>::type *out, float *part, uint32_t *status) {
+    constexpr bool CF32 = Elem<TC>::BYTES == 4;
+    constexpr int TILE = pd_tile<TC>(), KW = TILE / PD_WARPS, NH = WIDE ? 2 : 1;
+    extern __shared__ uint8_t pd_dyn[];
+    uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(pd_dyn) + 1023) & ~uintptr_t(1023));
+    float *spare = reinterpret_cast<float *>(ring + PD_NS * PD_STAGE);
+    __shared__ __align__(8) uint64_t full[PD_NS], empty[PD_NS];
+    __shared__ float join_m[2][8], join_l[2][8];
+    __shared__ volatile int dead;                            // a wait gave up
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < PD_NS; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], PD_WARPS);
+        }
+        mbar_init_fence();
+        dead = 0;
+    }
+    __syncthreads();
+    griddep_wait();
+    griddep_launch_dependents();
+
+    const int64_t total = walk_total<TC>(b, c, blockIdx.x == 0 && warp == 0 ? status : nullptr);
+    const int64_t u0 = total * blockIdx.x / gridDim.x, u1 = total * (blockIdx.x + 1) / gridDim.x;
+    if (u0 == u1) return;
+    PagedWalk w = walk_to<TC>(b, c, u0);
+
+    if (warp == PD_WARPS) {
+        // ---- fetch: lane = box (K or V, column block, rows of one page) ------------------
+        const int br = min(1 << c.page_shift, TILE), nb = TILE / br;
+        constexpr int CB = CF32 ? 4 : 2;                     // column blocks of 128 B
+        const int box = lane % nb, col = lane / nb % CB, side = lane / (nb * CB);
+        auto page_of = [&]() -> int {                        // n_pages reads as zeros
+            const int t = w.tile * TILE + box * br;
+            if (side > 1 || t >= w.len) return c.n_pages;
+            const int p = paged_page(b, c, w.s, t, status);
+            return p < 0 ? c.n_pages : p;
+        };
+        uint8_t *dst = ring + side * PD_SIDE + col * (PD_SIDE / CB) + box * br * 128;
+        int page = page_of(), e = 0;
+        bool ok = true;
+        for (int64_t u = u0; u < u1; ++u, ++e) {
+            const int head = w.head, slot = (w.tile * TILE + box * br) & ((1 << c.page_shift) - 1), now = page;
+            if (u + 1 < u1) {
+                walk_on<TC>(b, c, w, 1);
+                page = page_of();                            // under way while this tile waits for its stage
+            }
+            const int st = e % PD_NS;
+            if (e >= PD_NS) ok = mbar_wait(&empty[st], uint32_t(e / PD_NS - 1) & 1u, lane == 0 ? status : nullptr);
+            if (!__all_sync(FULL, ok)) break;
+            if (lane == 0) mbar_arrive_expect_tx(&full[st], PD_STAGE);
+            __syncwarp();
+            if (side < 2)
+                tma_load_4d(dst + st * PD_STAGE, side ? &tmv : &tmk, (CF32 ? 32 : 64) * col, slot, head, now, &full[st]);
+        }
+        // no copy outlives the CTA (bounded)
+        for (int d = e > PD_NS ? e - PD_NS : 0; d < e; ++d) mbar_wait(&full[d % PD_NS], uint32_t(d / PD_NS) & 1u, nullptr);
+        return;
+    }
+
+    // ---- the computing warps ---------------------------------------------------------
+    const int g = lane >> 2, t4 = lane & 3;                  // row g (and g + 8) of the products, column pair t4
+    const uint32_t ring_a = smem_addr(ring);
+    int e = 0;
+    bool ok = true;
+    for (int64_t u = u0; u < u1 && ok;) {
+        const int run = int(min(int64_t(w.tiles - w.tile), u1 - u));       // tiles of this (sequence, head) here
+        const typename Elem<T>::type *qs = q + w.s * q_stride + int64_t(w.head) * group * HD;
+        uint32_t qh[CF32 ? 1 : 8][2 * NH], ql[CF32 || Elem<T>::BYTES == 2 ? 1 : 8][2 * NH];
+        if constexpr (CF32) {                                // the group's rows in shared memory, zeros below
+            for (int i = threadIdx.x; i < 8 * NH * (HD / 4); i += PD_WARPS * 32)
+                *reinterpret_cast<float4 *>(spare + 4 * i) =
+                    i / (HD / 4) < group ? load_quad(qs + 4 * i) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            named_sync(1, PD_WARPS * 32);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+#pragma unroll
+                for (int x = 0; x < 2 * NH; ++x) {           // x: columns + 8 (bit 0), row + 8 (bit 1)
+                    const int row = g + 8 * (x >> 1), at = row * HD + 16 * k + 2 * t4 + 8 * (x & 1);
+                    if constexpr (Elem<T>::BYTES == 2) {
+                        qh[k][x] = row < group ? *reinterpret_cast<const uint32_t *>(qs + at) : 0u;
+                    } else {
+                        const float2 v = row < group ? *reinterpret_cast<const float2 *>(qs + at) : make_float2(0.0f, 0.0f);
+                        split_bf16(v.x, v.y, qh[k][x], ql[k][x]);
+                    }
+                }
+        }
+        float o[16][4];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+        float m[NH], l[NH];
+#pragma unroll
+        for (int h = 0; h < NH; ++h) m[h] = -INFINITY, l[h] = 0.0f;
+
+        for (int i = 0; i < run; ++i, ++e) {
+            const int st = e % PD_NS;
+            ok = __all_sync(FULL, mbar_wait(&full[st], uint32_t(e / PD_NS) & 1u, lane == 0 ? status : nullptr));
+            if (!ok) break;
+            const uint32_t ka = ring_a + st * PD_STAGE, va = ka + PD_SIDE;
+            const int left = w.len - (w.tile + i) * TILE - warp * KW;      // visible positions of this warp's KW
+            // scores: rows g, g + 8; columns (positions) 8 n + 2 t4, + 1
+            float s[KW / 8][4];
+#pragma unroll
+            for (int n = 0; n < KW / 8; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+            if constexpr (CF32) {
+                // k index t4 is dimension 32 d + 8 t4 + x, k index t4 + 4 is + 1 of it (x = 0, 2, then 4, 6): a
+                // permutation that query and key share, so both are read 16 bytes at a time without conflicts
+                const uint32_t row = ka + (warp * KW + g) * 128, qa = smem_addr(spare) + g * (HD * 4);
+#pragma unroll
+                for (int d = 0; d < 4; ++d)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const float4 kv = lds4(row + d * (PD_SIDE / 4) + (((2 * t4 + x) ^ g) << 4));
+                        const float kf[4] = {kv.x, kv.y, kv.z, kv.w};
+                        float qf[NH][4];
+#pragma unroll
+                        for (int h = 0; h < NH; ++h) {
+                            const float4 v = lds4(qa + h * 8 * (HD * 4) + (32 * d + 8 * t4 + 4 * x) * 4);
+                            qf[h][0] = v.x, qf[h][1] = v.y, qf[h][2] = v.z, qf[h][3] = v.w;
+                        }
+#pragma unroll
+                        for (int y = 0; y < 4; y += 2) {
+                            uint32_t bh[2], bl[2], ah[4] = {0, 0, 0, 0}, al[4] = {0, 0, 0, 0};
+                            split_tf32(kf[y], bh[0], bl[0]);
+                            split_tf32(kf[y + 1], bh[1], bl[1]);
+#pragma unroll
+                            for (int h = 0; h < NH; ++h) {
+                                split_tf32(qf[h][y], ah[h], al[h]);
+                                split_tf32(qf[h][y + 1], ah[2 + h], al[2 + h]);
+                            }
+                            mma_tf32(s[0], al[0], al[1], al[2], al[3], bh[0], bh[1]);
+                            mma_tf32(s[0], ah[0], ah[1], ah[2], ah[3], bl[0], bl[1]);
+                            mma_tf32(s[0], ah[0], ah[1], ah[2], ah[3], bh[0], bh[1]);
+                        }
+                    }
+            } else {
+                const int key = warp * KW + (lane >> 4) * 8 + (lane & 7);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const int chunk = 2 * k + ((lane >> 3) & 1);
+                    uint32_t r[4];
+                    ldsm4(ka + (chunk >> 3) * (PD_SIDE / 2) + key * 128 + (((chunk & 7) ^ (key & 7)) << 4), r);
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+                        if constexpr (Elem<T>::BYTES == 4)
+                            mma_bf16(s[n], ql[k][0], WIDE ? ql[k][2 * NH - 2] : 0u, ql[k][1], WIDE ? ql[k][2 * NH - 1] : 0u,
+                                     r[2 * n], r[2 * n + 1]);
+                        mma_bf16(s[n], qh[k][0], WIDE ? qh[k][2 * NH - 2] : 0u, qh[k][1], WIDE ? qh[k][2 * NH - 1] : 0u,
+                                 r[2 * n], r[2 * n + 1]);
+                    }
+                }
+            }
+            // softmax over this warp's positions
+            if (left < KW) {
+#pragma unroll
+                for (int n = 0; n < KW / 8; ++n)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+                        if (8 * n + 2 * t4 + (x & 1) >= left) s[n][x] = -INFINITY;
+            }
+            float f[NH];
+            bool grow = false;
+#pragma unroll
+            for (int h = 0; h < NH; ++h) {
+                float tm = -INFINITY;
+#pragma unroll
+                for (int n = 0; n < KW / 8; ++n) tm = fmaxf(tm, fmaxf(s[n][2 * h], s[n][2 * h + 1]));
+                tm = fmaxf(tm, __shfl_xor_sync(FULL, tm, 1));
+                tm = fmaxf(tm, __shfl_xor_sync(FULL, tm, 2));
+                f[h] = 1.0f;
+                if (tm > m[h]) {
+                    f[h] = ex2_approx_ftz((m[h] - tm) * PD_LOG2);
+                    m[h] = tm;
+                    grow = true;
+                }
+                const float off = m[h] == -INFINITY ? 0.0f : -m[h] * PD_LOG2;
+                float add = 0.0f;
+#pragma unroll
+                for (int n = 0; n < KW / 8; ++n)
+#pragma unroll
+                    for (int x = 2 * h; x < 2 * h + 2; ++x) {
+                        s[n][x] = ex2_approx_ftz(fmaf(s[n][x], PD_LOG2, off));
+                        add += s[n][x];
+                    }
+                l[h] = fmaf(l[h], f[h], add);
+            }
+            if (__any_sync(FULL, grow)) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+#pragma unroll
+                    for (int x = 0; x < 2 * NH; ++x) o[j][x] *= f[x >> 1];
+            }
+            // the weighted values
+            if constexpr (CF32) {
+                // k index t4 is position 2 t4, t4 + 4 is 2 t4 + 1: the columns this thread's scores have;
+                // column n of product (d, x) is dimension 32 d + 4 n + x
+                uint32_t ph[4] = {0, 0, 0, 0}, pl[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int h = 0; h < NH; ++h) {
+                    split_tf32(s[0][2 * h], ph[h], pl[h]);
+                    split_tf32(s[0][2 * h + 1], ph[2 + h], pl[2 + h]);
+                }
+                const int k0 = warp * KW + 2 * t4;
+                const bool live0 = 2 * t4 < left, live1 = 2 * t4 + 1 < left;
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    const uint32_t blk = va + d * (PD_SIDE / 4);
+                    const float4 v0 = lds4(blk + k0 * 128 + ((g ^ (k0 & 7)) << 4));
+                    const float4 v1 = lds4(blk + (k0 + 1) * 128 + ((g ^ ((k0 + 1) & 7)) << 4));
+                    const float a0[4] = {v0.x, v0.y, v0.z, v0.w}, a1[4] = {v1.x, v1.y, v1.z, v1.w};
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        uint32_t bh[2], bl[2];
+                        split_tf32(live0 ? a0[x] : 0.0f, bh[0], bl[0]);
+                        split_tf32(live1 ? a1[x] : 0.0f, bh[1], bl[1]);
+                        mma_tf32(o[4 * d + x], pl[0], pl[1], pl[2], pl[3], bh[0], bh[1]);
+                        mma_tf32(o[4 * d + x], ph[0], ph[1], ph[2], ph[3], bl[0], bl[1]);
+                        mma_tf32(o[4 * d + x], ph[0], ph[1], ph[2], ph[3], bh[0], bh[1]);
+                    }
+                }
+            } else {
+                uint32_t ph[4] = {0, 0, 0, 0}, pl[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int h = 0; h < NH; ++h) split_bf16(s[n][2 * h], s[n][2 * h + 1], ph[2 * n + h], pl[2 * n + h]);
+                // keep[n]: which of the positions 8 n + 2 t4, + 1 exist
+                uint32_t keep[2];
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+                    keep[n] = (8 * n + 2 * t4 < left ? 0xffffu : 0u) | (8 * n + 2 * t4 + 1 < left ? 0xffff0000u : 0u);
+                const int key = warp * KW + ((lane >> 3) & 1) * 8 + (lane & 7);
+#pragma unroll
+                for (int d = 0; d < 8; ++d) {
+                    const int chunk = 2 * d + (lane >> 4);
+                    uint32_t r[4];
+                    ldsm4_t(va + (chunk >> 3) * (PD_SIDE / 2) + key * 128 + (((chunk & 7) ^ (key & 7)) << 4), r);
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) r[x] &= keep[x & 1];
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+                        mma_bf16(o[2 * d + n], pl[0], pl[1], pl[2], pl[3], r[2 * n], r[2 * n + 1]);
+                        mma_bf16(o[2 * d + n], ph[0], ph[1], ph[2], ph[3], r[2 * n], r[2 * n + 1]);
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[st]);
+        }
+        if (!ok && lane == 0) dead = 1;
+        // join the four warps into warp 0, one after the other through shared memory
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+            l[h] += __shfl_xor_sync(FULL, l[h], 1);
+            l[h] += __shfl_xor_sync(FULL, l[h], 2);
+        }
+        for (int src = 1; src < PD_WARPS; ++src) {
+            named_sync(1, PD_WARPS * 32);
+            if (warp == src) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+#pragma unroll
+                    for (int x = 0; x < 2 * NH; ++x) spare[(j * 2 * NH + x) * 32 + lane] = o[j][x];
+#pragma unroll
+                for (int h = 0; h < NH; ++h)
+                    if (t4 == 0) join_m[h][g] = m[h], join_l[h][g] = l[h];
+            }
+            named_sync(1, PD_WARPS * 32);
+            if (warp == 0) {
+                float f0[NH], f1[NH];
+#pragma unroll
+                for (int h = 0; h < NH; ++h) {
+                    const float om = join_m[h][g], nm = fmaxf(m[h], om);
+                    f0[h] = m[h] == nm ? 1.0f : ex2_approx_ftz((m[h] - nm) * PD_LOG2);
+                    f1[h] = om == nm ? 1.0f : ex2_approx_ftz((om - nm) * PD_LOG2);
+                    m[h] = nm;
+                    l[h] = l[h] * f0[h] + join_l[h][g] * f1[h];
+                }
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+#pragma unroll
+                    for (int x = 0; x < 2 * NH; ++x)
+                        o[j][x] = fmaf(o[j][x], f0[x >> 1], spare[(j * 2 * NH + x) * 32 + lane] * f1[x >> 1]);
+            }
+        }
+        ok = dead == 0;                                      // the same for every warp: the next barrier follows the read
+        if (warp == 0 && ok) {
+            const bool whole = run == w.tiles;
+            const int slot = 2 * int(blockIdx.x) + (u != u0);
+#pragma unroll
+            for (int h = 0; h < NH; ++h) {
+                const int row = g + 8 * h;
+                if (row >= group) continue;
+                const float r = whole ? 1.0f / l[h] : 1.0f;
+                typename Elem<T>::type *dst = out + (int64_t(w.s) * n_heads + w.head * group + row) * HD;
+                float *pd = part + (int64_t(slot) * group + row) * PD_PART;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const int at = CF32 ? 32 * (j >> 2) + 8 * t4 + (j & 3) : 8 * j + 2 * t4;
+                    const float x = o[j][2 * h] * r, y = o[j][2 * h + 1] * r;
+                    if (whole) put2(dst + at, CF32 ? 4 : 1, x, y);
+                    else put2(pd + at, CF32 ? 4 : 1, x, y);
+                }
+                if (!whole && t4 == 0) pd[HD] = m[h], pd[HD + 1] = l[h];
+            }
+        }
+        u += run;
+        if (u < u1) walk_on<TC>(b, c, w, run);
+        named_sync(1, PD_WARPS * 32);
+    }
+}
+
+// Joins what the runs left of one (sequence, query head): o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i, in the
+// order of the positions.  Runs are recognised as the first kernel (of `runs` CTAs) cut them.
+template <typename T, typename TC>
+__global__ void __launch_bounds__(HD) paged_join_kernel(const PagedKV c, const PagedSeqs b, int n_heads, int group, int runs,
+                                                        typename Elem<T>::type *out, const float *part) {
+    griddep_wait();
+    const int s = int(blockIdx.x) / n_heads, h = int(blockIdx.x) % n_heads, kh = h / group, d = threadIdx.x;
+    const int tiles = (paged_len(b, c, s, nullptr) + pd_tile<TC>() - 1) / pd_tile<TC>();
+    typename Elem<T>::type *dst = out + int64_t(blockIdx.x) * HD + d;
+    auto put = [&](float v) {
+        if constexpr (Elem<T>::BYTES == 4) *dst = v;
+        else *dst = uint16_t(f32_to_bf16(v));
+    };
+    if (tiles == 0) {
+        put(0.0f);
+        return;
+    }
+    const int64_t total = walk_total<TC>(b, c, nullptr);
+    const int64_t a = walk_before<TC>(b, c, s) + int64_t(kh) * tiles, z = a + tiles - 1;     // first and last tile
+    // run i has the tiles total * i / runs .. total * (i + 1) / runs - 1
+    const int first = int(((a + 1) * runs - 1) / total), last = int(((z + 1) * runs - 1) / total);
+    if (first == last) return;                               // one run had it whole
+    auto row_of = [&](int i) {
+        const int slot = 2 * i + (i == first && a != total * i / runs);
+        return part + (int64_t(slot) * group + h % group) * PD_PART;
+    };
+    float m = -INFINITY;
+    for (int i = first; i <= last; ++i)
+        if (total * i / runs < total * (i + 1) / runs) m = fmaxf(m, row_of(i)[HD]);
+    float o = 0.0f, l = 0.0f;
+    for (int i = first; i <= last; ++i) {
+        if (total * i / runs == total * (i + 1) / runs) continue;          // a run without tiles
+        const float *p = row_of(i);
+        const float f = p[HD] == m ? 1.0f : ex2_approx_ftz((p[HD] - m) * PD_LOG2);
+        o = fmaf(p[d], f, o);
+        l = fmaf(p[HD + 1], f, l);
+    }
+    put(o / l);
+}
+
+size_t attention_paged_workspace(int n_heads, int n_kv, int sms) {
+    return size_t(2 * sms) * 2 * (n_heads / n_kv) * PD_PART * sizeof(float);
+}
+
+// Tensor map of the pages: boxes of 128 B by the rows of a page that one box takes.
+template <typename TC>
+static bool page_map(CUtensorMap *map, const void *base, const PagedKV &c) {
+    const uint64_t size = uint64_t(1) << c.page_shift, es = Elem<TC>::BYTES;
+    const uint64_t dims[4] = {HD, size, uint64_t(c.n_kv), uint64_t(c.n_pages)};
+    const uint64_t strides[3] = {HD * es, size * HD * es, uint64_t(c.page_stride) * es};
+    const uint32_t box[4] = {uint32_t(128 / es), uint32_t(size < uint64_t(pd_tile<TC>()) ? size : pd_tile<TC>()), 1, 1};
+    return encode_lines_map(map, base, es == 4 ? Q3CU_F32 : Q3CU_BF16, 4, dims, strides, box);
+}
+
+template <typename T, typename TC>
+static cudaError_t launch_split(const PagedKV &c, const PagedSeqs &b, const void *q, int64_t q_stride, int n_heads,
+                                void *work, void *out, uint32_t *status, cudaStream_t stream, int sms, int slot) {
+    typedef typename Elem<T>::type E;
+    CUtensorMap mk, mv;
+    if (!page_map<TC>(&mk, c.k, c) || !page_map<TC>(&mv, c.v, c)) return cudaErrorInvalidValue;
+    const int group = n_heads / c.n_kv, runs = 2 * sms;
+    auto *kernel = group > 8 ? paged_split_kernel<T, TC, true> : paged_split_kernel<T, TC, false>;
+    cudaError_t e = ensure_smem_attr(reinterpret_cast<const void *>(kernel), PD_SMEM, slot + (group > 8));
+    if (e != cudaSuccess) return e;
+    e = launch_dependent(kernel, dim3(runs), dim3(PD_THREADS), PD_SMEM, stream, mk, mv, c, b, static_cast<const E *>(q),
+                         q_stride, n_heads, group, static_cast<E *>(out), static_cast<float *>(work), status);
+    if (e != cudaSuccess) return e;
+    return launch_dependent(paged_join_kernel<T, TC>, dim3(unsigned(b.n_seqs) * unsigned(n_heads)), dim3(HD), 0, stream, c, b,
+                            n_heads, group, runs, static_cast<E *>(out), static_cast<const float *>(work));
+}
 
 cudaError_t launch_attention_paged(const PagedKV &c, q3cu_dtype cache_dt, const PagedSeqs &b, const void *q,
                                    q3cu_dtype dt, int64_t q_stride, int n_heads, void *work, void *out,
                                    uint32_t *status, cudaStream_t stream, int sms) {
-    const dim3 grid(unsigned((int64_t(b.n_seqs) * n_heads + 3) / 4)), block(128);
-    auto go = [&](auto kernel, auto *typed) {
-        typedef decltype(typed) P;
-        return launch_dependent(kernel, grid, block, 0, stream, c, b, static_cast<P>(const_cast<void *>(q)), q_stride,
-                                n_heads, static_cast<P>(out), status);
-    };
     if (dt == Q3CU_F32)
-        return cache_dt == Q3CU_F32 ? go(paged_rows_kernel<float, float>, (float *)nullptr)
-                                    : go(paged_rows_kernel<float, bf16raw>, (float *)nullptr);
-    return cache_dt == Q3CU_F32 ? go(paged_rows_kernel<bf16raw, float>, (uint16_t *)nullptr)
-                                : go(paged_rows_kernel<bf16raw, bf16raw>, (uint16_t *)nullptr);
+        return cache_dt == Q3CU_F32
+                   ? launch_split<float, float>(c, b, q, q_stride, n_heads, work, out, status, stream, sms, 33)
+                   : launch_split<float, bf16raw>(c, b, q, q_stride, n_heads, work, out, status, stream, sms, 35);
+    return cache_dt == Q3CU_F32
+               ? launch_split<bf16raw, float>(c, b, q, q_stride, n_heads, work, out, status, stream, sms, 37)
+               : launch_split<bf16raw, bf16raw>(c, b, q, q_stride, n_heads, work, out, status, stream, sms, 39);
 }
 
 }  // namespace q3

@@ -422,7 +422,7 @@ static bool page_map(CUtensorMap *map, const void *base, const PagedKV &c, int b
     const uint64_t dims[4] = {HD, size, uint64_t(c.n_kv), uint64_t(c.n_pages)};
     const uint64_t strides[3] = {HD * 2, size * HD * 2, uint64_t(c.page_stride) * 2};
     const uint32_t box[4] = {64, uint32_t(box_rows), 1, 1};
-    return encode_bf16_map(map, base, 4, dims, strides, box);
+    return encode_lines_map(map, base, Q3CU_BF16, 4, dims, strides, box);
 }
 
 cudaError_t launch_attention_prompt(const PagedKV &c, const PagedSeqs &b, int64_t rows, const void *q, q3cu_dtype dt,
@@ -436,7 +436,7 @@ cudaError_t launch_attention_prompt(const PagedKV &c, const PagedSeqs &b, int64_
     const uint64_t dims[3] = {HD, uint64_t(n_heads), uint64_t(rows)};
     const uint64_t strides[2] = {HD * 2, uint64_t(q_stride) * 2};
     const uint32_t box[3] = {64, uint32_t(group), uint32_t(qt)};
-    if (!encode_bf16_map(&mq, q, 3, dims, strides, box) || !page_map(&mk, c.k, c, br) || !page_map(&mv, c.v, c, br))
+    if (!encode_lines_map(&mq, q, Q3CU_BF16, 3, dims, strides, box) || !page_map(&mk, c.k, c, br) || !page_map(&mv, c.v, c, br))
         return cudaErrorInvalidValue;
     cudaError_t e = ensure_smem_attr(reinterpret_cast<const void *>(prompt_tc_kernel), PT_SMEM, 32);
     if (e != cudaSuccess) return e;

@@ -121,16 +121,17 @@ bool encode_row_lines_map_uncached(CUtensorMap *map, const void *base, uint64_t 
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-bool encode_bf16_map(CUtensorMap *map, const void *base, int rank, const uint64_t *dims, const uint64_t *strides,
-                     const uint32_t *box) {
+bool encode_lines_map(CUtensorMap *map, const void *base, q3cu_dtype dt, int rank, const uint64_t *dims,
+                      const uint64_t *strides, const uint32_t *box) {
     EncodeTiled enc = encoder();
-    if (!enc || box[0] != 64) return false;
+    if (!enc || box[0] != (dt == Q3CU_F32 ? 32 : 64)) return false;
     cuuint64_t d[4], st[3];
     for (int i = 0; i < rank; ++i) d[i] = dims[i];
     for (int i = 0; i + 1 < rank; ++i) st[i] = strides[i];
     const cuuint32_t estr[4] = {1, 1, 1, 1};
-    return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, cuuint32_t(rank), const_cast<void *>(base), d, st, box, estr,
-               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+    return enc(map, dt == Q3CU_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+               cuuint32_t(rank), const_cast<void *>(base), d, st, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 

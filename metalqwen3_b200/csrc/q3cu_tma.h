@@ -11,6 +11,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "q3cu.h"
+
 namespace q3 {
 
 // A row-major [rows][row_bytes] byte array viewed as 3-D for TMA: dim 0 = the
@@ -41,12 +43,12 @@ bool encode_rows_2d_map(CUtensorMap *map, const void *base, uint64_t rows, uint6
 bool encode_f32_2d_map(CUtensorMap *map, const void *base, uint64_t rows, uint64_t cols, uint32_t box_cols,
                        uint32_t box_rows, bool swizzle128);
 
-// A bf16 tensor of `rank` (3 or 4) dimensions, innermost first and dense in dimension 0 (strides[i]: bytes between
-// neighbours in dimension i + 1, multiples of 16), read in boxes of 64 elements by box[1..]; a box lands as lines
-// of 128 B with the 128-byte swizzle (1024-byte aligned), elements outside the tensor as zeros.  Encoded anew by
-// every call (a fraction of a microsecond).
-bool encode_bf16_map(CUtensorMap *map, const void *base, int rank, const uint64_t *dims, const uint64_t *strides,
-                     const uint32_t *box);
+// A tensor of `rank` (3 or 4) dimensions of dt, innermost first and dense in dimension 0 (strides[i]: bytes between
+// neighbours in dimension i + 1, multiples of 16), read in boxes of 128 B (64 bf16 or 32 f32) by box[1..]; a box
+// lands as lines of 128 B with the 128-byte swizzle (1024-byte aligned), elements outside the tensor as zeros.
+// Encoded anew by every call (a fraction of a microsecond).
+bool encode_lines_map(CUtensorMap *map, const void *base, q3cu_dtype dt, int rank, const uint64_t *dims,
+                      const uint64_t *strides, const uint32_t *box);
 
 #if defined(__CUDACC__)
 __device__ __forceinline__ void tma_load_2d(void *dst, const CUtensorMap *map, int x, int y, uint64_t *bar) {
