@@ -218,7 +218,8 @@ typedef struct {
     const int32_t *row_off;  /* [n_seqs + 1], rising from 0 (not read by q3cu_attention_paged) */
     const int32_t *kv_len;   /* [n_seqs] */
     const int32_t *pages;    /* [n_seqs][max_pages] */
-    int32_t n_seqs, max_pages;   /* max_pages * page_size < 2^31 */
+    int32_t n_seqs;              /* at most 2^24 */
+    int32_t max_pages;           /* max_pages * page_size < 2^31 */
 } q3cu_kv_batch;
 
 /* QK-RMSNorm and rotation of the packed rows, keys and values into the cache

@@ -55,11 +55,6 @@ kv_append_kernel(const PagedKV c, const PagedSeqs b, int64_t rows, const typenam
     const int64_t r = w / groups;
     const int u0 = int(w % groups) * APPEND_UNITS, units = n_heads + 2 * c.n_kv;
     if (r >= rows) return;
-    const int s = paged_seq_of(b, r);
-    if (s < 0) return;                                       // a row behind the last sequence
-    const int pos = paged_pos(b, c, s, r, lane == 0 ? status : nullptr);
-    if (pos < 0) return;                                     // padding, or beyond the table
-
     float2 lo[APPEND_UNITS], hi[APPEND_UNITS];
 #pragma unroll
     for (int i = 0; i < APPEND_UNITS; ++i) {
@@ -72,6 +67,11 @@ kv_append_kernel(const PagedKV c, const PagedSeqs b, int64_t rows, const typenam
         lo[i] = load_pair(x + 2 * lane);
         hi[i] = load_pair(x + 64 + 2 * lane);
     }
+    // the place, while the loads above are under way
+    const int s = paged_seq_of_warp(b, r);
+    if (s < 0) return;                                       // a row behind the last sequence
+    const int pos = paged_pos(b, c, s, r, lane == 0 ? status : nullptr);
+    if (pos < 0) return;                                     // padding, or beyond the table
     int page = -1;
     if (u0 + APPEND_UNITS > n_heads) page = paged_page(b, c, s, pos, lane == 0 ? status : nullptr);
     float cs[2], sn[2];

@@ -79,50 +79,70 @@ __device__ __forceinline__ void split_tf32(float x, uint32_t &hi, uint32_t &lo) 
     lo = __float_as_uint(x - __uint_as_float(hi));
 }
 
+// a / b for 0 <= a, 0 < b: 32-bit division where it serves (a 64-bit one is a chain of some hundred instructions).
+__device__ __forceinline__ int64_t quot(int64_t a, int b) {
+    return a < (int64_t(1) << 32) ? int64_t(uint32_t(a) / uint32_t(b)) : a / b;
+}
+
+// How `total` tiles are cut into `runs` runs: the first `more` have each + 1 tiles, the others `each`.
+struct PagedCut {
+    int64_t total, each;
+    int more;
+    __device__ __forceinline__ PagedCut(int64_t t, int runs) : total(t), each(quot(t, runs)), more(int(t - each * runs)) {}
+    __device__ __forceinline__ int64_t begin(int run) const { return each * run + min(run, more); }
+    __device__ __forceinline__ int run_of(int64_t u) const {                 // u < total
+        const int64_t edge = (each + 1) * more;
+        return u < edge ? int(each < INT32_MAX ? quot(u, int(each + 1)) : u / (each + 1))
+                        : more + int(each < INT32_MAX ? quot(u - edge, int(each)) : (u - edge) / each);
+    }
+};
+
 // A place in the batch's tiles: sequence, kv head, tile, and the sequence's length and tiles.
 struct PagedWalk {
     int s, head, tile, len, tiles;
 };
 template <typename TC>
-__device__ __forceinline__ int64_t walk_total(const PagedSeqs &b, const PagedKV &c, uint32_t *status) {
-    int64_t n = 0;
-    for (int s = threadIdx.x & 31; s < b.n_seqs; s += 32) n += (paged_len(b, c, s, status) + pd_tile<TC>() - 1) / pd_tile<TC>();
+__device__ __forceinline__ int tiles_of(int len) { return (len + pd_tile<TC>() - 1) / pd_tile<TC>(); }
+
+__device__ __forceinline__ int64_t warp_prefix(int64_t x) {                 // inclusive, over the lanes
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(FULL, n, o);
-    return n * c.n_kv;
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(FULL, x, o);
+        if ((threadIdx.x & 31) >= o) x += y;
+    }
+    return x;
 }
-// Tiles of the sequences before s (one warp).
+// The tiles of the whole batch, the run's [u0, u1) of them and the place of u0 (one warp; every lane returns it).
 template <typename TC>
-__device__ __forceinline__ int64_t walk_before(const PagedSeqs &b, const PagedKV &c, int s) {
-    int64_t n = 0;
-    for (int i = threadIdx.x & 31; i < s; i += 32) n += (paged_len(b, c, i, nullptr) + pd_tile<TC>() - 1) / pd_tile<TC>();
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(FULL, n, o);
-    return n * c.n_kv;
-}
-// The place of tile u < total (one warp; every lane returns it).
-template <typename TC>
-__device__ __forceinline__ PagedWalk walk_to(const PagedSeqs &b, const PagedKV &c, int64_t u) {
+__device__ __forceinline__ PagedWalk walk_run(const PagedSeqs &b, const PagedKV &c, int run, int runs, PagedCut &cut,
+                                              int64_t &u0, int64_t &u1, uint32_t *status) {
     PagedWalk w = {};
     const int lane = threadIdx.x & 31;
+    int64_t total = 0, end = 0;
+    int len = 0;
+    for (int s0 = 0; s0 < b.n_seqs; s0 += 32) {              // 32 sequences at a time
+        len = s0 + lane < b.n_seqs ? paged_len(b, c, s0 + lane, status) : 0;
+        end = warp_prefix(int64_t(tiles_of<TC>(len)) * c.n_kv);
+        total += __shfl_sync(FULL, end, 31);
+    }
+    cut = PagedCut(total, runs);
+    u0 = cut.begin(run);
+    u1 = cut.begin(run + 1);
+    int64_t u = u0;
     for (int s0 = 0; s0 < b.n_seqs; s0 += 32) {
-        const int len = s0 + lane < b.n_seqs ? paged_len(b, c, s0 + lane, nullptr) : 0;
-        const int tiles = (len + pd_tile<TC>() - 1) / pd_tile<TC>();
-        int64_t end = int64_t(tiles) * c.n_kv;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int64_t x = __shfl_up_sync(FULL, end, o);
-            if (lane >= o) end += x;
+        if (b.n_seqs > 32) {                                 // otherwise the lanes still hold them
+            len = s0 + lane < b.n_seqs ? paged_len(b, c, s0 + lane, nullptr) : 0;
+            end = warp_prefix(int64_t(tiles_of<TC>(len)) * c.n_kv);
         }
         const unsigned hit = __ballot_sync(FULL, u < end);
         if (hit) {
             const int l = __ffs(hit) - 1;
             w.s = s0 + l;
             w.len = __shfl_sync(FULL, len, l);
-            w.tiles = __shfl_sync(FULL, tiles, l);
+            w.tiles = tiles_of<TC>(w.len);
             const int64_t at = u - (__shfl_sync(FULL, end, l) - int64_t(w.tiles) * c.n_kv);
-            w.head = int(at / w.tiles);
-            w.tile = int(at % w.tiles);
+            w.head = int(quot(at, w.tiles));
+            w.tile = int(at - int64_t(w.head) * w.tiles);
             return w;
         }
         u -= __shfl_sync(FULL, end, 31);
@@ -141,7 +161,7 @@ __device__ __forceinline__ void walk_on(const PagedSeqs &b, const PagedKV &c, Pa
         if (++w.s >= b.n_seqs) return;
         w.len = paged_len(b, c, w.s, nullptr);
     } while (w.len == 0);
-    w.tiles = (w.len + pd_tile<TC>() - 1) / pd_tile<TC>();
+    w.tiles = tiles_of<TC>(w.len);
 }
 
 // One pair of result elements (row, dims at, at + step) as the output's type.
@@ -178,10 +198,15 @@ paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
     griddep_wait();
     griddep_launch_dependents();
 
-    const int64_t total = walk_total<TC>(b, c, blockIdx.x == 0 && warp == 0 ? status : nullptr);
-    const int64_t u0 = total * blockIdx.x / gridDim.x, u1 = total * (blockIdx.x + 1) / gridDim.x;
+    PagedCut cut(0, 1);
+    int64_t u0, u1;
+    PagedWalk w = walk_run<TC>(b, c, int(blockIdx.x), int(gridDim.x), cut, u0, u1,
+                               blockIdx.x == 0 && warp == 0 ? status : nullptr);
+    for (int s = int(blockIdx.x); s < b.n_seqs; s += int(gridDim.x))       // sequences without positions: zeros
+        if (b.kv_len[s] <= 0 || b.max_pages == 0)
+            for (int i = threadIdx.x; i < n_heads * (HD / 4); i += PD_THREADS)
+                store_quad(out + int64_t(s) * n_heads * HD + 4 * i, make_float4(0.0f, 0.0f, 0.0f, 0.0f));
     if (u0 == u1) return;
-    PagedWalk w = walk_to<TC>(b, c, u0);
 
     if (warp == PD_WARPS) {
         // ---- fetch: lane = box (K or V, column block, rows of one page) ------------------
@@ -469,48 +494,71 @@ paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
     }
 }
 
-// Joins what the runs left of one (sequence, query head): o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i, in the
-// order of the positions.  Runs are recognised as the first kernel (of `runs` CTAs) cut them.
+// Joins what the runs left of one query head, one CTA per run and head of the group; the CTA of the second run of a
+// (sequence, kv head) does it: o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i.  The
+// parts' maxima and sums are read side by side, one thread each; then two groups of 128 threads (thread = element) add
+// half of the weighted parts each, eight loads under way at a time.  The order of every sum is fixed.
+constexpr int PJ_GROUPS = 2, PJ_THREADS = PJ_GROUPS * HD, PJ_RUNS = 1024;
 template <typename T, typename TC>
-__global__ void __launch_bounds__(HD) paged_join_kernel(const PagedKV c, const PagedSeqs b, int n_heads, int group, int runs,
-                                                        typename Elem<T>::type *out, const float *part) {
+__global__ void __launch_bounds__(PJ_THREADS) paged_join_kernel(const PagedKV c, const PagedSeqs b, int n_heads, int group,
+                                                                int runs, typename Elem<T>::type *out, const float *part) {
+    __shared__ float weight[PJ_RUNS], red[2][PJ_THREADS / 32], sum[PJ_GROUPS][HD];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = threadIdx.x % HD, half_id = threadIdx.x / HD;
+    // Before the wait: the lengths are older than the first kernel, which has begun (this one starts when all its CTAs
+    // have passed their own wait).
+    PagedCut cut(0, 1);
+    int64_t u0, u1;
+    const int second = int(blockIdx.x) + 1;
+    const PagedWalk w = walk_run<TC>(b, c, second, runs, cut, u0, u1, nullptr);
+    if (u0 == u1 || w.tile == 0) return;                     // no tiles, or it begins with a new (sequence, head)
+    const int64_t a = u0 - w.tile;                           // the (sequence, head)'s first tile
+    const int first = second - 1, last = cut.run_of(a + w.tiles - 1), n = last - first + 1;
+    if (a < cut.begin(first)) return;                        // not the second of its runs
     griddep_wait();
-    const int s = int(blockIdx.x) / n_heads, h = int(blockIdx.x) % n_heads, kh = h / group, d = threadIdx.x;
-    const int tiles = (paged_len(b, c, s, nullptr) + pd_tile<TC>() - 1) / pd_tile<TC>();
-    typename Elem<T>::type *dst = out + int64_t(blockIdx.x) * HD + d;
-    auto put = [&](float v) {
-        if constexpr (Elem<T>::BYTES == 4) *dst = v;
-        else *dst = uint16_t(f32_to_bf16(v));
-    };
-    if (tiles == 0) {
-        put(0.0f);
-        return;
-    }
-    const int64_t total = walk_total<TC>(b, c, nullptr);
-    const int64_t a = walk_before<TC>(b, c, s) + int64_t(kh) * tiles, z = a + tiles - 1;     // first and last tile
-    // run i has the tiles total * i / runs .. total * (i + 1) / runs - 1
-    const int first = int(((a + 1) * runs - 1) / total), last = int(((z + 1) * runs - 1) / total);
-    if (first == last) return;                               // one run had it whole
-    auto row_of = [&](int i) {
-        const int slot = 2 * i + (i == first && a != total * i / runs);
-        return part + (int64_t(slot) * group + h % group) * PD_PART;
-    };
+    // part i: in the first slot of run first + i, but the second of a run that began before this (sequence, head)
+    const float *row = part + int(blockIdx.y) * PD_PART;
+    const int64_t run_stride = int64_t(2) * group * PD_PART;
+    const float *head = row + first * run_stride + (a != cut.begin(first) ? group * PD_PART : 0);
+    auto at = [&](int i) { return i == 0 ? head : row + (first + i) * run_stride; };
     float m = -INFINITY;
-    for (int i = first; i <= last; ++i)
-        if (total * i / runs < total * (i + 1) / runs) m = fmaxf(m, row_of(i)[HD]);
-    float o = 0.0f, l = 0.0f;
-    for (int i = first; i <= last; ++i) {
-        if (total * i / runs == total * (i + 1) / runs) continue;          // a run without tiles
-        const float *p = row_of(i);
-        const float f = p[HD] == m ? 1.0f : ex2_approx_ftz((p[HD] - m) * PD_LOG2);
-        o = fmaf(p[d], f, o);
-        l = fmaf(p[HD + 1], f, l);
+    for (int i = threadIdx.x; i < n; i += PJ_THREADS) {
+        weight[i] = at(i)[HD];
+        m = fmaxf(m, weight[i]);
     }
-    put(o / l);
+    m = warp_max(m);
+    if (lane == 0) red[0][warp] = m;
+    __syncthreads();
+    m = warp_max(red[0][lane % (PJ_THREADS / 32)]);
+    float l = 0.0f;
+    for (int i = threadIdx.x; i < n; i += PJ_THREADS) {
+        const float f = weight[i] == m ? 1.0f : ex2_approx_ftz((weight[i] - m) * PD_LOG2);
+        weight[i] = f;
+        l = fmaf(at(i)[HD + 1], f, l);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(FULL, l, o);
+    if (lane == 0) red[1][warp] = l;
+    __syncthreads();
+    float o = 0.0f;
+    const int i0 = n * half_id / PJ_GROUPS, i1 = n * (half_id + 1) / PJ_GROUPS;
+#pragma unroll 8
+    for (int i = i0; i < i1; ++i) o = fmaf(at(i)[d], weight[i], o);
+    sum[half_id][d] = o;
+    __syncthreads();
+    if (half_id) return;
+    l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < PJ_THREADS / 32; ++i) l += red[1][i];
+    o = (sum[0][d] + sum[1][d]) / l;
+    typename Elem<T>::type *dst = out + (int64_t(w.s) * n_heads + w.head * group + blockIdx.y) * HD + d;
+    if constexpr (Elem<T>::BYTES == 4) *dst = o;
+    else *dst = uint16_t(f32_to_bf16(o));
 }
 
+static int paged_runs(int sms) { return 2 * sms < PJ_RUNS ? 2 * sms : PJ_RUNS; }
+
 size_t attention_paged_workspace(int n_heads, int n_kv, int sms) {
-    return size_t(2 * sms) * 2 * (n_heads / n_kv) * PD_PART * sizeof(float);
+    return size_t(paged_runs(sms)) * 2 * (n_heads / n_kv) * PD_PART * sizeof(float);
 }
 
 // Tensor map of the pages: boxes of 128 B by the rows of a page that one box takes.
@@ -529,14 +577,14 @@ static cudaError_t launch_split(const PagedKV &c, const PagedSeqs &b, const void
     typedef typename Elem<T>::type E;
     CUtensorMap mk, mv;
     if (!page_map<TC>(&mk, c.k, c) || !page_map<TC>(&mv, c.v, c)) return cudaErrorInvalidValue;
-    const int group = n_heads / c.n_kv, runs = 2 * sms;
+    const int group = n_heads / c.n_kv, runs = paged_runs(sms);
     auto *kernel = group > 8 ? paged_split_kernel<T, TC, true> : paged_split_kernel<T, TC, false>;
     cudaError_t e = ensure_smem_attr(reinterpret_cast<const void *>(kernel), PD_SMEM, slot + (group > 8));
     if (e != cudaSuccess) return e;
     e = launch_dependent(kernel, dim3(runs), dim3(PD_THREADS), PD_SMEM, stream, mk, mv, c, b, static_cast<const E *>(q),
                          q_stride, n_heads, group, static_cast<E *>(out), static_cast<float *>(work), status);
     if (e != cudaSuccess) return e;
-    return launch_dependent(paged_join_kernel<T, TC>, dim3(unsigned(b.n_seqs) * unsigned(n_heads)), dim3(HD), 0, stream, c, b,
+    return launch_dependent(paged_join_kernel<T, TC>, dim3(runs - 1, group), dim3(PJ_THREADS), 0, stream, c, b,
                             n_heads, group, runs, static_cast<E *>(out), static_cast<const float *>(work));
 }
 

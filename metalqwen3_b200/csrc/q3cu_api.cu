@@ -497,7 +497,7 @@ static q3cu_status check_paged(const char *op, const q3cu_kv_cache *cache, const
     while (shift < 8 && (1 << shift) != cache->page_size) ++shift;
     if ((1 << shift) != cache->page_size)
         return fail(Q3CU_ERR_INVALID, "%s: page_size %d is not 16, 32, 64, 128 or 256", op, cache->page_size);
-    if (cache->n_kv <= 0 || cache->n_pages <= 0 || batch->n_seqs < 0 || batch->max_pages < 0)
+    if (cache->n_kv <= 0 || cache->n_pages <= 0 || batch->n_seqs < 0 || batch->n_seqs > (1 << 24) || batch->max_pages < 0)
         return fail(Q3CU_ERR_INVALID, "%s: n_kv=%d n_pages=%d n_seqs=%d max_pages=%d", op, cache->n_kv,
                     cache->n_pages, batch->n_seqs, batch->max_pages);
     if (n_heads < 0 || n_heads % cache->n_kv || n_heads / cache->n_kv > q3::PAGED_GROUP_MAX)

@@ -68,6 +68,28 @@ __host__ __device__ __forceinline__ int paged_seq_of(const PagedSeqs &b, int64_t
     return b.n_seqs > 0 && b.row_off[lo] <= r && r < b.row_off[lo + 1] ? lo : -1;
 }
 
+// The same by a whole warp: 33-way search, one round of loads for up to 31 sequences and two for up to 1,023.
+__device__ __forceinline__ int paged_seq_of_warp(const PagedSeqs &b, int64_t r) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, hi = b.n_seqs;                               // as above
+    int64_t at_lo = 0, at_hi = 0;
+    bool have_lo = false, have_hi = false;
+    while (hi - lo > 1 || !have_lo || !have_hi) {
+        // probes lo, lo + step, ..., and hi in the last lane
+        const int step = (hi - lo + 30) / 31, p = lane == 31 ? hi : min(lo + lane * step, hi);
+        const int64_t x = b.row_off[p];
+        const unsigned below = __ballot_sync(FULL, x <= r && p < hi) & 0x7fffffffu;
+        const int l = below ? 31 - __clz(below) : 0;         // the last probe at or before r
+        const int nl = __shfl_sync(FULL, p, l), nh = __shfl_sync(FULL, p, l + 1);
+        at_lo = __shfl_sync(FULL, x, l);
+        at_hi = __shfl_sync(FULL, x, l + 1);
+        have_lo = have_hi = true;
+        lo = nl;
+        hi = nh;
+    }
+    return b.n_seqs > 0 && at_lo <= r && r < at_hi ? lo : -1;
+}
+
 // Position of packed row r of sequence s (as paged_seq_of finds it): negative for padding before position 0, and,
 // flagged, beyond the table's pages.
 __host__ __device__ __forceinline__ int paged_pos(const PagedSeqs &b, const PagedKV &c, int s, int64_t r,
