@@ -17,14 +17,18 @@
 // binary32; the one rounding to fewer bits is the store.
 //
 // Bound by memory: every element is read once and written once.  A warp takes
-// APPEND_UNITS heads of one row: lane l holds elements 2l, 2l+1, 64+2l, 65+2l
-// of each, so both halves of a rotated pair are in one lane, a half row is one
-// contiguous access, and the two angles of a lane serve all its heads.
+// one row, or with few rows a part of its heads, in batches of APPEND_HEADS
+// heads of one kind: lane l holds elements 2l, 2l+1, 64+2l, 65+2l of each head,
+// so both halves of a rotated pair are in one lane, a half row is one contiguous
+// access, and the two angles of a lane, found once, serve all its heads.  The
+// row is on its way to L2 while the warp finds its sequence, position and page.
 #include "q3cu_paged.cuh"
 
 namespace q3 {
 
-constexpr int APPEND_UNITS = 4, APPEND_WARPS = 8;
+__device__ __forceinline__ void prefetch_l2(const void *p) { asm volatile("prefetch.global.L2 [%0];" :: "l"(p)); }
+
+constexpr int APPEND_HEADS = 4, APPEND_WARPS = 8;
 
 // Coherent loads: q_out may be q itself (a lane reads its elements before it stores them).
 __device__ __forceinline__ float2 load_pair(const float *p) { return *reinterpret_cast<const float2 *>(p); }
@@ -32,124 +36,153 @@ __device__ __forceinline__ float2 load_pair(const uint16_t *p) {
     const uint32_t u = *reinterpret_cast<const uint32_t *>(p);
     return make_float2(bf16_to_f32(u & 0xffffu), bf16_to_f32(u >> 16));
 }
-__device__ __forceinline__ void store_pair(void *base, int64_t at, bool bf16, float2 v) {
-    if (bf16)
-        *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(base) + at) = f32_to_bf16(v.x) | (f32_to_bf16(v.y) << 16);
-    else
-        *reinterpret_cast<float2 *>(static_cast<float *>(base) + at) = v;
+// v as elements at, at + 1 of base.
+template <bool BF16>
+__device__ __forceinline__ void store_pair(void *base, int64_t at, float2 v) {
+    if constexpr (BF16) *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(base) + at) = pack_bf16(v.x, v.y);
+    else *reinterpret_cast<float2 *>(static_cast<float *>(base) + at) = v;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(APPEND_WARPS * 32)
-kv_append_kernel(const PagedKV c, const PagedSeqs b, int64_t rows, const typename Elem<T>::type *q,
+// Up to APPEND_HEADS heads from x (this lane's elements of the first), `step` elements apart where they go; turned by
+// w if ROTATE, and normalised before if `norm` (the norm's weights are in w).
+struct Turn { float2 c[2], s[2]; };                          // weight * cosine, weight * sine of both halves
+template <typename E, bool BF16, bool ROTATE>
+__device__ __forceinline__ void append_heads(const E *x, int n, bool norm, float eps, const Turn &w, void *to, int64_t at,
+                                             int64_t step) {
+    float2 l[APPEND_HEADS], h[APPEND_HEADS];
+#pragma unroll
+    for (int i = 0; i < APPEND_HEADS; ++i) {
+        l[i] = h[i] = make_float2(0.0f, 0.0f);
+        if (i < n) {
+            l[i] = load_pair(x + i * HD);
+            h[i] = load_pair(x + i * HD + 64);
+        }
+    }
+    if constexpr (ROTATE) {
+        float g[APPEND_HEADS] = {1.0f, 1.0f, 1.0f, 1.0f};
+        if (norm) {
+#pragma unroll
+            for (int i = 0; i < APPEND_HEADS; ++i)
+                g[i] = fmaf(l[i].x, l[i].x, fmaf(l[i].y, l[i].y, fmaf(h[i].x, h[i].x, h[i].y * h[i].y)));
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+                for (int i = 0; i < APPEND_HEADS; ++i) g[i] += __shfl_xor_sync(FULL, g[i], o);
+#pragma unroll
+            for (int i = 0; i < APPEND_HEADS; ++i) g[i] = rsqrtf(fmaf(g[i], 1.0f / HD, eps));
+        }
+#pragma unroll
+        for (int i = 0; i < APPEND_HEADS; ++i) {
+            const float2 y = make_float2(g[i] * l[i].x, g[i] * l[i].y), z = make_float2(g[i] * h[i].x, g[i] * h[i].y);
+            l[i] = make_float2(fmaf(y.x, w.c[0].x, -(z.x * w.s[1].x)), fmaf(y.y, w.c[0].y, -(z.y * w.s[1].y)));
+            h[i] = make_float2(fmaf(y.x, w.s[0].x, z.x * w.c[1].x), fmaf(y.y, w.s[0].y, z.y * w.c[1].y));
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < APPEND_HEADS; ++i)
+        if (i < n) {
+            store_pair<BF16>(to, at + i * step, l[i]);
+            store_pair<BF16>(to, at + i * step + 64, h[i]);
+        }
+}
+
+template <typename T, bool QB, bool CB>
+__global__ void __launch_bounds__(APPEND_WARPS * 32, 4)
+kv_append_kernel(const PagedKV c, const PagedSeqs b, int rows, const typename Elem<T>::type *q,
                  const typename Elem<T>::type *k, const typename Elem<T>::type *v, int64_t q_stride,
                  int64_t kv_stride, int n_heads, const float *__restrict__ q_norm, const float *__restrict__ k_norm,
-                 const __grid_constant__ TurnFreq freq, float eps, void *q_out, int q_bf16, int cache_bf16,
-                 int groups, uint32_t *status) {
+                 const __grid_constant__ TurnFreq freq, float eps, void *q_out, uint32_t *status) {
+    typedef typename Elem<T>::type E;
     __shared__ double turn[64];
     if (threadIdx.x < 64) turn[threadIdx.x] = freq.v[threadIdx.x];
     __syncthreads();
     griddep_wait();
-    const int lane = threadIdx.x & 31;
-    const int64_t w = int64_t(blockIdx.x) * APPEND_WARPS + (threadIdx.x >> 5);
-    const int64_t r = w / groups;
-    const int u0 = int(w % groups) * APPEND_UNITS, units = n_heads + 2 * c.n_kv;
+    const int lane = threadIdx.x & 31, r = int(blockIdx.x) * APPEND_WARPS + int(threadIdx.x >> 5);
     if (r >= rows) return;
-    float2 lo[APPEND_UNITS], hi[APPEND_UNITS];
-#pragma unroll
-    for (int i = 0; i < APPEND_UNITS; ++i) {
-        const int u = u0 + i;
-        lo[i] = hi[i] = make_float2(0.0f, 0.0f);
-        if (u >= units) continue;
-        const typename Elem<T>::type *x = u < n_heads             ? q + r * q_stride + int64_t(u) * HD
-                                          : u < n_heads + c.n_kv  ? k + r * kv_stride + int64_t(u - n_heads) * HD
-                                                                  : v + r * kv_stride + int64_t(u - n_heads - c.n_kv) * HD;
-        lo[i] = load_pair(x + 2 * lane);
-        hi[i] = load_pair(x + 64 + 2 * lane);
+    // the row's batches: of query heads, of key heads, of value heads; this warp's are first .. last - 1
+    const int qn = (n_heads + APPEND_HEADS - 1) / APPEND_HEADS, kn = (c.n_kv + APPEND_HEADS - 1) / APPEND_HEADS;
+    const int first = (qn + 2 * kn) * int(blockIdx.y) / int(gridDim.y);
+    const int last = (qn + 2 * kn) * int(blockIdx.y + 1) / int(gridDim.y);
+    const E *qr = q + r * q_stride, *kr = k + r * kv_stride, *vr = v + r * kv_stride;
+    constexpr int LINES = APPEND_HEADS * HD * int(sizeof(E)) / 128;        // 128-byte lines of a batch
+    for (int i = lane + LINES * first; i < LINES * last; i += 32) {
+        const int x = i / LINES, heads = x < qn ? n_heads : c.n_kv, at = x < qn ? x : x < qn + kn ? x - qn : x - qn - kn;
+        const int e = at * APPEND_HEADS * HD + i % LINES * (128 / int(sizeof(E)));
+        if (e < heads * HD) prefetch_l2((x < qn ? qr : x < qn + kn ? kr : vr) + e);
     }
-    // the place, while the loads above are under way
+
     const int s = paged_seq_of_warp(b, r);
     if (s < 0) return;                                       // a row behind the last sequence
     const int pos = paged_pos(b, c, s, r, lane == 0 ? status : nullptr);
     if (pos < 0) return;                                     // padding, or beyond the table
-    int page = -1;
-    if (u0 + APPEND_UNITS > n_heads) page = paged_page(b, c, s, pos, lane == 0 ? status : nullptr);
+    const int page = last > qn ? paged_page(b, c, s, pos, lane == 0 ? status : nullptr) : -1;
     float cs[2], sn[2];
-    if (u0 < n_heads + c.n_kv) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const double t = double(pos) * turn[2 * lane + e];
-            const double half = 2.0 * (t - rint(t));         // half turns in [-1, 1]
-            const float h = float(half), rest = 3.14159265f * float(half - double(h));
-            float s0, c0;
-            sincospif(h, &s0, &c0);
-            sn[e] = fmaf(c0, rest, s0);
-            cs[e] = fmaf(-s0, rest, c0);
-        }
+    for (int e = 0; e < 2; ++e) {
+        const double t = double(pos) * turn[2 * lane + e];
+        const double half = 2.0 * (t - rint(t));             // half turns in [-1, 1]
+        const float h = float(half), rest = 3.14159265f * float(half - double(h));
+        float s0, c0;
+        sincospif(h, &s0, &c0);
+        sn[e] = fmaf(c0, rest, s0);
+        cs[e] = fmaf(-s0, rest, c0);
     }
-    float ss[APPEND_UNITS];
+    auto weighted = [&](const float *n) {
+        Turn w;
 #pragma unroll
-    for (int i = 0; i < APPEND_UNITS; ++i)
-        ss[i] = fmaf(lo[i].x, lo[i].x, fmaf(lo[i].y, lo[i].y, fmaf(hi[i].x, hi[i].x, hi[i].y * hi[i].y)));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-#pragma unroll
-        for (int i = 0; i < APPEND_UNITS; ++i) ss[i] += __shfl_xor_sync(FULL, ss[i], o);
-#pragma unroll
-    for (int i = 0; i < APPEND_UNITS; ++i) {
-        const int u = u0 + i;
-        if (u >= units) break;
-        float2 a = lo[i], d = hi[i];
-        if (u < n_heads + c.n_kv) {
-            const float *wn = u < n_heads ? q_norm : k_norm;
-            if (wn) {
-                const float g = 1.0f / sqrtf(ss[i] * (1.0f / HD) + eps);
-                const float2 w0 = __ldg(reinterpret_cast<const float2 *>(wn) + lane);
-                const float2 w1 = __ldg(reinterpret_cast<const float2 *>(wn) + 32 + lane);
-                a = make_float2(w0.x * (g * a.x), w0.y * (g * a.y));
-                d = make_float2(w1.x * (g * d.x), w1.y * (g * d.y));
-            }
-            const float2 y = a, z = d;
-            a = make_float2(fmaf(y.x, cs[0], -(z.x * sn[0])), fmaf(y.y, cs[1], -(z.y * sn[1])));
-            d = make_float2(fmaf(y.x, sn[0], z.x * cs[0]), fmaf(y.y, sn[1], z.y * cs[1]));
+        for (int y = 0; y < 2; ++y) {
+            const float2 f = n ? __ldg(reinterpret_cast<const float2 *>(n) + 32 * y + lane) : make_float2(1.0f, 1.0f);
+            w.c[y] = make_float2(f.x * cs[0], f.y * cs[1]);
+            w.s[y] = make_float2(f.x * sn[0], f.y * sn[1]);
         }
-        void *base;
-        int64_t at;
-        bool bf16;
-        if (u < n_heads) {
-            base = q_out;
-            at = (r * n_heads + u) * HD;
-            bf16 = q_bf16 != 0;
-        } else {
-            if (page < 0) continue;                          // flagged above; nothing is stored
-            const bool key = u < n_heads + c.n_kv;
-            base = key ? c.k : c.v;
-            at = paged_at(c, page, u - n_heads - (key ? 0 : c.n_kv), pos);
-            bf16 = cache_bf16 != 0;
-        }
-        store_pair(base, at + 2 * lane, bf16, a);
-        store_pair(base, at + 64 + 2 * lane, bf16, d);
+        return w;
+    };
+    Turn w = weighted(q_norm);
+    for (int x = first; x < min(last, qn); ++x) {
+        const int u = x * APPEND_HEADS;
+        append_heads<E, QB, true>(qr + u * HD + 2 * lane, n_heads - u, q_norm, eps, w, q_out,
+                                  (int64_t(r) * n_heads + u) * HD + 2 * lane, HD);
+    }
+    if (page < 0) return;                                    // no keys or values here, or a bad page (flagged): none stored
+    const int64_t at = paged_at(c, page, 0, pos) + 2 * lane, step = HD << c.page_shift;
+    w = weighted(k_norm);
+    for (int x = max(first, qn); x < min(last, qn + kn); ++x) {
+        const int u = (x - qn) * APPEND_HEADS;
+        append_heads<E, CB, true>(kr + u * HD + 2 * lane, c.n_kv - u, k_norm, eps, w, c.k, at + u * step, step);
+    }
+    for (int x = max(first, qn + kn); x < last; ++x) {
+        const int u = (x - qn - kn) * APPEND_HEADS;
+        append_heads<E, CB, false>(vr + u * HD + 2 * lane, c.n_kv - u, false, eps, w, c.v, at + u * step, step);
     }
 }
 
 cudaError_t launch_kv_append(const PagedKV &c, q3cu_dtype cache_dt, const PagedSeqs &b, int64_t rows, const void *q,
                              const void *k, const void *v, q3cu_dtype dt, int64_t q_stride, int64_t kv_stride,
                              int n_heads, const float *q_norm, const float *k_norm, const TurnFreq &freq, float eps,
-                             void *q_out, q3cu_dtype q_dt, uint32_t *status, cudaStream_t stream) {
-    const int groups = (n_heads + 2 * c.n_kv + APPEND_UNITS - 1) / APPEND_UNITS;
-    const int64_t blocks = (rows * groups + APPEND_WARPS - 1) / APPEND_WARPS;
-    if (blocks == 0) return cudaSuccess;
-    const dim3 grid = dim3(unsigned(blocks)), block = dim3(APPEND_WARPS * 32);
-    const int qb = q_dt == Q3CU_BF16, cb = cache_dt == Q3CU_BF16;
-    if (dt == Q3CU_F32)
-        return launch_dependent(kv_append_kernel<float>, grid, block, 0, stream, c, b, rows,
-                                static_cast<const float *>(q), static_cast<const float *>(k),
-                                static_cast<const float *>(v), q_stride, kv_stride, n_heads, q_norm, k_norm, freq, eps,
-                                q_out, qb, cb, groups, status);
-    return launch_dependent(kv_append_kernel<bf16raw>, grid, block, 0, stream, c, b, rows,
-                            static_cast<const uint16_t *>(q), static_cast<const uint16_t *>(k),
-                            static_cast<const uint16_t *>(v), q_stride, kv_stride, n_heads, q_norm, k_norm, freq, eps,
-                            q_out, qb, cb, groups, status);
+                             void *q_out, q3cu_dtype q_dt, uint32_t *status, cudaStream_t stream, int sms) {
+    // A row is split over warps only while the rows alone are fewer than 32 warps per SM.
+    const int64_t batches = (n_heads + APPEND_HEADS - 1) / APPEND_HEADS + (c.n_kv + APPEND_HEADS - 1) / APPEND_HEADS * 2;
+    const int64_t parts = rows >= 32 * sms ? 1 : (32 * int64_t(sms) + rows - 1) / rows;
+    const dim3 grid(unsigned((rows + APPEND_WARPS - 1) / APPEND_WARPS), unsigned(parts < batches ? parts : batches));
+    auto go = [&](auto kernel, auto *typed) {
+        typedef decltype(typed) P;
+        return launch_dependent(kernel, grid, dim3(APPEND_WARPS * 32), 0, stream, c, b, int(rows), static_cast<P>(q),
+                                static_cast<P>(k), static_cast<P>(v), q_stride, kv_stride, n_heads, q_norm, k_norm, freq,
+                                eps, q_out, status);
+    };
+    const int kind = 2 * (q_dt == Q3CU_BF16) + (cache_dt == Q3CU_BF16);
+    if (dt == Q3CU_F32) {
+        const float *t = nullptr;
+        return kind == 0   ? go(kv_append_kernel<float, false, false>, t)
+               : kind == 1 ? go(kv_append_kernel<float, false, true>, t)
+               : kind == 2 ? go(kv_append_kernel<float, true, false>, t)
+                           : go(kv_append_kernel<float, true, true>, t);
+    }
+    const uint16_t *t = nullptr;
+    return kind == 0   ? go(kv_append_kernel<bf16raw, false, false>, t)
+           : kind == 1 ? go(kv_append_kernel<bf16raw, false, true>, t)
+           : kind == 2 ? go(kv_append_kernel<bf16raw, true, false>, t)
+                       : go(kv_append_kernel<bf16raw, true, true>, t);
 }
 
 }  // namespace q3

@@ -69,9 +69,9 @@ __device__ __forceinline__ float4 lds4(uint32_t addr) {
 }
 // Two floats as bf16 (hi) and what that leaves of them as bf16 (lo).
 __device__ __forceinline__ void split_bf16(float x, float y, uint32_t &hi, uint32_t &lo) {
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(y), "f"(x));
+    hi = pack_bf16(x, y);
     const float rx = x - __uint_as_float(hi << 16), ry = y - __uint_as_float(hi & 0xffff0000u);
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(ry), "f"(rx));
+    lo = pack_bf16(rx, ry);
 }
 // A float's leading 11 bits (tf32) and the rest, exactly.
 __device__ __forceinline__ void split_tf32(float x, uint32_t &hi, uint32_t &lo) {
@@ -167,7 +167,7 @@ __device__ __forceinline__ void walk_on(const PagedSeqs &b, const PagedKV &c, Pa
 // One pair of result elements (row, dims at, at + step) as the output's type.
 __device__ __forceinline__ void put2(float *p, int step, float x, float y) { p[0] = x, p[step] = y; }
 __device__ __forceinline__ void put2(uint16_t *p, int step, float x, float y) {
-    if (step == 1) *reinterpret_cast<uint32_t *>(p) = f32_to_bf16(x) | (f32_to_bf16(y) << 16);
+    if (step == 1) *reinterpret_cast<uint32_t *>(p) = pack_bf16(x, y);
     else p[0] = uint16_t(f32_to_bf16(x)), p[step] = uint16_t(f32_to_bf16(y));
 }
 

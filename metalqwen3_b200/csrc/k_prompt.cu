@@ -97,12 +97,6 @@ __device__ __forceinline__ PromptItem prompt_item(const PagedSeqs &b, const Page
     return it;
 }
 
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-
 // Scores from column n of 32 on become -inf.
 __device__ __forceinline__ void mask32(uint32_t *v, int n) {
 #pragma unroll

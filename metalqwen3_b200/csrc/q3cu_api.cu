@@ -564,7 +564,7 @@ q3cu_status q3cu_kv_append(q3cu_ctx *ctx, const q3cu_kv_cache *cache, const q3cu
     if (q3cu_status st = use_device(ctx)) return st;
     return launched(q3::launch_kv_append(c, q3cu_dtype(cache->dtype), b, rows, q, k, v, dtype, q_stride, kv_stride,
                                          n_heads, q_norm, k_norm, turn_freq_for(ctx, theta), eps, q_out, q_dtype,
-                                         ctx->d_status, static_cast<cudaStream_t>(stream)),
+                                         ctx->d_status, static_cast<cudaStream_t>(stream), ctx->sms),
                     "kv_append launch");
 }
 

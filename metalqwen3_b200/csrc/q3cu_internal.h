@@ -147,7 +147,7 @@ struct TurnFreq { double v[64]; };     // theta^(-j/64) / (2 pi)
 cudaError_t launch_kv_append(const PagedKV &c, q3cu_dtype cache_dt, const PagedSeqs &b, int64_t rows, const void *q,
                              const void *k, const void *v, q3cu_dtype dt, int64_t q_stride, int64_t kv_stride,
                              int n_heads, const float *q_norm, const float *k_norm, const TurnFreq &freq, float eps,
-                             void *q_out, q3cu_dtype q_dt, uint32_t *status, cudaStream_t stream);
+                             void *q_out, q3cu_dtype q_dt, uint32_t *status, cudaStream_t stream, int sms);
 // One query row per sequence (row s of q: sequence s) over its kv_len keys.
 size_t attention_paged_workspace(int n_heads, int n_kv, int sms);
 cudaError_t launch_attention_paged(const PagedKV &c, q3cu_dtype cache_dt, const PagedSeqs &b, const void *q,

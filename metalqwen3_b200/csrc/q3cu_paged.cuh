@@ -108,6 +108,13 @@ __host__ __device__ __forceinline__ int paged_seen(const PagedSeqs &b, int s, in
     return n < 0 ? 0 : n < len ? int(n) : len;
 }
 
+// Two floats rounded to bf16, the first in the low half.
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
 // Four consecutive elements as floats, and a float4 stored as T.
 __device__ __forceinline__ float4 load_quad(const float *p) { return *reinterpret_cast<const float4 *>(p); }
 __device__ __forceinline__ float4 load_quad(const uint16_t *p) {
@@ -117,8 +124,7 @@ __device__ __forceinline__ float4 load_quad(const uint16_t *p) {
 }
 __device__ __forceinline__ void store_quad(float *p, float4 v) { *reinterpret_cast<float4 *>(p) = v; }
 __device__ __forceinline__ void store_quad(uint16_t *p, float4 v) {
-    *reinterpret_cast<uint2 *>(p) = make_uint2(f32_to_bf16(v.x) | (f32_to_bf16(v.y) << 16),
-                                               f32_to_bf16(v.z) | (f32_to_bf16(v.w) << 16));
+    *reinterpret_cast<uint2 *>(p) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
 }
 
 // Attention of one query row and head by one warp, straight from the formula:
