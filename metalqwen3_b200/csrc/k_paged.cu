@@ -29,6 +29,7 @@
 //
 // Positions at and beyond the length score -inf, and their values are masked to
 // zero in registers: unused page space may hold anything.
+#include "q3cu_mma.cuh"
 #include "q3cu_paged.cuh"
 #include "q3cu_tma.h"
 
@@ -43,41 +44,6 @@ constexpr float PD_LOG2 = ATT_SCALE * 1.44269504088896341f;  // scores to base-2
 constexpr int PD_PART = HD + 2;                              // floats of a row's partial result: 128, maximum, sum
 
 template <typename TC> __host__ __device__ constexpr int pd_tile() { return int(PD_SIDE) / (HD * Elem<TC>::BYTES); }   // positions of a stage
-
-__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma_tf32(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ float4 lds4(uint32_t addr) {
-    float4 v;
-    asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-    return v;
-}
-// Two floats as bf16 (hi) and what that leaves of them as bf16 (lo).
-__device__ __forceinline__ void split_bf16(float x, float y, uint32_t &hi, uint32_t &lo) {
-    hi = pack_bf16(x, y);
-    const float rx = x - __uint_as_float(hi << 16), ry = y - __uint_as_float(hi & 0xffff0000u);
-    lo = pack_bf16(rx, ry);
-}
-// A float's leading 11 bits (tf32) and the rest, exactly.
-__device__ __forceinline__ void split_tf32(float x, uint32_t &hi, uint32_t &lo) {
-    hi = __float_as_uint(x) & 0xffffe000u;
-    lo = __float_as_uint(x - __uint_as_float(hi));
-}
 
 // a / b for 0 <= a, 0 < b: 32-bit division where it serves (a 64-bit one is a chain of some hundred instructions).
 __device__ __forceinline__ int64_t quot(int64_t a, int b) {
@@ -561,22 +527,13 @@ size_t attention_paged_workspace(int n_heads, int n_kv, int sms) {
     return size_t(paged_runs(sms)) * 2 * (n_heads / n_kv) * PD_PART * sizeof(float);
 }
 
-// Tensor map of the pages: boxes of 128 B by the rows of a page that one box takes.
-template <typename TC>
-static bool page_map(CUtensorMap *map, const void *base, const PagedKV &c) {
-    const uint64_t size = uint64_t(1) << c.page_shift, es = Elem<TC>::BYTES;
-    const uint64_t dims[4] = {HD, size, uint64_t(c.n_kv), uint64_t(c.n_pages)};
-    const uint64_t strides[3] = {HD * es, size * HD * es, uint64_t(c.page_stride) * es};
-    const uint32_t box[4] = {uint32_t(128 / es), uint32_t(size < uint64_t(pd_tile<TC>()) ? size : pd_tile<TC>()), 1, 1};
-    return encode_lines_map(map, base, es == 4 ? Q3CU_F32 : Q3CU_BF16, 4, dims, strides, box);
-}
-
 template <typename T, typename TC>
 static cudaError_t launch_split(const PagedKV &c, const PagedSeqs &b, const void *q, int64_t q_stride, int n_heads,
                                 void *work, void *out, uint32_t *status, cudaStream_t stream, int sms, int slot) {
     typedef typename Elem<T>::type E;
     CUtensorMap mk, mv;
-    if (!page_map<TC>(&mk, c.k, c) || !page_map<TC>(&mv, c.v, c)) return cudaErrorInvalidValue;
+    const q3cu_dtype dt = Elem<TC>::BYTES == 4 ? Q3CU_F32 : Q3CU_BF16;
+    if (!encode_pages_map(&mk, c.k, c, dt, pd_tile<TC>()) || !encode_pages_map(&mv, c.v, c, dt, pd_tile<TC>())) return cudaErrorInvalidValue;
     const int group = n_heads / c.n_kv, runs = paged_runs(sms);
     auto *kernel = group > 8 ? paged_split_kernel<T, TC, true> : paged_split_kernel<T, TC, false>;
     cudaError_t e = ensure_smem_attr(reinterpret_cast<const void *>(kernel), PD_SMEM, slot + (group > 8));

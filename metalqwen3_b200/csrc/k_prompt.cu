@@ -52,51 +52,6 @@ constexpr uint32_t PT_IDESC_V = PT_IDESC | (1u << 16);
 constexpr float PT_LOG2 = ATT_SCALE * 1.44269504088896341f;  // scores to base-2 exponents
 constexpr float PT_LAZY = 8.0f / PT_LOG2;                    // growth of the maximum (as a raw score) that rescales O
 
-// The items of a launch, in the order of blockIdx: sequence by sequence, from a
-// sequence's last block (the most keys) to its first, kv heads innermost.
-struct PromptItem {
-    int s, head;             // sequence (-1: none), kv head
-    int first, rows;         // first query row within the sequence, the sequence's rows
-    int64_t base;            // the sequence's first packed row
-};
-__device__ __forceinline__ PromptItem prompt_item(const PagedSeqs &b, const PagedKV &c, int64_t total_rows, int per_block,
-                                                  int64_t block) {
-    PromptItem it;
-    it.s = -1;
-    it.head = int(block % c.n_kv);
-    int64_t left = block / c.n_kv;
-    const int lane = threadIdx.x & 31;
-    for (int s0 = 0; s0 < b.n_seqs; s0 += 32) {              // 32 sequences at a time, by one warp
-        const int s = s0 + lane;
-        int64_t lo = 0, hi = 0;
-        if (s < b.n_seqs) {
-            lo = b.row_off[s];
-            hi = b.row_off[s + 1];
-            if (hi > total_rows) hi = total_rows;
-            if (lo < 0 || hi < lo) lo = hi = 0;              // offsets that do not rise: no rows
-        }
-        const int n = int(hi - lo), blocks = (n + per_block - 1) / per_block;
-        int64_t end = blocks;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int64_t x = __shfl_up_sync(FULL, end, o);
-            if (lane >= o) end += x;
-        }
-        const unsigned hit = __ballot_sync(FULL, left < end);
-        if (hit) {
-            const int l = __ffs(hit) - 1;
-            const int64_t end_l = __shfl_sync(FULL, end, l);
-            it.s = s0 + l;
-            it.rows = __shfl_sync(FULL, n, l);
-            it.base = __shfl_sync(FULL, lo, l);
-            it.first = int(end_l - 1 - left) * per_block;    // the last block first
-            return it;
-        }
-        left -= __shfl_sync(FULL, end, 31);
-    }
-    return it;
-}
-
 // Scores from column n of 32 on become -inf.
 __device__ __forceinline__ void mask32(uint32_t *v, int n) {
 #pragma unroll
@@ -392,45 +347,17 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
     if (warp == 8) tc_free512(tbase);
 }
 
-// f32 prompts: a warp per row and head.
-__global__ void __launch_bounds__(128) prompt_rows_kernel(const PagedKV c, const PagedSeqs b, int64_t rows,
-                                                          const float *q, int64_t q_stride, int n_heads, float *out,
-                                                          uint32_t *status) {
-    griddep_wait();
-    const int lane = threadIdx.x & 31;
-    const int64_t w = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5);
-    const int64_t r = w / n_heads;
-    const int h = int(w % n_heads);
-    if (r >= rows) return;
-    const int s = paged_seq_of(b, r);
-    if (s < 0) return;
-    const int n = paged_seen(b, s, r, paged_len(b, c, s, lane == 0 ? status : nullptr));
-    float4 x = load_quad(q + r * q_stride + int64_t(h) * HD + 4 * lane);
-    x = make_float4(x.x * ATT_SCALE, x.y * ATT_SCALE, x.z * ATT_SCALE, x.w * ATT_SCALE);
-    store_quad(out + w * HD + 4 * lane, attend_row<float>(c, b, s, h / (n_heads / c.n_kv), n, x, status));
-}
-
-// Tensor map of the pages: boxes of 64 elements by the rows of a page that one box takes.
-static bool page_map(CUtensorMap *map, const void *base, const PagedKV &c, int box_rows) {
-    const uint64_t size = uint64_t(1) << c.page_shift;
-    const uint64_t dims[4] = {HD, size, uint64_t(c.n_kv), uint64_t(c.n_pages)};
-    const uint64_t strides[3] = {HD * 2, size * HD * 2, uint64_t(c.page_stride) * 2};
-    const uint32_t box[4] = {64, uint32_t(box_rows), 1, 1};
-    return encode_lines_map(map, base, Q3CU_BF16, 4, dims, strides, box);
-}
-
 cudaError_t launch_attention_prompt(const PagedKV &c, const PagedSeqs &b, int64_t rows, const void *q, q3cu_dtype dt,
                                     int64_t q_stride, int n_heads, void *out, uint32_t *status, cudaStream_t stream,
                                     int sms) {
-    if (dt == Q3CU_F32)
-        return launch_dependent(prompt_rows_kernel, dim3(unsigned((rows * n_heads + 3) / 4)), dim3(128), 0, stream, c, b,
-                                rows, static_cast<const float *>(q), q_stride, n_heads, static_cast<float *>(out), status);
-    const int group = n_heads / c.n_kv, qt = PT_ROWS / group, br = c.page_shift < 7 ? 1 << c.page_shift : PT_KEYS;
+    if (dt == Q3CU_F32) return launch_prompt_f32(c, b, rows, q, q_stride, n_heads, out, status, stream);
+    const int group = n_heads / c.n_kv, qt = PT_ROWS / group;
     CUtensorMap mq, mk, mv;
     const uint64_t dims[3] = {HD, uint64_t(n_heads), uint64_t(rows)};
     const uint64_t strides[2] = {HD * 2, uint64_t(q_stride) * 2};
     const uint32_t box[3] = {64, uint32_t(group), uint32_t(qt)};
-    if (!encode_lines_map(&mq, q, Q3CU_BF16, 3, dims, strides, box) || !page_map(&mk, c.k, c, br) || !page_map(&mv, c.v, c, br))
+    if (!encode_lines_map(&mq, q, Q3CU_BF16, 3, dims, strides, box) || !encode_pages_map(&mk, c.k, c, Q3CU_BF16, PT_KEYS) ||
+        !encode_pages_map(&mv, c.v, c, Q3CU_BF16, PT_KEYS))
         return cudaErrorInvalidValue;
     cudaError_t e = ensure_smem_attr(reinterpret_cast<const void *>(prompt_tc_kernel), PT_SMEM, 32);
     if (e != cudaSuccess) return e;

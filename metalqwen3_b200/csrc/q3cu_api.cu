@@ -610,8 +610,8 @@ q3cu_status q3cu_attention_prompt(q3cu_ctx *ctx, const q3cu_kv_cache *cache, con
     if (q3cu_status st = check_dtype(dtype)) return st;
     if (cache->dtype != dtype) return fail(Q3CU_ERR_INVALID, "attention_prompt: q and the cache differ in type");
     if (n_heads == 0) return fail(Q3CU_ERR_INVALID, "attention_prompt: n_heads is 0");
-    if (rows < 0 || rows > INT32_MAX / n_heads)
-        return fail(Q3CU_ERR_INVALID, "attention_prompt: rows %lld", (long long)rows);
+    if (rows < 0 || rows + b.n_seqs > INT32_MAX / n_heads)
+        return fail(Q3CU_ERR_INVALID, "attention_prompt: rows %lld, n_seqs %d", (long long)rows, b.n_seqs);
     if (rows == 0 || b.n_seqs == 0) return Q3CU_OK;
     if (q3cu_status st = check_rows("attention_prompt", "q", q, dtype, q_stride, n_heads)) return st;
     if (q3cu_status st = check_rows("attention_prompt", "out", out, dtype, int64_t(n_heads) * q3::PAGED_HD, n_heads)) return st;

@@ -157,6 +157,8 @@ cudaError_t launch_attention_paged(const PagedKV &c, q3cu_dtype cache_dt, const 
 cudaError_t launch_attention_prompt(const PagedKV &c, const PagedSeqs &b, int64_t rows, const void *q, q3cu_dtype dt,
                                     int64_t q_stride, int n_heads, void *out, uint32_t *status, cudaStream_t stream,
                                     int sms);
+cudaError_t launch_prompt_f32(const PagedKV &c, const PagedSeqs &b, int64_t rows, const void *q, int64_t q_stride,
+                              int n_heads, void *out, uint32_t *status, cudaStream_t stream);
 
 cudaError_t launch_swiglu(const void *hb, const void *hb2, q3cu_dtype dt, int64_t elems, void *out, int8_t *q,
                           float *s, uint32_t *status, cudaStream_t stream, int sms);

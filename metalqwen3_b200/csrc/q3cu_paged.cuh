@@ -160,6 +160,51 @@ __device__ __forceinline__ float4 attend_row(const PagedKV &c, const PagedSeqs &
     return make_float4(o.x * r, o.y * r, o.z * r, o.w * r);
 }
 
+// The items of a launch, in the order of blockIdx: sequence by sequence, from a
+// sequence's last block (the most keys) to its first, kv heads innermost.
+struct PromptItem {
+    int s, head;             // sequence (-1: none), kv head
+    int first, rows;         // first query row within the sequence, the sequence's rows
+    int64_t base;            // the sequence's first packed row
+};
+__device__ __forceinline__ PromptItem prompt_item(const PagedSeqs &b, const PagedKV &c, int64_t total_rows, int per_block,
+                                                  int64_t block) {
+    PromptItem it;
+    it.s = -1;
+    it.head = int(block % c.n_kv);
+    int64_t left = block / c.n_kv;
+    const int lane = threadIdx.x & 31;
+    for (int s0 = 0; s0 < b.n_seqs; s0 += 32) {              // 32 sequences at a time, by one warp
+        const int s = s0 + lane;
+        int64_t lo = 0, hi = 0;
+        if (s < b.n_seqs) {
+            lo = b.row_off[s];
+            hi = b.row_off[s + 1];
+            if (hi > total_rows) hi = total_rows;
+            if (lo < 0 || hi < lo) lo = hi = 0;              // offsets that do not rise: no rows
+        }
+        const int n = int(hi - lo), blocks = (n + per_block - 1) / per_block;
+        int64_t end = blocks;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t x = __shfl_up_sync(FULL, end, o);
+            if (lane >= o) end += x;
+        }
+        const unsigned hit = __ballot_sync(FULL, left < end);
+        if (hit) {
+            const int l = __ffs(hit) - 1;
+            const int64_t end_l = __shfl_sync(FULL, end, l);
+            it.s = s0 + l;
+            it.rows = __shfl_sync(FULL, n, l);
+            it.base = __shfl_sync(FULL, lo, l);
+            it.first = int(end_l - 1 - left) * per_block;    // the last block first
+            return it;
+        }
+        left -= __shfl_sync(FULL, end, 31);
+    }
+    return it;
+}
+
 constexpr float ATT_SCALE = 0.08838834764831845f;            // 1/sqrt(128)
 
 }  // namespace q3

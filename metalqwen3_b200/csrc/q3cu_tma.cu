@@ -135,4 +135,12 @@ bool encode_lines_map(CUtensorMap *map, const void *base, q3cu_dtype dt, int ran
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool encode_pages_map(CUtensorMap *map, const void *base, const PagedKV &c, q3cu_dtype dt, int keys) {
+    const uint64_t size = uint64_t(1) << c.page_shift, es = dt == Q3CU_F32 ? 4 : 2;
+    const uint64_t dims[4] = {PAGED_HD, size, uint64_t(c.n_kv), uint64_t(c.n_pages)};
+    const uint64_t strides[3] = {PAGED_HD * es, size * PAGED_HD * es, uint64_t(c.page_stride) * es};
+    const uint32_t box[4] = {uint32_t(128 / es), uint32_t(size < uint64_t(keys) ? size : keys), 1, 1};
+    return encode_lines_map(map, base, dt, 4, dims, strides, box);
+}
+
 }  // namespace q3

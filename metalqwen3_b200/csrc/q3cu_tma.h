@@ -11,7 +11,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
-#include "q3cu.h"
+#include "q3cu_internal.h"
 
 namespace q3 {
 
@@ -49,6 +49,9 @@ bool encode_f32_2d_map(CUtensorMap *map, const void *base, uint64_t rows, uint64
 // Encoded anew by every call (a fraction of a microsecond).
 bool encode_lines_map(CUtensorMap *map, const void *base, q3cu_dtype dt, int rank, const uint64_t *dims,
                       const uint64_t *strides, const uint32_t *box);
+
+// The pages of a cache's k or v (base) for tiles of `keys` positions: a box is 128 B by min(page size, keys) rows.
+bool encode_pages_map(CUtensorMap *map, const void *base, const PagedKV &c, q3cu_dtype dt, int keys);
 
 #if defined(__CUDACC__)
 __device__ __forceinline__ void tma_load_2d(void *dst, const CUtensorMap *map, int x, int y, uint64_t *bar) {
