@@ -10,7 +10,7 @@
 // group of g, so short chunks fill the tile and the keys are fetched once for
 // the whole group.  An item has two such tiles, which share the keys and take
 // turns: while one tile's scores go through the softmax, the tensor cores work
-// on the other's.  One CTA per item, 12 warps:
+// on the other's.  One CTA per item, twelve warps (two of them idle):
 //   warps 0-3, 4-7  the softmax of tile 0 and of tile 1: thread = row = tensor-
 //            memory lane.  Reads the 128 scores of a key tile, folds the
 //            maximum, writes the probabilities back as bf16 over the scores
@@ -52,6 +52,27 @@ constexpr uint32_t PT_IDESC_V = PT_IDESC | (1u << 16);
 constexpr float PT_LOG2 = ATT_SCALE * 1.44269504088896341f;  // scores to base-2 exponents
 constexpr float PT_LAZY = 8.0f / PT_LOG2;                    // growth of the maximum (as a raw score) that rescales O
 
+// 2^x of a pair without the special-function unit, which is as busy as the tensor cores when every exponential goes
+// through it: x = n + f with n whole and |f| <= 1/2, a polynomial for 2^f, n added to the exponent.  The coefficients
+// are the minimax fit of degree 3 to 2^f (relative error 7.5e-5, a fiftieth of the bf16 rounding that follows), found
+// by Remez exchange.  Below 2^-126 the result is 2^-126.
+__device__ __forceinline__ void exp2_poly(float &x, float &y) {
+    const f2 v = pk2(fmaxf(x, -126.0f), fmaxf(y, -126.0f)), magic = pk2(12582912.0f, 12582912.0f);   // 1.5 * 2^23
+    const f2 t = add2(v, magic), f = sub2(v, sub2(t, magic));
+    f2 p = pk2(0.0551716685295105f, 0.0551716685295105f);
+    p = fma2(p, f, pk2(0.2426111251115799f, 0.2426111251115799f));
+    p = fma2(p, f, pk2(0.6932609677314758f, 0.6932609677314758f));
+    p = fma2(p, f, pk2(0.9999280571937561f, 0.9999280571937561f));
+    float t0, t1, p0, p1;
+    up2(t, t0, t1);
+    up2(p, p0, p1);
+    x = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
+    y = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
+}
+#ifndef PT_POLY
+#define PT_POLY 8                                            // one pair of exponentials in PT_POLY / 2 by polynomial
+#endif
+
 // Scores from column n of 32 on become -inf.
 __device__ __forceinline__ void mask32(uint32_t *v, int n) {
 #pragma unroll
@@ -66,7 +87,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
     extern __shared__ uint8_t pt_dyn[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(pt_dyn) + 1023) & ~uintptr_t(1023));
     uint8_t *ring = smem + 2 * PT_TILE;
-    __shared__ __align__(8) uint64_t q_full, full[PT_NS], empty[PT_NS], s_full[2], p_full[2], o_full[2], drain;
+    __shared__ __align__(8) uint64_t q_full, full[PT_NS], empty[PT_NS], s_full[2], p_full[2][2], o_full[2], drain;
     __shared__ uint32_t tmem_sh;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -78,7 +99,8 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
         }
         for (int t = 0; t < 2; ++t) {
             mbar_init(&s_full[t], 1);
-            mbar_init(&p_full[t], 4);
+            mbar_init(&p_full[t][0], 4);
+            mbar_init(&p_full[t][1], 4);
             mbar_init(&o_full[t], 1);
         }
         mbar_init(&drain, 1);
@@ -109,121 +131,139 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
     }
     const int nkv = max(nt[0], nt[1]);
 
-    if (warp == 9) {
-        // ---- fetch -------------------------------------------------------------------
-        const int br = min(1 << c.page_shift, PT_KEYS), nb = PT_KEYS / br;      // rows of a box, boxes of a tile
-        if (nkv > 0) {
-            if (lane == 0) {
-                uint32_t bytes = 0;
-                for (int t = 0; t < 2; ++t)
-                    if (nt[t]) bytes += 2u * qt * group * 128;
-                mbar_arrive_expect_tx(&q_full, bytes);
-                for (int t = 0; t < 2; ++t)
-                    for (int h = 0; h < 2 && nt[t]; ++h)
-                        tma_load_3d(smem + t * PT_TILE + h * PT_HALF, &tmq, 64 * h, it.head * group,
-                                    int(it.base) + it.first + t * qt, &q_full);
-            }
-            __syncwarp();
-            int e = 0;
-            bool ok = true;
-            // lane = box: column half lane / nb, positions lane % nb
-            const int box = lane % nb, half = lane / nb;
-            auto page_of = [&](int j) -> int {               // n_pages reads as zeros
-                const int t = j * PT_KEYS + box * br;
-                if (half > 1 || t >= len) return c.n_pages;
-                const int p = paged_page(b, c, it.s, t, status);
-                return p < 0 ? c.n_pages : p;
-            };
-            int page = page_of(0);
-            for (int j = 0; j < nkv && ok; ++j) {
-                const int next = j + 1 < nkv ? page_of(j + 1) : 0;
-                const int slot = (j * PT_KEYS + box * br) & ((1 << c.page_shift) - 1);
-                for (int kv = 0; kv < 2 && ok; ++kv, ++e) {
-                    const int st = e % PT_NS;
-                    if (e >= PT_NS)
-                        ok = mbar_wait(&empty[st], uint32_t(e / PT_NS - 1) & 1u, lane == 0 ? status : nullptr);
-                    ok = __all_sync(FULL, ok);
-                    if (!ok) break;
-                    if (lane == 0) mbar_arrive_expect_tx(&full[st], PT_TILE);
-                    __syncwarp();
-                    if (half < 2)
-                        tma_load_4d(ring + st * PT_TILE + half * PT_HALF + box * br * 128, kv ? &tmv : &tmk, 64 * half, slot,
-                                    it.head, page, &full[st]);
+    // Registers move to the softmax: 256 threads x 208 + 128 x 88 is the launch's 384 x 168.
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if (warp == 9) {
+            // ---- fetch -------------------------------------------------------------------
+            const int br = min(1 << c.page_shift, PT_KEYS), nb = PT_KEYS / br;      // rows of a box, boxes of a tile
+            if (nkv > 0) {
+                if (lane == 0) {
+                    uint32_t bytes = 0;
+                    for (int t = 0; t < 2; ++t)
+                        if (nt[t]) bytes += 2u * qt * group * 128;
+                    mbar_arrive_expect_tx(&q_full, bytes);
+                    for (int t = 0; t < 2; ++t)
+                        for (int h = 0; h < 2 && nt[t]; ++h)
+                            tma_load_3d(smem + t * PT_TILE + h * PT_HALF, &tmq, 64 * h, it.head * group,
+                                        int(it.base) + it.first + t * qt, &q_full);
                 }
-                page = next;
-            }
-            // no copy outlives the CTA (bounded)
-            for (int d = e > PT_NS ? e - PT_NS : 0; d < e; ++d) mbar_wait(&full[d % PT_NS], uint32_t(d / PT_NS) & 1u, nullptr);
-            mbar_wait(&q_full, 0, nullptr);
-        }
-    } else if (warp == 8) {
-        // ---- products ----------------------------------------------------------------
-        if (nkv > 0) {
-            bool ok = mbar_wait(&q_full, 0, lane == 0 ? status : nullptr);
-            const uint32_t qa = smem_addr(smem), ra = smem_addr(ring);
-            auto wait = [&](uint64_t *bar, uint32_t parity) {
-                if (ok) ok = mbar_wait(bar, parity, lane == 0 ? status : nullptr);
-                ok = __all_sync(FULL, ok);
-                tc_fence_after();
-            };
-            auto scores = [&](int t, int e) {                // S_t = Q_t K^T
-                if (lane) return;
-                for (int k = 0; k < 8; ++k) {
-                    const uint32_t off = uint32_t(k / 4) * PT_HALF + uint32_t(k % 4) * 32;
-                    tc_mma_bf16_ss(tbase + t * 128, tc_sdesc(qa + t * PT_TILE + off),
-                                   tc_sdesc(ra + (e % PT_NS) * PT_TILE + off), PT_IDESC, uint32_t(k > 0));
-                }
-                tc_commit(&s_full[t]);
-            };
-            wait(&full[0], 0);
-            if (ok)
-                for (int t = 0; t < 2; ++t)
-                    if (nt[t]) scores(t, 0);
-            if (ok && lane == 0) tc_commit(&empty[0]);
-            for (int j = 0; j < nkv && ok; ++j) {
-                const int ev = 2 * j + 1, ek = 2 * j + 2;     // ring entries of V(j) and K(j + 1)
-                wait(&full[ev % PT_NS], uint32_t(ev / PT_NS) & 1u);
-                if (!ok) break;
-                if (j == nkv - 1 && len < nkv * PT_KEYS) {    // values behind the sequence's end: zeros
-                    for (int r = len - j * PT_KEYS + lane / 8; r < PT_KEYS; r += 4)
-                        for (int h = 0; h < 2; ++h)
-                            *reinterpret_cast<uint4 *>(ring + (ev % PT_NS) * PT_TILE + h * PT_HALF + r * 128 + (lane & 7) * 16) =
-                                make_uint4(0, 0, 0, 0);
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                }
-                for (int t = 0; t < 2 && ok; ++t) {
-                    if (j < nt[t]) {
-                        wait(&p_full[t], uint32_t(j) & 1u);
+                __syncwarp();
+                int e = 0;
+                bool ok = true;
+                // lane = box: column half lane / nb, positions lane % nb
+                const int box = lane % nb, half = lane / nb;
+                auto page_of = [&](int j) -> int {               // n_pages reads as zeros
+                    const int t = j * PT_KEYS + box * br;
+                    if (half > 1 || t >= len) return c.n_pages;
+                    const int p = paged_page(b, c, it.s, t, status);
+                    return p < 0 ? c.n_pages : p;
+                };
+                int page = page_of(0);
+                for (int j = 0; j < nkv && ok; ++j) {
+                    const int next = j + 1 < nkv ? page_of(j + 1) : 0;
+                    const int slot = (j * PT_KEYS + box * br) & ((1 << c.page_shift) - 1);
+                    for (int kv = 0; kv < 2 && ok; ++kv, ++e) {
+                        const int st = e % PT_NS;
+                        if (e >= PT_NS)
+                            ok = mbar_wait(&empty[st], uint32_t(e / PT_NS - 1) & 1u, lane == 0 ? status : nullptr);
+                        ok = __all_sync(FULL, ok);
                         if (!ok) break;
-                        if (lane == 0) {
-                            for (int k = 0; k < 8; ++k)      // O_t += P_t V, 16 keys at a time
-                                tc_mma_bf16_ts(tbase + 256 + t * 128, tbase + t * 128 + k * 8,
-                                               tc_sdesc_mn(ra + (ev % PT_NS) * PT_TILE + k * 2048, PT_HALF), PT_IDESC_V,
-                                               uint32_t(j > 0 || k > 0));
-                            if (j + 1 == nt[t]) tc_commit(&o_full[t]);
+                        if (lane == 0) mbar_arrive_expect_tx(&full[st], PT_TILE);
+                        __syncwarp();
+                        if (half < 2)
+                            tma_load_4d(ring + st * PT_TILE + half * PT_HALF + box * br * 128, kv ? &tmv : &tmk, 64 * half, slot,
+                                        it.head, page, &full[st]);
+                    }
+                    page = next;
+                }
+                // no copy outlives the CTA (bounded)
+                for (int d = e > PT_NS ? e - PT_NS : 0; d < e; ++d) mbar_wait(&full[d % PT_NS], uint32_t(d / PT_NS) & 1u, nullptr);
+                mbar_wait(&q_full, 0, nullptr);
+            }
+        } else if (warp == 8) {
+            // ---- products ----------------------------------------------------------------
+            if (nkv > 0) {
+                bool ok = mbar_wait(&q_full, 0, lane == 0 ? status : nullptr);
+                // operand descriptors of the first row tile and the first buffer; a 32 KB tile further is + 2048
+                const uint64_t dq = tc_sdesc(smem_addr(smem)), dk = tc_sdesc(smem_addr(ring)),
+                               dv = tc_sdesc_mn(smem_addr(ring), PT_HALF);
+                auto wait = [&](uint64_t *bar, uint32_t parity) {
+                    if (ok) ok = mbar_wait(bar, parity, lane == 0 ? status : nullptr);
+                    ok = __all_sync(FULL, ok);
+                    tc_fence_after();
+                };
+                auto scores = [&](int t, int buf) {          // S_t = Q_t K^T
+                    if (tc_elect()) {
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const uint32_t off = (uint32_t(k / 4) * PT_HALF + uint32_t(k % 4) * 32) >> 4;
+                            tc_mma_bf16_ss(tbase + t * 128, dq + t * (PT_TILE >> 4) + off, dk + buf * (PT_TILE >> 4) + off,
+                                           PT_IDESC, uint32_t(k > 0));
+                        }
+                        tc_commit(&s_full[t]);
+                    }
+                    __syncwarp();
+                };
+                wait(&full[0], 0);
+                if (ok)
+                    for (int t = 0; t < 2; ++t)
+                        if (nt[t]) scores(t, 0);
+                if (ok && tc_elect()) tc_commit(&empty[0]);
+                __syncwarp();
+                int bv = 1, bk = 2;                          // buffers of V(j) and K(j + 1), and how often each was filled before
+                uint32_t pv = 0, pk = 0;
+                for (int j = 0; j < nkv && ok; ++j) {
+                    wait(&full[bv], pv & 1u);
+                    if (!ok) break;
+                    if (j == nkv - 1 && len < nkv * PT_KEYS) {        // values behind the sequence's end: zeros
+                        for (int r = len - j * PT_KEYS + lane / 8; r < PT_KEYS; r += 4)
+                            for (int h = 0; h < 2; ++h)
+                                *reinterpret_cast<uint4 *>(ring + bv * PT_TILE + h * PT_HALF + r * 128 + (lane & 7) * 16) =
+                                    make_uint4(0, 0, 0, 0);
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                    }
+                    for (int t = 0; t < 2 && ok; ++t) {
+                        if (j < nt[t]) {
+#pragma unroll
+                            for (int half = 0; half < 2; ++half) {    // O_t += P_t V, 64 keys at a time
+                                wait(&p_full[t][half], uint32_t(j) & 1u);
+                                if (!ok) break;
+                                if (tc_elect()) {
+#pragma unroll
+                                    for (int k = 4 * half; k < 4 * half + 4; ++k)
+                                        tc_mma_bf16_ts(tbase + 256 + t * 128, tbase + t * 128 + k * 8,
+                                                       dv + bv * (PT_TILE >> 4) + k * (2048 >> 4), PT_IDESC_V,
+                                                       k > 0 ? 1u : uint32_t(j > 0));
+                                    if (half && j + 1 == nt[t]) tc_commit(&o_full[t]);
+                                }
+                                __syncwarp();
+                            }
+                            if (!ok) break;
+                        }
+                        if (j + 1 < nt[t]) {
+                            wait(&full[bk], pk & 1u);
+                            if (!ok) break;
+                            scores(t, bk);
                         }
                     }
-                    if (j + 1 < nt[t]) {
-                        wait(&full[ek % PT_NS], uint32_t(ek / PT_NS) & 1u);
-                        if (!ok) break;
-                        scores(t, ek);
+                    if (ok && tc_elect()) {
+                        tc_commit(&empty[bv]);
+                        if (j + 1 < nkv) tc_commit(&empty[bk]);
                     }
                     __syncwarp();
+                    if ((bv += 2) >= PT_NS) bv -= PT_NS, ++pv;
+                    if ((bk += 2) >= PT_NS) bk -= PT_NS, ++pk;
                 }
-                if (ok && lane == 0) {
-                    tc_commit(&empty[ev % PT_NS]);
-                    if (j + 1 < nkv) tc_commit(&empty[ek % PT_NS]);
-                }
-            }
-            // every product issued has completed before tensor memory is given back (bounded)
-            if (lane == 0) {
-                tc_commit(&drain);
+                // every product issued has completed before tensor memory is given back (bounded)
+                if (tc_elect()) tc_commit(&drain);
+                __syncwarp();
                 mbar_wait(&drain, 0, nullptr);
             }
-            __syncwarp();
         }
-    } else if (warp < 8) {
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         // ---- softmax -----------------------------------------------------------------
         const int t = warp >> 2, r = threadIdx.x & 127;      // row tile, row = tensor-memory lane
         const uint32_t lane_base = tbase + (uint32_t(32 * (warp & 3)) << 16);
@@ -238,22 +278,21 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
             ok = __all_sync(FULL, mbar_wait(&s_full[t], uint32_t(j) & 1u, lane == 0 ? status : nullptr));
             if (!ok) break;
             tc_fence_after();
-            // the maximum; the scores stay in tensor memory and are read again below, 32 at a time
-            const int n = limit - j * PT_KEYS;               // visible keys of the tile
-            const bool masked = (j + 1) * PT_KEYS > sure;
-            uint32_t u[2][32];
-            tc_ld32(ts, u[0]);
+            uint32_t u[128];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) tc_ld32(ts + 32 * x, u + 32 * x);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) tc_wait_ld32(u + 32 * x);
+            if ((j + 1) * PT_KEYS > sure) {
+#pragma unroll
+                for (int x = 0; x < 4; ++x) mask32(u + 32 * x, limit - j * PT_KEYS - 32 * x);
+            }
             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                uint32_t *v = u[x & 1];
-                tc_wait_ld32(v);
-                if (x < 3) tc_ld32(ts + 32 * (x + 1), u[(x + 1) & 1]);
-                if (masked) mask32(v, n - 32 * x);
+            for (int x = 0; x < 128; x += 8)
 #pragma unroll
-                for (int y = 0; y < 32; ++y) mx[y & 3] = fmaxf(mx[y & 3], __uint_as_float(v[y]));
-            }
-            tc_ld32(ts, u[0]);
+                for (int y = 0; y < 4; ++y)
+                    mx[y] = fmaxf(fmaxf(mx[y], __uint_as_float(u[x + y])), __uint_as_float(u[x + y + 4]));
             const float tile_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
             const bool grow = tile_max > m + PT_LAZY || (m == -INFINITY && tile_max > m);
             if (__any_sync(FULL, grow)) {
@@ -262,41 +301,48 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                 m = nm;
                 sum *= f;
                 if (j > 0) {                                 // O of the tiles before (their product has completed)
+#pragma unroll 1
+                    for (int x = 0; x < 8; ++x) {
+                        uint32_t o[16];
+                        tc_ld16(to + 16 * x, o);
+                        tc_wait_ld16(o);
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        uint32_t o[32];
-                        tc_ld32(to + 32 * x, o);
-                        tc_wait_ld32(o);
-#pragma unroll
-                        for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
-                        tc_st32(to + 32 * x, o);
+                        for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
+                        tc_st16(to + 16 * x, o);
                     }
                 }
             }
             const float off = m == -INFINITY ? 0.0f : -m * PT_LOG2;
-            float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            const f2 off2 = pk2(off, off), scale2 = pk2(PT_LOG2, PT_LOG2);
+            f2 part[2] = {pk2(0.0f, 0.0f), pk2(0.0f, 0.0f)};
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                uint32_t *v = u[x & 1];
-                tc_wait_ld32(v);
-                if (x < 3) tc_ld32(ts + 32 * (x + 1), u[(x + 1) & 1]);
-                if (masked) mask32(v, n - 32 * x);
+            for (int x = 0; x < 4; ++x) {                    // 32 probabilities at a time; two halves are handed over
                 uint32_t w[16];
 #pragma unroll
                 for (int y = 0; y < 32; y += 2) {
-                    const float p0 = ex2_approx_ftz(fmaf(__uint_as_float(v[y]), PT_LOG2, off));
-                    const float p1 = ex2_approx_ftz(fmaf(__uint_as_float(v[y + 1]), PT_LOG2, off));
-                    part[y & 2] += p0;
-                    part[(y & 2) + 1] += p1;
+                    const f2 e = fma2(pk2(__uint_as_float(u[32 * x + y]), __uint_as_float(u[32 * x + y + 1])), scale2, off2);
+                    float p0, p1;
+                    up2(e, p0, p1);
+                    if (y % PT_POLY == PT_POLY - 2) {
+                        exp2_poly(p0, p1);
+                    } else {
+                        p0 = ex2_approx_ftz(p0);
+                        p1 = ex2_approx_ftz(p1);
+                    }
+                    part[y / 2 & 1] = add2(part[y / 2 & 1], pk2(p0, p1));
                     w[y / 2] = pack_bf16(p0, p1);
                 }
-                tc_st16(ts + 16 * x, w);                     // over scores already read
+                tc_st16(ts + 16 * x, w);
+                if (x & 1) {
+                    tc_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full[t][x >> 1]);
+                }
             }
-            sum += (part[0] + part[1]) + (part[2] + part[3]);
-            tc_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[t]);
+            float s0, s1;
+            up2(add2(part[0], part[1]), s0, s1);
+            sum += s0 + s1;
         }
         // ---- the result ----------------------------------------------------------------
         if (nt[t] > 0 && ok) {

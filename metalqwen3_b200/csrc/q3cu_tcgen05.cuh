@@ -40,6 +40,14 @@ __device__ __forceinline__ uint64_t tc_sdesc_mn(uint32_t smem_addr, uint32_t mn_
            (uint64_t(1) << 46) | (uint64_t(2) << 61);
 }
 
+// One lane of a converged warp, always the same, known to the compiler as such: what it issues keeps its operands in
+// uniform registers (under a plain `lane == 0` every operand is moved there first, about 100 cycles per product).
+__device__ __forceinline__ bool tc_elect() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
+
 // D (tensor memory, f32) (+)= A * B, bf16 operands, K = 16.  A from shared
 // memory or, packed two to a column, from tensor memory; B from shared memory.
 __device__ __forceinline__ void tc_mma_bf16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -55,6 +63,21 @@ __device__ __forceinline__ void tc_mma_bf16_ts(uint32_t d, uint32_t a, uint64_t 
         :: "r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
 
+__device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(taddr) : "memory");
+}
+// The wait, with the loaded registers as operands: nothing that reads them can
+// be scheduled before it.
+__device__ __forceinline__ void tc_wait_ld16(uint32_t (&v)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
+                   "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
+                 :: "memory");
+}
 // 32 columns of this warp's 32 lanes to or from registers (thread = lane).  A load's registers hold the values only
 // after tc_wait_ld32.
 #define TC_R32(v, o) \
