@@ -10,7 +10,9 @@
 // group of g, so short chunks fill the tile and the keys are fetched once for
 // the whole group.  An item has two such tiles, which share the keys and take
 // turns: while one tile's scores go through the softmax, the tensor cores work
-// on the other's.  One CTA per item, twelve warps (two of them idle):
+// on the other's.  A CTA per SM takes items one after the
+// other, its warps each at their own pace, so that one item's first fetches and
+// products run beside the last softmax and the stores of the item before:
 //   warps 0-3, 4-7  the softmax of tile 0 and of tile 1: thread = row = tensor-
 //            memory lane.  Reads the 128 scores of a key tile, folds the
 //            maximum, writes the probabilities back as bf16 over the scores
@@ -21,8 +23,12 @@
 //            and sum share it) and keeps every value far inside binary32.
 //   warp 8   issues the products: S = Q K^T from shared memory, O += P V with P
 //            from tensor memory.
-//   warp 9   fetches Q and then the key and value tiles of 128 positions, page by page, by TMA
-//            into a ring of five 32 KB buffers.
+//   warp 9   finds the items, announces them in shared memory, and fetches Q and
+//            the key and value tiles of 128 positions, page by page, by TMA into
+//            a ring of five 32 KB buffers.
+//   warp 10  clears the values behind a sequence's end (below).
+// Items go from the longest to the shortest; a CTA that is done with one takes
+// over that of a CTA that has not started.
 // Tensor memory (512 columns): S0, S1, O0, O1; P_t lies over the first half of S_t.
 //
 // Masks: keys at and beyond the row's limit become -inf before the maximum.
@@ -80,19 +86,53 @@ __device__ __forceinline__ void mask32(uint32_t *v, int n) {
         if (y >= n) v[y] = 0xff800000u;
 }
 
+// The item of a round, as warp 9 announces it (s < 0: no more), with the key tiles of each row tile.
+struct PromptRound : PromptItem {
+    int nt[2];
+};
+// Asks for the work of a CTA of this launch that has not started (it then never does); the answer arrives on `bar`
+// (16 bytes).  After an answer of none, nothing more may be asked.
+__device__ __forceinline__ void take_over_cta(ulonglong2 *answer, uint64_t *bar) {
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
+                 :: "r"(smem_addr(answer)), "r"(smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ int64_t taken_cta(const ulonglong2 &answer) {     // its blockIdx.x, or -1
+    uint32_t got, x = 0;
+    asm volatile(
+        "{\n\t.reg .b128 h;\n\t.reg .pred p;\n\tmov.b128 h, {%2, %3};\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\tselp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n\t}"
+        : "=r"(got), "=r"(x) : "l"(answer.x), "l"(answer.y));
+    return got ? int64_t(x) : -1;
+}
+
+// A place in the ring, in the order of use: buffer and how often (parity) it was used before.
+struct RingAt {
+    int st = 0;
+    uint32_t ph = 0;
+    __device__ __forceinline__ void next() {
+        if (++st == PT_NS) st = 0, ph ^= 1u;
+    }
+};
+
 __global__ void __launch_bounds__(PT_THREADS, 1)
 prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
-                 const __grid_constant__ CUtensorMap tmv, const PagedKV c, const PagedSeqs b, int64_t rows,
-                 const uint16_t *q, int64_t q_stride, int n_heads, int group, uint16_t *out, uint32_t *status) {
+                 const __grid_constant__ CUtensorMap tmv, const PagedKV c, const PagedSeqs b, int rows,
+                 const uint16_t *q, int64_t q_stride, int n_heads, int group, const FastDiv per_block,
+                 const FastDiv by_group, uint16_t *out, uint32_t *status) {
     extern __shared__ uint8_t pt_dyn[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(pt_dyn) + 1023) & ~uintptr_t(1023));
     uint8_t *ring = smem + 2 * PT_TILE;
-    __shared__ __align__(8) uint64_t q_full, full[PT_NS], empty[PT_NS], s_full[2], p_full[2][2], o_full[2], drain;
+    __shared__ __align__(8) uint64_t q_full, q_empty, full[PT_NS], empty[PT_NS], s_full[2], p_full[2][2], o_full[2],
+        o_empty[2], item_full[2], item_empty[2], taken, tail_go, tail, drain;
+    __shared__ PromptRound item_sh[2];
+    __shared__ ulonglong2 taken_sh;
     __shared__ uint32_t tmem_sh;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         mbar_init(&q_full, 1);
+        mbar_init(&q_empty, 1);
         for (int i = 0; i < PT_NS; ++i) {
             mbar_init(&full[i], 1);
             mbar_init(&empty[i], 1);
@@ -102,7 +142,13 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
             mbar_init(&p_full[t][0], 4);
             mbar_init(&p_full[t][1], 4);
             mbar_init(&o_full[t], 1);
+            mbar_init(&o_empty[t], 4);
+            mbar_init(&item_full[t], 1);
+            mbar_init(&item_empty[t], 10);                   // warps 0-7, 8 and 10
         }
+        mbar_init(&taken, 1);
+        mbar_init(&tail_go, 1);
+        mbar_init(&tail, 1);
         mbar_init(&drain, 1);
         mbar_init_fence();
     }
@@ -114,152 +160,219 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
     griddep_wait();
 
     const int qt = PT_ROWS / group;                          // queries of a tile
-    const PromptItem it = prompt_item(b, c, rows, 2 * qt, blockIdx.x);
-    const bool item = it.s >= 0;
-    // position of the sequence's row i is pos0 + i; keys that row sees: min(len, pos + 1)
-    const int len = item ? paged_len(b, c, it.s, threadIdx.x == 0 ? status : nullptr) : 0;
-    const int64_t pos0 = item ? int64_t(b.kv_len[it.s]) - it.rows : 0;
-    auto seen = [&](int i) -> int {
-        const int64_t n = pos0 + i + 1;
-        return n < 0 ? 0 : n < len ? int(n) : len;
+    // the item of a round, copied from its announcement; false after the last, or if a wait gave up
+    auto next_item = [&](int round, PromptRound &it, bool whole_warp) -> bool {
+        bool ok = mbar_wait(&item_full[round & 1], uint32_t(round >> 1) & 1u, !whole_warp || lane == 0 ? status : nullptr);
+        if (whole_warp) ok = __all_sync(FULL, ok);
+        if (!ok) return false;
+        it = item_sh[round & 1];
+        if (whole_warp) __syncwarp();
+        if (!whole_warp || lane == 0) mbar_arrive(&item_empty[round & 1]);
+        return it.s >= 0;
     };
-    int nt[2];                                               // key tiles of each row tile
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        const int first = it.first + t * qt, last = min(first + qt, it.rows) - 1;
-        nt[t] = item && last >= first ? (seen(last) + PT_KEYS - 1) / PT_KEYS : 0;
-    }
-    const int nkv = max(nt[0], nt[1]);
 
     // Registers move to the softmax: 256 threads x 208 + 128 x 88 is the launch's 384 x 168.
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         if (warp == 9) {
-            // ---- fetch -------------------------------------------------------------------
-            const int br = min(1 << c.page_shift, PT_KEYS), nb = PT_KEYS / br;      // rows of a box, boxes of a tile
-            if (nkv > 0) {
+            // ---- items and copies ------------------------------------------------------------
+            const int br = min(1 << c.page_shift, PT_KEYS), nb = PT_KEYS / br;  // rows of a box, boxes of a tile
+            // lane = box: column half lane / nb, positions lane % nb
+            const int box = lane % nb, half = lane / nb;
+            RingAt at;
+            int entries = 0, qs = 0;                         // copies of tiles and of Q so far
+            bool ok = true;
+            PromptOrder order(b, c, rows, per_block, PT_KEYS, status);
+            PromptItem item = order.find(blockIdx.x);
+            // The first item is this CTA's own; the others are those of CTAs that have not started.  One is taken over
+            // when the copies for the item before are nearly all under way: no earlier, so that the CTA that is done
+            // first gets the next item, and no later, since finding it takes some thousand cycles.
+            auto take_over = [&](int round) -> PromptItem {
                 if (lane == 0) {
-                    uint32_t bytes = 0;
-                    for (int t = 0; t < 2; ++t)
-                        if (nt[t]) bytes += 2u * qt * group * 128;
-                    mbar_arrive_expect_tx(&q_full, bytes);
-                    for (int t = 0; t < 2; ++t)
-                        for (int h = 0; h < 2 && nt[t]; ++h)
-                            tma_load_3d(smem + t * PT_TILE + h * PT_HALF, &tmq, 64 * h, it.head * group,
-                                        int(it.base) + it.first + t * qt, &q_full);
+                    fence_proxy_async_smem();
+                    mbar_arrive_expect_tx(&taken, 16);
+                    take_over_cta(&taken_sh, &taken);
+                }
+                PromptItem none;
+                none.s = -1;
+                ok = __all_sync(FULL, mbar_wait(&taken, uint32_t(round) & 1u, lane == 0 ? status : nullptr));
+                if (!ok) return none;
+                const int64_t index = taken_cta(taken_sh);
+                __syncwarp();
+                return index < 0 ? none : order.find(index);
+            };
+            for (int round = 0; ok; ++round) {
+                PromptRound it;
+                static_cast<PromptItem &>(it) = item;
+                it.nt[0] = it.nt[1] = 0;
+                for (int t = 0; t < 2 && it.s >= 0; ++t) {
+                    const int first = it.first + t * qt, last = min(first + qt, it.rows) - 1;
+                    if (last >= first) it.nt[t] = (it.seen(last) + PT_KEYS - 1) / PT_KEYS;
+                }
+                if (round >= 2)
+                    ok = __all_sync(FULL, mbar_wait(&item_empty[round & 1], uint32_t((round >> 1) - 1) & 1u,
+                                                    lane == 0 ? status : nullptr));
+                if (!ok) break;
+                if (lane == 0) {
+                    item_sh[round & 1] = it;
+                    mbar_arrive(&item_full[round & 1]);
                 }
                 __syncwarp();
-                int e = 0;
-                bool ok = true;
-                // lane = box: column half lane / nb, positions lane % nb
-                const int box = lane % nb, half = lane / nb;
-                auto page_of = [&](int j) -> int {               // n_pages reads as zeros
+                if (it.s < 0) break;
+                const int nkv = max(it.nt[0], it.nt[1]);
+                if (nkv == 0) {
+                    item = take_over(round);
+                    continue;
+                }
+                auto page_of = [&](int j) -> int {           // n_pages reads as zeros
                     const int t = j * PT_KEYS + box * br;
-                    if (half > 1 || t >= len) return c.n_pages;
+                    if (half > 1 || t >= it.len) return c.n_pages;
                     const int p = paged_page(b, c, it.s, t, status);
                     return p < 0 ? c.n_pages : p;
                 };
                 int page = page_of(0);
+                if (qs) ok = __all_sync(FULL, mbar_wait(&q_empty, uint32_t(qs - 1) & 1u, lane == 0 ? status : nullptr));
+                if (!ok) break;
+                ++qs;
+                if (lane == 0) {
+                    uint32_t bytes = 0;
+                    for (int t = 0; t < 2; ++t)
+                        if (it.nt[t]) bytes += 2u * qt * group * 128;
+                    mbar_arrive_expect_tx(&q_full, bytes);
+                    for (int t = 0; t < 2; ++t)
+                        for (int h = 0; h < 2 && it.nt[t]; ++h)
+                            tma_load_3d(smem + t * PT_TILE + h * PT_HALF, &tmq, 64 * h, it.head * group,
+                                        it.base + it.first + t * qt, &q_full);
+                }
+                __syncwarp();
                 for (int j = 0; j < nkv && ok; ++j) {
                     const int next = j + 1 < nkv ? page_of(j + 1) : 0;
                     const int slot = (j * PT_KEYS + box * br) & ((1 << c.page_shift) - 1);
-                    for (int kv = 0; kv < 2 && ok; ++kv, ++e) {
-                        const int st = e % PT_NS;
-                        if (e >= PT_NS)
-                            ok = mbar_wait(&empty[st], uint32_t(e / PT_NS - 1) & 1u, lane == 0 ? status : nullptr);
+                    for (int kv = 0; kv < 2; ++kv) {
+                        if (entries >= PT_NS) ok = mbar_wait(&empty[at.st], at.ph ^ 1u, lane == 0 ? status : nullptr);
                         ok = __all_sync(FULL, ok);
                         if (!ok) break;
-                        if (lane == 0) mbar_arrive_expect_tx(&full[st], PT_TILE);
+                        if (lane == 0) mbar_arrive_expect_tx(&full[at.st], PT_TILE);
                         __syncwarp();
                         if (half < 2)
-                            tma_load_4d(ring + st * PT_TILE + half * PT_HALF + box * br * 128, kv ? &tmv : &tmk, 64 * half, slot,
-                                        it.head, page, &full[st]);
+                            tma_load_4d(ring + at.st * PT_TILE + half * PT_HALF + box * br * 128, kv ? &tmv : &tmk, 64 * half,
+                                        slot, it.head, page, &full[at.st]);
+                        at.next();
+                        ++entries;
                     }
                     page = next;
+                    if (j == max(0, nkv - 3) && ok) item = take_over(round);
                 }
-                // no copy outlives the CTA (bounded)
-                for (int d = e > PT_NS ? e - PT_NS : 0; d < e; ++d) mbar_wait(&full[d % PT_NS], uint32_t(d / PT_NS) & 1u, nullptr);
-                mbar_wait(&q_full, 0, nullptr);
             }
+            // no copy outlives the CTA (bounded)
+            for (int d = entries > PT_NS ? entries - PT_NS : 0; d < entries; ++d)
+                mbar_wait(&full[d % PT_NS], uint32_t(d / PT_NS) & 1u, nullptr);
+            if (qs) mbar_wait(&q_full, uint32_t(qs - 1) & 1u, nullptr);
         } else if (warp == 8) {
-            // ---- products ----------------------------------------------------------------
-            if (nkv > 0) {
-                bool ok = mbar_wait(&q_full, 0, lane == 0 ? status : nullptr);
+            // ---- products: one lane, which queues ahead while the tensor cores work -----------
+            if (tc_elect()) {
                 // operand descriptors of the first row tile and the first buffer; a 32 KB tile further is + 2048
                 const uint64_t dq = tc_sdesc(smem_addr(smem)), dk = tc_sdesc(smem_addr(ring)),
                                dv = tc_sdesc_mn(smem_addr(ring), PT_HALF);
-                auto wait = [&](uint64_t *bar, uint32_t parity) {
-                    if (ok) ok = mbar_wait(bar, parity, lane == 0 ? status : nullptr);
-                    ok = __all_sync(FULL, ok);
-                    tc_fence_after();
-                };
                 auto scores = [&](int t, int buf) {          // S_t = Q_t K^T
-                    if (tc_elect()) {
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            const uint32_t off = (uint32_t(k / 4) * PT_HALF + uint32_t(k % 4) * 32) >> 4;
-                            tc_mma_bf16_ss(tbase + t * 128, dq + t * (PT_TILE >> 4) + off, dk + buf * (PT_TILE >> 4) + off,
-                                           PT_IDESC, uint32_t(k > 0));
-                        }
-                        tc_commit(&s_full[t]);
+                    for (int k = 0; k < 8; ++k) {
+                        const uint32_t off = (uint32_t(k / 4) * PT_HALF + uint32_t(k % 4) * 32) >> 4;
+                        tc_mma_bf16_ss(tbase + t * 128, dq + t * (PT_TILE >> 4) + off, dk + buf * (PT_TILE >> 4) + off,
+                                       PT_IDESC, uint32_t(k > 0));
                     }
-                    __syncwarp();
+                    tc_commit(&s_full[t]);
                 };
-                wait(&full[0], 0);
-                if (ok)
-                    for (int t = 0; t < 2; ++t)
-                        if (nt[t]) scores(t, 0);
-                if (ok && tc_elect()) tc_commit(&empty[0]);
-                __syncwarp();
-                int bv = 1, bk = 2;                          // buffers of V(j) and K(j + 1), and how often each was filled before
-                uint32_t pv = 0, pk = 0;
-                for (int j = 0; j < nkv && ok; ++j) {
-                    wait(&full[bv], pv & 1u);
-                    if (!ok) break;
-                    if (j == nkv - 1 && len < nkv * PT_KEYS) {        // values behind the sequence's end: zeros
-                        for (int r = len - j * PT_KEYS + lane / 8; r < PT_KEYS; r += 4)
-                            for (int h = 0; h < 2; ++h)
-                                *reinterpret_cast<uint4 *>(ring + bv * PT_TILE + h * PT_HALF + r * 128 + (lane & 7) * 16) =
-                                    make_uint4(0, 0, 0, 0);
-                        fence_proxy_async_smem();
-                        __syncwarp();
-                    }
-                    for (int t = 0; t < 2 && ok; ++t) {
-                        if (j < nt[t]) {
+                auto values = [&](int t, int buf, int half, bool add) {      // O_t += P_t V over 64 keys
 #pragma unroll
-                            for (int half = 0; half < 2; ++half) {    // O_t += P_t V, 64 keys at a time
-                                wait(&p_full[t][half], uint32_t(j) & 1u);
-                                if (!ok) break;
-                                if (tc_elect()) {
+                    for (int k = 0; k < 4; ++k)
+                        tc_mma_bf16_ts(tbase + 256 + t * 128, tbase + t * 128 + (4 * half + k) * 8,
+                                       dv + buf * (PT_TILE >> 4) + (4 * half + k) * (2048 >> 4), PT_IDESC_V,
+                                       k > 0 ? 1u : uint32_t(add));
+                };
+                RingAt at;
+                int qs = 0, tails = 0;
+                uint32_t steps[2] = {0, 0}, outs[2] = {0, 0};                // key tiles and results of each row tile so far
+                bool ok = true;
+                PromptRound it;
+                for (int round = 0; ok && next_item(round, it, false); ++round) {
+                    const int nkv = max(it.nt[0], it.nt[1]);
+                    if (nkv == 0) continue;
+                    if (!(ok = mbar_wait(&q_full, uint32_t(qs++) & 1u, status))) break;
+                    if (!(ok = mbar_wait(&full[at.st], at.ph, status))) break;
+                    tc_fence_after();
+                    if (it.nt[0]) scores(0, at.st);
+                    if (it.nt[1]) scores(1, at.st);
+                    tc_commit(&empty[at.st]);
+                    if (nkv == 1) tc_commit(&q_empty);
+                    at.next();
+                    for (int j = 0; j < nkv; ++j) {
+                        const RingAt v = at;
+                        at.next();                           // K(j + 1), or the next item's K(0)
+                        if (j == max(0, nkv - 2) && it.len < nkv * PT_KEYS) mbar_arrive(&tail_go);
+                        if (!(ok = mbar_wait(&full[v.st], v.ph, status))) break;
+                        if (j == nkv - 1 && it.len < nkv * PT_KEYS)           // cleared behind the sequence's end
+                            if (!(ok = mbar_wait(&tail, uint32_t(tails++) & 1u, status))) break;
 #pragma unroll
-                                    for (int k = 4 * half; k < 4 * half + 4; ++k)
-                                        tc_mma_bf16_ts(tbase + 256 + t * 128, tbase + t * 128 + k * 8,
-                                                       dv + bv * (PT_TILE >> 4) + k * (2048 >> 4), PT_IDESC_V,
-                                                       k > 0 ? 1u : uint32_t(j > 0));
-                                    if (half && j + 1 == nt[t]) tc_commit(&o_full[t]);
+                        for (int t = 0; t < 2; ++t) {
+                            if (j < it.nt[t]) {
+                                if (j == 0 && outs[t] && !(ok = mbar_wait(&o_empty[t], (outs[t] - 1) & 1u, status))) break;
+                                for (int half = 0; half < 2 && ok; ++half) {
+                                    ok = mbar_wait(&p_full[t][half], steps[t] & 1u, status);
+                                    tc_fence_after();
+                                    if (ok) values(t, v.st, half, j > 0 || half > 0);
                                 }
-                                __syncwarp();
+                                if (!ok) break;
+                                ++steps[t];
+                                if (j + 1 == it.nt[t]) {
+                                    tc_commit(&o_full[t]);
+                                    ++outs[t];
+                                }
                             }
-                            if (!ok) break;
+                            if (j + 1 < it.nt[t]) {
+                                if (!(ok = mbar_wait(&full[at.st], at.ph, status))) break;
+                                tc_fence_after();
+                                scores(t, at.st);
+                            }
                         }
-                        if (j + 1 < nt[t]) {
-                            wait(&full[bk], pk & 1u);
-                            if (!ok) break;
-                            scores(t, bk);
+                        if (!ok) break;
+                        tc_commit(&empty[v.st]);
+                        if (j + 1 < nkv) {
+                            tc_commit(&empty[at.st]);
+                            if (j + 2 == nkv) tc_commit(&q_empty);            // the item's last scores
+                            at.next();
                         }
                     }
-                    if (ok && tc_elect()) {
-                        tc_commit(&empty[bv]);
-                        if (j + 1 < nkv) tc_commit(&empty[bk]);
-                    }
-                    __syncwarp();
-                    if ((bv += 2) >= PT_NS) bv -= PT_NS, ++pv;
-                    if ((bk += 2) >= PT_NS) bk -= PT_NS, ++pk;
                 }
                 // every product issued has completed before tensor memory is given back (bounded)
-                if (tc_elect()) tc_commit(&drain);
-                __syncwarp();
+                tc_commit(&drain);
                 mbar_wait(&drain, 0, nullptr);
+            }
+            __syncwarp();
+        } else if (warp == 10) {
+            // ---- values behind a sequence's end: zeros -----------------------------------------
+            PromptRound it;
+            int entries = 0, tails = 0;                      // of the ring, and cleared ends, in the items so far
+            bool ok = true;
+            for (int round = 0; ok && next_item(round, it, true); ++round) {
+                const int nkv = max(it.nt[0], it.nt[1]);
+                entries += 2 * nkv;
+                if (it.len >= nkv * PT_KEYS || nkv == 0) continue;
+                // The last tile's values.  The products are at the tile before, so the buffer's earlier use is over and
+                // the parity means this one.
+                const int last = entries - 1, st = last % PT_NS;
+                ok = __all_sync(FULL, mbar_wait(&tail_go, uint32_t(tails) & 1u, lane == 0 ? status : nullptr));
+                if (!ok) break;
+                ok = __all_sync(FULL, mbar_wait(&full[st], uint32_t(last / PT_NS) & 1u, lane == 0 ? status : nullptr));
+                if (!ok) break;
+                for (int x = (it.len - (nkv - 1) * PT_KEYS) * 8 + lane; x < PT_KEYS * 8; x += 32)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        *reinterpret_cast<uint4 *>(ring + st * PT_TILE + h * PT_HALF + x * 16) = make_uint4(0, 0, 0, 0);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&tail);
+                ++tails;
             }
         }
     } else {
@@ -268,122 +381,157 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
         const int t = warp >> 2, r = threadIdx.x & 127;      // row tile, row = tensor-memory lane
         const uint32_t lane_base = tbase + (uint32_t(32 * (warp & 3)) << 16);
         const uint32_t ts = lane_base + t * 128, to = lane_base + 256 + t * 128;
-        const int i = it.first + t * qt + r / group;         // the sequence's row
-        const bool live = item && r < qt * group && i < it.rows;
-        const int limit = live ? seen(i) : 0;
-        const int sure = item ? seen(it.first + t * qt) : 0; // keys that every row of the tile sees
-        float m = -INFINITY, sum = 0.0f;
+        const int r_query = t * qt + r / group, r_head = r % group;
+        const bool r_used = r < qt * group;
+        uint32_t steps = 0, outs = 0;                        // key tiles and results so far
         bool ok = true;
-        for (int j = 0; j < nt[t] && ok; ++j) {
-            ok = __all_sync(FULL, mbar_wait(&s_full[t], uint32_t(j) & 1u, lane == 0 ? status : nullptr));
-            if (!ok) break;
-            tc_fence_after();
-            uint32_t u[128];
+        PromptRound it;
+        for (int round = 0; ok && next_item(round, it, true); ++round) {
+            const int nt = it.nt[t], i = it.first + r_query; // i: the sequence's row
+            const bool live = r_used && i < it.rows;
+            const int limit = live ? it.seen(i) : 0;
+            const int sure = it.seen(it.first + t * qt);    // keys that every row of the tile sees
+            float m = -INFINITY, sum = 0.0f;
+            for (int j = 0; j < nt; ++j, ++steps) {
+                ok = __all_sync(FULL, mbar_wait(&s_full[t], steps & 1u, lane == 0 ? status : nullptr));
+                if (!ok) break;
+                tc_fence_after();
+                uint32_t u[128];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) tc_ld32(ts + 32 * x, u + 32 * x);
+                for (int x = 0; x < 4; ++x) tc_ld32(ts + 32 * x, u + 32 * x);
 #pragma unroll
-            for (int x = 0; x < 4; ++x) tc_wait_ld32(u + 32 * x);
-            if ((j + 1) * PT_KEYS > sure) {
+                for (int x = 0; x < 4; ++x) tc_wait_ld32(u + 32 * x);
+                if ((j + 1) * PT_KEYS > sure) {
 #pragma unroll
-                for (int x = 0; x < 4; ++x) mask32(u + 32 * x, limit - j * PT_KEYS - 32 * x);
-            }
-            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    for (int x = 0; x < 4; ++x) mask32(u + 32 * x, limit - j * PT_KEYS - 32 * x);
+                }
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int x = 0; x < 128; x += 8)
+                for (int x = 0; x < 128; x += 8)
 #pragma unroll
-                for (int y = 0; y < 4; ++y)
-                    mx[y] = fmaxf(fmaxf(mx[y], __uint_as_float(u[x + y])), __uint_as_float(u[x + y + 4]));
-            const float tile_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-            const bool grow = tile_max > m + PT_LAZY || (m == -INFINITY && tile_max > m);
-            if (__any_sync(FULL, grow)) {
-                const float nm = grow ? tile_max : m;
-                const float f = grow ? (m == -INFINITY ? 0.0f : ex2_approx_ftz((m - nm) * PT_LOG2)) : 1.0f;
-                m = nm;
-                sum *= f;
-                if (j > 0) {                                 // O of the tiles before (their product has completed)
+                    for (int y = 0; y < 4; ++y)
+                        mx[y] = fmaxf(fmaxf(mx[y], __uint_as_float(u[x + y])), __uint_as_float(u[x + y + 4]));
+                const float tile_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                const bool grow = tile_max > m + PT_LAZY || (m == -INFINITY && tile_max > m);
+                if (__any_sync(FULL, grow)) {
+                    const float nm = grow ? tile_max : m;
+                    const float f = grow ? (m == -INFINITY ? 0.0f : ex2_approx_ftz((m - nm) * PT_LOG2)) : 1.0f;
+                    m = nm;
+                    sum *= f;
+                    if (j > 0) {                                 // O of the tiles before (their product has completed)
 #pragma unroll 1
-                    for (int x = 0; x < 8; ++x) {
-                        uint32_t o[16];
-                        tc_ld16(to + 16 * x, o);
-                        tc_wait_ld16(o);
+                        for (int x = 0; x < 8; ++x) {
+                            uint32_t o[16];
+                            tc_ld16(to + 16 * x, o);
+                            tc_wait_ld16(o);
 #pragma unroll
-                        for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
-                        tc_st16(to + 16 * x, o);
+                            for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
+                            tc_st16(to + 16 * x, o);
+                        }
                     }
                 }
+                const float off = m == -INFINITY ? 0.0f : -m * PT_LOG2;
+                const f2 off2 = pk2(off, off), scale2 = pk2(PT_LOG2, PT_LOG2);
+                f2 part[2] = {pk2(0.0f, 0.0f), pk2(0.0f, 0.0f)};
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {                    // 32 probabilities at a time; two halves are handed over
+                    uint32_t w[16];
+#pragma unroll
+                    for (int y = 0; y < 32; y += 2) {
+                        const f2 e = fma2(pk2(__uint_as_float(u[32 * x + y]), __uint_as_float(u[32 * x + y + 1])), scale2, off2);
+                        float p0, p1;
+                        up2(e, p0, p1);
+                        if (y % PT_POLY == PT_POLY - 2) {
+                            exp2_poly(p0, p1);
+                        } else {
+                            p0 = ex2_approx_ftz(p0);
+                            p1 = ex2_approx_ftz(p1);
+                        }
+                        part[y / 2 & 1] = add2(part[y / 2 & 1], pk2(p0, p1));
+                        w[y / 2] = pack_bf16(p0, p1);
+                    }
+                    tc_st16(ts + 16 * x, w);
+                    if (x & 1) {
+                        tc_wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&p_full[t][x >> 1]);
+                    }
+                }
+                float s0, s1;
+                up2(add2(part[0], part[1]), s0, s1);
+                sum += s0 + s1;
             }
-            const float off = m == -INFINITY ? 0.0f : -m * PT_LOG2;
-            const f2 off2 = pk2(off, off), scale2 = pk2(PT_LOG2, PT_LOG2);
-            f2 part[2] = {pk2(0.0f, 0.0f), pk2(0.0f, 0.0f)};
+            // ---- the result ----------------------------------------------------------------
+            if (nt > 0 && ok) {
+                ok = __all_sync(FULL, mbar_wait(&o_full[t], outs++ & 1u, lane == 0 ? status : nullptr));
+                tc_fence_after();
+            }
+            if (ok) {
+                const float inv = limit > 0 ? 1.0f / sum : 0.0f;
+                const unsigned lives = __ballot_sync(FULL, live);
+                // Four lanes exchange their rows' pieces, so that they store 64 bytes of a row together.  This lane
+                // stores piece lane % 4 of rows (lane / 4) * 4 + k.
+                uint16_t *dst[4];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {                    // 32 probabilities at a time; two halves are handed over
-                uint32_t w[16];
-#pragma unroll
-                for (int y = 0; y < 32; y += 2) {
-                    const f2 e = fma2(pk2(__uint_as_float(u[32 * x + y]), __uint_as_float(u[32 * x + y + 1])), scale2, off2);
-                    float p0, p1;
-                    up2(e, p0, p1);
-                    if (y % PT_POLY == PT_POLY - 2) {
-                        exp2_poly(p0, p1);
-                    } else {
-                        p0 = ex2_approx_ftz(p0);
-                        p1 = ex2_approx_ftz(p1);
-                    }
-                    part[y / 2 & 1] = add2(part[y / 2 & 1], pk2(p0, p1));
-                    w[y / 2] = pack_bf16(p0, p1);
+                for (int k = 0; k < 4; ++k) {
+                    const int row = 32 * (warp & 3) + (lane & 28) + k, query = by_group(row);
+                    dst[k] = out + (int64_t(it.base + it.first + t * qt + query) * n_heads + it.head * group + row - query * group) * HD +
+                             8 * (lane & 3);
                 }
-                tc_st16(ts + 16 * x, w);
-                if (x & 1) {
-                    tc_wait_st();
+                f2 zero = pk2(0.0f, 0.0f);                   // becomes NaN with a value that is no number (or infinite)
+#pragma unroll 1
+                for (int x = 0; x < 4; ++x) {                // 32 columns: four 16-byte pieces of bf16
+                    uint32_t o[32], w[4][4];
+                    if (nt > 0) {
+                        tc_ld32(to + 32 * x, o);
+                        tc_wait_ld32(o);
+                    }
+#pragma unroll
+                    for (int z = 0; z < 32; z += 2) {
+                        const f2 v = mul2(pk2(__uint_as_float(o[z]), __uint_as_float(o[z + 1])), pk2(inv, inv));
+                        zero = fma2(v, pk2(0.0f, 0.0f), zero);
+                        float a, d;
+                        up2(v, a, d);
+                        w[z / 8][z / 2 & 3] = limit > 0 ? pack_bf16(a, d) : 0u;
+                    }
+#pragma unroll
+                    for (int s = 2; s > 0; s >>= 1)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (!(k & s))
+#pragma unroll
+                                for (int y = 0; y < 4; ++y) {
+                                    const uint32_t got = __shfl_xor_sync(FULL, lane & s ? w[k][y] : w[k ^ s][y], s);
+                                    if (lane & s) w[k][y] = got;
+                                    else w[k ^ s][y] = got;
+                                }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (lives >> ((lane & 28) + k) & 1u)
+                            st_cs_v4(dst[k] + 32 * x, make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]));
+                }
+                float z0, z1;
+                up2(zero, z0, z1);
+                const bool nan = z0 + z1 != 0.0f;
+                if (nt > 0) {                                // the next item's products may overwrite O
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&p_full[t][x >> 1]);
+                    if (lane == 0) mbar_arrive(&o_empty[t]);
                 }
-            }
-            float s0, s1;
-            up2(add2(part[0], part[1]), s0, s1);
-            sum += s0 + s1;
-        }
-        // ---- the result ----------------------------------------------------------------
-        if (nt[t] > 0 && ok) {
-            ok = __all_sync(FULL, mbar_wait(&o_full[t], 0, lane == 0 ? status : nullptr));
-            tc_fence_after();
-        }
-        if (ok && item) {
-            uint16_t *dst = out + ((it.base + i) * n_heads + it.head * group + r % group) * HD;
-            const float inv = limit > 0 ? 1.0f / sum : 0.0f;
-            bool nan = false;
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                uint32_t o[32];
-                if (nt[t] > 0) {
-                    tc_ld32(to + 32 * x, o);
-                    tc_wait_ld32(o);
+                // rows that came out as NaN, once more from the formula
+                unsigned again = __ballot_sync(FULL, live && limit > 0 && nan);
+                while (again) {
+                    const int l = __ffs(again) - 1;
+                    again &= again - 1;
+                    __syncwarp();
+                    const int il = __shfl_sync(FULL, i, l), n = __shfl_sync(FULL, limit, l);
+                    const int h = it.head * group + __shfl_sync(FULL, r_head, l);
+                    float4 x = load_quad(q + int64_t(it.base + il) * q_stride + int64_t(h) * HD + 4 * lane);
+                    x = make_float4(x.x * ATT_SCALE, x.y * ATT_SCALE, x.z * ATT_SCALE, x.w * ATT_SCALE);
+                    store_quad(out + (int64_t(it.base + il) * n_heads + h) * HD + 4 * lane,
+                               attend_row<bf16raw>(c, b, it.s, it.head, n, x, status));
                 }
-#pragma unroll
-                for (int y = 0; y < 32; y += 2) {
-                    const float a = __uint_as_float(o[y]) * inv, d = __uint_as_float(o[y + 1]) * inv;
-                    nan |= a != a || d != d;
-                    o[y / 2] = limit > 0 ? pack_bf16(a, d) : 0u;
-                }
-                if (live) {
-#pragma unroll
-                    for (int y = 0; y < 16; y += 4)
-                        st_cs_v4(dst + 32 * x + 2 * y, make_uint4(o[y], o[y + 1], o[y + 2], o[y + 3]));
-                }
-            }
-            // rows that came out as NaN, once more from the formula
-            unsigned again = __ballot_sync(FULL, live && limit > 0 && nan);
-            while (again) {
-                const int l = __ffs(again) - 1;
-                again &= again - 1;
-                __syncwarp();
-                const int il = __shfl_sync(FULL, i, l), n = __shfl_sync(FULL, limit, l);
-                const int h = it.head * group + __shfl_sync(FULL, r % group, l);
-                float4 x = load_quad(q + (it.base + il) * q_stride + int64_t(h) * HD + 4 * lane);
-                x = make_float4(x.x * ATT_SCALE, x.y * ATT_SCALE, x.z * ATT_SCALE, x.w * ATT_SCALE);
-                store_quad(out + ((it.base + il) * n_heads + h) * HD + 4 * lane,
-                           attend_row<bf16raw>(c, b, it.s, it.head, n, x, status));
             }
         }
     }
@@ -410,8 +558,8 @@ cudaError_t launch_attention_prompt(const PagedKV &c, const PagedSeqs &b, int64_
     // no more blocks of 2 * qt queries than this, however the rows are split into sequences
     const int64_t items = (rows / (2 * qt) + b.n_seqs) * c.n_kv;
     return launch_dependent(prompt_tc_kernel, dim3(unsigned(items)), dim3(PT_THREADS), PT_SMEM, stream, mq, mk, mv, c, b,
-                            rows, static_cast<const uint16_t *>(q), q_stride, n_heads, group,
-                            static_cast<uint16_t *>(out), status);
+                            int(rows), static_cast<const uint16_t *>(q), q_stride, n_heads, group, FastDiv(2 * qt),
+                            FastDiv(group), static_cast<uint16_t *>(out), status);
 }
 
 }  // namespace q3

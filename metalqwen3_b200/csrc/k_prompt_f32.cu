@@ -28,8 +28,8 @@ constexpr float PF_LOG2 = ATT_SCALE * 1.44269504088896341f;
 
 __global__ void __launch_bounds__(PF_THREADS, 2)
 prompt_f32_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, const PagedKV c,
-                  const PagedSeqs b, int64_t rows, const float *q, int64_t q_stride, int n_heads, int group, float *out,
-                  uint32_t *status) {
+                  const PagedSeqs b, int rows, const float *q, int64_t q_stride, int n_heads, int group,
+                  const FastDiv per_block, float *out, uint32_t *status) {
     extern __shared__ uint8_t pf_dyn[];
     uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(pf_dyn) + 1023) & ~uintptr_t(1023));
     float *qs = reinterpret_cast<float *>(ring + PF_NS * PF_STAGE);
@@ -43,22 +43,18 @@ prompt_f32_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant
         mbar_init_fence();
     }
     griddep_wait();
-    const int qt = PF_ROWS / group;                          // queries of an item
-    const PromptItem it = prompt_item(b, c, rows, qt, blockIdx.x);
+    const int qt = per_block.d;                              // queries of an item
+    const PromptItem it = PromptOrder(b, c, rows, per_block, PF_KEYS, warp == 0 ? status : nullptr).find(blockIdx.x);
     if (it.s < 0) return;
-    const int len = paged_len(b, c, it.s, threadIdx.x == 0 ? status : nullptr);
-    const int64_t pos0 = int64_t(b.kv_len[it.s]) - it.rows;
-    auto seen = [&](int i) -> int {                          // keys that the sequence's row i sees
-        const int64_t n = pos0 + i + 1;
-        return n < 0 ? 0 : n < len ? int(n) : len;
-    };
+    const int len = it.len;
+    auto seen = [&](int i) { return it.seen(i); };
     const int queries = min(qt, it.rows - it.first);
     const int nkv = (seen(it.first + queries - 1) + PF_KEYS - 1) / PF_KEYS;
     // the queries, 16-byte chunk x of row r at x ^ (r % 8) of its 128-byte block
     for (int x = threadIdx.x; x < PF_ROWS * (HD / 4); x += PF_THREADS) {
         const int r = x / (HD / 4), ch = x % (HD / 4);
         const bool live = r < queries * group;
-        const float4 v = live ? load_quad(q + (it.base + it.first + r / group) * q_stride +
+        const float4 v = live ? load_quad(q + int64_t(it.base + it.first + r / group) * q_stride +
                                           int64_t(it.head * group + r % group) * HD + 4 * ch)
                               : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         *reinterpret_cast<float4 *>(qs + r * HD + 4 * ((ch & 24) | ((ch ^ r) & 7))) = v;
@@ -230,7 +226,7 @@ prompt_f32_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant
         l[h] += __shfl_xor_sync(FULL, l[h], 2);
         const int r = 16 * warp + g + 8 * h;
         const float inv = limit[h] > 0 ? 1.0f / l[h] : 0.0f;
-        float *dst = out + ((it.base + i_of[h]) * n_heads + it.head * group + r % group) * HD + 8 * t4;
+        float *dst = out + (int64_t(it.base + i_of[h]) * n_heads + it.head * group + r % group) * HD + 8 * t4;
 #pragma unroll
         for (int d = 0; d < 4; ++d)
 #pragma unroll
@@ -254,9 +250,9 @@ prompt_f32_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant
             __syncwarp();
             const int i = __shfl_sync(FULL, i_of[h], first), n = __shfl_sync(FULL, limit[h], first);
             const int head = it.head * group + (16 * warp + first / 4 + 8 * h) % group;
-            float4 x = load_quad(q + (it.base + i) * q_stride + int64_t(head) * HD + 4 * lane);
+            float4 x = load_quad(q + int64_t(it.base + i) * q_stride + int64_t(head) * HD + 4 * lane);
             x = make_float4(x.x * ATT_SCALE, x.y * ATT_SCALE, x.z * ATT_SCALE, x.w * ATT_SCALE);
-            store_quad(out + ((it.base + i) * n_heads + head) * HD + 4 * lane,
+            store_quad(out + (int64_t(it.base + i) * n_heads + head) * HD + 4 * lane,
                        attend_row<float>(c, b, it.s, it.head, n, x, status));
         }
     }
@@ -272,8 +268,9 @@ cudaError_t launch_prompt_f32(const PagedKV &c, const PagedSeqs &b, int64_t rows
     if (e != cudaSuccess) return e;
     // no more items than this, however the rows are split into sequences
     const int64_t items = (rows / qt + b.n_seqs) * c.n_kv;
-    return launch_dependent(prompt_f32_kernel, dim3(unsigned(items)), dim3(PF_THREADS), PF_SMEM, stream, mk, mv, c, b, rows,
-                            static_cast<const float *>(q), q_stride, n_heads, group, static_cast<float *>(out), status);
+    return launch_dependent(prompt_f32_kernel, dim3(unsigned(items)), dim3(PF_THREADS), PF_SMEM, stream, mk, mv, c, b,
+                            int(rows), static_cast<const float *>(q), q_stride, n_heads, group, FastDiv(qt),
+                            static_cast<float *>(out), status);
 }
 
 }  // namespace q3

@@ -143,6 +143,22 @@ struct PagedSeqs {                     // q3cu_kv_batch
     const int32_t *row_off, *kv_len, *pages;
     int n_seqs, max_pages;
 };
+// n / d for 0 <= n < 2^31 by a multiplication: m = ceil(2^(31+L) / d), L = ceil(log2 d), n / d = (n m >> 32) >> (L - 1);
+// the excess of m over the quotient is below 2^L / d, which n < 2^31 does not raise to one.  (A division's conversions
+// would queue behind the exponentials of a softmax.)
+struct FastDiv {
+    int d;
+    uint32_t m;
+    int shift;               // L - 1; negative for d = 1
+    explicit FastDiv(int d_) : d(d_), m(0), shift(-1) {
+        int l = 0;
+        while ((1 << l) < d) ++l;
+        if (l) m = uint32_t(((uint64_t(1) << (31 + l)) + d - 1) / d), shift = l - 1;
+    }
+    __host__ __device__ int operator()(int n) const {
+        return shift < 0 ? n : int(uint32_t((uint64_t(uint32_t(n)) * m) >> 32) >> shift);
+    }
+};
 struct TurnFreq { double v[64]; };     // theta^(-j/64) / (2 pi)
 cudaError_t launch_kv_append(const PagedKV &c, q3cu_dtype cache_dt, const PagedSeqs &b, int64_t rows, const void *q,
                              const void *k, const void *v, q3cu_dtype dt, int64_t q_stride, int64_t kv_stride,

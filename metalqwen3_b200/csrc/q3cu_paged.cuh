@@ -160,50 +160,146 @@ __device__ __forceinline__ float4 attend_row(const PagedKV &c, const PagedSeqs &
     return make_float4(o.x * r, o.y * r, o.z * r, o.w * r);
 }
 
-// The items of a launch, in the order of blockIdx: sequence by sequence, from a
-// sequence's last block (the most keys) to its first, kv heads innermost.
+// ---- the work items of a prompt launch ------------------------------------------------------
+// A sequence's rows fall into blocks of `per_block` queries; a block under one kv head is an item.  Its work is the
+// number of key tiles that its last row sees.
 struct PromptItem {
     int s, head;             // sequence (-1: none), kv head
-    int first, rows;         // first query row within the sequence, the sequence's rows
-    int64_t base;            // the sequence's first packed row
+    int first, rows, len;    // first query row within the sequence; the sequence's rows and keys
+    int base, pos0;          // the sequence's first packed row and its position
+    __host__ __device__ __forceinline__ int seen(int i) const {            // keys that the sequence's row i sees
+        const int n = pos0 + i + 1;                          // at most the sequence's kv_len
+        return n < 0 ? 0 : n < len ? n : len;
+    }
 };
-__device__ __forceinline__ PromptItem prompt_item(const PagedSeqs &b, const PagedKV &c, int64_t total_rows, int per_block,
-                                                  int64_t block) {
-    PromptItem it;
-    it.s = -1;
-    it.head = int(block % c.n_kv);
-    int64_t left = block / c.n_kv;
-    const int lane = threadIdx.x & 31;
-    for (int s0 = 0; s0 < b.n_seqs; s0 += 32) {              // 32 sequences at a time, by one warp
-        const int s = s0 + lane;
-        int64_t lo = 0, hi = 0;
-        if (s < b.n_seqs) {
-            lo = b.row_off[s];
-            hi = b.row_off[s + 1];
-            if (hi > total_rows) hi = total_rows;
-            if (lo < 0 || hi < lo) lo = hi = 0;              // offsets that do not rise: no rows
-        }
-        const int n = int(hi - lo), blocks = (n + per_block - 1) / per_block;
-        int64_t end = blocks;
+// What a lane knows of its sequence.
+struct PromptSeq {
+    int base, pos0, rows, blocks, len;
+    // blocks whose last row sees at least `keys` keys
+    __host__ __device__ __forceinline__ int at_least(int keys, const FastDiv &per_block) const {
+        if (keys > len) return 0;
+        const int need = keys - pos0;                        // rows that it takes: at most all
+        return keys <= 0 || need <= 0 ? blocks : blocks - per_block(need - 1);
+    }
+};
+__host__ __device__ __forceinline__ PromptSeq prompt_seq(const PagedSeqs &b, const PagedKV &c, int total_rows,
+                                                         const FastDiv &per_block, int s, uint32_t *status) {
+    PromptSeq q = {0, 0, 0, 0, 0};
+    if (s >= b.n_seqs) return q;
+    int lo = b.row_off[s], hi = b.row_off[s + 1];
+    if (hi > total_rows) hi = total_rows;
+    if (lo < 0 || hi <= lo) return q;                        // no rows, or offsets that do not rise
+    const int kv_len = b.kv_len[s];
+    q.base = lo;
+    q.rows = hi - lo;
+    q.blocks = per_block(q.rows - 1) + 1;
+    q.pos0 = (kv_len < 0 ? 0 : kv_len) - q.rows;
+    q.len = paged_len(b, c, s, status);
+    return q;
+}
+__device__ __forceinline__ int lanes_before(int x) {         // sum over the lanes below this one
+    int y = x;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int64_t x = __shfl_up_sync(FULL, end, o);
-            if (lane >= o) end += x;
-        }
-        const unsigned hit = __ballot_sync(FULL, left < end);
-        if (hit) {
-            const int l = __ffs(hit) - 1;
-            const int64_t end_l = __shfl_sync(FULL, end, l);
-            it.s = s0 + l;
-            it.rows = __shfl_sync(FULL, n, l);
-            it.base = __shfl_sync(FULL, lo, l);
-            it.first = int(end_l - 1 - left) * per_block;    // the last block first
+    for (int o = 1; o < 32; o <<= 1) {
+        const int z = __shfl_up_sync(FULL, y, o);
+        if ((threadIdx.x & 31) >= o) y += z;
+    }
+    return y - x;
+}
+// The order of a launch's items: kv heads innermost, blocks from the most key tiles to the fewest, so that no long item
+// begins last.  Held by one warp, lane l with sequences l and l + 32; find() takes rising indices and returns the same
+// in every lane.  A block's place is found by the number of tiles at which the count of larger blocks passes its index:
+// the level of the item before or the next lower one mostly, bisection otherwise.  Past PROMPT_SORTED sequences, which
+// the lanes cannot hold, the order is sequence by sequence, the last block first.
+constexpr int PROMPT_SORTED = 64;
+struct PromptOrder {
+    PromptSeq q[2];
+    const PagedSeqs &b;
+    const PagedKV &c;
+    const FastDiv &per_block;
+    int total_rows, tile_keys;
+    uint32_t *status;
+    int hi, above;           // blocks of at least hi tiles: `above`, no more than the latest index
+
+    __device__ __forceinline__ PromptOrder(const PagedSeqs &b_, const PagedKV &c_, int total_rows_, const FastDiv &per_block_,
+                                           int tile_keys_, uint32_t *status_)
+        : b(b_), c(c_), per_block(per_block_), total_rows(total_rows_), tile_keys(tile_keys_), status(status_) {
+        const int lane = threadIdx.x & 31;
+        const bool sorted = b.n_seqs <= PROMPT_SORTED;
+        q[0] = prompt_seq(b, c, total_rows, per_block, sorted ? lane : b.n_seqs, status);
+        q[1] = prompt_seq(b, c, total_rows, per_block, sorted ? lane + 32 : b.n_seqs, status);
+        hi = (max(__reduce_max_sync(FULL, q[0].len), __reduce_max_sync(FULL, q[1].len)) + tile_keys - 1) / tile_keys + 1;
+        above = 0;
+    }
+    __device__ __forceinline__ int at_least(int x, int tiles) const {
+        return q[x].at_least(tiles ? (tiles - 1) * tile_keys + 1 : 0, per_block);
+    }
+    __device__ __forceinline__ int count(int tiles) const {
+        return int(__reduce_add_sync(FULL, at_least(0, tiles) + at_least(1, tiles)));
+    }
+    static __device__ __forceinline__ void take(PromptItem &it, const PromptSeq &from, int s, int l, int first) {
+        it.s = s;
+        it.rows = __shfl_sync(FULL, from.rows, l);
+        it.len = __shfl_sync(FULL, from.len, l);
+        it.base = __shfl_sync(FULL, from.base, l);
+        it.pos0 = __shfl_sync(FULL, from.pos0, l);
+        it.first = __shfl_sync(FULL, first, l);
+    }
+    __device__ __forceinline__ PromptItem find(int64_t index) {
+        PromptItem it;
+        it.s = -1;
+        it.head = int(uint32_t(index) % uint32_t(c.n_kv));
+        int left = int(uint32_t(index) / uint32_t(c.n_kv));
+        const int lane = threadIdx.x & 31;
+        if (b.n_seqs > PROMPT_SORTED) {
+            for (int s0 = 0; s0 < b.n_seqs; s0 += 32) {
+                const PromptSeq p = prompt_seq(b, c, total_rows, per_block, s0 + lane, status);
+                const int before = lanes_before(p.blocks);
+                const unsigned hit = __ballot_sync(FULL, left >= before && left < before + p.blocks);
+                if (hit) {
+                    const int l = __ffs(hit) - 1;
+                    take(it, p, s0 + l, l, (p.blocks - 1 - (left - before)) * per_block.d);
+                    return it;
+                }
+                left -= __reduce_add_sync(FULL, p.blocks);
+            }
             return it;
         }
-        left -= __shfl_sync(FULL, end, 31);
+        if (b.n_seqs == 1) {
+            const int blocks = __shfl_sync(FULL, q[0].blocks, 0);
+            if (left < blocks) take(it, q[0], 0, 0, (blocks - 1 - left) * per_block.d);
+            return it;
+        }
+        // to the level with above <= left < count(hi - 1)
+        int down = hi > 0 ? count(hi - 1) : 0;
+        if (down <= left) {
+            const int all = count(0);
+            if (hi == 0 || left >= all) return it;           // there are no more
+            int lo = 0, top = hi - 1;                        // count(lo) > left >= count(top)
+            above = down;
+            down = all;
+            while (top - lo > 1) {
+                const int mid = (lo + top) >> 1, n = count(mid);
+                if (n > left) lo = mid, down = n;
+                else top = mid, above = n;
+            }
+            hi = top;
+        }
+        left -= above;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const int more = at_least(x, hi), equal = at_least(x, hi - 1) - more, before = lanes_before(equal);
+            const unsigned hit = __ballot_sync(FULL, left >= before && left < before + equal);
+            if (hit) {
+                const int l = __ffs(hit) - 1;
+                take(it, q[x], 32 * x + l, l, (q[x].blocks - more - 1 - (left - before)) * per_block.d);
+                return it;
+            }
+            left -= __reduce_add_sync(FULL, equal);
+        }
+        return it;
     }
-    return it;
-}
+};
 
 constexpr float ATT_SCALE = 0.08838834764831845f;            // 1/sqrt(128)
 
