@@ -130,16 +130,27 @@ def _tensor(t, what, dtype=None, shape=None, device=None):
         raise ValueError(f"{what} must be on the context's GPU, it is on {t.device}")
     if dtype is not None and t.dtype != dtype:
         raise TypeError(f"{what} must be {dtype}, it is {t.dtype}")
-    if shape is not None and (t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape))):
+    if shape is not None and tuple(t.shape) != shape:
         raise ValueError(f"{what} must be {list(shape)}, it is {list(t.shape)}")
     return t
 
 
-def _rows(t, what):
-    """Row stride in elements of t [rows][heads][128], whose rows are dense."""
-    if t.numel() and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2])):
-        raise ValueError(f"{what}: the heads of a row must be contiguous, strides are {t.stride()}")
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1] * t.shape[2])
+def _rows(t, what, dtype, heads, rows, device):
+    """Checks t [rows][heads][128] (heads or rows None: any) with dense heads; returns (row stride in elements, rows,
+    heads, pointer)."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or shape[2] != 128 or (heads is not None and shape[1] != heads) or (
+            rows is not None and shape[0] != rows):
+        raise ValueError(f"{what} must be [{'rows' if rows is None else rows}][{'heads' if heads is None else heads}]"
+                         f"[128], it is {list(shape)}")
+    if t.get_device() != device:                    # -1 on the CPU
+        raise ValueError(f"{what} must be on the context's GPU, it is on {t.device}")
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError(f"{what} must be {dtype}, it is {t.dtype}")
+    n, h = shape[0], shape[1]
+    if (stride[2] != 1 or (h > 1 and stride[1] != 128)) and n * h:
+        raise ValueError(f"{what}: the heads of a row must be contiguous, strides are {stride}")
+    return stride[0] if n > 1 else max(stride[0], h * 128), n, h, t.data_ptr()
 
 
 class KVCache:
@@ -157,6 +168,7 @@ class KVCache:
         self.k, self.v, self.n_kv = k, v, n_kv
         self.c = _KVCache(k.data_ptr(), v.data_ptr(), k.stride(0) if n_pages > 1 else n_kv * size * hd, n_pages, n_kv,
                           size, hd, _dtype(k))
+        self.ref = C.byref(self.c)
 
 
 class KVBatch:
@@ -166,12 +178,15 @@ class KVBatch:
     def __init__(self, kv_len, pages, row_off=None):
         n = kv_len.numel()
         i32 = kv_len.new_empty(0).int().dtype
-        for t, what, shape in ((kv_len, "kv_len", (n,)), (pages, "pages", (n, None)), (row_off, "row_off", (n + 1,))):
+        if pages.dim() != 2:
+            raise ValueError(f"pages must be [n_seqs][max_pages], it is {list(pages.shape)}")
+        for t, what, shape in ((kv_len, "kv_len", (n,)), (pages, "pages", (n, pages.shape[1])), (row_off, "row_off", (n + 1,))):
             if t is not None and not _tensor(t, what, i32, shape).is_contiguous():
                 raise ValueError(f"{what} must be contiguous")
         self.kv_len, self.pages, self.row_off = kv_len, pages, row_off
         self.c = _KVBatch(None if row_off is None else row_off.data_ptr(), kv_len.data_ptr(), pages.data_ptr(), n,
                           pages.shape[1])
+        self.ref = C.byref(self.c)
 
 
 class Q3CU:
@@ -182,6 +197,7 @@ class Q3CU:
         self.torch = torch
         self.lib = load_library()
         self.device = device
+        self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         torch.cuda.set_device(device)
         h = C.c_void_p()
         self._check(self.lib.q3cu_init(device, C.byref(h)), "q3cu_init")
@@ -193,8 +209,10 @@ class Q3CU:
             raise Q3Error(status, op, (self.lib.q3cu_last_error_string() or b"").decode())
 
     def _stream(self, stream=None):
-        s = stream if stream is not None else self.torch.cuda.current_stream(self.device)
-        return C.c_void_p(s.cuda_stream)
+        if stream is not None:
+            return stream.cuda_stream
+        raw = self._raw_stream                  # the handle alone: a Stream object takes a microsecond to make
+        return raw(self.device) if raw else self.torch.cuda.current_stream(self.device).cuda_stream
 
     def close(self):
         if getattr(self, "ctx", None):
@@ -326,27 +344,30 @@ class Q3CU:
         """QK-norm (where weights are given) and rotation of the packed rows q [rows][n_heads][128] and
         k [rows][n_kv][128] (q may be None); keys and values into the cache; returns the rotated queries
         (out_dtype, the cache's type by default, or q_out).  q, k, v may be slices of one projection's rows."""
-        rows = k.shape[0]
-        _tensor(k, "k", None, (rows, cache.n_kv, 128), self.device)
-        _tensor(v, "v", k.dtype, (rows, cache.n_kv, 128), self.device)
-        for w, what in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-            if w is not None and not _tensor(w, what, self.torch.float32, (128,), self.device).is_contiguous():
-                raise ValueError(f"{what} must be contiguous")
-        kv_stride, q_stride, heads = _rows(k, "k"), 0, 0
-        if rows > 1 and _rows(v, "v") != kv_stride:
+        dev, dtype = self.device, k.dtype
+        kv_stride, rows, _, kp = _rows(k, "k", None, cache.n_kv, None, dev)
+        v_stride, _, _, vp = _rows(v, "v", dtype, cache.n_kv, rows, dev)
+        if v_stride != kv_stride:
             raise ValueError("k and v must have one row stride")
+        for w, what in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+            if w is not None and (w.dtype != self.torch.float32 or w.shape != (128,) or w.stride() != (1,)
+                                  or w.get_device() != dev):
+                raise ValueError(f"{what} must be 128 contiguous float32 on the context's GPU")
+        q_stride, heads, qp, op, ot = 0, 0, None, None, F32
         if q is not None:
-            heads = _tensor(q, "q", k.dtype, (rows, None, 128), self.device).shape[1]
-            q_stride = _rows(q, "q")
+            q_stride, _, heads, qp = _rows(q, "q", dtype, None, rows, dev)
             if q_out is None:
                 q_out = self.torch.empty((rows, heads, 128), dtype=out_dtype or cache.k.dtype, device=q.device)
-            if not _tensor(q_out, "q_out", out_dtype, (rows, heads, 128), self.device).is_contiguous():
+            _, _, _, op = _rows(q_out, "q_out", out_dtype, heads, rows, dev)
+            if not q_out.is_contiguous():
                 raise ValueError("q_out must be contiguous")
-        self._check(self.lib.q3cu_kv_append(self.ctx, C.byref(cache.c), C.byref(batch.c), rows, _ptr(q), _ptr(k),
-                                            _ptr(v), _dtype(k), q_stride, kv_stride, heads, _ptr(q_norm),
-                                            _ptr(k_norm), theta, eps, _ptr(q_out) if q is not None else None,
-                                            _dtype(q_out) if q is not None else F32, self._stream(stream)),
-                    "q3cu_kv_append")
+            ot = _dtype(q_out)
+        status = self.lib.q3cu_kv_append(self.ctx, cache.ref, batch.ref, rows, qp, kp, vp, _dtype(k), q_stride, kv_stride,
+                                         heads, None if q_norm is None else q_norm.data_ptr(),
+                                         None if k_norm is None else k_norm.data_ptr(), theta, eps, op, ot,
+                                         self._stream(stream))
+        if status:
+            self._check(status, "q3cu_kv_append")
         return q_out
 
     def attention_paged_workspace(self, cache, n_heads):
@@ -357,33 +378,37 @@ class Q3CU:
                     "q3cu_attention_paged_workspace")
         return self.torch.empty(n.value, dtype=self.torch.uint8, device=cache.k.device)
 
-    def _query(self, q, out, rows):
-        _tensor(q, "q", None, (rows, None, 128), self.device)
-        out = self.torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
-        if not _tensor(out, "out", q.dtype, tuple(q.shape), self.device).is_contiguous():
-            raise ValueError("out must be contiguous")
-        return out
-
     def attention_paged(self, cache, batch, q, out=None, work=None, stream=None):
         """One new token per sequence: q [n_seqs][n_heads][128] over each sequence's kv_len positions."""
-        out = self._query(q, out, batch.c.n_seqs)
+        stride, rows, heads, qp = _rows(q, "q", None, None, batch.c.n_seqs, self.device)
+        if out is None:
+            out = self.torch.empty((rows, heads, 128), dtype=q.dtype, device=q.device)
+        elif not out.is_contiguous():
+            raise ValueError("out must be contiguous")
+        op = _rows(out, "out", q.dtype, heads, rows, self.device)[3]
         if work is None:
-            work = self.attention_paged_workspace(cache, q.shape[1])
+            work = self.attention_paged_workspace(cache, heads)
             if stream is not None:
                 work.record_stream(stream)      # its memory is not given out again before the call has run
-        self._check(self.lib.q3cu_attention_paged(self.ctx, C.byref(cache.c), C.byref(batch.c), _ptr(q), _dtype(q),
-                                                  _rows(q, "q"), q.shape[1], _ptr(work),
-                                                  work.numel() * work.element_size(), _ptr(out),
-                                                  self._stream(stream)), "q3cu_attention_paged")
+        status = self.lib.q3cu_attention_paged(self.ctx, cache.ref, batch.ref, qp, _dtype(q), stride, heads,
+                                               work.data_ptr(), work.nbytes, op, self._stream(stream))
+        if status:
+            self._check(status, "q3cu_attention_paged")
         return out
 
     def attention_prompt(self, cache, batch, q, out=None, stream=None):
         """Causal attention of the packed rows q [rows][n_heads][128] over the cache, which holds their
         keys and values; rows behind the last sequence are not written."""
-        out = self._query(q, out, q.shape[0])
-        self._check(self.lib.q3cu_attention_prompt(self.ctx, C.byref(cache.c), C.byref(batch.c), q.shape[0], _ptr(q),
-                                                   _dtype(q), _rows(q, "q"), q.shape[1], _ptr(out),
-                                                   self._stream(stream)), "q3cu_attention_prompt")
+        stride, rows, heads, qp = _rows(q, "q", None, None, None, self.device)
+        if out is None:
+            out = self.torch.empty((rows, heads, 128), dtype=q.dtype, device=q.device)
+        elif not out.is_contiguous():
+            raise ValueError("out must be contiguous")
+        op = _rows(out, "out", q.dtype, heads, rows, self.device)[3]
+        status = self.lib.q3cu_attention_prompt(self.ctx, cache.ref, batch.ref, rows, qp, _dtype(q), stride, heads, op,
+                                                self._stream(stream))
+        if status:
+            self._check(status, "q3cu_attention_prompt")
         return out
 
     # -- host-pointer drop-in (numpy arrays, synchronous) -----------------------
