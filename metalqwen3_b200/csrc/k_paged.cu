@@ -38,7 +38,7 @@ namespace q3 {
 constexpr int PD_WARPS = 4, PD_THREADS = (PD_WARPS + 1) * 32;
 constexpr int PD_NS = 3;                                     // stages
 constexpr uint32_t PD_SIDE = 16384, PD_STAGE = 2 * PD_SIDE;  // K or V of a stage; both
-constexpr int PD_SPARE = 16 * HD * 4;                        // queries (f32 cache), then the join of the warps
+constexpr int PD_SPARE = 12288;                              // queries (f32 cache, at most 8 KB), then the join of the warps
 constexpr size_t PD_SMEM = size_t(PD_NS) * PD_STAGE + PD_SPARE + 1024;
 constexpr float PD_LOG2 = ATT_SCALE * 1.44269504088896341f;  // scores to base-2 exponents
 constexpr int PD_PART = HD + 2;                              // floats of a row's partial result: 128, maximum, sum
@@ -70,10 +70,11 @@ struct PagedWalk {
 template <typename TC>
 __device__ __forceinline__ int tiles_of(int len) { return (len + pd_tile<TC>() - 1) / pd_tile<TC>(); }
 
-__device__ __forceinline__ int64_t warp_prefix(int64_t x) {                 // inclusive, over the lanes
+// Inclusive sum over the lanes; 32 sequences have at most 2^31 / 32 tiles each.
+__device__ __forceinline__ uint32_t warp_prefix(uint32_t x) {
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int64_t y = __shfl_up_sync(FULL, x, o);
+        const uint32_t y = __shfl_up_sync(FULL, x, o);
         if ((threadIdx.x & 31) >= o) x += y;
     }
     return x;
@@ -84,34 +85,35 @@ __device__ __forceinline__ PagedWalk walk_run(const PagedSeqs &b, const PagedKV 
                                               int64_t &u0, int64_t &u1, uint32_t *status) {
     PagedWalk w = {};
     const int lane = threadIdx.x & 31;
-    int64_t total = 0, end = 0;
+    int64_t total = 0;                                       // in tiles of one kv head
+    uint32_t end = 0;
     int len = 0;
     for (int s0 = 0; s0 < b.n_seqs; s0 += 32) {              // 32 sequences at a time
         len = s0 + lane < b.n_seqs ? paged_len(b, c, s0 + lane, status) : 0;
-        end = warp_prefix(int64_t(tiles_of<TC>(len)) * c.n_kv);
+        end = warp_prefix(uint32_t(tiles_of<TC>(len)));
         total += __shfl_sync(FULL, end, 31);
     }
-    cut = PagedCut(total, runs);
+    cut = PagedCut(total * c.n_kv, runs);
     u0 = cut.begin(run);
     u1 = cut.begin(run + 1);
     int64_t u = u0;
     for (int s0 = 0; s0 < b.n_seqs; s0 += 32) {
         if (b.n_seqs > 32) {                                 // otherwise the lanes still hold them
             len = s0 + lane < b.n_seqs ? paged_len(b, c, s0 + lane, nullptr) : 0;
-            end = warp_prefix(int64_t(tiles_of<TC>(len)) * c.n_kv);
+            end = warp_prefix(uint32_t(tiles_of<TC>(len)));
         }
-        const unsigned hit = __ballot_sync(FULL, u < end);
+        const unsigned hit = __ballot_sync(FULL, u < int64_t(end) * c.n_kv);
         if (hit) {
             const int l = __ffs(hit) - 1;
             w.s = s0 + l;
             w.len = __shfl_sync(FULL, len, l);
             w.tiles = tiles_of<TC>(w.len);
-            const int64_t at = u - (__shfl_sync(FULL, end, l) - int64_t(w.tiles) * c.n_kv);
+            const int64_t at = u - int64_t(__shfl_sync(FULL, end, l) - uint32_t(w.tiles)) * c.n_kv;
             w.head = int(quot(at, w.tiles));
             w.tile = int(at - int64_t(w.head) * w.tiles);
             return w;
         }
-        u -= __shfl_sync(FULL, end, 31);
+        u -= int64_t(__shfl_sync(FULL, end, 31)) * c.n_kv;
     }
     return w;
 }
@@ -149,7 +151,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
     uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(pd_dyn) + 1023) & ~uintptr_t(1023));
     float *spare = reinterpret_cast<float *>(ring + PD_NS * PD_STAGE);
     __shared__ __align__(8) uint64_t full[PD_NS], empty[PD_NS];
-    __shared__ float join_m[2][8], join_l[2][8];
+    __shared__ float join_m[3][2][8], join_l[3][2][8];
     __shared__ volatile int dead;                            // a wait gave up
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -176,9 +178,9 @@ paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
 
     if (warp == PD_WARPS) {
         // ---- fetch: lane = box (K or V, column block, rows of one page) ------------------
-        const int br = min(1 << c.page_shift, TILE), nb = TILE / br;
-        constexpr int CB = CF32 ? 4 : 2;                     // column blocks of 128 B
-        const int box = lane % nb, col = lane / nb % CB, side = lane / (nb * CB);
+        constexpr int TS = CF32 ? 5 : 6, CS = CF32 ? 2 : 1, CB = 1 << CS;     // log2 of TILE; column blocks of 128 B
+        const int bs = min(c.page_shift, TS), br = 1 << bs, ns = TS - bs;     // rows of a box; log2 of boxes of a tile
+        const int box = lane & ((1 << ns) - 1), col = (lane >> ns) & (CB - 1), side = lane >> (ns + CS);
         auto page_of = [&]() -> int {                        // n_pages reads as zeros
             const int t = w.tile * TILE + box * br;
             if (side > 1 || t >= w.len) return c.n_pages;
@@ -249,9 +251,11 @@ paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
             const uint32_t ka = ring_a + st * PD_STAGE, va = ka + PD_SIDE;
             const int left = w.len - (w.tile + i) * TILE - warp * KW;      // visible positions of this warp's KW
             // scores: rows g, g + 8; columns (positions) 8 n + 2 t4, + 1
-            float s[KW / 8][4];
+            float s[KW / 8][4], low[2][4];                   // low: of the low parts, so that no chain of products is long
 #pragma unroll
             for (int n = 0; n < KW / 8; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+#pragma unroll
+            for (int n = 0; n < 2; ++n) low[n][0] = low[n][1] = low[n][2] = low[n][3] = 0.0f;
             if constexpr (CF32) {
                 // k index t4 is dimension 32 d + 8 t4 + x, k index t4 + 4 is + 1 of it (x = 0, 2, then 4, 6): a
                 // permutation that query and key share, so both are read 16 bytes at a time without conflicts
@@ -278,8 +282,8 @@ paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
                                 split_tf32(qf[h][y], ah[h], al[h]);
                                 split_tf32(qf[h][y + 1], ah[2 + h], al[2 + h]);
                             }
-                            mma_tf32(s[0], al[0], al[1], al[2], al[3], bh[0], bh[1]);
-                            mma_tf32(s[0], ah[0], ah[1], ah[2], ah[3], bl[0], bl[1]);
+                            mma_tf32(low[0], al[0], al[1], al[2], al[3], bh[0], bh[1]);
+                            mma_tf32(low[1], ah[0], ah[1], ah[2], ah[3], bl[0], bl[1]);
                             mma_tf32(s[0], ah[0], ah[1], ah[2], ah[3], bh[0], bh[1]);
                         }
                     }
@@ -293,12 +297,21 @@ paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
 #pragma unroll
                     for (int n = 0; n < 2; ++n) {
                         if constexpr (Elem<T>::BYTES == 4)
-                            mma_bf16(s[n], ql[k][0], WIDE ? ql[k][2 * NH - 2] : 0u, ql[k][1], WIDE ? ql[k][2 * NH - 1] : 0u,
+                            mma_bf16(low[n], ql[k][0], WIDE ? ql[k][2 * NH - 2] : 0u, ql[k][1], WIDE ? ql[k][2 * NH - 1] : 0u,
                                      r[2 * n], r[2 * n + 1]);
                         mma_bf16(s[n], qh[k][0], WIDE ? qh[k][2 * NH - 2] : 0u, qh[k][1], WIDE ? qh[k][2 * NH - 1] : 0u,
                                  r[2 * n], r[2 * n + 1]);
                     }
                 }
+            }
+            if constexpr (CF32) {
+#pragma unroll
+                for (int x = 0; x < 4; ++x) s[0][x] += low[0][x] + low[1][x];
+            } else if constexpr (Elem<T>::BYTES == 4) {
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) s[n][x] += low[n][x];
             }
             // softmax over this warp's positions
             if (left < KW) {
@@ -398,39 +411,53 @@ paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
             if (lane == 0) mbar_arrive(&empty[st]);
         }
         if (!ok && lane == 0) dead = 1;
-        // join the four warps into warp 0, one after the other through shared memory
+        // join the four warps into warp 0 through shared memory
 #pragma unroll
         for (int h = 0; h < NH; ++h) {
             l[h] += __shfl_xor_sync(FULL, l[h], 1);
             l[h] += __shfl_xor_sync(FULL, l[h], 2);
         }
-        for (int src = 1; src < PD_WARPS; ++src) {
+        constexpr int AT_ONCE = WIDE ? 1 : 3;                // warps whose results fit the spare memory
+#pragma unroll
+        for (int src = 1; src < PD_WARPS; src += AT_ONCE) {
             named_sync(1, PD_WARPS * 32);
-            if (warp == src) {
+            if (warp >= src && warp < src + AT_ONCE) {
+                float *to = spare + (warp - src) * (16 * 2 * NH * 32);
 #pragma unroll
                 for (int j = 0; j < 16; ++j)
 #pragma unroll
-                    for (int x = 0; x < 2 * NH; ++x) spare[(j * 2 * NH + x) * 32 + lane] = o[j][x];
+                    for (int x = 0; x < 2 * NH; ++x) to[(j * 2 * NH + x) * 32 + lane] = o[j][x];
 #pragma unroll
                 for (int h = 0; h < NH; ++h)
-                    if (t4 == 0) join_m[h][g] = m[h], join_l[h][g] = l[h];
+                    if (t4 == 0) join_m[warp - src][h][g] = m[h], join_l[warp - src][h][g] = l[h];
             }
             named_sync(1, PD_WARPS * 32);
             if (warp == 0) {
-                float f0[NH], f1[NH];
+                float f0[NH], f1[AT_ONCE][NH];
 #pragma unroll
                 for (int h = 0; h < NH; ++h) {
-                    const float om = join_m[h][g], nm = fmaxf(m[h], om);
+                    float nm = m[h];
+#pragma unroll
+                    for (int i = 0; i < AT_ONCE; ++i) nm = fmaxf(nm, join_m[i][h][g]);
                     f0[h] = m[h] == nm ? 1.0f : ex2_approx_ftz((m[h] - nm) * PD_LOG2);
-                    f1[h] = om == nm ? 1.0f : ex2_approx_ftz((om - nm) * PD_LOG2);
+                    l[h] *= f0[h];
+#pragma unroll
+                    for (int i = 0; i < AT_ONCE; ++i) {
+                        const float om = join_m[i][h][g];
+                        f1[i][h] = om == nm ? 1.0f : ex2_approx_ftz((om - nm) * PD_LOG2);
+                        l[h] = fmaf(join_l[i][h][g], f1[i][h], l[h]);
+                    }
                     m[h] = nm;
-                    l[h] = l[h] * f0[h] + join_l[h][g] * f1[h];
                 }
 #pragma unroll
                 for (int j = 0; j < 16; ++j)
 #pragma unroll
-                    for (int x = 0; x < 2 * NH; ++x)
-                        o[j][x] = fmaf(o[j][x], f0[x >> 1], spare[(j * 2 * NH + x) * 32 + lane] * f1[x >> 1]);
+                    for (int x = 0; x < 2 * NH; ++x) {
+                        o[j][x] *= f0[x >> 1];
+#pragma unroll
+                        for (int i = 0; i < AT_ONCE; ++i)
+                            o[j][x] = fmaf(spare[((i * 16 + j) * 2 * NH + x) * 32 + lane], f1[i][x >> 1], o[j][x]);
+                    }
             }
         }
         ok = dead == 0;                                      // the same for every warp: the next barrier follows the read
@@ -486,6 +513,11 @@ __global__ void __launch_bounds__(PJ_THREADS) paged_join_kernel(const PagedKV c,
     const int64_t run_stride = int64_t(2) * group * PD_PART;
     const float *head = row + first * run_stride + (a != cut.begin(first) ? group * PD_PART : 0);
     auto at = [&](int i) { return i == 0 ? head : row + (first + i) * run_stride; };
+    // the first parts of this thread's half are on their way together with the maxima and sums
+    const int i0 = n * half_id / PJ_GROUPS, i1 = n * (half_id + 1) / PJ_GROUPS;
+    float v[8];
+#pragma unroll
+    for (int x = 0; x < 8; ++x) v[x] = i0 + x < i1 ? at(i0 + x)[d] : 0.0f;
     float m = -INFINITY;
     for (int i = threadIdx.x; i < n; i += PJ_THREADS) {
         weight[i] = at(i)[HD];
@@ -506,9 +538,11 @@ __global__ void __launch_bounds__(PJ_THREADS) paged_join_kernel(const PagedKV c,
     if (lane == 0) red[1][warp] = l;
     __syncthreads();
     float o = 0.0f;
-    const int i0 = n * half_id / PJ_GROUPS, i1 = n * (half_id + 1) / PJ_GROUPS;
+#pragma unroll
+    for (int x = 0; x < 8; ++x)
+        if (i0 + x < i1) o = fmaf(v[x], weight[i0 + x], o);
 #pragma unroll 8
-    for (int i = i0; i < i1; ++i) o = fmaf(at(i)[d], weight[i], o);
+    for (int i = i0 + 8; i < i1; ++i) o = fmaf(at(i)[d], weight[i], o);
     sum[half_id][d] = o;
     __syncthreads();
     if (half_id) return;
