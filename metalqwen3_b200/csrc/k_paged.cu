@@ -21,11 +21,11 @@
 //
 // The products run on mma.sync with the group's query heads as the 16 rows of
 // the tile: at one to sixteen query rows the tensor cores are mostly idle by
-// either path, and the operands come straight from registers.  Nothing is
-// rounded below 16 bits of mantissa on the way: an f32 query against a bf16
-// cache is two bf16 parts (the keys are exact), a probability is two bf16 parts,
-// and an f32 cache is multiplied as tf32 parts, high x high + high x low +
-// low x high, whose remainder is 2^-21 of the product.  Sums are binary32.
+// either path, and the operands come straight from registers.  They lose nothing
+// that an f32 result would show: an f32 query against a bf16 cache is three bf16
+// parts (the keys are exact), and so is a probability, two where the result is
+// bf16; an f32 cache is multiplied as tf32 parts, high x high + high x low +
+// low x high, whose remainder is 2^-22 of the product.  Sums are binary32.
 //
 // Positions at and beyond the length score -inf, and their values are masked to
 // zero in registers: unused page space may hold anything.
@@ -217,11 +217,24 @@ paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
     for (int64_t u = u0; u < u1 && ok;) {
         const int run = int(min(int64_t(w.tiles - w.tile), u1 - u));       // tiles of this (sequence, head) here
         const typename Elem<T>::type *qs = q + w.s * q_stride + int64_t(w.head) * group * HD;
-        uint32_t qh[CF32 ? 1 : 8][2 * NH], ql[CF32 || Elem<T>::BYTES == 2 ? 1 : 8][2 * NH];
+        constexpr bool PARTS3 = !CF32 && Elem<T>::BYTES == 4;                // f32 queries, bf16 cache
+        uint32_t qf[CF32 || PARTS3 ? 1 : 8][2 * NH];         // bf16 queries, bf16 cache: operands in registers
         if constexpr (CF32) {                                // the group's rows in shared memory, zeros below
             for (int i = threadIdx.x; i < 8 * NH * (HD / 4); i += PD_WARPS * 32)
                 *reinterpret_cast<float4 *>(spare + 4 * i) =
                     i / (HD / 4) < group ? load_quad(qs + 4 * i) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            named_sync(1, PD_WARPS * 32);
+        } else if constexpr (PARTS3) {
+            // three bf16 parts of the group's rows in shared memory, zeros below; 16-byte chunk x of row r at x ^ (r % 8)
+            for (int i = threadIdx.x; i < 8 * NH * (HD / 2); i += PD_WARPS * 32) {
+                const int row = i / (HD / 2), col = 2 * (i % (HD / 2));
+                const float2 v = row < group ? *reinterpret_cast<const float2 *>(qs + row * HD + col) : make_float2(0.0f, 0.0f);
+                uint32_t part[3];
+                split_bf16(v.x, v.y, part);
+#pragma unroll
+                for (int x = 0; x < 3; ++x)
+                    reinterpret_cast<uint32_t *>(spare)[((x * 8 * NH + row) * HD + (col ^ ((row & 7) << 3))) / 2] = part[x];
+            }
             named_sync(1, PD_WARPS * 32);
         } else {
 #pragma unroll
@@ -229,12 +242,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
 #pragma unroll
                 for (int x = 0; x < 2 * NH; ++x) {           // x: columns + 8 (bit 0), row + 8 (bit 1)
                     const int row = g + 8 * (x >> 1), at = row * HD + 16 * k + 2 * t4 + 8 * (x & 1);
-                    if constexpr (Elem<T>::BYTES == 2) {
-                        qh[k][x] = row < group ? *reinterpret_cast<const uint32_t *>(qs + at) : 0u;
-                    } else {
-                        const float2 v = row < group ? *reinterpret_cast<const float2 *>(qs + at) : make_float2(0.0f, 0.0f);
-                        split_bf16(v.x, v.y, qh[k][x], ql[k][x]);
-                    }
+                    qf[k][x] = row < group ? *reinterpret_cast<const uint32_t *>(qs + at) : 0u;
                 }
         }
         float o[16][4];
@@ -251,11 +259,9 @@ paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
             const uint32_t ka = ring_a + st * PD_STAGE, va = ka + PD_SIDE;
             const int left = w.len - (w.tile + i) * TILE - warp * KW;      // visible positions of this warp's KW
             // scores: rows g, g + 8; columns (positions) 8 n + 2 t4, + 1
-            float s[KW / 8][4], low[2][4];                   // low: of the low parts, so that no chain of products is long
+            float s[KW / 8][4];
 #pragma unroll
             for (int n = 0; n < KW / 8; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
-#pragma unroll
-            for (int n = 0; n < 2; ++n) low[n][0] = low[n][1] = low[n][2] = low[n][3] = 0.0f;
             if constexpr (CF32) {
                 // k index t4 is dimension 32 d + 8 t4 + x, k index t4 + 4 is + 1 of it (x = 0, 2, then 4, 6): a
                 // permutation that query and key share, so both are read 16 bytes at a time without conflicts
@@ -272,6 +278,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
                             const float4 v = lds4(qa + h * 8 * (HD * 4) + (32 * d + 8 * t4 + 4 * x) * 4);
                             qf[h][0] = v.x, qf[h][1] = v.y, qf[h][2] = v.z, qf[h][3] = v.w;
                         }
+                        float part[4] = {}, low[4] = {};
 #pragma unroll
                         for (int y = 0; y < 4; y += 2) {
                             uint32_t bh[2], bl[2], ah[4] = {0, 0, 0, 0}, al[4] = {0, 0, 0, 0};
@@ -282,36 +289,68 @@ paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
                                 split_tf32(qf[h][y], ah[h], al[h]);
                                 split_tf32(qf[h][y + 1], ah[2 + h], al[2 + h]);
                             }
-                            mma_tf32(low[0], al[0], al[1], al[2], al[3], bh[0], bh[1]);
-                            mma_tf32(low[1], ah[0], ah[1], ah[2], ah[3], bl[0], bl[1]);
-                            mma_tf32(s[0], ah[0], ah[1], ah[2], ah[3], bh[0], bh[1]);
+                            mma_tf32(low, al[0], al[1], al[2], al[3], bh[0], bh[1]);
+                            mma_tf32(low, ah[0], ah[1], ah[2], ah[3], bl[0], bl[1]);
+                            mma_tf32(part, ah[0], ah[1], ah[2], ah[3], bh[0], bh[1]);
                         }
+                        add_to(part, low);
+                        add_to(s[0], part);
                     }
             } else {
                 const int key = warp * KW + (lane >> 4) * 8 + (lane & 7);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
+                auto keys = [&](int k, uint32_t (&r)[4]) {   // dimensions 16 k ..; positions 0-7 in r[0], r[1], 8-15 in r[2], r[3]
                     const int chunk = 2 * k + ((lane >> 3) & 1);
-                    uint32_t r[4];
                     ldsm4(ka + (chunk >> 3) * (PD_SIDE / 2) + key * 128 + (((chunk & 7) ^ (key & 7)) << 4), r);
+                };
+                if constexpr (PARTS3) {
+                    // a lane's address in the parts: WIDE rows 0-15 of chunks 2 k, 2 k + 1, otherwise rows 0-7 of four chunks
+                    const int row = WIDE ? lane & 15 : lane & 7, first = WIDE ? lane >> 4 : lane >> 3;
+                    const uint32_t qa = smem_addr(spare) + row * (HD * 2);
 #pragma unroll
-                    for (int n = 0; n < 2; ++n) {
-                        if constexpr (Elem<T>::BYTES == 4)
-                            mma_bf16(low[n], ql[k][0], WIDE ? ql[k][2 * NH - 2] : 0u, ql[k][1], WIDE ? ql[k][2 * NH - 1] : 0u,
+                    for (int k = 0; k < 8; k += 2) {
+                        uint32_t r[2][4], a[3][2][4];
+                        keys(k, r[0]);
+                        keys(k + 1, r[1]);
+#pragma unroll
+                        for (int x = 0; x < 3; ++x) {
+                            const uint32_t pa = qa + x * 8 * NH * (HD * 2);
+                            if constexpr (WIDE) {            // rows 0-7, 8-15 of chunk 2 k, then of 2 k + 1
+                                ldsm4(pa + (((2 * k + first) ^ (row & 7)) << 4), a[x][0]);
+                                ldsm4(pa + (((2 * k + 2 + first) ^ (row & 7)) << 4), a[x][1]);
+                            } else {
+                                uint32_t v[4];
+                                ldsm4(pa + (((2 * k + first) ^ row) << 4), v);
+#pragma unroll
+                                for (int y = 0; y < 2; ++y)
+                                    a[x][y][0] = v[2 * y], a[x][y][1] = 0u, a[x][y][2] = v[2 * y + 1], a[x][y][3] = 0u;
+                            }
+                        }
+                        float part[2][4] = {}, low[2][4] = {};
+#pragma unroll
+                        for (int y = 0; y < 2; ++y)
+#pragma unroll
+                            for (int n = 0; n < 2; ++n) {
+                                mma_bf16(low[n], a[2][y][0], a[2][y][1], a[2][y][2], a[2][y][3], r[y][2 * n], r[y][2 * n + 1]);
+                                mma_bf16(low[n], a[1][y][0], a[1][y][1], a[1][y][2], a[1][y][3], r[y][2 * n], r[y][2 * n + 1]);
+                                mma_bf16(part[n], a[0][y][0], a[0][y][1], a[0][y][2], a[0][y][3], r[y][2 * n], r[y][2 * n + 1]);
+                            }
+#pragma unroll
+                        for (int n = 0; n < 2; ++n) {
+                            add_to(part[n], low[n]);
+                            add_to(s[n], part[n]);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        uint32_t r[4];
+                        keys(k, r);
+#pragma unroll
+                        for (int n = 0; n < 2; ++n)
+                            mma_bf16(s[n], qf[k][0], WIDE ? qf[k][2 * NH - 2] : 0u, qf[k][1], WIDE ? qf[k][2 * NH - 1] : 0u,
                                      r[2 * n], r[2 * n + 1]);
-                        mma_bf16(s[n], qh[k][0], WIDE ? qh[k][2 * NH - 2] : 0u, qh[k][1], WIDE ? qh[k][2 * NH - 1] : 0u,
-                                 r[2 * n], r[2 * n + 1]);
                     }
                 }
-            }
-            if constexpr (CF32) {
-#pragma unroll
-                for (int x = 0; x < 4; ++x) s[0][x] += low[0][x] + low[1][x];
-            } else if constexpr (Elem<T>::BYTES == 4) {
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) s[n][x] += low[n][x];
             }
             // softmax over this warp's positions
             if (left < KW) {
@@ -376,17 +415,25 @@ paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
                         uint32_t bh[2], bl[2];
                         split_tf32(live0 ? a0[x] : 0.0f, bh[0], bl[0]);
                         split_tf32(live1 ? a1[x] : 0.0f, bh[1], bl[1]);
-                        mma_tf32(o[4 * d + x], pl[0], pl[1], pl[2], pl[3], bh[0], bh[1]);
-                        mma_tf32(o[4 * d + x], ph[0], ph[1], ph[2], ph[3], bl[0], bl[1]);
-                        mma_tf32(o[4 * d + x], ph[0], ph[1], ph[2], ph[3], bh[0], bh[1]);
+                        float part[4] = {};
+                        mma_tf32(part, pl[0], pl[1], pl[2], pl[3], bh[0], bh[1]);
+                        mma_tf32(part, ph[0], ph[1], ph[2], ph[3], bl[0], bl[1]);
+                        mma_tf32(part, ph[0], ph[1], ph[2], ph[3], bh[0], bh[1]);
+                        add_to(o[4 * d + x], part);
                     }
                 }
             } else {
-                uint32_t ph[4] = {0, 0, 0, 0}, pl[4] = {0, 0, 0, 0};
+                constexpr int PARTS = Elem<T>::BYTES == 4 ? 3 : 2;
+                uint32_t p[PARTS][4] = {};
 #pragma unroll
                 for (int n = 0; n < 2; ++n)
 #pragma unroll
-                    for (int h = 0; h < NH; ++h) split_bf16(s[n][2 * h], s[n][2 * h + 1], ph[2 * n + h], pl[2 * n + h]);
+                    for (int h = 0; h < NH; ++h) {
+                        uint32_t part[PARTS];
+                        split_bf16(s[n][2 * h], s[n][2 * h + 1], part);
+#pragma unroll
+                        for (int x = 0; x < PARTS; ++x) p[x][2 * n + h] = part[x];
+                    }
                 // keep[n]: which of the positions 8 n + 2 t4, + 1 exist
                 uint32_t keep[2];
 #pragma unroll
@@ -402,8 +449,11 @@ paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
                     for (int x = 0; x < 4; ++x) r[x] &= keep[x & 1];
 #pragma unroll
                     for (int n = 0; n < 2; ++n) {
-                        mma_bf16(o[2 * d + n], pl[0], pl[1], pl[2], pl[3], r[2 * n], r[2 * n + 1]);
-                        mma_bf16(o[2 * d + n], ph[0], ph[1], ph[2], ph[3], r[2 * n], r[2 * n + 1]);
+                        float part[4] = {};
+#pragma unroll
+                        for (int x = PARTS - 1; x >= 0; --x)
+                            mma_bf16(part, p[x][0], p[x][1], p[x][2], p[x][3], r[2 * n], r[2 * n + 1]);
+                        add_to(o[2 * d + n], part);
                     }
                 }
             }

@@ -136,12 +136,16 @@ prompt_f32_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant
                     split_tf32(v.y, bh[1], bl[1]);
                     split_tf32(v.z, bh[2], bl[2]);
                     split_tf32(v.w, bh[3], bl[3]);
+                    float part[4] = {};
 #pragma unroll
                     for (int y = 0; y < 2; ++y) {
-                        mma_tf32(s[n], al[y][0], al[y][1], al[y][2], al[y][3], bh[2 * y], bh[2 * y + 1]);
-                        mma_tf32(s[n], ah[y][0], ah[y][1], ah[y][2], ah[y][3], bl[2 * y], bl[2 * y + 1]);
-                        mma_tf32(s[n], ah[y][0], ah[y][1], ah[y][2], ah[y][3], bh[2 * y], bh[2 * y + 1]);
+                        mma_tf32(part, al[y][0], al[y][1], al[y][2], al[y][3], bh[2 * y], bh[2 * y + 1]);
+                        mma_tf32(part, ah[y][0], ah[y][1], ah[y][2], ah[y][3], bl[2 * y], bl[2 * y + 1]);
                     }
+#pragma unroll
+                    for (int y = 0; y < 2; ++y)
+                        mma_tf32(part, ah[y][0], ah[y][1], ah[y][2], ah[y][3], bh[2 * y], bh[2 * y + 1]);
+                    add_to(s[n], part);
                 }
             }
         if (base + PF_KEYS > sure) {
@@ -186,17 +190,20 @@ prompt_f32_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant
         // k index t4 is position 8 n + 2 t4, t4 + 4 the next one: the columns this thread's scores have; column i of
         // product (d, x) is dimension 32 d + 4 i + x
         const bool tail = base + PF_KEYS > len;
+        uint32_t ph[4][4], pl[4][4];
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-            uint32_t ph[4], pl[4];
+        for (int n = 0; n < 4; ++n)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                split_tf32(s[n][2 * h], ph[h], pl[h]);
-                split_tf32(s[n][2 * h + 1], ph[2 + h], pl[2 + h]);
+                split_tf32(s[n][2 * h], ph[n][h], pl[n][h]);
+                split_tf32(s[n][2 * h + 1], ph[n][2 + h], pl[n][2 + h]);
             }
-            const int k0 = 8 * n + 2 * t4;
 #pragma unroll
-            for (int d = 0; d < 4; ++d) {
+        for (int d = 0; d < 4; ++d) {
+            float part[4][4] = {};
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const int k0 = 8 * n + 2 * t4;
                 const uint32_t blk = va + d * (PF_SIDE / 4) + k0 * 128;
                 float4 v0 = lds4(blk + ((g ^ (2 * t4)) << 4)), v1 = lds4(blk + 128 + ((g ^ (2 * t4 + 1)) << 4));
                 if (tail) {
@@ -209,11 +216,13 @@ prompt_f32_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant
                     uint32_t bh[2], bl[2];
                     split_tf32(a0[x], bh[0], bl[0]);
                     split_tf32(a1[x], bh[1], bl[1]);
-                    mma_tf32(o[4 * d + x], pl[0], pl[1], pl[2], pl[3], bh[0], bh[1]);
-                    mma_tf32(o[4 * d + x], ph[0], ph[1], ph[2], ph[3], bl[0], bl[1]);
-                    mma_tf32(o[4 * d + x], ph[0], ph[1], ph[2], ph[3], bh[0], bh[1]);
+                    mma_tf32(part[x], pl[n][0], pl[n][1], pl[n][2], pl[n][3], bh[0], bh[1]);
+                    mma_tf32(part[x], ph[n][0], ph[n][1], ph[n][2], ph[n][3], bl[0], bl[1]);
+                    mma_tf32(part[x], ph[n][0], ph[n][1], ph[n][2], ph[n][3], bh[0], bh[1]);
                 }
             }
+#pragma unroll
+            for (int x = 0; x < 4; ++x) add_to(o[4 * d + x], part[x]);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[st]);
