@@ -79,6 +79,16 @@ public:
                      float *out_f32, int8_t *out_q, float *out_s, q3cu_stream stream);
     void attention(const float *q, const float *key_cache, const float *value_cache, int pos, int n_heads,
                    int kv_dim, int kv_mul, float *att, int att_stride, float *probs, float *xb, q3cu_stream stream);
+    // the paged key-value cache (q3cu_kv_append, q3cu_attention_paged, q3cu_attention_prompt)
+    void kvAppend(const q3cu_kv_cache &cache, const q3cu_kv_batch &batch, int64_t rows, const void *q, const void *k,
+                  const void *v, q3cu_dtype dt, int64_t q_stride, int64_t kv_stride, int n_heads, const float *q_norm,
+                  const float *k_norm, void *q_out, q3cu_dtype q_dt, q3cu_stream stream, float theta = 1e6f,
+                  float eps = 1e-6f);
+    size_t attentionPagedWorkspace(int n_heads, int n_kv);
+    void attentionPaged(const q3cu_kv_cache &cache, const q3cu_kv_batch &batch, const void *q, q3cu_dtype dt,
+                        int64_t q_stride, int n_heads, void *work, size_t work_bytes, void *out, q3cu_stream stream);
+    void attentionPrompt(const q3cu_kv_cache &cache, const q3cu_kv_batch &batch, int64_t rows, const void *q,
+                         q3cu_dtype dt, int64_t q_stride, int n_heads, void *out, q3cu_stream stream);
     // synchronises `stream` and throws if a kernel flagged a device-side error
     void checkDeviceStatus(q3cu_stream stream);
 

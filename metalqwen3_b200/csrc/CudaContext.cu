@@ -101,6 +101,29 @@ void CudaContext::attention(const float *q, const float *key_cache, const float 
                          stream),
           "attention");
 }
+void CudaContext::kvAppend(const q3cu_kv_cache &cache, const q3cu_kv_batch &batch, int64_t rows, const void *q,
+                           const void *k, const void *v, q3cu_dtype dt, int64_t q_stride, int64_t kv_stride, int n_heads,
+                           const float *q_norm, const float *k_norm, void *q_out, q3cu_dtype q_dt, q3cu_stream stream,
+                           float theta, float eps) {
+    check(q3cu_kv_append(ctx_, &cache, &batch, rows, q, k, v, dt, q_stride, kv_stride, n_heads, q_norm, k_norm, theta, eps,
+                         q_out, q_dt, stream),
+          "kvAppend");
+}
+size_t CudaContext::attentionPagedWorkspace(int n_heads, int n_kv) {
+    size_t bytes = 0;
+    check(q3cu_attention_paged_workspace(ctx_, n_heads, n_kv, &bytes), "attentionPagedWorkspace");
+    return bytes;
+}
+void CudaContext::attentionPaged(const q3cu_kv_cache &cache, const q3cu_kv_batch &batch, const void *q, q3cu_dtype dt,
+                                 int64_t q_stride, int n_heads, void *work, size_t work_bytes, void *out,
+                                 q3cu_stream stream) {
+    check(q3cu_attention_paged(ctx_, &cache, &batch, q, dt, q_stride, n_heads, work, work_bytes, out, stream),
+          "attentionPaged");
+}
+void CudaContext::attentionPrompt(const q3cu_kv_cache &cache, const q3cu_kv_batch &batch, int64_t rows, const void *q,
+                                  q3cu_dtype dt, int64_t q_stride, int n_heads, void *out, q3cu_stream stream) {
+    check(q3cu_attention_prompt(ctx_, &cache, &batch, rows, q, dt, q_stride, n_heads, out, stream), "attentionPrompt");
+}
 void CudaContext::checkDeviceStatus(q3cu_stream stream) {
     check(q3cu_device_status(ctx_, stream, nullptr), "checkDeviceStatus");
 }

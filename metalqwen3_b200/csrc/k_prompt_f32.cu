@@ -136,15 +136,14 @@ prompt_f32_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant
                     split_tf32(v.y, bh[1], bl[1]);
                     split_tf32(v.z, bh[2], bl[2]);
                     split_tf32(v.w, bh[3], bl[3]);
-                    float part[4] = {};
+                    float part[4] = {}, low[4] = {};
 #pragma unroll
                     for (int y = 0; y < 2; ++y) {
-                        mma_tf32(part, al[y][0], al[y][1], al[y][2], al[y][3], bh[2 * y], bh[2 * y + 1]);
-                        mma_tf32(part, ah[y][0], ah[y][1], ah[y][2], ah[y][3], bl[2 * y], bl[2 * y + 1]);
-                    }
-#pragma unroll
-                    for (int y = 0; y < 2; ++y)
+                        mma_tf32(low, al[y][0], al[y][1], al[y][2], al[y][3], bh[2 * y], bh[2 * y + 1]);
                         mma_tf32(part, ah[y][0], ah[y][1], ah[y][2], ah[y][3], bh[2 * y], bh[2 * y + 1]);
+                        mma_tf32(low, ah[y][0], ah[y][1], ah[y][2], ah[y][3], bl[2 * y], bl[2 * y + 1]);
+                    }
+                    add_to(part, low);
                     add_to(s[n], part);
                 }
             }
@@ -200,7 +199,7 @@ prompt_f32_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant
             }
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
-            float part[4][4] = {};
+            float part[4][4] = {}, low[4][4] = {};
 #pragma unroll
             for (int n = 0; n < 4; ++n) {
                 const int k0 = 8 * n + 2 * t4;
@@ -216,13 +215,13 @@ prompt_f32_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant
                     uint32_t bh[2], bl[2];
                     split_tf32(a0[x], bh[0], bl[0]);
                     split_tf32(a1[x], bh[1], bl[1]);
-                    mma_tf32(part[x], pl[n][0], pl[n][1], pl[n][2], pl[n][3], bh[0], bh[1]);
-                    mma_tf32(part[x], ph[n][0], ph[n][1], ph[n][2], ph[n][3], bl[0], bl[1]);
+                    mma_tf32(low[x], pl[n][0], pl[n][1], pl[n][2], pl[n][3], bh[0], bh[1]);
+                    mma_tf32(low[x], ph[n][0], ph[n][1], ph[n][2], ph[n][3], bl[0], bl[1]);
                     mma_tf32(part[x], ph[n][0], ph[n][1], ph[n][2], ph[n][3], bh[0], bh[1]);
                 }
             }
 #pragma unroll
-            for (int x = 0; x < 4; ++x) add_to(o[4 * d + x], part[x]);
+            for (int x = 0; x < 4; ++x) add_to(part[x], low[x]), add_to(o[4 * d + x], part[x]);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[st]);
