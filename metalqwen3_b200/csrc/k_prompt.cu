@@ -317,7 +317,9 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                         for (int t = 0; t < 2; ++t) {
                             if (j < it.nt[t]) {
                                 if (j == 0 && outs[t] && !(ok = mbar_wait(&o_empty[t], (outs[t] - 1) & 1u, status))) break;
-                                for (int half = 0; half < 2 && ok; ++half) {
+#pragma unroll
+                                for (int half = 0; half < 2; ++half) {
+                                    if (!ok) break;
                                     ok = mbar_wait(&p_full[t][half], steps[t] & 1u, status);
                                     tc_fence_after();
                                     if (ok) values(t, v.st, half, j > 0 || half > 0);
