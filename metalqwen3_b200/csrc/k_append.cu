@@ -101,8 +101,8 @@ kv_append_kernel(const PagedKV c, const PagedSeqs b, int rows, const typename El
     if (r >= rows) return;
     // the row's batches: of query heads, of key heads, of value heads; this warp's are first .. last - 1
     const int qn = (n_heads + APPEND_HEADS - 1) / APPEND_HEADS, kn = (c.n_kv + APPEND_HEADS - 1) / APPEND_HEADS;
-    const int first = (qn + 2 * kn) * int(blockIdx.y) / int(gridDim.y);
-    const int last = (qn + 2 * kn) * int(blockIdx.y + 1) / int(gridDim.y);
+    const int first = int(int64_t(qn + 2 * kn) * blockIdx.y / gridDim.y);
+    const int last = int(int64_t(qn + 2 * kn) * (blockIdx.y + 1) / gridDim.y);
     const E *qr = q + r * q_stride, *kr = k + r * kv_stride, *vr = v + r * kv_stride;
     constexpr int LINES = APPEND_HEADS * HD * int(sizeof(E)) / 128;        // 128-byte lines of a batch
     for (int i = lane + LINES * first; i < LINES * last; i += 32) {
@@ -161,7 +161,8 @@ cudaError_t launch_kv_append(const PagedKV &c, q3cu_dtype cache_dt, const PagedS
                              int n_heads, const float *q_norm, const float *k_norm, const TurnFreq &freq, float eps,
                              void *q_out, q3cu_dtype q_dt, uint32_t *status, cudaStream_t stream, int sms) {
     // A row is split over warps only while the rows alone are fewer than 32 warps per SM.
-    const int64_t batches = (n_heads + APPEND_HEADS - 1) / APPEND_HEADS + (c.n_kv + APPEND_HEADS - 1) / APPEND_HEADS * 2;
+    const int64_t all = (n_heads + APPEND_HEADS - 1) / APPEND_HEADS + (c.n_kv + APPEND_HEADS - 1) / APPEND_HEADS * 2;
+    const int64_t batches = all < 65535 ? all : 65535;       // a grid's height
     const int64_t parts = rows >= 32 * sms ? 1 : (32 * int64_t(sms) + rows - 1) / rows;
     const dim3 grid(unsigned((rows + APPEND_WARPS - 1) / APPEND_WARPS), unsigned(parts < batches ? parts : batches));
     auto go = [&](auto kernel, auto *typed) {

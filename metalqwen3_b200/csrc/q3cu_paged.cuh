@@ -219,7 +219,8 @@ struct PromptOrder {
     const FastDiv &per_block;
     int total_rows, tile_keys;
     uint32_t *status;
-    int hi, above;           // blocks of at least hi tiles: `above`, no more than the latest index
+    int hi, above;           // sorted: blocks of at least hi tiles are `above`, no more than the latest index
+    int from, passed;        // otherwise: the 32 sequences of the latest index, and the blocks before them
 
     __device__ __forceinline__ PromptOrder(const PagedSeqs &b_, const PagedKV &c_, int total_rows_, const FastDiv &per_block_,
                                            int tile_keys_, uint32_t *status_)
@@ -229,7 +230,7 @@ struct PromptOrder {
         q[0] = prompt_seq(b, c, total_rows, per_block, sorted ? lane : b.n_seqs, status);
         q[1] = prompt_seq(b, c, total_rows, per_block, sorted ? lane + 32 : b.n_seqs, status);
         hi = (max(__reduce_max_sync(FULL, q[0].len), __reduce_max_sync(FULL, q[1].len)) + tile_keys - 1) / tile_keys + 1;
-        above = 0;
+        above = from = passed = 0;
     }
     __device__ __forceinline__ int at_least(int x, int tiles) const {
         return q[x].at_least(tiles ? (tiles - 1) * tile_keys + 1 : 0, per_block);
@@ -252,16 +253,16 @@ struct PromptOrder {
         int left = int(uint32_t(index) / uint32_t(c.n_kv));
         const int lane = threadIdx.x & 31;
         if (b.n_seqs > PROMPT_SORTED) {
-            for (int s0 = 0; s0 < b.n_seqs; s0 += 32) {
-                const PromptSeq p = prompt_seq(b, c, total_rows, per_block, s0 + lane, status);
-                const int before = lanes_before(p.blocks);
+            for (; from < b.n_seqs; from += 32) {
+                const PromptSeq p = prompt_seq(b, c, total_rows, per_block, from + lane, status);
+                const int before = passed + lanes_before(p.blocks);
                 const unsigned hit = __ballot_sync(FULL, left >= before && left < before + p.blocks);
                 if (hit) {
                     const int l = __ffs(hit) - 1;
-                    take(it, p, s0 + l, l, (p.blocks - 1 - (left - before)) * per_block.d);
+                    take(it, p, from + l, l, (p.blocks - 1 - (left - before)) * per_block.d);
                     return it;
                 }
-                left -= __reduce_add_sync(FULL, p.blocks);
+                passed += __reduce_add_sync(FULL, p.blocks);
             }
             return it;
         }

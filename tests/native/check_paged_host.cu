@@ -1,7 +1,7 @@
 // Host checks of the paged-cache operators, no GPU: the index arithmetic the kernels share (every table entry and
 // cache row it reaches stays inside its array, whatever the lengths, offsets and page ids say) and the entry points'
 // refusals (each returns before its first CUDA call).  Includes the API's source for a context without a device.
-#include <cassert>
+#include <algorithm>
 #include <climits>
 #include <cstdlib>
 #include <vector>
@@ -62,6 +62,43 @@ static void indices() {
     }
     const q3::PagedKV big{nullptr, nullptr, int64_t(1) << 36, INT_MAX, 8, 8};
     EXPECT(q3::paged_at(big, INT_MAX - 1, 7, 255) == (int64_t(1) << 36) * (INT_MAX - 1) + (7 * 256 + 255) * 128);
+}
+
+// The blocks of prompt rows: divisions by multiplication, and the count of blocks that see a number of keys.
+static void blocks() {
+    for (int d = 1; d <= 256; ++d) {
+        const q3::FastDiv div(d);
+        for (int i = 0; i < 2000; ++i) {
+            const int q = int(rnd() * 128u % (INT_MAX / d)), n = q * d;
+            for (int x : {i, n, n + d - 1, n - 1, INT_MAX - i}) EXPECT(x < 0 || div(x) == x / d);
+        }
+    }
+    for (int trial = 0; trial < 20000; ++trial) {
+        const int32_t off[2] = {int32_t(rnd() % 50) - 3, int32_t(rnd() % 700) - 3}, pages = 0;
+        const int32_t len = rnd() % 8 ? int32_t(rnd() % 900) : wild();
+        const q3::PagedKV c{nullptr, nullptr, 0, 1, 1, 4};
+        const q3::PagedSeqs b{off, &len, &pages, 1, int(rnd() % 60)};
+        const int total = rnd() % 600;
+        const q3::FastDiv per(1 + rnd() % 64);
+        const q3::PromptSeq q = q3::prompt_seq(b, c, total, per, 0, nullptr);
+        if (off[0] < 0 || off[1] <= off[0] || total <= off[0]) {
+            EXPECT(q.blocks == 0 && q.rows == 0);
+            continue;
+        }
+        const int rows = std::min(off[1], total) - off[0];
+        EXPECT(q.rows == rows && q.base == off[0] && q.blocks == (rows + per.d - 1) / per.d);
+        EXPECT(q.len >= 0 && q.len <= 16 * b.max_pages && (len < 0 || q.pos0 == len - rows));
+        const q3::PromptItem item{0, 0, 0, q.rows, q.len, q.base, q.pos0};
+        for (int i = 0; i < rows; ++i) {
+            const int64_t pos = int64_t(len < 0 ? 0 : len) - rows + i;
+            EXPECT(item.seen(i) == int(std::max<int64_t>(0, std::min<int64_t>(q.len, pos + 1))));
+        }
+        for (int keys : {0, 1, 16, 17, 128, 129, q.len, q.len + 1, 700}) {
+            int n = 0;
+            for (int i = 0; i < q.blocks; ++i) n += item.seen(std::min((i + 1) * per.d, rows) - 1) >= keys;
+            EXPECT(q.at_least(keys, per) == n);
+        }
+    }
 }
 
 static void refusals() {
@@ -169,6 +206,7 @@ static void refusals() {
 
 int main() {
     indices();
+    blocks();
     refusals();
     std::printf("ok\n");
     return 0;

@@ -177,6 +177,25 @@ def test_append(q3, io, cache_t, out_t, heads, n_kv, page, rows, lens):
         assert torch.equal(now[~touched], was[~touched])
 
 
+def test_append_many_sequences(q3):
+    """300 sequences of 0 to 3 rows: each row finds its own."""
+    g = np.random.default_rng(5)
+    rows = [int(r) for r in g.integers(0, 4, 300)]
+    lens = [r + int(x) for r, x in zip(rows, g.integers(0, 200, 300))]
+    p = Paged(lens, 2, 16, F32, seed=9, fill=0.0)
+    off = offsets(rows)
+    q, k, v = (queries(off[-1], 2, F32, s) for s in (10, 11, 12))
+    out = q3.kv_append(*p.handles(off), q, k, v)
+    for s in range(300):
+        if rows[s]:
+            mine, pos = slice(off[s], off[s + 1]), torch.arange(lens[s] - rows[s], lens[s], device="cuda")
+            page_id, slot = p.where(s, pos)
+            check_rotated(out[mine], q[mine], None, pos, F32)
+            check_rotated(p.k[page_id, :, slot], k[mine], None, pos, F32)
+            assert torch.equal(p.v[page_id, :, slot], v[mine])
+    assert q3.device_status() == 0
+
+
 def test_append_far_positions_no_norm_no_queries_in_place(q3):
     """Positions past 2,000,000 (pages before the row's are never read), the rotation alone, q_out = q, and keys and
     values alone."""
@@ -350,6 +369,29 @@ def test_attention_prompt(q3, dtype, heads, n_kv, page, rows, lens):
         if r:
             check_attention(out[first:first + r], q[first:first + r], k, v, seen, dtype, H if dtype == BF16 else 0.0)
         first += r
+    assert q3.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n_seqs", [33, 50, 64, 65, 100])
+def test_attention_prompt_many_sequences(q3, dtype, n_seqs):
+    """More sequences than a warp has lanes, and than it sorts: rows of 0 to 300, prefixes of 0 to 400."""
+    g = np.random.default_rng(n_seqs)
+    rows = [int(r) if r < 40 or i % 9 == 0 else int(r) % 40 for i, r in enumerate(g.integers(0, 300, n_seqs))]
+    lens = [r + int(x) for r, x in zip(rows, g.integers(0, 400, n_seqs) * g.integers(0, 2, n_seqs))]
+    p = Paged(lens, 2, 16, dtype, seed=47).fill(48)
+    off = offsets(rows)
+    q = queries(off[-1], 4, dtype, 49)
+    out = q3.attention_prompt(*p.handles(off), q)
+    for s in range(n_seqs):
+        if rows[s]:
+            k, v = p.rows(s)
+            mine = slice(off[s], off[s + 1])
+            check_attention(out[mine], q[mine], k, v, range(lens[s] - rows[s] + 1, lens[s] + 1), dtype,
+                            H if dtype == BF16 else 0.0)
+    one = q3.attention_paged(*p.handles(), queries(n_seqs, 4, dtype, 50))
+    for s in range(n_seqs):
+        check_attention(one[s:s + 1], queries(n_seqs, 4, dtype, 50)[s:s + 1], *p.rows(s), [lens[s]], dtype)
     assert q3.device_status() == 0
 
 
