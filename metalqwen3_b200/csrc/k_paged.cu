@@ -15,17 +15,18 @@
 //
 // A CTA is one fetching warp and four computing warps around a ring of three
 // 32 KB stages, filled page by page by TMA (128-byte swizzle).  A stage is K
-// and V of 64 positions in bf16 or 32 in f32; each computing warp takes a
-// quarter of them, with its own running maximum, sum and result, and the four
-// are joined when the run leaves the (sequence, head).
+// and V of 64 positions in bf16 or 32 in f32; each computing warp takes 16 of
+// them (of every other stage in f32), with its own running maximum, sum and
+// result, and the four are joined when the run leaves the (sequence, head).
 //
-// The products run on mma.sync with the group's query heads as the 16 rows of
-// the tile: at one to sixteen query rows the tensor cores are mostly idle by
-// either path, and the operands come straight from registers.  They lose nothing
-// that an f32 result would show: an f32 query against a bf16 cache is three bf16
-// parts (the keys are exact), and so is a probability, two where the result is
-// bf16; an f32 cache is multiplied as tf32 parts, high x high + high x low +
-// low x high, whose remainder is 2^-22 of the product.  Sums are binary32.
+// The products run on mma.sync with 16 positions as the rows and eight query
+// heads as the columns, scores = K Q^T and result = V^T P^T, so that a group of
+// eight heads or fewer leaves none of a product unused beyond its missing heads;
+// the keys and values are read as they lie.  They lose nothing that an f32 result
+// would show: an f32 query against a bf16 cache is three bf16 parts (the keys are
+// exact), and so is a probability, two where the result is bf16; an f32 cache is
+// multiplied as tf32 parts, high x high + high x low + low x high, whose remainder
+// is 2^-22 of the product.  Sums are binary32.
 //
 // Positions at and beyond the length score -inf, and their values are masked to
 // zero in registers: unused page space may hold anything.
@@ -139,19 +140,19 @@ __device__ __forceinline__ void put2(uint16_t *p, int step, float x, float y) {
     else p[0] = uint16_t(f32_to_bf16(x)), p[step] = uint16_t(f32_to_bf16(y));
 }
 
-// WIDE: more than 8 query heads to a kv head (rows 8-15 of the products are used).
+// WIDE: more than 8 query heads to a kv head (two blocks of columns).
 template <typename T, typename TC, bool WIDE>
 __global__ void __launch_bounds__(PD_THREADS, 2)
 paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, const PagedKV c,
                    const PagedSeqs b, const typename Elem<T>::type *q, int64_t q_stride, int n_heads, int group,
                    typename Elem<T>::type *out, float *part, uint32_t *status) {
     constexpr bool CF32 = Elem<TC>::BYTES == 4;
-    constexpr int TILE = pd_tile<TC>(), KW = TILE / PD_WARPS, NH = WIDE ? 2 : 1;
+    constexpr int TILE = pd_tile<TC>(), NH = WIDE ? 2 : 1;   // NH: blocks of eight heads
     extern __shared__ uint8_t pd_dyn[];
     uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(pd_dyn) + 1023) & ~uintptr_t(1023));
     float *spare = reinterpret_cast<float *>(ring + PD_NS * PD_STAGE);
     __shared__ __align__(8) uint64_t full[PD_NS], empty[PD_NS];
-    __shared__ float join_m[3][2][8], join_l[3][2][8];
+    __shared__ float join_m[3][8 * NH], join_l[3][8 * NH];
     __shared__ volatile int dead;                            // a wait gave up
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -210,22 +211,26 @@ paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
     }
 
     // ---- the computing warps ---------------------------------------------------------
-    const int g = lane >> 2, t4 = lane & 3;                  // row g (and g + 8) of the products, column pair t4
+    const int g = lane >> 2, t4 = lane & 3;                  // products: row g (and g + 8), columns 2 t4 and + 1
     const uint32_t ring_a = smem_addr(ring);
+    const int key0 = CF32 ? 16 * (warp & 1) : 16 * warp;     // this warp's 16 positions of a tile
     int e = 0;
     bool ok = true;
     for (int64_t u = u0; u < u1 && ok;) {
         const int run = int(min(int64_t(w.tiles - w.tile), u1 - u));       // tiles of this (sequence, head) here
         const typename Elem<T>::type *qs = q + w.s * q_stride + int64_t(w.head) * group * HD;
         constexpr bool PARTS3 = !CF32 && Elem<T>::BYTES == 4;                // f32 queries, bf16 cache
-        uint32_t qf[CF32 || PARTS3 ? 1 : 8][2 * NH];         // bf16 queries, bf16 cache: operands in registers
-        if constexpr (CF32) {                                // the group's rows in shared memory, zeros below
-            for (int i = threadIdx.x; i < 8 * NH * (HD / 4); i += PD_WARPS * 32)
-                *reinterpret_cast<float4 *>(spare + 4 * i) =
-                    i / (HD / 4) < group ? load_quad(qs + 4 * i) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        uint32_t qf[CF32 || PARTS3 ? 1 : 8][NH][2];          // bf16 queries, bf16 cache: operands in registers
+        if constexpr (CF32) {
+            // the group's rows in shared memory, zeros below; 16-byte chunk x of row r at x ^ (r % 8) of its 128 bytes
+            for (int i = threadIdx.x; i < 8 * NH * (HD / 4); i += PD_WARPS * 32) {
+                const int row = i / (HD / 4), ch = i % (HD / 4);
+                *reinterpret_cast<float4 *>(spare + row * HD + 4 * ((ch & 24) | ((ch ^ row) & 7))) =
+                    row < group ? load_quad(qs + row * HD + 4 * ch) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
             named_sync(1, PD_WARPS * 32);
         } else if constexpr (PARTS3) {
-            // three bf16 parts of the group's rows in shared memory, zeros below; 16-byte chunk x of row r at x ^ (r % 8)
+            // three bf16 parts of the rows, zeros below; chunk x of row r at x ^ (r % 8)
             for (int i = threadIdx.x; i < 8 * NH * (HD / 2); i += PD_WARPS * 32) {
                 const int row = i / (HD / 2), col = 2 * (i % (HD / 2));
                 const float2 v = row < group ? *reinterpret_cast<const float2 *>(qs + row * HD + col) : make_float2(0.0f, 0.0f);
@@ -240,220 +245,227 @@ paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
 #pragma unroll
             for (int k = 0; k < 8; ++k)
 #pragma unroll
-                for (int x = 0; x < 2 * NH; ++x) {           // x: columns + 8 (bit 0), row + 8 (bit 1)
-                    const int row = g + 8 * (x >> 1), at = row * HD + 16 * k + 2 * t4 + 8 * (x & 1);
-                    qf[k][x] = row < group ? *reinterpret_cast<const uint32_t *>(qs + at) : 0u;
-                }
+                for (int n = 0; n < NH; ++n)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {            // dimensions 16 k + 2 t4 (+ 1), and 8 further
+                        const int row = 8 * n + g;
+                        qf[k][n][x] = row < group ? *reinterpret_cast<const uint32_t *>(qs + row * HD + 16 * k + 2 * t4 + 8 * x) : 0u;
+                    }
         }
-        float o[16][4];
+        // o[j][n]: dimensions (rows) of block j by heads 8 n + 2 t4, + 1.  In bf16 the rows g and g + 8 are dimensions
+        // 16 j + g and 8 further; in f32 32 (j / 2) + 4 g + 2 (j % 2) and the next one.
+        float o[8][NH][4];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
-        float m[NH], l[NH];
+        for (int j = 0; j < 8; ++j)
 #pragma unroll
-        for (int h = 0; h < NH; ++h) m[h] = -INFINITY, l[h] = 0.0f;
+            for (int n = 0; n < NH; ++n) o[j][n][0] = o[j][n][1] = o[j][n][2] = o[j][n][3] = 0.0f;
+        float m[NH][2], l[NH][2];                            // of heads 8 n + 2 t4, + 1; l over this lane's positions
+#pragma unroll
+        for (int n = 0; n < NH; ++n) m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.0f;
 
         for (int i = 0; i < run; ++i, ++e) {
             const int st = e % PD_NS;
             ok = __all_sync(FULL, mbar_wait(&full[st], uint32_t(e / PD_NS) & 1u, lane == 0 ? status : nullptr));
             if (!ok) break;
+            if (CF32 && ((e ^ (warp >> 1)) & 1)) {           // an f32 tile is two warps' work, the next one the others'
+                if (lane == 0) mbar_arrive(&empty[st]);
+                continue;
+            }
             const uint32_t ka = ring_a + st * PD_STAGE, va = ka + PD_SIDE;
-            const int left = w.len - (w.tile + i) * TILE - warp * KW;      // visible positions of this warp's KW
-            // scores: rows g, g + 8; columns (positions) 8 n + 2 t4, + 1
-            float s[KW / 8][4];
+            const int left = w.len - (w.tile + i) * TILE - key0;             // visible ones of this warp's 16
+            float s[NH][4];                                  // positions g and g + 8 by heads 8 n + 2 t4, + 1
 #pragma unroll
-            for (int n = 0; n < KW / 8; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+            for (int n = 0; n < NH; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
             if constexpr (CF32) {
-                // k index t4 is dimension 32 d + 8 t4 + x, k index t4 + 4 is + 1 of it (x = 0, 2, then 4, 6): a
-                // permutation that query and key share, so both are read 16 bytes at a time without conflicts
-                const uint32_t row = ka + (warp * KW + g) * 128, qa = smem_addr(spare) + g * (HD * 4);
+                // k index t4 is dimension 32 d + 8 t4 + 4 x + y, k index t4 + 4 is y + 1 (y = 0, 2): an order that query
+                // and key share, so that both are read 16 bytes at a time without conflicts
+                const uint32_t kr = ka + (key0 + g) * 128, qa = smem_addr(spare) + g * (HD * 4);
 #pragma unroll
                 for (int d = 0; d < 4; ++d)
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        const float4 kv = lds4(row + d * (PD_SIDE / 4) + (((2 * t4 + x) ^ g) << 4));
-                        const float kf[4] = {kv.x, kv.y, kv.z, kv.w};
-                        float qf[NH][4];
+                        const uint32_t ch = uint32_t((2 * t4 + x) ^ g) << 4;
+                        const float4 v0 = lds4(kr + d * (PD_SIDE / 4) + ch), v1 = lds4(kr + d * (PD_SIDE / 4) + 8 * 128 + ch);
+                        uint32_t ah[2][4], al[2][4];
+                        split_tf32(v0.x, ah[0][0], al[0][0]);
+                        split_tf32(v1.x, ah[0][1], al[0][1]);
+                        split_tf32(v0.y, ah[0][2], al[0][2]);
+                        split_tf32(v1.y, ah[0][3], al[0][3]);
+                        split_tf32(v0.z, ah[1][0], al[1][0]);
+                        split_tf32(v1.z, ah[1][1], al[1][1]);
+                        split_tf32(v0.w, ah[1][2], al[1][2]);
+                        split_tf32(v1.w, ah[1][3], al[1][3]);
 #pragma unroll
-                        for (int h = 0; h < NH; ++h) {
-                            const float4 v = lds4(qa + h * 8 * (HD * 4) + (32 * d + 8 * t4 + 4 * x) * 4);
-                            qf[h][0] = v.x, qf[h][1] = v.y, qf[h][2] = v.z, qf[h][3] = v.w;
-                        }
-                        float part[4] = {}, low[4] = {};
+                        for (int n = 0; n < NH; ++n) {
+                            const float4 v = lds4(qa + n * 8 * (HD * 4) + 128 * d + ch);
+                            uint32_t bh[4], bl[4];
+                            split_tf32(v.x, bh[0], bl[0]);
+                            split_tf32(v.y, bh[1], bl[1]);
+                            split_tf32(v.z, bh[2], bl[2]);
+                            split_tf32(v.w, bh[3], bl[3]);
+                            float part[4] = {}, low[4] = {};
 #pragma unroll
-                        for (int y = 0; y < 4; y += 2) {
-                            uint32_t bh[2], bl[2], ah[4] = {0, 0, 0, 0}, al[4] = {0, 0, 0, 0};
-                            split_tf32(kf[y], bh[0], bl[0]);
-                            split_tf32(kf[y + 1], bh[1], bl[1]);
-#pragma unroll
-                            for (int h = 0; h < NH; ++h) {
-                                split_tf32(qf[h][y], ah[h], al[h]);
-                                split_tf32(qf[h][y + 1], ah[2 + h], al[2 + h]);
+                            for (int y = 0; y < 2; ++y) {
+                                mma_tf32(low, al[y][0], al[y][1], al[y][2], al[y][3], bh[2 * y], bh[2 * y + 1]);
+                                mma_tf32(part, ah[y][0], ah[y][1], ah[y][2], ah[y][3], bh[2 * y], bh[2 * y + 1]);
+                                mma_tf32(low, ah[y][0], ah[y][1], ah[y][2], ah[y][3], bl[2 * y], bl[2 * y + 1]);
                             }
-                            mma_tf32(low, al[0], al[1], al[2], al[3], bh[0], bh[1]);
-                            mma_tf32(low, ah[0], ah[1], ah[2], ah[3], bl[0], bl[1]);
-                            mma_tf32(part, ah[0], ah[1], ah[2], ah[3], bh[0], bh[1]);
+                            add_to(part, low);
+                            add_to(s[n], part);
                         }
-                        add_to(part, low);
-                        add_to(s[0], part);
                     }
             } else {
-                const int key = warp * KW + (lane >> 4) * 8 + (lane & 7);
-                auto keys = [&](int k, uint32_t (&r)[4]) {   // dimensions 16 k ..; positions 0-7 in r[0], r[1], 8-15 in r[2], r[3]
-                    const int chunk = 2 * k + ((lane >> 3) & 1);
-                    ldsm4(ka + (chunk >> 3) * (PD_SIDE / 2) + key * 128 + (((chunk & 7) ^ (key & 7)) << 4), r);
+                const int key = key0 + ((lane >> 3) & 1) * 8 + (lane & 7);
+                auto keys = [&](int k, uint32_t (&a)[4]) {   // the 16 positions by dimensions 16 k ..
+                    const int chunk = 2 * k + (lane >> 4);
+                    ldsm4(ka + (chunk >> 3) * (PD_SIDE / 2) + key * 128 + (((chunk & 7) ^ (key & 7)) << 4), a);
                 };
                 if constexpr (PARTS3) {
-                    // a lane's address in the parts: WIDE rows 0-15 of chunks 2 k, 2 k + 1, otherwise rows 0-7 of four chunks
-                    const int row = WIDE ? lane & 15 : lane & 7, first = WIDE ? lane >> 4 : lane >> 3;
-                    const uint32_t qa = smem_addr(spare) + row * (HD * 2);
+                    const uint32_t qa = smem_addr(spare) + (lane & 7) * (HD * 2);
 #pragma unroll
-                    for (int k = 0; k < 8; k += 2) {
-                        uint32_t r[2][4], a[3][2][4];
-                        keys(k, r[0]);
-                        keys(k + 1, r[1]);
+                    for (int k = 0; k < 8; k += 2) {         // 32 dimensions
+                        uint32_t a[2][4];
+                        keys(k, a[0]);
+                        keys(k + 1, a[1]);
 #pragma unroll
-                        for (int x = 0; x < 3; ++x) {
-                            const uint32_t pa = qa + x * 8 * NH * (HD * 2);
-                            if constexpr (WIDE) {            // rows 0-7, 8-15 of chunk 2 k, then of 2 k + 1
-                                ldsm4(pa + (((2 * k + first) ^ (row & 7)) << 4), a[x][0]);
-                                ldsm4(pa + (((2 * k + 2 + first) ^ (row & 7)) << 4), a[x][1]);
-                            } else {
-                                uint32_t v[4];
-                                ldsm4(pa + (((2 * k + first) ^ row) << 4), v);
+                        for (int n = 0; n < NH; ++n) {
+                            float part[4] = {}, low[4] = {};
 #pragma unroll
-                                for (int y = 0; y < 2; ++y)
-                                    a[x][y][0] = v[2 * y], a[x][y][1] = 0u, a[x][y][2] = v[2 * y + 1], a[x][y][3] = 0u;
+                            for (int x = 2; x >= 0; --x) {
+                                uint32_t bq[4];              // chunks 2 k .. 2 k + 3 of heads 8 n ..
+                                ldsm4(qa + (x * NH + n) * 8 * (HD * 2) + (((2 * k + (lane >> 3)) ^ (lane & 7)) << 4), bq);
+                                mma_bf16(x ? low : part, a[0][0], a[0][1], a[0][2], a[0][3], bq[0], bq[1]);
+                                mma_bf16(x ? low : part, a[1][0], a[1][1], a[1][2], a[1][3], bq[2], bq[3]);
                             }
-                        }
-                        float part[2][4] = {}, low[2][4] = {};
-#pragma unroll
-                        for (int y = 0; y < 2; ++y)
-#pragma unroll
-                            for (int n = 0; n < 2; ++n) {
-                                mma_bf16(low[n], a[2][y][0], a[2][y][1], a[2][y][2], a[2][y][3], r[y][2 * n], r[y][2 * n + 1]);
-                                mma_bf16(low[n], a[1][y][0], a[1][y][1], a[1][y][2], a[1][y][3], r[y][2 * n], r[y][2 * n + 1]);
-                                mma_bf16(part[n], a[0][y][0], a[0][y][1], a[0][y][2], a[0][y][3], r[y][2 * n], r[y][2 * n + 1]);
-                            }
-#pragma unroll
-                        for (int n = 0; n < 2; ++n) {
-                            add_to(part[n], low[n]);
-                            add_to(s[n], part[n]);
+                            add_to(part, low);
+                            add_to(s[n], part);
                         }
                     }
                 } else {
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
-                        uint32_t r[4];
-                        keys(k, r);
+                        uint32_t a[4];
+                        keys(k, a);
 #pragma unroll
-                        for (int n = 0; n < 2; ++n)
-                            mma_bf16(s[n], qf[k][0], WIDE ? qf[k][2 * NH - 2] : 0u, qf[k][1], WIDE ? qf[k][2 * NH - 1] : 0u,
-                                     r[2 * n], r[2 * n + 1]);
+                        for (int n = 0; n < NH; ++n) mma_bf16(s[n], a[0], a[1], a[2], a[3], qf[k][n][0], qf[k][n][1]);
                     }
                 }
             }
-            // softmax over this warp's positions
-            if (left < KW) {
+            // softmax over the 16 positions, which the lanes of one t4 share
+            if (left < 16) {
 #pragma unroll
-                for (int n = 0; n < KW / 8; ++n)
+                for (int n = 0; n < NH; ++n)
 #pragma unroll
                     for (int x = 0; x < 4; ++x)
-                        if (8 * n + 2 * t4 + (x & 1) >= left) s[n][x] = -INFINITY;
+                        if (g + 8 * (x >> 1) >= left) s[n][x] = -INFINITY;
             }
-            float f[NH];
+            float f[NH][2];
             bool grow = false;
 #pragma unroll
-            for (int h = 0; h < NH; ++h) {
-                float tm = -INFINITY;
+            for (int n = 0; n < NH; ++n)
 #pragma unroll
-                for (int n = 0; n < KW / 8; ++n) tm = fmaxf(tm, fmaxf(s[n][2 * h], s[n][2 * h + 1]));
-                tm = fmaxf(tm, __shfl_xor_sync(FULL, tm, 1));
-                tm = fmaxf(tm, __shfl_xor_sync(FULL, tm, 2));
-                f[h] = 1.0f;
-                if (tm > m[h]) {
-                    f[h] = ex2_approx_ftz((m[h] - tm) * PD_LOG2);
-                    m[h] = tm;
-                    grow = true;
-                }
-                const float off = m[h] == -INFINITY ? 0.0f : -m[h] * PD_LOG2;
-                float add = 0.0f;
+                for (int h = 0; h < 2; ++h) {
+                    float tm = fmaxf(s[n][h], s[n][2 + h]);
 #pragma unroll
-                for (int n = 0; n < KW / 8; ++n)
-#pragma unroll
-                    for (int x = 2 * h; x < 2 * h + 2; ++x) {
-                        s[n][x] = ex2_approx_ftz(fmaf(s[n][x], PD_LOG2, off));
-                        add += s[n][x];
+                    for (int x = 4; x < 32; x <<= 1) tm = fmaxf(tm, __shfl_xor_sync(FULL, tm, x));
+                    f[n][h] = 1.0f;
+                    if (tm > m[n][h]) {
+                        f[n][h] = ex2_approx_ftz((m[n][h] - tm) * PD_LOG2);
+                        m[n][h] = tm;
+                        grow = true;
                     }
-                l[h] = fmaf(l[h], f[h], add);
-            }
+                    const float off = m[n][h] == -INFINITY ? 0.0f : -m[n][h] * PD_LOG2;
+                    s[n][h] = ex2_approx_ftz(fmaf(s[n][h], PD_LOG2, off));
+                    s[n][2 + h] = ex2_approx_ftz(fmaf(s[n][2 + h], PD_LOG2, off));
+                    l[n][h] = fmaf(l[n][h], f[n][h], s[n][h] + s[n][2 + h]);
+                }
             if (__any_sync(FULL, grow)) {
 #pragma unroll
-                for (int j = 0; j < 16; ++j)
+                for (int j = 0; j < 8; ++j)
 #pragma unroll
-                    for (int x = 0; x < 2 * NH; ++x) o[j][x] *= f[x >> 1];
+                    for (int n = 0; n < NH; ++n)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) o[j][n][x] *= f[n][x & 1];
             }
             // the weighted values
             if constexpr (CF32) {
-                // k index t4 is position 2 t4, t4 + 4 is 2 t4 + 1: the columns this thread's scores have;
-                // column n of product (d, x) is dimension 32 d + 4 n + x
-                uint32_t ph[4] = {0, 0, 0, 0}, pl[4] = {0, 0, 0, 0};
+                // In a block of eight positions k index t4 is position 2 t4, t4 + 4 the next one, and heads are columns:
+                // the probabilities of lanes 8 t4 + g / 2 and 4 further, of head g % 2 there.
+                uint32_t ph[2][NH][2], pl[2][NH][2];
 #pragma unroll
-                for (int h = 0; h < NH; ++h) {
-                    split_tf32(s[0][2 * h], ph[h], pl[h]);
-                    split_tf32(s[0][2 * h + 1], ph[2 + h], pl[2 + h]);
-                }
-                const int k0 = warp * KW + 2 * t4;
-                const bool live0 = 2 * t4 < left, live1 = 2 * t4 + 1 < left;
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int n = 0; n < NH; ++n)
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const int from = 8 * t4 + 4 * x + (g >> 1);
+                            const float p0 = __shfl_sync(FULL, s[n][2 * kb], from), p1 = __shfl_sync(FULL, s[n][2 * kb + 1], from);
+                            split_tf32(g & 1 ? p1 : p0, ph[kb][n][x], pl[kb][n][x]);
+                        }
 #pragma unroll
                 for (int d = 0; d < 4; ++d) {
-                    const uint32_t blk = va + d * (PD_SIDE / 4);
-                    const float4 v0 = lds4(blk + k0 * 128 + ((g ^ (k0 & 7)) << 4));
-                    const float4 v1 = lds4(blk + (k0 + 1) * 128 + ((g ^ ((k0 + 1) & 7)) << 4));
-                    const float a0[4] = {v0.x, v0.y, v0.z, v0.w}, a1[4] = {v1.x, v1.y, v1.z, v1.w};
+                    float part[2][NH][4] = {}, low[2][NH][4] = {};
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        uint32_t bh[2], bl[2];
-                        split_tf32(live0 ? a0[x] : 0.0f, bh[0], bl[0]);
-                        split_tf32(live1 ? a1[x] : 0.0f, bh[1], bl[1]);
-                        float part[4] = {};
-                        mma_tf32(part, pl[0], pl[1], pl[2], pl[3], bh[0], bh[1]);
-                        mma_tf32(part, ph[0], ph[1], ph[2], ph[3], bl[0], bl[1]);
-                        mma_tf32(part, ph[0], ph[1], ph[2], ph[3], bh[0], bh[1]);
-                        add_to(o[4 * d + x], part);
+                    for (int kb = 0; kb < 2; ++kb) {
+                        const int k0 = key0 + 8 * kb + 2 * t4;
+                        const uint32_t at = va + d * (PD_SIDE / 4) + k0 * 128;
+                        const float4 v0 = lds4(at + ((g ^ (2 * t4)) << 4)), v1 = lds4(at + 128 + ((g ^ (2 * t4 + 1)) << 4));
+                        const bool live0 = 8 * kb + 2 * t4 < left, live1 = 8 * kb + 2 * t4 + 1 < left;
+                        const float x0[4] = {v0.x, v0.y, v0.z, v0.w}, x1[4] = {v1.x, v1.y, v1.z, v1.w};
+#pragma unroll
+                        for (int y = 0; y < 2; ++y) {
+                            uint32_t ah[4], al[4];
+                            split_tf32(live0 ? x0[2 * y] : 0.0f, ah[0], al[0]);
+                            split_tf32(live0 ? x0[2 * y + 1] : 0.0f, ah[1], al[1]);
+                            split_tf32(live1 ? x1[2 * y] : 0.0f, ah[2], al[2]);
+                            split_tf32(live1 ? x1[2 * y + 1] : 0.0f, ah[3], al[3]);
+#pragma unroll
+                            for (int n = 0; n < NH; ++n) {
+                                mma_tf32(low[y][n], al[0], al[1], al[2], al[3], ph[kb][n][0], ph[kb][n][1]);
+                                mma_tf32(part[y][n], ah[0], ah[1], ah[2], ah[3], ph[kb][n][0], ph[kb][n][1]);
+                                mma_tf32(low[y][n], ah[0], ah[1], ah[2], ah[3], pl[kb][n][0], pl[kb][n][1]);
+                            }
+                        }
                     }
+#pragma unroll
+                    for (int y = 0; y < 2; ++y)
+#pragma unroll
+                        for (int n = 0; n < NH; ++n) {
+                            add_to(part[y][n], low[y][n]);
+                            add_to(o[2 * d + y][n], part[y][n]);
+                        }
                 }
             } else {
                 constexpr int PARTS = Elem<T>::BYTES == 4 ? 3 : 2;
-                uint32_t p[PARTS][4] = {};
+                uint32_t p[PARTS][NH][2];                    // positions by heads: the scores' blocks, transposed
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
+                for (int n = 0; n < NH; ++n)
 #pragma unroll
-                    for (int h = 0; h < NH; ++h) {
+                    for (int x = 0; x < 2; ++x) {
                         uint32_t part[PARTS];
-                        split_bf16(s[n][2 * h], s[n][2 * h + 1], part);
+                        split_bf16(s[n][2 * x], s[n][2 * x + 1], part);
 #pragma unroll
-                        for (int x = 0; x < PARTS; ++x) p[x][2 * n + h] = part[x];
+                        for (int y = 0; y < PARTS; ++y) p[y][n][x] = transpose8x8(part[y]);
                     }
-                // keep[n]: which of the positions 8 n + 2 t4, + 1 exist
+                // keep[x]: which of the positions 8 x + 2 t4, + 1 exist
                 uint32_t keep[2];
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
-                    keep[n] = (8 * n + 2 * t4 < left ? 0xffffu : 0u) | (8 * n + 2 * t4 + 1 < left ? 0xffff0000u : 0u);
-                const int key = warp * KW + ((lane >> 3) & 1) * 8 + (lane & 7);
+                for (int x = 0; x < 2; ++x)
+                    keep[x] = (8 * x + 2 * t4 < left ? 0xffffu : 0u) | (8 * x + 2 * t4 + 1 < left ? 0xffff0000u : 0u);
+                const int key = key0 + (lane >> 4) * 8 + (lane & 7);
 #pragma unroll
-                for (int d = 0; d < 8; ++d) {
-                    const int chunk = 2 * d + (lane >> 4);
-                    uint32_t r[4];
-                    ldsm4_t(va + (chunk >> 3) * (PD_SIDE / 2) + key * 128 + (((chunk & 7) ^ (key & 7)) << 4), r);
+                for (int j = 0; j < 8; ++j) {
+                    const int chunk = 2 * j + ((lane >> 3) & 1);
+                    uint32_t a[4];                           // dimensions 16 j + g, + 8 by positions 0-7, then by 8-15
+                    ldsm4_t(va + (chunk >> 3) * (PD_SIDE / 2) + key * 128 + (((chunk & 7) ^ (key & 7)) << 4), a);
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) r[x] &= keep[x & 1];
+                    for (int x = 0; x < 4; ++x) a[x] &= keep[x >> 1];
 #pragma unroll
-                    for (int n = 0; n < 2; ++n) {
+                    for (int n = 0; n < NH; ++n) {
                         float part[4] = {};
 #pragma unroll
-                        for (int x = PARTS - 1; x >= 0; --x)
-                            mma_bf16(part, p[x][0], p[x][1], p[x][2], p[x][3], r[2 * n], r[2 * n + 1]);
-                        add_to(o[2 * d + n], part);
+                        for (int y = PARTS - 1; y >= 0; --y) mma_bf16(part, a[0], a[1], a[2], a[3], p[y][n][0], p[y][n][1]);
+                        add_to(o[j][n], part);
                     }
                 }
             }
@@ -463,51 +475,62 @@ paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
         if (!ok && lane == 0) dead = 1;
         // join the four warps into warp 0 through shared memory
 #pragma unroll
-        for (int h = 0; h < NH; ++h) {
-            l[h] += __shfl_xor_sync(FULL, l[h], 1);
-            l[h] += __shfl_xor_sync(FULL, l[h], 2);
-        }
+        for (int n = 0; n < NH; ++n)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) l[n][h] += __shfl_xor_sync(FULL, l[n][h], x);
         constexpr int AT_ONCE = WIDE ? 1 : 3;                // warps whose results fit the spare memory
 #pragma unroll
         for (int src = 1; src < PD_WARPS; src += AT_ONCE) {
             named_sync(1, PD_WARPS * 32);
             if (warp >= src && warp < src + AT_ONCE) {
-                float *to = spare + (warp - src) * (16 * 2 * NH * 32);
+                float *to = spare + (warp - src) * (8 * NH * 4 * 32) + lane;
 #pragma unroll
-                for (int j = 0; j < 16; ++j)
+                for (int j = 0; j < 8; ++j)
 #pragma unroll
-                    for (int x = 0; x < 2 * NH; ++x) to[(j * 2 * NH + x) * 32 + lane] = o[j][x];
+                    for (int n = 0; n < NH; ++n)
 #pragma unroll
-                for (int h = 0; h < NH; ++h)
-                    if (t4 == 0) join_m[warp - src][h][g] = m[h], join_l[warp - src][h][g] = l[h];
+                        for (int x = 0; x < 4; ++x) to[((j * NH + n) * 4 + x) * 32] = o[j][n][x];
+                if (g == 0)
+#pragma unroll
+                    for (int n = 0; n < NH; ++n)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+                            join_m[warp - src][8 * n + 2 * t4 + h] = m[n][h], join_l[warp - src][8 * n + 2 * t4 + h] = l[n][h];
             }
             named_sync(1, PD_WARPS * 32);
             if (warp == 0) {
-                float f0[NH], f1[AT_ONCE][NH];
+                float f0[NH][2], f1[AT_ONCE][NH][2];
 #pragma unroll
-                for (int h = 0; h < NH; ++h) {
-                    float nm = m[h];
+                for (int n = 0; n < NH; ++n)
 #pragma unroll
-                    for (int i = 0; i < AT_ONCE; ++i) nm = fmaxf(nm, join_m[i][h][g]);
-                    f0[h] = m[h] == nm ? 1.0f : ex2_approx_ftz((m[h] - nm) * PD_LOG2);
-                    l[h] *= f0[h];
+                    for (int h = 0; h < 2; ++h) {
+                        const int head = 8 * n + 2 * t4 + h;
+                        float nm = m[n][h];
 #pragma unroll
-                    for (int i = 0; i < AT_ONCE; ++i) {
-                        const float om = join_m[i][h][g];
-                        f1[i][h] = om == nm ? 1.0f : ex2_approx_ftz((om - nm) * PD_LOG2);
-                        l[h] = fmaf(join_l[i][h][g], f1[i][h], l[h]);
+                        for (int i = 0; i < AT_ONCE; ++i) nm = fmaxf(nm, join_m[i][head]);
+                        f0[n][h] = m[n][h] == nm ? 1.0f : ex2_approx_ftz((m[n][h] - nm) * PD_LOG2);
+                        l[n][h] *= f0[n][h];
+#pragma unroll
+                        for (int i = 0; i < AT_ONCE; ++i) {
+                            const float om = join_m[i][head];
+                            f1[i][n][h] = om == nm ? 1.0f : ex2_approx_ftz((om - nm) * PD_LOG2);
+                            l[n][h] = fmaf(join_l[i][head], f1[i][n][h], l[n][h]);
+                        }
+                        m[n][h] = nm;
                     }
-                    m[h] = nm;
-                }
 #pragma unroll
-                for (int j = 0; j < 16; ++j)
+                for (int j = 0; j < 8; ++j)
 #pragma unroll
-                    for (int x = 0; x < 2 * NH; ++x) {
-                        o[j][x] *= f0[x >> 1];
+                    for (int n = 0; n < NH; ++n)
 #pragma unroll
-                        for (int i = 0; i < AT_ONCE; ++i)
-                            o[j][x] = fmaf(spare[((i * 16 + j) * 2 * NH + x) * 32 + lane], f1[i][x >> 1], o[j][x]);
-                    }
+                        for (int x = 0; x < 4; ++x) {
+                            o[j][n][x] *= f0[n][x & 1];
+#pragma unroll
+                            for (int i = 0; i < AT_ONCE; ++i)
+                                o[j][n][x] = fmaf(spare[(((i * 8 + j) * NH + n) * 4 + x) * 32 + lane], f1[i][n][x & 1], o[j][n][x]);
+                        }
             }
         }
         ok = dead == 0;                                      // the same for every warp: the next barrier follows the read
@@ -515,21 +538,23 @@ paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
             const bool whole = run == w.tiles;
             const int slot = 2 * int(blockIdx.x) + (u != u0);
 #pragma unroll
-            for (int h = 0; h < NH; ++h) {
-                const int row = g + 8 * h;
-                if (row >= group) continue;
-                const float r = whole ? 1.0f / l[h] : 1.0f;
-                typename Elem<T>::type *dst = out + (int64_t(w.s) * n_heads + w.head * group + row) * HD;
-                float *pd = part + (int64_t(slot) * group + row) * PD_PART;
+            for (int n = 0; n < NH; ++n)
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const int at = CF32 ? 32 * (j >> 2) + 8 * t4 + (j & 3) : 8 * j + 2 * t4;
-                    const float x = o[j][2 * h] * r, y = o[j][2 * h + 1] * r;
-                    if (whole) put2(dst + at, CF32 ? 4 : 1, x, y);
-                    else put2(pd + at, CF32 ? 4 : 1, x, y);
+                for (int h = 0; h < 2; ++h) {
+                    const int row = 8 * n + 2 * t4 + h;
+                    if (row >= group) continue;
+                    const float r = whole ? 1.0f / l[n][h] : 1.0f;
+                    typename Elem<T>::type *dst = out + (int64_t(w.s) * n_heads + w.head * group + row) * HD;
+                    float *pd = part + (int64_t(slot) * group + row) * PD_PART;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const int at = CF32 ? 32 * (j >> 1) + 4 * g + 2 * (j & 1) : 16 * j + g;
+                        const float x = o[j][n][h] * r, y = o[j][n][2 + h] * r;
+                        if (whole) put2(dst + at, CF32 ? 1 : 8, x, y);
+                        else put2(pd + at, CF32 ? 1 : 8, x, y);
+                    }
+                    if (!whole && g == 0) pd[HD] = m[n][h], pd[HD + 1] = l[n][h];
                 }
-                if (!whole && t4 == 0) pd[HD] = m[h], pd[HD + 1] = l[h];
-            }
         }
         u += run;
         if (u < u1) walk_on<TC>(b, c, w, run);
