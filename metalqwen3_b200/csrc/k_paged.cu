@@ -30,6 +30,10 @@
 //
 // Positions at and beyond the length score -inf, and their values are masked to
 // zero in registers: unused page space may hold anything.
+//
+// Measured: 64 sequences of up to 16,384 (32/8 heads, f32 queries, bf16 cache)
+// 331 us, 6.4 TB/s; one of 100,003 (bf16) 72 to 75 us, 5.6 TB/s, where the CTAs'
+// equal shares end up to 12 us apart; one of 512 (16/8, f32) 8.5 us, all latency.
 #include "q3cu_mma.cuh"
 #include "q3cu_paged.cuh"
 #include "q3cu_tma.h"

