@@ -228,7 +228,8 @@ struct PromptOrder {
         const int lane = threadIdx.x & 31;
         const bool sorted = b.n_seqs <= PROMPT_SORTED;
         q[0] = prompt_seq(b, c, total_rows, per_block, sorted ? lane : b.n_seqs, status);
-        q[1] = prompt_seq(b, c, total_rows, per_block, sorted ? lane + 32 : b.n_seqs, status);
+        q[1] = PromptSeq{0, 0, 0, 0, 0};
+        if (sorted && b.n_seqs > 32) q[1] = prompt_seq(b, c, total_rows, per_block, lane + 32, status);
         hi = (max(__reduce_max_sync(FULL, q[0].len), __reduce_max_sync(FULL, q[1].len)) + tile_keys - 1) / tile_keys + 1;
         above = from = passed = 0;
     }
@@ -236,7 +237,7 @@ struct PromptOrder {
         return q[x].at_least(tiles ? (tiles - 1) * tile_keys + 1 : 0, per_block);
     }
     __device__ __forceinline__ int count(int tiles) const {
-        return int(__reduce_add_sync(FULL, at_least(0, tiles) + at_least(1, tiles)));
+        return int(__reduce_add_sync(FULL, at_least(0, tiles) + (b.n_seqs > 32 ? at_least(1, tiles) : 0)));
     }
     static __device__ __forceinline__ void take(PromptItem &it, const PromptSeq &from, int s, int l, int first) {
         it.s = s;

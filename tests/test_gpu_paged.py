@@ -540,6 +540,67 @@ def test_captured_step_replayed(q3):
     assert q3.device_status() == 0
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_captured_prompts_replayed(q3, dtype):
+    """A captured append and prompt attention, replayed with other offsets and lengths, more items than the GPU has SMs."""
+    rows_max, heads, n_kv = 1500, 16, 8
+    p = Paged([900, 1100, 700], n_kv, 16, dtype, seed=64).fill(65)
+    off = torch.tensor([0, 300, 900, 1400], dtype=torch.int32, device="cuda")
+    x = queries(rows_max, heads + 2 * n_kv, F32, 66)
+    from metalqwen3_b200.q3cu import KVBatch
+    cache, batch = p.handles()[0], KVBatch(p.kv_len, p.table, off)
+    rq, out = (torch.full((rows_max, heads, 128), 5.0, dtype=dtype, device="cuda") for _ in range(2))
+
+    def step():
+        q3.kv_append(cache, batch, x[:, :heads], x[:, heads:heads + n_kv], x[:, heads + n_kv:], q_out=rq)
+        q3.attention_prompt(cache, batch, rq, out=out)
+
+    p.kv_len.copy_(torch.tensor([300, 600, 500], dtype=torch.int32))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for rows, lens in (((300, 600, 500), (300, 600, 500)), ((1, 1100, 399), (1, 1100, 700)), ((0, 0, 64), (0, 900, 64)),
+                       ((800, 33, 600), (900, 1033, 650))):
+        off.copy_(torch.tensor(offsets(rows), dtype=torch.int32))
+        p.kv_len.copy_(torch.tensor(lens, dtype=torch.int32))
+        out.fill_(5.0)
+        graph.replay()
+        first = 0
+        for s, (r, n) in enumerate(zip(rows, lens)):
+            if r:
+                k, v = (t[:n] for t in p.rows(s))
+                pick = sorted({0, 1 % r, r // 3, r // 2, r - 1})           # the others are the same code
+                at = torch.tensor([first + i for i in pick], device="cuda")
+                check_attention(out[at], rq[at], k, v, [n - r + 1 + i for i in pick], dtype, H if dtype == BF16 else 0.0)
+                assert torch.isfinite(out[first:first + r]).all()
+            first += r
+        assert (out[first:] == 5.0).all()
+    assert q3.device_status() == 0
+
+
+def test_calls_on_a_given_stream(q3):
+    """`stream` in place of the current one, with the binding's own outputs and workspace."""
+    p = Paged([70, 1200], 2, 16, BF16, seed=67).fill(68)
+    q, k = queries(2, 8, BF16, 69), queries(2, 2, BF16, 70)
+    cache, batch = p.handles([0, 1, 2])
+    want = q3.attention_paged(cache, batch, q), q3.attention_prompt(cache, batch, q)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for _ in range(10):
+        got = q3.attention_paged(cache, batch, q, stream=side), q3.attention_prompt(cache, batch, q, stream=side)
+        side.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    rq = q3.kv_append(cache, batch, q, k, k, stream=side)
+    side.synchronize()
+    check_rotated(rq, q, None, torch.tensor([69, 1199], device="cuda"), BF16)
+    assert q3.device_status(side) == 0
+
+
 def test_two_streams_at_once(q3):
     """Calls on two streams with a workspace each, many times: every result equals the call alone."""
     sets = []
