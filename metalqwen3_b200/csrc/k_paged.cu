@@ -284,7 +284,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
                 // k index t4 is dimension 32 d + 8 t4 + 4 x + y, k index t4 + 4 is y + 1 (y = 0, 2): an order that query
                 // and key share, so that both are read 16 bytes at a time without conflicts
                 const uint32_t kr = ka + (key0 + g) * 128, qa = smem_addr(spare) + g * (HD * 4);
-#pragma unroll
+#pragma unroll 1
                 for (int d = 0; d < 4; ++d)
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
@@ -540,24 +540,25 @@ paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
         ok = dead == 0;                                      // the same for every warp: the next barrier follows the read
         if (warp == 0 && ok) {
             const bool whole = run == w.tiles;
-            const int slot = 2 * int(blockIdx.x) + (u != u0);
+            const int at0 = CF32 ? 4 * g : g, step = CF32 ? 1 : 8;           // this lane's first element, and to its pair
+            auto block = [](int j) { return CF32 ? 32 * (j >> 1) + 2 * (j & 1) : 16 * j; };
 #pragma unroll
             for (int n = 0; n < NH; ++n)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int row = 8 * n + 2 * t4 + h;
                     if (row >= group) continue;
-                    const float r = whole ? 1.0f / l[n][h] : 1.0f;
-                    typename Elem<T>::type *dst = out + (int64_t(w.s) * n_heads + w.head * group + row) * HD;
-                    float *pd = part + (int64_t(slot) * group + row) * PD_PART;
+                    if (whole) {
+                        const float r = 1.0f / l[n][h];
+                        typename Elem<T>::type *dst = out + (int64_t(w.s) * n_heads + w.head * group + row) * HD + at0;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const int at = CF32 ? 32 * (j >> 1) + 4 * g + 2 * (j & 1) : 16 * j + g;
-                        const float x = o[j][n][h] * r, y = o[j][n][2 + h] * r;
-                        if (whole) put2(dst + at, CF32 ? 1 : 8, x, y);
-                        else put2(pd + at, CF32 ? 1 : 8, x, y);
+                        for (int j = 0; j < 8; ++j) put2(dst + block(j), step, o[j][n][h] * r, o[j][n][2 + h] * r);
+                    } else {
+                        float *pd = part + ((2 * int64_t(blockIdx.x) + (u != u0)) * group + row) * PD_PART;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) put2(pd + at0 + block(j), step, o[j][n][h], o[j][n][2 + h]);
+                        if (g == 0) pd[HD] = m[n][h], pd[HD + 1] = l[n][h];
                     }
-                    if (!whole && g == 0) pd[HD] = m[n][h], pd[HD + 1] = l[n][h];
                 }
         }
         u += run;
