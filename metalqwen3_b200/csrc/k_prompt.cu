@@ -88,13 +88,6 @@ __device__ __forceinline__ void exp2_poly(float &x, float &y) {
 }
 constexpr int PT_POLY = 8;                                   // one pair of exponentials in PT_POLY / 2 by polynomial
 
-// Scores from column n of 32 on become -inf.
-__device__ __forceinline__ void mask32(uint32_t *v, int n) {
-#pragma unroll
-    for (int y = 0; y < 32; ++y)
-        if (y >= n) v[y] = 0xff800000u;
-}
-
 // The item of a round, as warp 9 announces it (s < 0: no more), with the key tiles of each row tile.
 struct PromptRound : PromptItem {
     int nt[2];

@@ -1,286 +1,359 @@
 // k_prompt_f32.cu -- causal attention of packed f32 prompt rows over an f32 paged cache.
 //
-// The operation of k_prompt.cu, with nothing rounded below binary32's sums: a
-// product of two f32 operands is taken as tf32 parts, high x high + high x low
-// + low x high (the dropped low x low is 2^-22 of it), on mma.sync, in short
-// chains that are added in binary32.  That is three tensor-core products for one, and still ahead of
-// the FMA units.
+// The operation of k_prompt.cu, with nothing rounded below binary32's sums: each
+// f32 operand is taken as three bf16 parts (24 bits of mantissa, split_bf16), and
+// a product as the six products of parts that count (what is dropped is 2^-25 of
+// it), on tcgen05 with binary32 accumulators.  The tensor cores cut their sums
+// where binary32 would round them, so the small products go first and each key
+// tile's P V starts afresh: the result itself is kept in registers and summed by
+// ordinary additions.
 //
-// A work item is 64 rows -- row r is query r / g, head r % g of a group of g
-// query heads -- against one kv head.  Four computing warps take 16 rows each
-// over all keys, 32 at a time, with the running maximum and sum of the softmax;
-// one warp fetches the key and value tiles page by page (TMA, 128-byte swizzle,
-// two stages).  Two CTAs share an SM, so one's softmax runs beside the other's
-// products.  The operands' index orders are chosen so that every shared-memory
-// read is 16 bytes wide and free of bank conflicts (see the comments below).
-// 2,000 rows in three prompts (16/8 heads): 166 us, 38 TFLOP/s of the operator,
-// three times that of the tensor cores, whose mma.sync pipe is busy half the time.
-// Masks and rows that come out as NaN are treated as in k_prompt.cu; values
-// behind the sequence's end are masked in registers.
+// A work item is 128 rows -- row r is query r / g, head r % g of a group of g
+// query heads -- against one kv head, 64 keys at a time, one CTA per SM:
+//   warps 0-3    thread = row = tensor-memory lane.  Splits the row's query into
+//                tensor memory once.  For each key tile: the running maximum and
+//                sum of the softmax, the probabilities as three parts over the
+//                scores, then the tile before's P V into the row's 128 registers.
+//   warp 4       issues the products, queries and probabilities (the A operands)
+//                from tensor memory, keys and values from shared memory.  The
+//                next tile's scores are issued before this tile's P V, so that
+//                the softmax runs beside them.
+//   warps 8-11   read the keys, page by page, split them and store the parts as
+//                the swizzled operand tiles, two stages; warps 12-15 the values.
+// Tensor memory (512 columns): the query's parts 0-191, two slots of 96 for scores
+// and the probabilities' parts over them, the tile's P V 384-511.
+//
+// Masks and rows that come out as NaN are treated as in k_prompt.cu; keys and values
+// behind the sequence's end are stored as zeros.  (An infinity splits into
+// infinity and NaN, so its rows go the way of NaN rows, which ends in the formula.)
 #include "q3cu_mma.cuh"
 #include "q3cu_paged.cuh"
+#include "q3cu_tcgen05.cuh"
 #include "q3cu_tma.h"
 
 namespace q3 {
 
-constexpr int PF_WARPS = 4, PF_THREADS = (PF_WARPS + 1) * 32, PF_ROWS = 16 * PF_WARPS, PF_KEYS = 32, PF_NS = 2;
-constexpr uint32_t PF_SIDE = PF_KEYS * HD * 4, PF_STAGE = 2 * PF_SIDE;
-constexpr size_t PF_SMEM = size_t(PF_NS) * PF_STAGE + size_t(PF_ROWS) * HD * 4 + 1024;
+constexpr int PF_ROWS = 128, PF_KEYS = 64, PF_THREADS = 16 * 32, PF_NS = 2;
+constexpr uint32_t PF_HALF = PF_KEYS * 128;                  // bytes of 64 keys x 64 elements of a part
+constexpr uint32_t PF_PART = 2 * PF_HALF, PF_TILE = 3 * PF_PART;
+constexpr size_t PF_SMEM = size_t(PF_NS) * 2 * PF_TILE + 1024;
+constexpr uint32_t PF_SLOT = 192, PF_OUT = 384;              // tensor-memory columns: first slot, P V
+// Instruction descriptors (f32 accumulator, bf16 A and B, M = 128): scores, N = 64 keys, and P V, N = 128, B MN-major.
+constexpr uint32_t PF_IDESC_BASE = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(128 / 16) << 24);
+constexpr uint32_t PF_IDESC = PF_IDESC_BASE | (uint32_t(PF_KEYS / 8) << 17);
+constexpr uint32_t PF_IDESC_V = PF_IDESC_BASE | (uint32_t(HD / 8) << 17) | (1u << 16);
 constexpr float PF_LOG2 = ATT_SCALE * 1.44269504088896341f;
+// The products of parts from the smallest, the parts' numbers as hexadecimal digits from the right: low x high,
+// high x low, mid x mid, mid x high, high x mid, high x high.
+constexpr uint32_t PF_A = 0x001102, PF_B = 0x010120;
+__host__ __device__ constexpr uint32_t pf_part(uint32_t parts, int x) { return parts >> (4 * x) & 15u; }
+// Column of a slot where a part of 32 probabilities lies: those of keys 32 .. 63 (half 1) are stored first, over columns
+// whose scores have been read (32 ..) or that have none (64 ..).
+__host__ __device__ constexpr uint32_t pf_col(int half, uint32_t part) { return half ? 64 + part * 16 - part / 2 * 48 : part * 16; }
 
-__global__ void __launch_bounds__(PF_THREADS, 2)
-prompt_f32_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, const PagedKV c,
-                  const PagedSeqs b, int rows, const float *q, int64_t q_stride, int n_heads, int group,
+// 16 floats as three bf16 parts each, packed in pairs, to columns at[0 .. 2] of this thread's tensor-memory lane.
+__device__ __forceinline__ void store_parts16(const float (&x)[16], uint32_t at0, uint32_t at1, uint32_t at2) {
+    uint32_t w[3][8];
+#pragma unroll
+    for (int y = 0; y < 8; ++y) {
+        uint32_t p[3];
+        split_bf16<3>(x[2 * y], x[2 * y + 1], p);
+        w[0][y] = p[0];
+        w[1][y] = p[1];
+        w[2][y] = p[2];
+    }
+    tc_st8(at0, w[0]);
+    tc_st8(at1, w[1]);
+    tc_st8(at2, w[2]);
+}
+
+__global__ void __launch_bounds__(PF_THREADS, 1)
+prompt_f32_kernel(const PagedKV c, const PagedSeqs b, int rows, const float *q, int64_t q_stride, int n_heads, int group,
                   const FastDiv per_block, float *out, uint32_t *status) {
     extern __shared__ uint8_t pf_dyn[];
-    uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(pf_dyn) + 1023) & ~uintptr_t(1023));
-    float *qs = reinterpret_cast<float *>(ring + PF_NS * PF_STAGE);
-    __shared__ __align__(8) uint64_t full[PF_NS], empty[PF_NS];
+    uint8_t *tiles = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(pf_dyn) + 1023) & ~uintptr_t(1023));
+    // tiles of keys (side 0) and values (side 1), two stages each
+    __shared__ __align__(8) uint64_t full[2][PF_NS], empty[2][PF_NS], q_full, s_full[2], p_full, o_full, drain;
+    __shared__ PromptItem item_sh;
+    __shared__ uint32_t tmem_sh;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < PF_NS; ++i) {
-            mbar_init(&full[i], 1);
-            mbar_init(&empty[i], PF_WARPS);
+            for (int side = 0; side < 2; ++side) {
+                mbar_init(&full[side][i], 4);
+                mbar_init(&empty[side][i], 1);
+            }
+            mbar_init(&s_full[i], 1);
         }
+        mbar_init(&q_full, 4);
+        mbar_init(&p_full, 4);
+        mbar_init(&o_full, 1);
+        mbar_init(&drain, 1);
         mbar_init_fence();
     }
+    if (warp == 4) tc_alloc512(&tmem_sh);
     griddep_wait();
-    const int qt = per_block.d;                              // queries of an item
-    const PromptItem it = PromptOrder(b, c, rows, per_block, PF_KEYS, warp == 0 ? status : nullptr).find(blockIdx.x);
-    if (it.s < 0) return;
-    const int len = it.len;
-    auto seen = [&](int i) { return it.seen(i); };
-    const int queries = min(qt, it.rows - it.first);
-    const int nkv = (seen(it.first + queries - 1) + PF_KEYS - 1) / PF_KEYS;
-    // the queries, 16-byte chunk x of row r at x ^ (r % 8) of its 128-byte block
-    for (int x = threadIdx.x; x < PF_ROWS * (HD / 4); x += PF_THREADS) {
-        const int r = x / (HD / 4), ch = x % (HD / 4);
-        const bool live = r < queries * group;
-        const float4 v = live ? load_quad(q + int64_t(it.base + it.first + r / group) * q_stride +
-                                          int64_t(it.head * group + r % group) * HD + 4 * ch)
-                              : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        *reinterpret_cast<float4 *>(qs + r * HD + 4 * ((ch & 24) | ((ch ^ r) & 7))) = v;
+    if (warp == 8) {
+        const PromptItem found = PromptOrder(b, c, rows, per_block, PF_KEYS, status).find(blockIdx.x);
+        if (lane == 0) item_sh = found;
     }
+    tc_fence_before();
     __syncthreads();
+    tc_fence_after();
+    const uint32_t tbase = tmem_sh;
+    const PromptItem it = item_sh;
+    const int queries = it.s < 0 ? 0 : min(per_block.d, it.rows - it.first);
+    const int nkv = it.s < 0 ? 0 : (it.seen(it.first + queries - 1) + PF_KEYS - 1) / PF_KEYS;
 
-    if (warp == PF_WARPS) {
-        // ---- fetch: lane = box (K or V, 32 columns, rows of one page) --------------------
-        const int br = min(1 << c.page_shift, PF_KEYS), nb = PF_KEYS / br;
-        const int box = lane % nb, col = lane / nb % 4, side = lane / (4 * nb);
-        auto page_of = [&](int j) -> int {                   // n_pages reads as zeros
-            const int t = j * PF_KEYS + box * br;
-            if (side > 1 || t >= len) return c.n_pages;
-            const int p = paged_page(b, c, it.s, t, status);
-            return p < 0 ? c.n_pages : p;
-        };
-        int page = nkv ? page_of(0) : 0, e = 0;
-        bool ok = true;
-        for (; e < nkv; ++e) {
-            const int st = e % PF_NS, now = page, slot = (e * PF_KEYS + box * br) & ((1 << c.page_shift) - 1);
-            if (e + 1 < nkv) page = page_of(e + 1);
-            if (e >= PF_NS) ok = mbar_wait(&empty[st], uint32_t(e / PF_NS - 1) & 1u, lane == 0 ? status : nullptr);
-            if (!__all_sync(FULL, ok)) break;
-            if (lane == 0) mbar_arrive_expect_tx(&full[st], PF_STAGE);
+    // Registers move to the rows: 128 threads x 224 + 384 x 96 is the launch's 512 x 128.
+    if (warp >= 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+        if (warp >= 8) {
+            // ---- keys (warps 8-11) or values: 16 of a tile's rows per warp, in one page --------
+            const int side = (warp - 8) >> 2, first = 16 * (warp & 3);
+            const float *src = static_cast<const float *>(side ? c.v : c.k);
+            const int chunk = lane & 15, row = lane >> 4;    // elements 8 chunk .. + 7 of rows row, row + 2, ...
+            uint8_t *dst = tiles + side * PF_NS * PF_TILE + (chunk >> 3) * PF_HALF;
+            auto page_of = [&](int j) -> int {
+                const int t = j * PF_KEYS + first;
+                return t < it.len ? paged_page(b, c, it.s, t, lane == 0 ? status : nullptr) : -1;
+            };
+            int page = nkv ? page_of(0) : -1;
+            for (int j = 0; j < nkv; ++j) {
+                const int st = j & 1, t = j * PF_KEYS + first;
+                const float *at = src + (page < 0 ? 0 : paged_at(c, page, it.head, t)) + 8 * chunk;
+                const int n = page < 0 ? 0 : it.len - t;     // rows from n on read as zeros
+                float4 x[8][2];
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        x[u][h] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        if (row + 2 * u < n) x[u][h] = load_quad(at + (row + 2 * u) * HD + 4 * h);
+                    }
+                if (j + 1 < nkv) page = page_of(j + 1);
+                if (j >= PF_NS &&
+                    !__all_sync(FULL, mbar_wait(&empty[side][st], uint32_t((j >> 1) - 1) & 1u, lane == 0 ? status : nullptr)))
+                    break;
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const int r = first + row + 2 * u;
+                    uint32_t w[4][3];
+                    split_bf16<3>(x[u][0].x, x[u][0].y, w[0]);
+                    split_bf16<3>(x[u][0].z, x[u][0].w, w[1]);
+                    split_bf16<3>(x[u][1].x, x[u][1].y, w[2]);
+                    split_bf16<3>(x[u][1].z, x[u][1].w, w[3]);
+#pragma unroll
+                    for (int p = 0; p < 3; ++p)
+                        *reinterpret_cast<uint4 *>(dst + st * PF_TILE + p * PF_PART + r * 128 + (((chunk ^ r) & 7) << 4)) =
+                            make_uint4(w[0][p], w[1][p], w[2][p], w[3][p]);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&full[side][st]);
+            }
+        } else if (warp == 4) {
+            // ---- products -----------------------------------------------------------------
+            if (nkv && tc_elect()) {
+                const uint64_t dk = tc_sdesc(smem_addr(tiles)), dv = tc_sdesc_mn(smem_addr(tiles + PF_NS * PF_TILE), PF_HALF);
+                auto scores = [&](int st) {                  // S = Q K^T
+#pragma unroll
+                    for (int x = 0; x < 6; ++x)
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            tc_mma_bf16_ts(tbase + PF_SLOT + 96 * st, tbase + 64 * pf_part(PF_A, x) + 8 * k,
+                                           dk + ((st * PF_TILE + pf_part(PF_B, x) * PF_PART + (k / 4) * PF_HALF + (k % 4) * 32) >> 4),
+                                           PF_IDESC, uint32_t(x + k > 0));
+                    tc_commit(&s_full[st]);
+                    tc_commit(&empty[0][st]);
+                };
+                auto values = [&](int st) {                  // P V of one tile
+#pragma unroll
+                    for (int x = 0; x < 6; ++x)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            tc_mma_bf16_ts(tbase + PF_OUT, tbase + PF_SLOT + 96 * st + pf_col(k / 2, pf_part(PF_A, x)) + 8 * (k % 2),
+                                           dv + ((st * PF_TILE + pf_part(PF_B, x) * PF_PART + k * 2048) >> 4), PF_IDESC_V,
+                                           uint32_t(x + k > 0));
+                    tc_commit(&o_full);
+                    tc_commit(&empty[1][st]);
+                };
+                bool ok = mbar_wait(&q_full, 0, status) && mbar_wait(&full[0][0], 0, status);
+                if (ok) {
+                    tc_fence_after();
+                    scores(0);
+                }
+                for (int j = 0; ok && j < nkv; ++j) {
+                    if (j + 1 < nkv) {
+                        // over the probabilities of tile j - 1, whose products are before these in the pipe
+                        if (!(ok = mbar_wait(&full[0][(j + 1) & 1], uint32_t((j + 1) >> 1) & 1u, status))) break;
+                        tc_fence_after();
+                        scores((j + 1) & 1);
+                    }
+                    ok = mbar_wait(&full[1][j & 1], uint32_t(j >> 1) & 1u, status) &&
+                         mbar_wait(&p_full, uint32_t(j) & 1u, status);
+                    if (!ok) break;
+                    tc_fence_after();
+                    values(j & 1);
+                }
+                // every product issued has completed before tensor memory is given back (bounded)
+                tc_commit(&drain);
+                mbar_wait(&drain, 0, nullptr);
+            }
             __syncwarp();
-            if (side < 2)
-                tma_load_4d(ring + st * PF_STAGE + side * PF_SIDE + col * (PF_SIDE / 4) + box * br * 128,
-                            side ? &tmv : &tmk, 32 * col, slot, it.head, now, &full[st]);
         }
-        // no copy outlives the CTA (bounded)
-        for (int d = e > PF_NS ? e - PF_NS : 0; d < e; ++d) mbar_wait(&full[d % PF_NS], uint32_t(d / PF_NS) & 1u, nullptr);
-        return;
-    }
-
-    const int g = lane >> 2, t4 = lane & 3;                  // rows g, g + 8 of the warp's 16; column pair t4
-    int limit[2], i_of[2];
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        // ---- rows ---------------------------------------------------------------------
+        const int r = threadIdx.x, r_query = r / group, i = it.first + r_query;
+        const int head = it.head * group + r - r_query * group;
+        const bool live = r_query < queries;
+        const int limit = live ? it.seen(i) : 0;
+        const int sure = queries ? it.seen(it.first) : 0;    // keys that every row sees
+        const uint32_t lane_base = tbase + (uint32_t(32 * warp) << 16);
+        bool ok = true;
+        if (nkv) {
+            const float *row = q + int64_t(it.base + i) * q_stride + int64_t(head) * HD;
+#pragma unroll 2
+            for (int x = 0; x < HD / 16; ++x) {
+                float v[16];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int r = 16 * warp + g + 8 * h;
-        i_of[h] = it.first + r / group;
-        limit[h] = r < queries * group ? seen(i_of[h]) : 0;
-    }
-    const int sure = seen(it.first);                         // keys that every row sees
-    float o[16][4];
+                for (int y = 0; y < 4; ++y) {
+                    const float4 f = live ? load_quad(row + 16 * x + 4 * y) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    v[4 * y] = f.x;
+                    v[4 * y + 1] = f.y;
+                    v[4 * y + 2] = f.z;
+                    v[4 * y + 3] = f.w;
+                }
+                store_parts16(v, lane_base + 8 * x, lane_base + 64 + 8 * x, lane_base + 128 + 8 * x);
+            }
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_full);
+        }
+        float o[HD];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-    const uint32_t qa = smem_addr(qs) + (16 * warp + g) * (HD * 4), ring_a = smem_addr(ring);
-    bool ok = true;
-    for (int j = 0; j < nkv; ++j) {
-        const int st = j % PF_NS, base = j * PF_KEYS;
-        ok = __all_sync(FULL, mbar_wait(&full[st], uint32_t(j / PF_NS) & 1u, lane == 0 ? status : nullptr));
-        if (!ok) break;
-        const uint32_t ka = ring_a + st * PF_STAGE, va = ka + PF_SIDE;
-        float s[4][4];
+        for (int x = 0; x < HD; ++x) o[x] = 0.0f;
+        float m = -INFINITY, sum = 0.0f, f_before = 0.0f;
+        // adds the P V of the latest tile, whose maximum was `f` times further up than what o holds
+        auto add_tile = [&](float f) {
 #pragma unroll
-        for (int n = 0; n < 4; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
-        // k index t4 is dimension 32 d + 8 t4 + 4 x + y, k index t4 + 4 is y + 1 (y = 0, 2): an order that query and
-        // key share, so a lane reads 16 bytes of either, and the swizzle spreads eight rows over all banks
+            for (int x = 0; x < HD / 32; ++x) {
+                uint32_t u[32];
+                tc_ld32(lane_base + PF_OUT + 32 * x, u);
+                tc_wait_ld32(u);
 #pragma unroll
-        for (int d = 0; d < 4; ++d)
+                for (int y = 0; y < 32; ++y) o[32 * x + y] = fmaf(o[32 * x + y], f, __uint_as_float(u[y]));
+            }
+        };
+        for (int j = 0; j < nkv; ++j) {
+            ok = __all_sync(FULL, mbar_wait(&s_full[j & 1], uint32_t(j >> 1) & 1u, lane == 0 ? status : nullptr));
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t slot = lane_base + PF_SLOT + 96 * (j & 1);
+            const int left = limit - j * PF_KEYS;            // columns of this tile that the row sees
+            const bool mask = (j + 1) * PF_KEYS > sure;
+            float tile_max = -INFINITY;
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                const uint32_t ch = uint32_t((2 * t4 + x) ^ g) << 4;
-                uint32_t ah[2][4], al[2][4];                 // [y / 2]: rows g, g + 8 of k index t4, then of t4 + 4
+                uint32_t u[32];
+                tc_ld32(slot + 32 * x, u);
+                tc_wait_ld32(u);
+                if (mask) mask32(u, left - 32 * x);
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float4 v = lds4(qa + h * 8 * (HD * 4) + 128 * d + ch);
-                    split_tf32(v.x, ah[0][h], al[0][h]);
-                    split_tf32(v.y, ah[0][2 + h], al[0][2 + h]);
-                    split_tf32(v.z, ah[1][h], al[1][h]);
-                    split_tf32(v.w, ah[1][2 + h], al[1][2 + h]);
-                }
+                for (int y = 0; y < 32; ++y) mx[y & 3] = fmaxf(mx[y & 3], __uint_as_float(u[y]));
+                tile_max = fmaxf(tile_max, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+            }
+            float f = 1.0f;
+            if (tile_max > m) {
+                f = ex2_approx_ftz((m - tile_max) * PF_LOG2);
+                m = tile_max;
+            }
+            const float off = m == -INFINITY ? 0.0f : -m * PF_LOG2;
+            float add[2] = {0.0f, 0.0f};
 #pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                    const float4 v = lds4(ka + d * (PF_SIDE / 4) + (8 * n + g) * 128 + ch);
-                    uint32_t bh[4], bl[4];
-                    split_tf32(v.x, bh[0], bl[0]);
-                    split_tf32(v.y, bh[1], bl[1]);
-                    split_tf32(v.z, bh[2], bl[2]);
-                    split_tf32(v.w, bh[3], bl[3]);
-                    float part[4] = {}, low[4] = {};
+            for (int x = 1; x >= 0; --x) {
+                uint32_t u[32];
+                tc_ld32(slot + 32 * x, u);
+                tc_wait_ld32(u);
+                if (mask) mask32(u, left - 32 * x);
 #pragma unroll
-                    for (int y = 0; y < 2; ++y) {
-                        mma_tf32(low, al[y][0], al[y][1], al[y][2], al[y][3], bh[2 * y], bh[2 * y + 1]);
-                        mma_tf32(part, ah[y][0], ah[y][1], ah[y][2], ah[y][3], bh[2 * y], bh[2 * y + 1]);
-                        mma_tf32(low, ah[y][0], ah[y][1], ah[y][2], ah[y][3], bl[2 * y], bl[2 * y + 1]);
+                for (int z = 0; z < 2; ++z) {
+                    float p[16];
+#pragma unroll
+                    for (int y = 0; y < 16; ++y) {
+                        p[y] = ex2_approx_ftz(fmaf(__uint_as_float(u[16 * z + y]), PF_LOG2, off));
+                        add[y & 1] += p[y];
                     }
-                    add_to(part, low);
-                    add_to(s[n], part);
+                    store_parts16(p, slot + pf_col(x, 0) + 8 * z, slot + pf_col(x, 1) + 8 * z, slot + pf_col(x, 2) + 8 * z);
                 }
             }
-        if (base + PF_KEYS > sure) {
-#pragma unroll
-            for (int n = 0; n < 4; ++n)
-#pragma unroll
-                for (int x = 0; x < 4; ++x)
-                    if (base + 8 * n + 2 * t4 + (x & 1) >= limit[x >> 1]) s[n][x] = -INFINITY;
-        }
-        float f[2];
-        bool grow = false;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            float tm = -INFINITY;
-#pragma unroll
-            for (int n = 0; n < 4; ++n) tm = fmaxf(tm, fmaxf(s[n][2 * h], s[n][2 * h + 1]));
-            tm = fmaxf(tm, __shfl_xor_sync(FULL, tm, 1));
-            tm = fmaxf(tm, __shfl_xor_sync(FULL, tm, 2));
-            f[h] = 1.0f;
-            if (tm > m[h]) {
-                f[h] = ex2_approx_ftz((m[h] - tm) * PF_LOG2);
-                m[h] = tm;
-                grow = true;
+            sum = fmaf(sum, f, add[0] + add[1]);
+            if (j > 0) {
+                ok = __all_sync(FULL, mbar_wait(&o_full, uint32_t(j - 1) & 1u, lane == 0 ? status : nullptr));
+                if (!ok) break;
+                tc_fence_after();
+                add_tile(f_before);
             }
-            const float off = m[h] == -INFINITY ? 0.0f : -m[h] * PF_LOG2;
-            float add = 0.0f;
-#pragma unroll
-            for (int n = 0; n < 4; ++n)
-#pragma unroll
-                for (int x = 2 * h; x < 2 * h + 2; ++x) {
-                    s[n][x] = ex2_approx_ftz(fmaf(s[n][x], PF_LOG2, off));
-                    add += s[n][x];
-                }
-            l[h] = fmaf(l[h], f[h], add);
+            f_before = f;
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full);
         }
-        if (__any_sync(FULL, grow)) {
-#pragma unroll
-            for (int x = 0; x < 16; ++x)
-#pragma unroll
-                for (int y = 0; y < 4; ++y) o[x][y] *= f[y >> 1];
-        }
-        // k index t4 is position 8 n + 2 t4, t4 + 4 the next one: the columns this thread's scores have; column i of
-        // product (d, x) is dimension 32 d + 4 i + x
-        const bool tail = base + PF_KEYS > len;
-        uint32_t ph[4][4], pl[4][4];
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                split_tf32(s[n][2 * h], ph[n][h], pl[n][h]);
-                split_tf32(s[n][2 * h + 1], ph[n][2 + h], pl[n][2 + h]);
+        if (nkv && ok) {
+            ok = __all_sync(FULL, mbar_wait(&o_full, uint32_t(nkv - 1) & 1u, lane == 0 ? status : nullptr));
+            if (ok) {
+                tc_fence_after();
+                add_tile(f_before);
             }
-#pragma unroll
-        for (int d = 0; d < 4; ++d) {
-            float part[4][4] = {}, low[4][4] = {};
-#pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                const int k0 = 8 * n + 2 * t4;
-                const uint32_t blk = va + d * (PF_SIDE / 4) + k0 * 128;
-                float4 v0 = lds4(blk + ((g ^ (2 * t4)) << 4)), v1 = lds4(blk + 128 + ((g ^ (2 * t4 + 1)) << 4));
-                if (tail) {
-                    if (base + k0 >= len) v0 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    if (base + k0 + 1 >= len) v1 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                }
-                const float a0[4] = {v0.x, v0.y, v0.z, v0.w}, a1[4] = {v1.x, v1.y, v1.z, v1.w};
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    uint32_t bh[2], bl[2];
-                    split_tf32(a0[x], bh[0], bl[0]);
-                    split_tf32(a1[x], bh[1], bl[1]);
-                    mma_tf32(low[x], pl[n][0], pl[n][1], pl[n][2], pl[n][3], bh[0], bh[1]);
-                    mma_tf32(low[x], ph[n][0], ph[n][1], ph[n][2], ph[n][3], bl[0], bl[1]);
-                    mma_tf32(part[x], ph[n][0], ph[n][1], ph[n][2], ph[n][3], bh[0], bh[1]);
-                }
-            }
-#pragma unroll
-            for (int x = 0; x < 4; ++x) add_to(part[x], low[x]), add_to(o[4 * d + x], part[x]);
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&empty[st]);
-    }
-    if (!ok) return;
-    bool nan[2] = {false, false};
+        if (ok) {
+            const float inv = limit > 0 ? 1.0f / sum : 0.0f;
+            float *dst = out + (int64_t(it.base + i) * n_heads + head) * HD;
+            bool nan = false;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        l[h] += __shfl_xor_sync(FULL, l[h], 1);
-        l[h] += __shfl_xor_sync(FULL, l[h], 2);
-        const int r = 16 * warp + g + 8 * h;
-        const float inv = limit[h] > 0 ? 1.0f / l[h] : 0.0f;
-        float *dst = out + (int64_t(it.base + i_of[h]) * n_heads + it.head * group + r % group) * HD + 8 * t4;
-#pragma unroll
-        for (int d = 0; d < 4; ++d)
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
+            for (int x = 0; x < HD; x += 4) {
                 float v[4];
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    v[x] = limit[h] > 0 ? o[4 * d + x][2 * h + y] * inv : 0.0f;
-                    nan[h] |= v[x] != v[x];
+                for (int y = 0; y < 4; ++y) {
+                    v[y] = limit > 0 ? o[x + y] * inv : 0.0f;
+                    nan |= v[y] != v[y];
                 }
-                if (r < queries * group) store_quad(dst + 32 * d + 4 * y, make_float4(v[0], v[1], v[2], v[3]));
+                if (live) store_quad(dst + x, make_float4(v[0], v[1], v[2], v[3]));
             }
-    }
-    // rows that came out as NaN, once more from the formula
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        unsigned again = __ballot_sync(FULL, nan[h] && limit[h] > 0);
-        while (again) {
-            const int first = (__ffs(again) - 1) & ~3;       // the row's four lanes
-            again &= ~(15u << first);
-            __syncwarp();
-            const int i = __shfl_sync(FULL, i_of[h], first), n = __shfl_sync(FULL, limit[h], first);
-            const int head = it.head * group + (16 * warp + first / 4 + 8 * h) % group;
-            float4 x = load_quad(q + int64_t(it.base + i) * q_stride + int64_t(head) * HD + 4 * lane);
-            x = make_float4(x.x * ATT_SCALE, x.y * ATT_SCALE, x.z * ATT_SCALE, x.w * ATT_SCALE);
-            store_quad(out + (int64_t(it.base + i) * n_heads + head) * HD + 4 * lane,
-                       attend_row<float>(c, b, it.s, it.head, n, x, status));
+            // rows that came out as NaN, once more from the formula
+            unsigned again = __ballot_sync(FULL, live && limit > 0 && nan);
+            while (again) {
+                const int l = __ffs(again) - 1;
+                again &= again - 1;
+                __syncwarp();
+                const int il = __shfl_sync(FULL, i, l), n = __shfl_sync(FULL, limit, l), h = __shfl_sync(FULL, head, l);
+                float4 x = load_quad(q + int64_t(it.base + il) * q_stride + int64_t(h) * HD + 4 * lane);
+                x = make_float4(x.x * ATT_SCALE, x.y * ATT_SCALE, x.z * ATT_SCALE, x.w * ATT_SCALE);
+                store_quad(out + (int64_t(it.base + il) * n_heads + h) * HD + 4 * lane,
+                           attend_row<float>(c, b, it.s, it.head, n, x, status));
+            }
         }
     }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 4) tc_free512(tbase);
 }
 
 cudaError_t launch_prompt_f32(const PagedKV &c, const PagedSeqs &b, int64_t rows, const void *q, int64_t q_stride,
                               int n_heads, void *out, uint32_t *status, cudaStream_t stream) {
     const int group = n_heads / c.n_kv, qt = PF_ROWS / group;
-    CUtensorMap mk, mv;
-    if (!encode_pages_map(&mk, c.k, c, Q3CU_F32, PF_KEYS) || !encode_pages_map(&mv, c.v, c, Q3CU_F32, PF_KEYS))
-        return cudaErrorInvalidValue;
     cudaError_t e = ensure_smem_attr(reinterpret_cast<const void *>(prompt_f32_kernel), PF_SMEM, 41);
     if (e != cudaSuccess) return e;
     // no more items than this, however the rows are split into sequences
     const int64_t items = (rows / qt + b.n_seqs) * c.n_kv;
-    return launch_dependent(prompt_f32_kernel, dim3(unsigned(items)), dim3(PF_THREADS), PF_SMEM, stream, mk, mv, c, b,
-                            int(rows), static_cast<const float *>(q), q_stride, n_heads, group, FastDiv(qt),
-                            static_cast<float *>(out), status);
+    return launch_dependent(prompt_f32_kernel, dim3(unsigned(items)), dim3(PF_THREADS), PF_SMEM, stream, c, b, int(rows),
+                            static_cast<const float *>(q), q_stride, n_heads, group, FastDiv(qt), static_cast<float *>(out),
+                            status);
 }
 
 }  // namespace q3

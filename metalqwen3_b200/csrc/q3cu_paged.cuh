@@ -303,6 +303,13 @@ struct PromptOrder {
     }
 };
 
+// Scores from column n of 32 on become -inf.
+__device__ __forceinline__ void mask32(uint32_t *v, int n) {
+#pragma unroll
+    for (int y = 0; y < 32; ++y)
+        if (y >= n) v[y] = 0xff800000u;
+}
+
 constexpr float ATT_SCALE = 0.08838834764831845f;            // 1/sqrt(128)
 
 }  // namespace q3
