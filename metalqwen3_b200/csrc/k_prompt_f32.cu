@@ -23,6 +23,13 @@
 // Tensor memory (512 columns): the query's parts 0-191, two slots of 96 for scores
 // and the probabilities' parts over them, the tile's P V 384-511.
 //
+// Bound by the instructions that split, exponentiate and add, beside a tensor pipe that is busy 72 % of the cycles
+// when the prompt is long: 4,096 rows (32/8 heads) take 606 to 650 us (1.3 PFLOP/s of bf16 parts, at 1.6 GHz under
+// the power cap), 2,000 rows in three prompts (16/8) 52 us, of which the longest prompt's last block is 42.
+// Measured and left out: two threads to a row (they and the splitting warps then spill registers: 80 us for the three
+// prompts), the next tile's loads ahead of this tile's split (57 us: the splitting warps then keep the rows' warps
+// waiting for issue slots), parts by truncation in place of rounding (57 us, and a larger error).
+//
 // Masks and rows that come out as NaN are treated as in k_prompt.cu; keys and values
 // behind the sequence's end are stored as zeros.  (An infinity splits into
 // infinity and NaN, so its rows go the way of NaN rows, which ends in the formula.)
@@ -65,6 +72,14 @@ __device__ __forceinline__ void store_parts16(const float (&x)[16], uint32_t at0
     tc_st8(at0, w[0]);
     tc_st8(at1, w[1]);
     tc_st8(at2, w[2]);
+}
+
+// Eight consecutive floats, 32 bytes aligned, in one load.
+__device__ __forceinline__ void load_eight(const float *p, float4 (&v)[2]) {
+    asm volatile("ld.global.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=f"(v[0].x), "=f"(v[0].y), "=f"(v[0].z), "=f"(v[0].w), "=f"(v[1].x), "=f"(v[1].y), "=f"(v[1].z),
+                   "=f"(v[1].w)
+                 : "l"(p) : "memory");
 }
 
 __global__ void __launch_bounds__(PF_THREADS, 1)
@@ -112,26 +127,33 @@ prompt_f32_kernel(const PagedKV c, const PagedSeqs b, int rows, const float *q, 
             // ---- keys (warps 8-11) or values: 16 of a tile's rows per warp, in one page --------
             const int side = (warp - 8) >> 2, first = 16 * (warp & 3);
             const float *src = static_cast<const float *>(side ? c.v : c.k);
+            const bool wide = reinterpret_cast<uintptr_t>(src) % 32 == 0;    // (a page's stride is a multiple of 32 bytes)
             const int chunk = lane & 15, row = lane >> 4;    // elements 8 chunk .. + 7 of rows row, row + 2, ...
             uint8_t *dst = tiles + side * PF_NS * PF_TILE + (chunk >> 3) * PF_HALF;
-            auto page_of = [&](int j) -> int {
+            // a page id is loaded one tile ahead
+            auto id_of = [&](int j) -> int {
                 const int t = j * PF_KEYS + first;
-                return t < it.len ? paged_page(b, c, it.s, t, lane == 0 ? status : nullptr) : -1;
+                return t < it.len ? b.pages[int64_t(it.s) * b.max_pages + (t >> c.page_shift)] : -1;
             };
-            int page = nkv ? page_of(0) : -1;
+            int next = nkv ? id_of(0) : -1;
             for (int j = 0; j < nkv; ++j) {
-                const int st = j & 1, t = j * PF_KEYS + first;
-                const float *at = src + (page < 0 ? 0 : paged_at(c, page, it.head, t)) + 8 * chunk;
-                const int n = page < 0 ? 0 : it.len - t;     // rows from n on read as zeros
+                const int st = j & 1, t = j * PF_KEYS + first, id = next;
+                if (j + 1 < nkv) next = id_of(j + 1);
+                const bool good = id >= 0 && id < c.n_pages;
+                if (!good && t < it.len && lane == 0) flag_bad_index(status);
+                const int n = good ? it.len - t : 0;         // rows from n on read as zeros
+                const float *at = src + (good ? paged_at(c, id, it.head, t) : 0) + row * HD + 8 * chunk;
                 float4 x[8][2];
+                if (n >= 16 && wide) {
 #pragma unroll
-                for (int u = 0; u < 8; ++u)
+                    for (int u = 0; u < 8; ++u) load_eight(at + 2 * u * HD, x[u]);
+                } else {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        x[u][h] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                        if (row + 2 * u < n) x[u][h] = load_quad(at + (row + 2 * u) * HD + 4 * h);
-                    }
-                if (j + 1 < nkv) page = page_of(j + 1);
+                    for (int u = 0; u < 8; ++u)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+                            x[u][h] = 2 * u + row < n ? load_quad(at + 2 * u * HD + 4 * h) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                }
                 if (j >= PF_NS &&
                     !__all_sync(FULL, mbar_wait(&empty[side][st], uint32_t((j >> 1) - 1) & 1u, lane == 0 ? status : nullptr)))
                     break;
@@ -214,18 +236,25 @@ prompt_f32_kernel(const PagedKV c, const PagedSeqs b, int rows, const float *q, 
         bool ok = true;
         if (nkv) {
             const float *row = q + int64_t(it.base + i) * q_stride + int64_t(head) * HD;
-#pragma unroll 2
-            for (int x = 0; x < HD / 16; ++x) {
-                float v[16];
 #pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                    const float4 f = live ? load_quad(row + 16 * x + 4 * y) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    v[4 * y] = f.x;
-                    v[4 * y + 1] = f.y;
-                    v[4 * y + 2] = f.z;
-                    v[4 * y + 3] = f.w;
+            for (int z = 0; z < 2; ++z) {                    // 64 elements' loads at a time
+                float4 f[16];
+#pragma unroll
+                for (int y = 0; y < 16; ++y)
+                    f[y] = live ? load_quad(row + 64 * z + 4 * y) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    float v[16];
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) {
+                        v[4 * y] = f[4 * x + y].x;
+                        v[4 * y + 1] = f[4 * x + y].y;
+                        v[4 * y + 2] = f[4 * x + y].z;
+                        v[4 * y + 3] = f[4 * x + y].w;
+                    }
+                    const uint32_t at = lane_base + 32 * z + 8 * x;
+                    store_parts16(v, at, at + 64, at + 128);
                 }
-                store_parts16(v, lane_base + 8 * x, lane_base + 64 + 8 * x, lane_base + 128 + 8 * x);
             }
             tc_wait_st();
             tc_fence_before();
@@ -312,18 +341,29 @@ prompt_f32_kernel(const PagedKV c, const PagedSeqs b, int rows, const float *q, 
         }
         if (ok) {
             const float inv = limit > 0 ? 1.0f / sum : 0.0f;
-            float *dst = out + (int64_t(it.base + i) * n_heads + head) * HD;
             bool nan = false;
+            // through shared memory (its tiles are done with), so that a warp stores a row at a time: chunk x of the
+            // warp's row l at x ^ (l % 8)
+            uint8_t *stage = tiles + warp * 32 * (HD * 4);
 #pragma unroll
-            for (int x = 0; x < HD; x += 4) {
+            for (int x = 0; x < HD / 4; ++x) {
                 float v[4];
 #pragma unroll
                 for (int y = 0; y < 4; ++y) {
-                    v[y] = limit > 0 ? o[x + y] * inv : 0.0f;
+                    v[y] = limit > 0 ? o[4 * x + y] * inv : 0.0f;
                     nan |= v[y] != v[y];
                 }
-                if (live) store_quad(dst + x, make_float4(v[0], v[1], v[2], v[3]));
+                *reinterpret_cast<float4 *>(stage + lane * (HD * 4) + ((x ^ (lane & 7)) << 4)) = make_float4(v[0], v[1], v[2], v[3]);
             }
+            __syncwarp();
+            const unsigned lives = __ballot_sync(FULL, live);
+            for (int l = 0; l < 32; ++l) {
+                const int at = __shfl_sync(FULL, i * n_heads + head, l);     // below rows * n_heads
+                if (lives >> l & 1u)
+                    store_quad(out + (int64_t(it.base) * n_heads + at) * HD + 4 * lane,
+                               *reinterpret_cast<const float4 *>(stage + l * (HD * 4) + ((lane ^ (l & 7)) << 4)));
+            }
+            __syncwarp();
             // rows that came out as NaN, once more from the formula
             unsigned again = __ballot_sync(FULL, live && limit > 0 && nan);
             while (again) {

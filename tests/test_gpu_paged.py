@@ -451,6 +451,52 @@ def test_attention_prompt_strides_and_bad_pages(q3, dtype):
     check_attention(got, q, k, v, range(1, n + 1), dtype, H if dtype == BF16 else 0.0)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_caches_at_16_bytes(q3, dtype):
+    """Pages that begin 16 bytes behind a 32-byte boundary, which is all that is asked for."""
+    n, off16 = 150, 16 // torch.empty((), dtype=dtype).element_size()
+    p = Paged([n], 2, 16, dtype, seed=70).fill(71)
+    for name in ("k", "v"):
+        x = getattr(p, name)
+        buf = torch.full((x.numel() + off16,), NAN, dtype=dtype, device="cuda")
+        moved = buf[off16:].view(x.shape)
+        assert buf.data_ptr() % 32 == 0 and moved.data_ptr() % 32 == 16
+        moved.copy_(x)
+        setattr(p, name, moved)
+    q = queries(n, 8, dtype, 72)
+    check_attention(q3.attention_prompt(*p.handles([0, n]), q), q, *p.rows(0), range(1, n + 1), dtype,
+                    H if dtype == BF16 else 0.0)
+    check_attention(q3.attention_paged(*p.handles(), q[-1:]), q[-1:], *p.rows(0), [n], dtype)
+    x, w, at = queries(n, 8, dtype, 73), torch.ones(128, device="cuda"), torch.arange(n, device="cuda")
+    k, v = x[:, 4:6], x[:, 6:]
+    got = q3.kv_append(*p.handles([0, n]), x[:, :4], k, v, w, w)
+    check_rotated(got, x[:, :4], w, at, dtype)
+    check_rotated(p.rows(0)[0].to(dtype), k, w, at, dtype)
+    assert torch.equal(p.rows(0)[1], v.double())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attention_prompt_infinities(q3, dtype):
+    """An infinite key element makes a score -inf (weight 0) or +inf (a row of NaN), an infinite value one column."""
+    n = 130
+    p = Paged([n], 2, 16, dtype, seed=74).fill(75)
+    q = queries(n, 4, dtype, 76)
+    page, slot = p.where(0, [70])
+    p.k[page, 0, slot, 5] = math.inf
+    p.v[page, 1, slot, 9] = math.inf
+    got, (k, v) = q3.attention_prompt(*p.handles([0, n]), q).double(), p.rows(0)
+    rounding = H if dtype == BF16 else 0.0
+    up = (q[:, :2, 5] > 0) & (torch.arange(n, device="cuda") >= 70)[:, None]
+    assert up.any() and (~up).any() and got[:, :2][up].isnan().all()
+    for h in range(2):
+        keep = (~up[:, h]).nonzero()[:, 0]
+        check_attention(got[keep, h:h + 1], q[keep, h:h + 1], k[:, :1], v[:, :1], keep + 1, dtype, rounding)
+    assert (got[70:, 2:, 9] == math.inf).all()
+    v[70, 1, 9] = 0.0
+    got[70:, 2:, 9] = attend(q[70:, 2:].double(), k[:, 1:], v[:, 1:], range(71, n + 1))[0][:, :, 9]
+    check_attention(got[:, 2:], q[:, 2:], k[:, 1:], v[:, 1:], range(1, n + 1), dtype, rounding)
+
+
 def test_offsets_that_do_not_rise(q3):
     """Broken row offsets touch nothing outside the rows and fault nothing."""
     p = Paged([50, 50, 50], 2, 16, BF16, seed=43).fill(44)
