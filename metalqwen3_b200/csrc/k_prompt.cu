@@ -545,10 +545,17 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
     if (warp == 8) tc_free512(tbase);
 }
 
+// An SM holds one CTA, and a cluster lies within one group of SMs, so a few SMs of each group stay over.
+int prompt_cluster(int64_t items, int64_t tiles, int sms) {
+    int ctas = 1;
+    while (ctas < 8 && 2 * ctas * items <= sms - sms / 8 && 2 * ctas <= tiles / PROMPT_PART) ctas *= 2;
+    return ctas;
+}
+
 cudaError_t launch_attention_prompt(const PagedKV &c, const PagedSeqs &b, int64_t rows, const void *q, q3cu_dtype dt,
                                     int64_t q_stride, int n_heads, void *out, uint32_t *status, cudaStream_t stream,
                                     int sms) {
-    if (dt == Q3CU_F32) return launch_prompt_f32(c, b, rows, q, q_stride, n_heads, out, status, stream);
+    if (dt == Q3CU_F32) return launch_prompt_f32(c, b, rows, q, q_stride, n_heads, out, status, stream, sms);
     const int group = n_heads / c.n_kv, qt = PT_ROWS / group;
     CUtensorMap mq, mk, mv;
     const uint64_t dims[3] = {HD, uint64_t(n_heads), uint64_t(rows)};

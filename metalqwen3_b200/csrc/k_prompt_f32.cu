@@ -23,6 +23,10 @@
 // Tensor memory (512 columns): the query's parts 0-191, two slots of 96 for scores
 // and the probabilities' parts over them, the tile's P V 384-511.
 //
+// With fewer items than SMs a cluster of up to eight CTAs takes an item, each a part of its key tiles, and joins the
+// parts through shared memory (join_parts): 16 rows behind 8,000 positions (32/8 heads) 260 -> 45 us, 30 behind 30,000
+// 1,140 -> 150 us.
+//
 // Bound by the instructions that split, exponentiate and add, beside a tensor pipe that is busy 72 % of the cycles
 // when the prompt is long: 4,096 rows (32/8 heads) take 606 to 650 us (1.3 PFLOP/s of bf16 parts, at 1.6 GHz under
 // the power cap), 2,000 rows in three prompts (16/8) 52 us, of which the longest prompt's last block is 42.
@@ -82,14 +86,16 @@ __device__ __forceinline__ void load_eight(const float *p, float4 (&v)[2]) {
                  : "l"(p) : "memory");
 }
 
+template <bool SPLIT>
 __global__ void __launch_bounds__(PF_THREADS, 1)
 prompt_f32_kernel(const PagedKV c, const PagedSeqs b, int rows, const float *q, int64_t q_stride, int n_heads, int group,
-                  const FastDiv per_block, float *out, uint32_t *status) {
+                  const FastDiv per_block, int ctas, float *out, uint32_t *status) {
     extern __shared__ uint8_t pf_dyn[];
     uint8_t *tiles = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(pf_dyn) + 1023) & ~uintptr_t(1023));
     // tiles of keys (side 0) and values (side 1), two stages each
     __shared__ __align__(8) uint64_t full[2][PF_NS], empty[2][PF_NS], q_full, s_full[2], p_full, o_full, drain;
     __shared__ PromptItem item_sh;
+    __shared__ float2 stat_sh[SPLIT ? PF_ROWS : 1];          // maximum and sum of a shared item's rows
     __shared__ uint32_t tmem_sh;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -109,7 +115,7 @@ prompt_f32_kernel(const PagedKV c, const PagedSeqs b, int rows, const float *q, 
     if (warp == 4) tc_alloc512(&tmem_sh);
     griddep_wait();
     if (warp == 8) {
-        const PromptItem found = PromptOrder(b, c, rows, per_block, PF_KEYS, status).find(blockIdx.x);
+        const PromptItem found = PromptOrder(b, c, rows, per_block, PF_KEYS, status).find(SPLIT ? blockIdx.x / unsigned(ctas) : blockIdx.x);
         if (lane == 0) item_sh = found;
     }
     tc_fence_before();
@@ -117,8 +123,14 @@ prompt_f32_kernel(const PagedKV c, const PagedSeqs b, int rows, const float *q, 
     tc_fence_after();
     const uint32_t tbase = tmem_sh;
     const PromptItem it = item_sh;
-    const int queries = it.s < 0 ? 0 : min(per_block.d, it.rows - it.first);
-    const int nkv = it.s < 0 ? 0 : (it.seen(it.first + queries - 1) + PF_KEYS - 1) / PF_KEYS;
+    const int block_queries = it.s < 0 ? 0 : min(per_block.d, it.rows - it.first);
+    const int tiles_all = it.s < 0 ? 0 : (it.seen(it.first + block_queries - 1) + PF_KEYS - 1) / PF_KEYS;
+    // this CTA's part of the item's key tiles: nkv from j0 on
+    const int rank = SPLIT ? int(blockIdx.x % unsigned(ctas)) : 0, parts = SPLIT ? prompt_parts(ctas, tiles_all) : 1;
+    const bool mine = rank < parts;
+    const int j0 = SPLIT && mine ? prompt_part(tiles_all, parts, rank) : 0;
+    const int nkv = !SPLIT ? tiles_all : mine ? prompt_part(tiles_all, parts, rank + 1) - j0 : 0;
+    const int queries = mine ? block_queries : 0;
 
     // Registers move to the rows: 128 threads x 224 + 384 x 96 is the launch's 512 x 128.
     if (warp >= 4) {
@@ -132,12 +144,12 @@ prompt_f32_kernel(const PagedKV c, const PagedSeqs b, int rows, const float *q, 
             uint8_t *dst = tiles + side * PF_NS * PF_TILE + (chunk >> 3) * PF_HALF;
             // a page id is loaded one tile ahead
             auto id_of = [&](int j) -> int {
-                const int t = j * PF_KEYS + first;
+                const int t = (j0 + j) * PF_KEYS + first;
                 return t < it.len ? b.pages[int64_t(it.s) * b.max_pages + (t >> c.page_shift)] : -1;
             };
             int next = nkv ? id_of(0) : -1;
             for (int j = 0; j < nkv; ++j) {
-                const int st = j & 1, t = j * PF_KEYS + first, id = next;
+                const int st = j & 1, t = (j0 + j) * PF_KEYS + first, id = next;
                 if (j + 1 < nkv) next = id_of(j + 1);
                 const bool good = id >= 0 && id < c.n_pages;
                 if (!good && t < it.len && lane == 0) flag_bad_index(status);
@@ -281,8 +293,8 @@ prompt_f32_kernel(const PagedKV c, const PagedSeqs b, int rows, const float *q, 
             if (!ok) break;
             tc_fence_after();
             const uint32_t slot = lane_base + PF_SLOT + 96 * (j & 1);
-            const int left = limit - j * PF_KEYS;            // columns of this tile that the row sees
-            const bool mask = (j + 1) * PF_KEYS > sure;
+            const int left = limit - (j0 + j) * PF_KEYS;            // columns of this tile that the row sees
+            const bool mask = (j0 + j + 1) * PF_KEYS > sure;
             float tile_max = -INFINITY;
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
@@ -340,7 +352,7 @@ prompt_f32_kernel(const PagedKV c, const PagedSeqs b, int rows, const float *q, 
             }
         }
         if (ok) {
-            const float inv = limit > 0 ? 1.0f / sum : 0.0f;
+            const float inv = SPLIT && parts > 1 ? 1.0f : limit > 0 ? 1.0f / sum : 0.0f;
             bool nan = false;
             // through shared memory (its tiles are done with), so that a warp stores a row at a time: chunk x of the
             // warp's row l at x ^ (l % 8)
@@ -356,7 +368,7 @@ prompt_f32_kernel(const PagedKV c, const PagedSeqs b, int rows, const float *q, 
                 *reinterpret_cast<float4 *>(stage + lane * (HD * 4) + ((x ^ (lane & 7)) << 4)) = make_float4(v[0], v[1], v[2], v[3]);
             }
             __syncwarp();
-            const unsigned lives = __ballot_sync(FULL, live);
+            const unsigned lives = __ballot_sync(FULL, live && !(SPLIT && parts > 1));
             for (int l = 0; l < 32; ++l) {
                 const int at = __shfl_sync(FULL, i * n_heads + head, l);     // below rows * n_heads
                 if (lives >> l & 1u)
@@ -365,7 +377,7 @@ prompt_f32_kernel(const PagedKV c, const PagedSeqs b, int rows, const float *q, 
             }
             __syncwarp();
             // rows that came out as NaN, once more from the formula
-            unsigned again = __ballot_sync(FULL, live && limit > 0 && nan);
+            unsigned again = __ballot_sync(FULL, live && limit > 0 && nan && !(SPLIT && parts > 1));
             while (again) {
                 const int l = __ffs(again) - 1;
                 again &= again - 1;
@@ -377,23 +389,47 @@ prompt_f32_kernel(const PagedKV c, const PagedSeqs b, int rows, const float *q, 
                            attend_row<float>(c, b, it.s, it.head, n, x, status));
             }
         }
+        if constexpr (SPLIT) stat_sh[r] = make_float2(m, ok ? sum : -1.0f);
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     if (warp == 4) tc_free512(tbase);
+    if constexpr (SPLIT) {
+        if (parts == 1 || !mine) return;                     // the same for all of a part's threads
+        cluster_sync();
+        for (int r = prompt_part(PF_ROWS, parts, rank) + warp; r < prompt_part(PF_ROWS, parts, rank + 1); r += PF_THREADS / 32) {
+            const int query = r / group, i = it.first + query, head = it.head * group + r - query * group;
+            if (query >= queries) break;
+            const int limit = it.seen(i);
+            bool ok;
+            float4 v = join_parts(smem_addr(tiles) + r * (HD * 4), smem_addr(&stat_sh[r]), r, parts, PF_LOG2, ok);
+            if (!ok) continue;
+            float *dst = out + (int64_t(it.base + i) * n_heads + head) * HD + 4 * lane;
+            if (limit <= 0) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (__any_sync(FULL, v.x != v.x || v.y != v.y || v.z != v.z || v.w != v.w)) {
+                const float4 x = load_quad(q + int64_t(it.base + i) * q_stride + int64_t(head) * HD + 4 * lane);
+                v = attend_row<float>(c, b, it.s, it.head, limit,
+                                      make_float4(x.x * ATT_SCALE, x.y * ATT_SCALE, x.z * ATT_SCALE, x.w * ATT_SCALE), status);
+            }
+            store_quad(dst, v);
+        }
+        cluster_sync();                                      // no CTA's shared memory goes while others read it
+    }
 }
 
 cudaError_t launch_prompt_f32(const PagedKV &c, const PagedSeqs &b, int64_t rows, const void *q, int64_t q_stride,
-                              int n_heads, void *out, uint32_t *status, cudaStream_t stream) {
+                              int n_heads, void *out, uint32_t *status, cudaStream_t stream, int sms) {
     const int group = n_heads / c.n_kv, qt = PF_ROWS / group;
-    cudaError_t e = ensure_smem_attr(reinterpret_cast<const void *>(prompt_f32_kernel), PF_SMEM, 41);
-    if (e != cudaSuccess) return e;
     // no more items than this, however the rows are split into sequences
     const int64_t items = (rows / qt + b.n_seqs) * c.n_kv;
-    return launch_dependent(prompt_f32_kernel, dim3(unsigned(items)), dim3(PF_THREADS), PF_SMEM, stream, c, b, int(rows),
-                            static_cast<const float *>(q), q_stride, n_heads, group, FastDiv(qt), static_cast<float *>(out),
-                            status);
+    const int ctas = prompt_cluster(items, (int64_t(b.max_pages) << c.page_shift) / PF_KEYS, sms);
+    auto kernel = ctas > 1 ? prompt_f32_kernel<true> : prompt_f32_kernel<false>;
+    cudaError_t e = ensure_smem_attr(reinterpret_cast<const void *>(kernel), PF_SMEM, ctas > 1 ? 42 : 41);
+    if (e != cudaSuccess) return e;
+    return launch_clusters(kernel, ctas, dim3(unsigned(items * ctas)), dim3(PF_THREADS), PF_SMEM, stream, c, b, int(rows),
+                           static_cast<const float *>(q), q_stride, n_heads, group, FastDiv(qt), ctas,
+                           static_cast<float *>(out), status);
 }
 
 }  // namespace q3

@@ -26,20 +26,29 @@ cudaError_t ensure_smem_attr(const void *kernel, size_t bytes, int slot);
 // earlier launch writes or reads (every thread that does, on every path), and
 // griddep_launch_dependents() where its own successor may start.  When the
 // previous work is not a kernel the launch behaves as an ordinary one.
+// In clusters of `cluster` CTAs where that is more than one.
 template <typename... KArgs, typename... Args>
-cudaError_t launch_dependent(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
-                             Args... args) {
+cudaError_t launch_clusters(void (*kernel)(KArgs...), int cluster, dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                            Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = unsigned(cluster);
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+template <typename... KArgs, typename... Args>
+cudaError_t launch_dependent(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                             Args... args) {
+    return launch_clusters(kernel, 1, grid, block, smem, stream, args...);
 }
 
 // The failure-path self-test: one CTA whose bounded wait on a barrier that
@@ -174,7 +183,10 @@ cudaError_t launch_attention_prompt(const PagedKV &c, const PagedSeqs &b, int64_
                                     int64_t q_stride, int n_heads, void *out, uint32_t *status, cudaStream_t stream,
                                     int sms);
 cudaError_t launch_prompt_f32(const PagedKV &c, const PagedSeqs &b, int64_t rows, const void *q, int64_t q_stride,
-                              int n_heads, void *out, uint32_t *status, cudaStream_t stream);
+                              int n_heads, void *out, uint32_t *status, cudaStream_t stream, int sms);
+// CTAs that share an item of a prompt launch of at most `items` items, each with no more than `tiles` key tiles: 1, 2, 4
+// or 8.
+int prompt_cluster(int64_t items, int64_t tiles, int sms);
 
 cudaError_t launch_swiglu(const void *hb, const void *hb2, q3cu_dtype dt, int64_t elems, void *out, int8_t *q,
                           float *s, uint32_t *status, cudaStream_t stream, int sms);

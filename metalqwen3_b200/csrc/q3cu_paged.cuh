@@ -303,6 +303,54 @@ struct PromptOrder {
     }
 };
 
+// ---- items that a cluster shares --------------------------------------------------------------
+// When there are fewer items than SMs, a cluster of CTAs takes an item: part p of its key tiles goes to the CTA of rank
+// p, and the parts' unnormalised results are joined through the cluster's shared memory.  A part has at least
+// PROMPT_PART tiles.
+constexpr int PROMPT_PART = 4;
+__host__ __device__ __forceinline__ int prompt_parts(int ctas, int tiles) {
+    const int most = tiles / PROMPT_PART;
+    return most < 1 ? 1 : most < ctas ? most : ctas;
+}
+// First tile of part p (of `parts`: behind the last).
+__host__ __device__ __forceinline__ int prompt_part(int tiles, int parts, int p) { return int(int64_t(tiles) * p / parts); }
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t peer_smem(uint32_t addr, int rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+// A row of `parts` parts by one warp: its results lie, 16-byte chunk x of the 128 floats at x ^ (r % 8), at `row` of each
+// CTA's shared memory, and (maximum, sum) at `stat`; a negative sum marks a part that was given up, which makes `ok`
+// false.  Returns lane's chunk; `scale` makes scores base-2 exponents.
+__device__ __forceinline__ float4 join_parts(uint32_t row, uint32_t stat, int r, int parts, float scale, bool &ok) {
+    const int lane = threadIdx.x & 31;
+    float m = -INFINITY, l = 0.0f;
+    if (lane < parts)
+        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(m), "=f"(l) : "r"(peer_smem(stat, lane)) : "memory");
+    ok = !__any_sync(FULL, l < 0.0f);
+    float top = m;
+#pragma unroll
+    for (int x = 4; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, x));
+    const float w = m == -INFINITY ? 0.0f : ex2_approx_ftz((m - top) * scale);
+    float sum = w * l;
+#pragma unroll
+    for (int x = 4; x > 0; x >>= 1) sum += __shfl_xor_sync(FULL, sum, x);
+    const float inv = 1.0f / __shfl_sync(FULL, sum, 0);
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int p = 0; p < parts; ++p) {
+        const float f = __shfl_sync(FULL, w, p);
+        float4 v;
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                     : "r"(peer_smem(row + uint32_t((lane ^ (r & 7)) << 4), p)) : "memory");
+        o = make_float4(fmaf(f, v.x, o.x), fmaf(f, v.y, o.y), fmaf(f, v.z, o.z), fmaf(f, v.w, o.w));
+    }
+    return make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+}
+
 // Scores from column n of 32 on become -inf.
 __device__ __forceinline__ void mask32(uint32_t *v, int n) {
 #pragma unroll

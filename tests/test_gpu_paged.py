@@ -497,6 +497,75 @@ def test_attention_prompt_infinities(q3, dtype):
     check_attention(got[:, 2:], q[:, 2:], k[:, 1:], v[:, 1:], range(1, n + 1), dtype, rounding)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("heads,n_kv,page,rows,lens", [
+    (32, 8, 16, [16], [1000]), (16, 1, 64, [100], [3001]), (8, 2, 16, [70, 3, 0, 5], [900, 2000, 40, 5]),
+    (4, 4, 32, [500], [500]), (5, 1, 256, [37, 1], [2600, 4097]), (12, 4, 16, [33], [513]), (2, 2, 128, [1], [6000]),
+    (16, 8, 16, [40, 30], [20, 1100]), (32, 8, 16, [65], [2111]), (8, 8, 16, [3, 3], [1500, 700]),
+])
+def test_attention_prompt_few_rows_many_keys(q3, dtype, heads, n_kv, page, rows, lens):
+    """Few items, whose keys several multiprocessors share."""
+    p = Paged(lens, n_kv, page, dtype, seed=80).fill(81)
+    q = queries(sum(rows), heads, dtype, 82)
+    off = offsets(rows)
+    out = torch.full(q.shape, 3.0, dtype=dtype, device="cuda")
+    q3.attention_prompt(*p.handles(off), q, out=out)
+    for s, n in enumerate(lens):
+        a, b = off[s], off[s + 1]
+        seen = [max(0, n - rows[s] + i + 1) for i in range(rows[s])]
+        check_attention(out[a:b], q[a:b], *p.rows(s), seen, dtype, H if dtype == BF16 else 0.0)
+    again = q3.attention_prompt(*p.handles(off), q)
+    assert torch.equal(again, out) and q3.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attention_prompt_few_rows_bad_pages_and_nan(q3, dtype):
+    """Of keys that several multiprocessors share: a page outside the cache reads as zeros, a NaN at a hidden position
+    stays hidden and one that is seen shows in its rows."""
+    from metalqwen3_b200.q3cu import DEV_BAD_INDEX
+    n, rows = 2000, 20
+    p = Paged([n], 2, 16, dtype, seed=83).fill(84)
+    k, v = p.rows(0)
+    for i, bad in ((3, -1), (60, 1 << 29), (120, p.n_pages)):
+        p.table[0, i] = bad
+        k[16 * i:16 * i + 16] = 0
+        v[16 * i:16 * i + 16] = 0
+    page, slot = p.where(0, [n - 8])
+    p.k[page, 0, slot, 7] = NAN
+    p.v[page, 1, slot, 3] = NAN
+    q = queries(rows, 8, dtype, 85)
+    got = q3.attention_prompt(*p.handles([0, rows]), q)
+    assert q3.device_status() == DEV_BAD_INDEX and q3.device_status() == 0
+    seen = torch.arange(n - rows + 1, n + 1)
+    before = rows - 8                                        # rows that end before position n - 8
+    check_attention(got[:before], q[:before], k, v, seen[:before], dtype, H if dtype == BF16 else 0.0)
+    assert got[before:, :4].isnan().all() and got[before:, 4:, 3].isnan().all()
+    got[before:, 4:, 3] = 0.0
+    assert not got[before:, 4:].isnan().any()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_captured_few_rows_replayed(q3, dtype):
+    """A captured call is replayed while the sequences grow from a few keys, which one multiprocessor takes, to many."""
+    p = Paged([3000, 1200], 2, 16, dtype, seed=86).fill(87)
+    cache, batch = p.handles([0, 9, 14])
+    q = queries(14, 8, dtype, 88)
+    out = torch.zeros_like(q)
+    q3.attention_prompt(cache, batch, q, out=out)
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        q3.attention_prompt(cache, batch, q, out=out)
+    for lens in ((9, 5), (300, 1200), (3000, 40), (1030, 520), (0, 3)):
+        p.kv_len.copy_(torch.tensor(lens, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        for s, (a, b) in enumerate(((0, 9), (9, 14))):
+            k, v = p.rows(s)
+            seen = [max(0, lens[s] - (b - a) + i + 1) for i in range(b - a)]
+            check_attention(out[a:b], q[a:b], k[:lens[s]], v[:lens[s]], seen, dtype, H if dtype == BF16 else 0.0)
+
+
 def test_offsets_that_do_not_rise(q3):
     """Broken row offsets touch nothing outside the rows and fault nothing."""
     p = Paged([50, 50, 50], 2, 16, BF16, seed=43).fill(44)
