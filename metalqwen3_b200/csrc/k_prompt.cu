@@ -38,6 +38,10 @@
 // to 8,192 (32/8) 178 us, 988 TFLOP/s; 4,096 rows in six prompts (32/8) 50 us.
 // Tensor memory (512 columns): S0, S1, O0, O1; P_t lies over the first half of S_t.
 //
+// With few items (prompt_tc_kernel<true>) a cluster of up to eight CTAs takes one, each a part of its key tiles, and joins
+// the parts through shared memory (join_parts): 16 rows behind 8,000 positions (32/8 heads) 120 -> 26 us, 100 rows
+// behind 8,000 138 -> 38 us, 30 behind 30,000 440 -> 69 us.
+//
 // Masks: keys at and beyond the row's limit become -inf before the maximum.
 // Their probability is exactly 0, but 0 times a NaN or an infinity in V is not:
 // the values behind the sequence's end (never written, anything may be there) are
@@ -51,10 +55,14 @@
 #include "q3cu_tcgen05.cuh"
 #include "q3cu_tma.h"
 
+#include <atomic>
+#include <type_traits>
+
 namespace q3 {
 
 constexpr int PT_ROWS = 128, PT_KEYS = 128;                  // rows of a tile, keys of a tile
 constexpr int PT_THREADS = 12 * 32;
+constexpr int PT_WHOLE = 8;                                  // key tiles from which on an item may be shared
 constexpr int PT_NS = 5;                                     // K / V buffers in flight
 constexpr uint32_t PT_HALF = PT_ROWS * 128;                  // bytes of 128 rows x 64 elements
 constexpr uint32_t PT_TILE = 2 * PT_HALF;                    // 32 KB
@@ -91,6 +99,13 @@ constexpr int PT_POLY = 8;                                   // one pair of expo
 // The item of a round, as warp 9 announces it (s < 0: no more), with the key tiles of each row tile.
 struct PromptRound : PromptItem {
     int nt[2];
+    __device__ __forceinline__ int from() const { return 0; }
+};
+// Of an item that `parts` CTAs share: nt counts this CTA's key tiles, the first of which is j0.  (One that has no part
+// has no rows either.)
+struct PromptShare : PromptItem {
+    int nt[2], j0, parts;
+    __device__ __forceinline__ int from() const { return j0; }
 };
 // Asks for the work of a CTA of this launch that has not started (it then never does); the answer arrives on `bar`
 // (16 bytes).  After an answer of none, nothing more may be asked.
@@ -117,17 +132,20 @@ struct RingAt {
     }
 };
 
+// SPLIT: clusters of `ctas` CTAs, each with one item.
+template <bool SPLIT>
 __global__ void __launch_bounds__(PT_THREADS, 1)
 prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
                  const __grid_constant__ CUtensorMap tmv, const PagedKV c, const PagedSeqs b, int rows,
                  const uint16_t *q, int64_t q_stride, int n_heads, int group, const FastDiv per_block,
-                 const FastDiv by_group, uint16_t *out, uint32_t *status) {
+                 const FastDiv by_group, int ctas, uint16_t *out, uint32_t *status) {
+    typedef typename std::conditional<SPLIT, PromptShare, PromptRound>::type Round;
     extern __shared__ uint8_t pt_dyn[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(pt_dyn) + 1023) & ~uintptr_t(1023));
     uint8_t *ring = smem + 2 * PT_TILE;
     __shared__ __align__(8) uint64_t q_full, q_empty, full[PT_NS], empty[PT_NS], s_full[2], p_full[2][2], o_full[2],
         o_empty[2], item_full[2], item_empty[2], taken, tail_go, tail, drain;
-    __shared__ PromptRound item_sh[2];
+    __shared__ Round item_sh[2];
     __shared__ ulonglong2 taken_sh;
     __shared__ uint32_t tmem_sh;
 
@@ -162,8 +180,9 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
     griddep_wait();
 
     const int qt = PT_ROWS / group;                          // queries of a tile
+    float2 stat = make_float2(-INFINITY, -1.0f);             // SPLIT: maximum and sum of this thread's row, -1: given up
     // the item of a round, copied from its announcement; false after the last, or if a wait gave up
-    auto next_item = [&](int round, PromptRound &it, bool whole_warp) -> bool {
+    auto next_item = [&](int round, Round &it, bool whole_warp) -> bool {
         bool ok = mbar_wait(&item_full[round & 1], uint32_t(round >> 1) & 1u, !whole_warp || lane == 0 ? status : nullptr);
         if (whole_warp) ok = __all_sync(FULL, ok);
         if (!ok) return false;
@@ -185,18 +204,19 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
             int entries = 0, qs = 0;                         // copies of tiles and of Q so far
             bool ok = true;
             PromptOrder order(b, c, rows, per_block, PT_KEYS, status);
-            PromptItem item = order.find(blockIdx.x);
+            PromptItem item = order.find(SPLIT ? blockIdx.x / unsigned(ctas) : blockIdx.x);
             // The first item is this CTA's own; the others are those of CTAs that have not started.  One is taken over
             // when the copies for the item before are nearly all under way: no earlier, so that the CTA that is done
             // first gets the next item, and no later, since finding it takes some thousand cycles.
             auto take_over = [&](int round) -> PromptItem {
+                PromptItem none;
+                none.s = -1;
+                if constexpr (SPLIT) return none;
                 if (lane == 0) {
                     fence_proxy_async_smem();
                     mbar_arrive_expect_tx(&taken, 16);
                     take_over_cta(&taken_sh, &taken);
                 }
-                PromptItem none;
-                none.s = -1;
                 ok = __all_sync(FULL, mbar_wait(&taken, uint32_t(round) & 1u, lane == 0 ? status : nullptr));
                 if (!ok) return none;
                 const int64_t index = taken_cta(taken_sh);
@@ -204,12 +224,21 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                 return index < 0 ? none : order.find(index);
             };
             for (int round = 0; ok; ++round) {
-                PromptRound it;
+                Round it;
                 static_cast<PromptItem &>(it) = item;
                 it.nt[0] = it.nt[1] = 0;
                 for (int t = 0; t < 2 && it.s >= 0; ++t) {
                     const int first = it.first + t * qt, last = min(first + qt, it.rows) - 1;
                     if (last >= first) it.nt[t] = (it.seen(last) + PT_KEYS - 1) / PT_KEYS;
+                }
+                if constexpr (SPLIT) {
+                    const int all = max(it.nt[0], it.nt[1]), rank = int(blockIdx.x % unsigned(ctas));
+                    it.parts = it.s < 0 ? 1 : prompt_parts(ctas, all, PT_WHOLE);
+                    const bool mine = rank < it.parts;
+                    it.j0 = mine ? prompt_part(all, it.parts, rank) : 0;
+                    const int end = mine ? prompt_part(all, it.parts, rank + 1) : 0;
+                    for (int t = 0; t < 2; ++t) it.nt[t] = max(min(it.nt[t], end) - it.j0, 0);
+                    if (!mine) it.rows = 0;
                 }
                 if (round >= 2)
                     ok = __all_sync(FULL, mbar_wait(&item_empty[round & 1], uint32_t((round >> 1) - 1) & 1u,
@@ -227,7 +256,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                     continue;
                 }
                 auto page_of = [&](int j) -> int {           // n_pages reads as zeros
-                    const int t = j * PT_KEYS + box * br;
+                    const int t = (it.from() + j) * PT_KEYS + box * br;
                     if (half > 1 || t >= it.len) return c.n_pages;
                     const int p = paged_page(b, c, it.s, t, status);
                     return p < 0 ? c.n_pages : p;
@@ -249,7 +278,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                 __syncwarp();
                 for (int j = 0; j < nkv && ok; ++j) {
                     const int next = j + 1 < nkv ? page_of(j + 1) : 0;
-                    const int slot = (j * PT_KEYS + box * br) & ((1 << c.page_shift) - 1);
+                    const int slot = ((it.from() + j) * PT_KEYS + box * br) & ((1 << c.page_shift) - 1);
                     for (int kv = 0; kv < 2; ++kv) {
                         if (entries >= PT_NS) ok = mbar_wait(&empty[at.st], at.ph ^ 1u, lane == 0 ? status : nullptr);
                         ok = __all_sync(FULL, ok);
@@ -296,7 +325,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                 int qs = 0, tails = 0;
                 uint32_t steps[2] = {0, 0}, outs[2] = {0, 0};                // key tiles and results of each row tile so far
                 bool ok = true;
-                PromptRound it;
+                Round it;
                 for (int round = 0; ok && next_item(round, it, false); ++round) {
                     const int nkv = max(it.nt[0], it.nt[1]);
                     if (nkv == 0) continue;
@@ -311,9 +340,9 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                     for (int j = 0; j < nkv; ++j) {
                         const RingAt v = at;
                         at.next();                           // K(j + 1), or the next item's K(0)
-                        if (j == max(0, nkv - 2) && it.len < nkv * PT_KEYS) mbar_arrive(&tail_go);
+                        if (j == max(0, nkv - 2) && it.len < (it.from() + nkv) * PT_KEYS) mbar_arrive(&tail_go);
                         if (!(ok = mbar_wait(&full[v.st], v.ph, status))) break;
-                        if (j == nkv - 1 && it.len < nkv * PT_KEYS)           // cleared behind the sequence's end
+                        if (j == nkv - 1 && it.len < (it.from() + nkv) * PT_KEYS)     // cleared behind the sequence's end
                             if (!(ok = mbar_wait(&tail, uint32_t(tails++) & 1u, status))) break;
 #pragma unroll
                         for (int t = 0; t < 2; ++t) {
@@ -355,13 +384,13 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
             __syncwarp();
         } else if (warp == 10) {
             // ---- values behind a sequence's end: zeros -----------------------------------------
-            PromptRound it;
+            Round it;
             int entries = 0, tails = 0;                      // of the ring, and cleared ends, in the items so far
             bool ok = true;
             for (int round = 0; ok && next_item(round, it, true); ++round) {
                 const int nkv = max(it.nt[0], it.nt[1]);
                 entries += 2 * nkv;
-                if (it.len >= nkv * PT_KEYS || nkv == 0) continue;
+                if (it.len >= (it.from() + nkv) * PT_KEYS || nkv == 0) continue;
                 // The last tile's values.  The products are at the tile before, so the buffer's earlier use is over and
                 // the parity means this one.
                 const int last = entries - 1, st = last % PT_NS;
@@ -369,7 +398,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                 if (!ok) break;
                 ok = __all_sync(FULL, mbar_wait(&full[st], uint32_t(last / PT_NS) & 1u, lane == 0 ? status : nullptr));
                 if (!ok) break;
-                for (int x = (it.len - (nkv - 1) * PT_KEYS) * 8 + lane; x < PT_KEYS * 8; x += 32)
+                for (int x = (it.len - (it.from() + nkv - 1) * PT_KEYS) * 8 + lane; x < PT_KEYS * 8; x += 32)
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
                         *reinterpret_cast<uint4 *>(ring + st * PT_TILE + h * PT_HALF + x * 16) = make_uint4(0, 0, 0, 0);
@@ -389,7 +418,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
         const bool r_used = r < qt * group;
         uint32_t steps = 0, outs = 0;                        // key tiles and results so far
         bool ok = true;
-        PromptRound it;
+        Round it;
         for (int round = 0; ok && next_item(round, it, true); ++round) {
             const int nt = it.nt[t], i = it.first + r_query; // i: the sequence's row
             const bool live = r_used && i < it.rows;
@@ -405,9 +434,9 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                 for (int x = 0; x < 4; ++x) tc_ld32(ts + 32 * x, u + 32 * x);
 #pragma unroll
                 for (int x = 0; x < 4; ++x) tc_wait_ld32(u + 32 * x);
-                if ((j + 1) * PT_KEYS > sure) {
+                if ((it.from() + j + 1) * PT_KEYS > sure) {
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) mask32(u + 32 * x, limit - j * PT_KEYS - 32 * x);
+                    for (int x = 0; x < 4; ++x) mask32(u + 32 * x, limit - (it.from() + j) * PT_KEYS - 32 * x);
                 }
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -470,6 +499,10 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
             if (nt > 0 && ok) {
                 ok = __all_sync(FULL, mbar_wait(&o_full[t], outs++ & 1u, lane == 0 ? status : nullptr));
                 tc_fence_after();
+            }
+            if constexpr (SPLIT) {
+                if (ok) stat = make_float2(m, sum);
+                if (it.parts > 1) continue;                  // joined below
             }
             if (ok) {
                 const float inv = limit > 0 ? 1.0f / sum : 0.0f;
@@ -542,20 +575,94 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    if constexpr (SPLIT) {
+        const Round it = item_sh[0];
+        const int rank = int(blockIdx.x % unsigned(ctas));
+        if (it.parts > 1 && rank < it.parts) {               // the same for all of the CTA
+            float2 *stats = reinterpret_cast<float2 *>(smem);
+            if (warp < 8) {                                  // the rows' results, 128 KB in the ring's place
+                stats[threadIdx.x] = stat;
+                const int t = warp >> 2;
+                uint8_t *row = ring + threadIdx.x * (HD * 4);
+#pragma unroll 1
+                for (int x = 0; x < 4; ++x) {
+                    uint32_t o[32];
+                    if (it.nt[t]) {
+                        tc_ld32(tbase + (uint32_t(32 * (warp & 3)) << 16) + 256 + t * 128 + 32 * x, o);
+                        tc_wait_ld32(o);
+                    } else {
+#pragma unroll
+                        for (int y = 0; y < 32; ++y) o[y] = 0u;
+                    }
+#pragma unroll
+                    for (int y = 0; y < 8; ++y)
+                        *reinterpret_cast<uint4 *>(row + (((8 * x + y) ^ (lane & 7)) << 4)) =
+                            make_uint4(o[4 * y], o[4 * y + 1], o[4 * y + 2], o[4 * y + 3]);
+                }
+                tc_fence_before();
+            }
+            cluster_sync();
+            for (int r = prompt_part(2 * PT_ROWS, it.parts, rank) + warp; r < prompt_part(2 * PT_ROWS, it.parts, rank + 1);
+                 r += PT_THREADS / 32) {
+                const int in_tile = r & 127, query = by_group(in_tile), i = it.first + (r >> 7) * qt + query;
+                const int head = it.head * group + in_tile - query * group;
+                if (query >= qt || i >= it.rows) continue;
+                const int limit = it.seen(i);
+                bool ok;
+                float4 v = join_parts(smem_addr(ring) + r * (HD * 4), smem_addr(stats + r), r, it.parts, PT_LOG2, ok);
+                if (!ok) continue;
+                if (limit <= 0) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (__any_sync(FULL, v.x != v.x || v.y != v.y || v.z != v.z || v.w != v.w)) {
+                    const float4 x = load_quad(q + int64_t(it.base + i) * q_stride + int64_t(head) * HD + 4 * lane);
+                    v = attend_row<bf16raw>(c, b, it.s, it.head, limit,
+                                            make_float4(x.x * ATT_SCALE, x.y * ATT_SCALE, x.z * ATT_SCALE, x.w * ATT_SCALE),
+                                            status);
+                }
+                store_quad(out + (int64_t(it.base + i) * n_heads + head) * HD + 4 * lane, v);
+            }
+            cluster_sync();                                  // no CTA's shared memory goes while others read it
+            tc_fence_after();
+        }
+    }
     if (warp == 8) tc_free512(tbase);
 }
 
-// An SM holds one CTA, and a cluster lies within one group of SMs, so a few SMs of each group stay over.
-int prompt_cluster(int64_t items, int64_t tiles, int sms) {
-    int ctas = 1;
-    while (ctas < 8 && 2 * ctas * items <= sms - sms / 8 && 2 * ctas <= tiles / PROMPT_PART) ctas *= 2;
-    return ctas;
+// The largest cluster of which the GPU holds as many at once as there are items (an SM holds one CTA, and a cluster lies
+// within one group of SMs: 15 of 8, 33 of 4, 74 of 2 on a B200).
+int prompt_cluster(const void *kernel, int slot, int threads, size_t smem, int64_t items, int64_t tiles) {
+    static std::atomic<int> room[64][2][9];                  // clusters of a size that the device holds, plus 1; 0: not asked
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 1;
+    for (int ctas = 8; ctas > 1; --ctas) {
+        if (ctas > tiles / PROMPT_PART) continue;
+        int n = room[dev][slot][ctas].load(std::memory_order_relaxed);
+        if (n == 0) {
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(unsigned(ctas));
+            cfg.blockDim = dim3(unsigned(threads));
+            cfg.dynamicSmemBytes = smem;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = unsigned(ctas);
+            attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+            cfg.attrs = attr;
+            cfg.numAttrs = 1;
+            int held = 0;
+            if (cudaOccupancyMaxActiveClusters(&held, kernel, &cfg) != cudaSuccess) {
+                cudaGetLastError();
+                held = 0;
+            }
+            room[dev][slot][ctas].store(n = held + 1, std::memory_order_relaxed);
+        }
+        if (items < n) return ctas;
+    }
+    return 1;
 }
 
 cudaError_t launch_attention_prompt(const PagedKV &c, const PagedSeqs &b, int64_t rows, const void *q, q3cu_dtype dt,
                                     int64_t q_stride, int n_heads, void *out, uint32_t *status, cudaStream_t stream,
                                     int sms) {
-    if (dt == Q3CU_F32) return launch_prompt_f32(c, b, rows, q, q_stride, n_heads, out, status, stream, sms);
+    if (dt == Q3CU_F32) return launch_prompt_f32(c, b, rows, q, q_stride, n_heads, out, status, stream);
     const int group = n_heads / c.n_kv, qt = PT_ROWS / group;
     CUtensorMap mq, mk, mv;
     const uint64_t dims[3] = {HD, uint64_t(n_heads), uint64_t(rows)};
@@ -564,13 +671,17 @@ cudaError_t launch_attention_prompt(const PagedKV &c, const PagedSeqs &b, int64_
     if (!encode_lines_map(&mq, q, Q3CU_BF16, 3, dims, strides, box) || !encode_pages_map(&mk, c.k, c, Q3CU_BF16, PT_KEYS) ||
         !encode_pages_map(&mv, c.v, c, Q3CU_BF16, PT_KEYS))
         return cudaErrorInvalidValue;
-    cudaError_t e = ensure_smem_attr(reinterpret_cast<const void *>(prompt_tc_kernel), PT_SMEM, 32);
-    if (e != cudaSuccess) return e;
     // no more blocks of 2 * qt queries than this, however the rows are split into sequences
     const int64_t items = (rows / (2 * qt) + b.n_seqs) * c.n_kv;
-    return launch_dependent(prompt_tc_kernel, dim3(unsigned(items)), dim3(PT_THREADS), PT_SMEM, stream, mq, mk, mv, c, b,
-                            int(rows), static_cast<const uint16_t *>(q), q_stride, n_heads, group, FastDiv(2 * qt),
-                            FastDiv(group), static_cast<uint16_t *>(out), status);
+    cudaError_t e = ensure_smem_attr(reinterpret_cast<const void *>(prompt_tc_kernel<true>), PT_SMEM, 43);
+    if (e == cudaSuccess) e = ensure_smem_attr(reinterpret_cast<const void *>(prompt_tc_kernel<false>), PT_SMEM, 32);
+    if (e != cudaSuccess) return e;
+    const int ctas = prompt_cluster(reinterpret_cast<const void *>(prompt_tc_kernel<true>), 0, PT_THREADS, PT_SMEM, items,
+                                    (int64_t(b.max_pages) << c.page_shift) / PT_KEYS);
+    auto kernel = ctas > 1 ? prompt_tc_kernel<true> : prompt_tc_kernel<false>;
+    return launch_clusters(kernel, ctas, dim3(unsigned(items * ctas)), dim3(PT_THREADS), PT_SMEM, stream, mq, mk, mv, c, b,
+                           int(rows), static_cast<const uint16_t *>(q), q_stride, n_heads, group, FastDiv(2 * qt),
+                           FastDiv(group), ctas, static_cast<uint16_t *>(out), status);
 }
 
 }  // namespace q3

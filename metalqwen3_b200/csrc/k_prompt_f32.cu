@@ -45,6 +45,7 @@
 namespace q3 {
 
 constexpr int PF_ROWS = 128, PF_KEYS = 64, PF_THREADS = 16 * 32, PF_NS = 2;
+constexpr int PF_WHOLE = 4;                                  // key tiles from which on an item may be shared
 constexpr uint32_t PF_HALF = PF_KEYS * 128;                  // bytes of 64 keys x 64 elements of a part
 constexpr uint32_t PF_PART = 2 * PF_HALF, PF_TILE = 3 * PF_PART;
 constexpr size_t PF_SMEM = size_t(PF_NS) * 2 * PF_TILE + 1024;
@@ -126,7 +127,7 @@ prompt_f32_kernel(const PagedKV c, const PagedSeqs b, int rows, const float *q, 
     const int block_queries = it.s < 0 ? 0 : min(per_block.d, it.rows - it.first);
     const int tiles_all = it.s < 0 ? 0 : (it.seen(it.first + block_queries - 1) + PF_KEYS - 1) / PF_KEYS;
     // this CTA's part of the item's key tiles: nkv from j0 on
-    const int rank = SPLIT ? int(blockIdx.x % unsigned(ctas)) : 0, parts = SPLIT ? prompt_parts(ctas, tiles_all) : 1;
+    const int rank = SPLIT ? int(blockIdx.x % unsigned(ctas)) : 0, parts = SPLIT ? prompt_parts(ctas, tiles_all, PF_WHOLE) : 1;
     const bool mine = rank < parts;
     const int j0 = SPLIT && mine ? prompt_part(tiles_all, parts, rank) : 0;
     const int nkv = !SPLIT ? tiles_all : mine ? prompt_part(tiles_all, parts, rank + 1) - j0 : 0;
@@ -419,14 +420,16 @@ prompt_f32_kernel(const PagedKV c, const PagedSeqs b, int rows, const float *q, 
 }
 
 cudaError_t launch_prompt_f32(const PagedKV &c, const PagedSeqs &b, int64_t rows, const void *q, int64_t q_stride,
-                              int n_heads, void *out, uint32_t *status, cudaStream_t stream, int sms) {
+                              int n_heads, void *out, uint32_t *status, cudaStream_t stream) {
     const int group = n_heads / c.n_kv, qt = PF_ROWS / group;
     // no more items than this, however the rows are split into sequences
     const int64_t items = (rows / qt + b.n_seqs) * c.n_kv;
-    const int ctas = prompt_cluster(items, (int64_t(b.max_pages) << c.page_shift) / PF_KEYS, sms);
-    auto kernel = ctas > 1 ? prompt_f32_kernel<true> : prompt_f32_kernel<false>;
-    cudaError_t e = ensure_smem_attr(reinterpret_cast<const void *>(kernel), PF_SMEM, ctas > 1 ? 42 : 41);
+    cudaError_t e = ensure_smem_attr(reinterpret_cast<const void *>(prompt_f32_kernel<true>), PF_SMEM, 42);
+    if (e == cudaSuccess) e = ensure_smem_attr(reinterpret_cast<const void *>(prompt_f32_kernel<false>), PF_SMEM, 41);
     if (e != cudaSuccess) return e;
+    const int ctas = prompt_cluster(reinterpret_cast<const void *>(prompt_f32_kernel<true>), 1, PF_THREADS, PF_SMEM, items,
+                                    (int64_t(b.max_pages) << c.page_shift) / PF_KEYS);
+    auto kernel = ctas > 1 ? prompt_f32_kernel<true> : prompt_f32_kernel<false>;
     return launch_clusters(kernel, ctas, dim3(unsigned(items * ctas)), dim3(PF_THREADS), PF_SMEM, stream, c, b, int(rows),
                            static_cast<const float *>(q), q_stride, n_heads, group, FastDiv(qt), ctas,
                            static_cast<float *>(out), status);

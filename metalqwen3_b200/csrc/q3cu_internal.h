@@ -183,10 +183,10 @@ cudaError_t launch_attention_prompt(const PagedKV &c, const PagedSeqs &b, int64_
                                     int64_t q_stride, int n_heads, void *out, uint32_t *status, cudaStream_t stream,
                                     int sms);
 cudaError_t launch_prompt_f32(const PagedKV &c, const PagedSeqs &b, int64_t rows, const void *q, int64_t q_stride,
-                              int n_heads, void *out, uint32_t *status, cudaStream_t stream, int sms);
-// CTAs that share an item of a prompt launch of at most `items` items, each with no more than `tiles` key tiles: 1, 2, 4
-// or 8.
-int prompt_cluster(int64_t items, int64_t tiles, int sms);
+                              int n_heads, void *out, uint32_t *status, cudaStream_t stream);
+// CTAs (1 to 8) that share an item of a prompt launch of at most `items` items, each with no more than `tiles` key tiles;
+// `kernel` (of `slot` 0 or 1) is the one for shared items, its shared memory allowed.
+int prompt_cluster(const void *kernel, int slot, int threads, size_t smem, int64_t items, int64_t tiles);
 
 cudaError_t launch_swiglu(const void *hb, const void *hb2, q3cu_dtype dt, int64_t elems, void *out, int8_t *q,
                           float *s, uint32_t *status, cudaStream_t stream, int sms);

@@ -305,12 +305,13 @@ struct PromptOrder {
 
 // ---- items that a cluster shares --------------------------------------------------------------
 // When there are fewer items than SMs, a cluster of CTAs takes an item: part p of its key tiles goes to the CTA of rank
-// p, and the parts' unnormalised results are joined through the cluster's shared memory.  A part has at least
-// PROMPT_PART tiles.
-constexpr int PROMPT_PART = 4;
-__host__ __device__ __forceinline__ int prompt_parts(int ctas, int tiles) {
-    const int most = tiles / PROMPT_PART;
-    return most < 1 ? 1 : most < ctas ? most : ctas;
+// p, and the parts' unnormalised results are joined through the cluster's shared memory, which costs about 4 us.  A part
+// has at least PROMPT_PART tiles, and an item of fewer than `least` tiles stays whole (bf16, tiles of 128 keys of 1.3 us:
+// 600 keys take 19 us whole and 23 in two parts, 1,000 keys 22 and, in four, 17; f32, tiles of 64 keys of 1.9 us: 500
+// keys 27 whole and 20 in four).
+constexpr int PROMPT_PART = 2;
+__host__ __device__ __forceinline__ int prompt_parts(int ctas, int tiles, int least) {
+    return tiles < least ? 1 : tiles / PROMPT_PART < ctas ? tiles / PROMPT_PART : ctas;
 }
 // First tile of part p (of `parts`: behind the last).
 __host__ __device__ __forceinline__ int prompt_part(int tiles, int parts, int p) { return int(int64_t(tiles) * p / parts); }
