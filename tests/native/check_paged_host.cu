@@ -204,9 +204,23 @@ static void refusals() {
     EXPECT(q3cu_attention_paged_workspace(nullptr, 4, 2, &need) == Q3CU_ERR_NOT_INIT);
 }
 
+// The parts of a shared item cover its key tiles once, in order, none of fewer tiles than a part may have.
+static void parts() {
+    for (int ctas = 1; ctas <= 8; ++ctas)
+        for (int tiles : {0, 1, 2, 3, 4, 5, 7, 8, 9, 15, 16, 17, 63, 64, 1000, 1 << 24, INT_MAX / 64})
+            for (int least : {4, 8}) {
+                const int n = q3::prompt_parts(ctas, tiles, least);
+                EXPECT(n >= 1 && n <= ctas && (tiles >= least || n == 1));
+                EXPECT(q3::prompt_part(tiles, n, 0) == 0 && q3::prompt_part(tiles, n, n) == tiles);
+                for (int p = 0; p < n && n > 1; ++p)
+                    EXPECT(q3::prompt_part(tiles, n, p + 1) - q3::prompt_part(tiles, n, p) >= q3::PROMPT_PART);
+            }
+}
+
 int main() {
     indices();
     blocks();
+    parts();
     refusals();
     std::printf("ok\n");
     return 0;
