@@ -138,7 +138,13 @@ def _tensor(t, what, dtype=None, shape=None, device=None):
 def _rows(t, what, dtype, heads, rows, device):
     """Checks t [rows][heads][128] (heads or rows None: any) with dense heads; returns (row stride in elements, rows,
     heads, pointer)."""
-    shape, stride = t.shape, t.stride()
+    shape = t.shape
+    if len(shape) == 3 and t.get_device() == device and (dtype is None or t.dtype is dtype):
+        n, h, d = shape
+        row, head, element = t.stride()
+        if d == 128 and (heads is None or h == heads) and (rows is None or n == rows) and (
+                element == 1 and (head == 128 or h < 2) or n * h == 0):
+            return row if n > 1 or row > h * 128 else h * 128, n, h, t.data_ptr()
     if len(shape) != 3 or shape[2] != 128 or (heads is not None and shape[1] != heads) or (
             rows is not None and shape[0] != rows):
         raise ValueError(f"{what} must be [{'rows' if rows is None else rows}][{'heads' if heads is None else heads}]"
@@ -147,10 +153,7 @@ def _rows(t, what, dtype, heads, rows, device):
         raise ValueError(f"{what} must be on the context's GPU, it is on {t.device}")
     if dtype is not None and t.dtype != dtype:
         raise TypeError(f"{what} must be {dtype}, it is {t.dtype}")
-    n, h = shape[0], shape[1]
-    if (stride[2] != 1 or (h > 1 and stride[1] != 128)) and n * h:
-        raise ValueError(f"{what}: the heads of a row must be contiguous, strides are {stride}")
-    return stride[0] if n > 1 else max(stride[0], h * 128), n, h, t.data_ptr()
+    raise ValueError(f"{what}: the heads of a row must be contiguous, strides are {t.stride()}")
 
 
 class KVCache:
