@@ -566,6 +566,26 @@ def test_captured_few_rows_replayed(q3, dtype):
             check_attention(out[a:b], q[a:b], k[:lens[s]], v[:lens[s]], seen, dtype, H if dtype == BF16 else 0.0)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_few_rows_on_two_streams(q3, dtype):
+    """Clusters of two calls wait for multiprocessors beside each other, and each call's result is as alone."""
+    sets = []
+    for seed, rows, lens in ((90, [20, 3], [1900, 800]), (93, [40], [2500])):
+        p = Paged(lens, 8, 16, dtype, seed=seed).fill(seed + 1)
+        q = queries(sum(rows), 16, dtype, seed + 2)
+        cache, batch = p.handles(offsets(rows))
+        sets.append((p, cache, batch, q, q3.attention_prompt(cache, batch, q), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(12):
+        for i, (_, cache, batch, q, _, stream) in enumerate(sets):
+            with torch.cuda.stream(stream):
+                outs[i].append(q3.attention_prompt(cache, batch, q))
+    torch.cuda.synchronize()
+    for got, (_, _, _, _, alone, _) in zip(outs, sets):
+        assert all(torch.equal(g, alone) for g in got)
+
+
 def test_offsets_that_do_not_rise(q3):
     """Broken row offsets touch nothing outside the rows and fault nothing."""
     p = Paged([50, 50, 50], 2, 16, BF16, seed=43).fill(44)
