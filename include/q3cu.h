@@ -264,8 +264,8 @@ q3cu_status q3cu_attention_paged_workspace(q3cu_ctx *ctx, int n_heads, int n_kv,
  * 0..p.  A whole prompt has kv_len equal to its rows; a chunk behind a cached
  * prefix has more.  q: [rows][n_heads][128] with q_stride elements between
  * rows; out: [rows][n_heads][128], other memory than q.  Both of the cache's type: bf16 runs on the tensor cores with
- * probabilities rounded to bf16 (the sums binary32), f32 throughout in
- * binary32.  Grouped heads, scale, softmax, empty rows, unused page space, bad
+ * probabilities rounded to bf16 (the sums binary32), f32 with binary32's
+ * accuracy (elements below 2^-109 keep fewer bits).  Grouped heads, scale, softmax, empty rows, unused page space, bad
  * pages and alignment as above.  Sequences with one row are allowed, but
  * q3cu_attention_paged is made for them. */
 q3cu_status q3cu_attention_prompt(q3cu_ctx *ctx, const q3cu_kv_cache *cache, const q3cu_kv_batch *batch,

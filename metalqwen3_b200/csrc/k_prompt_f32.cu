@@ -36,7 +36,8 @@
 //
 // Masks and rows that come out as NaN are treated as in k_prompt.cu; keys and values
 // behind the sequence's end are stored as zeros.  (An infinity splits into
-// infinity and NaN, so its rows go the way of NaN rows, which ends in the formula.)
+// infinity and NaN, so its rows go the way of NaN rows, which ends in the formula.  An element below 2^-109 keeps fewer
+// bits: its last part would be below bf16's least normal number, 2^-126.)
 #include "q3cu_mma.cuh"
 #include "q3cu_paged.cuh"
 #include "q3cu_tcgen05.cuh"
