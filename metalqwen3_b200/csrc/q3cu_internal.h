@@ -24,7 +24,10 @@ cudaError_t ensure_smem_attr(const void *kernel, size_t bytes, int slot);
 // kernel: its CTAs may start before that kernel has completed, so the kernel
 // calls griddep_wait() before it reads or writes any global memory that an
 // earlier launch writes or reads (every thread that does, on every path), and
-// griddep_launch_dependents() where its own successor may start.  When the
+// griddep_launch_dependents() where its own successor may start.  At least one
+// CTA waits whatever it finds to do: the successor waits for this grid alone,
+// and a grid that ends without waiting may end before its predecessor,
+// which that successor then does not wait for.  When the
 // previous work is not a kernel the launch behaves as an ordinary one.
 // In clusters of `cluster` CTAs where that is more than one.
 template <typename... KArgs, typename... Args>
