@@ -217,6 +217,16 @@ class Q3CU:
         raw = self._raw_stream                  # the handle alone: a Stream object takes a microsecond to make
         return raw(self.device) if raw else self.torch.cuda.current_stream(self.device).cuda_stream
 
+    def _make(self, stream, make, *args, **kwargs):
+        """What a call makes for itself, by torch's function `make`.  Where a stream is given the memory is
+        that stream's own: what lies free in the current stream's may still be in use by work that is pending there."""
+        if stream is None:
+            return make(*args, **kwargs)
+        with self.torch.cuda.stream(stream):
+            t = make(*args, **kwargs)
+        t.record_stream(self.torch.cuda.current_stream(self.device))       # where the caller may read it
+        return t
+
     def close(self):
         if getattr(self, "ctx", None):
             self.lib.q3cu_destroy(self.ctx)
@@ -243,15 +253,17 @@ class Q3CU:
     # -- device-pointer ops ----------------------------------------------------
     def rmsnorm(self, x, w, eps=1e-6, out=None, stream=None):
         rows, dim = x.shape
-        out = self.torch.empty_like(x) if out is None else out
+        out = self._make(stream, self.torch.empty_like, x) if out is None else out
         self._check(self.lib.q3cu_rmsnorm(self.ctx, _ptr(x), _dtype(x), _ptr(w), rows, dim, eps, _ptr(out),
                                           self._stream(stream)), "q3cu_rmsnorm")
         return out
 
     def rmsnorm_q8(self, x, w, eps=1e-6, q=None, s=None, stream=None):
         rows, dim = x.shape
-        q = self.torch.empty((rows, dim), dtype=self.torch.int8, device=x.device) if q is None else q
-        s = self.torch.empty((rows, dim // GS), dtype=self.torch.float32, device=x.device) if s is None else s
+        if q is None:
+            q = self._make(stream, self.torch.empty, (rows, dim), dtype=self.torch.int8, device=x.device)
+        if s is None:
+            s = self._make(stream, self.torch.empty, (rows, dim // GS), dtype=self.torch.float32, device=x.device)
         self._check(self.lib.q3cu_rmsnorm_q8(self.ctx, _ptr(x), _dtype(x), _ptr(w), rows, dim, eps, _ptr(q),
                                              _ptr(s), self._stream(stream)), "q3cu_rmsnorm_q8")
         return q, s
@@ -273,8 +285,10 @@ class Q3CU:
 
     def swiglu_q8(self, hb, hb2, q=None, s=None, stream=None):
         rows, hidden = hb.shape
-        q = self.torch.empty((rows, hidden), dtype=self.torch.int8, device=hb.device) if q is None else q
-        s = self.torch.empty((rows, hidden // GS), dtype=self.torch.float32, device=hb.device) if s is None else s
+        if q is None:
+            q = self._make(stream, self.torch.empty, (rows, hidden), dtype=self.torch.int8, device=hb.device)
+        if s is None:
+            s = self._make(stream, self.torch.empty, (rows, hidden // GS), dtype=self.torch.float32, device=hb.device)
         self._check(self.lib.q3cu_swiglu_q8(self.ctx, _ptr(hb), _ptr(hb2), _dtype(hb), rows, hidden, _ptr(q), _ptr(s),
                                             self._stream(stream)), "q3cu_swiglu_q8")
         return q, s
@@ -286,15 +300,17 @@ class Q3CU:
 
     def quantize_q8(self, x, q=None, s=None, stream=None):
         rows, n = x.shape
-        q = self.torch.empty((rows, n), dtype=self.torch.int8, device=x.device) if q is None else q
-        s = self.torch.empty((rows, n // GS), dtype=self.torch.float32, device=x.device) if s is None else s
+        q = self._make(stream, self.torch.empty, (rows, n), dtype=self.torch.int8, device=x.device) if q is None else q
+        if s is None:
+            s = self._make(stream, self.torch.empty, (rows, n // GS), dtype=self.torch.float32, device=x.device)
         self._check(self.lib.q3cu_quantize_q8(self.ctx, _ptr(x), _dtype(x), rows, n, _ptr(q), _ptr(s),
                                               self._stream(stream)), "q3cu_quantize_q8")
         return q, s
 
     def dequantize_q8(self, q, s, out=None, stream=None):
         n = q.numel()
-        out = self.torch.empty(q.shape, dtype=self.torch.float32, device=q.device) if out is None else out
+        if out is None:
+            out = self._make(stream, self.torch.empty, q.shape, dtype=self.torch.float32, device=q.device)
         self._check(self.lib.q3cu_dequantize_q8(self.ctx, _ptr(q), _ptr(s), n, _ptr(out), self._stream(stream)),
                     "q3cu_dequantize_q8")
         return out
@@ -304,10 +320,10 @@ class Q3CU:
         n = ids.numel()
         T = self.torch
         if want_f32 and out is None:
-            out = T.empty((n, dim), dtype=T.float32, device=tq.device)
+            out = self._make(stream, T.empty, (n, dim), dtype=T.float32, device=tq.device)
         if want_q8 and oq is None:
-            oq = T.empty((n, dim), dtype=T.int8, device=tq.device)
-            os_ = T.empty((n, dim // GS), dtype=T.float32, device=tq.device)
+            oq = self._make(stream, T.empty, (n, dim), dtype=T.int8, device=tq.device)
+            os_ = self._make(stream, T.empty, (n, dim // GS), dtype=T.float32, device=tq.device)
         self._check(self.lib.q3cu_embed_gather(self.ctx, _ptr(tq), _ptr(ts), vocab, dim, _ptr(ids), n,
                                                _ptr(out if want_f32 else None), _ptr(oq if want_q8 else None),
                                                _ptr(os_ if want_q8 else None), self._stream(stream)),
@@ -320,7 +336,8 @@ class Q3CU:
         d = wq.shape[0]
         if wq.shape[1] != n:
             raise ValueError(f"W is {tuple(wq.shape)}, x rows have {n} elements")
-        out = self.torch.empty((B, d), dtype=self.torch.float32, device=xq.device) if out is None else out
+        if out is None:
+            out = self._make(stream, self.torch.empty, (B, d), dtype=self.torch.float32, device=xq.device)
         self._check(self.lib.q3cu_matmul_q8(self.ctx, _ptr(xq), _ptr(xs), B, _ptr(wq), _ptr(ws), n, d, _ptr(out),
                                             self._stream(stream)), "q3cu_matmul_q8")
         return out
@@ -333,9 +350,9 @@ class Q3CU:
         T = self.torch
         n_heads = q.numel() // 128
         kv_dim = key_cache.shape[-1]
-        att = T.zeros((n_heads, pos + 1), dtype=T.float32, device=q.device) if att is None else att
-        probs = T.zeros_like(att) if probs is None else probs
-        xb = T.empty((n_heads, 128), dtype=T.float32, device=q.device) if xb is None else xb
+        att = self._make(stream, T.zeros, (n_heads, pos + 1), dtype=T.float32, device=q.device) if att is None else att
+        probs = self._make(stream, T.zeros_like, att) if probs is None else probs
+        xb = self._make(stream, T.empty, (n_heads, 128), dtype=T.float32, device=q.device) if xb is None else xb
         self._check(self.lib.q3cu_attention(self.ctx, _ptr(q), _ptr(key_cache), _ptr(value_cache), pos, n_heads,
                                             kv_dim, kv_mul, _ptr(att), att.shape[-1], _ptr(probs), _ptr(xb),
                                             self._stream(stream)), "q3cu_attention")
@@ -360,7 +377,8 @@ class Q3CU:
         if q is not None:
             q_stride, _, heads, qp = _rows(q, "q", dtype, None, rows, dev)
             if q_out is None:
-                q_out = self.torch.empty((rows, heads, 128), dtype=out_dtype or cache.k.dtype, device=q.device)
+                q_out = self._make(stream, self.torch.empty, (rows, heads, 128), dtype=out_dtype or cache.k.dtype,
+                                   device=q.device)
             _, _, _, op = _rows(q_out, "q_out", out_dtype, heads, rows, dev)
             if not q_out.is_contiguous():
                 raise ValueError("q_out must be contiguous")
@@ -373,26 +391,25 @@ class Q3CU:
             self._check(status, "q3cu_kv_append")
         return q_out
 
-    def attention_paged_workspace(self, cache, n_heads):
+    def attention_paged_workspace(self, cache, n_heads, stream=None):
         """A workspace for attention_paged with these head counts, for any batch; calls that may run at
-        the same time (other streams, captured graphs replayed side by side) need one each."""
+        the same time (other streams, captured graphs replayed side by side) need one each.  `stream`: where it is
+        used, if not on the current one."""
         n = C.c_size_t(0)
         self._check(self.lib.q3cu_attention_paged_workspace(self.ctx, n_heads, cache.n_kv, C.byref(n)),
                     "q3cu_attention_paged_workspace")
-        return self.torch.empty(n.value, dtype=self.torch.uint8, device=cache.k.device)
+        return self._make(stream, self.torch.empty, n.value, dtype=self.torch.uint8, device=cache.k.device)
 
     def attention_paged(self, cache, batch, q, out=None, work=None, stream=None):
         """One new token per sequence: q [n_seqs][n_heads][128] over each sequence's kv_len positions."""
         stride, rows, heads, qp = _rows(q, "q", None, None, batch.c.n_seqs, self.device)
         if out is None:
-            out = self.torch.empty((rows, heads, 128), dtype=q.dtype, device=q.device)
+            out = self._make(stream, self.torch.empty, (rows, heads, 128), dtype=q.dtype, device=q.device)
         elif not out.is_contiguous():
             raise ValueError("out must be contiguous")
         op = _rows(out, "out", q.dtype, heads, rows, self.device)[3]
         if work is None:
-            work = self.attention_paged_workspace(cache, heads)
-            if stream is not None:
-                work.record_stream(stream)      # its memory is not given out again before the call has run
+            work = self.attention_paged_workspace(cache, heads, stream)
         status = self.lib.q3cu_attention_paged(self.ctx, cache.ref, batch.ref, qp, _dtype(q), stride, heads,
                                                work.data_ptr(), work.nbytes, op, self._stream(stream))
         if status:
@@ -404,7 +421,7 @@ class Q3CU:
         keys and values; rows behind the last sequence are not written."""
         stride, rows, heads, qp = _rows(q, "q", None, None, None, self.device)
         if out is None:
-            out = self.torch.empty((rows, heads, 128), dtype=q.dtype, device=q.device)
+            out = self._make(stream, self.torch.empty, (rows, heads, 128), dtype=q.dtype, device=q.device)
         elif not out.is_contiguous():
             raise ValueError("out must be contiguous")
         op = _rows(out, "out", q.dtype, heads, rows, self.device)[3]

@@ -52,3 +52,41 @@ def test_nothing_to_join_then_dependent_kernels(q3, dtype, lens):
             live = torch.tensor(lens, device="cuda") > 0     # padding rows are not turned
             assert torch.equal(outs[i], alone[i % 8, 0]) and torch.equal(turned[i][live], alone[i % 8, 1][live])
     assert q3.device_status() == 0
+
+
+def test_current_and_given_stream_at_once(q3):
+    """Calls on the current stream and, with nothing between them, on a given one: the memory that they make for
+    themselves is apart, and each result is as alone."""
+    sets = []
+    for i in range(2):
+        p = Paged([30000, 7000], 2, 16, BF16, seed=120 + i).fill(122 + i)
+        q = queries(2, 32, BF16, 124 + i)
+        cache, batch = p.handles([0, 1, 2])
+        rows = queries(2, 36, BF16, 126 + i)
+        sets.append((p, cache, batch, q, rows))
+
+    def calls(i, stream=None):
+        _, cache, batch, q, rows = sets[i]
+        one = q3.attention_paged(cache, batch, q, stream=stream)
+        prompt = q3.attention_prompt(cache, batch, q, stream=stream)
+        return one, prompt, q3.kv_append(other, batch, rows[:, :32], rows[:, 32:34], rows[:, 34:], stream=stream)
+
+    p = sets[0][0]                                           # appended to, and read by nothing
+    other = type(sets[0][1])(torch.zeros_like(p.k), torch.zeros_like(p.v))
+    alone = []
+    for i in range(2):
+        alone.append(calls(i))
+        torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    freed = torch.empty((2, 32, 128), dtype=BF16, device="cuda")
+    at = freed.data_ptr()
+    del freed
+    assert all(t.data_ptr() != at for t in calls(1, side))
+    got = []
+    for _ in range(50):
+        got.append((0, calls(0)))
+        got.append((1, calls(1, side)))
+    torch.cuda.synchronize()
+    for i, results in got:
+        assert all(torch.equal(a, b) for a, b in zip(results, alone[i]))
+    assert q3.device_status() == 0 and q3.device_status(side) == 0
