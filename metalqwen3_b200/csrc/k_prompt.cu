@@ -76,14 +76,15 @@ constexpr float PT_LAZY = 8.0f / PT_LOG2;                    // growth of the ma
 // 2^x of a pair without the special-function unit, which is as busy as the tensor cores when every exponential goes
 // through it: x = n + f with n whole and |f| <= 1/2, a polynomial for 2^f, times 2^n.  The coefficients are the minimax
 // fit of degree 3 to 2^f (relative error 7.5e-5, a fiftieth of the bf16 rounding that follows), found by Remez exchange.
-// Below 2^-126 the result is 2^-126; a NaN stays one.
+// Below 2^-126.5 the result is 0 (n = -127 makes the exponent's bits 0), as a masked score of -inf has to give; a NaN
+// stays one.
 __device__ __forceinline__ float max_nan(float x, float y) {
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
     return r;
 }
 __device__ __forceinline__ void exp2_poly(float &x, float &y) {
-    const f2 v = pk2(max_nan(x, -126.0f), max_nan(y, -126.0f)), magic = pk2(12582912.0f, 12582912.0f);   // 1.5 * 2^23
+    const f2 v = pk2(max_nan(x, -127.0f), max_nan(y, -127.0f)), magic = pk2(12582912.0f, 12582912.0f);   // 1.5 * 2^23
     const f2 t = add2(v, magic), f = sub2(v, sub2(t, magic));
     f2 p = pk2(0.0551716685295105f, 0.0551716685295105f);
     p = fma2(p, f, pk2(0.2426111251115799f, 0.2426111251115799f));

@@ -1,9 +1,11 @@
 """The paged-cache operators where one element, one order or one stream decides.  Formulas, tolerances and helpers are
 those of test_gpu_paged.py."""
+import math
+
 import pytest
 import torch
 
-from test_gpu_paged import BF16, F32, Paged, check_attention, queries
+from test_gpu_paged import BF16, F32, H, NAN, Paged, check_attention, queries
 
 pytestmark = pytest.mark.gpu
 
@@ -90,3 +92,28 @@ def test_current_and_given_stream_at_once(q3):
     for i, results in got:
         assert all(torch.equal(a, b) for a, b in zip(results, alone[i]))
     assert q3.device_status() == 0 and q3.device_status(side) == 0
+
+
+def rounding(dtype):
+    return H if dtype == BF16 else 0.0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("what", [math.inf, -math.inf, NAN, 3e38, -3e38])
+@pytest.mark.parametrize("n,rows,at", [(300, 300, 200), (600, 600, 290), (2000, 20, 1986)])
+def test_hidden_values_reach_no_earlier_row(q3, dtype, what, n, rows, at):
+    """A value in one column of one position, at each of eight positions running: rows before it are as if it was not
+    there, in whole items and in those that several multiprocessors share."""
+    p = Paged([n], 2, 16, dtype, seed=100).fill(101)
+    page, slot = p.where(0, range(n))
+    q = queries(rows, 8, dtype, 102)
+    clean = p.v.clone()
+    for hidden in range(at, at + 8):
+        p.v.copy_(clean)
+        p.v[page[hidden], :, slot[hidden], 17 * (hidden - at)] = what
+        got = q3.attention_prompt(*p.handles([0, rows]), q)
+        k, v = p.rows(0)
+        before = hidden - (n - rows)
+        check_attention(got[:before], q[:before], k[:hidden], v[:hidden], range(n - rows + 1, hidden + 1), dtype,
+                        rounding(dtype))
+    assert q3.device_status() == 0
