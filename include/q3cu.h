@@ -252,7 +252,9 @@ q3cu_status q3cu_kv_append(q3cu_ctx *ctx, const q3cu_kv_cache *cache, const q3cu
  * same time need one each.  What a page holds beyond a sequence's last
  * position is never used, NaN included.  A page id outside the cache sets
  * Q3CU_DEV_BAD_INDEX and reads as zeros; a kv_len beyond the table sets it and
- * is cut. */
+ * is cut.  An infinite element at one of the sequence's own positions may make
+ * results NaN that the formula gives another value: with a key those of its
+ * heads, with a value those of its column. */
 q3cu_status q3cu_attention_paged(q3cu_ctx *ctx, const q3cu_kv_cache *cache, const q3cu_kv_batch *batch,
                                  const void *q, q3cu_dtype dtype, int64_t q_stride, int n_heads, void *work,
                                  size_t work_bytes, void *out, q3cu_stream stream);

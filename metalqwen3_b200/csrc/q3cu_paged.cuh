@@ -130,7 +130,8 @@ __device__ __forceinline__ void store_quad(uint16_t *p, float4 v) {
 // Attention of one query row and head by one warp, straight from the formula:
 // lane l holds elements 4l .. 4l+3 of q (scaled by 1/sqrt(128)), of every key
 // and value and of the result.  The running maximum and sum of the softmax, one pass over
-// the keys 0 .. n-1 of sequence s.  Returns zeros for n = 0.
+// the keys 0 .. n-1 of sequence s.  A score of -inf (an infinite key) weighs nothing; a row that has no other is 0 / 0.
+// Returns zeros for n = 0.
 template <typename TC>
 __device__ __forceinline__ float4 attend_row(const PagedKV &c, const PagedSeqs &b, int s, int head, int n, float4 q,
                                              uint32_t *status) {
@@ -150,7 +151,8 @@ __device__ __forceinline__ float4 attend_row(const PagedKV &c, const PagedSeqs &
         float d = fmaf(q.x, k.x, fmaf(q.y, k.y, fmaf(q.z, k.z, q.w * k.w)));
 #pragma unroll
         for (int x = 16; x > 0; x >>= 1) d += __shfl_xor_sync(FULL, d, x);
-        const float nm = fmaxf(m, d), f = m == nm ? 1.0f : expf(m - nm), p = expf(d - nm);
+        const float nm = fmaxf(m, d), f = m == nm ? 1.0f : expf(m - nm);
+        const float p = d == -INFINITY ? 0.0f : expf(d - nm);              // also while nm is -inf
         m = nm;
         sum = fmaf(sum, f, p);
         o = make_float4(fmaf(o.x, f, p * v.x), fmaf(o.y, f, p * v.y), fmaf(o.z, f, p * v.z), fmaf(o.w, f, p * v.w));

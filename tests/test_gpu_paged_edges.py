@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_paged import BF16, F32, H, NAN, Paged, check_attention, queries
+from test_gpu_paged import BF16, F32, H, NAN, Paged, attend, check_attention, queries
 
 pytestmark = pytest.mark.gpu
 
@@ -116,4 +116,52 @@ def test_hidden_values_reach_no_earlier_row(q3, dtype, what, n, rows, at):
         before = hidden - (n - rows)
         check_attention(got[:before], q[:before], k[:hidden], v[:hidden], range(n - rows + 1, hidden + 1), dtype,
                         rounding(dtype))
+    assert q3.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,rows,at", [(150, 150, 0), (150, 150, 1), (150, 150, 63), (150, 150, 64), (300, 300, 127),
+                                       (300, 300, 128), (1500, 10, 0), (1500, 10, 1486)])
+def test_infinite_keys_and_values(q3, dtype, n, rows, at):
+    """An infinite element of a key, wherever the key lies, makes its score -inf (weight 0: the other keys share the row)
+    or +inf (a row of NaN); an infinite value makes its column infinite."""
+    p = Paged([n], 2, 16, dtype, seed=103).fill(104)
+    page, slot = p.where(0, [at])
+    p.k[page, 0, slot, 5] = math.inf
+    p.v[page, 1, slot, 9] = math.inf
+    q = queries(rows, 4, dtype, 105)
+    got, (k, v) = q3.attention_prompt(*p.handles([0, rows]), q).double(), p.rows(0)
+    position = torch.arange(n - rows, n, device="cuda")
+    sees = position >= at
+    up = (q[:, :2, 5] > 0) & sees[:, None]
+    assert up.any() and (sees[:, None] & ~up).any() and got[:, :2][up].isnan().all()
+    for h in range(2):
+        keep = (~up[:, h] & (position > 0)).nonzero()[:, 0]       # row 0 has no other key
+        check_attention(got[keep, h:h + 1], q[keep, h:h + 1], k[:, :1], v[:, :1], position[keep] + 1, dtype,
+                        rounding(dtype))
+    assert (got[sees, 2:, 9] == math.inf).all()
+    v[at, 1, 9] = 0.0
+    got[sees, 2:, 9] = attend(q[sees][:, 2:].double(), k[:, 1:], v[:, 1:], position[sees] + 1)[0][:, :, 9]
+    check_attention(got[:, 2:], q[:, 2:], k[:, 1:], v[:, 1:], position + 1, dtype, rounding(dtype))
+    assert q3.device_status() == 0
+
+
+@pytest.mark.parametrize("io,cache_t", [(F32, F32), (F32, BF16), (BF16, BF16), (BF16, F32)])
+@pytest.mark.parametrize("n,at", [(1, 0), (40, 0), (40, 39), (3000, 0), (3000, 1777), (3000, 2999)])
+def test_one_token_infinities_are_right_or_nan(q3, io, cache_t, n, at):
+    """An infinite key's heads and an infinite value's column are as the formula has them or NaN, the others as ever."""
+    p = Paged([n], 2, 16, cache_t, seed=106).fill(107)
+    page, slot = p.where(0, [at])
+    p.k[page, 0, slot, 5] = math.inf
+    p.v[page, 1, slot, 9] = math.inf
+    q = queries(1, 4, io, 108)
+    got, (k, v) = q3.attention_paged(*p.handles(), q).double(), p.rows(0)
+    for h in range(2):                                       # a score of +inf, or -inf and no other: NaN
+        if not got[:, h].isnan().all():
+            assert n > 1 and q[0, h, 5] < 0
+            check_attention(got[:, h:h + 1], q[:, h:h + 1], k[:, :1], v[:, :1], [n], io)
+    assert ((got[:, 2:, 9] == math.inf) | got[:, 2:, 9].isnan()).all()
+    v[at, 1, 9] = 0.0
+    got[:, 2:, 9] = attend(q[:, 2:].double(), k[:, 1:], v[:, 1:], [n])[0][:, :, 9]
+    check_attention(got[:, 2:], q[:, 2:], k[:, 1:], v[:, 1:], [n], io)
     assert q3.device_status() == 0
