@@ -209,8 +209,9 @@ __device__ __forceinline__ int lanes_before(int x) {         // sum over the lan
     return y - x;
 }
 // The order of a launch's items: kv heads innermost, blocks from the most key tiles to the fewest, so that no long item
-// begins last.  Held by one warp, lane l with sequences l and l + 32; find() takes rising indices and returns the same
-// in every lane.  A block's place is found by the number of tiles at which the count of larger blocks passes its index:
+// begins last.  Held by one warp, lane l with sequences l and l + 32; find() returns the same in every lane.  It takes any
+// indices, rising ones quickest: a smaller one than before begins the search anew (the CTAs that are taken over come in no
+// promised order).  A block's place is found by the number of tiles at which the count of larger blocks passes its index:
 // the level of the item before or the next lower one mostly, bisection otherwise.  Past PROMPT_SORTED sequences, which
 // the lanes cannot hold, the order is sequence by sequence, the last block first.
 constexpr int PROMPT_SORTED = 64;
@@ -221,6 +222,7 @@ struct PromptOrder {
     const FastDiv &per_block;
     int total_rows, tile_keys;
     uint32_t *status;
+    int latest;              // the latest index, of blocks
     int hi, above;           // sorted: blocks of at least hi tiles are `above`, no more than the latest index
     int from, passed;        // otherwise: the 32 sequences of the latest index, and the blocks before them
 
@@ -232,8 +234,11 @@ struct PromptOrder {
         q[0] = prompt_seq(b, c, total_rows, per_block, sorted ? lane : b.n_seqs, status);
         q[1] = PromptSeq{0, 0, 0, 0, 0};
         if (sorted && b.n_seqs > 32) q[1] = prompt_seq(b, c, total_rows, per_block, lane + 32, status);
+        restart();
+    }
+    __device__ __forceinline__ void restart() {
         hi = (max(__reduce_max_sync(FULL, q[0].len), __reduce_max_sync(FULL, q[1].len)) + tile_keys - 1) / tile_keys + 1;
-        above = from = passed = 0;
+        latest = above = from = passed = 0;
     }
     __device__ __forceinline__ int at_least(int x, int tiles) const {
         return q[x].at_least(tiles ? (tiles - 1) * tile_keys + 1 : 0, per_block);
@@ -255,6 +260,8 @@ struct PromptOrder {
         it.head = int(uint32_t(index) % uint32_t(c.n_kv));
         int left = int(uint32_t(index) / uint32_t(c.n_kv));
         const int lane = threadIdx.x & 31;
+        if (left < latest) restart();
+        latest = left;
         if (b.n_seqs > PROMPT_SORTED) {
             for (; from < b.n_seqs; from += 32) {
                 const PromptSeq p = prompt_seq(b, c, total_rows, per_block, from + lane, status);

@@ -1,6 +1,8 @@
 """The paged-cache operators where one element, one order or one stream decides.  Formulas, tolerances and helpers are
 those of test_gpu_paged.py."""
 import math
+import os
+import subprocess
 
 import pytest
 import torch
@@ -165,3 +167,15 @@ def test_one_token_infinities_are_right_or_nan(q3, io, cache_t, n, at):
     got[:, 2:, 9] = attend(q[:, 2:].double(), k[:, 1:], v[:, 1:], [n])[0][:, :, 9]
     check_attention(got[:, 2:], q[:, 2:], k[:, 1:], v[:, 1:], [n], io)
     assert q3.device_status() == 0
+
+
+def test_prompt_items_in_any_order(tmp_path):
+    """Every item of a launch is found at its index, whatever order the indices come in (check_prompt_order.cu)."""
+    from metalqwen3_b200.build import CSRC
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    exe = str(tmp_path / "check_prompt_order")
+    subprocess.run(["nvcc", "-gencode", "arch=compute_100a,code=sm_100a", "-std=c++17", "--fmad=false", "-I", CSRC, "-I",
+                    os.path.join(root, "include"), os.path.join(root, "tests", "native", "check_prompt_order.cu"), "-o", exe],
+                   check=True)
+    out = subprocess.run([exe], capture_output=True, text=True, timeout=120)
+    assert out.returncode == 0 and out.stdout.strip() == "ok", out.stdout + out.stderr
