@@ -45,12 +45,17 @@
 // Masks: keys at and beyond the row's limit become -inf before the maximum.
 // Their probability is exactly 0, but 0 times a NaN or an infinity in V is not:
 // the values behind the sequence's end (never written, anything may be there) are
-// zeroed in shared memory, and a row whose result is NaN is computed again from
-// the formula by one warp (attend_row), so that a value at a later position of
-// the sequence never reaches an earlier row.
+// zeroed in shared memory, and a row that comes out with elements that are no
+// numbers is computed again from the formula by one warp (attend_row), so that a
+// value at a later position of the sequence never reaches an earlier row.  That is
+// some hundred times slower than the tile, so it is done only where it may change
+// the row (SecondLook): a prompt of 4,096 rows (32/8) takes 0.14 ms, 1.3 with a NaN
+// that all rows see, and 24 with one in the last value, which spoils a tile.
 //
 // Every wait is bounded; a wait that gives up sets Q3CU_DEV_TIMEOUT and the CTA
-// drains its own copies and products, frees tensor memory and returns.
+// drains its own copies and products, frees tensor memory and returns.  So that no
+// other warp's wait gives up meanwhile, a warp computes rows again for a second at
+// most; past that (32 rows of 170,000 keys) the rest stay NaN, with the same bit set.
 #include "q3cu_paged.cuh"
 #include "q3cu_tcgen05.cuh"
 #include "q3cu_tma.h"
@@ -95,6 +100,7 @@ __device__ __forceinline__ void exp2_poly(float &x, float &y) {
     up2(mul2(p, pk2(__uint_as_float((__float_as_uint(t0) << 23) + 0x3f800000u),
                     __uint_as_float((__float_as_uint(t1) << 23) + 0x3f800000u))), x, y);
 }
+constexpr uint64_t PT_AGAIN_NS = 1000000000;                 // the longest that a warp computes rows again: others wait for it
 constexpr int PT_POLY = 8;                                   // one pair of exponentials in PT_POLY / 2 by polynomial
 
 // The item of a round, as warp 9 announces it (s < 0: no more), with the key tiles of each row tile.
@@ -557,18 +563,26 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&o_empty[t]);
                 }
-                // rows that came out as NaN, once more from the formula
+                // rows that came out as no numbers, once more from the formula
                 unsigned again = __ballot_sync(FULL, live && limit > 0 && nan);
+                SecondLook<bf16raw> second;
+                const uint64_t began = again ? global_ns() : 0;
                 while (again) {
+                    if (global_ns() - began > PT_AGAIN_NS) {
+                        if (lane == 0) flag_timeout(status);
+                        break;
+                    }
                     const int l = __ffs(again) - 1;
                     again &= again - 1;
                     __syncwarp();
+                    second.look(t, c, b, it.s, it.head, it.seen(it.first + t * qt), min(it.len, it.nt[t] * PT_KEYS));
                     const int il = __shfl_sync(FULL, i, l), n = __shfl_sync(FULL, limit, l);
                     const int h = it.head * group + __shfl_sync(FULL, r_head, l);
                     float4 x = load_quad(q + int64_t(it.base + il) * q_stride + int64_t(h) * HD + 4 * lane);
+                    if (!second.wanted(n, x)) continue;
                     x = make_float4(x.x * ATT_SCALE, x.y * ATT_SCALE, x.z * ATT_SCALE, x.w * ATT_SCALE);
                     store_quad(out + (int64_t(it.base + il) * n_heads + h) * HD + 4 * lane,
-                               attend_row<bf16raw>(c, b, it.s, it.head, n, x, status));
+                               attend_row<bf16raw, 4>(c, b, it.s, it.head, n, x, status));
                 }
             }
         }
@@ -603,6 +617,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                 tc_fence_before();
             }
             cluster_sync();
+            SecondLook<bf16raw> second;
             for (int r = prompt_part(2 * PT_ROWS, it.parts, rank) + warp; r < prompt_part(2 * PT_ROWS, it.parts, rank + 1);
                  r += PT_THREADS / 32) {
                 const int in_tile = r & 127, query = by_group(in_tile), i = it.first + (r >> 7) * qt + query;
@@ -613,11 +628,14 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                 float4 v = join_parts(smem_addr(ring) + r * (HD * 4), smem_addr(stats + r), r, it.parts, PT_LOG2, ok);
                 if (!ok) continue;
                 if (limit <= 0) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (__any_sync(FULL, v.x != v.x || v.y != v.y || v.z != v.z || v.w != v.w)) {
+                if (limit > 0 && __any_sync(FULL, !all_finite(v))) {
+                    const int first = it.first + (r >> 7) * qt, seen = it.seen(min(first + qt, it.rows) - 1);
+                    second.look(r >> 7, c, b, it.s, it.head, it.seen(first), min(it.len, (seen + PT_KEYS - 1) / PT_KEYS * PT_KEYS));
                     const float4 x = load_quad(q + int64_t(it.base + i) * q_stride + int64_t(head) * HD + 4 * lane);
-                    v = attend_row<bf16raw>(c, b, it.s, it.head, limit,
-                                            make_float4(x.x * ATT_SCALE, x.y * ATT_SCALE, x.z * ATT_SCALE, x.w * ATT_SCALE),
-                                            status);
+                    if (second.wanted(limit, x))
+                        v = attend_row<bf16raw, 4>(c, b, it.s, it.head, limit,
+                                                make_float4(x.x * ATT_SCALE, x.y * ATT_SCALE, x.z * ATT_SCALE, x.w * ATT_SCALE),
+                                                status);
                 }
                 store_quad(out + (int64_t(it.base + i) * n_heads + head) * HD + 4 * lane, v);
             }

@@ -34,10 +34,10 @@
 // prompts), the next tile's loads ahead of this tile's split (57 us: the splitting warps then keep the rows' warps
 // waiting for issue slots), parts by truncation in place of rounding (57 us, and a larger error).
 //
-// Masks and rows that come out as NaN are treated as in k_prompt.cu; keys and values
-// behind the sequence's end are stored as zeros.  (An infinity splits into
-// infinity and NaN, so its rows go the way of NaN rows, which ends in the formula.  An element below 2^-109 keeps fewer
-// bits: its last part would be below bf16's least normal number, 2^-126.)
+// Masks and rows that come out as NaN are treated as in k_prompt.cu (SecondLook in q3cu_paged.cuh); keys and values
+// behind the sequence's end are stored as zeros.  (An infinity splits into infinity and NaN, so its rows go the way of
+// NaN rows and are computed from the formula.  An element below 2^-109 keeps fewer bits: its last part would be below
+// bf16's least normal number, 2^-126.)
 #include "q3cu_mma.cuh"
 #include "q3cu_paged.cuh"
 #include "q3cu_tcgen05.cuh"
@@ -86,6 +86,21 @@ __device__ __forceinline__ void load_eight(const float *p, float4 (&v)[2]) {
                  : "=f"(v[0].x), "=f"(v[0].y), "=f"(v[0].z), "=f"(v[0].w), "=f"(v[1].x), "=f"(v[1].y), "=f"(v[1].z),
                    "=f"(v[1].w)
                  : "l"(p) : "memory");
+}
+
+// Row r of an item once more from the formula, where that may give numbers; false where not.
+template <int STEP>
+__device__ __forceinline__ bool look_again(SecondLook<float> &second, const PagedKV &c, const PagedSeqs &b,
+                                           const PromptItem &it, int group, int r, const float *q, int64_t q_stride,
+                                           uint32_t *status, float4 &v) {
+    const int lane = threadIdx.x & 31, query = r / group, i = it.first + query, limit = it.seen(i);
+    const int last = it.seen(min(it.first + PF_ROWS / group, it.rows) - 1);
+    second.look(0, c, b, it.s, it.head, it.seen(it.first), min(it.len, (last + PF_KEYS - 1) / PF_KEYS * PF_KEYS));
+    const float4 x = load_quad(q + int64_t(it.base + i) * q_stride + int64_t(it.head * group + r - query * group) * HD + 4 * lane);
+    if (!second.wanted(limit, x)) return false;
+    v = attend_row<float, STEP>(c, b, it.s, it.head, limit,
+                          make_float4(x.x * ATT_SCALE, x.y * ATT_SCALE, x.z * ATT_SCALE, x.w * ATT_SCALE), status);
+    return true;
 }
 
 template <bool SPLIT>
@@ -378,17 +393,21 @@ prompt_f32_kernel(const PagedKV c, const PagedSeqs b, int rows, const float *q, 
                                *reinterpret_cast<const float4 *>(stage + l * (HD * 4) + ((lane ^ (l & 7)) << 4)));
             }
             __syncwarp();
-            // rows that came out as NaN, once more from the formula
+            // rows that came out as NaN, once more from the formula; the item is read anew, so that it takes no registers until
+            // then (1.2 us of the three prompts' 54)
             unsigned again = __ballot_sync(FULL, live && limit > 0 && nan && !(SPLIT && parts > 1));
-            while (again) {
-                const int l = __ffs(again) - 1;
-                again &= again - 1;
+            if (again) {
+                const PromptItem *same = &item_sh;
+                asm volatile("" : "+l"(same) :: "memory");
+                SecondLook<float> second;
                 __syncwarp();
-                const int il = __shfl_sync(FULL, i, l), n = __shfl_sync(FULL, limit, l), h = __shfl_sync(FULL, head, l);
-                float4 x = load_quad(q + int64_t(it.base + il) * q_stride + int64_t(h) * HD + 4 * lane);
-                x = make_float4(x.x * ATT_SCALE, x.y * ATT_SCALE, x.z * ATT_SCALE, x.w * ATT_SCALE);
-                store_quad(out + (int64_t(it.base + il) * n_heads + h) * HD + 4 * lane,
-                           attend_row<float>(c, b, it.s, it.head, n, x, status));
+                for (; again; again &= again - 1) {
+                    const int row = 32 * warp + __ffs(again) - 1, query = row / group;
+                    float4 v;
+                    if (look_again<8>(second, c, b, *same, group, row, q, q_stride, status, v))
+                        store_quad(out + (int64_t(same->base + same->first + query) * n_heads + same->head * group + row - query * group) * HD +
+                                       4 * lane, v);
+                }
             }
         }
         if constexpr (SPLIT) stat_sh[r] = make_float2(m, ok ? sum : -1.0f);
@@ -400,6 +419,7 @@ prompt_f32_kernel(const PagedKV c, const PagedSeqs b, int rows, const float *q, 
     if constexpr (SPLIT) {
         if (parts == 1 || !mine) return;                     // the same for all of a part's threads
         cluster_sync();
+        SecondLook<float> second;
         for (int r = prompt_part(PF_ROWS, parts, rank) + warp; r < prompt_part(PF_ROWS, parts, rank + 1); r += PF_THREADS / 32) {
             const int query = r / group, i = it.first + query, head = it.head * group + r - query * group;
             if (query >= queries) break;
@@ -407,14 +427,10 @@ prompt_f32_kernel(const PagedKV c, const PagedSeqs b, int rows, const float *q, 
             bool ok;
             float4 v = join_parts(smem_addr(tiles) + r * (HD * 4), smem_addr(&stat_sh[r]), r, parts, PF_LOG2, ok);
             if (!ok) continue;
-            float *dst = out + (int64_t(it.base + i) * n_heads + head) * HD + 4 * lane;
             if (limit <= 0) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (__any_sync(FULL, v.x != v.x || v.y != v.y || v.z != v.z || v.w != v.w)) {
-                const float4 x = load_quad(q + int64_t(it.base + i) * q_stride + int64_t(head) * HD + 4 * lane);
-                v = attend_row<float>(c, b, it.s, it.head, limit,
-                                      make_float4(x.x * ATT_SCALE, x.y * ATT_SCALE, x.z * ATT_SCALE, x.w * ATT_SCALE), status);
-            }
-            store_quad(dst, v);
+            if (__any_sync(FULL, v.x != v.x || v.y != v.y || v.z != v.z || v.w != v.w))
+                look_again<4>(second, c, b, it, group, r, q, q_stride, status, v);
+            store_quad(out + (int64_t(it.base + i) * n_heads + head) * HD + 4 * lane, v);
         }
         cluster_sync();                                      // no CTA's shared memory goes while others read it
     }

@@ -29,6 +29,10 @@ __host__ __device__ __forceinline__ void flag_bad_index(uint32_t *status) {
 #endif
 }
 
+__device__ __forceinline__ void flag_timeout(uint32_t *status) {
+    if (status) atomicOr(status, Q3CU_DEV_TIMEOUT);
+}
+
 // Keys a sequence holds: kv_len, no more than its table row has pages for (a
 // longer kv_len is flagged) and no fewer than none.
 __host__ __device__ __forceinline__ int paged_len(const PagedSeqs &b, const PagedKV &c, int s, uint32_t *status) {
@@ -127,12 +131,18 @@ __device__ __forceinline__ void store_quad(uint16_t *p, float4 v) {
     *reinterpret_cast<uint2 *>(p) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
 }
 
+// Whether none of them is infinite or NaN.
+__device__ __forceinline__ bool all_finite(float4 v) {
+    return fmaf(v.x, 0.0f, fmaf(v.y, 0.0f, fmaf(v.z, 0.0f, v.w * 0.0f))) == 0.0f;
+}
+
 // Attention of one query row and head by one warp, straight from the formula:
 // lane l holds elements 4l .. 4l+3 of q (scaled by 1/sqrt(128)), of every key
 // and value and of the result.  The running maximum and sum of the softmax, one pass over
-// the keys 0 .. n-1 of sequence s.  A score of -inf (an infinite key) weighs nothing; a row that has no other is 0 / 0.
-// Returns zeros for n = 0.
-template <typename TC>
+// the keys 0 .. n-1 of sequence s, STEP at a time (a page holds them all): 0.18 us a key by fours, 0.15 by eights, whose
+// registers cost every bf16 prompt 1 %.  A score of -inf (an infinite key) weighs nothing; a row that has no other is
+// 0 / 0.  Returns zeros for n = 0.
+template <typename TC, int STEP>
 __device__ __forceinline__ float4 attend_row(const PagedKV &c, const PagedSeqs &b, int s, int head, int n, float4 q,
                                              uint32_t *status) {
     const typename Elem<TC>::type *kp = static_cast<const typename Elem<TC>::type *>(c.k);
@@ -140,27 +150,114 @@ __device__ __forceinline__ float4 attend_row(const PagedKV &c, const PagedSeqs &
     const int lane = threadIdx.x & 31;
     float m = -INFINITY, sum = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int t = 0; t < n; ++t) {
+    for (int t = 0; t < n; t += STEP) {
         const int page = paged_page(b, c, s, t, lane == 0 ? status : nullptr);
-        float4 k = make_float4(0.0f, 0.0f, 0.0f, 0.0f), v = k;
-        if (page >= 0) {
-            const int64_t at = paged_at(c, page, head, t) + 4 * lane;
-            k = load_quad(kp + at);
-            v = load_quad(vp + at);
-        }
-        float d = fmaf(q.x, k.x, fmaf(q.y, k.y, fmaf(q.z, k.z, q.w * k.w)));
+        const int64_t at = page >= 0 ? paged_at(c, page, head, t) + 4 * lane : 0;
+        float4 k[STEP], v[STEP];
 #pragma unroll
-        for (int x = 16; x > 0; x >>= 1) d += __shfl_xor_sync(FULL, d, x);
-        const float nm = fmaxf(m, d), f = m == nm ? 1.0f : expf(m - nm);
-        const float p = d == -INFINITY ? 0.0f : expf(d - nm);              // also while nm is -inf
+        for (int u = 0; u < STEP; ++u) {
+            k[u] = v[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (page >= 0 && t + u < n) {
+                k[u] = load_quad(kp + at + u * HD);
+                v[u] = load_quad(vp + at + u * HD);
+            }
+        }
+        float d[STEP], nm = m;
+#pragma unroll
+        for (int u = 0; u < STEP; ++u) {
+            d[u] = fmaf(q.x, k[u].x, fmaf(q.y, k[u].y, fmaf(q.z, k[u].z, q.w * k[u].w)));
+#pragma unroll
+            for (int x = 16; x > 0; x >>= 1) d[u] += __shfl_xor_sync(FULL, d[u], x);
+            if (t + u >= n) d[u] = -INFINITY;
+            nm = fmaxf(nm, d[u]);
+        }
+        const float f = m == nm ? 1.0f : expf(m - nm);
         m = nm;
-        sum = fmaf(sum, f, p);
-        o = make_float4(fmaf(o.x, f, p * v.x), fmaf(o.y, f, p * v.y), fmaf(o.z, f, p * v.z), fmaf(o.w, f, p * v.w));
+        sum *= f;
+        o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+#pragma unroll
+        for (int u = 0; u < STEP; ++u) {
+            const float p = d[u] == -INFINITY ? 0.0f : expf(d[u] - nm);    // also while nm is -inf
+            sum += p;
+            o = make_float4(fmaf(p, v[u].x, o.x), fmaf(p, v[u].y, o.y), fmaf(p, v[u].z, o.z), fmaf(p, v[u].w, o.w));
+        }
+        // nothing changes a row of NaN any more
+        if (__all_sync(FULL, sum != sum || (o.x != o.x && o.y != o.y && o.z != o.z && o.w != o.w))) break;
     }
     if (n == 0) return o;
     const float r = 1.0f / sum;
     return make_float4(o.x * r, o.y * r, o.z * r, o.w * r);
 }
+
+// ---- rows that are computed again ----------------------------------------------------------------
+// A tile of rows under one kv head shares the products of its key tiles, so 0 times a value that a row does not see may
+// make that row NaN, and elements near the end of a type's range may overflow on the way.  Rows that come out as no
+// numbers are computed again from the formula, unless that can only give NaN once more: a key or value that is NaN, where
+// all else is ordinary, is not looked for again in every row that sees it.
+// What one warp finds out about a tile of rows.
+template <typename TC> struct SecondLook {
+    int tile = -1;           // looked at; of it:
+    int last;                // the last position that not all rows see whose value is no finite number, or -1
+    bool huge;               // the keys or values hold infinities or elements from 2^100 on
+    // The first row of tile `id` sees the keys 0 .. lo - 1, and its key tiles end at hi.
+    __device__ __forceinline__ void look(int id, const PagedKV &c, const PagedSeqs &b, int s, int head, int lo, int hi) {
+        if (tile == id) return;
+        tile = id;
+        last = -1;
+        huge = false;
+        typedef typename Elem<TC>::type E;
+        const int lane = threadIdx.x & 31;
+        for (int t = hi - 1; t >= lo && last < 0; t -= 4) {
+            bool odd[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int page = t - u >= lo ? paged_page(b, c, s, t - u, nullptr) : -1;
+                odd[u] = page >= 0 && !all_finite(load_quad(static_cast<const E *>(c.v) + paged_at(c, page, head, t - u) + 4 * lane));
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (__any_sync(FULL, odd[u]) && last < 0) last = t - u;
+        }
+        // the positions of a page lie one after the other: 16 bytes a lane
+        constexpr int STEP = 16 / Elem<TC>::BYTES * 32;      // elements of a load by the warp
+        for (int t = 0; t < hi && !huge; t += 16) {
+            const int page = paged_page(b, c, s, t, nullptr);
+            if (page < 0) continue;
+            const int64_t at = paged_at(c, page, head, t) + lane * (16 / Elem<TC>::BYTES);
+            const int n = min(16, hi - t) * HD / STEP;       // loads (a position is half of one, or one)
+            for (int side = 0; side < 2; ++side) {
+                const E *p = static_cast<const E *>(side ? c.v : c.k) + at;
+                uint32_t top = 0;                            // the largest magnitude that is no NaN
+#pragma unroll 4
+                for (int u = 0; u < n; ++u) top = max(top, magnitude(p + u * STEP));
+                if (n * STEP < min(16, hi - t) * HD && lane < 16) top = max(top, magnitude(p + n * STEP));
+                huge |= top >= 0x71800000u;
+            }
+            huge = __any_sync(FULL, huge);
+        }
+    }
+    // whether a row that sees `limit` keys is to be computed again (q: its query, a quad a lane)
+    __device__ __forceinline__ bool wanted(int limit, float4 q) const {
+        const float top = fmaxf(fmaxf(fabsf(q.x), fabsf(q.y)), fmaxf(fabsf(q.z), fabsf(q.w)));
+        return huge || limit <= last || __any_sync(FULL, top >= 0x1p100f);
+    }
+    static __device__ __forceinline__ uint32_t no_nan(uint32_t bits) {
+        bits &= 0x7fffffffu;
+        return bits > 0x7f800000u ? 0u : bits;
+    }
+    // the largest magnitude, as binary32's bits, of 16 bytes of elements that are no NaN
+    static __device__ __forceinline__ uint32_t magnitude(const typename Elem<TC>::type *p) {
+        const uint4 w = *reinterpret_cast<const uint4 *>(p);
+        const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (Elem<TC>::BYTES == 4) top = max(top, no_nan(x[i]));
+            else top = max(top, max(no_nan(x[i] << 16), no_nan(x[i] & 0xffff0000u)));
+        }
+        return top;
+    }
+};
 
 // ---- the work items of a prompt launch ------------------------------------------------------
 // A sequence's rows fall into blocks of `per_block` queries; a block under one kv head is an item.  Its work is the

@@ -179,3 +179,92 @@ def test_prompt_items_in_any_order(tmp_path):
                    check=True)
     out = subprocess.run([exe], capture_output=True, text=True, timeout=120)
     assert out.returncode == 0 and out.stdout.strip() == "ok", out.stdout + out.stderr
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,rows", [(4096, 4096), (20000, 24)])
+def test_a_nan_is_not_looked_for_in_every_row(q3, dtype, n, rows):
+    """A NaN that all rows see, in a key or in one column of a value: NaN where the formula has it, every other column
+    right, and no row-by-row computation, which would take some hundred times the call's usual time."""
+    p = Paged([n], 2, 64, dtype, seed=130).fill(131)
+    q = queries(rows, 8, dtype, 132)
+    handles, out = p.handles([0, rows]), torch.empty_like(q)
+    page, slot = p.where(0, [0])
+    pick = torch.tensor(sorted({0, 1, rows // 3, rows - 2, rows - 1}), device="cuda")
+    seen = pick + (n - rows + 1)
+
+    def call():
+        start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        start.record()
+        q3.attention_prompt(*handles, q, out=out)
+        end.record()
+        end.synchronize()
+        return start.elapsed_time(end)
+
+    call()
+    usual = min(call() for _ in range(5))
+    p.v[page, :, slot, 3] = NAN
+    assert min(call() for _ in range(3)) < 60 * usual
+    assert out[:, :, 3].isnan().all() and not out[:, :, 4:].isnan().any()
+    k, v = p.rows(0)
+    v[0, :, 3] = 0.0
+    got = out[pick].double()
+    got[:, :, 3] = attend(q[pick].double(), k, v, seen)[0][:, :, 3]
+    check_attention(got, q[pick], k, v, seen, dtype, rounding(dtype))
+    p.k[page, 0, slot, 7] = NAN
+    assert min(call() for _ in range(3)) < 60 * usual
+    assert out[:, :4].isnan().all() and not out[:, 4:, 4:].isnan().any()
+    assert q3.device_status() == 0
+
+
+def test_values_near_the_end_of_the_range(q3):
+    """bf16 values whose weighted sums would pass the range while the maximum lags: the result is finite, in whole and in
+    shared items."""
+    for n, rows in ((300, 300), (2000, 20)):
+        p = Paged([n], 2, 16, BF16, seed=133).fill(134)
+        page, slot = p.where(0, range(n))
+        p.v[page, :, slot, 11] = 3e36
+        ramp = torch.arange(n, device="cuda")[:, None] * (0.02 if n == 300 else 0.003)    # later keys score higher
+        p.k[page, :, slot, 0] = ramp.to(BF16)
+        q = queries(rows, 8, BF16, 135)
+        q[:, :, 0] = 8.0
+        got = q3.attention_prompt(*p.handles([0, rows]), q)
+        assert torch.isfinite(got).all()
+        check_attention(got, q, *p.rows(0), range(n - rows + 1, n + 1), BF16, H)
+    assert q3.device_status() == 0
+
+
+@pytest.mark.parametrize("n,rows", [(300, 300), (2000, 20)])
+def test_f32_elements_that_their_parts_do_not_hold(q3, n, rows):
+    """Elements that round to infinity in bf16: a value, and queries against keys that are as small."""
+    p = Paged([n], 2, 16, F32, seed=136).fill(137)
+    page, slot = p.where(0, range(n))
+    at = n - rows // 2
+    p.v[page[at], 1, slot[at], 11] = 3.4e38
+    p.k[page, :, slot, 0] *= 3e-38
+    q = queries(rows, 8, F32, 138)
+    q[::2, :, 0] = 3.4e38
+    got = q3.attention_prompt(*p.handles([0, rows]), q)
+    check_attention(got, q, *p.rows(0), range(n - rows + 1, n + 1), F32)
+    assert torch.isfinite(got).all() and q3.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,rows,at", [(300, 300, 200), (2000, 20, 1990)])
+def test_seen_and_hidden_nans(q3, dtype, n, rows, at):
+    """A NaN that every row sees in one column and one that only the rows from `at` on see in another."""
+    p = Paged([n], 2, 16, dtype, seed=139).fill(140)
+    page, slot = p.where(0, [0, at])
+    p.v[page[0], :, slot[0], 3] = NAN
+    p.v[page[1], :, slot[1], 50] = NAN
+    q = queries(rows, 8, dtype, 141)
+    got = q3.attention_prompt(*p.handles([0, rows]), q).double()
+    sees = torch.arange(n - rows, n, device="cuda") >= at
+    assert got[:, :, 3].isnan().all() and got[sees][:, :, 50].isnan().all()
+    k, v = p.rows(0)
+    v[0, :, 3] = v[at, :, 50] = 0.0
+    want = attend(q.double(), k, v, range(n - rows + 1, n + 1))[0]
+    got[:, :, 3] = want[:, :, 3]
+    got[sees, :, 50] = want[sees][:, :, 50]
+    check_attention(got, q, k, v, range(n - rows + 1, n + 1), dtype, rounding(dtype))
+    assert q3.device_status() == 0
