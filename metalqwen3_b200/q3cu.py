@@ -168,7 +168,7 @@ class KVCache:
                 n_pages > 1 and k.stride(0) != v.stride(0)):
             raise ValueError("a page must be contiguous, and k and v have one page stride")
         _tensor(k, "k"), _tensor(v, "v")
-        self.k, self.v, self.n_kv = k, v, n_kv
+        self.k, self.v, self.n_kv, self.device = k, v, n_kv, k.get_device()
         self.c = _KVCache(k.data_ptr(), v.data_ptr(), k.stride(0) if n_pages > 1 else n_kv * size * hd, n_pages, n_kv,
                           size, hd, _dtype(k))
         self.ref = C.byref(self.c)
@@ -183,8 +183,9 @@ class KVBatch:
         i32 = kv_len.new_empty(0).int().dtype
         if pages.dim() != 2:
             raise ValueError(f"pages must be [n_seqs][max_pages], it is {list(pages.shape)}")
+        self.device = kv_len.get_device()
         for t, what, shape in ((kv_len, "kv_len", (n,)), (pages, "pages", (n, pages.shape[1])), (row_off, "row_off", (n + 1,))):
-            if t is not None and not _tensor(t, what, i32, shape).is_contiguous():
+            if t is not None and not _tensor(t, what, i32, shape, self.device).is_contiguous():
                 raise ValueError(f"{what} must be contiguous")
         self.kv_len, self.pages, self.row_off = kv_len, pages, row_off
         self.c = _KVBatch(None if row_off is None else row_off.data_ptr(), kv_len.data_ptr(), pages.data_ptr(), n,
@@ -359,12 +360,21 @@ class Q3CU:
         return xb, probs
 
     # -- the paged key-value cache -----------------------------------------------
+    def _elsewhere(self, cache, batch, work=None):
+        """Refuses what lies on another device than the context's, which its kernels could not reach."""
+        for what, t in (("cache", cache), ("batch", batch)):
+            if t.device != self.device:
+                raise ValueError(f"the {what} must be on the context's GPU, it is on cuda:{t.device}")
+        raise ValueError(f"work must be contiguous memory on the context's GPU, it is on {work.device}")
+
     def kv_append(self, cache, batch, q, k, v, q_norm=None, k_norm=None, theta=1e6, eps=1e-6, q_out=None,
                   out_dtype=None, stream=None):
         """QK-norm (where weights are given) and rotation of the packed rows q [rows][n_heads][128] and
         k [rows][n_kv][128] (q may be None); keys and values into the cache; returns the rotated queries
         (out_dtype, the cache's type by default, or q_out).  q, k, v may be slices of one projection's rows."""
         dev, dtype = self.device, k.dtype
+        if cache.device != dev or batch.device != dev:
+            self._elsewhere(cache, batch)
         kv_stride, rows, _, kp = _rows(k, "k", None, cache.n_kv, None, dev)
         v_stride, _, _, vp = _rows(v, "v", dtype, cache.n_kv, rows, dev)
         if v_stride != kv_stride:
@@ -402,6 +412,9 @@ class Q3CU:
 
     def attention_paged(self, cache, batch, q, out=None, work=None, stream=None):
         """One new token per sequence: q [n_seqs][n_heads][128] over each sequence's kv_len positions."""
+        if cache.device != self.device or batch.device != self.device or (
+                work is not None and (work.get_device() != self.device or not work.is_contiguous())):
+            self._elsewhere(cache, batch, work)
         stride, rows, heads, qp = _rows(q, "q", None, None, batch.c.n_seqs, self.device)
         if out is None:
             out = self._make(stream, self.torch.empty, (rows, heads, 128), dtype=q.dtype, device=q.device)
@@ -419,6 +432,8 @@ class Q3CU:
     def attention_prompt(self, cache, batch, q, out=None, stream=None):
         """Causal attention of the packed rows q [rows][n_heads][128] over the cache, which holds their
         keys and values; rows behind the last sequence are not written."""
+        if cache.device != self.device or batch.device != self.device:
+            self._elsewhere(cache, batch)
         stride, rows, heads, qp = _rows(q, "q", None, None, None, self.device)
         if out is None:
             out = self._make(stream, self.torch.empty, (rows, heads, 128), dtype=q.dtype, device=q.device)

@@ -104,3 +104,28 @@ def test_calls_make_their_memory_on_their_stream(binding, given):
     assert {args[-1] for name, args in binding.lib.calls if "workspace" not in name} == {on.cuda_stream}
     if given:
         assert binding.attention_paged_workspace(cache, 4, stream=stream).made_on is on
+
+
+def test_memory_elsewhere_is_refused(binding):
+    """A cache, a batch or a workspace on another GPU or on the host, or a workspace that is not all there, reaches no
+    kernel."""
+    cache, batch = cache_and_batch()
+    far_cache, far_batch = cache_and_batch(1)
+    q, k = Tensor((3, 4, 128)), Tensor((3, 2, 128))
+    for c, b in ((far_cache, batch), (cache, far_batch)):
+        for call in (lambda: binding.kv_append(c, b, q, k, k), lambda: binding.attention_paged(c, b, q),
+                     lambda: binding.attention_prompt(c, b, q)):
+            with pytest.raises(ValueError, match="must be on the context's GPU"):
+                call()
+    spread = Tensor((1,), torch.uint8)
+    spread.t, spread.nbytes = spread.t.expand(1 << 20), 1 << 20
+    for work in (Tensor((1 << 20,), torch.uint8, -1), Tensor((1 << 20,), torch.uint8, 1), spread):
+        with pytest.raises(ValueError, match="work must be contiguous memory on the context's GPU"):
+            binding.attention_paged(cache, batch, q, work=work)
+    assert not binding.lib.calls
+    i32 = torch.int32
+    for pages, row_off in ((1, 0), (0, 1), (0, -1)):
+        with pytest.raises(ValueError, match="must be on the context's GPU"):
+            q3cu.KVBatch(Tensor((3,), i32), Tensor((3, 2), i32, pages), Tensor((4,), i32, row_off))
+    binding.attention_paged(cache, batch, q, work=Tensor((1 << 20,), torch.uint8))
+    assert binding.lib.calls
