@@ -219,7 +219,7 @@ typedef struct {
     const int32_t *kv_len;   /* [n_seqs] */
     const int32_t *pages;    /* [n_seqs][max_pages] */
     int32_t n_seqs;              /* at most 2^24 */
-    int32_t max_pages;           /* max_pages * page_size < 2^31 */
+    int32_t max_pages;           /* max_pages * page_size <= 2^31 - 512 */
 } q3cu_kv_batch;
 
 /* QK-RMSNorm and rotation of the packed rows, keys and values into the cache

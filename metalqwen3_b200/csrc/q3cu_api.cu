@@ -503,9 +503,10 @@ static q3cu_status check_paged(const char *op, const q3cu_kv_cache *cache, const
     if (n_heads < 0 || n_heads % cache->n_kv || n_heads / cache->n_kv > q3::PAGED_GROUP_MAX)
         return fail(Q3CU_ERR_INVALID, "%s: n_heads %d is not a multiple of n_kv %d up to 16 times it", op, n_heads,
                     cache->n_kv);
-    if (int64_t(batch->max_pages) * cache->page_size > INT32_MAX)
-        return fail(Q3CU_ERR_INVALID, "%s: max_pages %d * page_size %d does not fit 31 bits", op, batch->max_pages,
-                    cache->page_size);
+    // positions are 32-bit, and lengths are rounded up to whole key tiles
+    if (int64_t(batch->max_pages) * cache->page_size > q3::PAGED_LEN_MAX)
+        return fail(Q3CU_ERR_INVALID, "%s: max_pages %d * page_size %d is more than %d", op, batch->max_pages,
+                    cache->page_size, q3::PAGED_LEN_MAX);
     const int64_t dense = int64_t(cache->n_kv) * cache->page_size * q3::PAGED_HD;
     if (cache->page_stride < dense || cache->page_stride > (int64_t(1) << 36))
         return fail(Q3CU_ERR_INVALID, "%s: page_stride %lld, a page has %lld elements", op,

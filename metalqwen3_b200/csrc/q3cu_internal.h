@@ -146,6 +146,7 @@ cudaError_t launch_attention_rows(const float *q, const float *kc, const float *
 // ---- the paged key-value cache (k_append.cu, k_paged.cu, k_prompt.cu) ----
 constexpr int PAGED_HD = 128;          // head_dim
 constexpr int PAGED_GROUP_MAX = 16;    // query heads to a kv head
+constexpr int PAGED_LEN_MAX = INT32_MAX - 511;                 // positions of a sequence: 2^31 - 512
 struct PagedKV {                       // q3cu_kv_cache, checked
     void *k, *v;
     int64_t page_stride;               // elements
