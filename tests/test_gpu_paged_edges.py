@@ -268,3 +268,37 @@ def test_seen_and_hidden_nans(q3, dtype, n, rows, at):
     got[sees, :, 50] = want[sees][:, :, 50]
     check_attention(got, q, k, v, range(n - rows + 1, n + 1), dtype, rounding(dtype))
     assert q3.device_status() == 0
+
+
+def mean_error(got, want):
+    return float((got.double() - want).abs().mean() / want.abs().mean())
+
+
+def parts(x, count):
+    """x (binary64) rounded to a sum of `count` bf16."""
+    left, total = x.clone(), torch.zeros_like(x)
+    for _ in range(count):
+        part = left.to(BF16).double()
+        total, left = total + part, left - part
+    return total
+
+
+@pytest.mark.parametrize("n,rows", [(1, 1), (64, 64), (513, 40), (1500, 600), (4096, 40), (4096, 600)])
+def test_f32_results_keep_all_their_parts(q3, n, rows):
+    """f32 results within 1e-6 = 17 u of the formula on average.  Roundings to nearest average out: a score's chains of at
+    most 128 products and the exponential move a weight by some 10 u, the sums of the weighted values, at most n / 64
+    tiles one after the other, by sqrt(n / 64) u.  A third bf16 part that is lost from an operand does not pass: it costs
+    some 2e-6 = 34 u, as the oracle shows."""
+    p = Paged([n], 2, 16, F32, seed=142).fill(143)
+    q = queries(rows, 8, F32, 144)
+    (k, v), seen = p.rows(0), range(n - rows + 1, n + 1)
+    want = attend(q.double(), k, v, seen)[0]
+    assert mean_error(q3.attention_prompt(*p.handles([0, rows]), q), want) < 1e-6
+    assert mean_error(q3.attention_paged(*p.handles(), q[-1:]), want[-1:]) < 1e-6
+    assert mean_error(attend(q.double(), k, parts(v, 2), seen)[0], want) > 1.2e-6
+    if n > 1:
+        assert mean_error(attend(parts(q.double(), 2), k, v, seen)[0], want) > 1.2e-6
+    b = Paged([n], 2, 16, BF16, seed=145).fill(146)
+    k, v = b.rows(0)
+    one = attend(q[-1:].double(), k, v, [n])[0]
+    assert mean_error(q3.attention_paged(*b.handles(), q[-1:]), one) < 1e-6
