@@ -7,7 +7,7 @@ import subprocess
 import pytest
 import torch
 
-from test_gpu_paged import BF16, F32, H, NAN, Paged, attend, check_attention, queries
+from test_gpu_paged import BF16, F32, H, NAN, Paged, attend, check_attention, offsets, queries
 
 pytestmark = pytest.mark.gpu
 
@@ -302,3 +302,24 @@ def test_f32_results_keep_all_their_parts(q3, n, rows):
     k, v = b.rows(0)
     one = attend(q[-1:].double(), k, v, [n])[0]
     assert mean_error(q3.attention_paged(*b.handles(), q[-1:]), one) < 1e-6
+
+
+@pytest.mark.parametrize("cache_t", [F32, BF16])
+@pytest.mark.parametrize("heads,n_kv", [(7, 1), (9, 1), (11, 1), (26, 2), (45, 3)])
+def test_odd_groups(q3, cache_t, heads, n_kv):
+    """Groups of query heads that fill neither a tile's 128 rows nor a product's eight columns."""
+    rows, lens = [70, 33, 0, 5, 1], [700, 33, 0, 64, 1]
+    p = Paged(lens, n_kv, 32, cache_t, seed=147).fill(148)
+    off = offsets(rows)
+    for io in (F32, BF16):
+        q = queries(5, heads, io, 149)
+        got = q3.attention_paged(*p.handles(), q)
+        for s, n in enumerate(lens):
+            check_attention(got[s:s + 1], q[s:s + 1], *p.rows(s), [n], io)
+    q = queries(off[-1], heads, cache_t, 150)
+    got = q3.attention_prompt(*p.handles(off), q)
+    for s, (r, n) in enumerate(zip(rows, lens)):
+        mine = slice(off[s], off[s + 1])
+        if r:
+            check_attention(got[mine], q[mine], *p.rows(s), range(n - r + 1, n + 1), cache_t, rounding(cache_t))
+    assert q3.device_status() == 0
