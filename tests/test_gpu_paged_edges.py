@@ -323,3 +323,36 @@ def test_odd_groups(q3, cache_t, heads, n_kv):
         if r:
             check_attention(got[mine], q[mine], *p.rows(s), range(n - r + 1, n + 1), cache_t, rounding(cache_t))
     assert q3.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_thousands_of_sequences(q3, dtype):
+    """Prompts of one to three rows and empty ones, thousands of them: results, and a time that grows with their number and
+    not with its square."""
+    from metalqwen3_b200.q3cu import KVBatch, KVCache
+    k, v = (queries(64 * 16, 2, dtype, s).view(64, 16, 2, 128).transpose(1, 2).contiguous() for s in (151, 152))
+    cache, usual = KVCache(k, v), []
+    for n in (2500, 20000):
+        rows = torch.arange(n) % 4
+        off = torch.cat([torch.zeros(1, dtype=torch.long), rows.cumsum(0)])
+        lens = rows + torch.arange(n) % 13
+        table = (torch.arange(n) * 7 % 64)[:, None]
+        batch = KVBatch(*(t.int().cuda() for t in (lens, table, off)))
+        q = queries(int(off[-1]), 4, dtype, 153)
+        got = q3.attention_prompt(cache, batch, q)
+        times = []
+        for _ in range(4):
+            start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            start.record()
+            q3.attention_prompt(cache, batch, q, out=got)
+            end.record()
+            end.synchronize()
+            times.append(start.elapsed_time(end))
+        usual.append(min(times))
+        for s in list(range(0, n, n // 37)) + [n - 1]:
+            a, b, page, m = int(off[s]), int(off[s + 1]), int(table[s]), int(lens[s])
+            if b > a:
+                check_attention(got[a:b], q[a:b], k[page].transpose(0, 1)[:m].double(), v[page].transpose(0, 1)[:m].double(),
+                                range(m - (b - a) + 1, m + 1), dtype, rounding(dtype))
+    assert usual[1] < 24 * usual[0], usual                   # 8 times the sequences
+    assert q3.device_status() == 0
