@@ -356,3 +356,22 @@ def test_thousands_of_sequences(q3, dtype):
                                 range(m - (b - a) + 1, m + 1), dtype, rounding(dtype))
     assert usual[1] < 24 * usual[0], usual                   # 8 times the sequences
     assert q3.device_status() == 0
+
+
+def test_empty_slots_between_sequences(q3):
+    """Runs of tiles that go from one sequence over thousands of empty ones to the next."""
+    from metalqwen3_b200.q3cu import KVBatch, KVCache
+    n, pages = 30000, 40
+    k, v = (queries(64 * 16, 2, BF16, s).view(64, 16, 2, 128).transpose(1, 2).contiguous() for s in (155, 156))
+    table = (torch.arange(n)[:, None] * 5 + torch.arange(pages)) % 64
+    q = queries(n, 4, BF16, 157)
+    for busy in ([0, 1, 31, 32, 33, 20000, 29999], list(range(300)) + list(range(29700, 30000))):
+        lens = torch.zeros(n, dtype=torch.int32)
+        lens[busy] = torch.tensor([640 - 3 * (i % 200) for i in range(len(busy))], dtype=torch.int32)
+        got = q3.attention_paged(KVCache(k, v), KVBatch(lens.cuda(), table.int().cuda()), q)
+        for s in busy[::max(1, len(busy) // 40)] + [busy[-1]]:
+            m = int(lens[s])
+            kk, vv = (t[table[s]].transpose(0, 1).reshape(2, -1, 128).transpose(0, 1)[:m].double() for t in (k, v))
+            check_attention(got[s:s + 1], q[s:s + 1], kk, vv, [m], BF16)
+        assert (got[(lens == 0).cuda()] == 0).all() and not got[(lens > 0).cuda()].isnan().any()
+    assert q3.device_status() == 0
