@@ -215,7 +215,8 @@ typedef struct {
  * kernels run.  pages[s][i] is the page of positions i * page_size ...;
  * entries beyond the last position are not read. */
 typedef struct {
-    const int32_t *row_off;  /* [n_seqs + 1], rising from 0 (not read by q3cu_attention_paged) */
+    const int32_t *row_off;  /* [n_seqs + 1], rising from 0 to no more than the call's rows (not read by
+                                q3cu_attention_paged) */
     const int32_t *kv_len;   /* [n_seqs] */
     const int32_t *pages;    /* [n_seqs][max_pages] */
     int32_t n_seqs;              /* at most 2^24 */
@@ -268,8 +269,11 @@ q3cu_status q3cu_attention_paged_workspace(q3cu_ctx *ctx, int n_heads, int n_kv,
  * rows; out: [rows][n_heads][128], other memory than q.  Both of the cache's type: bf16 runs on the tensor cores with
  * probabilities rounded to bf16 (the sums binary32), f32 with binary32's
  * accuracy (elements below 2^-109 keep fewer bits).  Grouped heads, scale, softmax, empty rows, unused page space, bad
- * pages and alignment as above.  Sequences with one row are allowed, but
- * q3cu_attention_paged is made for them. */
+ * pages and alignment as above.  A NaN or infinity at a position changes no row
+ * before it; where one would, the row is computed again by itself, at some 0.2 us
+ * a key (a bf16 prompt does so for a second at most in one tile of rows; what is
+ * left then stays NaN and Q3CU_DEV_TIMEOUT is set).  Sequences with one row are
+ * allowed, but q3cu_attention_paged is made for them. */
 q3cu_status q3cu_attention_prompt(q3cu_ctx *ctx, const q3cu_kv_cache *cache, const q3cu_kv_batch *batch,
                                   int64_t rows, const void *q, q3cu_dtype dtype, int64_t q_stride, int n_heads,
                                   void *out, q3cu_stream stream);

@@ -32,7 +32,10 @@
 // zero in registers: unused page space may hold anything.
 //
 // Measured: 64 sequences of up to 16,384 (32/8 heads, f32 queries, bf16 cache)
-// 331 us, 6.4 TB/s; one of 100,003 (bf16) 72 to 75 us, 5.6 TB/s, where the CTAs'
+// 332 to 345 us, 6.1 to 6.4 TB/s; of up to 8,192 over an f32 cache (32/8) 341 us, 6.5
+// TB/s, but 83 us, 3.4 TB/s, with 16 query heads to a kv head (instructions of two
+// blocks of products to each key, and a join of 4,720 CTAs; bf16 51 us, 2.7 TB/s);
+// one of 100,003 (bf16) 71 us, 5.8 TB/s, where the CTAs'
 // equal shares end up to 12 us apart; one of 512 (16/8, f32) 8.5 us, all latency.
 #include "q3cu_mma.cuh"
 #include "q3cu_paged.cuh"

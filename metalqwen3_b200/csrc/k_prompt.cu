@@ -33,14 +33,15 @@
 // Bound by the tensor cores and what keeps them waiting: a step (128 keys, two
 // row tiles) has 2,048 cycles of products and takes 2,990, the time from a tile's
 // last probabilities to its next scores and through the softmax, which the other
-// tile fills in part.  A prompt of 16,384 (40/8 heads) measured 2.22 ms, 1,238
-// TFLOP/s, at 1.6 GHz under the power cap; 2,043 rows in chunks behind prefixes of up
-// to 8,192 (32/8) 178 us, 988 TFLOP/s; 4,096 rows in six prompts (32/8) 50 us.
+// tile fills in part.  Over changing inputs a prompt of 16,384 (40/8 heads) takes
+// 2.55 ms, 1,078 TFLOP/s, at 1.6 GHz under the power cap; 2,043 rows in chunks behind
+// prefixes of up to 8,192 (32/8) 200 us, 880 TFLOP/s; 4,096 rows in six prompts (32/8)
+// 54 us.  A replayed graph on one input: 2.15 to 2.3 ms, 175 and 50 us.
 // Tensor memory (512 columns): S0, S1, O0, O1; P_t lies over the first half of S_t.
 //
 // With few items (prompt_tc_kernel<true>) a cluster of up to eight CTAs takes one, each a part of its key tiles, and joins
-// the parts through shared memory (join_parts): 16 rows behind 8,000 positions (32/8 heads) 120 -> 26 us, 100 rows
-// behind 8,000 138 -> 38 us, 30 behind 30,000 440 -> 69 us.
+// the parts through shared memory (join_parts): 16 rows behind 8,000 positions (32/8 heads) 120 -> 28 us, 100 rows
+// behind 8,000 138 -> 36 us, 30 behind 30,000 440 -> 62 us.  Up to 64 of 148 SMs work then (8 kv heads).
 //
 // Masks: keys at and beyond the row's limit become -inf before the maximum.
 // Their probability is exactly 0, but 0 times a NaN or an infinity in V is not:
@@ -52,7 +53,8 @@
 // the row (SecondLook): a prompt of 4,096 rows (32/8) takes 0.14 ms, 1.3 with a NaN
 // that all rows see, and 24 with one in the last value, which spoils a tile.
 //
-// Every wait is bounded; a wait that gives up sets Q3CU_DEV_TIMEOUT and the CTA
+// Every wait is bounded (2 s; the longest, for the next item, lasts as long as an
+// item, some 10 ns a key); a wait that gives up sets Q3CU_DEV_TIMEOUT and the CTA
 // drains its own copies and products, frees tensor memory and returns.  So that no
 // other warp's wait gives up meanwhile, a warp computes rows again for a second at
 // most; past that (32 rows of 170,000 keys) the rest stay NaN, with the same bit set.

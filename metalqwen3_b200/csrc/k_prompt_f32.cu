@@ -24,12 +24,13 @@
 // and the probabilities' parts over them, the tile's P V 384-511.
 //
 // With fewer items than SMs a cluster of up to eight CTAs takes an item, each a part of its key tiles, and joins the
-// parts through shared memory (join_parts): 16 rows behind 8,000 positions (32/8 heads) 260 -> 45 us, 30 behind 30,000
-// 1,140 -> 150 us.
+// parts through shared memory (join_parts): 16 rows behind 8,000 positions (32/8 heads) 260 -> 51 us, 30 behind 30,000
+// 1,140 -> 147 us.
 //
 // Bound by the instructions that split, exponentiate and add, beside a tensor pipe that is busy 72 % of the cycles
-// when the prompt is long: 4,096 rows (32/8 heads) take 606 to 650 us (1.3 PFLOP/s of bf16 parts, at 1.6 GHz under
-// the power cap), 2,000 rows in three prompts (16/8) 52 us, of which the longest prompt's last block is 42.
+// when the prompt is long: 4,096 rows (32/8 heads) take 584 us in a replayed graph on one input and 665 over changing
+// inputs (1.2 PFLOP/s of bf16 parts, at 1.6 GHz under the power cap), 2,000 rows in three prompts (16/8) 54 and 56 us,
+// of which the longest prompt's last block is 42.
 // Measured and left out: two threads to a row (they and the splitting warps then spill registers: 80 us for the three
 // prompts), the next tile's loads ahead of this tile's split (57 us: the splitting warps then keep the rows' warps
 // waiting for issue slots), parts by truncation in place of rounding (57 us, and a larger error).
