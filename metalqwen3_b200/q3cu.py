@@ -223,9 +223,12 @@ class Q3CU:
         that stream's own: what lies free in the current stream's may still be in use by work that is pending there."""
         if stream is None:
             return make(*args, **kwargs)
-        with self.torch.cuda.stream(stream):
+        cuda = self.torch.cuda
+        if not isinstance(stream, cuda.Stream):      # anything with a stream's handle
+            stream = cuda.ExternalStream(stream.cuda_stream, self.device)
+        with cuda.stream(stream):
             t = make(*args, **kwargs)
-        t.record_stream(self.torch.cuda.current_stream(self.device))       # where the caller may read it
+        t.record_stream(cuda.current_stream(self.device))       # where the caller may read it
         return t
 
     def close(self):

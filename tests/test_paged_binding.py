@@ -56,7 +56,11 @@ def binding():
     main = Stream(7)
 
     class Cuda:
-        current = main
+        current, Stream = main, Stream
+
+        @staticmethod
+        def ExternalStream(handle, device):
+            return Stream(handle)
 
         @contextlib.contextmanager
         def stream(self, s):
@@ -104,6 +108,16 @@ def test_calls_make_their_memory_on_their_stream(binding, given):
     assert {args[-1] for name, args in binding.lib.calls if "workspace" not in name} == {on.cuda_stream}
     if given:
         assert binding.attention_paged_workspace(cache, 4, stream=stream).made_on is on
+
+
+def test_a_stream_known_by_its_handle(binding):
+    """What has a stream's handle and nothing else of torch's streams."""
+    class Handle:
+        cuda_stream = 11
+
+    cache, batch = cache_and_batch()
+    binding.attention_paged(cache, batch, Tensor((3, 4, 128)), stream=Handle())
+    assert [t.made_on.cuda_stream for t in binding.torch.made] == [11, 11]
 
 
 def test_memory_elsewhere_is_refused(binding):
