@@ -84,6 +84,13 @@ public:
                   const void *v, q3cu_dtype dt, int64_t q_stride, int64_t kv_stride, int n_heads, const float *q_norm,
                   const float *k_norm, void *q_out, q3cu_dtype q_dt, q3cu_stream stream, float theta = 1e6f,
                   float eps = 1e-6f);
+    // with the rotation that `rope` describes (q3cu_kv_append_rope), and rows read back (q3cu_kv_read)
+    void kvAppend(const q3cu_kv_cache &cache, const q3cu_kv_batch &batch, int64_t rows, const void *q, const void *k,
+                  const void *v, q3cu_dtype dt, int64_t q_stride, int64_t kv_stride, int n_heads, const float *q_norm,
+                  const float *k_norm, void *q_out, q3cu_dtype q_dt, q3cu_stream stream, const q3cu_rope &rope,
+                  float eps = 1e-6f);
+    void kvRead(const q3cu_kv_cache &cache, const q3cu_kv_batch &batch, int64_t rows, void *k, void *v, q3cu_dtype dt,
+                int64_t kv_stride, q3cu_stream stream);
     size_t attentionPagedWorkspace(int n_heads, int n_kv);
     void attentionPaged(const q3cu_kv_cache &cache, const q3cu_kv_batch &batch, const void *q, q3cu_dtype dt,
                         int64_t q_stride, int n_heads, void *work, size_t work_bytes, void *out, q3cu_stream stream);

@@ -57,7 +57,11 @@ typedef enum {
     Q3CU_ERR_FORMAT = 10     /* checkpoint header: bad magic, version or group size     */
 } q3cu_status;
 
-typedef enum { Q3CU_F32 = 0, Q3CU_BF16 = 1 } q3cu_dtype;
+typedef enum {
+    Q3CU_F32 = 0,
+    Q3CU_BF16 = 1,
+    Q3CU_Q8_0 = 8            /* of a paged cache only (q3cu_kv_cache_q8) */
+} q3cu_dtype;
 
 /* Bits of the device status word (q3cu_device_status). */
 #define Q3CU_DEV_BAD_INDEX 0x1u
@@ -206,6 +210,19 @@ typedef struct {
     int32_t dtype;           /* q3cu_dtype of k and v */
 } q3cu_kv_cache;
 
+/* A cache of Q8_0 values: `codes` has dtype Q3CU_Q8_0, its k and v are pages of
+ * int8 codes, its page_stride is a multiple of 16; every 64 codes of a row have
+ * a scale beside them.  A position and kv head take 136 bytes of k and of v, where bf16
+ * takes 256.  The calls below take it as &cache.codes: a q3cu_kv_cache of dtype
+ * Q3CU_Q8_0 is always the first member of one of these.  A scale that is
+ * infinite or NaN makes NaN of what it multiplies. */
+typedef struct {
+    q3cu_kv_cache codes;
+    float *k_scale, *v_scale;    /* pages of [n_kv][page_size][2], 16-byte aligned (device) */
+    int64_t scale_stride;        /* floats between the starts of two pages' scales: at least n_kv * page_size * 2,
+                                    and a multiple of 4 */
+} q3cu_kv_cache_q8;
+
 /* The packed token rows of n_seqs sequences.  Sequence s owns rows row_off[s]
  * .. row_off[s+1]-1, the last of which is at position kv_len[s] - 1: kv_len
  * counts the sequence's positions with the new rows.  Rows at or behind
@@ -240,6 +257,42 @@ q3cu_status q3cu_kv_append(q3cu_ctx *ctx, const q3cu_kv_cache *cache, const q3cu
                            const void *q, const void *k, const void *v, q3cu_dtype dtype, int64_t q_stride,
                            int64_t kv_stride, int n_heads, const float *q_norm, const float *k_norm, float theta,
                            float eps, void *q_out, q3cu_dtype q_dtype, q3cu_stream stream);
+
+/* How heads are rotated, where it is not the whole head by halves at one theta. */
+typedef enum { Q3CU_ROPE_HALVES = 0, Q3CU_ROPE_PAIRS = 1 } q3cu_rope_layout;
+typedef enum { Q3CU_ROPE_UNSCALED = 0, Q3CU_ROPE_LINEAR = 1, Q3CU_ROPE_YARN = 2 } q3cu_rope_scaling;
+typedef struct {
+    float theta;             /* pair j < dim / 2 turns by theta^(-2 j / dim) a position, before scaling */
+    int32_t dim;             /* the first dim elements of a head are rotated: a multiple of 4 up to 128 */
+    int32_t layout;          /* q3cu_rope_layout: pair j is elements (j, j + dim / 2), or (2 j, 2 j + 1) */
+    int32_t scaling;         /* q3cu_rope_scaling: none; every frequency divided by factor; or YaRN (Peng et al., 2023):
+                                pairs that turn more than beta_fast times over `original` positions keep their
+                                frequency, those that turn less than beta_slow times have it divided by factor, with a
+                                linear ramp over the pairs between (its ends rounded outwards to whole pairs) */
+    float factor;            /* at least 1 (read when scaled) */
+    float original;          /* positions trained on (YaRN) */
+    float beta_fast, beta_slow;  /* YaRN: 32 and 1 usually */
+    float gain;              /* factor of cosines and sines; 0: 1, and 0.1 ln(factor) + 1 with YaRN */
+    const double *freq;      /* NULL, or [dim / 2] radians a position of each pair (host memory, read by the call), in
+                                place of theta and scaling */
+} q3cu_rope;
+
+/* q3cu_kv_append with the rotation that `rope` describes (host memory).  Into a Q8_0 cache the rows are
+ * quantised as they are written: the codes and scales are those that
+ * q3cu_quantize_q8 makes of the f32 rows. */
+q3cu_status q3cu_kv_append_rope(q3cu_ctx *ctx, const q3cu_kv_cache *cache, const q3cu_kv_batch *batch, int64_t rows,
+                                const void *q, const void *k, const void *v, q3cu_dtype dtype, int64_t q_stride,
+                                int64_t kv_stride, int n_heads, const float *q_norm, const float *k_norm,
+                                const q3cu_rope *rope, float eps, void *q_out, q3cu_dtype q_dtype, q3cu_stream stream);
+
+/* Reads the packed rows' keys and values back from the cache: k and v
+ * [rows][n_kv][128] of `dtype` (f32 or bf16) with kv_stride elements between
+ * rows.  A cache of any type; a Q8_0 code times its scale is rounded to f32, and
+ * then to bf16 where that is asked for.  Padding rows, rows on a bad page or at a position beyond the
+ * table (both flagged) are zeros; rows behind the last sequence are left as
+ * they are.  Pointers 16-byte aligned, the stride a multiple of 16 bytes. */
+q3cu_status q3cu_kv_read(q3cu_ctx *ctx, const q3cu_kv_cache *cache, const q3cu_kv_batch *batch, int64_t rows, void *k,
+                         void *v, q3cu_dtype dtype, int64_t kv_stride, q3cu_stream stream);
 
 /* Attention of one new token per sequence: row s of q ([n_seqs][n_heads][128]
  * of `dtype`, q_stride elements between rows) over positions 0..kv_len[s]-1 of

@@ -109,6 +109,18 @@ void CudaContext::kvAppend(const q3cu_kv_cache &cache, const q3cu_kv_batch &batc
                          q_out, q_dt, stream),
           "kvAppend");
 }
+void CudaContext::kvAppend(const q3cu_kv_cache &cache, const q3cu_kv_batch &batch, int64_t rows, const void *q,
+                           const void *k, const void *v, q3cu_dtype dt, int64_t q_stride, int64_t kv_stride, int n_heads,
+                           const float *q_norm, const float *k_norm, void *q_out, q3cu_dtype q_dt, q3cu_stream stream,
+                           const q3cu_rope &rope, float eps) {
+    check(q3cu_kv_append_rope(ctx_, &cache, &batch, rows, q, k, v, dt, q_stride, kv_stride, n_heads, q_norm, k_norm, &rope,
+                              eps, q_out, q_dt, stream),
+          "kvAppend");
+}
+void CudaContext::kvRead(const q3cu_kv_cache &cache, const q3cu_kv_batch &batch, int64_t rows, void *k, void *v,
+                         q3cu_dtype dt, int64_t kv_stride, q3cu_stream stream) {
+    check(q3cu_kv_read(ctx_, &cache, &batch, rows, k, v, dt, kv_stride, stream), "kvRead");
+}
 size_t CudaContext::attentionPagedWorkspace(int n_heads, int n_kv) {
     size_t bytes = 0;
     check(q3cu_attention_paged_workspace(ctx_, n_heads, n_kv, &bytes), "attentionPagedWorkspace");

@@ -10,6 +10,16 @@
 // The key heads go to their page slots in the cache's type, the value heads are
 // converted and stored beside them, the query heads go to q_out.
 //
+// Other rotations (TurnForm): the first `dim` elements of a head, as halves or as
+// neighbouring pairs, cosine and sine times a gain, any frequencies.  A lane's four
+// elements are chosen so that both elements of its two pairs are its own, and the
+// rest of the head is dealt to the lanes beyond.
+//
+// A Q8_0 cache: s = max|o| / 127 over each 64 elements, codes o / s rounded half
+// away from zero, with the operations of q3cu_quantize_q8 (the same codes and
+// scales from the same f32 rows).  The maxima are taken over the warp by one
+// instruction each; a lane stores two codes of each of its two element pairs.
+//
 // The angle is formed in binary64 as turns, p * (theta^(-j/64) / 2 pi) less its
 // nearest whole number, so it is as exact at position 100,000 as at 0 (a
 // binary32 product is off by up to 0.004 rad there); the remainder is carried
@@ -26,6 +36,8 @@
 // TB/s, f32 to f32 38.5 us, 5.2 TB/s; one row: 3.3 us.
 #include "q3cu_paged.cuh"
 
+#include <type_traits>
+
 namespace q3 {
 
 __device__ __forceinline__ void prefetch_l2(const void *p) { asm volatile("prefetch.global.L2 [%0];" :: "l"(p)); }
@@ -39,25 +51,75 @@ __device__ __forceinline__ float2 load_pair(const uint16_t *p) {
     return make_float2(bf16_to_f32(u & 0xffffu), bf16_to_f32(u >> 16));
 }
 // v as elements at, at + 1 of base.
-template <bool BF16>
+enum AppendAs { AS_F32, AS_BF16, AS_Q8 };
+template <AppendAs AS>
 __device__ __forceinline__ void store_pair(void *base, int64_t at, float2 v) {
-    if constexpr (BF16) *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(base) + at) = pack_bf16(v.x, v.y);
+    if constexpr (AS == AS_BF16) *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(base) + at) = pack_bf16(v.x, v.y);
     else *reinterpret_cast<float2 *>(static_cast<float *>(base) + at) = v;
 }
 
-// Up to APPEND_HEADS heads from x (this lane's elements of the first), `step` elements apart where they go; turned by
-// w if ROTATE, and normalised before if `norm` (the norm's weights are in w).
+// Where a lane's elements lie in a head, two at lo and two at hi, and which of its two pairs are rotated: pair 0 is
+// (lo, hi) and pair 1 (lo + 1, hi + 1), or with neighbouring pairs (lo, lo + 1) and (hi, hi + 1).
+// WHOLE: the whole head by halves, so lo = 2 lane, hi = 64 + lo and all are rotated.
+template <bool WHOLE> struct Place {
+    __device__ __forceinline__ Place(int, int, bool) {}
+    __device__ __forceinline__ int lo() const { return 2 * (threadIdx.x & 31); }
+    __device__ __forceinline__ int hi() const { return 64 + lo(); }
+    __device__ __forceinline__ int angle(int e) const { return lo() + e; }
+    __device__ __forceinline__ bool turned(int) const { return true; }
+    __device__ __forceinline__ bool paired() const { return false; }
+};
+template <> struct Place<false> {
+    int lo_, hi_, half;
+    bool pairs;
+    __device__ __forceinline__ Place(int lane, int dim, bool p) : half(dim / 2), pairs(p) {
+        const int beyond = lane - dim / 4;                   // lanes behind the rotated ones
+        lo_ = pairs || beyond < 0 ? 2 * lane : dim + 2 * beyond;
+        hi_ = pairs ? 64 + lo_ : beyond < 0 ? half + lo_ : dim + (HD - dim) / 2 + 2 * beyond;
+    }
+    __device__ __forceinline__ int lo() const { return lo_; }
+    __device__ __forceinline__ int hi() const { return hi_; }
+    __device__ __forceinline__ int angle(int e) const {      // which frequency, below 64
+        return pairs ? (threadIdx.x & 31) + 32 * e : 2 * (threadIdx.x & 31) + e;
+    }
+    __device__ __forceinline__ bool turned(int e) const { return angle(e) < half; }
+    __device__ __forceinline__ bool paired() const { return pairs; }
+};
+__device__ __forceinline__ void swap_inner(float2 &l, float2 &h) {
+    const float x = l.y;
+    l.y = h.x;
+    h.x = x;
+}
+
+// A head's Q8_0 codes and scales from every lane's elements l (two at lo) and h (two at hi): elements `at` of base, scales
+// at `scale`.
+__device__ __forceinline__ void store_q8(void *base, int64_t at, float *scale, int lo, int hi, float2 l, float2 h) {
+    const float a = amax_fold(amax_fold(0.0f, l.x), l.y), b = amax_fold(amax_fold(0.0f, h.x), h.y);
+    const float low = fmaxf(lo < GS ? a : 0.0f, hi < GS ? b : 0.0f), high = fmaxf(lo < GS ? 0.0f : a, hi < GS ? 0.0f : b);
+    // magnitudes compare as their bits do
+    const Q8Scale g0 = q8_prepare(__uint_as_float(__reduce_max_sync(FULL, __float_as_uint(low))));
+    const Q8Scale g1 = q8_prepare(__uint_as_float(__reduce_max_sync(FULL, __float_as_uint(high))));
+    const Q8Scale gl = lo < GS ? g0 : g1, gh = hi < GS ? g0 : g1;
+    uint8_t *p = static_cast<uint8_t *>(base) + at;
+    *reinterpret_cast<uint16_t *>(p + lo) = uint16_t(q8_code_g(l.x, gl) | q8_code_g(l.y, gl) << 8);
+    *reinterpret_cast<uint16_t *>(p + hi) = uint16_t(q8_code_g(h.x, gh) | q8_code_g(h.y, gh) << 8);
+    if ((threadIdx.x & 31) == 0) *reinterpret_cast<float2 *>(scale) = make_float2(g0.scale, g1.scale);
+}
+
+// Up to APPEND_HEADS heads from x (the first head's first element), `step` elements apart where they go (`at`: the first
+// one's first); turned by w if ROTATE, and normalised before if `norm` (the norm's weights are in w).
 struct Turn { float2 c[2], s[2]; };                          // weight * cosine, weight * sine of both halves
-template <typename E, bool BF16, bool ROTATE>
-__device__ __forceinline__ void append_heads(const E *x, int n, bool norm, float eps, const Turn &w, void *to, int64_t at,
-                                             int64_t step) {
+template <typename E, AppendAs AS, bool ROTATE, bool WHOLE>
+__device__ __forceinline__ void append_heads(const E *x, int n, bool norm, float eps, const Place<WHOLE> &place, const Turn &w,
+                                             void *to, int64_t at, int64_t step, float *scale) {
+    const int lo = place.lo(), hi = place.hi();
     float2 l[APPEND_HEADS], h[APPEND_HEADS];
 #pragma unroll
     for (int i = 0; i < APPEND_HEADS; ++i) {
         l[i] = h[i] = make_float2(0.0f, 0.0f);
         if (i < n) {
-            l[i] = load_pair(x + i * HD);
-            h[i] = load_pair(x + i * HD + 64);
+            l[i] = load_pair(x + i * HD + lo);
+            h[i] = load_pair(x + i * HD + hi);
         }
     }
     if constexpr (ROTATE) {
@@ -75,25 +137,35 @@ __device__ __forceinline__ void append_heads(const E *x, int n, bool norm, float
         }
 #pragma unroll
         for (int i = 0; i < APPEND_HEADS; ++i) {
+            if (place.paired()) swap_inner(l[i], h[i]);
             const float2 y = make_float2(g[i] * l[i].x, g[i] * l[i].y), z = make_float2(g[i] * h[i].x, g[i] * h[i].y);
             l[i] = make_float2(fmaf(y.x, w.c[0].x, -(z.x * w.s[1].x)), fmaf(y.y, w.c[0].y, -(z.y * w.s[1].y)));
             h[i] = make_float2(fmaf(y.x, w.s[0].x, z.x * w.c[1].x), fmaf(y.y, w.s[0].y, z.y * w.c[1].y));
+            if constexpr (!WHOLE) {                          // the cosine is 1; a sine of 0 times infinity would be NaN
+                if (!place.turned(0)) l[i].x = y.x * w.c[0].x, h[i].x = z.x * w.c[1].x;
+                if (!place.turned(1)) l[i].y = y.y * w.c[0].y, h[i].y = z.y * w.c[1].y;
+            }
+            if (place.paired()) swap_inner(l[i], h[i]);
         }
     }
 #pragma unroll
     for (int i = 0; i < APPEND_HEADS; ++i)
         if (i < n) {
-            store_pair<BF16>(to, at + i * step, l[i]);
-            store_pair<BF16>(to, at + i * step + 64, h[i]);
+            if constexpr (AS == AS_Q8) {
+                store_q8(to, at + i * step, scale + i * (step / GS), lo, hi, l[i], h[i]);
+            } else {
+                store_pair<AS>(to, at + i * step + lo, l[i]);
+                store_pair<AS>(to, at + i * step + hi, h[i]);
+            }
         }
 }
 
-template <typename T, bool QB, bool CB>
+template <typename T, AppendAs QA, AppendAs CA, bool WHOLE>
 __global__ void __launch_bounds__(APPEND_WARPS * 32, 4)
 kv_append_kernel(const PagedKV c, const PagedSeqs b, int rows, const typename Elem<T>::type *q,
                  const typename Elem<T>::type *k, const typename Elem<T>::type *v, int64_t q_stride,
                  int64_t kv_stride, int n_heads, const float *__restrict__ q_norm, const float *__restrict__ k_norm,
-                 const __grid_constant__ TurnFreq freq, float eps, void *q_out, uint32_t *status) {
+                 const __grid_constant__ TurnFreq freq, const TurnForm form, float eps, void *q_out, uint32_t *status) {
     typedef typename Elem<T>::type E;
     __shared__ double turn[64];
     if (threadIdx.x < 64) turn[threadIdx.x] = freq.v[threadIdx.x];
@@ -118,74 +190,174 @@ kv_append_kernel(const PagedKV c, const PagedSeqs b, int rows, const typename El
     const int pos = paged_pos(b, c, s, r, lane == 0 ? status : nullptr);
     if (pos < 0) return;                                     // padding, or beyond the table
     const int page = last > qn ? paged_page(b, c, s, pos, lane == 0 ? status : nullptr) : -1;
+    const Place<WHOLE> place(lane, form.dim, form.pairs);
     float cs[2], sn[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-        const double t = double(pos) * turn[2 * lane + e];
+        const double t = double(pos) * turn[place.angle(e)];
         const double half = 2.0 * (t - rint(t));             // half turns in [-1, 1]
         const float h = float(half), rest = 3.14159265f * float(half - double(h));
         float s0, c0;
         sincospif(h, &s0, &c0);
         sn[e] = fmaf(c0, rest, s0);
         cs[e] = fmaf(-s0, rest, c0);
+        if constexpr (!WHOLE) {
+            sn[e] = place.turned(e) ? sn[e] * form.gain : 0.0f;
+            cs[e] = place.turned(e) ? cs[e] * form.gain : 1.0f;
+        }
     }
     auto weighted = [&](const float *n) {
         Turn w;
+        float2 f[2];
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+            f[y] = n ? __ldg(reinterpret_cast<const float2 *>(n + (y ? place.hi() : place.lo()))) : make_float2(1.0f, 1.0f);
+        if (place.paired()) swap_inner(f[0], f[1]);
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
-            const float2 f = n ? __ldg(reinterpret_cast<const float2 *>(n) + 32 * y + lane) : make_float2(1.0f, 1.0f);
-            w.c[y] = make_float2(f.x * cs[0], f.y * cs[1]);
-            w.s[y] = make_float2(f.x * sn[0], f.y * sn[1]);
+            w.c[y] = make_float2(f[y].x * cs[0], f[y].y * cs[1]);
+            w.s[y] = make_float2(f[y].x * sn[0], f[y].y * sn[1]);
         }
         return w;
     };
     Turn w = weighted(q_norm);
     for (int x = first; x < min(last, qn); ++x) {
         const int u = x * APPEND_HEADS;
-        append_heads<E, QB, true>(qr + u * HD + 2 * lane, n_heads - u, q_norm, eps, w, q_out,
-                                  (int64_t(r) * n_heads + u) * HD + 2 * lane, HD);
+        append_heads<E, QA, true, WHOLE>(qr + u * HD, n_heads - u, q_norm, eps, place, w, q_out,
+                                         (int64_t(r) * n_heads + u) * HD, HD, nullptr);
     }
     if (page < 0) return;                                    // no keys or values here, or a bad page (flagged): none stored
-    const int64_t at = paged_at(c, page, 0, pos) + 2 * lane, step = HD << c.page_shift;
+    const int64_t at = paged_at(c, page, 0, pos), step = HD << c.page_shift;
+    // the scales of head 0, those of head h h * (step / 64) further
+    const int64_t sc = int64_t(page) * c.scale_stride + 2 * (pos & ((1 << c.page_shift) - 1));
     w = weighted(k_norm);
     for (int x = max(first, qn); x < min(last, qn + kn); ++x) {
         const int u = (x - qn) * APPEND_HEADS;
-        append_heads<E, CB, true>(kr + u * HD + 2 * lane, c.n_kv - u, k_norm, eps, w, c.k, at + u * step, step);
+        append_heads<E, CA, true, WHOLE>(kr + u * HD, c.n_kv - u, k_norm, eps, place, w, c.k, at + u * step, step,
+                                         c.k_scale + (sc + u * (step / GS)));
     }
     for (int x = max(first, qn + kn); x < last; ++x) {
         const int u = (x - qn - kn) * APPEND_HEADS;
-        append_heads<E, CB, false>(vr + u * HD + 2 * lane, c.n_kv - u, false, eps, w, c.v, at + u * step, step);
+        append_heads<E, CA, false, WHOLE>(vr + u * HD, c.n_kv - u, false, eps, place, w, c.v, at + u * step, step,
+                                          c.v_scale + (sc + u * (step / GS)));
     }
 }
 
 cudaError_t launch_kv_append(const PagedKV &c, q3cu_dtype cache_dt, const PagedSeqs &b, int64_t rows, const void *q,
                              const void *k, const void *v, q3cu_dtype dt, int64_t q_stride, int64_t kv_stride,
-                             int n_heads, const float *q_norm, const float *k_norm, const TurnFreq &freq, float eps,
-                             void *q_out, q3cu_dtype q_dt, uint32_t *status, cudaStream_t stream, int sms) {
+                             int n_heads, const float *q_norm, const float *k_norm, const TurnFreq &freq,
+                             const TurnForm &form, float eps, void *q_out, q3cu_dtype q_dt, uint32_t *status,
+                             cudaStream_t stream, int sms) {
     // A row is split over warps only while the rows alone are fewer than 32 warps per SM.
     const int64_t all = (n_heads + APPEND_HEADS - 1) / APPEND_HEADS + (c.n_kv + APPEND_HEADS - 1) / APPEND_HEADS * 2;
     const int64_t batches = all < 65535 ? all : 65535;       // a grid's height
     const int64_t parts = rows >= 32 * sms ? 1 : (32 * int64_t(sms) + rows - 1) / rows;
     const dim3 grid(unsigned((rows + APPEND_WARPS - 1) / APPEND_WARPS), unsigned(parts < batches ? parts : batches));
+    const bool whole = form.dim == HD && !form.pairs && form.gain == 1.0f;
     auto go = [&](auto kernel, auto *typed) {
         typedef decltype(typed) P;
         return launch_dependent(kernel, grid, dim3(APPEND_WARPS * 32), 0, stream, c, b, int(rows), static_cast<P>(q),
                                 static_cast<P>(k), static_cast<P>(v), q_stride, kv_stride, n_heads, q_norm, k_norm, freq,
-                                eps, q_out, status);
+                                form, eps, q_out, status);
     };
-    const int kind = 2 * (q_dt == Q3CU_BF16) + (cache_dt == Q3CU_BF16);
+    auto cached = [&](auto type, auto qa, auto *typed) {     // by the cache's type and the rotation's form
+        typedef decltype(type) T;
+        constexpr AppendAs QA = decltype(qa)::value;
+        if (cache_dt == Q3CU_Q8_0)
+            return whole ? go(kv_append_kernel<T, QA, AS_Q8, true>, typed) : go(kv_append_kernel<T, QA, AS_Q8, false>, typed);
+        if (cache_dt == Q3CU_BF16)
+            return whole ? go(kv_append_kernel<T, QA, AS_BF16, true>, typed) : go(kv_append_kernel<T, QA, AS_BF16, false>, typed);
+        return whole ? go(kv_append_kernel<T, QA, AS_F32, true>, typed) : go(kv_append_kernel<T, QA, AS_F32, false>, typed);
+    };
+    const std::integral_constant<AppendAs, AS_F32> f32;
+    const std::integral_constant<AppendAs, AS_BF16> bf16;
     if (dt == Q3CU_F32) {
         const float *t = nullptr;
-        return kind == 0   ? go(kv_append_kernel<float, false, false>, t)
-               : kind == 1 ? go(kv_append_kernel<float, false, true>, t)
-               : kind == 2 ? go(kv_append_kernel<float, true, false>, t)
-                           : go(kv_append_kernel<float, true, true>, t);
+        return q_dt == Q3CU_F32 ? cached(float(), f32, t) : cached(float(), bf16, t);
     }
     const uint16_t *t = nullptr;
-    return kind == 0   ? go(kv_append_kernel<bf16raw, false, false>, t)
-           : kind == 1 ? go(kv_append_kernel<bf16raw, false, true>, t)
-           : kind == 2 ? go(kv_append_kernel<bf16raw, true, false>, t)
-                       : go(kv_append_kernel<bf16raw, true, true>, t);
+    return q_dt == Q3CU_F32 ? cached(bf16raw(), f32, t) : cached(bf16raw(), bf16, t);
+}
+
+// ---- reading rows back ------------------------------------------------------------------------
+// The rows' keys and values as they are in the cache (Q8_0: code times scale), dense.  Bound by memory: a warp takes one
+// row, or with few rows a part of its heads, READ_HEADS heads of k or of v at a time; a lane holds four
+// consecutive elements of a head.
+constexpr int READ_HEADS = 8;
+template <AppendAs CA, AppendAs AS>
+__device__ __forceinline__ void read_heads(const void *from, const float *scale, int64_t at, int64_t step, int n, bool there,
+                                           void *to) {
+    const int lane = threadIdx.x & 31;
+    float4 x[READ_HEADS];
+    uint32_t code[READ_HEADS];
+    float s[READ_HEADS];
+#pragma unroll
+    for (int i = 0; i < READ_HEADS; ++i) {
+        x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        code[i] = 0;
+        s[i] = 0.0f;
+        if (i >= n || !there) continue;
+        const int64_t e = at + i * step + 4 * lane;
+        if constexpr (CA == AS_Q8) {
+            code[i] = *reinterpret_cast<const uint32_t *>(static_cast<const uint8_t *>(from) + e);
+            s[i] = scale[i * (step / GS) + (lane >> 4)];
+        } else if constexpr (CA == AS_BF16) {
+            x[i] = load_quad(static_cast<const uint16_t *>(from) + e);
+        } else {
+            x[i] = load_quad(static_cast<const float *>(from) + e);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < READ_HEADS; ++i) {
+        if (i >= n) continue;
+        if constexpr (CA == AS_Q8) {
+            const float4 y = q8_floats(code[i]);
+            if (there) x[i] = make_float4(s[i] * y.x, s[i] * y.y, s[i] * y.z, s[i] * y.w);
+        }
+        if constexpr (AS == AS_BF16) store_quad(static_cast<uint16_t *>(to) + i * HD + 4 * lane, x[i]);
+        else store_quad(static_cast<float *>(to) + i * HD + 4 * lane, x[i]);
+    }
+}
+
+template <AppendAs CA, AppendAs AS>
+__global__ void __launch_bounds__(APPEND_WARPS * 32)
+kv_read_kernel(const PagedKV c, const PagedSeqs b, int rows, void *k, void *v, int64_t kv_stride, uint32_t *status) {
+    griddep_wait();
+    const int lane = threadIdx.x & 31, r = int(blockIdx.x) * APPEND_WARPS + int(threadIdx.x >> 5);
+    if (r >= rows) return;
+    const int s = paged_seq_of_warp(b, r);
+    if (s < 0) return;                                       // a row behind the last sequence
+    const int pos = paged_pos(b, c, s, r, lane == 0 ? status : nullptr);
+    const int page = pos < 0 ? -1 : paged_page(b, c, s, pos, lane == 0 ? status : nullptr);
+    const int64_t step = HD << c.page_shift, at = page < 0 ? 0 : paged_at(c, page, 0, pos);
+    const int64_t sc = page < 0 ? 0 : int64_t(page) * c.scale_stride + 2 * (pos & ((1 << c.page_shift) - 1));
+    const int n = (c.n_kv + READ_HEADS - 1) / READ_HEADS;    // batches of k, and of v
+    const int first = int(int64_t(2 * n) * blockIdx.y / gridDim.y), last = int(int64_t(2 * n) * (blockIdx.y + 1) / gridDim.y);
+    constexpr int BYTES = AS == AS_BF16 ? 2 : 4;
+    for (int x = first; x < last; ++x) {
+        const bool side = x >= n;
+        const int u = (side ? x - n : x) * READ_HEADS;
+        read_heads<CA, AS>(side ? c.v : c.k, (side ? c.v_scale : c.k_scale) + (sc + u * (step / GS)), at + u * step, step,
+                           c.n_kv - u, page >= 0, static_cast<uint8_t *>(side ? v : k) + (r * kv_stride + u * HD) * BYTES);
+    }
+}
+
+cudaError_t launch_kv_read(const PagedKV &c, q3cu_dtype cache_dt, const PagedSeqs &b, int64_t rows, void *k, void *v,
+                           q3cu_dtype dt, int64_t kv_stride, uint32_t *status, cudaStream_t stream, int sms) {
+    // a row is split over warps as above
+    const int64_t all = 2 * ((int64_t(c.n_kv) + READ_HEADS - 1) / READ_HEADS), batches = all < 65535 ? all : 65535;
+    const int64_t parts = rows >= 32 * sms ? 1 : (32 * int64_t(sms) + rows - 1) / rows;
+    const dim3 grid(unsigned((rows + APPEND_WARPS - 1) / APPEND_WARPS), unsigned(parts < batches ? parts : batches));
+    auto go = [&](auto kernel) {
+        return launch_dependent(kernel, grid, dim3(APPEND_WARPS * 32), 0, stream, c, b, int(rows), k, v, kv_stride, status);
+    };
+    if (dt == Q3CU_F32)
+        return cache_dt == Q3CU_Q8_0   ? go(kv_read_kernel<AS_Q8, AS_F32>)
+               : cache_dt == Q3CU_BF16 ? go(kv_read_kernel<AS_BF16, AS_F32>)
+                                       : go(kv_read_kernel<AS_F32, AS_F32>);
+    return cache_dt == Q3CU_Q8_0   ? go(kv_read_kernel<AS_Q8, AS_BF16>)
+           : cache_dt == Q3CU_BF16 ? go(kv_read_kernel<AS_BF16, AS_BF16>)
+                                   : go(kv_read_kernel<AS_F32, AS_BF16>);
 }
 
 }  // namespace q3

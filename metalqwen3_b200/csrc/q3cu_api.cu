@@ -34,6 +34,8 @@ struct q3cu_ctx {
     std::map<std::pair<int, uint32_t>, q3::InvFreq> inv_freq;   // (head_dim, bits of theta)
     float turn_theta = 0.0f;                                    // the theta turn_freq was made for (0: none)
     q3::TurnFreq turn_freq{};
+    q3cu_rope rope{};                                          // what rope_freq was made for (theta 0: none)
+    q3::TurnFreq rope_freq{};
     bool alive = false;
 };
 
@@ -104,6 +106,37 @@ const q3::TurnFreq &turn_freq_for(q3cu_ctx *ctx, float theta) {
         for (int j = 0; j < 64; ++j) ctx->turn_freq.v[j] = std::pow(double(theta), -j / 64.0) / 6.283185307179586476925;
     ctx->turn_theta = theta;
     return ctx->turn_freq;
+}
+
+// The frequencies of `r` (checked) in turns a position.
+const q3::TurnFreq &rope_freq_for(q3cu_ctx *ctx, const q3cu_rope &r) {
+    const double turn = 6.283185307179586476925;
+    const int pairs = r.dim / 2;
+    q3::TurnFreq &f = ctx->rope_freq;
+    if (r.freq) {                                              // the caller's own: their values may change between calls
+        ctx->rope.theta = 0.0f;
+        for (int j = 0; j < 64; ++j) f.v[j] = j < pairs ? r.freq[j] / turn : 0.0;
+        return f;
+    }
+    q3cu_rope &was = ctx->rope;
+    if (was.theta == r.theta && was.dim == r.dim && was.scaling == r.scaling && was.factor == r.factor &&
+        was.original == r.original && was.beta_fast == r.beta_fast && was.beta_slow == r.beta_slow)
+        return f;
+    was = r;
+    // YaRN: the pair that turns `turns` times over the original length, as a real number
+    auto pair_of = [&](double turns) { return r.dim * std::log(r.original / (turns * turn)) / (2.0 * std::log(double(r.theta))); };
+    double low = 0.0, high = 0.0;
+    if (r.scaling == Q3CU_ROPE_YARN) {
+        low = std::fmax(std::floor(pair_of(r.beta_fast)), 0.0);
+        high = std::fmin(std::ceil(pair_of(r.beta_slow)), r.dim - 1.0);
+    }
+    for (int j = 0; j < 64; ++j) {
+        const double plain = j < pairs ? std::pow(double(r.theta), -2.0 * j / r.dim) / turn : 0.0;
+        double slow = r.scaling == Q3CU_ROPE_LINEAR ? 1.0 : 0.0;     // share of the divided frequency
+        if (r.scaling == Q3CU_ROPE_YARN) slow = std::fmin(std::fmax((j - low) / std::fmax(high - low, 0.001), 0.0), 1.0);
+        f.v[j] = plain * (1.0 - slow) + (slow > 0.0 ? plain / r.factor * slow : 0.0);
+    }
+    return f;
 }
 
 // The softmax kernel balances rows across SMs with a pair of device counters
@@ -490,7 +523,9 @@ q3cu_status q3cu_attention(q3cu_ctx *ctx, const float *q, const float *key_cache
 static q3cu_status check_paged(const char *op, const q3cu_kv_cache *cache, const q3cu_kv_batch *batch, int n_heads,
                                bool with_rows, q3::PagedKV &c, q3::PagedSeqs &b) {
     if (!cache || !batch) return fail(Q3CU_ERR_INVALID, "%s: cache or batch is NULL", op);
-    if (q3cu_status st = check_dtype(q3cu_dtype(cache->dtype))) return st;
+    const bool q8 = cache->dtype == Q3CU_Q8_0;
+    if (!q8)
+        if (q3cu_status st = check_dtype(q3cu_dtype(cache->dtype))) return st;
     if (cache->head_dim != q3::PAGED_HD)
         return fail(Q3CU_ERR_INVALID, "%s: head_dim %d: only 128 is supported", op, cache->head_dim);
     int shift = 4;
@@ -511,8 +546,8 @@ static q3cu_status check_paged(const char *op, const q3cu_kv_cache *cache, const
     if (cache->page_stride < dense || cache->page_stride > (int64_t(1) << 36))
         return fail(Q3CU_ERR_INVALID, "%s: page_stride %lld, a page has %lld elements", op,
                     (long long)cache->page_stride, (long long)dense);
-    if (cache->page_stride % 8)
-        return fail(Q3CU_ERR_ALIGN, "%s: page_stride must be a multiple of 8 elements", op);
+    if (cache->page_stride % (q8 ? 16 : 8))
+        return fail(Q3CU_ERR_ALIGN, "%s: page_stride must be a multiple of %d elements", op, q8 ? 16 : 8);
     if (!cache->k || !cache->v) return fail(Q3CU_ERR_INVALID, "%s: cache pointer is NULL", op);
     if (!aligned(cache->k, 16) || !aligned(cache->v, 16))
         return fail(Q3CU_ERR_ALIGN, "%s: cache pages must be 16-byte aligned", op);
@@ -520,7 +555,20 @@ static q3cu_status check_paged(const char *op, const q3cu_kv_cache *cache, const
         return fail(Q3CU_ERR_INVALID, "%s: batch pointer is NULL", op);
     if (!aligned(batch->row_off, 4) || !aligned(batch->kv_len, 4) || !aligned(batch->pages, 4))
         return fail(Q3CU_ERR_ALIGN, "%s: batch arrays must be 4-byte aligned", op);
-    c = {cache->k, cache->v, cache->page_stride, cache->n_pages, cache->n_kv, shift};
+    c = {cache->k, cache->v, cache->page_stride, cache->n_pages, cache->n_kv, shift, nullptr, nullptr, 0};
+    if (q8) {
+        const q3cu_kv_cache_q8 *x = reinterpret_cast<const q3cu_kv_cache_q8 *>(cache);
+        const int64_t scales = int64_t(cache->n_kv) * cache->page_size * (q3::PAGED_HD / Q3CU_GROUP_SIZE);
+        if (!x->k_scale || !x->v_scale) return fail(Q3CU_ERR_INVALID, "%s: scale pointer is NULL", op);
+        if (x->scale_stride < scales || x->scale_stride > (int64_t(1) << 36))
+            return fail(Q3CU_ERR_INVALID, "%s: scale_stride %lld, a page has %lld scales", op, (long long)x->scale_stride,
+                        (long long)scales);
+        if (x->scale_stride % 4 || !aligned(x->k_scale, 16) || !aligned(x->v_scale, 16))
+            return fail(Q3CU_ERR_ALIGN, "%s: scales must be 16-byte aligned, scale_stride a multiple of 4", op);
+        c.k_scale = x->k_scale;
+        c.v_scale = x->v_scale;
+        c.scale_stride = x->scale_stride;
+    }
     b = {batch->row_off, batch->kv_len, batch->pages, batch->n_seqs, batch->max_pages};
     return Q3CU_OK;
 }
@@ -537,11 +585,40 @@ static q3cu_status check_rows(const char *op, const char *name, const void *p, q
     return Q3CU_OK;
 }
 
-q3cu_status q3cu_kv_append(q3cu_ctx *ctx, const q3cu_kv_cache *cache, const q3cu_kv_batch *batch, int64_t rows,
-                           const void *q, const void *k, const void *v, q3cu_dtype dtype, int64_t q_stride,
-                           int64_t kv_stride, int n_heads, const float *q_norm, const float *k_norm, float theta,
-                           float eps, void *q_out, q3cu_dtype q_dtype, q3cu_stream stream) {
-    CHECK_CTX(ctx);
+// Checks a rotation's description.
+static q3cu_status check_rope(const char *op, const q3cu_rope &r) {
+    if (r.dim < 4 || r.dim > q3::PAGED_HD || r.dim % 4)
+        return fail(Q3CU_ERR_INVALID, "%s: rope dim %d is not a multiple of 4 up to 128", op, r.dim);
+    if (r.layout != Q3CU_ROPE_HALVES && r.layout != Q3CU_ROPE_PAIRS)
+        return fail(Q3CU_ERR_INVALID, "%s: unknown rope layout %d", op, r.layout);
+    if (!(r.gain >= 0.0f) || std::isinf(r.gain)) return fail(Q3CU_ERR_INVALID, "%s: rope gain must be positive, or 0", op);
+    if (r.freq) {
+        for (int j = 0; j < r.dim / 2; ++j)
+            if (!std::isfinite(r.freq[j])) return fail(Q3CU_ERR_INVALID, "%s: rope freq[%d] is not finite", op, j);
+        return Q3CU_OK;
+    }
+    if (!(r.theta > 0.0f) || std::isinf(r.theta)) return fail(Q3CU_ERR_INVALID, "%s: theta must be positive", op);
+    if (r.scaling == Q3CU_ROPE_UNSCALED) return Q3CU_OK;
+    if (r.scaling != Q3CU_ROPE_LINEAR && r.scaling != Q3CU_ROPE_YARN)
+        return fail(Q3CU_ERR_INVALID, "%s: unknown rope scaling %d", op, r.scaling);
+    if (!(r.factor >= 1.0f) || std::isinf(r.factor))
+        return fail(Q3CU_ERR_INVALID, "%s: rope factor must be at least 1", op);
+    if (r.scaling == Q3CU_ROPE_YARN &&
+        (!(r.original > 0.0f) || std::isinf(r.original) || !(r.beta_slow > 0.0f) || !(r.beta_fast > r.beta_slow) ||
+         std::isinf(r.beta_fast) || !(r.theta > 1.0f)))
+        return fail(Q3CU_ERR_INVALID, "%s: YaRN needs theta > 1, original > 0 and beta_fast > beta_slow > 0", op);
+    return Q3CU_OK;
+}
+static q3::TurnForm rope_form(const q3cu_rope &r) {
+    const bool yarn = !r.freq && r.scaling == Q3CU_ROPE_YARN;
+    return {r.dim, r.layout == Q3CU_ROPE_PAIRS,
+            r.gain > 0.0f ? r.gain : yarn ? float(0.1 * std::log(double(r.factor)) + 1.0) : 1.0f};
+}
+
+static q3cu_status append_common(q3cu_ctx *ctx, const q3cu_kv_cache *cache, const q3cu_kv_batch *batch, int64_t rows,
+                                 const void *q, const void *k, const void *v, q3cu_dtype dtype, int64_t q_stride,
+                                 int64_t kv_stride, int n_heads, const float *q_norm, const float *k_norm, float theta,
+                                 const q3cu_rope *rope, float eps, void *q_out, q3cu_dtype q_dtype, q3cu_stream stream) {
     q3::PagedKV c;
     q3::PagedSeqs b;
     if (q3cu_status st = check_paged("kv_append", cache, batch, n_heads, true, c, b)) return st;
@@ -549,7 +626,11 @@ q3cu_status q3cu_kv_append(q3cu_ctx *ctx, const q3cu_kv_cache *cache, const q3cu
     if (q3cu_status st = check_dtype(q_dtype)) return st;
     if (rows < 0 || rows > INT32_MAX / (n_heads + 2 * int64_t(c.n_kv)))
         return fail(Q3CU_ERR_INVALID, "kv_append: rows %lld", (long long)rows);
-    if (!(theta > 0.0f) || std::isinf(theta)) return fail(Q3CU_ERR_INVALID, "kv_append: theta must be positive");
+    if (rope) {
+        if (q3cu_status st = check_rope("kv_append", *rope)) return st;
+    } else if (!(theta > 0.0f) || std::isinf(theta)) {
+        return fail(Q3CU_ERR_INVALID, "kv_append: theta must be positive");
+    }
     if (rows == 0 || b.n_seqs == 0) return Q3CU_OK;
     if (n_heads > 0) {
         if (q3cu_status st = check_rows("kv_append", "q", q, dtype, q_stride, n_heads)) return st;
@@ -564,9 +645,47 @@ q3cu_status q3cu_kv_append(q3cu_ctx *ctx, const q3cu_kv_cache *cache, const q3cu
         return fail(Q3CU_ERR_ALIGN, "kv_append: norm weights must be 16-byte aligned");
     if (q3cu_status st = use_device(ctx)) return st;
     return launched(q3::launch_kv_append(c, q3cu_dtype(cache->dtype), b, rows, q, k, v, dtype, q_stride, kv_stride,
-                                         n_heads, q_norm, k_norm, turn_freq_for(ctx, theta), eps, q_out, q_dtype,
-                                         ctx->d_status, static_cast<cudaStream_t>(stream), ctx->sms),
+                                         n_heads, q_norm, k_norm, rope ? rope_freq_for(ctx, *rope) : turn_freq_for(ctx, theta),
+                                         rope ? rope_form(*rope) : q3::TurnForm{q3::PAGED_HD, false, 1.0f}, eps, q_out,
+                                         q_dtype, ctx->d_status, static_cast<cudaStream_t>(stream), ctx->sms),
                     "kv_append launch");
+}
+
+q3cu_status q3cu_kv_append(q3cu_ctx *ctx, const q3cu_kv_cache *cache, const q3cu_kv_batch *batch, int64_t rows,
+                           const void *q, const void *k, const void *v, q3cu_dtype dtype, int64_t q_stride,
+                           int64_t kv_stride, int n_heads, const float *q_norm, const float *k_norm, float theta,
+                           float eps, void *q_out, q3cu_dtype q_dtype, q3cu_stream stream) {
+    CHECK_CTX(ctx);
+    return append_common(ctx, cache, batch, rows, q, k, v, dtype, q_stride, kv_stride, n_heads, q_norm, k_norm, theta,
+                         nullptr, eps, q_out, q_dtype, stream);
+}
+
+q3cu_status q3cu_kv_append_rope(q3cu_ctx *ctx, const q3cu_kv_cache *cache, const q3cu_kv_batch *batch, int64_t rows,
+                                const void *q, const void *k, const void *v, q3cu_dtype dtype, int64_t q_stride,
+                                int64_t kv_stride, int n_heads, const float *q_norm, const float *k_norm,
+                                const q3cu_rope *rope, float eps, void *q_out, q3cu_dtype q_dtype, q3cu_stream stream) {
+    CHECK_CTX(ctx);
+    if (!rope) return fail(Q3CU_ERR_INVALID, "kv_append_rope: rope is NULL");
+    return append_common(ctx, cache, batch, rows, q, k, v, dtype, q_stride, kv_stride, n_heads, q_norm, k_norm, 0.0f, rope,
+                         eps, q_out, q_dtype, stream);
+}
+
+q3cu_status q3cu_kv_read(q3cu_ctx *ctx, const q3cu_kv_cache *cache, const q3cu_kv_batch *batch, int64_t rows, void *k,
+                         void *v, q3cu_dtype dtype, int64_t kv_stride, q3cu_stream stream) {
+    CHECK_CTX(ctx);
+    q3::PagedKV c;
+    q3::PagedSeqs b;
+    if (q3cu_status st = check_paged("kv_read", cache, batch, 0, true, c, b)) return st;
+    if (q3cu_status st = check_dtype(dtype)) return st;
+    if (rows < 0 || rows > INT32_MAX / (2 * int64_t(c.n_kv))) return fail(Q3CU_ERR_INVALID, "kv_read: rows %lld", (long long)rows);
+    if (rows == 0 || b.n_seqs == 0) return Q3CU_OK;
+    if (q3cu_status st = check_rows("kv_read", "k", k, dtype, kv_stride, c.n_kv)) return st;
+    if (q3cu_status st = check_rows("kv_read", "v", v, dtype, kv_stride, c.n_kv)) return st;
+    if (k == v) return fail(Q3CU_ERR_INVALID, "kv_read: k and v are the same memory");
+    if (q3cu_status st = use_device(ctx)) return st;
+    return launched(q3::launch_kv_read(c, q3cu_dtype(cache->dtype), b, rows, k, v, dtype, kv_stride, ctx->d_status,
+                                       static_cast<cudaStream_t>(stream), ctx->sms),
+                    "kv_read launch");
 }
 
 q3cu_status q3cu_attention_paged_workspace(q3cu_ctx *ctx, int n_heads, int n_kv, size_t *bytes) {
@@ -584,6 +703,7 @@ q3cu_status q3cu_attention_paged(q3cu_ctx *ctx, const q3cu_kv_cache *cache, cons
     q3::PagedKV c;
     q3::PagedSeqs b;
     if (q3cu_status st = check_paged("attention_paged", cache, batch, n_heads, false, c, b)) return st;
+    if (cache->dtype == Q3CU_Q8_0) return fail(Q3CU_ERR_INVALID, "attention_paged: not over a Q8_0 cache");
     if (q3cu_status st = check_dtype(dtype)) return st;
     if (n_heads == 0) return fail(Q3CU_ERR_INVALID, "attention_paged: n_heads is 0");
     if (b.n_seqs > INT32_MAX / n_heads) return fail(Q3CU_ERR_INVALID, "attention_paged: n_seqs %d", b.n_seqs);
@@ -609,6 +729,7 @@ q3cu_status q3cu_attention_prompt(q3cu_ctx *ctx, const q3cu_kv_cache *cache, con
     q3::PagedSeqs b;
     if (q3cu_status st = check_paged("attention_prompt", cache, batch, n_heads, true, c, b)) return st;
     if (q3cu_status st = check_dtype(dtype)) return st;
+    if (cache->dtype == Q3CU_Q8_0) return fail(Q3CU_ERR_INVALID, "attention_prompt: not over a Q8_0 cache");
     if (cache->dtype != dtype) return fail(Q3CU_ERR_INVALID, "attention_prompt: q and the cache differ in type");
     if (n_heads == 0) return fail(Q3CU_ERR_INVALID, "attention_prompt: n_heads is 0");
     if (rows < 0 || rows + b.n_seqs > INT32_MAX / n_heads)

@@ -151,6 +151,8 @@ struct PagedKV {                       // q3cu_kv_cache, checked
     void *k, *v;
     int64_t page_stride;               // elements
     int n_pages, n_kv, page_shift;     // page_size = 1 << page_shift
+    float *k_scale, *v_scale;          // Q8_0: [n_kv][page_size][2] of a page, scale_stride floats apart
+    int64_t scale_stride;
 };
 struct PagedSeqs {                     // q3cu_kv_batch
     const int32_t *row_off, *kv_len, *pages;
@@ -172,11 +174,20 @@ struct FastDiv {
         return shift < 0 ? n : int(uint32_t((uint64_t(uint32_t(n)) * m) >> 32) >> shift);
     }
 };
-struct TurnFreq { double v[64]; };     // theta^(-j/64) / (2 pi)
+struct TurnFreq { double v[64]; };     // turns a position of each rotated pair: theta^(-j/64) / (2 pi) for the whole head
+// The first `dim` elements of a head are rotated, in neighbouring pairs or by halves.
+struct TurnForm {
+    int dim;
+    bool pairs;
+    float gain;                        // of cosines and sines
+};
 cudaError_t launch_kv_append(const PagedKV &c, q3cu_dtype cache_dt, const PagedSeqs &b, int64_t rows, const void *q,
                              const void *k, const void *v, q3cu_dtype dt, int64_t q_stride, int64_t kv_stride,
-                             int n_heads, const float *q_norm, const float *k_norm, const TurnFreq &freq, float eps,
-                             void *q_out, q3cu_dtype q_dt, uint32_t *status, cudaStream_t stream, int sms);
+                             int n_heads, const float *q_norm, const float *k_norm, const TurnFreq &freq,
+                             const TurnForm &form, float eps, void *q_out, q3cu_dtype q_dt, uint32_t *status,
+                             cudaStream_t stream, int sms);
+cudaError_t launch_kv_read(const PagedKV &c, q3cu_dtype cache_dt, const PagedSeqs &b, int64_t rows, void *k, void *v,
+                           q3cu_dtype dt, int64_t kv_stride, uint32_t *status, cudaStream_t stream, int sms);
 // One query row per sequence (row s of q: sequence s) over its kv_len keys.
 size_t attention_paged_workspace(int n_heads, int n_kv, int sms);
 cudaError_t launch_attention_paged(const PagedKV &c, q3cu_dtype cache_dt, const PagedSeqs &b, const void *q,

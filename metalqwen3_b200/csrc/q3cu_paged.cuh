@@ -131,6 +131,14 @@ __device__ __forceinline__ void store_quad(uint16_t *p, float4 v) {
     *reinterpret_cast<uint2 *>(p) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
 }
 
+// Four Q8_0 codes as floats: code + 128 as the low byte of 2^23 + it, less 2^23 + 128 (exact, and on the common pipes
+// where a conversion is not).
+__device__ __forceinline__ float4 q8_floats(uint32_t codes) {
+    codes ^= 0x80808080u;
+    auto one = [&](uint32_t pick) { return __uint_as_float(__byte_perm(codes, 0x4b000000u, pick)) - 8388736.0f; };
+    return make_float4(one(0x7440), one(0x7441), one(0x7442), one(0x7443));
+}
+
 // Whether none of them is infinite or NaN.
 __device__ __forceinline__ bool all_finite(float4 v) {
     return fmaf(v.x, 0.0f, fmaf(v.y, 0.0f, fmaf(v.z, 0.0f, v.w * 0.0f))) == 0.0f;

@@ -15,7 +15,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libq3cu.so")
 HEADER = os.path.join(os.path.dirname(HERE), "include", "q3cu.h")
 
-F32, BF16 = 0, 1
+F32, BF16, Q8_0 = 0, 1, 8
 GS = 64
 DEV_BAD_INDEX, DEV_TIMEOUT = 0x1, 0x2
 STATUS = {0: "OK", 1: "ERR_INVALID", 2: "ERR_ALIGN", 3: "ERR_GROUP", 4: "ERR_CUDA", 5: "ERR_INDEX",
@@ -34,6 +34,16 @@ class Q3Error(RuntimeError):
 class _KVCache(C.Structure):             # q3cu_kv_cache
     _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("page_stride", C.c_int64), ("n_pages", C.c_int32),
                 ("n_kv", C.c_int32), ("page_size", C.c_int32), ("head_dim", C.c_int32), ("dtype", C.c_int32)]
+
+
+class _KVCacheQ8(_KVCache):              # q3cu_kv_cache_q8: behind its first member
+    _fields_ = [("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("scale_stride", C.c_int64)]
+
+
+class _Rope(C.Structure):                # q3cu_rope
+    _fields_ = [("theta", C.c_float), ("dim", C.c_int32), ("layout", C.c_int32), ("scaling", C.c_int32),
+                ("factor", C.c_float), ("original", C.c_float), ("beta_fast", C.c_float), ("beta_slow", C.c_float),
+                ("gain", C.c_float), ("freq", C.POINTER(C.c_double))]
 
 
 class _KVBatch(C.Structure):             # q3cu_kv_batch
@@ -80,6 +90,9 @@ def load_library(path: str = LIB_PATH) -> C.CDLL:
                 "q3cu_attention": (st, [vp, vp, vp, vp, i32, i32, i32, i32, vp, i32, vp, vp, vp]),
                 "q3cu_kv_append": (st, [vp, C.POINTER(_KVCache), C.POINTER(_KVBatch), i64, vp, vp, vp, i32, i64, i64,
                                         i32, vp, vp, f32, f32, vp, i32, vp]),
+                "q3cu_kv_append_rope": (st, [vp, C.POINTER(_KVCache), C.POINTER(_KVBatch), i64, vp, vp, vp, i32, i64, i64,
+                                             i32, vp, vp, C.POINTER(_Rope), f32, vp, i32, vp]),
+                "q3cu_kv_read": (st, [vp, C.POINTER(_KVCache), C.POINTER(_KVBatch), i64, vp, vp, i32, i64, vp]),
                 "q3cu_attention_paged": (st, [vp, C.POINTER(_KVCache), C.POINTER(_KVBatch), vp, i32, i64, i32, vp,
                                               C.c_size_t, vp, vp]),
                 "q3cu_attention_paged_workspace": (st, [vp, i32, i32, C.POINTER(C.c_size_t)]),
@@ -157,10 +170,11 @@ def _rows(t, what, dtype, heads, rows, device):
 
 
 class KVCache:
-    """One layer's paged key-value cache: k and v [n_pages][n_kv][page_size][128] of one type (f32 or bf16).
-    A page is dense; pages may lie further apart (the same stride in k and v)."""
+    """One layer's paged key-value cache: k and v [n_pages][n_kv][page_size][128] of one type: f32, bf16 or, with the
+    scales k_scale and v_scale [n_pages][n_kv][page_size][2] in f32, int8 codes (Q8_0).
+    A page is dense; pages may lie further apart (the same stride in k and v, and in their scales)."""
 
-    def __init__(self, k, v):
+    def __init__(self, k, v, k_scale=None, v_scale=None):
         if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
             raise ValueError("k and v must be [n_pages][n_kv][page_size][128] of one type on one GPU")
         n_pages, n_kv, size, hd = k.shape
@@ -169,8 +183,47 @@ class KVCache:
             raise ValueError("a page must be contiguous, and k and v have one page stride")
         _tensor(k, "k"), _tensor(v, "v")
         self.k, self.v, self.n_kv, self.device = k, v, n_kv, k.get_device()
-        self.c = _KVCache(k.data_ptr(), v.data_ptr(), k.stride(0) if n_pages > 1 else n_kv * size * hd, n_pages, n_kv,
-                          size, hd, _dtype(k))
+        self.k_scale, self.v_scale = k_scale, v_scale
+        pages = (k.data_ptr(), v.data_ptr(), k.stride(0) if n_pages > 1 else n_kv * size * hd, n_pages, n_kv, size, hd)
+        self.quantised = str(k.dtype) == "torch.int8"
+        if self.quantised:
+            if k_scale is None or v_scale is None:
+                raise ValueError("a Q8_0 cache needs k_scale and v_scale")
+            shape = (n_pages, n_kv, size, hd // GS)
+            for t, what in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+                if str(_tensor(t, what, None, shape, self.device).dtype) != "torch.float32":
+                    raise TypeError(f"{what} must be torch.float32, it is {t.dtype}")
+                if t.stride()[1:] != (size * shape[3], shape[3], 1) or (n_pages > 1 and t.stride(0) != k_scale.stride(0)):
+                    raise ValueError("a page's scales must be contiguous, and k_scale and v_scale have one page stride")
+            self.c = _KVCacheQ8(*pages, Q8_0, k_scale.data_ptr(), v_scale.data_ptr(),
+                                k_scale.stride(0) if n_pages > 1 else n_kv * size * shape[3])
+        else:
+            if k_scale is not None or v_scale is not None:
+                raise ValueError("scales belong to int8 codes")
+            self.c = _KVCache(*pages, _dtype(k))
+        self.ref = C.byref(self.c)
+
+
+class Rope:
+    """How kv_append rotates heads (q3cu_rope in include/q3cu.h): the first `dim` elements, by halves or interleaved
+    (neighbouring pairs); `scaling` None, "linear" or "yarn" with its `factor` (and the `original` length); `gain` of
+    cosines and sines (None: the scaling's own); or `freq`, dim / 2 radians a position, in place of theta and scaling."""
+
+    SCALINGS = {None: 0, "linear": 1, "yarn": 2}
+
+    def __init__(self, theta=1e6, dim=128, interleaved=False, scaling=None, factor=1.0, original=0, beta_fast=32.0,
+                 beta_slow=1.0, gain=None, freq=None):
+        if scaling not in self.SCALINGS:
+            raise ValueError(f"scaling must be one of {list(self.SCALINGS)}, it is {scaling!r}")
+        if gain is not None and not gain > 0:
+            raise ValueError(f"gain must be positive, it is {gain}")
+        if freq is not None:
+            freq = [float(f) for f in freq]
+            if 2 * len(freq) != dim:
+                raise ValueError(f"freq must have dim / 2 = {dim // 2} values, it has {len(freq)}")
+        self.freq = None if freq is None else (C.c_double * len(freq))(*freq)
+        self.c = _Rope(theta, dim, int(bool(interleaved)), self.SCALINGS[scaling], factor, original, beta_fast, beta_slow,
+                       0.0 if gain is None else gain, self.freq)
         self.ref = C.byref(self.c)
 
 
@@ -371,10 +424,11 @@ class Q3CU:
         raise ValueError(f"work must be contiguous memory on the context's GPU, it is on {work.device}")
 
     def kv_append(self, cache, batch, q, k, v, q_norm=None, k_norm=None, theta=1e6, eps=1e-6, q_out=None,
-                  out_dtype=None, stream=None):
-        """QK-norm (where weights are given) and rotation of the packed rows q [rows][n_heads][128] and
-        k [rows][n_kv][128] (q may be None); keys and values into the cache; returns the rotated queries
-        (out_dtype, the cache's type by default, or q_out).  q, k, v may be slices of one projection's rows."""
+                  out_dtype=None, stream=None, rope=None):
+        """QK-norm (where weights are given) and rotation (by `theta`, or as a Rope says) of the packed rows
+        q [rows][n_heads][128] and k [rows][n_kv][128] (q may be None); keys and values into the cache; returns the
+        rotated queries (q_out, or of out_dtype: by default the cache's type, bf16 for a Q8_0 cache).  q, k, v may be
+        slices of one projection's rows."""
         dev, dtype = self.device, k.dtype
         if cache.device != dev or batch.device != dev:
             self._elsewhere(cache, batch)
@@ -390,19 +444,42 @@ class Q3CU:
         if q is not None:
             q_stride, _, heads, qp = _rows(q, "q", dtype, None, rows, dev)
             if q_out is None:
-                q_out = self._make(stream, self.torch.empty, (rows, heads, 128), dtype=out_dtype or cache.k.dtype,
-                                   device=q.device)
+                q_out = self._make(stream, self.torch.empty, (rows, heads, 128), device=q.device, dtype=out_dtype or (
+                    self.torch.bfloat16 if cache.quantised else cache.k.dtype))
             _, _, _, op = _rows(q_out, "q_out", out_dtype, heads, rows, dev)
             if not q_out.is_contiguous():
                 raise ValueError("q_out must be contiguous")
             ot = _dtype(q_out)
-        status = self.lib.q3cu_kv_append(self.ctx, cache.ref, batch.ref, rows, qp, kp, vp, _dtype(k), q_stride, kv_stride,
-                                         heads, None if q_norm is None else q_norm.data_ptr(),
-                                         None if k_norm is None else k_norm.data_ptr(), theta, eps, op, ot,
-                                         self._stream(stream))
+        call = self.lib.q3cu_kv_append if rope is None else self.lib.q3cu_kv_append_rope
+        status = call(self.ctx, cache.ref, batch.ref, rows, qp, kp, vp, _dtype(k), q_stride, kv_stride,
+                      heads, None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(),
+                      theta if rope is None else rope.ref, eps, op, ot, self._stream(stream))
         if status:
             self._check(status, "q3cu_kv_append")
         return q_out
+
+    def kv_read(self, cache, batch, rows=None, dtype=None, k_out=None, v_out=None, stream=None):
+        """The packed rows' keys and values as the cache holds them: (k, v) [rows][n_kv][128], into k_out and v_out
+        (f32 or bf16, rows may lie further apart) or new ones of `dtype` (the cache's type by default, bf16 for Q8_0; give
+        `rows` then)."""
+        dev = self.device
+        if cache.device != dev or batch.device != dev:
+            self._elsewhere(cache, batch)
+        if (k_out is None) != (v_out is None) or (k_out is None and rows is None):
+            raise ValueError("give k_out and v_out, or the number of rows")
+        if k_out is None:
+            dtype = dtype or (self.torch.bfloat16 if cache.quantised else cache.k.dtype)
+            k_out, v_out = (self._make(stream, self.torch.empty, (rows, cache.n_kv, 128), dtype=dtype, device=cache.k.device)
+                            for _ in range(2))
+        stride, rows, _, kp = _rows(k_out, "k_out", dtype, cache.n_kv, rows, dev)
+        v_stride, _, _, vp = _rows(v_out, "v_out", k_out.dtype, cache.n_kv, rows, dev)
+        if v_stride != stride:
+            raise ValueError("k_out and v_out must have one row stride")
+        status = self.lib.q3cu_kv_read(self.ctx, cache.ref, batch.ref, rows, kp, vp, _dtype(k_out), stride,
+                                       self._stream(stream))
+        if status:
+            self._check(status, "q3cu_kv_read")
+        return k_out, v_out
 
     def attention_paged_workspace(self, cache, n_heads, stream=None):
         """A workspace for attention_paged with these head counts, for any batch; calls that may run at
