@@ -39,6 +39,7 @@
 // equal shares end up to 12 us apart; one of 512 (16/8, f32) 8.5 us, all latency.
 #include "q3cu_mma.cuh"
 #include "q3cu_paged.cuh"
+#include "q3cu_split.cuh"
 #include "q3cu_tma.h"
 
 namespace q3 {
@@ -48,118 +49,15 @@ constexpr int PD_NS = 3;                                     // stages
 constexpr uint32_t PD_SIDE = 16384, PD_STAGE = 2 * PD_SIDE;  // K or V of a stage; both
 constexpr int PD_SPARE = 12288;                              // queries (f32 cache, at most 8 KB), then the join of the warps
 constexpr size_t PD_SMEM = size_t(PD_NS) * PD_STAGE + PD_SPARE + 1024;
-constexpr float PD_LOG2 = ATT_SCALE * 1.44269504088896341f;  // scores to base-2 exponents
-constexpr int PD_PART = HD + 2;                              // floats of a row's partial result: 128, maximum, sum
-
 template <typename TC> __host__ __device__ constexpr int pd_tile() { return int(PD_SIDE) / (HD * Elem<TC>::BYTES); }   // positions of a stage
 
-// a / b for 0 <= a, 0 < b: 32-bit division where it serves (a 64-bit one is a chain of some hundred instructions).
-__device__ __forceinline__ int64_t quot(int64_t a, int b) {
-    return a < (int64_t(1) << 32) ? int64_t(uint32_t(a) / uint32_t(b)) : a / b;
-}
-
-// How `total` tiles are cut into `runs` runs: the first `more` have each + 1 tiles, the others `each`.
-struct PagedCut {
-    int64_t total, each;
-    int more;
-    __device__ __forceinline__ PagedCut(int64_t t, int runs) : total(t), each(quot(t, runs)), more(int(t - each * runs)) {}
-    __device__ __forceinline__ int64_t begin(int run) const { return each * run + min(run, more); }
-    __device__ __forceinline__ int run_of(int64_t u) const {                 // u < total
-        const int64_t edge = (each + 1) * more;
-        return u < edge ? int(each < INT32_MAX ? quot(u, int(each + 1)) : u / (each + 1))
-                        : more + int(each < INT32_MAX ? quot(u - edge, int(each)) : (u - edge) / each);
-    }
-};
-
-// A place in the batch's tiles: sequence, kv head, tile, and the sequence's length and tiles.
-struct PagedWalk {
-    int s, head, tile, len, tiles;
-};
-template <typename TC>
-__device__ __forceinline__ int tiles_of(int len) { return (len + pd_tile<TC>() - 1) / pd_tile<TC>(); }
-
-// Inclusive sum over the lanes; 32 sequences have at most 2^31 / 32 tiles each.
-__device__ __forceinline__ uint32_t warp_prefix(uint32_t x) {
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t y = __shfl_up_sync(FULL, x, o);
-        if ((threadIdx.x & 31) >= o) x += y;
-    }
-    return x;
-}
-// The tiles of the whole batch, the run's [u0, u1) of them and the place of u0 (one warp; every lane returns it).
-template <typename TC>
-__device__ __forceinline__ PagedWalk walk_run(const PagedSeqs &b, const PagedKV &c, int run, int runs, PagedCut &cut,
-                                              int64_t &u0, int64_t &u1, uint32_t *status) {
-    PagedWalk w = {};
-    const int lane = threadIdx.x & 31;
-    int64_t total = 0;                                       // in tiles of one kv head
-    uint32_t end = 0;
-    int len = 0;
-    for (int s0 = 0; s0 < b.n_seqs; s0 += 32) {              // 32 sequences at a time
-        len = s0 + lane < b.n_seqs ? paged_len(b, c, s0 + lane, status) : 0;
-        end = warp_prefix(uint32_t(tiles_of<TC>(len)));
-        total += __shfl_sync(FULL, end, 31);
-    }
-    cut = PagedCut(total * c.n_kv, runs);
-    u0 = cut.begin(run);
-    u1 = cut.begin(run + 1);
-    int64_t u = u0;
-    for (int s0 = 0; s0 < b.n_seqs; s0 += 32) {
-        if (b.n_seqs > 32) {                                 // otherwise the lanes still hold them
-            len = s0 + lane < b.n_seqs ? paged_len(b, c, s0 + lane, nullptr) : 0;
-            end = warp_prefix(uint32_t(tiles_of<TC>(len)));
-        }
-        const unsigned hit = __ballot_sync(FULL, u < int64_t(end) * c.n_kv);
-        if (hit) {
-            const int l = __ffs(hit) - 1;
-            w.s = s0 + l;
-            w.len = __shfl_sync(FULL, len, l);
-            w.tiles = tiles_of<TC>(w.len);
-            const int64_t at = u - int64_t(__shfl_sync(FULL, end, l) - uint32_t(w.tiles)) * c.n_kv;
-            w.head = int(quot(at, w.tiles));
-            w.tile = int(at - int64_t(w.head) * w.tiles);
-            return w;
-        }
-        u -= int64_t(__shfl_sync(FULL, end, 31)) * c.n_kv;
-    }
-    return w;
-}
-// `n` tiles further, which lie in the same (sequence, head) or begin the next one that has any (one warp: 32 sequences at
-// a time, so that a million empty ones take 3 ms and not 100, while others wait).
-template <typename TC>
-__device__ __forceinline__ void walk_on(const PagedSeqs &b, const PagedKV &c, PagedWalk &w, int n) {
-    w.tile += n;
-    if (w.tile < w.tiles) return;
-    w.tile = 0;
-    if (++w.head < c.n_kv) return;
-    w.head = 0;
-    for (++w.s; w.s < b.n_seqs; w.s += 32) {
-        const int s = w.s + int(threadIdx.x & 31), len = s < b.n_seqs ? paged_len(b, c, s, nullptr) : 0;
-        const unsigned some = __ballot_sync(FULL, len > 0);
-        if (some) {
-            const int l = __ffs(some) - 1;
-            w.s += l;
-            w.len = __shfl_sync(FULL, len, l);
-            w.tiles = tiles_of<TC>(w.len);
-            return;
-        }
-    }
-}
-
-// One pair of result elements (row, dims at, at + step) as the output's type.
-__device__ __forceinline__ void put2(float *p, int step, float x, float y) { p[0] = x, p[step] = y; }
-__device__ __forceinline__ void put2(uint16_t *p, int step, float x, float y) {
-    if (step == 1) *reinterpret_cast<uint32_t *>(p) = pack_bf16(x, y);
-    else p[0] = uint16_t(f32_to_bf16(x)), p[step] = uint16_t(f32_to_bf16(y));
-}
-
-// WIDE: more than 8 query heads to a kv head (two blocks of columns).
-template <typename T, typename TC, bool WIDE>
+// WIDE: more than 8 query heads to a kv head (two blocks of columns).  Seqs: whole sequences, or their tails behind what
+// they share, whose results go to `tails` ([n_seqs][n_heads] rows of PD_PART floats) if they are not all of a sequence.
+template <typename T, typename TC, bool WIDE, typename Seqs>
 __global__ void __launch_bounds__(PD_THREADS, 2)
 paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, const PagedKV c,
-                   const PagedSeqs b, const typename Elem<T>::type *q, int64_t q_stride, int n_heads, int group,
-                   typename Elem<T>::type *out, float *part, uint32_t *status) {
+                   const Seqs b, const typename Elem<T>::type *q, int64_t q_stride, int n_heads, int group,
+                   typename Elem<T>::type *out, float *part, float *tails, uint32_t *status) {
     constexpr bool CF32 = Elem<TC>::BYTES == 4;
     constexpr int TILE = pd_tile<TC>(), NH = WIDE ? 2 : 1;   // NH: blocks of eight heads
     extern __shared__ uint8_t pd_dyn[];
@@ -183,7 +81,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
 
     PagedCut cut(0, 1);
     int64_t u0, u1;
-    PagedWalk w = walk_run<TC>(b, c, int(blockIdx.x), int(gridDim.x), cut, u0, u1,
+    PagedWalk w = walk_run<TILE>(b, c, int(blockIdx.x), int(gridDim.x), cut, u0, u1,
                                blockIdx.x == 0 && warp == 0 ? status : nullptr);
     for (int s = int(blockIdx.x); s < b.n_seqs; s += int(gridDim.x))       // sequences without positions: zeros
         if (b.kv_len[s] <= 0 || b.max_pages == 0)
@@ -197,8 +95,8 @@ paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
         const int bs = min(c.page_shift, TS), br = 1 << bs, ns = TS - bs;     // rows of a box; log2 of boxes of a tile
         const int box = lane & ((1 << ns) - 1), col = (lane >> ns) & (CB - 1), side = lane >> (ns + CS);
         auto page_of = [&]() -> int {                        // n_pages reads as zeros
-            const int t = w.tile * TILE + box * br;
-            if (side > 1 || t >= w.len) return c.n_pages;
+            const int t = w.template pos<TILE, Seqs>(w.tile) + box * br;
+            if (side > 1 || t >= w.len || (Seqs::TAILS && t + br <= w.from)) return c.n_pages;
             const int p = paged_page(b, c, w.s, t, status);
             return p < 0 ? c.n_pages : p;
         };
@@ -206,9 +104,9 @@ paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
         int page = page_of(), e = 0;
         bool ok = true;
         for (int64_t u = u0; u < u1; ++u, ++e) {
-            const int head = w.head, slot = (w.tile * TILE + box * br) & ((1 << c.page_shift) - 1), now = page;
+            const int head = w.head, slot = (w.template pos<TILE, Seqs>(w.tile) + box * br) & ((1 << c.page_shift) - 1), now = page;
             if (u + 1 < u1) {
-                walk_on<TC>(b, c, w, 1);
+                walk_on<TILE>(b, c, w, 1);
                 page = page_of();                            // under way while this tile waits for its stage
             }
             const int st = e % PD_NS;
@@ -286,7 +184,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
                 continue;
             }
             const uint32_t ka = ring_a + st * PD_STAGE, va = ka + PD_SIDE;
-            const int left = w.len - (w.tile + i) * TILE - key0;             // visible ones of this warp's 16
+            const int key_pos = w.template pos<TILE, Seqs>(w.tile + i) + key0, left = w.len - key_pos;   // visible ones of this warp's 16
             float s[NH][4];                                  // positions g and g + 8 by heads 8 n + 2 t4, + 1
 #pragma unroll
             for (int n = 0; n < NH; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
@@ -373,6 +271,15 @@ paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
                     for (int x = 0; x < 4; ++x)
                         if (g + 8 * (x >> 1) >= left) s[n][x] = -INFINITY;
             }
+            // tails: how many of the 16 lie before the span (in its first tile)
+            const int early = Seqs::TAILS ? w.from - key_pos : 0;
+            if (Seqs::TAILS && early > 0) {
+#pragma unroll
+                for (int n = 0; n < NH; ++n)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+                        if (g + 8 * (x >> 1) < early) s[n][x] = -INFINITY;
+            }
             float f[NH][2];
             bool grow = false;
 #pragma unroll
@@ -424,7 +331,9 @@ paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
                         const int k0 = key0 + 8 * kb + 2 * t4;
                         const uint32_t at = va + d * (PD_SIDE / 4) + k0 * 128;
                         const float4 v0 = lds4(at + ((g ^ (2 * t4)) << 4)), v1 = lds4(at + 128 + ((g ^ (2 * t4 + 1)) << 4));
-                        const bool live0 = 8 * kb + 2 * t4 < left, live1 = 8 * kb + 2 * t4 + 1 < left;
+                        const int p0 = 8 * kb + 2 * t4;
+                        const bool live0 = p0 < left && (!Seqs::TAILS || p0 >= early);
+                        const bool live1 = p0 + 1 < left && (!Seqs::TAILS || p0 + 1 >= early);
                         const float x0[4] = {v0.x, v0.y, v0.z, v0.w}, x1[4] = {v1.x, v1.y, v1.z, v1.w};
 #pragma unroll
                         for (int y = 0; y < 2; ++y) {
@@ -466,6 +375,10 @@ paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
 #pragma unroll
                 for (int x = 0; x < 2; ++x)
                     keep[x] = (8 * x + 2 * t4 < left ? 0xffffu : 0u) | (8 * x + 2 * t4 + 1 < left ? 0xffff0000u : 0u);
+                if (Seqs::TAILS && early > 0)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x)
+                        keep[x] &= (8 * x + 2 * t4 >= early ? 0xffffu : 0u) | (8 * x + 2 * t4 + 1 >= early ? 0xffff0000u : 0u);
                 const int key = key0 + (lane >> 4) * 8 + (lane & 7);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
@@ -558,13 +471,15 @@ paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
                 for (int h = 0; h < 2; ++h) {
                     const int row = 8 * n + 2 * t4 + h;
                     if (row >= group) continue;
-                    if (whole) {
+                    if (whole && (!Seqs::TAILS || w.from == 0)) {
                         const float r = 1.0f / l[n][h];
                         typename Elem<T>::type *dst = out + (int64_t(w.s) * n_heads + w.head * group + row) * HD + at0;
 #pragma unroll
                         for (int j = 0; j < 8; ++j) put2(dst + block(j), step, o[j][n][h] * r, o[j][n][2 + h] * r);
                     } else {
-                        float *pd = part + ((2 * int64_t(blockIdx.x) + (u != u0)) * group + row) * PD_PART;
+                        float *pd = Seqs::TAILS && whole
+                                        ? tails + (int64_t(w.s) * n_heads + w.head * group + row) * PD_PART
+                                        : part + ((2 * int64_t(blockIdx.x) + (u != u0)) * group + row) * PD_PART;
 #pragma unroll
                         for (int j = 0; j < 8; ++j) put2(pd + at0 + block(j), step, o[j][n][h], o[j][n][2 + h]);
                         if (g == 0) pd[HD] = m[n][h], pd[HD + 1] = l[n][h];
@@ -572,118 +487,58 @@ paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
                 }
         }
         u += run;
-        if (u < u1) walk_on<TC>(b, c, w, run);
+        if (u < u1) walk_on<TILE>(b, c, w, run);
         named_sync(1, PD_WARPS * 32);
     }
 }
 
-// Joins what the runs left of one query head, one CTA per run and head of the group; the CTA of the second run of a
-// (sequence, kv head) does it: o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i.  The
-// parts' maxima and sums are read side by side, one thread each; then two groups of 128 threads (thread = element) add
-// half of the weighted parts each, eight loads under way at a time.  The order of every sum is fixed.
-constexpr int PJ_GROUPS = 2, PJ_THREADS = PJ_GROUPS * HD, PJ_RUNS = 1024;
-template <typename T, typename TC>
-__global__ void __launch_bounds__(PJ_THREADS) paged_join_kernel(const PagedKV c, const PagedSeqs b, int n_heads, int group,
-                                                                int runs, typename Elem<T>::type *out, const float *part) {
-    __shared__ float weight[PJ_RUNS], red[2][PJ_THREADS / 32], sum[PJ_GROUPS][HD];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = threadIdx.x % HD, half_id = threadIdx.x / HD;
-    // Before the wait: the lengths are older than the first kernel, which has begun (this one starts when all its CTAs
-    // have passed their own wait).
-    PagedCut cut(0, 1);
-    int64_t u0, u1;
-    const int second = int(blockIdx.x) + 1;
-    const PagedWalk w = walk_run<TC>(b, c, second, runs, cut, u0, u1, nullptr);
-    const int64_t a = u0 - w.tile;                           // the (sequence, head)'s first tile
-    const int first = second - 1;
-    // it has tiles, does not begin with a new (sequence, head), and is the second of that one's runs
-    const bool joins = u0 != u1 && w.tile != 0 && a >= cut.begin(first);
-    // The first CTA waits whatever it finds: the next launch waits for this grid alone, which must not end before the first
-    // kernel.  (Were all to wait: 1.6 us more for nine ragged sequences, since not all fit beside that kernel.)
-    if (!joins && blockIdx.x + blockIdx.y > 0) return;
-    griddep_wait();
-    if (!joins) return;
-    const int last = cut.run_of(a + w.tiles - 1), n = last - first + 1;
-    // part i: in the first slot of run first + i, but the second of a run that began before this (sequence, head)
-    const float *row = part + int(blockIdx.y) * PD_PART;
-    const int64_t run_stride = int64_t(2) * group * PD_PART;
-    const float *head = row + first * run_stride + (a != cut.begin(first) ? group * PD_PART : 0);
-    auto at = [&](int i) { return i == 0 ? head : row + (first + i) * run_stride; };
-    // the first parts of this thread's half are on their way together with the maxima and sums
-    const int i0 = n * half_id / PJ_GROUPS, i1 = n * (half_id + 1) / PJ_GROUPS;
-    float v[8];
-#pragma unroll
-    for (int x = 0; x < 8; ++x) v[x] = i0 + x < i1 ? at(i0 + x)[d] : 0.0f;
-    float m = -INFINITY;
-    for (int i = threadIdx.x; i < n; i += PJ_THREADS) {
-        weight[i] = at(i)[HD];
-        m = fmaxf(m, weight[i]);
-    }
-    m = warp_max(m);
-    if (lane == 0) red[0][warp] = m;
-    __syncthreads();
-    m = warp_max(red[0][lane % (PJ_THREADS / 32)]);
-    float l = 0.0f;
-    for (int i = threadIdx.x; i < n; i += PJ_THREADS) {
-        const float f = weight[i] == m ? 1.0f : ex2_approx_ftz((weight[i] - m) * PD_LOG2);
-        weight[i] = f;
-        l = fmaf(at(i)[HD + 1], f, l);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(FULL, l, o);
-    if (lane == 0) red[1][warp] = l;
-    __syncthreads();
-    float o = 0.0f;
-#pragma unroll
-    for (int x = 0; x < 8; ++x)
-        if (i0 + x < i1) o = fmaf(v[x], weight[i0 + x], o);
-#pragma unroll 8
-    for (int i = i0 + 8; i < i1; ++i) o = fmaf(at(i)[d], weight[i], o);
-    sum[half_id][d] = o;
-    __syncthreads();
-    if (half_id) return;
-    l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < PJ_THREADS / 32; ++i) l += red[1][i];
-    o = (sum[0][d] + sum[1][d]) / l;
-    typename Elem<T>::type *dst = out + (int64_t(w.s) * n_heads + w.head * group + blockIdx.y) * HD + d;
-    if constexpr (Elem<T>::BYTES == 4) *dst = o;
-    else *dst = uint16_t(f32_to_bf16(o));
-}
-
-static int paged_runs(int sms) { return 2 * sms < PJ_RUNS ? 2 * sms : PJ_RUNS; }
 
 size_t attention_paged_workspace(int n_heads, int n_kv, int sms) {
     return size_t(paged_runs(sms)) * 2 * (n_heads / n_kv) * PD_PART * sizeof(float);
 }
 
-template <typename T, typename TC>
-static cudaError_t launch_split(const PagedKV &c, const PagedSeqs &b, const void *q, int64_t q_stride, int n_heads,
-                                void *work, void *out, uint32_t *status, cudaStream_t stream, int sms, int slot) {
+// The first kernel alone.
+template <typename T, typename TC, typename Seqs>
+static cudaError_t launch_split(const PagedKV &c, const Seqs &b, const void *q, int64_t q_stride, int n_heads, float *part,
+                                float *tails, void *out, uint32_t *status, cudaStream_t stream, int runs, int slot) {
     typedef typename Elem<T>::type E;
     CUtensorMap mk, mv;
     const q3cu_dtype dt = Elem<TC>::BYTES == 4 ? Q3CU_F32 : Q3CU_BF16;
     if (!encode_pages_map(&mk, c.k, c, dt, pd_tile<TC>()) || !encode_pages_map(&mv, c.v, c, dt, pd_tile<TC>())) return cudaErrorInvalidValue;
-    const int group = n_heads / c.n_kv, runs = paged_runs(sms);
-    auto *kernel = group > 8 ? paged_split_kernel<T, TC, true> : paged_split_kernel<T, TC, false>;
+    const int group = n_heads / c.n_kv;
+    auto *kernel = group > 8 ? paged_split_kernel<T, TC, true, Seqs> : paged_split_kernel<T, TC, false, Seqs>;
     cudaError_t e = ensure_smem_attr(reinterpret_cast<const void *>(kernel), PD_SMEM, slot + (group > 8));
     if (e != cudaSuccess) return e;
-    e = launch_dependent(kernel, dim3(runs), dim3(PD_THREADS), PD_SMEM, stream, mk, mv, c, b, static_cast<const E *>(q),
-                         q_stride, n_heads, group, static_cast<E *>(out), static_cast<float *>(work), status);
+    return launch_dependent(kernel, dim3(runs), dim3(PD_THREADS), PD_SMEM, stream, mk, mv, c, b, static_cast<const E *>(q),
+                            q_stride, n_heads, group, static_cast<E *>(out), part, tails, status);
+}
+
+template <typename T, typename TC>
+static cudaError_t launch_whole(const PagedKV &c, const PagedSeqs &b, const void *q, int64_t q_stride, int n_heads,
+                                void *work, void *out, uint32_t *status, cudaStream_t stream, int sms, int slot) {
+    const int runs = paged_runs(sms);
+    float *part = static_cast<float *>(work);
+    cudaError_t e = launch_split<T, TC>(c, WholeSeqs{b}, q, q_stride, n_heads, part, nullptr, out, status, stream, runs, slot);
     if (e != cudaSuccess) return e;
-    return launch_dependent(paged_join_kernel<T, TC>, dim3(runs - 1, group), dim3(PJ_THREADS), 0, stream, c, b,
-                            n_heads, group, runs, static_cast<E *>(out), static_cast<const float *>(work));
+    return launch_paged_join<T, pd_tile<TC>()>(c, b, n_heads, runs, out, part, stream);
 }
 
 cudaError_t launch_attention_paged(const PagedKV &c, q3cu_dtype cache_dt, const PagedSeqs &b, const void *q,
                                    q3cu_dtype dt, int64_t q_stride, int n_heads, void *work, void *out,
                                    uint32_t *status, cudaStream_t stream, int sms) {
+    if (cache_dt == Q3CU_Q8_0) return launch_paged_q8(c, b, q, dt, q_stride, n_heads, work, out, status, stream, sms);
     if (dt == Q3CU_F32)
         return cache_dt == Q3CU_F32
-                   ? launch_split<float, float>(c, b, q, q_stride, n_heads, work, out, status, stream, sms, 33)
-                   : launch_split<float, bf16raw>(c, b, q, q_stride, n_heads, work, out, status, stream, sms, 35);
+                   ? launch_whole<float, float>(c, b, q, q_stride, n_heads, work, out, status, stream, sms, 33)
+                   : launch_whole<float, bf16raw>(c, b, q, q_stride, n_heads, work, out, status, stream, sms, 35);
     return cache_dt == Q3CU_F32
-               ? launch_split<bf16raw, float>(c, b, q, q_stride, n_heads, work, out, status, stream, sms, 37)
-               : launch_split<bf16raw, bf16raw>(c, b, q, q_stride, n_heads, work, out, status, stream, sms, 39);
+               ? launch_whole<bf16raw, float>(c, b, q, q_stride, n_heads, work, out, status, stream, sms, 37)
+               : launch_whole<bf16raw, bf16raw>(c, b, q, q_stride, n_heads, work, out, status, stream, sms, 39);
+}
+
+cudaError_t launch_tails_bf16(const PagedKV &c, const TailSeqs &b, const void *q, int64_t q_stride, int n_heads, float *part,
+                              float *tails, void *out, uint32_t *status, cudaStream_t stream, int runs) {
+    return launch_split<bf16raw, bf16raw>(c, b, q, q_stride, n_heads, part, tails, out, status, stream, runs, 48);
 }
 
 }  // namespace q3

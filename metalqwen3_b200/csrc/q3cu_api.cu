@@ -703,7 +703,6 @@ q3cu_status q3cu_attention_paged(q3cu_ctx *ctx, const q3cu_kv_cache *cache, cons
     q3::PagedKV c;
     q3::PagedSeqs b;
     if (q3cu_status st = check_paged("attention_paged", cache, batch, n_heads, false, c, b)) return st;
-    if (cache->dtype == Q3CU_Q8_0) return fail(Q3CU_ERR_INVALID, "attention_paged: not over a Q8_0 cache");
     if (q3cu_status st = check_dtype(dtype)) return st;
     if (n_heads == 0) return fail(Q3CU_ERR_INVALID, "attention_paged: n_heads is 0");
     if (b.n_seqs > INT32_MAX / n_heads) return fail(Q3CU_ERR_INVALID, "attention_paged: n_seqs %d", b.n_seqs);

@@ -193,6 +193,9 @@ size_t attention_paged_workspace(int n_heads, int n_kv, int sms);
 cudaError_t launch_attention_paged(const PagedKV &c, q3cu_dtype cache_dt, const PagedSeqs &b, const void *q,
                                    q3cu_dtype dt, int64_t q_stride, int n_heads, void *work, void *out,
                                    uint32_t *status, cudaStream_t stream, int sms);
+// The same over a Q8_0 cache (k_paged_q8.cu).
+cudaError_t launch_paged_q8(const PagedKV &c, const PagedSeqs &b, const void *q, q3cu_dtype dt, int64_t q_stride,
+                            int n_heads, void *work, void *out, uint32_t *status, cudaStream_t stream, int sms);
 // Packed query rows, causal: a row at position p over the keys 0..p.
 cudaError_t launch_attention_prompt(const PagedKV &c, const PagedSeqs &b, int64_t rows, const void *q, q3cu_dtype dt,
                                     int64_t q_stride, int n_heads, void *out, uint32_t *status, cudaStream_t stream,

@@ -124,23 +124,37 @@ bool encode_row_lines_map_uncached(CUtensorMap *map, const void *base, uint64_t 
 bool encode_lines_map(CUtensorMap *map, const void *base, q3cu_dtype dt, int rank, const uint64_t *dims,
                       const uint64_t *strides, const uint32_t *box) {
     EncodeTiled enc = encoder();
-    if (!enc || box[0] != (dt == Q3CU_F32 ? 32 : 64)) return false;
+    if (!enc || box[0] != (dt == Q3CU_F32 ? 32 : dt == Q3CU_Q8_0 ? 128 : 64)) return false;
     cuuint64_t d[4], st[3];
     for (int i = 0; i < rank; ++i) d[i] = dims[i];
     for (int i = 0; i + 1 < rank; ++i) st[i] = strides[i];
     const cuuint32_t estr[4] = {1, 1, 1, 1};
-    return enc(map, dt == Q3CU_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
-               cuuint32_t(rank), const_cast<void *>(base), d, st, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+    const CUtensorMapDataType type = dt == Q3CU_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                     : dt == Q3CU_Q8_0 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                                       : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    return enc(map, type, cuuint32_t(rank), const_cast<void *>(base), d, st, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 bool encode_pages_map(CUtensorMap *map, const void *base, const PagedKV &c, q3cu_dtype dt, int keys) {
-    const uint64_t size = uint64_t(1) << c.page_shift, es = dt == Q3CU_F32 ? 4 : 2;
+    const uint64_t size = uint64_t(1) << c.page_shift, es = dt == Q3CU_F32 ? 4 : dt == Q3CU_Q8_0 ? 1 : 2;
     const uint64_t dims[4] = {PAGED_HD, size, uint64_t(c.n_kv), uint64_t(c.n_pages)};
     const uint64_t strides[3] = {PAGED_HD * es, size * PAGED_HD * es, uint64_t(c.page_stride) * es};
     const uint32_t box[4] = {uint32_t(128 / es), uint32_t(size < uint64_t(keys) ? size : keys), 1, 1};
     return encode_lines_map(map, base, dt, 4, dims, strides, box);
+}
+
+bool encode_scales_map(CUtensorMap *map, const void *base, const PagedKV &c, int keys) {
+    EncodeTiled enc = encoder();
+    if (!enc) return false;
+    const uint64_t size = uint64_t(1) << c.page_shift;
+    const cuuint64_t dims[3] = {2 * size, cuuint64_t(c.n_kv), cuuint64_t(c.n_pages)};
+    const cuuint64_t strides[2] = {size * 8, cuuint64_t(c.scale_stride) * 4};
+    const cuuint32_t box[3] = {cuuint32_t(2 * (size < uint64_t(keys) ? size : keys)), 1, 1}, estr[3] = {1, 1, 1};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<void *>(base), dims, strides, box, estr,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 }  // namespace q3

@@ -44,7 +44,7 @@ bool encode_f32_2d_map(CUtensorMap *map, const void *base, uint64_t rows, uint64
                        uint32_t box_rows, bool swizzle128);
 
 // A tensor of `rank` (3 or 4) dimensions of dt, innermost first and dense in dimension 0 (strides[i]: bytes between
-// neighbours in dimension i + 1, multiples of 16), read in boxes of 128 B (64 bf16 or 32 f32) by box[1..]; a box
+// neighbours in dimension i + 1, multiples of 16), read in boxes of 128 B (64 bf16, 32 f32 or 128 codes) by box[1..]; a box
 // lands as lines of 128 B with the 128-byte swizzle (1024-byte aligned), elements outside the tensor as zeros.
 // Encoded anew by every call (a fraction of a microsecond).
 bool encode_lines_map(CUtensorMap *map, const void *base, q3cu_dtype dt, int rank, const uint64_t *dims,
@@ -52,6 +52,10 @@ bool encode_lines_map(CUtensorMap *map, const void *base, q3cu_dtype dt, int ran
 
 // The pages of a cache's k or v (base) for tiles of `keys` positions: a box is 128 B by min(page size, keys) rows.
 bool encode_pages_map(CUtensorMap *map, const void *base, const PagedKV &c, q3cu_dtype dt, int keys);
+
+// The scales of a Q8_0 cache's k or v (base) for tiles of `keys` positions: a box is min(page size, keys) positions' pairs
+// of one kv head, dense; x is twice the slot, y the head, z the page.  Pages outside the cache read as zeros.
+bool encode_scales_map(CUtensorMap *map, const void *base, const PagedKV &c, int keys);
 
 #if defined(__CUDACC__)
 __device__ __forceinline__ void tma_load_2d(void *dst, const CUtensorMap *map, int x, int y, uint64_t *bar) {

@@ -1,0 +1,152 @@
+"""Attention over a Q8_0 paged cache against the formula in binary64 over the products of codes and scales.
+
+Tolerances as in test_gpu_paged.py.  What is different here stays within their terms: f32 queries and weights are two f16
+parts (2 u each), sums of products of codes are exact up to the tensor cores' cut (2 u a step of 16, 8 steps), scales are
+one rounding each.  An f16 part is no finer than 2^-25, half its least number, and the largest query element of a row (the
+largest value scale of 32 positions) is lifted to 2^14 or more, so that an element is also off by up to 2^-39 of the row's
+largest: a score by 128 * 2^-39 max|q| max|k| / sqrt(128), a result of n positions by n 2^-39 (128 / 127) max|v|.
+Where the result is bf16 a weight is one f16 part: 2^-11 relative each.  Prompts round every element
+of the cache to bf16 as well (2^-8 relative): a score moves by at most 2^-8 A, a value by 2^-8 of itself.
+"""
+import math
+
+import pytest
+import torch
+
+from test_gpu_kv_forms import I8, Quantised
+from test_gpu_paged import BF16, DECODE, F32, H, U, attend, offsets, queries
+
+pytestmark = pytest.mark.gpu
+W = 2.0 ** -11
+
+
+def check_attention(got, q, k, v, seen, dtype, weight_rounding=0.0, element_rounding=0.0):
+    o, pv, a = attend(q.double(), k, v, seen)
+    n, top = max(1, k.shape[0]), lambda x: float(x.abs().max()) if x.numel() else 0.0
+    ds = (160 * U + element_rounding) * a + math.sqrt(128) * 2.0 ** -39 * top(q) * top(k)
+    tol = (torch.expm1(2 * ds) + (n + 64) * U + weight_rounding + element_rounding) * pv + n * 2.0 ** -39 * 1.01 * top(v)
+    if dtype == BF16:
+        tol = tol + H * (o.abs() + tol)
+    bad = ~((got.double() - o).abs() <= tol + 1e-30)
+    assert not bad.any(), (int(bad.sum()), bad.nonzero()[:4].tolist(), float((got.double() - o).abs().max()),
+                           float(tol.max()))
+
+
+@pytest.mark.parametrize("io", [F32, BF16])
+@pytest.mark.parametrize("heads,n_kv,page,lens", DECODE + [(10, 2, 256, [127, 128, 129, 255, 256, 257, 700]),
+                                                           (3, 1, 128, [33, 95, 96, 97, 4000])])
+def test_attention_paged(q3, io, heads, n_kv, page, lens):
+    p = Quantised(lens, n_kv, page, seed=11).fill(12)
+    q = queries(len(lens), heads, io, 13)
+    cache, batch = p.handles()
+    got = q3.attention_paged(cache, batch, q)
+    for s, n in enumerate(lens):
+        k, v = p.rows(s)
+        check_attention(got[s:s + 1], q[s:s + 1], k, v, [n], io, W if io == BF16 else 0.0)
+    assert q3.device_status() == 0
+
+
+def test_attention_paged_peaked_flat_and_uneven(q3):
+    """Scores in the thousands, all equal, queries and scales far from 1, and scales that differ by 10^6 within a tile."""
+    for scale, size in ((60.0, 1.0), (0.0, 1.0), (1e-12, 1e9), (1e15, 1e-14)):
+        p = Quantised([777, 64], 2, 16, seed=14).fill(15, size)
+        q = queries(2, 8, F32, 16, scale)
+        got = q3.attention_paged(*p.handles(), q)
+        for s, n in enumerate(p.lens):
+            check_attention(got[s:s + 1], q[s:s + 1], *p.rows(s), [n], F32)
+    p = Quantised([300], 2, 16, seed=14).fill(15)
+    page, slot = p.where(0, range(0, 300, 3))
+    p.vs[page, :, slot] *= 1e-6
+    p.ks[page, :, slot] *= 1e-3
+    q = queries(1, 8, F32, 16)
+    check_attention(q3.attention_paged(*p.handles(), q), q, *p.rows(0), [300], F32)
+
+
+def test_attention_paged_strides_and_work(q3):
+    """Pages (and their scales) further apart than they are large; queries inside wider rows; any workspace contents."""
+    p = Quantised([100, 257, 0], 4, 32, seed=17, gap=4096 + 32).fill(18)
+    wide = queries(3, 24, F32, 19)
+    q = wide[:, 4:12]
+    cache, batch = p.handles()
+    out = torch.empty((3, 8, 128), device="cuda")
+    work = torch.full((q3.attention_paged_workspace(cache, 8).numel(),), 255, dtype=torch.uint8, device="cuda")
+    for _ in range(2):
+        assert q3.attention_paged(cache, batch, q, out=out, work=work) is out
+        for s, n in enumerate(p.lens):
+            check_attention(out[s:s + 1], q[s:s + 1], *p.rows(s), [n], F32)
+
+
+def test_attention_paged_bad_pages(q3):
+    """Bad page ids read as zeros and are flagged; a length beyond the table is cut; a negative one is empty."""
+    from metalqwen3_b200.q3cu import DEV_BAD_INDEX
+    p = Quantised([100, 40, 50, 50], 2, 16, seed=20).fill(21)
+    k, v = p.rows(0)
+    for i, bad in ((1, -3), (4, p.n_pages)):
+        p.table[0, i] = bad
+        k[16 * i:16 * i + 16] = 0
+        v[16 * i:16 * i + 16] = 0
+    cap = p.max_pages * 16
+    p.table[2] = p.table[0, 0]                  # one page many times over: a full table row
+    p.kv_len[2], p.kv_len[3] = cap + 1, -5
+    q = queries(4, 4, F32, 22)
+    got = q3.attention_paged(*p.handles(), q)
+    assert q3.device_status() == DEV_BAD_INDEX and q3.device_status() == 0
+    check_attention(got[:1], q[:1], k, v, [100], F32)
+    check_attention(got[1:2], q[1:2], *p.rows(1), [40], F32)
+    again = torch.arange(cap, device="cuda") % 16
+    page = p.table[0, 0].long()
+    kk, vv = ((t[page].double() * c[page].double().repeat_interleave(64, -1)).transpose(0, 1)[again]
+              for t, c in ((p.k, p.ks), (p.v, p.vs)))
+    check_attention(got[2:3], q[2:3], kk, vv, [cap], F32)
+    assert (got[3] == 0).all()
+
+
+@pytest.mark.parametrize("io", [F32, BF16])
+def test_appended_and_attended_as_a_graph(q3, io):
+    """A serving step's append and attention, captured and replayed while the sequences grow."""
+    lens, heads, n_kv = [5, 130, 31], 8, 2
+    p = Quantised([n + 40 for n in lens], n_kv, 16, seed=30).fill(31)
+    qkv = queries(3, heads + 2 * n_kv, F32, 32)
+    cache, batch = p.handles([0, 1, 2, 3])
+    work, out = q3.attention_paged_workspace(cache, heads), torch.empty((3, heads, 128), dtype=io, device="cuda")
+    q_out = torch.empty_like(out)
+
+    def step():
+        q3.kv_append(cache, batch, qkv[:, :heads], qkv[:, heads:heads + n_kv], qkv[:, heads + n_kv:], q_out=q_out)
+        q3.attention_paged(cache, batch, q_out, out=out, work=work)
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        step()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            step()
+    for n in (1, 7, 40):
+        now = [x + n for x in lens]
+        p.kv_len.copy_(torch.tensor(now, dtype=torch.int32))
+        qkv.copy_(queries(3, heads + 2 * n_kv, F32, 33 + n))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for s, x in enumerate(now):
+            p.lens = now
+            check_attention(out[s:s + 1], q_out[s:s + 1], *p.rows(s), [x], io, W if io == BF16 else 0.0)
+    assert q3.device_status() == 0
+
+
+def test_unused_scales_and_nan(q3):
+    """NaN scales behind the length (there everywhere: the pool is full of them) reach nothing; one at a value of the
+    sequence reaches its 64 elements only, one at a key its head only."""
+    p = Quantised([100, 50], 2, 16, seed=40).fill(41)
+    q = queries(2, 4, F32, 42)
+    clean = q3.attention_paged(*p.handles(), q)
+    assert torch.isfinite(clean).all()
+    page, slot = p.where(0, [70])
+    p.vs[page, 1, slot, 1] = math.nan
+    got = q3.attention_paged(*p.handles(), q)
+    assert torch.isnan(got[0, 2:, 64:]).all()
+    assert torch.equal(got[0, 2:, :64], clean[0, 2:, :64]) and torch.equal(got[0, :2], clean[0, :2])
+    assert torch.equal(got[1], clean[1])
+    p.ks[page, 0, slot, 0] = math.nan
+    got = q3.attention_paged(*p.handles(), q)
+    assert torch.isnan(got[0, :2]).all() and torch.equal(got[1], clean[1])
