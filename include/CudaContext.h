@@ -94,6 +94,11 @@ public:
     size_t attentionPagedWorkspace(int n_heads, int n_kv);
     void attentionPaged(const q3cu_kv_cache &cache, const q3cu_kv_batch &batch, const void *q, q3cu_dtype dt,
                         int64_t q_stride, int n_heads, void *work, size_t work_bytes, void *out, q3cu_stream stream);
+    // where groups of sequences share their first positions (q3cu_attention_shared)
+    size_t attentionSharedWorkspace(int n_seqs, int n_heads, int n_kv);
+    void attentionShared(const q3cu_kv_cache &cache, const q3cu_kv_batch &batch, const q3cu_kv_prefix &prefix, const void *q,
+                         q3cu_dtype dt, int64_t q_stride, int n_heads, void *work, size_t work_bytes, void *out,
+                         q3cu_stream stream);
     void attentionPrompt(const q3cu_kv_cache &cache, const q3cu_kv_batch &batch, int64_t rows, const void *q,
                          q3cu_dtype dt, int64_t q_stride, int n_heads, void *out, q3cu_stream stream);
     // synchronises `stream` and throws if a kernel flagged a device-side error

@@ -132,6 +132,17 @@ void CudaContext::attentionPaged(const q3cu_kv_cache &cache, const q3cu_kv_batch
     check(q3cu_attention_paged(ctx_, &cache, &batch, q, dt, q_stride, n_heads, work, work_bytes, out, stream),
           "attentionPaged");
 }
+size_t CudaContext::attentionSharedWorkspace(int n_seqs, int n_heads, int n_kv) {
+    size_t bytes = 0;
+    check(q3cu_attention_shared_workspace(ctx_, n_seqs, n_heads, n_kv, &bytes), "attentionSharedWorkspace");
+    return bytes;
+}
+void CudaContext::attentionShared(const q3cu_kv_cache &cache, const q3cu_kv_batch &batch, const q3cu_kv_prefix &prefix,
+                                  const void *q, q3cu_dtype dt, int64_t q_stride, int n_heads, void *work,
+                                  size_t work_bytes, void *out, q3cu_stream stream) {
+    check(q3cu_attention_shared(ctx_, &cache, &batch, &prefix, q, dt, q_stride, n_heads, work, work_bytes, out, stream),
+          "attentionShared");
+}
 void CudaContext::attentionPrompt(const q3cu_kv_cache &cache, const q3cu_kv_batch &batch, int64_t rows, const void *q,
                                   q3cu_dtype dt, int64_t q_stride, int n_heads, void *out, q3cu_stream stream) {
     check(q3cu_attention_prompt(ctx_, &cache, &batch, rows, q, dt, q_stride, n_heads, out, stream), "attentionPrompt");

@@ -1,0 +1,37 @@
+// k_prompt_q8.cu -- causal attention of packed prompt rows over a Q8_0 paged cache: the kernel of k_prompt.cu (its header
+// has the mathematics, the work items and the warps) with four more warps, which make the operands.
+//
+// TMA brings a key or value tile's codes and scales, 17 KB, to one of three stages; warps 12-15 turn each into the 32 KB
+// bf16 tile that the tensor cores read, code times scale rounded once, zeros behind the sequence's end (so no warp clears
+// values here).  Three such tiles are in flight where a bf16 cache has five; the codes ahead of them make up for it.  The
+// rounding (2^-8 of an element at most) is the price of one product for a score: exact codes would need one for each of a head's
+// two scales, twice the accumulators, for which tensor memory has no room beside two row tiles.
+//
+// Bound as k_prompt.cu is, and by the conversion's 2.75 instructions an element, which take a fifth of the issue slots of
+// a step.
+#include "q3cu_prompt.cuh"
+
+namespace q3 {
+
+cudaError_t launch_prompt_q8(const PagedKV &c, const PagedSeqs &b, int64_t rows, const void *q, int64_t q_stride, int n_heads,
+                             void *out, uint32_t *status, cudaStream_t stream) {
+    const int group = n_heads / c.n_kv, qt = PT_ROWS / group;
+    CUtensorMap mq, mk, mv, mks, mvs;
+    if (!encode_prompt_q_map(&mq, q, n_heads, rows, q_stride, group) || !encode_pages_map(&mk, c.k, c, Q3CU_Q8_0, PT_KEYS) ||
+        !encode_pages_map(&mv, c.v, c, Q3CU_Q8_0, PT_KEYS) || !encode_scales_map(&mks, c.k_scale, c, PT_KEYS) ||
+        !encode_scales_map(&mvs, c.v_scale, c, PT_KEYS))
+        return cudaErrorInvalidValue;
+    typedef PromptShape<true> Shape;
+    const int64_t items = (rows / (2 * qt) + b.n_seqs) * c.n_kv;             // as in k_prompt.cu
+    auto *whole = prompt_tc_kernel<PT_ITEMS, true>, *cluster = prompt_tc_kernel<PT_CLUSTER, true>;
+    cudaError_t e = ensure_smem_attr(reinterpret_cast<const void *>(cluster), Shape::SMEM, 56);
+    if (e == cudaSuccess) e = ensure_smem_attr(reinterpret_cast<const void *>(whole), Shape::SMEM, 57);
+    if (e != cudaSuccess) return e;
+    const int ctas = prompt_cluster(reinterpret_cast<const void *>(cluster), 2, Shape::THREADS, Shape::SMEM, items,
+                                    (int64_t(b.max_pages) << c.page_shift) / PT_KEYS);
+    return launch_clusters(ctas > 1 ? cluster : whole, ctas, dim3(unsigned(items * ctas)), dim3(Shape::THREADS), Shape::SMEM,
+                           stream, mq, mk, mv, mks, mvs, SharedOut{}, c, b, int(rows), static_cast<const uint16_t *>(q),
+                           q_stride, n_heads, group, FastDiv(2 * qt), FastDiv(group), ctas, static_cast<uint16_t *>(out), status);
+}
+
+}  // namespace q3

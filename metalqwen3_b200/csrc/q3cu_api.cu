@@ -728,8 +728,9 @@ q3cu_status q3cu_attention_prompt(q3cu_ctx *ctx, const q3cu_kv_cache *cache, con
     q3::PagedSeqs b;
     if (q3cu_status st = check_paged("attention_prompt", cache, batch, n_heads, true, c, b)) return st;
     if (q3cu_status st = check_dtype(dtype)) return st;
-    if (cache->dtype == Q3CU_Q8_0) return fail(Q3CU_ERR_INVALID, "attention_prompt: not over a Q8_0 cache");
-    if (cache->dtype != dtype) return fail(Q3CU_ERR_INVALID, "attention_prompt: q and the cache differ in type");
+    if (cache->dtype == Q3CU_Q8_0 && dtype != Q3CU_BF16)
+        return fail(Q3CU_ERR_INVALID, "attention_prompt: q must be bf16 over a Q8_0 cache");
+    if (cache->dtype != Q3CU_Q8_0 && cache->dtype != dtype) return fail(Q3CU_ERR_INVALID, "attention_prompt: q and the cache differ in type");
     if (n_heads == 0) return fail(Q3CU_ERR_INVALID, "attention_prompt: n_heads is 0");
     if (rows < 0 || rows + b.n_seqs > INT32_MAX / n_heads)
         return fail(Q3CU_ERR_INVALID, "attention_prompt: rows %lld, n_seqs %d", (long long)rows, b.n_seqs);
@@ -738,9 +739,49 @@ q3cu_status q3cu_attention_prompt(q3cu_ctx *ctx, const q3cu_kv_cache *cache, con
     if (q3cu_status st = check_rows("attention_prompt", "out", out, dtype, int64_t(n_heads) * q3::PAGED_HD, n_heads)) return st;
     if (out == q) return fail(Q3CU_ERR_INVALID, "attention_prompt: out must be other memory than q");
     if (q3cu_status st = use_device(ctx)) return st;
-    return launched(q3::launch_attention_prompt(c, b, rows, q, dtype, q_stride, n_heads, out, ctx->d_status,
+    return launched(q3::launch_attention_prompt(c, q3cu_dtype(cache->dtype), b, rows, q, dtype, q_stride, n_heads, out, ctx->d_status,
                                                 static_cast<cudaStream_t>(stream), ctx->sms),
                     "attention_prompt launch");
+}
+
+q3cu_status q3cu_attention_shared_workspace(q3cu_ctx *ctx, int n_seqs, int n_heads, int n_kv, size_t *bytes) {
+    CHECK_CTX(ctx);
+    if (!bytes || n_kv <= 0 || n_heads <= 0 || n_heads % n_kv || n_heads / n_kv > q3::PAGED_GROUP_MAX || n_seqs < 0 ||
+        n_seqs > (1 << 24))
+        return fail(Q3CU_ERR_INVALID, "attention_shared_workspace: n_seqs %d, n_heads %d, n_kv %d", n_seqs, n_heads, n_kv);
+    *bytes = q3::attention_shared_workspace(n_seqs, n_heads, n_kv, ctx->sms);
+    return Q3CU_OK;
+}
+
+q3cu_status q3cu_attention_shared(q3cu_ctx *ctx, const q3cu_kv_cache *cache, const q3cu_kv_batch *batch,
+                                  const q3cu_kv_prefix *prefix, const void *q, q3cu_dtype dtype, int64_t q_stride,
+                                  int n_heads, void *work, size_t work_bytes, void *out, q3cu_stream stream) {
+    CHECK_CTX(ctx);
+    q3::PagedKV c;
+    q3::PagedSeqs b;
+    if (q3cu_status st = check_paged("attention_shared", cache, batch, n_heads, false, c, b)) return st;
+    if (dtype != Q3CU_BF16 || cache->dtype == Q3CU_F32)
+        return fail(Q3CU_ERR_INVALID, "attention_shared: q must be bf16, the cache bf16 or Q8_0");
+    if (!prefix || prefix->n_groups < 0 || prefix->n_groups > (1 << 24) ||
+        (prefix->n_groups > 0 && (!prefix->seq_off || !prefix->len)))
+        return fail(Q3CU_ERR_INVALID, "attention_shared: prefix or one of its arrays is NULL, or n_groups out of range");
+    if (!aligned(prefix->seq_off, 4) || !aligned(prefix->len, 4))
+        return fail(Q3CU_ERR_ALIGN, "attention_shared: prefix arrays must be 4-byte aligned");
+    if (n_heads == 0) return fail(Q3CU_ERR_INVALID, "attention_shared: n_heads is 0");
+    if (b.n_seqs > INT32_MAX / n_heads) return fail(Q3CU_ERR_INVALID, "attention_shared: n_seqs %d", b.n_seqs);
+    if (b.n_seqs == 0) return Q3CU_OK;
+    if (q3cu_status st = check_rows("attention_shared", "q", q, dtype, q_stride, n_heads)) return st;
+    if (q3cu_status st = check_rows("attention_shared", "out", out, dtype, int64_t(n_heads) * q3::PAGED_HD, n_heads)) return st;
+    if (out == q) return fail(Q3CU_ERR_INVALID, "attention_shared: out must be other memory than q");
+    const size_t need = q3::attention_shared_workspace(b.n_seqs, n_heads, c.n_kv, ctx->sms);
+    if (!work || work_bytes < need)
+        return fail(Q3CU_ERR_INVALID, "attention_shared: work of %zu bytes, need %zu", work ? work_bytes : size_t(0), need);
+    if (!aligned(work, 32)) return fail(Q3CU_ERR_ALIGN, "attention_shared: work must be 32-byte aligned");
+    if (q3cu_status st = use_device(ctx)) return st;
+    return launched(q3::launch_attention_shared(c, q3cu_dtype(cache->dtype), b, prefix->seq_off, prefix->len,
+                                                prefix->n_groups, q, q_stride, n_heads, work, out, ctx->d_status,
+                                                static_cast<cudaStream_t>(stream), ctx->sms),
+                    "attention_shared launch");
 }
 
 // ---------------------------------------------------------------------------

@@ -252,6 +252,11 @@ __device__ __forceinline__ U8 ld_v8(const void *p) {
                    "=r"(v.w[6]), "=r"(v.w[7]) : "l"(p) : "memory");
     return v;
 }
+__device__ __forceinline__ void st_v8(void *p, const U8 &v) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                 :: "l"(p), "r"(v.w[0]), "r"(v.w[1]), "r"(v.w[2]), "r"(v.w[3]), "r"(v.w[4]), "r"(v.w[5]),
+                    "r"(v.w[6]), "r"(v.w[7]) : "memory");
+}
 __device__ __forceinline__ void st_cs_v8(void *p, const U8 &v) {
     asm volatile("st.global.cs.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
                  :: "l"(p), "r"(v.w[0]), "r"(v.w[1]), "r"(v.w[2]), "r"(v.w[3]), "r"(v.w[4]), "r"(v.w[5]),

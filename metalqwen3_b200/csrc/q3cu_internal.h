@@ -197,13 +197,22 @@ cudaError_t launch_attention_paged(const PagedKV &c, q3cu_dtype cache_dt, const 
 cudaError_t launch_paged_q8(const PagedKV &c, const PagedSeqs &b, const void *q, q3cu_dtype dt, int64_t q_stride,
                             int n_heads, void *work, void *out, uint32_t *status, cudaStream_t stream, int sms);
 // Packed query rows, causal: a row at position p over the keys 0..p.
-cudaError_t launch_attention_prompt(const PagedKV &c, const PagedSeqs &b, int64_t rows, const void *q, q3cu_dtype dt,
-                                    int64_t q_stride, int n_heads, void *out, uint32_t *status, cudaStream_t stream,
-                                    int sms);
+cudaError_t launch_attention_prompt(const PagedKV &c, q3cu_dtype cache_dt, const PagedSeqs &b, int64_t rows, const void *q,
+                                    q3cu_dtype dt, int64_t q_stride, int n_heads, void *out, uint32_t *status,
+                                    cudaStream_t stream, int sms);
+// bf16 rows over a Q8_0 cache (k_prompt_q8.cu).
+cudaError_t launch_prompt_q8(const PagedKV &c, const PagedSeqs &b, int64_t rows, const void *q, int64_t q_stride, int n_heads,
+                             void *out, uint32_t *status, cudaStream_t stream);
+// One bf16 query row per sequence over a bf16 or Q8_0 cache, where sequences off[g] .. off[g+1] - 1 share their first len[g]
+// positions (k_shared.cu).
+size_t attention_shared_workspace(int n_seqs, int n_heads, int n_kv, int sms);
+cudaError_t launch_attention_shared(const PagedKV &c, q3cu_dtype cache_dt, const PagedSeqs &b, const int32_t *off,
+                                    const int32_t *len, int n_groups, const void *q, int64_t q_stride, int n_heads,
+                                    void *work, void *out, uint32_t *status, cudaStream_t stream, int sms);
 cudaError_t launch_prompt_f32(const PagedKV &c, const PagedSeqs &b, int64_t rows, const void *q, int64_t q_stride,
                               int n_heads, void *out, uint32_t *status, cudaStream_t stream);
 // CTAs (1 to 8) that share an item of a prompt launch of at most `items` items, each with no more than `tiles` key tiles;
-// `kernel` (of `slot` 0 or 1) is the one for shared items, its shared memory allowed.
+// `kernel` (of `slot` 0 to 2) is the one for shared items, its shared memory allowed.
 int prompt_cluster(const void *kernel, int slot, int threads, size_t smem, int64_t items, int64_t tiles);
 
 cudaError_t launch_swiglu(const void *hb, const void *hb2, q3cu_dtype dt, int64_t elems, void *out, int8_t *q,

@@ -19,6 +19,12 @@ template <> struct Elem<bf16raw> {
     static constexpr int BYTES = 2;
 };
 
+struct q8raw {};                                             // Q8_0: codes here, their scales beside them
+template <> struct Elem<q8raw> {
+    typedef uint8_t type;
+    static constexpr int BYTES = 1;
+};
+
 // (Host and device: the index arithmetic is also checked on the CPU.)
 __host__ __device__ __forceinline__ void flag_bad_index(uint32_t *status) {
     if (!status) return;
@@ -58,6 +64,12 @@ __host__ __device__ __forceinline__ int paged_page(const PagedSeqs &b, const Pag
 __host__ __device__ __forceinline__ int64_t paged_at(const PagedKV &c, int page, int head, int t) {
     const int slot = t & ((1 << c.page_shift) - 1);
     return int64_t(page) * c.page_stride + ((int64_t(head) << c.page_shift) + slot) * HD;
+}
+
+// Index of (page, kv head, slot)'s first scale (Q8_0).
+__host__ __device__ __forceinline__ int64_t paged_scale_at(const PagedKV &c, int page, int head, int t) {
+    const int slot = t & ((1 << c.page_shift) - 1);
+    return int64_t(page) * c.scale_stride + ((int64_t(head) << c.page_shift) + slot) * 2;
 }
 
 // The sequence of packed row r: the last s with row_off[s] <= r, or -1 when r
@@ -139,6 +151,20 @@ __device__ __forceinline__ float4 q8_floats(uint32_t codes) {
     return make_float4(one(0x7440), one(0x7441), one(0x7442), one(0x7443));
 }
 
+// Four elements of a key or value: `at` in the cache, of the row whose scales begin at index `scale` (Q8_0; lane as in
+// attend_row).
+template <typename TC>
+__device__ __forceinline__ float4 cached_quad(const PagedKV &c, bool value, int64_t at, int64_t scale) {
+    const typename Elem<TC>::type *p = static_cast<const typename Elem<TC>::type *>(value ? c.v : c.k) + at;
+    if constexpr (Elem<TC>::BYTES == 1) {
+        const float4 x = q8_floats(*reinterpret_cast<const uint32_t *>(p));
+        const float s = (value ? c.v_scale : c.k_scale)[scale + ((threadIdx.x & 31) >> 4)];
+        return make_float4(s * x.x, s * x.y, s * x.z, s * x.w);
+    } else {
+        return load_quad(p);
+    }
+}
+
 // Whether none of them is infinite or NaN.
 __device__ __forceinline__ bool all_finite(float4 v) {
     return fmaf(v.x, 0.0f, fmaf(v.y, 0.0f, fmaf(v.z, 0.0f, v.w * 0.0f))) == 0.0f;
@@ -153,21 +179,20 @@ __device__ __forceinline__ bool all_finite(float4 v) {
 template <typename TC, int STEP>
 __device__ __forceinline__ float4 attend_row(const PagedKV &c, const PagedSeqs &b, int s, int head, int n, float4 q,
                                              uint32_t *status) {
-    const typename Elem<TC>::type *kp = static_cast<const typename Elem<TC>::type *>(c.k);
-    const typename Elem<TC>::type *vp = static_cast<const typename Elem<TC>::type *>(c.v);
     const int lane = threadIdx.x & 31;
     float m = -INFINITY, sum = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (int t = 0; t < n; t += STEP) {
         const int page = paged_page(b, c, s, t, lane == 0 ? status : nullptr);
         const int64_t at = page >= 0 ? paged_at(c, page, head, t) + 4 * lane : 0;
+        const int64_t scale = Elem<TC>::BYTES == 1 && page >= 0 ? paged_scale_at(c, page, head, t) : 0;
         float4 k[STEP], v[STEP];
 #pragma unroll
         for (int u = 0; u < STEP; ++u) {
             k[u] = v[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             if (page >= 0 && t + u < n) {
-                k[u] = load_quad(kp + at + u * HD);
-                v[u] = load_quad(vp + at + u * HD);
+                k[u] = cached_quad<TC>(c, false, at + u * HD, scale + 2 * u);
+                v[u] = cached_quad<TC>(c, true, at + u * HD, scale + 2 * u);
             }
         }
         float d[STEP], nm = m;
@@ -264,6 +289,36 @@ template <typename TC> struct SecondLook {
             else top = max(top, max(no_nan(x[i] << 16), no_nan(x[i] & 0xffff0000u)));
         }
         return top;
+    }
+};
+// Over a Q8_0 cache only a scale can be no finite number, or large.
+template <> struct SecondLook<q8raw> {
+    int tile = -1, last;
+    bool huge;
+    __device__ __forceinline__ void look(int id, const PagedKV &c, const PagedSeqs &b, int s, int head, int lo, int hi) {
+        if (tile == id) return;
+        tile = id;
+        last = -1;
+        huge = false;
+        const int lane = threadIdx.x & 31;
+        // 16 positions, which one page holds: a lane looks at one scale of K and of V
+        for (int t = 0; t < hi; t += 16) {
+            const int page = paged_page(b, c, s, t, nullptr), at = t + (lane >> 1);
+            if (page < 0) continue;
+            float k = 0.0f, v = 0.0f;
+            if (at < hi) {
+                const int64_t i = paged_scale_at(c, page, head, t) + lane;
+                k = fabsf(c.k_scale[i]);
+                v = fabsf(c.v_scale[i]);
+            }
+            huge |= __any_sync(FULL, k >= 0x1p93f || v >= 0x1p93f);          // times 127: 2^100
+            const unsigned odd = __ballot_sync(FULL, at >= lo && !(v < INFINITY));
+            if (odd) last = t + ((31 - __clz(odd)) >> 1);
+        }
+    }
+    __device__ __forceinline__ bool wanted(int limit, float4 q) const {
+        const float top = fmaxf(fmaxf(fabsf(q.x), fabsf(q.y)), fmaxf(fabsf(q.z), fabsf(q.w)));
+        return huge || limit <= last || __any_sync(FULL, top >= 0x1p100f);
     }
 };
 

@@ -78,7 +78,8 @@ struct TailSeqs : PagedSeqs {
     PagedGroups groups;
     __device__ __forceinline__ PagedSpan span(const PagedKV &c, int s, uint32_t *status) const {
         const int g = groups.of(s, n_seqs), from = g < 0 ? 0 : groups.shared(g, *this, c, nullptr);
-        return {from, paged_len(*this, c, s, status)};
+        const int len = paged_len(*this, c, s, status);
+        return {len < from ? 0 : from, len};                 // one that holds fewer attends by itself
     }
 };
 

@@ -51,6 +51,10 @@ class _KVBatch(C.Structure):             # q3cu_kv_batch
                 ("max_pages", C.c_int32)]
 
 
+class _KVPrefix(C.Structure):            # q3cu_kv_prefix
+    _fields_ = [("seq_off", C.c_void_p), ("len", C.c_void_p), ("n_groups", C.c_int32)]
+
+
 def header_functions(path: str = HEADER) -> list[str]:
     """Names of the entry points declared in include/q3cu.h."""
     text = open(path).read()
@@ -96,6 +100,9 @@ def load_library(path: str = LIB_PATH) -> C.CDLL:
                 "q3cu_attention_paged": (st, [vp, C.POINTER(_KVCache), C.POINTER(_KVBatch), vp, i32, i64, i32, vp,
                                               C.c_size_t, vp, vp]),
                 "q3cu_attention_paged_workspace": (st, [vp, i32, i32, C.POINTER(C.c_size_t)]),
+                "q3cu_attention_shared": (st, [vp, C.POINTER(_KVCache), C.POINTER(_KVBatch), C.POINTER(_KVPrefix), vp, i32,
+                                               i64, i32, vp, C.c_size_t, vp, vp]),
+                "q3cu_attention_shared_workspace": (st, [vp, i32, i32, i32, C.POINTER(C.c_size_t)]),
                 "q3cu_attention_prompt": (st, [vp, C.POINTER(_KVCache), C.POINTER(_KVBatch), i64, vp, i32, i64, i32,
                                                vp, vp]),
                 "q3cu_execute_attention": (st, [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, C.c_uint64,
@@ -243,6 +250,22 @@ class KVBatch:
         self.kv_len, self.pages, self.row_off = kv_len, pages, row_off
         self.c = _KVBatch(None if row_off is None else row_off.data_ptr(), kv_len.data_ptr(), pages.data_ptr(), n,
                           pages.shape[1])
+        self.ref = C.byref(self.c)
+
+
+class KVPrefix:
+    """Groups of sequences that begin alike: seq_off [n_groups + 1] and length [n_groups], int32 on the GPU (the meaning
+    of each: q3cu_kv_prefix in include/q3cu.h)."""
+
+    def __init__(self, seq_off, length):
+        n = length.numel()
+        i32 = length.new_empty(0).int().dtype
+        self.device = length.get_device()
+        for t, what, shape in ((seq_off, "seq_off", (n + 1,)), (length, "length", (n,))):
+            if not _tensor(t, what, i32, shape, self.device).is_contiguous():
+                raise ValueError(f"{what} must be contiguous")
+        self.seq_off, self.length = seq_off, length
+        self.c = _KVPrefix(seq_off.data_ptr(), length.data_ptr(), n)
         self.ref = C.byref(self.c)
 
 
@@ -416,10 +439,10 @@ class Q3CU:
         return xb, probs
 
     # -- the paged key-value cache -----------------------------------------------
-    def _elsewhere(self, cache, batch, work=None):
+    def _elsewhere(self, cache, batch, work=None, prefix=None):
         """Refuses what lies on another device than the context's, which its kernels could not reach."""
-        for what, t in (("cache", cache), ("batch", batch)):
-            if t.device != self.device:
+        for what, t in (("cache", cache), ("batch", batch), ("prefix", prefix)):
+            if t is not None and t.device != self.device:
                 raise ValueError(f"the {what} must be on the context's GPU, it is on cuda:{t.device}")
         raise ValueError(f"work must be contiguous memory on the context's GPU, it is on {work.device}")
 
@@ -509,9 +532,37 @@ class Q3CU:
             self._check(status, "q3cu_attention_paged")
         return out
 
+    def attention_shared_workspace(self, cache, n_seqs, n_heads, stream=None):
+        """A workspace for attention_shared with these head counts and at most n_seqs sequences; calls that may run at
+        the same time need one each.  `stream`: where it is used, if not on the current one."""
+        n = C.c_size_t(0)
+        self._check(self.lib.q3cu_attention_shared_workspace(self.ctx, n_seqs, n_heads, cache.n_kv, C.byref(n)),
+                    "q3cu_attention_shared_workspace")
+        return self._make(stream, self.torch.empty, n.value, dtype=self.torch.uint8, device=cache.k.device)
+
+    def attention_shared(self, cache, batch, prefix, q, out=None, work=None, stream=None):
+        """attention_paged where groups of sequences share their first positions (a KVPrefix), which are attended to once
+        for the whole group; q and out bf16, the cache bf16 or Q8_0."""
+        if cache.device != self.device or batch.device != self.device or prefix.device != self.device or (
+                work is not None and (work.get_device() != self.device or not work.is_contiguous())):
+            self._elsewhere(cache, batch, work, prefix)
+        stride, rows, heads, qp = _rows(q, "q", None, None, batch.c.n_seqs, self.device)
+        if out is None:
+            out = self._make(stream, self.torch.empty, (rows, heads, 128), dtype=q.dtype, device=q.device)
+        elif not out.is_contiguous():
+            raise ValueError("out must be contiguous")
+        op = _rows(out, "out", q.dtype, heads, rows, self.device)[3]
+        if work is None:
+            work = self.attention_shared_workspace(cache, rows, heads, stream)
+        status = self.lib.q3cu_attention_shared(self.ctx, cache.ref, batch.ref, prefix.ref, qp, _dtype(q), stride, heads,
+                                                work.data_ptr(), work.nbytes, op, self._stream(stream))
+        if status:
+            self._check(status, "q3cu_attention_shared")
+        return out
+
     def attention_prompt(self, cache, batch, q, out=None, stream=None):
-        """Causal attention of the packed rows q [rows][n_heads][128] over the cache, which holds their
-        keys and values; rows behind the last sequence are not written."""
+        """Causal attention of the packed rows q [rows][n_heads][128] (the cache's type, bf16 over a Q8_0 cache) over the
+        cache, which holds their keys and values; rows behind the last sequence are not written."""
         if cache.device != self.device or batch.device != self.device:
             self._elsewhere(cache, batch)
         stride, rows, heads, qp = _rows(q, "q", None, None, None, self.device)

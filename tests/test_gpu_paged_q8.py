@@ -6,25 +6,26 @@ one rounding each.  An f16 part is no finer than 2^-25, half its least number, a
 largest value scale of 32 positions) is lifted to 2^14 or more, so that an element is also off by up to 2^-39 of the row's
 largest: a score by 128 * 2^-39 max|q| max|k| / sqrt(128), a result of n positions by n 2^-39 (128 / 127) max|v|.
 Where the result is bf16 a weight is one f16 part: 2^-11 relative each.  Prompts round every element
-of the cache to bf16 as well (2^-8 relative): a score moves by at most 2^-8 A, a value by 2^-8 of itself.
+of the cache to bf16 on its way to the products: their formula is taken over the rounded elements.
 """
 import math
 
+import numpy as np
 import pytest
 import torch
 
 from test_gpu_kv_forms import I8, Quantised
-from test_gpu_paged import BF16, DECODE, F32, H, U, attend, offsets, queries
+from test_gpu_paged import BF16, DECODE, F32, H, PROMPT, U, attend, offsets, queries
 
 pytestmark = pytest.mark.gpu
 W = 2.0 ** -11
 
 
-def check_attention(got, q, k, v, seen, dtype, weight_rounding=0.0, element_rounding=0.0):
+def check_attention(got, q, k, v, seen, dtype, weight_rounding=0.0):
     o, pv, a = attend(q.double(), k, v, seen)
     n, top = max(1, k.shape[0]), lambda x: float(x.abs().max()) if x.numel() else 0.0
-    ds = (160 * U + element_rounding) * a + math.sqrt(128) * 2.0 ** -39 * top(q) * top(k)
-    tol = (torch.expm1(2 * ds) + (n + 64) * U + weight_rounding + element_rounding) * pv + n * 2.0 ** -39 * 1.01 * top(v)
+    ds = 160 * U * a + math.sqrt(128) * 2.0 ** -39 * top(q) * top(k)
+    tol = (torch.expm1(2 * ds) + (n + 64) * U + weight_rounding) * pv + n * 2.0 ** -39 * 1.01 * top(v)
     if dtype == BF16:
         tol = tol + H * (o.abs() + tol)
     bad = ~((got.double() - o).abs() <= tol + 1e-30)
@@ -150,3 +151,90 @@ def test_unused_scales_and_nan(q3):
     p.ks[page, 0, slot, 0] = math.nan
     got = q3.attention_paged(*p.handles(), q)
     assert torch.isnan(got[0, :2]).all() and torch.equal(got[1], clean[1])
+
+
+# ---- prompts -----------------------------------------------------------------------------------
+
+def rounded(p, s):
+    """Keys and values of sequence s as the prompts' products take them."""
+    page, slot = p.where(s, range(max(p.lens[s], 0)))
+    return tuple((t[page, :, slot].float() * c[page, :, slot].repeat_interleave(64, -1)).to(BF16).double()
+                 for t, c in ((p.k, p.ks), (p.v, p.vs)))
+
+
+@pytest.mark.parametrize("heads,n_kv,page,rows,lens", PROMPT + [(32, 8, 64, [3], [7000]), (8, 1, 16, [100, 20], [2500, 3000])])
+def test_attention_prompt(q3, heads, n_kv, page, rows, lens):
+    """Whole prompts, chunks behind a prefix (few rows behind a long one share an item), rows that see nothing, rows behind
+    the last sequence."""
+    p = Quantised(lens, n_kv, page, seed=31).fill(32)
+    total = sum(rows)
+    q = queries(total + 3, heads, BF16, 33)
+    out = torch.full((total + 3, heads, 128), 7.0, dtype=BF16, device="cuda")
+    assert q3.attention_prompt(*p.handles(offsets(rows)), q, out=out) is out
+    assert (out[total:] == 7.0).all()
+    first = 0
+    for s, (r, n) in enumerate(zip(rows, lens)):
+        if r:
+            check_attention(out[first:first + r], q[first:first + r], *rounded(p, s), [max(0, n - r + 1 + i) for i in range(r)],
+                            BF16, H)
+        first += r
+    assert q3.device_status() == 0
+
+
+@pytest.mark.parametrize("n_seqs", [33, 100])
+def test_attention_prompt_many_sequences(q3, n_seqs):
+    g = np.random.default_rng(n_seqs)
+    rows = [int(r) if r < 40 or i % 9 == 0 else int(r) % 40 for i, r in enumerate(g.integers(0, 300, n_seqs))]
+    lens = [r + int(x) for r, x in zip(rows, g.integers(0, 400, n_seqs) * g.integers(0, 2, n_seqs))]
+    p = Quantised(lens, 2, 16, seed=47).fill(48)
+    off = offsets(rows)
+    q = queries(off[-1], 4, BF16, 49)
+    out = q3.attention_prompt(*p.handles(off), q)
+    for s in range(n_seqs):
+        if rows[s]:
+            mine = slice(off[s], off[s + 1])
+            check_attention(out[mine], q[mine], *rounded(p, s), range(lens[s] - rows[s] + 1, lens[s] + 1), BF16, H)
+    assert q3.device_status() == 0
+
+
+def test_attention_prompt_long(q3):
+    """Many items to a CTA, and many key tiles to an item; strides, bad pages."""
+    from metalqwen3_b200.q3cu import DEV_BAD_INDEX
+    n = 2500
+    p = Quantised([n], 4, 16, seed=40, gap=4096 + 32).fill(41)
+    k, v = rounded(p, 0)
+    for i, bad in ((2, -1), (9, 1 << 30)):
+        p.table[0, i] = bad
+        k[16 * i:16 * i + 16] = 0
+        v[16 * i:16 * i + 16] = 0
+    q = queries(n, 48, BF16, 42)[:, 8:40]
+    got = q3.attention_prompt(*p.handles([0, n]), q)
+    assert q3.device_status() == DEV_BAD_INDEX and q3.device_status() == 0
+    some = list(range(0, n, 97)) + [n - 1]
+    check_attention(got[some], q[some], k, v, [i + 1 for i in some], BF16, H)
+
+
+def test_attention_prompt_hides_later_rows(q3):
+    """NaN and infinite scales at later positions reach no earlier row; what a row sees of them it shows."""
+    n = 150
+    for rows in (n, 3):                         # a prompt, and its last rows alone
+        p = Quantised([n], 2, 16, seed=34).fill(35)
+        page, slot = p.where(0, range(n))
+        for at, what in ((147, math.nan), (148, math.inf)):
+            p.vs[page[at], :, slot[at], 1] = what
+            p.ks[page[at], 1, slot[at], 0] = what
+        q = queries(rows, 8, BF16, 36)
+        got = q3.attention_prompt(*p.handles([0, rows]), q)
+        k, v = (t[:147] for t in rounded(p, 0))
+        early = rows - 3
+        if early:
+            check_attention(got[:early], q[:early], k, v, range(1, early + 1), BF16, H)
+        assert torch.isnan(got[early:, :4, 64:]).all() and torch.isnan(got[early:, 4:]).all()
+        assert torch.isfinite(got[early, :4, :64]).all()
+
+
+def test_attention_prompt_peaked_and_flat(q3):
+    for scale in (40.0, 0.0):
+        p = Quantised([333], 2, 32, seed=37).fill(38, scale if scale else 1.0)
+        q = queries(333, 8, BF16, 39, scale)
+        check_attention(q3.attention_prompt(*p.handles([0, 333]), q), q, *rounded(p, 0), range(1, 334), BF16, H)
