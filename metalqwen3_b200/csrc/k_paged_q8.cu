@@ -30,6 +30,7 @@
 //
 // Positions at and beyond the length, and before a tail, score -inf and weigh
 // exactly 0: unused page space may hold anything, scales that are NaN included.
+#include "q3cu_f16.cuh"
 #include "q3cu_mma.cuh"
 #include "q3cu_paged.cuh"
 #include "q3cu_split.cuh"
@@ -49,40 +50,6 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
                                         uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-// Two bytes of `codes` (already with the top bits flipped: code + 128), by a selector that puts 0x64 above each, as f16.
-__device__ __forceinline__ uint32_t codes_f16(uint32_t codes, uint32_t pick) {
-    uint32_t r;
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(__byte_perm(codes, 0x64646464u, pick)), "r"(0x64806480u));  // - 1152
-    return r;
-}
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-__device__ __forceinline__ float2 f16_pair(uint32_t x) {
-    float2 v;
-    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.f32.f16 %0, l;\n\tcvt.f32.f16 %1, h;\n\t}" : "=f"(v.x), "=f"(v.y) : "r"(x));
-    return v;
-}
-// x and y as PARTS f16 each, every one the nearest to what the ones before leave.
-template <int PARTS>
-__device__ __forceinline__ void split_f16(float x, float y, uint32_t (&part)[PARTS]) {
-#pragma unroll
-    for (int i = 0; i < PARTS; ++i) {
-        part[i] = pack_f16(x, y);
-        if (i + 1 < PARTS) {
-            const float2 v = f16_pair(part[i]);
-            x -= v.x;
-            y -= v.y;
-        }
-    }
-}
-// The power of two that brings a magnitude (as binary32's bits) to [2^14, 2^15), no more than 2^126, and its inverse.
-__device__ __forceinline__ float lift(uint32_t bits) { return __uint_as_float(uint32_t(min(268 - int(bits >> 23), 253)) << 23); }
-__device__ __forceinline__ float lift_back(uint32_t bits) {
-    return __uint_as_float(uint32_t(254 - min(268 - int(bits >> 23), 253)) << 23);
 }
 __device__ __forceinline__ int pq_row(int g) { return ((g & 1) << 2) | ((g & 7) >> 1); }   // the position of row g of eight
 

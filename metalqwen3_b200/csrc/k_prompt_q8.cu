@@ -2,12 +2,23 @@
 // has the mathematics, the work items and the warps) with four more warps, which make the operands.
 //
 // TMA brings a key or value tile's codes and scales, 17 KB, to one of three stages; warps 12-15 turn each into the 32 KB
-// bf16 tile that the tensor cores read, code times scale rounded once, zeros behind the sequence's end (so no warp clears
-// values here).  Three such tiles are in flight where a bf16 cache has five; the codes ahead of them make up for it.  The
-// rounding (2^-8 of an element at most) is the price of one product for a score: exact codes would need one for each of a head's
-// two scales, twice the accumulators, for which tensor memory has no room beside two row tiles.
+// operand tile that the tensor cores read, zeros behind the sequence's end (so no warp clears values here).  Three such
+// tiles are in flight where a bf16 cache has five; the codes ahead of them make up for it.
 //
-// Bound as k_prompt.cu is, and by the conversion's 2.75 instructions an element, which take a fifth of the issue slots of
+// The operands are f16: a code times its scale has more than bf16's 8 bits, and rounding keys and values to bf16 doubled the
+// error of the result (0.0039 of it against 0.0017 now, which is the result's own rounding).  f16 has 11 bits but little
+// range, so everything is lifted by powers of two:
+//   keys, values  by tile: the largest scale to [2^14, 2^15), codes as code / 128.  An element is rounded by 2^-10 of itself
+//                 (its scale and the product, 2^-11 each) and by no less than 2^-39 of the tile's largest.
+//   queries       by row, by the same warps when an item begins; exact, but for 2^-39 of the row's largest.
+//   probabilities times 2^7, by 2^-11 of themselves and no less than 2^-32.
+// The inverse lifts of query and keys go into the factor that makes scores exponents.  O is kept times the smallest lift of
+// the value tiles so far: a tile of larger values takes O down with it (in binary32, on the path that rescales O for a larger
+// maximum), a tile of smaller ones has its probabilities lowered.  Where the scales of one tile differ by more than 2^24,
+// rows that see only a part of the tile are computed again from the formula, so that a later position takes no bits from
+// an earlier row (SecondLook).
+//
+// Bound as k_prompt.cu is, and by the conversion's 1.75 instructions an element, which take an eighth of the issue slots of
 // a step.
 #include "q3cu_prompt.cuh"
 

@@ -2,6 +2,7 @@
 // k_prompt_q8.cu (over Q8_0 caches) and k_shared.cu (what groups of sequences share).
 #pragma once
 
+#include "q3cu_f16.cuh"
 #include "q3cu_paged.cuh"
 #include "q3cu_split.cuh"
 #include "q3cu_tcgen05.cuh"
@@ -25,6 +26,8 @@ template <bool Q8> struct PromptShape {
 // Instruction descriptors: f32 accumulator, bf16 A and B, M = N = 128; B K-major (K) or MN-major (V).
 constexpr uint32_t PT_IDESC = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(128 / 8) << 17) | (uint32_t(128 / 16) << 24);
 constexpr uint32_t PT_IDESC_V = PT_IDESC | (1u << 16);
+constexpr uint32_t PT_F16 = (1u << 7) | (1u << 10);          // the bits that say bf16 where f16 has none
+constexpr int PT_BIAS = 7;                                   // Q8_0: probabilities are times 2^7 in f16, at most 2^15
 constexpr float PT_LOG2 = ATT_SCALE * 1.44269504088896341f;  // scores to base-2 exponents
 constexpr float PT_LAZY = 8.0f / PT_LOG2;                    // growth of the maximum (as a raw score) that rescales O
 
@@ -189,13 +192,38 @@ struct NoOrder {             // in place of a PromptOrder
     __device__ __forceinline__ PromptItem find(int64_t) { return {}; }
 };
 
-// ---- a Q8_0 tile as bf16 --------------------------------------------------------------------------
-// 128 rows' codes (128-byte swizzle) and scales at `raw` become the 32 KB operand tile at `to`, by four warps: a lane takes
-// 16 codes of eight rows.  Rows from `rows` on are zeros.  code + 128 in the low byte of 2^23 + it, less 2^23 + 128,
-// times the scale, rounded once: 2.75 instructions an element.
-__device__ __forceinline__ void q8_tile(const uint8_t *raw, uint8_t *to, int rows) {
+// ---- Q8_0 tiles and their queries as f16 ------------------------------------------------------------
+// What the rows of a converted tile were multiplied by: 2^(e - 7), and whether their scales differ by more than 2^24.
+struct TileLift {
+    int e;
+    bool uneven;
+};
+// 128 rows' codes (128-byte swizzle) and scales at `raw` become the 32 KB f16 operand tile at `to`, by four warps: a lane
+// takes 16 codes of eight rows.  Rows from `rows` on are zeros.  The scales are lifted by the power of two that brings the
+// largest finite one to [2^14, 2^15) and rounded to f16 (2^-11), code / 128 is exact, the product is rounded once more:
+// 1.75 instructions an element.
+__device__ __forceinline__ TileLift q8_tile(const uint8_t *raw, uint8_t *to, int rows) {
     const int lane = threadIdx.x & 31, key0 = int(threadIdx.x >> 5 & 3) * 32 + (lane & 7);
     const float *scales = reinterpret_cast<const float *>(raw + PT_KEYS * HD);
+    uint32_t top = 0, low = 0x7f7fffffu;                     // of the scales that count, as bits
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(scales + 8 * lane + 4 * x);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+            const uint32_t m = w[y] & 0x7fffffffu;
+            const bool counts = 4 * lane + 2 * x + y / 2 < rows && m < 0x7f800000u;
+            top = counts ? max(top, m) : top;
+            low = counts && m ? min(low, m) : low;
+        }
+    }
+    top = __reduce_max_sync(FULL, top);
+    low = __reduce_min_sync(FULL, low);
+    TileLift lifted;
+    lifted.e = min(141 - int(top >> 23), 126);
+    lifted.uneven = top && (top >> 23) - (low >> 23) > 24;
+    const float up = __uint_as_float(uint32_t(lifted.e + 127) << 23);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int key = key0 + 8 * i;
@@ -203,21 +231,16 @@ __device__ __forceinline__ void q8_tile(const uint8_t *raw, uint8_t *to, int row
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             const int ch = (lane >> 3) + 4 * half;           // codes 16 ch ..
-            const float s = key < rows ? half ? sc.y : sc.x : 0.0f;
-            const f2 s2 = pk2(s, s), off = pk2(-8388736.0f, -8388736.0f);
+            const float s = key < rows ? (half ? sc.y : sc.x) * up : 0.0f;
+            const uint32_t s2 = pack_f16(s, s);
             const uint4 v = *reinterpret_cast<const uint4 *>(raw + key * HD + ((ch ^ (key & 7)) << 4));
             const uint32_t words[4] = {v.x, v.y, v.z, v.w};
             uint32_t w[8];
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
                 const uint32_t u = words[y] ^ 0x80808080u;
-                auto one = [&](uint32_t pick) { return __uint_as_float(__byte_perm(u, 0x4b000000u, pick)); };
-#pragma unroll
-                for (int z = 0; z < 2; ++z) {
-                    float a, d;
-                    up2(mul2(add2(pk2(one(0x7440 + 2 * z), one(0x7441 + 2 * z)), off), s2), a, d);
-                    w[2 * y + z] = pack_bf16(a, d);
-                }
+                w[2 * y] = mul_f16(codes_f16_128th(u, 0x4140), s2);
+                w[2 * y + 1] = mul_f16(codes_f16_128th(u, 0x4342), s2);
             }
             uint8_t *row = to + half * PT_HALF + key * 128;  // 64 elements, chunks of 8
             const int c0 = 2 * (lane >> 3);
@@ -225,6 +248,28 @@ __device__ __forceinline__ void q8_tile(const uint8_t *raw, uint8_t *to, int row
             *reinterpret_cast<uint4 *>(row + (((c0 + 1) ^ (key & 7)) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
         }
     }
+    return lifted;
+}
+// The bf16 queries of a row tile become f16 in their places, each row lifted so that its largest element lies in
+// [2^14, 2^15); one thread a row.  Returns the inverse of the row's lift.
+__device__ __forceinline__ float q_tile_f16(uint8_t *tile, int row) {
+    uint8_t *at = tile + row * 128;
+    uint32_t top = 0;
+#pragma unroll 4
+    for (int x = 0; x < 16; ++x) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(at + (x >> 3) * PT_HALF + ((x & 7) << 4));
+        top = __vmaxu2(top, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
+    }
+    top = max(top & 0xffffu, top >> 16) << 16;
+    const float up = lift(top);
+#pragma unroll 4
+    for (int x = 0; x < 16; ++x) {
+        uint4 *p = reinterpret_cast<uint4 *>(at + (x >> 3) * PT_HALF + ((x & 7) << 4));
+        const uint4 v = *p;
+        auto two = [&](uint32_t w) { return pack_f16(bf16_to_f32(w & 0xffffu) * up, bf16_to_f32(w >> 16) * up); };
+        *p = make_uint4(two(v.x), two(v.y), two(v.z), two(v.w));
+    }
+    return lift_back(top);
 }
 
 // PT_ITEMS: a CTA takes items one after the other; PT_CLUSTER: clusters of `ctas` CTAs, each with one item; PT_SHARED: a run
@@ -245,7 +290,12 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(pt_dyn) + 1023) & ~uintptr_t(1023));
     uint8_t *ring = smem + 2 * PT_TILE, *raw = ring + PT_NS * PT_TILE;       // raw: Q8_0 codes and scales
     __shared__ __align__(8) uint64_t q_full, q_empty, full[PT_NS], empty[PT_NS], s_full[2], p_full[2][2], o_full[2],
-        o_empty[2], item_full[2], item_empty[2], taken, tail_go, tail, drain, raw_full[Q8 ? RAWS : 1], raw_empty[Q8 ? RAWS : 1];
+        o_empty[2], item_full[2], item_empty[2], taken, tail_go, tail, drain, raw_full[Q8 ? RAWS : 1], raw_empty[Q8 ? RAWS : 1],
+        q_ready;
+    // Q8_0: the inverse lifts of the queries' rows (by item), and of the tiles in turn: keys' inverse, values' exponent
+    __shared__ float q_back[Q8 ? 2 : 1][Q8 ? 2 * PT_ROWS : 1], k_back[2];
+    __shared__ int v_lift[2];
+    __shared__ bool rough[2];                                // scales of keys or values are uneven
     __shared__ Round item_sh[2];
     __shared__ ulonglong2 taken_sh;
     __shared__ uint32_t tmem_sh;
@@ -254,6 +304,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
     if (threadIdx.x == 0) {
         mbar_init(&q_full, 1);
         mbar_init(&q_empty, 1);
+        mbar_init(&q_ready, 4);
         for (int i = 0; i < PT_NS; ++i) {
             mbar_init(&full[i], Q8 ? 4 : 1);                 // Q8_0: the warps that convert
             mbar_init(&empty[i], 1);
@@ -287,6 +338,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
 
     const int qt = PT_ROWS / group;                          // queries of a tile
     float2 stat = make_float2(-INFINITY, -1.0f);             // SPLIT: maximum and sum of this thread's row, -1: given up
+    [[maybe_unused]] float part_back = 1.0f;                 // and what its O is to be multiplied by (Q8_0)
     // the item of a round, copied from its announcement; false after the last, or if a wait gave up
     auto next_item = [&](int round, Round &it, bool whole_warp) -> bool {
         bool ok = mbar_wait(&item_full[round & 1], uint32_t(round >> 1) & 1u, !whole_warp || lane == 0 ? status : nullptr);
@@ -459,7 +511,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                     for (int k = 0; k < 8; ++k) {
                         const uint32_t off = (uint32_t(k / 4) * PT_HALF + uint32_t(k % 4) * 32) >> 4;
                         tc_mma_bf16_ss(tbase + t * 128, dq + t * (PT_TILE >> 4) + off, dk + buf * (PT_TILE >> 4) + off,
-                                       PT_IDESC, uint32_t(k > 0));
+                                       Q8 ? PT_IDESC & ~PT_F16 : PT_IDESC, uint32_t(k > 0));
                     }
                     tc_commit(&s_full[t]);
                 };
@@ -467,7 +519,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
                         tc_mma_bf16_ts(tbase + 256 + t * 128, tbase + t * 128 + (4 * half + k) * 8,
-                                       dv + buf * (PT_TILE >> 4) + (4 * half + k) * (2048 >> 4), PT_IDESC_V,
+                                       dv + buf * (PT_TILE >> 4) + (4 * half + k) * (2048 >> 4), Q8 ? PT_IDESC_V & ~PT_F16 : PT_IDESC_V,
                                        k > 0 ? 1u : uint32_t(add));
                 };
                 RingAt at;
@@ -478,7 +530,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                 for (int round = 0; ok && next_item(round, it, false); ++round) {
                     const int nkv = max(it.nt[0], it.nt[1]);
                     if (nkv == 0) continue;
-                    if (!(ok = mbar_wait(&q_full, uint32_t(qs++) & 1u, status))) break;
+                    if (!(ok = mbar_wait(Q8 ? &q_ready : &q_full, uint32_t(qs++) & 1u, status))) break;
                     if (!(ok = mbar_wait(&full[at.st], at.ph, status))) break;
                     tc_fence_after();
                     if (it.nt[0]) scores(0, at.st);
@@ -536,16 +588,33 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
             Round it;
             ::q3::RingAt<Q8 ? RAWS : 1> from;
             RingAt to;
-            int entries = 0;
+            int entries = 0, qs = 0;
             bool ok = true;
             for (int round = 0; ok && next_item(round, it, true); ++round) {
                 const int nkv = max(it.nt[0], it.nt[1]);
+                if (nkv) {
+                    ok = __all_sync(FULL, mbar_wait(&q_full, uint32_t(qs) & 1u, lane == 0 ? status : nullptr));
+                    if (!ok) break;
+                    const int r = threadIdx.x & 127;
+                    for (int t = 0; t < 2; ++t)
+                        if (it.nt[t]) q_back[qs & 1][t * PT_ROWS + r] = q_tile_f16(smem + t * PT_TILE, r);
+                    ++qs;
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&q_ready);
+                }
+                bool odd = false;                            // K or V of this tile is uneven
                 for (int x = 0; x < 2 * nkv; ++x) {
                     ok = mbar_wait(&raw_full[from.st], from.ph, lane == 0 ? status : nullptr);
                     if (entries >= PT_NS) ok = ok && mbar_wait(&empty[to.st], to.ph ^ 1u, lane == 0 ? status : nullptr);
                     ok = __all_sync(FULL, ok);
                     if (!ok) break;
-                    q8_tile(raw + from.st * PT_RAW, ring + to.st * PT_TILE, it.len - (it.from() + x / 2) * PT_KEYS);
+                    const TileLift l = q8_tile(raw + from.st * PT_RAW, ring + to.st * PT_TILE, it.len - (it.from() + x / 2) * PT_KEYS);
+                    odd = l.uneven || (x & 1 && odd);
+                    if (threadIdx.x == 12 * 32) {            // every warp finds the same
+                        if (x & 1) v_lift[entries >> 1 & 1] = l.e, rough[entries >> 1 & 1] = odd;
+                        else k_back[entries >> 1 & 1] = __uint_as_float(uint32_t(134 - l.e) << 23);
+                    }
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) {
@@ -593,8 +662,11 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
         const int r_query = t * qt + r / group, r_head = r % group;
         const bool r_used = r < qt * group;
         uint32_t steps = 0, outs = 0;                        // key tiles and results so far
+        [[maybe_unused]] RingAt vt;                          // Q8_0: the values' tile
+        [[maybe_unused]] uint32_t qs = 0, tiles = 0;         // queries and key tiles of either row tile so far
         bool ok = true;
         Round it;
+        if constexpr (Q8) vt.next();
         for (int round = 0; ok && next_item(round, it, true); ++round) {
             const int nt = it.nt[t], i = it.first + r_query; // i: the sequence's row
             // (PT_SHARED: a sequence that holds fewer positions attends by itself)
@@ -602,6 +674,11 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
             const int limit = SHARED ? it.len : live ? it.seen(i) : 0;
             const int sure = SHARED ? it.len : it.seen(it.first + t * qt);   // keys that every row of the tile sees
             float m = -INFINITY, sum = 0.0f;
+            // Q8_0: S is q . k times 1 / (row's and tile's inverse lifts), O is times 2^lift
+            [[maybe_unused]] float row_back = 0.0f;
+            [[maybe_unused]] int lifted = 0;
+            [[maybe_unused]] bool redo = false;              // a tile that the row sees in part is uneven
+            const int nkv = max(it.nt[0], it.nt[1]);
             for (int j = 0; j < nt; ++j, ++steps) {
                 ok = __all_sync(FULL, mbar_wait(&s_full[t], steps & 1u, lane == 0 ? status : nullptr));
                 if (!ok) break;
@@ -621,13 +698,37 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
 #pragma unroll
                     for (int y = 0; y < 4; ++y)
                         mx[y] = fmaxf(fmaxf(mx[y], __uint_as_float(u[x + y])), __uint_as_float(u[x + y + 4]));
-                const float tile_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                float tile_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                float unit = PT_LOG2, lower = 1.0f;          // of S to exponents; what O is to be multiplied by besides
+                [[maybe_unused]] int shift = 0;              // of the probabilities' exponents
+                bool sink = false;
+                if constexpr (Q8) {
+                    ok = __all_sync(FULL, mbar_wait(&full[vt.st], vt.ph, lane == 0 ? status : nullptr));
+                    if (!ok) break;
+                    // (the queries were converted before this tile; q_ready may be a phase ahead by now)
+                    if (j == 0) row_back = q_back[qs & 1][t * PT_ROWS + r];
+                    const float back = fmaxf(row_back * k_back[tiles + j & 1], 0x1p-120f);
+                    const int e = v_lift[tiles + j & 1];
+                    redo |= !SHARED && rough[tiles + j & 1] && limit < min(it.len, (it.from() + j + 1) * PT_KEYS);
+                    vt.next();
+                    vt.next();
+                    tile_max *= back;
+                    unit *= back;
+                    if (j == 0) lifted = e;
+                    sink = e < lifted;                       // larger values than before: O goes down
+                    if (sink) {
+                        lower = e - lifted < -126 ? 0.0f : __uint_as_float(uint32_t(127 + e - lifted) << 23);
+                        lifted = e;
+                    }
+                    shift = max(lifted - e, -64);            // smaller ones: their probabilities go down
+                }
                 const bool grow = tile_max > m + PT_LAZY || (m == -INFINITY && tile_max > m);
-                if (__any_sync(FULL, grow)) {
+                if (__any_sync(FULL, grow) || sink) {
                     const float nm = grow ? tile_max : m;
-                    const float f = grow ? (m == -INFINITY ? 0.0f : ex2_approx_ftz((m - nm) * PT_LOG2)) : 1.0f;
+                    float f = grow ? (m == -INFINITY ? 0.0f : ex2_approx_ftz((m - nm) * PT_LOG2)) : 1.0f;
                     m = nm;
                     sum *= f;
+                    if constexpr (Q8) f *= lower;
                     if (j > 0) {                                 // O of the tiles before (their product has completed)
 #pragma unroll 1
                         for (int x = 0; x < 8; ++x) {
@@ -640,8 +741,9 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                         }
                     }
                 }
-                const float off = m == -INFINITY ? 0.0f : -m * PT_LOG2;
-                const f2 off2 = pk2(off, off), scale2 = pk2(PT_LOG2, PT_LOG2);
+                float off = m == -INFINITY ? 0.0f : -m * PT_LOG2;
+                if constexpr (Q8) off += float(shift + PT_BIAS);
+                const f2 off2 = pk2(off, off), scale2 = pk2(unit, unit);
                 f2 part[2] = {pk2(0.0f, 0.0f), pk2(0.0f, 0.0f)};
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {                    // 32 probabilities at a time; two halves are handed over
@@ -658,7 +760,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                             p1 = ex2_approx_ftz(p1);
                         }
                         part[y / 2 & 1] = add2(part[y / 2 & 1], pk2(p0, p1));
-                        w[y / 2] = pack_bf16(p0, p1);
+                        w[y / 2] = Q8 ? pack_f16(p0, p1) : pack_bf16(p0, p1);
                     }
                     tc_st16(ts + 16 * x, w);
                     if (x & 1) {
@@ -670,7 +772,16 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                 }
                 float s0, s1;
                 up2(add2(part[0], part[1]), s0, s1);
-                sum += s0 + s1;
+                if constexpr (Q8) sum = fmaf(s0 + s1, __uint_as_float(uint32_t(127 - PT_BIAS - shift) << 23), sum);
+                else sum += s0 + s1;
+            }
+            // what O is to be multiplied by (values are 2^7 below their lift, probabilities 2^7 above; NaN: to be done again)
+            [[maybe_unused]] float o_back = 1.0f;
+            if constexpr (Q8) {
+                for (int j = nt; j < nkv; ++j) vt.next(), vt.next();
+                tiles += nkv;
+                qs += nkv > 0;
+                o_back = redo ? __uint_as_float(0x7fffffffu) : ldexpf(1.0f, -lifted);
             }
             // ---- the result ----------------------------------------------------------------
             if (nt > 0 && ok) {
@@ -679,6 +790,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
             }
             if constexpr (SPLIT) {
                 if (ok) stat = make_float2(m, sum);
+                if constexpr (Q8) part_back = o_back;
                 if (it.parts > 1) continue;                  // joined below
             }
             if constexpr (SHARED) {
@@ -696,7 +808,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                             for (int y = 0; y < 4; ++y) {
                                 U8 v;
 #pragma unroll
-                                for (int z = 0; z < 8; ++z) v.w[z] = o[8 * y + z];
+                                for (int z = 0; z < 8; ++z) v.w[z] = Q8 ? __float_as_uint(__uint_as_float(o[8 * y + z]) * o_back) : o[8 * y + z];
                                 st_v8(sh.o + row * HD + 32 * x + 8 * y, v);
                             }
                     }
@@ -707,7 +819,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                 continue;
             }
             if (ok) {
-                const float inv = limit > 0 ? 1.0f / sum : 0.0f;
+                const float inv = limit > 0 ? (Q8 ? o_back / sum : 1.0f / sum) : 0.0f;
                 const unsigned lives = __ballot_sync(FULL, live);
                 // Four lanes exchange their rows' pieces, so that they store 64 bytes of a row together.  This lane
                 // stores piece lane % 4 of rows (lane / 4) * 4 + k.
@@ -804,6 +916,9 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
 #pragma unroll
                         for (int y = 0; y < 32; ++y) o[y] = 0u;
                     }
+                    if constexpr (Q8)
+#pragma unroll
+                        for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * part_back);
 #pragma unroll
                     for (int y = 0; y < 8; ++y)
                         *reinterpret_cast<uint4 *>(row + (((8 * x + y) ^ (lane & 7)) << 4)) =

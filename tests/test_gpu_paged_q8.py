@@ -5,8 +5,11 @@ parts (2 u each), sums of products of codes are exact up to the tensor cores' cu
 one rounding each.  An f16 part is no finer than 2^-25, half its least number, and the largest query element of a row (the
 largest value scale of 32 positions) is lifted to 2^14 or more, so that an element is also off by up to 2^-39 of the row's
 largest: a score by 128 * 2^-39 max|q| max|k| / sqrt(128), a result of n positions by n 2^-39 (128 / 127) max|v|.
-Where the result is bf16 a weight is one f16 part: 2^-11 relative each.  Prompts round every element
-of the cache to bf16 on its way to the products: their formula is taken over the rounded elements.
+Where the result is bf16 a weight is one f16 part: 2^-11 relative each, in prompts too.  Prompts round scales and then
+products of code and scale to f16 on their way: their formula is taken over the rounded elements (in f16 after
+multiplication by a power of two, so that the rounding is that of 11 bits at any size; what lies 2^-39 below the largest
+is within the terms above).  Their probabilities are no finer than 2^-25 where the largest are 2^7 to 2^15:
+n 2^-32 max|v| for values of one size.
 """
 import math
 
@@ -21,11 +24,11 @@ pytestmark = pytest.mark.gpu
 W = 2.0 ** -11
 
 
-def check_attention(got, q, k, v, seen, dtype, weight_rounding=0.0):
+def check_attention(got, q, k, v, seen, dtype, weight_rounding=0.0, floor=2.0 ** -39):
     o, pv, a = attend(q.double(), k, v, seen)
     n, top = max(1, k.shape[0]), lambda x: float(x.abs().max()) if x.numel() else 0.0
     ds = 160 * U * a + math.sqrt(128) * 2.0 ** -39 * top(q) * top(k)
-    tol = (torch.expm1(2 * ds) + (n + 64) * U + weight_rounding) * pv + n * 2.0 ** -39 * 1.01 * top(v)
+    tol = (torch.expm1(2 * ds) + (n + 64) * U + weight_rounding) * pv + n * floor * 1.01 * top(v)
     if dtype == BF16:
         tol = tol + H * (o.abs() + tol)
     bad = ~((got.double() - o).abs() <= tol + 1e-30)
@@ -158,8 +161,14 @@ def test_unused_scales_and_nan(q3):
 def rounded(p, s):
     """Keys and values of sequence s as the prompts' products take them."""
     page, slot = p.where(s, range(max(p.lens[s], 0)))
-    return tuple((t[page, :, slot].float() * c[page, :, slot].repeat_interleave(64, -1)).to(BF16).double()
-                 for t, c in ((p.k, p.ks), (p.v, p.vs)))
+    out = []
+    for t, c in ((p.k, p.ks), (p.v, p.vs)):
+        scale = c[page, :, slot]
+        top = float(scale.nan_to_num(0.0, 0.0, 0.0).abs().max()) if scale.numel() else 0.0
+        up = 2.0 ** (14 - math.floor(math.log2(top))) if top else 1.0
+        x = (scale * up).half().repeat_interleave(64, -1) * (t[page, :, slot].half() / 128)
+        out.append(x.double() * (128 / up))
+    return tuple(out)
 
 
 @pytest.mark.parametrize("heads,n_kv,page,rows,lens", PROMPT + [(32, 8, 64, [3], [7000]), (8, 1, 16, [100, 20], [2500, 3000])])
@@ -176,7 +185,7 @@ def test_attention_prompt(q3, heads, n_kv, page, rows, lens):
     for s, (r, n) in enumerate(zip(rows, lens)):
         if r:
             check_attention(out[first:first + r], q[first:first + r], *rounded(p, s), [max(0, n - r + 1 + i) for i in range(r)],
-                            BF16, H)
+                            BF16, W, 2.0 ** -32)
         first += r
     assert q3.device_status() == 0
 
@@ -193,7 +202,7 @@ def test_attention_prompt_many_sequences(q3, n_seqs):
     for s in range(n_seqs):
         if rows[s]:
             mine = slice(off[s], off[s + 1])
-            check_attention(out[mine], q[mine], *rounded(p, s), range(lens[s] - rows[s] + 1, lens[s] + 1), BF16, H)
+            check_attention(out[mine], q[mine], *rounded(p, s), range(lens[s] - rows[s] + 1, lens[s] + 1), BF16, W, 2.0 ** -32)
     assert q3.device_status() == 0
 
 
@@ -211,7 +220,7 @@ def test_attention_prompt_long(q3):
     got = q3.attention_prompt(*p.handles([0, n]), q)
     assert q3.device_status() == DEV_BAD_INDEX and q3.device_status() == 0
     some = list(range(0, n, 97)) + [n - 1]
-    check_attention(got[some], q[some], k, v, [i + 1 for i in some], BF16, H)
+    check_attention(got[some], q[some], k, v, [i + 1 for i in some], BF16, W, 2.0 ** -32)
 
 
 def test_attention_prompt_hides_later_rows(q3):
@@ -228,7 +237,7 @@ def test_attention_prompt_hides_later_rows(q3):
         k, v = (t[:147] for t in rounded(p, 0))
         early = rows - 3
         if early:
-            check_attention(got[:early], q[:early], k, v, range(1, early + 1), BF16, H)
+            check_attention(got[:early], q[:early], k, v, range(1, early + 1), BF16, W, 2.0 ** -32)
         assert torch.isnan(got[early:, :4, 64:]).all() and torch.isnan(got[early:, 4:]).all()
         assert torch.isfinite(got[early, :4, :64]).all()
 
@@ -237,4 +246,44 @@ def test_attention_prompt_peaked_and_flat(q3):
     for scale in (40.0, 0.0):
         p = Quantised([333], 2, 32, seed=37).fill(38, scale if scale else 1.0)
         q = queries(333, 8, BF16, 39, scale)
-        check_attention(q3.attention_prompt(*p.handles([0, 333]), q), q, *rounded(p, 0), range(1, 334), BF16, H)
+        check_attention(q3.attention_prompt(*p.handles([0, 333]), q), q, *rounded(p, 0), range(1, 334), BF16, W, 2.0 ** -32)
+
+
+def test_attention_prompt_uneven_scales(q3):
+    """Values and keys of very different sizes: tiles of larger values after smaller ones and the other way round; within a
+    tile, a later position 2^40 times larger takes no bits from earlier rows."""
+    n = 600
+    g = torch.Generator(device="cuda").manual_seed(60)
+    for sizes in ([2.0 ** (i // 128 * 3) for i in range(n)], [2.0 ** -(i // 128 * 3) for i in range(n)],
+                  [2.0 ** (i % 7) for i in range(n)]):
+        p = Quantised([n], 2, 16, seed=61).fill(62)
+        page, slot = p.where(0, range(n))
+        f = torch.tensor(sizes, device="cuda")
+        p.vs[page, :, slot] *= f[:, None, None]
+        p.ks[page, :, slot] *= torch.rand((n, 1, 1), generator=g, device="cuda") * 0.9 + 0.1
+        q = queries(n, 8, BF16, 63)
+        got = q3.attention_prompt(*p.handles([0, n]), q)
+        # as far as the rows see: a value's part of the error is relative to the largest it may be summed with
+        for a, b in ((0, 128), (128, 300), (300, n)):
+            check_attention(got[a:b], q[a:b], *(t[:b] for t in rounded(p, 0)), range(a + 1, b + 1), BF16, W, 2.0 ** -32)
+    for rows in (n, 5):
+        p = Quantised([n], 2, 16, seed=64).fill(65)
+        page, slot = p.where(0, range(n))
+        clean = q3.attention_prompt(*p.handles([0, rows]), q[:rows])
+        p.vs[page[n - 2], :, slot[n - 2]] *= 2.0 ** 40
+        p.ks[page[n - 1], :, slot[n - 1]] *= 2.0 ** 40
+        got = q3.attention_prompt(*p.handles([0, rows]), q[:rows])
+        check_attention(got[:rows - 2], q[:rows - 2], *(t[:n - 2] for t in p.rows(0)),
+                        range(n - rows + 1, n - 1), BF16, 2.0 ** -8)
+        assert torch.isfinite(clean).all()
+    assert q3.device_status() == 0
+
+
+def test_attention_prompt_sizes(q3):
+    """Queries, keys and values far from 1."""
+    for size_q, size_kv in ((1e-6, 1e6), (1e8, 1e-8), (1.0, 1e-20), (1e20, 1e-20), (1e-30, 1.0)):
+        p = Quantised([300], 2, 16, seed=66).fill(67, size_kv)
+        q = queries(300, 8, BF16, 68, size_q)
+        got = q3.attention_prompt(*p.handles([0, 300]), q)
+        check_attention(got, q, *rounded(p, 0), range(1, 301), BF16, W, 2.0 ** -32)
+    assert q3.device_status() == 0
