@@ -11,10 +11,11 @@ __device__ __forceinline__ uint32_t codes_f16(uint32_t codes, uint32_t pick) {
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(__byte_perm(codes, 0x64646464u, pick)), "r"(0x64806480u));  // - 1152
     return r;
 }
-// The same over 128: 8 + (code + 128) / 128 by a selector that puts 0x48 above each, less 9.
-__device__ __forceinline__ uint32_t codes_f16_128th(uint32_t codes, uint32_t pick) {
+// Two bytes of `codes`, in the lower halves of the 16-bit words of b, as f16 over 128: 8 + (code + 128) / 128, whose sign bit
+// a logical operation flips and whose upper byte it puts there, less 9.
+__device__ __forceinline__ uint32_t codes_f16_128th(uint32_t b) {
     uint32_t r;
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(__byte_perm(codes, 0x48484848u, pick)), "r"(0x48804880u));
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"((b & 0x00ff00ffu) ^ 0x48804880u), "r"(0x48804880u));
     return r;
 }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {

@@ -54,7 +54,8 @@ __device__ __forceinline__ void exp2_poly(float &x, float &y) {
                     __uint_as_float((__float_as_uint(t1) << 23) + 0x3f800000u))), x, y);
 }
 constexpr uint64_t PT_AGAIN_NS = 1000000000;                 // the longest that a warp computes rows again: others wait for it
-constexpr int PT_POLY = 8;                                   // one pair of exponentials in PT_POLY / 2 by polynomial
+constexpr int PT_POLY = 8;                                   // one pair of exponentials in PT_POLY / 2 by polynomial (Q8_0:
+                                                             // none, the conversion needs the same pipes)
 
 // The item of a round, as warp 9 announces it (s < 0: no more), with the key tiles of each row tile.
 struct PromptRound : PromptItem {
@@ -198,12 +199,10 @@ struct TileLift {
     int e;
     bool uneven;
 };
-// 128 rows' codes (128-byte swizzle) and scales at `raw` become the 32 KB f16 operand tile at `to`, by four warps: a lane
-// takes 16 codes of eight rows.  Rows from `rows` on are zeros.  The scales are lifted by the power of two that brings the
-// largest finite one to [2^14, 2^15) and rounded to f16 (2^-11), code / 128 is exact, the product is rounded once more:
-// 1.75 instructions an element.
-__device__ __forceinline__ TileLift q8_tile(const uint8_t *raw, uint8_t *to, int rows) {
-    const int lane = threadIdx.x & 31, key0 = int(threadIdx.x >> 5 & 3) * 32 + (lane & 7);
+// The lift of 128 rows by their scales, of which those before `rows` count (one warp; every lane returns it): by the power of
+// two that brings the largest finite one to [2^14, 2^15).
+__device__ __forceinline__ TileLift q8_lift(const uint8_t *raw, int rows) {
+    const int lane = threadIdx.x & 31;
     const float *scales = reinterpret_cast<const float *>(raw + PT_KEYS * HD);
     uint32_t top = 0, low = 0x7f7fffffu;                     // of the scales that count, as bits
 #pragma unroll
@@ -220,10 +219,18 @@ __device__ __forceinline__ TileLift q8_tile(const uint8_t *raw, uint8_t *to, int
     }
     top = __reduce_max_sync(FULL, top);
     low = __reduce_min_sync(FULL, low);
-    TileLift lifted;
-    lifted.e = min(141 - int(top >> 23), 126);
-    lifted.uneven = top && (top >> 23) - (low >> 23) > 24;
-    const float up = __uint_as_float(uint32_t(lifted.e + 127) << 23);
+    return {min(141 - int(top >> 23), 126), top && (top >> 23) - (low >> 23) > 24};
+}
+// 128 rows' codes (128-byte swizzle) and scales at `raw` become the 32 KB f16 operand tile at `to`, by four warps: a lane
+// takes 16 codes of eight rows.  Rows from `rows` on are zeros.  The lifted scales are rounded to f16 (2^-11), code / 128 is
+// exact, the product is rounded once more: 1.75 instructions an element.  A word's codes become the pairs (0, 2) and (1, 3), one
+// logical operation each and a permutation for the second (in byte order each takes a permutation, and the signs one
+// operation more): of four dimensions the middle two change places, in the queries (q_tile_f16) and the result (column) as
+// well.
+__device__ __forceinline__ void q8_tile(const uint8_t *raw, uint8_t *to, int rows, int e) {
+    const int lane = threadIdx.x & 31, key0 = int(threadIdx.x >> 5 & 3) * 32 + (lane & 7);
+    const float *scales = reinterpret_cast<const float *>(raw + PT_KEYS * HD);
+    const float up = __uint_as_float(uint32_t(e + 127) << 23);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int key = key0 + 8 * i;
@@ -238,9 +245,8 @@ __device__ __forceinline__ TileLift q8_tile(const uint8_t *raw, uint8_t *to, int
             uint32_t w[8];
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
-                const uint32_t u = words[y] ^ 0x80808080u;
-                w[2 * y] = mul_f16(codes_f16_128th(u, 0x4140), s2);
-                w[2 * y + 1] = mul_f16(codes_f16_128th(u, 0x4342), s2);
+                w[2 * y] = mul_f16(codes_f16_128th(words[y]), s2);
+                w[2 * y + 1] = mul_f16(codes_f16_128th(__byte_perm(words[y], 0, 0x4341)), s2);
             }
             uint8_t *row = to + half * PT_HALF + key * 128;  // 64 elements, chunks of 8
             const int c0 = 2 * (lane >> 3);
@@ -248,26 +254,35 @@ __device__ __forceinline__ TileLift q8_tile(const uint8_t *raw, uint8_t *to, int
             *reinterpret_cast<uint4 *>(row + (((c0 + 1) ^ (key & 7)) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
         }
     }
-    return lifted;
 }
+// Where dimension x of a head is in the result of a Q8_0 tile's product.
+template <bool Q8> __host__ __device__ constexpr int column(int x) { return Q8 && ((x & 3) == 1 || (x & 3) == 2) ? x ^ 3 : x; }
 // The bf16 queries of a row tile become f16 in their places, each row lifted so that its largest element lies in
-// [2^14, 2^15); one thread a row.  Returns the inverse of the row's lift.
+// [2^14, 2^15); one thread a row, its 16-byte chunks in an order in which the lanes' lie in different banks.  Returns the
+// inverse of the row's lift.
 __device__ __forceinline__ float q_tile_f16(uint8_t *tile, int row) {
     uint8_t *at = tile + row * 128;
+    auto chunk = [&](int x) { return reinterpret_cast<uint4 *>(at + (x >> 3) * PT_HALF + (((x ^ row) & 7) << 4)); };
     uint32_t top = 0;
-#pragma unroll 4
+#pragma unroll
     for (int x = 0; x < 16; ++x) {
-        const uint4 v = *reinterpret_cast<const uint4 *>(at + (x >> 3) * PT_HALF + ((x & 7) << 4));
+        const uint4 v = *chunk(x);
         top = __vmaxu2(top, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
     }
     top = max(top & 0xffffu, top >> 16) << 16;
     const float up = lift(top);
-#pragma unroll 4
-    for (int x = 0; x < 16; ++x) {
-        uint4 *p = reinterpret_cast<uint4 *>(at + (x >> 3) * PT_HALF + ((x & 7) << 4));
-        const uint4 v = *p;
-        auto two = [&](uint32_t w) { return pack_f16(bf16_to_f32(w & 0xffffu) * up, bf16_to_f32(w >> 16) * up); };
-        *p = make_uint4(two(v.x), two(v.y), two(v.z), two(v.w));
+#pragma unroll
+    for (int x0 = 0; x0 < 16; x0 += 4) {
+        uint4 v[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) v[x] = *chunk(x0 + x);
+        auto low = [&](uint32_t a, uint32_t b) { return pack_f16(bf16_to_f32(a & 0xffffu) * up, bf16_to_f32(b & 0xffffu) * up); };
+        auto high = [&](uint32_t a, uint32_t b) {
+            return pack_f16(__uint_as_float(a & 0xffff0000u) * up, __uint_as_float(b & 0xffff0000u) * up);
+        };
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+            *chunk(x0 + x) = make_uint4(low(v[x].x, v[x].y), high(v[x].x, v[x].y), low(v[x].z, v[x].w), high(v[x].z, v[x].w));
     }
     return lift_back(top);
 }
@@ -291,7 +306,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
     uint8_t *ring = smem + 2 * PT_TILE, *raw = ring + PT_NS * PT_TILE;       // raw: Q8_0 codes and scales
     __shared__ __align__(8) uint64_t q_full, q_empty, full[PT_NS], empty[PT_NS], s_full[2], p_full[2][2], o_full[2],
         o_empty[2], item_full[2], item_empty[2], taken, tail_go, tail, drain, raw_full[Q8 ? RAWS : 1], raw_empty[Q8 ? RAWS : 1],
-        q_ready;
+        q_ready, lifts[2];
     // Q8_0: the inverse lifts of the queries' rows (by item), and of the tiles in turn: keys' inverse, values' exponent
     __shared__ float q_back[Q8 ? 2 : 1][Q8 ? 2 * PT_ROWS : 1], k_back[2];
     __shared__ int v_lift[2];
@@ -320,6 +335,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
             mbar_init(&o_full[t], 1);
             mbar_init(&o_empty[t], 4);
             mbar_init(&item_full[t], 1);
+            mbar_init(&lifts[t], 1);
             mbar_init(&item_empty[t], Q8 ? 13 : 10);         // warps 0-7, 8 and 10, or 12-15
         }
         mbar_init(&taken, 1);
@@ -603,18 +619,34 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&q_ready);
                 }
-                bool odd = false;                            // K or V of this tile is uneven
+                // Entry 2 n is the keys of the n-th key tile, 2 n + 1 its values.  Both lifts are found, and announced,
+                // before the keys are converted, so that no softmax waits for them; but after the buffer of the values two
+                // tiles before is free, when no softmax needs that tile's any more.
+                TileLift lift[2];
                 for (int x = 0; x < 2 * nkv; ++x) {
-                    ok = mbar_wait(&raw_full[from.st], from.ph, lane == 0 ? status : nullptr);
-                    if (entries >= PT_NS) ok = ok && mbar_wait(&empty[to.st], to.ph ^ 1u, lane == 0 ? status : nullptr);
+                    const int rows = it.len - (it.from() + x / 2) * PT_KEYS, n = entries >> 1;
+                    if (x & 1) {
+                        if (entries >= PT_NS) ok = mbar_wait(&empty[to.st], to.ph ^ 1u, lane == 0 ? status : nullptr);
+                    } else {
+                        ::q3::RingAt<Q8 ? RAWS : 1> values = from;
+                        values.next();
+                        ok = mbar_wait(&raw_full[from.st], from.ph, lane == 0 ? status : nullptr) &&
+                             mbar_wait(&raw_full[values.st], values.ph, lane == 0 ? status : nullptr);
+                        ok = __all_sync(FULL, ok);
+                        if (!ok) break;
+                        lift[0] = q8_lift(raw + from.st * PT_RAW, rows);
+                        lift[1] = q8_lift(raw + values.st * PT_RAW, rows);
+                        if (entries >= PT_NS) ok = mbar_wait(&empty[to.st], to.ph ^ 1u, lane == 0 ? status : nullptr);
+                        if (threadIdx.x == 12 * 32) {        // every warp finds the same
+                            k_back[n & 1] = __uint_as_float(uint32_t(134 - lift[0].e) << 23);
+                            v_lift[n & 1] = lift[1].e;
+                            rough[n & 1] = lift[0].uneven || lift[1].uneven;
+                            mbar_arrive(&lifts[n & 1]);
+                        }
+                    }
                     ok = __all_sync(FULL, ok);
                     if (!ok) break;
-                    const TileLift l = q8_tile(raw + from.st * PT_RAW, ring + to.st * PT_TILE, it.len - (it.from() + x / 2) * PT_KEYS);
-                    odd = l.uneven || (x & 1 && odd);
-                    if (threadIdx.x == 12 * 32) {            // every warp finds the same
-                        if (x & 1) v_lift[entries >> 1 & 1] = l.e, rough[entries >> 1 & 1] = odd;
-                        else k_back[entries >> 1 & 1] = __uint_as_float(uint32_t(134 - l.e) << 23);
-                    }
+                    q8_tile(raw + from.st * PT_RAW, ring + to.st * PT_TILE, rows, x & 1 ? lift[1].e : lift[0].e);
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) {
@@ -662,11 +694,9 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
         const int r_query = t * qt + r / group, r_head = r % group;
         const bool r_used = r < qt * group;
         uint32_t steps = 0, outs = 0;                        // key tiles and results so far
-        [[maybe_unused]] RingAt vt;                          // Q8_0: the values' tile
-        [[maybe_unused]] uint32_t qs = 0, tiles = 0;         // queries and key tiles of either row tile so far
+        [[maybe_unused]] uint32_t qs = 0, tiles = 0;         // Q8_0: queries and key tiles of either row tile so far
         bool ok = true;
         Round it;
-        if constexpr (Q8) vt.next();
         for (int round = 0; ok && next_item(round, it, true); ++round) {
             const int nt = it.nt[t], i = it.first + r_query; // i: the sequence's row
             // (PT_SHARED: a sequence that holds fewer positions attends by itself)
@@ -703,15 +733,14 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                 [[maybe_unused]] int shift = 0;              // of the probabilities' exponents
                 bool sink = false;
                 if constexpr (Q8) {
-                    ok = __all_sync(FULL, mbar_wait(&full[vt.st], vt.ph, lane == 0 ? status : nullptr));
+                    const uint32_t n = tiles + j;
+                    ok = __all_sync(FULL, mbar_wait(&lifts[n & 1], n >> 1 & 1u, lane == 0 ? status : nullptr));
                     if (!ok) break;
                     // (the queries were converted before this tile; q_ready may be a phase ahead by now)
                     if (j == 0) row_back = q_back[qs & 1][t * PT_ROWS + r];
-                    const float back = fmaxf(row_back * k_back[tiles + j & 1], 0x1p-120f);
-                    const int e = v_lift[tiles + j & 1];
-                    redo |= !SHARED && rough[tiles + j & 1] && limit < min(it.len, (it.from() + j + 1) * PT_KEYS);
-                    vt.next();
-                    vt.next();
+                    const float back = fmaxf(row_back * k_back[n & 1], 0x1p-120f);
+                    const int e = v_lift[n & 1];
+                    redo |= !SHARED && rough[n & 1] && limit < min(it.len, (it.from() + j + 1) * PT_KEYS);
                     tile_max *= back;
                     unit *= back;
                     if (j == 0) lifted = e;
@@ -748,12 +777,20 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {                    // 32 probabilities at a time; two halves are handed over
                     uint32_t w[16];
+                    // Q8_0: the last 32 scores are read a second time rather than kept (registers)
+                    if constexpr (Q8) {
+                        if (x == 2) tc_ld32(ts + 96, u + 96);
+                        if (x == 3) {
+                            tc_wait_ld32(u + 96);
+                            if ((it.from() + j + 1) * PT_KEYS > sure) mask32(u + 96, limit - (it.from() + j) * PT_KEYS - 96);
+                        }
+                    }
 #pragma unroll
                     for (int y = 0; y < 32; y += 2) {
                         const f2 e = fma2(pk2(__uint_as_float(u[32 * x + y]), __uint_as_float(u[32 * x + y + 1])), scale2, off2);
                         float p0, p1;
                         up2(e, p0, p1);
-                        if (y % PT_POLY == PT_POLY - 2) {
+                        if (y % PT_POLY == PT_POLY - 2 && !Q8) {
                             exp2_poly(p0, p1);
                         } else {
                             p0 = ex2_approx_ftz(p0);
@@ -778,7 +815,6 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
             // what O is to be multiplied by (values are 2^7 below their lift, probabilities 2^7 above; NaN: to be done again)
             [[maybe_unused]] float o_back = 1.0f;
             if constexpr (Q8) {
-                for (int j = nt; j < nkv; ++j) vt.next(), vt.next();
                 tiles += nkv;
                 qs += nkv > 0;
                 o_back = redo ? __uint_as_float(0x7fffffffu) : ldexpf(1.0f, -lifted);
@@ -808,7 +844,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                             for (int y = 0; y < 4; ++y) {
                                 U8 v;
 #pragma unroll
-                                for (int z = 0; z < 8; ++z) v.w[z] = Q8 ? __float_as_uint(__uint_as_float(o[8 * y + z]) * o_back) : o[8 * y + z];
+                                for (int z = 0; z < 8; ++z) v.w[z] = Q8 ? __float_as_uint(__uint_as_float(o[column<Q8>(8 * y + z)]) * o_back) : o[8 * y + z];
                                 st_v8(sh.o + row * HD + 32 * x + 8 * y, v);
                             }
                     }
@@ -840,7 +876,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                     }
 #pragma unroll
                     for (int z = 0; z < 32; z += 2) {
-                        const f2 v = mul2(pk2(__uint_as_float(o[z]), __uint_as_float(o[z + 1])), pk2(inv, inv));
+                        const f2 v = mul2(pk2(__uint_as_float(o[column<Q8>(z)]), __uint_as_float(o[column<Q8>(z + 1)])), pk2(inv, inv));
                         zero = fma2(v, pk2(0.0f, 0.0f), zero);
                         float a, d;
                         up2(v, a, d);
@@ -922,7 +958,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
 #pragma unroll
                     for (int y = 0; y < 8; ++y)
                         *reinterpret_cast<uint4 *>(row + (((8 * x + y) ^ (lane & 7)) << 4)) =
-                            make_uint4(o[4 * y], o[4 * y + 1], o[4 * y + 2], o[4 * y + 3]);
+                            make_uint4(o[4 * y], o[column<Q8>(4 * y + 1)], o[column<Q8>(4 * y + 2)], o[4 * y + 3]);
                 }
                 tc_fence_before();
             }
