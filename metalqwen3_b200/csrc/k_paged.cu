@@ -52,7 +52,7 @@ constexpr size_t PD_SMEM = size_t(PD_NS) * PD_STAGE + PD_SPARE + 1024;
 template <typename TC> __host__ __device__ constexpr int pd_tile() { return int(PD_SIDE) / (HD * Elem<TC>::BYTES); }   // positions of a stage
 
 // WIDE: more than 8 query heads to a kv head (two blocks of columns).  Seqs: whole sequences, or their tails behind what
-// they share, whose results go to `tails` ([n_seqs][n_heads] rows of PD_PART floats) if they are not all of a sequence.
+// they share, whose results go to `tails` ([n_seqs][n_heads] rows of SHARED_ROW floats) if they are not all of a sequence.
 template <typename T, typename TC, bool WIDE, typename Seqs>
 __global__ void __launch_bounds__(PD_THREADS, 2)
 paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, const PagedKV c,
@@ -103,10 +103,12 @@ paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
         uint8_t *dst = ring + side * PD_SIDE + col * (PD_SIDE / CB) + box * br * 128;
         int page = page_of(), e = 0;
         bool ok = true;
-        for (int64_t u = u0; u < u1; ++u, ++e) {
+        for (int64_t u = Seqs::TAILS ? u0 + w.lead : u0, next; u < u1; u = next, ++e) {
+            next = u + 1;
             const int head = w.head, slot = (w.template pos<TILE, Seqs>(w.tile) + box * br) & ((1 << c.page_shift) - 1), now = page;
-            if (u + 1 < u1) {
+            if (next < u1) {
                 walk_on<TILE>(b, c, w, 1);
+                if (Seqs::TAILS) next += w.lead;
                 page = page_of();                            // under way while this tile waits for its stage
             }
             const int st = e % PD_NS;
@@ -129,7 +131,9 @@ paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
     int e = 0;
     bool ok = true;
     for (int64_t u = u0; u < u1 && ok;) {
-        const int run = int(min(int64_t(w.tiles - w.tile), u1 - u));       // tiles of this (sequence, head) here
+        const int lead = Seqs::TAILS ? w.lead : 0, units = int(min(int64_t(lead) + w.tiles - w.tile, u1 - u));
+        const int run = units - lead;                        // tiles of this (sequence, head) here
+        if (Seqs::TAILS && run <= 0) break;                  // it begins where the run ends
         const typename Elem<T>::type *qs = q + w.s * q_stride + int64_t(w.head) * group * HD;
         constexpr bool PARTS3 = !CF32 && Elem<T>::BYTES == 4;                // f32 queries, bf16 cache
         uint32_t qf[CF32 || PARTS3 ? 1 : 8][NH][2];          // bf16 queries, bf16 cache: operands in registers
@@ -463,6 +467,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
         ok = dead == 0;                                      // the same for every warp: the next barrier follows the read
         if (warp == 0 && ok) {
             const bool whole = run == w.tiles;
+            constexpr int ROW = Seqs::TAILS ? SHARED_ROW : PD_PART;
             const int at0 = CF32 ? 4 * g : g, step = CF32 ? 1 : 8;           // this lane's first element, and to its pair
             auto block = [](int j) { return CF32 ? 32 * (j >> 1) + 2 * (j & 1) : 16 * j; };
 #pragma unroll
@@ -478,15 +483,15 @@ paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
                         for (int j = 0; j < 8; ++j) put2(dst + block(j), step, o[j][n][h] * r, o[j][n][2 + h] * r);
                     } else {
                         float *pd = Seqs::TAILS && whole
-                                        ? tails + (int64_t(w.s) * n_heads + w.head * group + row) * PD_PART
-                                        : part + ((2 * int64_t(blockIdx.x) + (u != u0)) * group + row) * PD_PART;
+                                        ? tails + (int64_t(w.s) * n_heads + w.head * group + row) * ROW
+                                        : part + ((2 * int64_t(blockIdx.x) + (u != u0)) * group + row) * ROW;
 #pragma unroll
                         for (int j = 0; j < 8; ++j) put2(pd + at0 + block(j), step, o[j][n][h], o[j][n][2 + h]);
                         if (g == 0) pd[HD] = m[n][h], pd[HD + 1] = l[n][h];
                     }
                 }
         }
-        u += run;
+        u += units;
         if (u < u1) walk_on<TILE>(b, c, w, run);
         named_sync(1, PD_WARPS * 32);
     }

@@ -115,11 +115,13 @@ paged_q8_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
         uint8_t *dst = ring + (kind < 2 ? kind * PQ_CODES + box * br * HD : 2 * PQ_CODES + (kind & 1) * PQ_SCALES + box * br * 8);
         int page = page_of(), e = 0;
         bool ok = true;
-        for (int64_t u = u0; u < u1; ++u, ++e) {
+        for (int64_t u = Seqs::TAILS ? u0 + w.lead : u0, next; u < u1; u = next, ++e) {
+            next = u + 1;
             const int head = w.head, now = page;
             const int slot = (w.template pos<PQ_TILE, Seqs>(w.tile) + box * br) & ((1 << c.page_shift) - 1);
-            if (u + 1 < u1) {
+            if (next < u1) {
                 walk_on<PQ_TILE>(b, c, w, 1);
+                if (Seqs::TAILS) next += w.lead;
                 page = page_of();                            // under way while this tile waits for its stage
             }
             const int st = e % PQ_NS;
@@ -142,7 +144,9 @@ paged_q8_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
     int e = 0;
     bool ok = true;
     for (int64_t u = u0; u < u1 && ok;) {
-        const int run = int(min(int64_t(w.tiles - w.tile), u1 - u));       // tiles of this (sequence, head) here
+        const int lead = Seqs::TAILS ? w.lead : 0, units = int(min(int64_t(lead) + w.tiles - w.tile, u1 - u));
+        const int run = units - lead;                        // tiles of this (sequence, head) here
+        if (Seqs::TAILS && run <= 0) break;                  // it begins where the run ends
         const typename Elem<T>::type *qs = q + w.s * q_stride + int64_t(w.head) * group * HD;
         // the group's rows as f16 parts in shared memory, lifted, zeros below; 16-byte piece x of row r at x ^ (r % 2)
         for (int r = warp; r < 8 * NH; r += PQ_WARPS) {
@@ -406,6 +410,7 @@ paged_q8_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
         ok = dead == 0;                                      // the same for every warp: the next barrier follows the read
         if (warp == 0 && ok) {
             const bool whole = run == w.tiles;
+            constexpr int ROW = Seqs::TAILS ? SHARED_ROW : PD_PART;
 #pragma unroll
             for (int n = 0; n < NH; ++n)
 #pragma unroll
@@ -419,15 +424,15 @@ paged_q8_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
                         for (int j = 0; j < 8; ++j) put2(dst + 16 * j, 1, o[j][n][h] * r, o[j][n][2 + h] * r);
                     } else {
                         float *pd = Seqs::TAILS && whole
-                                        ? tails + (int64_t(w.s) * n_heads + w.head * group + row) * PD_PART
-                                        : part + ((2 * int64_t(blockIdx.x) + (u != u0)) * group + row) * PD_PART;
+                                        ? tails + (int64_t(w.s) * n_heads + w.head * group + row) * ROW
+                                        : part + ((2 * int64_t(blockIdx.x) + (u != u0)) * group + row) * ROW;
 #pragma unroll
                         for (int j = 0; j < 8; ++j) put2(pd + 2 * g + 16 * j, 1, o[j][n][h], o[j][n][2 + h]);
                         if (g == 0) pd[HD] = m[n][h], pd[HD + 1] = l[n][h];
                     }
                 }
         }
-        u += run;
+        u += units;
         if (u < u1) walk_on<PQ_TILE>(b, c, w, run);
         named_sync(1, PQ_WARPS * 32);
     }

@@ -18,103 +18,80 @@
 
 namespace q3 {
 
-constexpr int SJ_WARPS = 4;
-// What the join of (sequence s, kv head) reads, found by one warp.
-struct JoinPlan {
-    int shared_first, shared_n;      // runs that have a part of the shared positions
-    int tail_first, tail_n;
-    int slot;                        // this sequence's first row in a slot of the shared results
-    bool skip, shared_late, tail_late;       // part 0 is the second of its run
-};
+constexpr int SJ_WARPS = 4, SJ_PARTS = 8;                    // parts of a row under way at a time
 
+// One CTA per (sequence, kv head), one warp per query head of the group at a time.
 template <int TILE>
 __global__ void __launch_bounds__(SJ_WARPS * 32)
 shared_join_kernel(const SharedOut sh, const PagedKV c, const TailSeqs b, const FastDiv per_block, int n_heads, int group,
                    int shared_runs, int tail_runs, const float *part, const float *tails, uint16_t *out) {
-    __shared__ JoinPlan plan_sh;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int s = int(blockIdx.x / unsigned(c.n_kv)), kv = int(blockIdx.x % unsigned(c.n_kv));
-    // before the wait: lengths and tables are older than the launches before this one
-    if (warp == 0) {
-        JoinPlan p = {};
-        const PagedSpan mine = b.span(c, s, nullptr);
-        int64_t total = 0, before = 0;                       // tiles of the tails, of one kv head
-        for (int s0 = 0; s0 < b.n_seqs; s0 += 32) {
-            const int n = s0 + lane < b.n_seqs ? b.span(c, s0 + lane, nullptr).tiles<TILE>() : 0;
-            const uint32_t end = warp_prefix(uint32_t(n));
-            if (s >= s0 && s < s0 + 32) before = total + __shfl_sync(FULL, end - uint32_t(n), s - s0);
-            total += __shfl_sync(FULL, end, 31);
-        }
-        const int tiles = mine.tiles<TILE>();
-        if (tiles > 0) {
-            const PagedCut cut(total * c.n_kv, tail_runs);
-            const int64_t a = before * c.n_kv + int64_t(kv) * tiles;
-            p.tail_first = cut.run_of(a);
-            p.tail_n = cut.run_of(a + tiles - 1) - p.tail_first + 1;
-            p.tail_late = a != cut.begin(p.tail_first);
-        }
-        if (mine.from > 0) {
-            const int g = b.groups.of(s, b.n_seqs), at = s - b.groups.off[g];
-            int64_t first;
-            const PagedCut cut(shared_units(sh, b, c, per_block, g, first, nullptr) * c.n_kv, shared_runs);
-            const int keys = (mine.from + PT_KEYS - 1) / PT_KEYS, block = per_block(at);
-            const int blocks = per_block(b.groups.count(g, b.n_seqs) - 1) + 1;
-            const int64_t a = first * c.n_kv + (int64_t(kv) * blocks + block) * keys;
-            p.shared_first = cut.run_of(a);
-            p.shared_n = cut.run_of(a + keys - 1) - p.shared_first + 1;
-            p.shared_late = a != cut.begin(p.shared_first);
-            p.slot = (at - block * per_block.d) * group;
-        }
-        // nothing to do: no positions, or all of them written by the kernel before
-        p.skip = p.shared_n == 0 && p.tail_n <= 1;
-        if (lane == 0) plan_sh = p;
+    // Before the wait: the plan is older than the launch before this one, which has begun.  Runs are kept within what the
+    // workspace holds, whatever the plan says.
+    const PagedSpan mine = b.span(c, s, nullptr);
+    const int64_t tails_before = b.before[s], tails_all = b.before[b.n_seqs], shared_all = sh.group[b.n_seqs].units;
+    const SharedGroup of = sh.group[s];
+    const int tiles = mine.tiles<TILE>();
+    int tail_first = 0, tail_n = 0, shared_first = 0, shared_n = 0, slot = 0;
+    bool tail_late = false, shared_late = false;             // part 0 is the second of its run
+    if (tiles > 0) {
+        const PagedCut cut(tails_all * c.n_kv, tail_runs);
+        const int64_t a = tails_before * c.n_kv + int64_t(kv) * (TAIL_LEAD + tiles);
+        tail_first = cut.run_of(a + TAIL_LEAD);
+        tail_n = cut.run_of(a + TAIL_LEAD + tiles - 1) - tail_first + 1;
+        tail_late = a > cut.begin(tail_first);
     }
-    __syncthreads();
+    if (mine.from > 0) {
+        const PagedCut cut(shared_all * c.n_kv, shared_runs);
+        const int keys = (mine.from + PT_KEYS - 1) / PT_KEYS, at = s - of.first, block = per_block(at);
+        const int64_t a = of.units * c.n_kv + (int64_t(kv) * (per_block(of.count - 1) + 1) + block) * keys;
+        shared_first = min(max(cut.run_of(a), 0), shared_runs - 1);
+        shared_n = min(max(cut.run_of(a + keys - 1), shared_first), shared_runs - 1) - shared_first + 1;
+        shared_late = a > cut.begin(shared_first);
+        slot = (at - block * per_block.d) * group;
+    }
     griddep_wait();
-    const JoinPlan p = plan_sh;
-    if (p.skip) return;
-    const int64_t rows = int64_t(b.n_seqs) * n_heads;
-    const int n = p.shared_n + p.tail_n;
+    const int n = shared_n + tail_n;
+    if (shared_n == 0 && tail_n <= 1) return;                // no positions, or all of them written by the launch before
     for (int h = warp; h < group; h += SJ_WARPS) {
         const int64_t row = int64_t(s) * n_heads + kv * group + h;
-        auto shared_row = [&](int i) {                       // part i < shared_n
-            return p.shared_n == 1 ? row
-                                   : rows + (2 * int64_t(p.shared_first + i) + (i == 0 && p.shared_late)) * sh.slot_rows + p.slot + h;
-        };
-        auto tail_part = [&](int i) -> const float * {       // part i < tail_n
-            return p.tail_n == 1 ? tails + row * PD_PART
-                                 : part + ((2 * int64_t(p.tail_first + i) + (i == 0 && p.tail_late)) * group + h) * PD_PART;
-        };
-        auto stat = [&](int i) -> float2 {
-            if (i < p.shared_n) return sh.stat[shared_row(i)];
-            const float *t = tail_part(i - p.shared_n);
-            return make_float2(t[HD], t[HD + 1]);
+        auto at = [&](int i) -> const float * {              // part i: 128 elements, maximum, sum
+            if (i < shared_n)
+                return sh.rows + SHARED_ROW * (shared_n == 1 ? row
+                                                             : int64_t(b.n_seqs) * n_heads +
+                                                                   (2 * int64_t(shared_first + i) + (i == 0 && shared_late)) * sh.slot_rows + slot + h);
+            i -= shared_n;
+            return tail_n == 1 ? tails + row * SHARED_ROW
+                               : part + ((2 * int64_t(tail_first + i) + (i == 0 && tail_late)) * group + h) * SHARED_ROW;
         };
         float m = -INFINITY;
-        for (int i = lane; i < n; i += 32) m = fmaxf(m, stat(i).x);
+        for (int i = lane; i < n; i += 32) m = fmaxf(m, at(i)[HD]);
         m = warp_max(m);
         float l = 0.0f;
         float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         for (int i0 = 0; i0 < n; i0 += 32) {
+            const float *mine_at = at(min(i0 + lane, n - 1));
             float w = 0.0f;
             if (i0 + lane < n) {
-                const float2 x = stat(i0 + lane);
+                const float2 x = *reinterpret_cast<const float2 *>(mine_at + HD);
                 w = x.x == m ? 1.0f : ex2_approx_ftz((x.x - m) * PD_LOG2);
                 l = fmaf(x.y, w, l);
             }
             const int end = min(32, n - i0);
-#pragma unroll 4
-            for (int i = 0; i < end; ++i) {
-                const float f = __shfl_sync(FULL, w, i);
-                float4 v;
-                if (i0 + i < p.shared_n) {
-                    v = *reinterpret_cast<const float4 *>(sh.o + shared_row(i0 + i) * HD + 4 * lane);
-                } else {
-                    const float2 *t = reinterpret_cast<const float2 *>(tail_part(i0 + i - p.shared_n) + 4 * lane);
-                    const float2 a = t[0], d = t[1];
-                    v = make_float4(a.x, a.y, d.x, d.y);
+            for (int i = 0; i < end; i += SJ_PARTS) {
+                float4 v[SJ_PARTS];
+#pragma unroll
+                for (int k = 0; k < SJ_PARTS; ++k) {
+                    const float *p = reinterpret_cast<const float *>(__shfl_sync(FULL, reinterpret_cast<uint64_t>(mine_at), min(i + k, 31)));
+                    v[k] = i + k < end ? *reinterpret_cast<const float4 *>(p + 4 * lane) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 }
-                o = make_float4(fmaf(f, v.x, o.x), fmaf(f, v.y, o.y), fmaf(f, v.z, o.z), fmaf(f, v.w, o.w));
+#pragma unroll
+                for (int k = 0; k < SJ_PARTS; ++k) {
+                    const float f = __shfl_sync(FULL, w, min(i + k, 31));
+                    if (i + k < end)
+                        o = make_float4(fmaf(f, v[k].x, o.x), fmaf(f, v[k].y, o.y), fmaf(f, v[k].z, o.z), fmaf(f, v[k].w, o.w));
+                }
             }
         }
 #pragma unroll
@@ -124,21 +101,23 @@ shared_join_kernel(const SharedOut sh, const PagedKV c, const TailSeqs b, const 
     }
 }
 
-// The workspace: results of the shared positions and their maxima and sums, whole tails, parts of tails.
+// The workspace: rows of the shared positions, of whole tails, of parts of tails, then the plan.
 struct SharedWork {
-    size_t stat, tails, part, bytes;
+    size_t tails, part, spans, before, group, bytes;
     int slot_rows;
 };
 static SharedWork shared_work(int n_seqs, int n_heads, int n_kv, int sms) {
     auto round = [](size_t x) { return (x + 255) / 256 * 256; };
     const int group = n_heads / n_kv, block = 2 * (PT_ROWS / group);
+    const size_t row = SHARED_ROW * sizeof(float), rows = size_t(n_seqs) * n_heads;
     SharedWork w;
     w.slot_rows = (n_seqs < block ? n_seqs : block) * group;
-    const size_t rows = size_t(n_seqs) * n_heads, all = rows + size_t(2) * sms * w.slot_rows;
-    w.stat = round(all * HD * sizeof(float));
-    w.tails = w.stat + round(all * sizeof(float2));
-    w.part = w.tails + round(rows * PD_PART * sizeof(float));
-    w.bytes = w.part + size_t(paged_runs(sms)) * 2 * group * PD_PART * sizeof(float);
+    w.tails = round((rows + size_t(2) * sms * w.slot_rows) * row);
+    w.part = w.tails + round(rows * row);
+    w.spans = w.part + round(size_t(paged_runs(sms)) * 2 * group * row);
+    w.before = w.spans + round(size_t(n_seqs) * sizeof(int2));
+    w.group = w.before + round((size_t(n_seqs) + 1) * sizeof(int64_t));
+    w.bytes = w.group + round((size_t(n_seqs) + 1) * sizeof(SharedGroup));
     return w;
 }
 size_t attention_shared_workspace(int n_seqs, int n_heads, int n_kv, int sms) {
@@ -173,11 +152,19 @@ cudaError_t launch_attention_shared(const PagedKV &c, q3cu_dtype cache_dt, const
     const SharedWork w = shared_work(b.n_seqs, n_heads, c.n_kv, sms);
     uint8_t *base = static_cast<uint8_t *>(work);
     float *tails = reinterpret_cast<float *>(base + w.tails), *part = reinterpret_cast<float *>(base + w.part);
-    const PagedGroups groups{off, len, n_groups};
-    const SharedOut sh{groups, reinterpret_cast<float *>(base), reinterpret_cast<float2 *>(base + w.stat), w.slot_rows};
+    if (n_groups == 0)                                       // (its parts fit where those of the tails would lie)
+        return launch_attention_paged(c, cache_dt, b, q, Q3CU_BF16, q_stride, n_heads, part, out, status, stream, sms);
+    const SharedOut sh{PagedGroups{off, len, n_groups},
+                       reinterpret_cast<float *>(base),
+                       w.slot_rows,
+                       reinterpret_cast<int2 *>(base + w.spans),
+                       reinterpret_cast<int64_t *>(base + w.before),
+                       reinterpret_cast<SharedGroup *>(base + w.group),
+                       cache_dt == Q3CU_Q8_0 ? PD_TAIL_Q8 : PD_TAIL_BF16};
     TailSeqs seqs;
     static_cast<PagedSeqs &>(seqs) = b;
-    seqs.groups = groups;
+    seqs.spans = sh.spans;
+    seqs.before = sh.before;
     const bool q8 = cache_dt == Q3CU_Q8_0;
     cudaError_t e = q8 ? launch_prefixes<true>(sh, c, b, q, q_stride, n_heads, status, stream, sms)
                        : launch_prefixes<false>(sh, c, b, q, q_stride, n_heads, status, stream, sms);

@@ -103,13 +103,22 @@ template <int NS> struct RingAt {
 // ---- what groups of sequences share ---------------------------------------------------------------
 // The items of a PT_SHARED launch, in the order group, kv head, block of `per_block` sequences; each is as many units as
 // the shared positions have key tiles.  All units are cut into one run per CTA (PagedCut).  A run that covers all of an item
-// leaves its rows' results at row (sequence, head) of `out`; one that begins or ends inside leaves them in slot 2 run, or
-// 2 run + 1 if the run began with another item, of the slots behind.
+// leaves its rows' results at row (sequence, head); one that begins or ends inside leaves them in slot 2 run, or 2 run + 1 if
+// the run began with another item, of the slots behind.
+// What the launches behind need to know of a sequence: its span, the units of the sequences before it (TailSeqs), and of its
+// group the first sequence, the number of sequences and the units of the groups before (of one kv head).
+struct SharedGroup {
+    int first, count;
+    int64_t units;
+};
 struct SharedOut {
     PagedGroups groups;
-    float *o;                // rows of 128: [n_seqs][n_heads], then [runs][2][slot_rows]
-    float2 *stat;            // their maxima and sums
+    float *rows;             // of SHARED_ROW floats: [n_seqs][n_heads], then [runs][2][slot_rows]
     int slot_rows;
+    int2 *spans;             // the plan
+    int64_t *before;
+    SharedGroup *group;      // [n_seqs + 1], the last with the units of all groups
+    int tail_tile;           // positions of a tile of the sequences' own part
 };
 struct SharedWalk {
     int g, head, block, tile, len, tiles, blocks;            // blocks of the group's sequences
@@ -133,39 +142,39 @@ __device__ __forceinline__ int64_t warp_prefix64(int64_t x) {                // 
     }
     return x;
 }
-// The units of all groups (of one kv head), and those before group g (one warp; every lane returns them).
-__device__ __forceinline__ int64_t shared_units(const SharedOut &sh, const PagedSeqs &b, const PagedKV &c,
-                                                const FastDiv &per_block, int g, int64_t &before, uint32_t *status) {
-    const int lane = threadIdx.x & 31;
-    int64_t total = 0;
-    before = 0;
-    for (int g0 = 0; g0 < sh.groups.n; g0 += 32) {
-        const int64_t x = SharedWalk::units(sh, b, c, per_block, g0 + lane, status), end = warp_prefix64(x);
-        if (g >= g0 && g < g0 + 32) before = total + __shfl_sync(FULL, end - x, g - g0);
-        total += __shfl_sync(FULL, end, 31);
-    }
-    return total;
-}
-// The place of unit u, which some group holds (one warp; every lane returns it).
-__device__ __forceinline__ SharedWalk shared_find(const SharedOut &sh, const PagedSeqs &b, const PagedKV &c,
-                                                  const FastDiv &per_block, int64_t u) {
+// A run's units [u, u1) of all, and the place of u (one warp; every lane returns it).
+__device__ __forceinline__ SharedWalk shared_run(const SharedOut &sh, const PagedSeqs &b, const PagedKV &c,
+                                                 const FastDiv &per_block, int run, int runs, int64_t &u, int64_t &u1) {
     const int lane = threadIdx.x & 31;
     SharedWalk w = {};
+    int64_t total = 0, x = 0, end = 0;
     for (int g0 = 0; g0 < sh.groups.n; g0 += 32) {
-        const int64_t x = SharedWalk::units(sh, b, c, per_block, g0 + lane, nullptr), end = warp_prefix64(x);
-        const unsigned hit = __ballot_sync(FULL, u < end * c.n_kv);
+        x = SharedWalk::units(sh, b, c, per_block, g0 + lane, nullptr);
+        end = warp_prefix64(x);
+        total += __shfl_sync(FULL, end, 31);
+    }
+    const PagedCut cut(total * c.n_kv, runs);
+    u = cut.begin(run);
+    u1 = cut.begin(run + 1);
+    if (u == u1) return w;
+    int64_t left = u;
+    for (int g0 = 0; g0 < sh.groups.n; g0 += 32) {
+        if (sh.groups.n > 32) {                              // otherwise the lanes still hold them
+            x = SharedWalk::units(sh, b, c, per_block, g0 + lane, nullptr);
+            end = warp_prefix64(x);
+        }
+        const unsigned hit = __ballot_sync(FULL, left < end * c.n_kv);
         if (hit) {
             const int l = __ffs(hit) - 1;
             w.g = g0 + l;
             w.enter(sh, b, c, per_block);
-            int64_t at = u - __shfl_sync(FULL, end - x, l) * c.n_kv;
-            const int64_t item = at / w.tiles;
+            const int64_t at = left - __shfl_sync(FULL, end - x, l) * c.n_kv, item = quot(at, w.tiles);
             w.tile = int(at - item * w.tiles);
-            w.head = int(item / w.blocks);
+            w.head = int(quot(item, w.blocks));
             w.block = int(item - int64_t(w.head) * w.blocks);
             return w;
         }
-        u -= __shfl_sync(FULL, end, 31) * c.n_kv;
+        left -= __shfl_sync(FULL, end, 31) * c.n_kv;
     }
     return w;
 }
@@ -187,7 +196,43 @@ __device__ __forceinline__ void shared_next(const SharedOut &sh, const PagedSeqs
         }
     }
 }
-
+// The plan for the launches behind, by one warp beside the products of its CTA.  (A group's units are left with its first
+// sequence, from where the others take them.  With offsets that do not rise, groups may overlap: then what is found
+// here is of no use, but the launches behind stay within the workspace.)
+__device__ __forceinline__ void shared_plan(const SharedOut &sh, const PagedSeqs &b, const PagedKV &c, const FastDiv &per_block,
+                                            uint32_t *status) {
+    const int lane = threadIdx.x & 31;
+    int64_t total = 0;
+    for (int g0 = 0; g0 < sh.groups.n; g0 += 32) {
+        const int64_t x = SharedWalk::units(sh, b, c, per_block, g0 + lane, status), end = warp_prefix64(x);
+        if (x) sh.group[sh.groups.off[g0 + lane]].units = total + end - x;
+        total += __shfl_sync(FULL, end, 31);
+    }
+    if (lane == 0) sh.group[b.n_seqs].units = total;
+    __syncwarp();
+    int64_t sum = 0;
+    for (int s0 = 0; s0 < b.n_seqs; s0 += 32) {
+        const int s = s0 + lane;
+        uint32_t units = 0;
+        if (s < b.n_seqs) {
+            const int len = paged_len(b, c, s, status), g = sh.groups.of(s, b.n_seqs);
+            int from = g < 0 ? 0 : sh.groups.shared(g, b, c, nullptr);
+            if (len < from) from = 0;                        // one that holds fewer attends by itself
+            if (from) {
+                const int first = sh.groups.off[g];
+                sh.group[s].first = first;
+                sh.group[s].count = sh.groups.count(g, b.n_seqs);
+                if (s != first) sh.group[s].units = sh.group[first].units;
+            }
+            sh.spans[s] = make_int2(from, len);
+            if (len > from) units = uint32_t(TAIL_LEAD + (len + sh.tail_tile - 1) / sh.tail_tile - from / sh.tail_tile);
+        }
+        const uint32_t end = warp_prefix(units);
+        if (s < b.n_seqs) sh.before[s] = sum + (end - units);
+        sum += __shfl_sync(FULL, end, 31);
+    }
+    if (lane == 0) sh.before[b.n_seqs] = sum;
+}
 struct NoOrder {             // in place of a PromptOrder
     __device__ __forceinline__ NoOrder(const PagedSeqs &, const PagedKV &, int, const FastDiv &, int, uint32_t *) {}
     __device__ __forceinline__ PromptItem find(int64_t) { return {}; }
@@ -405,12 +450,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                 }
             };
             if constexpr (SHARED) {
-                int64_t before;
-                const PagedCut cut(shared_units(sh, b, c, per_block, -1, before, blockIdx.x == 0 ? status : nullptr) * c.n_kv,
-                                   int(gridDim.x));
-                u = cut.begin(int(blockIdx.x));
-                u1 = cut.begin(int(blockIdx.x) + 1);
-                if (u < u1) walk = shared_find(sh, b, c, per_block, u);
+                walk = shared_run(sh, b, c, per_block, int(blockIdx.x), int(gridDim.x), u, u1);
             }
             typedef typename std::conditional<SHARED, NoOrder, PromptOrder>::type Order;
             Order order(b, c, rows, per_block, PT_KEYS, status);
@@ -658,6 +698,8 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                     ++entries;
                 }
             }
+        } else if (SHARED && warp == 11) {
+            if (blockIdx.x == 0) shared_plan(sh, b, c, per_block, status);
         } else if (!Q8 && warp == 10) {
             // ---- values behind a sequence's end: zeros -----------------------------------------
             Round it;
@@ -833,7 +875,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                 if (ok && nt > 0) {
                     const int64_t row = it.dst < 0 ? int64_t(it.base + i) * n_heads + it.head * group + r_head
                                                    : int64_t(b.n_seqs) * n_heads + it.dst + r_query * group + r_head;
-                    if (live) sh.stat[row] = make_float2(m, sum);
+                    if (live) *reinterpret_cast<float2 *>(sh.rows + row * SHARED_ROW + HD) = make_float2(m, sum);
 #pragma unroll 1
                     for (int x = 0; x < 4; ++x) {
                         uint32_t o[32];
@@ -845,7 +887,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                                 U8 v;
 #pragma unroll
                                 for (int z = 0; z < 8; ++z) v.w[z] = Q8 ? __float_as_uint(__uint_as_float(o[column<Q8>(8 * y + z)]) * o_back) : o[8 * y + z];
-                                st_v8(sh.o + row * HD + 32 * x + 8 * y, v);
+                                st_v8(sh.rows + row * SHARED_ROW + 32 * x + 8 * y, v);
                             }
                     }
                     tc_fence_before();                       // the next item's products may overwrite O

@@ -72,20 +72,24 @@ struct PagedGroups {
         return n > 0 && count(lo, n_seqs) > 0 && off[lo] <= s && s < off[lo + 1] ? lo : -1;
     }
 };
-// The batch's sequences behind what they share.
+// The batch's sequences behind what they share, as the launch before this one planned them (SharedPlan).  A (sequence, head) of
+// T tiles is TAIL_LEAD + T units of the cut: what it costs to begin and end one is worth about two tiles.
+constexpr int TAIL_LEAD = 2;
+constexpr int SHARED_ROW = 136;                              // floats of a row's part there: 128, maximum, sum (32-byte aligned)
 struct TailSeqs : PagedSeqs {
     static constexpr bool TAILS = true;
-    PagedGroups groups;
-    __device__ __forceinline__ PagedSpan span(const PagedKV &c, int s, uint32_t *status) const {
-        const int g = groups.of(s, n_seqs), from = g < 0 ? 0 : groups.shared(g, *this, c, nullptr);
-        const int len = paged_len(*this, c, s, status);
-        return {len < from ? 0 : from, len};                 // one that holds fewer attends by itself
+    const int2 *spans;       // from, len
+    const int64_t *before;   // [n_seqs + 1] units of the sequences before, of one kv head
+    __device__ __forceinline__ PagedSpan span(const PagedKV &, int s, uint32_t *) const {
+        const int2 x = spans[s];
+        return {x.x, x.y};
     }
 };
 
 // A place in the batch's tiles: sequence, kv head, tile, and the sequence's span and tiles.
 struct PagedWalk {
     int s, head, tile, from, len, tiles;
+    int lead;                // tails: units before the tile
     template <int TILE, typename Seqs> __device__ __forceinline__ int pos(int at) const {    // of tile `at`'s first row
         return (Seqs::TAILS ? from / TILE + at : at) * TILE;
     }
@@ -106,6 +110,40 @@ __device__ __forceinline__ PagedWalk walk_run(const Seqs &b, const PagedKV &c, i
                                               int64_t &u0, int64_t &u1, uint32_t *status) {
     PagedWalk w = {};
     const int lane = threadIdx.x & 31;
+    if constexpr (Seqs::TAILS) {
+        // up to 256 sequences are searched in one round of loads
+        constexpr int ROUND = 8;
+        cut = PagedCut(b.before[b.n_seqs] * c.n_kv, runs);
+        u0 = cut.begin(run);
+        u1 = cut.begin(run + 1);
+        if (u0 == u1) return w;
+        for (int s0 = 0; s0 < b.n_seqs; s0 += 32 * ROUND) {
+            int64_t x[ROUND];                                // of sequences s0 + 32 r + lane
+#pragma unroll
+            for (int r = 0; r < ROUND; ++r) x[r] = b.before[min(s0 + 32 * r + lane, b.n_seqs)];
+            const int64_t end = b.before[min(s0 + 32 * ROUND, b.n_seqs)];
+            if (u0 >= end * c.n_kv) continue;
+#pragma unroll
+            for (int r = ROUND - 1; r >= 0; --r) {           // the last sequence that begins at or before u0
+                const unsigned hit = __ballot_sync(FULL, s0 + 32 * r + lane < b.n_seqs && x[r] * c.n_kv <= u0);
+                if (hit) {
+                    const int l = 31 - __clz(hit);
+                    w.s = s0 + 32 * r + l;
+                    const PagedSpan mine = b.span(c, w.s, nullptr);
+                    w.from = mine.from;
+                    w.len = mine.len;
+                    w.tiles = mine.tiles<TILE>();
+                    const int64_t at = u0 - __shfl_sync(FULL, x[r], l) * c.n_kv;
+                    w.head = int(quot(at, TAIL_LEAD + w.tiles));
+                    const int unit = int(at - int64_t(w.head) * (TAIL_LEAD + w.tiles));
+                    w.tile = max(unit - TAIL_LEAD, 0);
+                    w.lead = max(TAIL_LEAD - unit, 0);
+                    return w;
+                }
+            }
+        }
+        return w;
+    }
     int64_t total = 0;                                       // in tiles of one kv head
     uint32_t end = 0;
     PagedSpan len = {0, 0};
@@ -127,9 +165,8 @@ __device__ __forceinline__ PagedWalk walk_run(const Seqs &b, const PagedKV &c, i
         if (hit) {
             const int l = __ffs(hit) - 1;
             w.s = s0 + l;
-            w.from = Seqs::TAILS ? __shfl_sync(FULL, len.from, l) : 0;
             w.len = __shfl_sync(FULL, len.len, l);
-            w.tiles = PagedSpan{w.from, w.len}.tiles<TILE>();
+            w.tiles = PagedSpan{0, w.len}.tiles<TILE>();
             const int64_t at = u - int64_t(__shfl_sync(FULL, end, l) - uint32_t(w.tiles)) * c.n_kv;
             w.head = int(quot(at, w.tiles));
             w.tile = int(at - int64_t(w.head) * w.tiles);
@@ -144,8 +181,10 @@ __device__ __forceinline__ PagedWalk walk_run(const Seqs &b, const PagedKV &c, i
 template <int TILE, typename Seqs>
 __device__ __forceinline__ void walk_on(const Seqs &b, const PagedKV &c, PagedWalk &w, int n) {
     w.tile += n;
+    w.lead = 0;
     if (w.tile < w.tiles) return;
     w.tile = 0;
+    if (Seqs::TAILS) w.lead = TAIL_LEAD;
     if (++w.head < c.n_kv) return;
     w.head = 0;
     for (++w.s; w.s < b.n_seqs; w.s += 32) {
