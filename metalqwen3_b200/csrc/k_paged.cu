@@ -103,6 +103,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
         uint8_t *dst = ring + side * PD_SIDE + col * (PD_SIDE / CB) + box * br * 128;
         int page = page_of(), e = 0;
         bool ok = true;
+        [[maybe_unused]] const uint64_t once = Seqs::TAILS ? evict_first_policy() : 0;
         for (int64_t u = Seqs::TAILS ? u0 + w.lead : u0, next; u < u1; u = next, ++e) {
             next = u + 1;
             const int head = w.head, slot = (w.template pos<TILE, Seqs>(w.tile) + box * br) & ((1 << c.page_shift) - 1), now = page;
@@ -116,8 +117,12 @@ paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
             if (!__all_sync(FULL, ok)) break;
             if (lane == 0) mbar_arrive_expect_tx(&full[st], PD_STAGE);
             __syncwarp();
-            if (side < 2)
-                tma_load_4d(dst + st * PD_STAGE, side ? &tmv : &tmk, (CF32 ? 32 : 64) * col, slot, head, now, &full[st]);
+            if (side < 2) {
+                // tails: read once, while the shared positions' results wait in L2
+                if constexpr (Seqs::TAILS)
+                    tma_load_4d_once(dst + st * PD_STAGE, side ? &tmv : &tmk, (CF32 ? 32 : 64) * col, slot, head, now, &full[st], once);
+                else tma_load_4d(dst + st * PD_STAGE, side ? &tmv : &tmk, (CF32 ? 32 : 64) * col, slot, head, now, &full[st]);
+            }
         }
         // no copy outlives the CTA (bounded)
         for (int d = e > PD_NS ? e - PD_NS : 0; d < e; ++d) mbar_wait(&full[d % PD_NS], uint32_t(d / PD_NS) & 1u, nullptr);

@@ -115,6 +115,7 @@ paged_q8_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
         uint8_t *dst = ring + (kind < 2 ? kind * PQ_CODES + box * br * HD : 2 * PQ_CODES + (kind & 1) * PQ_SCALES + box * br * 8);
         int page = page_of(), e = 0;
         bool ok = true;
+        const uint64_t once = evict_first_policy();
         for (int64_t u = Seqs::TAILS ? u0 + w.lead : u0, next; u < u1; u = next, ++e) {
             next = u + 1;
             const int head = w.head, now = page;
@@ -129,8 +130,9 @@ paged_q8_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
             if (!__all_sync(FULL, ok)) break;
             if (lane == 0) mbar_arrive_expect_tx(&full[st], PQ_STAGE);
             __syncwarp();
-            if (kind < 2) tma_load_4d(dst + st * PQ_STAGE, kind ? &tmv : &tmk, 0, slot, head, now, &full[st]);
-            else if (kind < 4) tma_load_3d(dst + st * PQ_STAGE, kind & 1 ? &tmvs : &tmks, 2 * slot, head, now, &full[st]);
+            // read once (and tails while the shared positions' results wait in L2)
+            if (kind < 2) tma_load_4d_once(dst + st * PQ_STAGE, kind ? &tmv : &tmk, 0, slot, head, now, &full[st], once);
+            else if (kind < 4) tma_load_3d_once(dst + st * PQ_STAGE, kind & 1 ? &tmvs : &tmks, 2 * slot, head, now, &full[st], once);
         }
         // no copy outlives the CTA (bounded)
         for (int d = e > PQ_NS ? e - PQ_NS : 0; d < e; ++d) mbar_wait(&full[d % PQ_NS], uint32_t(d / PQ_NS) & 1u, nullptr);

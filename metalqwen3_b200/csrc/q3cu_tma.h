@@ -84,6 +84,30 @@ __device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, i
            "r"(y), "r"(z), "r"(w), "r"(static_cast<uint32_t>(__cvta_generic_to_shared(bar)))
         : "memory");
 }
+// The same for what is read once: it leaves L2 before other lines do (policy: of evict_first_policy).
+__device__ __forceinline__ uint64_t evict_first_policy() {
+    uint64_t p;
+    asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+    return p;
+}
+__device__ __forceinline__ void tma_load_3d_once(void *dst, const CUtensorMap *map, int x, int y, int z, uint64_t *bar,
+                                                 uint64_t policy) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint "
+        "[%0], [%1, {%2, %3, %4}], [%5], %6;"
+        :: "r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))), "l"(reinterpret_cast<uint64_t>(map)), "r"(x),
+           "r"(y), "r"(z), "r"(static_cast<uint32_t>(__cvta_generic_to_shared(bar))), "l"(policy)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_4d_once(void *dst, const CUtensorMap *map, int x, int y, int z, int w, uint64_t *bar,
+                                                 uint64_t policy) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint "
+        "[%0], [%1, {%2, %3, %4, %5}], [%6], %7;"
+        :: "r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))), "l"(reinterpret_cast<uint64_t>(map)), "r"(x),
+           "r"(y), "r"(z), "r"(w), "r"(static_cast<uint32_t>(__cvta_generic_to_shared(bar))), "l"(policy)
+        : "memory");
+}
 // Tiled 2-D tensor store of the box at (x, y) from shared memory at src, in the
 // thread's bulk async-group (the caller commits it).  Out-of-range parts of the
 // box are not written.
