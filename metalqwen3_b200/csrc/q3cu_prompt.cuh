@@ -276,17 +276,21 @@ __device__ __forceinline__ void q8_tile(const uint8_t *raw, uint8_t *to, int row
     const int lane = threadIdx.x & 31, key0 = int(threadIdx.x >> 5 & 3) * 32 + (lane & 7);
     const float *scales = reinterpret_cast<const float *>(raw + PT_KEYS * HD);
     const float up = __uint_as_float(uint32_t(e + 127) << 23);
+    uint4 v[4][2];                                           // codes 16 ch .., ch = lane / 8 and 4 further, of rows key0 + 8 i
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+            v[i][half] = *reinterpret_cast<const uint4 *>(raw + (key0 + 8 * i) * HD + ((((lane >> 3) + 4 * half) ^ (key0 & 7)) << 4));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int key = key0 + 8 * i;
         const float2 sc = *reinterpret_cast<const float2 *>(scales + 2 * key);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-            const int ch = (lane >> 3) + 4 * half;           // codes 16 ch ..
             const float s = key < rows ? (half ? sc.y : sc.x) * up : 0.0f;
             const uint32_t s2 = pack_f16(s, s);
-            const uint4 v = *reinterpret_cast<const uint4 *>(raw + key * HD + ((ch ^ (key & 7)) << 4));
-            const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+            const uint32_t words[4] = {v[i][half].x, v[i][half].y, v[i][half].z, v[i][half].w};
             uint32_t w[8];
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
@@ -819,8 +823,9 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {                    // 32 probabilities at a time; two halves are handed over
                     uint32_t w[16];
-                    // Q8_0: the last 32 scores are read a second time rather than kept (registers)
-                    if constexpr (Q8) {
+                    // Q8_0: the last 32 scores are read a second time rather than kept, where registers are short (prompts:
+                    // 296 us without for the chunks of 243)
+                    if constexpr (Q8 && !SHARED) {
                         if (x == 2) tc_ld32(ts + 96, u + 96);
                         if (x == 3) {
                             tc_wait_ld32(u + 96);

@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from test_gpu_kv_forms import I8, Quantised
-from test_gpu_paged import BF16, F32, H, Paged, queries
+from test_gpu_paged import BF16, F32, H, Paged, attend, queries
 from test_gpu_paged_q8 import check_attention, rounded
 
 pytestmark = pytest.mark.gpu
@@ -53,6 +53,15 @@ class Shared:
             check_attention(got[s:s + 1], q[s:s + 1], *self.rows(s), [self.lens[s]], BF16, H)
 
 
+def check_average(sh, got, q):
+    """The root mean square of all errors.  Rounding the result and the probabilities to bf16 moves each by up to 2^-8 of
+    itself, and if evenly spread by 2^-8 / sqrt(3) on average: the two together by 2^-8 sqrt(2 / 3) = 0.0032 of the results'
+    average where, as here, probabilities and values are independent; the rest is far below.  A key too many or too few
+    among a thousand shows."""
+    want = torch.cat([attend(q[s:s + 1].double(), *sh.rows(s), [n])[0] for s, n in enumerate(sh.lens)])
+    assert (got.double() - want).pow(2).mean().sqrt() <= 0.0033 * want.pow(2).mean().sqrt() + 1e-30
+
+
 CASES = [
     # groups of (sequences, shared positions); positions behind them
     (32, 8, 64, [(5, 700)], [1, 90, 64, 33, 7]),
@@ -81,6 +90,7 @@ def test_attention_shared(q3, q8, heads, n_kv, page, groups, own):
     if any(n == 1 and s for n, s in groups):    # a sequence alone attends to its own pages, which are all there
         assert int(sh.p.table[0, 0]) >= 0
     sh.check(out, q)
+    check_average(sh, out, q)
 
 
 @pytest.mark.parametrize("q8", [False, True])
