@@ -100,9 +100,27 @@ __device__ __forceinline__ void store_q8(void *base, int64_t at, float *scale, i
     const Q8Scale g0 = q8_prepare(__uint_as_float(__reduce_max_sync(FULL, __float_as_uint(low))));
     const Q8Scale g1 = q8_prepare(__uint_as_float(__reduce_max_sync(FULL, __float_as_uint(high))));
     const Q8Scale gl = lo < GS ? g0 : g1, gh = hi < GS ? g0 : g1;
+    // the fast codes of q8_encode_lane, a pair at a time; a lane near a tie, or of an exact group, does its four again
+    uint32_t code[2];
+    bool fix = gl.exact || gh.exact;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float inv = i ? gh.inv : gl.inv;
+        const f2 magic = pk2(12582912.0f, 12582912.0f), q = mul2(i ? pk2(h.x, h.y) : pk2(l.x, l.y), pk2(inv, inv));
+        const f2 t = add2(q, magic), d = sub2(q, sub2(t, magic));
+        float d0, d1, t0, t1;
+        up2(d, d0, d1);
+        up2(t, t0, t1);
+        fix |= !(fabsf(d0) <= 0.49993896484375f) | !(fabsf(d1) <= 0.49993896484375f);
+        code[i] = __byte_perm(__float_as_uint(t0), __float_as_uint(t1), 0x0040);
+    }
+    if (__builtin_expect(fix, 0)) {
+        code[0] = q8_code_slow(l.x, gl.scale) | q8_code_slow(l.y, gl.scale) << 8;
+        code[1] = q8_code_slow(h.x, gh.scale) | q8_code_slow(h.y, gh.scale) << 8;
+    }
     uint8_t *p = static_cast<uint8_t *>(base) + at;
-    *reinterpret_cast<uint16_t *>(p + lo) = uint16_t(q8_code_g(l.x, gl) | q8_code_g(l.y, gl) << 8);
-    *reinterpret_cast<uint16_t *>(p + hi) = uint16_t(q8_code_g(h.x, gh) | q8_code_g(h.y, gh) << 8);
+    *reinterpret_cast<uint16_t *>(p + lo) = uint16_t(code[0]);
+    *reinterpret_cast<uint16_t *>(p + hi) = uint16_t(code[1]);
     if ((threadIdx.x & 31) == 0) *reinterpret_cast<float2 *>(scale) = make_float2(g0.scale, g1.scale);
 }
 
@@ -185,9 +203,9 @@ kv_append_kernel(const PagedKV c, const PagedSeqs b, int rows, const typename El
         if (e < heads * HD) prefetch_l2((x < qn ? qr : x < qn + kn ? kr : vr) + e);
     }
 
-    const int s = paged_seq_of_warp(b, r);
+    int pos;
+    const int s = paged_row_of_warp(b, c, r, pos, status);
     if (s < 0) return;                                       // a row behind the last sequence
-    const int pos = paged_pos(b, c, s, r, lane == 0 ? status : nullptr);
     if (pos < 0) return;                                     // padding, or beyond the table
     const int page = last > qn ? paged_page(b, c, s, pos, lane == 0 ? status : nullptr) : -1;
     const Place<WHOLE> place(lane, form.dim, form.pairs);
@@ -281,63 +299,79 @@ cudaError_t launch_kv_append(const PagedKV &c, q3cu_dtype cache_dt, const PagedS
 
 // ---- reading rows back ------------------------------------------------------------------------
 // The rows' keys and values as they are in the cache (Q8_0: code times scale), dense.  Bound by memory: a warp takes one
-// row, or with few rows a part of its heads, READ_HEADS heads of k or of v at a time; a lane holds four
-// consecutive elements of a head.
+// row, or with few rows a part of its heads, READ_HEADS heads of k or of v at a time; a lane stores 16 bytes of a head, so
+// that 32 lanes hold one head of an f32 result or two of a bf16 one.
 constexpr int READ_HEADS = 8;
 template <AppendAs CA, AppendAs AS>
-__device__ __forceinline__ void read_heads(const void *from, const float *scale, int64_t at, int64_t step, int n, bool there,
-                                           void *to) {
-    const int lane = threadIdx.x & 31;
-    float4 x[READ_HEADS];
-    uint32_t code[READ_HEADS];
-    float s[READ_HEADS];
+__device__ __forceinline__ void read_heads(const void *pool, const float *scales, int64_t at, int64_t scale_at, int64_t step, int n,
+                                           bool there, void *to) {
+    constexpr int VEC = AS == AS_BF16 ? 8 : 4, SIDE = VEC / 4, LANES = HD / VEC;         // elements of a lane, heads at once
+    typedef typename std::conditional<CA == AS_Q8, uint8_t, typename std::conditional<CA == AS_BF16, uint16_t, float>::type>::type E;
+    const int lane = threadIdx.x & 31, mine = SIDE == 2 ? lane / LANES : 0, e = lane % LANES * VEC;
+    const E *from = static_cast<const E *>(pool) + at + mine * step + e;
+    const float *scale = scales + scale_at + mine * (step / GS) + e / GS;
+    constexpr int N = READ_HEADS / SIDE;
+    float4 x[N][SIDE];
+    uint32_t code[N][SIDE];
+    float s[N];
 #pragma unroll
-    for (int i = 0; i < READ_HEADS; ++i) {
-        x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        code[i] = 0;
+    for (int i = 0; i < N; ++i) {
+#pragma unroll
+        for (int y = 0; y < SIDE; ++y) x[i][y] = make_float4(0.0f, 0.0f, 0.0f, 0.0f), code[i][y] = 0x80808080u;
         s[i] = 0.0f;
-        if (i >= n || !there) continue;
-        const int64_t e = at + i * step + 4 * lane;
+        if (SIDE * i + mine >= n || !there) continue;
+        const E *p = from + SIDE * i * step;
         if constexpr (CA == AS_Q8) {
-            code[i] = *reinterpret_cast<const uint32_t *>(static_cast<const uint8_t *>(from) + e);
-            s[i] = scale[i * (step / GS) + (lane >> 4)];
-        } else if constexpr (CA == AS_BF16) {
-            x[i] = load_quad(static_cast<const uint16_t *>(from) + e);
+            if constexpr (SIDE == 2) {
+                const uint2 w = *reinterpret_cast<const uint2 *>(p);
+                code[i][0] = w.x, code[i][1] = w.y;
+            } else {
+                code[i][0] = *reinterpret_cast<const uint32_t *>(p);
+            }
+            s[i] = scale[SIDE * i * (step / GS)];
         } else {
-            x[i] = load_quad(static_cast<const float *>(from) + e);
+#pragma unroll
+            for (int y = 0; y < SIDE; ++y) x[i][y] = load_quad(p + 4 * y);
         }
     }
 #pragma unroll
-    for (int i = 0; i < READ_HEADS; ++i) {
-        if (i >= n) continue;
+    for (int i = 0; i < N; ++i) {
+        if (SIDE * i + mine >= n) continue;
         if constexpr (CA == AS_Q8) {
-            const float4 y = q8_floats(code[i]);
-            if (there) x[i] = make_float4(s[i] * y.x, s[i] * y.y, s[i] * y.z, s[i] * y.w);
+            if (there)
+#pragma unroll
+                for (int y = 0; y < SIDE; ++y) {
+                    const float4 f = q8_floats(code[i][y]);
+                    x[i][y] = make_float4(s[i] * f.x, s[i] * f.y, s[i] * f.z, s[i] * f.w);
+                }
         }
-        if constexpr (AS == AS_BF16) store_quad(static_cast<uint16_t *>(to) + i * HD + 4 * lane, x[i]);
-        else store_quad(static_cast<float *>(to) + i * HD + 4 * lane, x[i]);
+        if constexpr (SIDE == 2)
+            *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(to) + (SIDE * i + mine) * HD + e) =
+                make_uint4(pack_bf16(x[i][0].x, x[i][0].y), pack_bf16(x[i][0].z, x[i][0].w), pack_bf16(x[i][1].x, x[i][1].y),
+                           pack_bf16(x[i][1].z, x[i][1].w));
+        else store_quad(static_cast<float *>(to) + i * HD + e, x[i][0]);
     }
 }
 
 template <AppendAs CA, AppendAs AS>
-__global__ void __launch_bounds__(APPEND_WARPS * 32)
+__global__ void __launch_bounds__(APPEND_WARPS * 32, 8)
 kv_read_kernel(const PagedKV c, const PagedSeqs b, int rows, void *k, void *v, int64_t kv_stride, uint32_t *status) {
     griddep_wait();
     const int lane = threadIdx.x & 31, r = int(blockIdx.x) * APPEND_WARPS + int(threadIdx.x >> 5);
     if (r >= rows) return;
-    const int s = paged_seq_of_warp(b, r);
+    int pos;
+    const int s = paged_row_of_warp(b, c, r, pos, status);
     if (s < 0) return;                                       // a row behind the last sequence
-    const int pos = paged_pos(b, c, s, r, lane == 0 ? status : nullptr);
     const int page = pos < 0 ? -1 : paged_page(b, c, s, pos, lane == 0 ? status : nullptr);
     const int64_t step = HD << c.page_shift, at = page < 0 ? 0 : paged_at(c, page, 0, pos);
-    const int64_t sc = page < 0 ? 0 : int64_t(page) * c.scale_stride + 2 * (pos & ((1 << c.page_shift) - 1));
+    const int64_t sc = page < 0 || CA != AS_Q8 ? 0 : paged_scale_at(c, page, 0, pos);
     const int n = (c.n_kv + READ_HEADS - 1) / READ_HEADS;    // batches of k, and of v
     const int first = int(int64_t(2 * n) * blockIdx.y / gridDim.y), last = int(int64_t(2 * n) * (blockIdx.y + 1) / gridDim.y);
     constexpr int BYTES = AS == AS_BF16 ? 2 : 4;
     for (int x = first; x < last; ++x) {
         const bool side = x >= n;
         const int u = (side ? x - n : x) * READ_HEADS;
-        read_heads<CA, AS>(side ? c.v : c.k, (side ? c.v_scale : c.k_scale) + (sc + u * (step / GS)), at + u * step, step,
+        read_heads<CA, AS>(side ? c.v : c.k, side ? c.v_scale : c.k_scale, at + u * step, sc + u * (step / GS), step,
                            c.n_kv - u, page >= 0, static_cast<uint8_t *>(side ? v : k) + (r * kv_stride + u * HD) * BYTES);
     }
 }

@@ -117,6 +117,30 @@ __host__ __device__ __forceinline__ int paged_pos(const PagedSeqs &b, const Page
     return -1;
 }
 
+// Sequence and position of packed row r (as paged_seq_of_warp and paged_pos find them) by a whole warp: for up to 31
+// sequences one round of loads in place of two.
+__device__ __forceinline__ int paged_row_of_warp(const PagedSeqs &b, const PagedKV &c, int64_t r, int &pos, uint32_t *status) {
+    const int lane = threadIdx.x & 31;
+    int s;
+    if (b.n_seqs < 32) {
+        const int off = b.row_off[min(lane, b.n_seqs)], len = b.kv_len[min(lane, b.n_seqs - 1)];
+        const unsigned below = __ballot_sync(FULL, off <= r && lane < b.n_seqs);
+        s = below ? 31 - __clz(below) : 0;
+        const int end = __shfl_sync(FULL, off, s + 1), n = __shfl_sync(FULL, len, s);
+        if (!below || r >= end) return -1;
+        const int64_t p = int64_t(n) - end + r;
+        pos = p < 0 ? -1 : int(min(p, int64_t(INT32_MAX)));
+        if (p >= int64_t(b.max_pages) << c.page_shift) {
+            if (lane == 0) flag_bad_index(status);
+            pos = -1;
+        }
+        return s;
+    }
+    s = paged_seq_of_warp(b, r);
+    if (s >= 0) pos = paged_pos(b, c, s, r, lane == 0 ? status : nullptr);
+    return s;
+}
+
 // Keys that packed row r of sequence s attends to: the positions up to its own, as far as the sequence holds them
 // (`len` of paged_len).
 __host__ __device__ __forceinline__ int paged_seen(const PagedSeqs &b, int s, int64_t r, int len) {
