@@ -89,7 +89,9 @@ paged_q8_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
         dead = 0;
     }
     __syncthreads();
-    griddep_wait();
+    // Tails do not wait for the launch before, whose results they do not need: it began behind the plan's, and what is older.
+    // The first CTA waits for it at its end, since the launch behind waits for this grid alone.
+    if constexpr (!Seqs::TAILS) griddep_wait();
     griddep_launch_dependents();
 
     PagedCut cut(0, 1);
@@ -100,7 +102,10 @@ paged_q8_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
         if (b.kv_len[s] <= 0 || b.max_pages == 0)
             for (int i = threadIdx.x; i < n_heads * (HD / 4); i += PQ_THREADS)
                 store_quad(out + int64_t(s) * n_heads * HD + 4 * i, make_float4(0.0f, 0.0f, 0.0f, 0.0f));
-    if (u0 == u1) return;
+    if (u0 == u1) {
+        if (Seqs::TAILS && blockIdx.x == 0) griddep_wait();
+        return;
+    }
 
     if (warp == PQ_WARPS) {
         // ---- fetch: lane = box (codes of K or V, or their scales; rows of one page) --------
@@ -136,6 +141,7 @@ paged_q8_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
         }
         // no copy outlives the CTA (bounded)
         for (int d = e > PQ_NS ? e - PQ_NS : 0; d < e; ++d) mbar_wait(&full[d % PQ_NS], uint32_t(d / PQ_NS) & 1u, nullptr);
+        if (Seqs::TAILS && blockIdx.x == 0) griddep_wait();
         return;
     }
 

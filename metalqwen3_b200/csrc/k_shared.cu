@@ -2,13 +2,16 @@
 // positions: those are attended to once for the whole group.
 //
 // Query head h of sequence s: o = sum_t softmax_t(q . k_t / sqrt(128)) v_t over its kv_len positions, the first len[g] of
-// which lie on the pages of the group's first sequence.  Three launches, joined by the softmax's maxima and sums:
+// which lie on the pages of the group's first sequence.  Four launches, joined by the softmax's maxima and sums:
 //
+//   plan              one CTA: which groups share something, and how the work of the others is cut.  Lengths and groups are
+//                     read here and by no launch behind, so that a captured step can be replayed while they change.
 //   shared positions  the tensor-core kernel of k_prompt.cu (q3cu_prompt.cuh, PT_SHARED) with sequences in the place of
 //                     prompt rows: row r of a tile is sequence r / g, head r % g of the g query heads of a kv head, and
 //                     all rows see the same keys.  The units are key tiles (128 positions) of (group, kv head, block of
 //                     two row tiles), cut into one equal run per SM.
 //   own positions     the first kernel of one-token attention (k_paged.cu, k_paged_q8.cu), over positions len[g] and up.
+//                     It does not wait for the launch before: its CTAs take the SMs as those finish.
 //   join              shared_join_kernel: a warp per (sequence, head) adds the parts,
 //                     o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i.
 //
@@ -27,11 +30,10 @@ shared_join_kernel(const SharedOut sh, const PagedKV c, const TailSeqs b, const 
                    int shared_runs, int tail_runs, const float *part, const float *tails, uint16_t *out) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int s = int(blockIdx.x / unsigned(c.n_kv)), kv = int(blockIdx.x % unsigned(c.n_kv));
-    // Before the wait: the plan is older than the launch before this one, which has begun.  Runs are kept within what the
-    // workspace holds, whatever the plan says.
+    // before the wait: the plan is older than the launch before this one, which has begun
     const PagedSpan mine = b.span(c, s, nullptr);
-    const int64_t tails_before = b.before[s], tails_all = b.before[b.n_seqs], shared_all = sh.group[b.n_seqs].units;
-    const SharedGroup of = sh.group[s];
+    const int64_t tails_before = b.before[s], tails_all = b.before[b.n_seqs], shared_all = sh.plan.all->units;
+    const SharedEntry of = sh.plan.of[s];
     const int tiles = mine.tiles<TILE>();
     int tail_first = 0, tail_n = 0, shared_first = 0, shared_n = 0, slot = 0;
     bool tail_late = false, shared_late = false;             // part 0 is the second of its run
@@ -46,8 +48,8 @@ shared_join_kernel(const SharedOut sh, const PagedKV c, const TailSeqs b, const 
         const PagedCut cut(shared_all * c.n_kv, shared_runs);
         const int keys = (mine.from + PT_KEYS - 1) / PT_KEYS, at = s - of.first, block = per_block(at);
         const int64_t a = of.units * c.n_kv + (int64_t(kv) * (per_block(of.count - 1) + 1) + block) * keys;
-        shared_first = min(max(cut.run_of(a), 0), shared_runs - 1);
-        shared_n = min(max(cut.run_of(a + keys - 1), shared_first), shared_runs - 1) - shared_first + 1;
+        shared_first = cut.run_of(a);
+        shared_n = cut.run_of(a + keys - 1) - shared_first + 1;
         shared_late = a > cut.begin(shared_first);
         slot = (at - block * per_block.d) * group;
     }
@@ -101,9 +103,106 @@ shared_join_kernel(const SharedOut sh, const PagedKV c, const TailSeqs b, const 
     }
 }
 
+// ---- the plan ------------------------------------------------------------------------------------
+constexpr int SP_THREADS = 1024;
+// Inclusive sums over the CTA of two numbers of each thread; `all_x`, `all_y`: of all.
+__device__ __forceinline__ void block_prefix(int64_t &x, int &y, int64_t &all_x, int &all_y) {
+    __shared__ int64_t sum_x[32];
+    __shared__ int sum_y[32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    auto prefix = [&](int64_t &u, int &v) {
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t pu = __shfl_up_sync(FULL, u, o);
+            const int pv = __shfl_up_sync(FULL, v, o);
+            if (lane >= o) u += pu, v += pv;
+        }
+    };
+    prefix(x, y);
+    __syncthreads();                                         // the sums of a call before are read
+    if (lane == 31) sum_x[warp] = x, sum_y[warp] = y;
+    __syncthreads();
+    int64_t u = sum_x[lane];
+    int v = sum_y[lane];
+    prefix(u, v);
+    all_x = __shfl_sync(FULL, u, 31);
+    all_y = __shfl_sync(FULL, v, 31);
+    u = __shfl_sync(FULL, u, max(warp - 1, 0));
+    v = __shfl_sync(FULL, v, max(warp - 1, 0));
+    if (warp) x += u, y += v;
+}
+
+// One CTA.  Offsets that do not rise may make groups overlap, or more groups than there is room for: then those that come
+// too late, and sequences that find no entry of their own group, share nothing.
+__global__ void __launch_bounds__(SP_THREADS)
+shared_plan_kernel(const PagedGroups groups, const SharedPlan plan, const PagedKV c, const PagedSeqs b, const FastDiv per_block,
+                   int tail_tile, uint32_t *status) {
+    __shared__ int off_sh[SP_THREADS + 1];
+    griddep_wait();
+    griddep_launch_dependents();
+    const int tid = int(threadIdx.x), room = shared_entries(b.n_seqs);
+    const bool held = groups.n <= SP_THREADS;                // the offsets fit shared memory
+    const int my_len = tid < b.n_seqs ? paged_len(b, c, tid, status) : 0;    // on its way meanwhile
+    int64_t units = 0;
+    int n = 0;
+    for (int g0 = 0; g0 < groups.n; g0 += SP_THREADS) {
+        const int g = g0 + tid, shared = g < groups.n ? groups.shared(g, b, c, status) : 0;
+        if (held && g < groups.n) off_sh[g] = groups.off[g];
+        if (held && tid == 0) off_sh[groups.n] = groups.off[groups.n];
+        const int count = shared ? groups.count(g, b.n_seqs) : 0;
+        int64_t mine = shared ? int64_t((shared + PT_KEYS - 1) / PT_KEYS) * (per_block(count - 1) + 1) : 0, x = mine, all_x;
+        int one = shared > 0, y = one, all_y;
+        block_prefix(x, y, all_x, all_y);
+        const int index = n + y - one;
+        if (n + all_y > room) {                              // (the same for all threads)
+            if (index >= room) mine = 0, one = 0;
+            x = mine, y = one;
+            block_prefix(x, y, all_x, all_y);
+        }
+        if (one) {
+            const int first = groups.off[g];
+            plan.entries[index] = {first, count, shared, 0, units + x - mine};
+            plan.entry[first] = index;
+        }
+        units += all_x;
+        n += all_y;
+    }
+    if (tid == 0) *plan.all = {0, n, 0, 0, units};
+    __syncthreads();
+    int64_t sum = 0;
+    for (int s0 = 0; s0 < b.n_seqs; s0 += SP_THREADS) {
+        const int s = s0 + tid;
+        int64_t x = 0, all_x;
+        int y = 0, all_y;
+        if (s < b.n_seqs) {
+            const int len = s0 ? paged_len(b, c, s, status) : my_len;
+            int from = 0;
+            const PagedGroups near{held ? off_sh : groups.off, groups.len, groups.n};
+            const int g = n ? near.of(s, b.n_seqs) : -1;
+            if (g >= 0) {
+                const int first = near.off[g], count = near.count(g, b.n_seqs), index = count > 1 ? plan.entry[first] : -1;
+                if (index >= 0 && index < n) {
+                    const SharedEntry e = plan.entries[index];
+                    if (e.first == first && e.count == count && len >= e.len) {      // one that holds fewer attends by itself
+                        from = e.len;
+                        plan.of[s] = e;
+                    }
+                }
+            }
+            plan.spans[s] = make_int2(from, len);
+            if (len > from) x = TAIL_LEAD + (len + tail_tile - 1) / tail_tile - from / tail_tile;
+        }
+        const int64_t mine = x;
+        block_prefix(x, y, all_x, all_y);
+        if (s < b.n_seqs) plan.before[s] = sum + x - mine;
+        sum += all_x;
+    }
+    if (tid == 0) plan.before[b.n_seqs] = sum;
+}
+
 // The workspace: rows of the shared positions, of whole tails, of parts of tails, then the plan.
 struct SharedWork {
-    size_t tails, part, spans, before, group, bytes;
+    size_t tails, part, spans, before, entry, entries, of, bytes;
     int slot_rows;
 };
 static SharedWork shared_work(int n_seqs, int n_heads, int n_kv, int sms) {
@@ -116,8 +215,10 @@ static SharedWork shared_work(int n_seqs, int n_heads, int n_kv, int sms) {
     w.part = w.tails + round(rows * row);
     w.spans = w.part + round(size_t(paged_runs(sms)) * 2 * group * row);
     w.before = w.spans + round(size_t(n_seqs) * sizeof(int2));
-    w.group = w.before + round((size_t(n_seqs) + 1) * sizeof(int64_t));
-    w.bytes = w.group + round((size_t(n_seqs) + 1) * sizeof(SharedGroup));
+    w.entry = w.before + round((size_t(n_seqs) + 1) * sizeof(int64_t));
+    w.entries = w.entry + round(size_t(n_seqs) * sizeof(int));
+    w.of = w.entries + round((size_t(shared_entries(n_seqs)) + 1) * sizeof(SharedEntry));       // and one for all
+    w.bytes = w.of + round(size_t(n_seqs) * sizeof(SharedEntry));
     return w;
 }
 size_t attention_shared_workspace(int n_seqs, int n_heads, int n_kv, int sms) {
@@ -154,26 +255,28 @@ cudaError_t launch_attention_shared(const PagedKV &c, q3cu_dtype cache_dt, const
     float *tails = reinterpret_cast<float *>(base + w.tails), *part = reinterpret_cast<float *>(base + w.part);
     if (n_groups == 0)                                       // (its parts fit where those of the tails would lie)
         return launch_attention_paged(c, cache_dt, b, q, Q3CU_BF16, q_stride, n_heads, part, out, status, stream, sms);
-    const SharedOut sh{PagedGroups{off, len, n_groups},
-                       reinterpret_cast<float *>(base),
-                       w.slot_rows,
-                       reinterpret_cast<int2 *>(base + w.spans),
-                       reinterpret_cast<int64_t *>(base + w.before),
-                       reinterpret_cast<SharedGroup *>(base + w.group),
-                       cache_dt == Q3CU_Q8_0 ? PD_TAIL_Q8 : PD_TAIL_BF16};
+    SharedEntry *entries = reinterpret_cast<SharedEntry *>(base + w.entries);
+    const SharedPlan plan{reinterpret_cast<int2 *>(base + w.spans), reinterpret_cast<int64_t *>(base + w.before),
+                          reinterpret_cast<int *>(base + w.entry), entries, reinterpret_cast<SharedEntry *>(base + w.of),
+                          entries + shared_entries(b.n_seqs)};
+    const SharedOut sh{plan, reinterpret_cast<float *>(base), w.slot_rows};
     TailSeqs seqs;
     static_cast<PagedSeqs &>(seqs) = b;
-    seqs.spans = sh.spans;
-    seqs.before = sh.before;
+    seqs.spans = plan.spans;
+    seqs.before = plan.before;
     const bool q8 = cache_dt == Q3CU_Q8_0;
-    cudaError_t e = q8 ? launch_prefixes<true>(sh, c, b, q, q_stride, n_heads, status, stream, sms)
-                       : launch_prefixes<false>(sh, c, b, q, q_stride, n_heads, status, stream, sms);
+    const FastDiv per_block(2 * (PT_ROWS / group));
+    cudaError_t e = launch_dependent(shared_plan_kernel, dim3(1), dim3(SP_THREADS), 0, stream, PagedGroups{off, len, n_groups},
+                                     plan, c, b, per_block, q8 ? PD_TAIL_Q8 : PD_TAIL_BF16, status);
+    if (e != cudaSuccess) return e;
+    e = q8 ? launch_prefixes<true>(sh, c, b, q, q_stride, n_heads, status, stream, sms)
+           : launch_prefixes<false>(sh, c, b, q, q_stride, n_heads, status, stream, sms);
     if (e != cudaSuccess) return e;
     e = (q8 ? launch_tails_q8 : launch_tails_bf16)(c, seqs, q, q_stride, n_heads, part, tails, out, status, stream, runs);
     if (e != cudaSuccess) return e;
     auto *join = q8 ? shared_join_kernel<PD_TAIL_Q8> : shared_join_kernel<PD_TAIL_BF16>;
     return launch_dependent(join, dim3(unsigned(b.n_seqs) * unsigned(c.n_kv)), dim3(SJ_WARPS * 32), 0, stream, sh, c, seqs,
-                            FastDiv(2 * (PT_ROWS / group)), n_heads, group, sms, runs, part, tails, static_cast<uint16_t *>(out));
+                            per_block, n_heads, group, sms, runs, part, tails, static_cast<uint16_t *>(out));
 }
 
 }  // namespace q3

@@ -105,134 +105,77 @@ template <int NS> struct RingAt {
 // the shared positions have key tiles.  All units are cut into one run per CTA (PagedCut).  A run that covers all of an item
 // leaves its rows' results at row (sequence, head); one that begins or ends inside leaves them in slot 2 run, or 2 run + 1 if
 // the run began with another item, of the slots behind.
-// What the launches behind need to know of a sequence: its span, the units of the sequences before it (TailSeqs), and of its
-// group the first sequence, the number of sequences and the units of the groups before (of one kv head).
-struct SharedGroup {
-    int first, count;
+// The plan of a call, which its first launch makes (shared_plan_kernel): the groups that share something, with the units before
+// them (of one kv head), and of each sequence the span and units of its own part (TailSeqs) and its group.
+struct SharedEntry {
+    int first, count, len;   // first sequence, sequences, positions
+    int pad;
     int64_t units;
 };
+struct SharedPlan {
+    int2 *spans;             // [n_seqs]
+    int64_t *before;         // [n_seqs + 1]
+    int *entry;              // [n_seqs]: the entry whose first sequence it is
+    SharedEntry *entries;    // [shared_entries(n_seqs)]
+    SharedEntry *of;         // [n_seqs]: the entry of a sequence (where its span begins behind 0)
+    SharedEntry *all;        // count: the entries; units: of all
+};
+__host__ __device__ __forceinline__ int shared_entries(int n_seqs) { return n_seqs / 2 + 1; }
 struct SharedOut {
-    PagedGroups groups;
+    SharedPlan plan;
     float *rows;             // of SHARED_ROW floats: [n_seqs][n_heads], then [runs][2][slot_rows]
     int slot_rows;
-    int2 *spans;             // the plan
-    int64_t *before;
-    SharedGroup *group;      // [n_seqs + 1], the last with the units of all groups
-    int tail_tile;           // positions of a tile of the sequences' own part
 };
 struct SharedWalk {
-    int g, head, block, tile, len, tiles, blocks;            // blocks of the group's sequences
-    __device__ __forceinline__ void enter(const SharedOut &sh, const PagedSeqs &b, const PagedKV &c, const FastDiv &per_block) {
-        len = sh.groups.shared(g, b, c, nullptr);
-        tiles = (len + PT_KEYS - 1) / PT_KEYS;
-        blocks = tiles ? per_block(sh.groups.count(g, b.n_seqs) - 1) + 1 : 0;
-    }
-    // units of group g, in tiles of one kv head
-    static __device__ __forceinline__ int64_t units(const SharedOut &sh, const PagedSeqs &b, const PagedKV &c,
-                                                    const FastDiv &per_block, int g, uint32_t *status) {
-        const int n = g < sh.groups.n ? sh.groups.shared(g, b, c, status) : 0;
-        return n ? int64_t((n + PT_KEYS - 1) / PT_KEYS) * (per_block(sh.groups.count(g, b.n_seqs) - 1) + 1) : 0;
+    SharedEntry e;
+    int index, head, block, tile, tiles, blocks;             // index of the entry, tiles of its positions, blocks of its sequences
+    __device__ __forceinline__ void enter(const FastDiv &per_block) {
+        tiles = (e.len + PT_KEYS - 1) / PT_KEYS;
+        blocks = per_block(e.count - 1) + 1;
     }
 };
-__device__ __forceinline__ int64_t warp_prefix64(int64_t x) {                // inclusive sum over the lanes
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int64_t y = __shfl_up_sync(FULL, x, o);
-        if ((threadIdx.x & 31) >= o) x += y;
-    }
-    return x;
-}
 // A run's units [u, u1) of all, and the place of u (one warp; every lane returns it).
-__device__ __forceinline__ SharedWalk shared_run(const SharedOut &sh, const PagedSeqs &b, const PagedKV &c,
-                                                 const FastDiv &per_block, int run, int runs, int64_t &u, int64_t &u1) {
-    const int lane = threadIdx.x & 31;
+__device__ __forceinline__ SharedWalk shared_run(const SharedPlan &plan, const PagedKV &c, const FastDiv &per_block, int n_seqs,
+                                                 int run, int runs, int64_t &u, int64_t &u1) {
+    const int lane = threadIdx.x & 31, room = shared_entries(n_seqs);
+    const SharedEntry all = *plan.all;
+    SharedEntry mine = plan.entries[min(lane, room - 1)];    // under way together
     SharedWalk w = {};
-    int64_t total = 0, x = 0, end = 0;
-    for (int g0 = 0; g0 < sh.groups.n; g0 += 32) {
-        x = SharedWalk::units(sh, b, c, per_block, g0 + lane, nullptr);
-        end = warp_prefix64(x);
-        total += __shfl_sync(FULL, end, 31);
-    }
-    const PagedCut cut(total * c.n_kv, runs);
+    const PagedCut cut(all.units * c.n_kv, runs);
     u = cut.begin(run);
     u1 = cut.begin(run + 1);
     if (u == u1) return w;
-    int64_t left = u;
-    for (int g0 = 0; g0 < sh.groups.n; g0 += 32) {
-        if (sh.groups.n > 32) {                              // otherwise the lanes still hold them
-            x = SharedWalk::units(sh, b, c, per_block, g0 + lane, nullptr);
-            end = warp_prefix64(x);
-        }
-        const unsigned hit = __ballot_sync(FULL, left < end * c.n_kv);
-        if (hit) {
-            const int l = __ffs(hit) - 1;
-            w.g = g0 + l;
-            w.enter(sh, b, c, per_block);
-            const int64_t at = left - __shfl_sync(FULL, end - x, l) * c.n_kv, item = quot(at, w.tiles);
-            w.tile = int(at - item * w.tiles);
-            w.head = int(quot(item, w.blocks));
-            w.block = int(item - int64_t(w.head) * w.blocks);
-            return w;
-        }
-        left -= __shfl_sync(FULL, end, 31) * c.n_kv;
+    for (int i0 = 0; i0 < all.count; i0 += 32) {
+        if (i0) mine = plan.entries[min(i0 + lane, room - 1)];
+        const unsigned hit = __ballot_sync(FULL, i0 + lane < all.count && mine.units * c.n_kv <= u);
+        const int64_t end = i0 + 32 < all.count ? plan.entries[i0 + 32].units : all.units;
+        if (u >= end * c.n_kv) continue;
+        const int l = 31 - __clz(hit);                       // the last that begins at or before u
+        w.index = i0 + l;
+        w.e.first = __shfl_sync(FULL, mine.first, l);
+        w.e.count = __shfl_sync(FULL, mine.count, l);
+        w.e.len = __shfl_sync(FULL, mine.len, l);
+        w.enter(per_block);
+        const int64_t at = u - __shfl_sync(FULL, mine.units, l) * c.n_kv, item = quot(at, w.tiles);
+        w.tile = int(at - item * w.tiles);
+        w.head = int(quot(item, w.blocks));
+        w.block = int(item - int64_t(w.head) * w.blocks);
+        return w;
     }
+    u = u1;
     return w;
 }
-// To the item behind (one warp: 32 groups at a time).
-__device__ __forceinline__ void shared_next(const SharedOut &sh, const PagedSeqs &b, const PagedKV &c, const FastDiv &per_block,
-                                            SharedWalk &w) {
+// To the item behind.
+__device__ __forceinline__ void shared_next(const SharedPlan &plan, const PagedKV &c, const FastDiv &per_block, SharedWalk &w) {
     w.tile = 0;
     if (++w.block < w.blocks) return;
     w.block = 0;
     if (++w.head < c.n_kv) return;
     w.head = 0;
-    for (++w.g; w.g < sh.groups.n; w.g += 32) {
-        const int g = w.g + int(threadIdx.x & 31);
-        const unsigned some = __ballot_sync(FULL, SharedWalk::units(sh, b, c, per_block, g, nullptr) > 0);
-        if (some) {
-            w.g += __ffs(some) - 1;
-            w.enter(sh, b, c, per_block);
-            return;
-        }
-    }
+    w.e = plan.entries[++w.index];
+    w.enter(per_block);
 }
-// The plan for the launches behind, by one warp beside the products of its CTA.  (A group's units are left with its first
-// sequence, from where the others take them.  With offsets that do not rise, groups may overlap: then what is found
-// here is of no use, but the launches behind stay within the workspace.)
-__device__ __forceinline__ void shared_plan(const SharedOut &sh, const PagedSeqs &b, const PagedKV &c, const FastDiv &per_block,
-                                            uint32_t *status) {
-    const int lane = threadIdx.x & 31;
-    int64_t total = 0;
-    for (int g0 = 0; g0 < sh.groups.n; g0 += 32) {
-        const int64_t x = SharedWalk::units(sh, b, c, per_block, g0 + lane, status), end = warp_prefix64(x);
-        if (x) sh.group[sh.groups.off[g0 + lane]].units = total + end - x;
-        total += __shfl_sync(FULL, end, 31);
-    }
-    if (lane == 0) sh.group[b.n_seqs].units = total;
-    __syncwarp();
-    int64_t sum = 0;
-    for (int s0 = 0; s0 < b.n_seqs; s0 += 32) {
-        const int s = s0 + lane;
-        uint32_t units = 0;
-        if (s < b.n_seqs) {
-            const int len = paged_len(b, c, s, status), g = sh.groups.of(s, b.n_seqs);
-            int from = g < 0 ? 0 : sh.groups.shared(g, b, c, nullptr);
-            if (len < from) from = 0;                        // one that holds fewer attends by itself
-            if (from) {
-                const int first = sh.groups.off[g];
-                sh.group[s].first = first;
-                sh.group[s].count = sh.groups.count(g, b.n_seqs);
-                if (s != first) sh.group[s].units = sh.group[first].units;
-            }
-            sh.spans[s] = make_int2(from, len);
-            if (len > from) units = uint32_t(TAIL_LEAD + (len + sh.tail_tile - 1) / sh.tail_tile - from / sh.tail_tile);
-        }
-        const uint32_t end = warp_prefix(units);
-        if (s < b.n_seqs) sh.before[s] = sum + (end - units);
-        sum += __shfl_sync(FULL, end, 31);
-    }
-    if (lane == 0) sh.before[b.n_seqs] = sum;
-}
+
 struct NoOrder {             // in place of a PromptOrder
     __device__ __forceinline__ NoOrder(const PagedSeqs &, const PagedKV &, int, const FastDiv &, int, uint32_t *) {}
     __device__ __forceinline__ PromptItem find(int64_t) { return {}; }
@@ -439,22 +382,22 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                 if constexpr (SHARED) {
                     if (u == u1) return;
                     const int tiles = int(min(int64_t(walk.tiles - walk.tile), u1 - u));
-                    it.s = it.base = sh.groups.off[walk.g];
+                    it.s = it.base = walk.e.first;
                     it.head = walk.head;
-                    it.rows = sh.groups.count(walk.g, b.n_seqs);
+                    it.rows = walk.e.count;
                     it.first = walk.block * 2 * qt;
-                    it.len = walk.len;
+                    it.len = walk.e.len;
                     it.pos0 = 0;
                     it.j0 = walk.tile;
                     for (int t = 0; t < 2; ++t) it.nt[t] = it.first + t * qt < it.rows ? tiles : 0;
                     it.dst = tiles == walk.tiles ? -1 : (2 * int64_t(blockIdx.x) + (fragment > 0)) * sh.slot_rows;
                     ++fragment;
                     u += tiles;
-                    if (u < u1) shared_next(sh, b, c, per_block, walk);
+                    if (u < u1) shared_next(sh.plan, c, per_block, walk);
                 }
             };
             if constexpr (SHARED) {
-                walk = shared_run(sh, b, c, per_block, int(blockIdx.x), int(gridDim.x), u, u1);
+                walk = shared_run(sh.plan, c, per_block, b.n_seqs, int(blockIdx.x), int(gridDim.x), u, u1);
             }
             typedef typename std::conditional<SHARED, NoOrder, PromptOrder>::type Order;
             Order order(b, c, rows, per_block, PT_KEYS, status);
@@ -702,8 +645,6 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                     ++entries;
                 }
             }
-        } else if (SHARED && warp == 11) {
-            if (blockIdx.x == 0) shared_plan(sh, b, c, per_block, status);
         } else if (!Q8 && warp == 10) {
             // ---- values behind a sequence's end: zeros -----------------------------------------
             Round it;

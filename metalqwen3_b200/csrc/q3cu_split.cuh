@@ -72,7 +72,7 @@ struct PagedGroups {
         return n > 0 && count(lo, n_seqs) > 0 && off[lo] <= s && s < off[lo + 1] ? lo : -1;
     }
 };
-// The batch's sequences behind what they share, as the launch before this one planned them (SharedPlan).  A (sequence, head) of
+// The batch's sequences behind what they share, as a launch before this one planned them (SharedPlan).  A (sequence, head) of
 // T tiles is TAIL_LEAD + T units of the cut: what it costs to begin and end one is worth about two tiles.
 constexpr int TAIL_LEAD = 2;
 constexpr int SHARED_ROW = 136;                              // floats of a row's part there: 128, maximum, sum (32-byte aligned)
