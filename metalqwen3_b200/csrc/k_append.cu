@@ -266,10 +266,15 @@ cudaError_t launch_kv_append(const PagedKV &c, q3cu_dtype cache_dt, const PagedS
                              int n_heads, const float *q_norm, const float *k_norm, const TurnFreq &freq,
                              const TurnForm &form, float eps, void *q_out, q3cu_dtype q_dt, uint32_t *status,
                              cudaStream_t stream, int sms) {
-    // A row is split over warps only while the rows alone are fewer than 32 warps per SM.
+    // A row is split over warps while the rows alone are fewer than 32 warps per SM, and so that a warp has no more than 4
+    // batches (6 of bf16 rows, whose batches are half the bytes): the warps that end last then have less to do by
+    // themselves, for the angles found once more.  Whole rows a warp: 32,000 f32 rows (32/8 heads, Q8_0) 277 against 254
+    // us, 9,000 88 against 84, 16,384 bf16 rows (bf16 cache) 82 against 72 (in threes 78); 16,384 bf16 rows (Q8_0) 109
+    // against 111.
     const int64_t all = (n_heads + APPEND_HEADS - 1) / APPEND_HEADS + (c.n_kv + APPEND_HEADS - 1) / APPEND_HEADS * 2;
     const int64_t batches = all < 65535 ? all : 65535;       // a grid's height
-    const int64_t parts = rows >= 32 * sms ? 1 : (32 * int64_t(sms) + rows - 1) / rows;
+    const int64_t most = dt == Q3CU_F32 ? 4 : 6, fill = (32 * int64_t(sms) + rows - 1) / rows, few = (batches + most - 1) / most;
+    const int64_t parts = fill > few ? fill : few;
     const dim3 grid(unsigned((rows + APPEND_WARPS - 1) / APPEND_WARPS), unsigned(parts < batches ? parts : batches));
     const bool whole = form.dim == HD && !form.pairs && form.gain == 1.0f;
     auto go = [&](auto kernel, auto *typed) {
@@ -378,7 +383,7 @@ kv_read_kernel(const PagedKV c, const PagedSeqs b, int rows, void *k, void *v, i
 
 cudaError_t launch_kv_read(const PagedKV &c, q3cu_dtype cache_dt, const PagedSeqs &b, int64_t rows, void *k, void *v,
                            q3cu_dtype dt, int64_t kv_stride, uint32_t *status, cudaStream_t stream, int sms) {
-    // a row is split over warps as above
+    // a row is split over warps while the rows alone are fewer than 32 warps per SM
     const int64_t all = 2 * ((int64_t(c.n_kv) + READ_HEADS - 1) / READ_HEADS), batches = all < 65535 ? all : 65535;
     const int64_t parts = rows >= 32 * sms ? 1 : (32 * int64_t(sms) + rows - 1) / rows;
     const dim3 grid(unsigned((rows + APPEND_WARPS - 1) / APPEND_WARPS), unsigned(parts < batches ? parts : batches));
