@@ -32,8 +32,9 @@
 // so both halves of a rotated pair are in one lane, a half row is one contiguous
 // access, and the two angles of a lane, found once, serve all its heads.  The
 // row is on its way to L2 while the warp finds its sequence, position and page.
-// 4,096 rows (32/8 heads): f32 to bf16 30.4 us, 5.0 TB/s, bf16 to bf16 24.1 us, 4.2
-// TB/s, f32 to f32 38.5 us, 5.2 TB/s; one row: 3.3 us.
+// 4,096 rows (32/8 heads): f32 to bf16 28.2 us, 5.4 TB/s, bf16 to bf16 23.6 us, 4.3
+// TB/s, f32 to f32 35.6 us, 5.7 TB/s, f32 to f32 queries and Q8_0 38 us, 4.4 TB/s (the
+// codes' instructions); one row: 3.0 us, into Q8_0 6.4 us.
 #include "q3cu_paged.cuh"
 
 #include <type_traits>
@@ -193,8 +194,11 @@ kv_append_kernel(const PagedKV c, const PagedSeqs b, int rows, const typename El
     if (r >= rows) return;
     // the row's batches: of query heads, of key heads, of value heads; this warp's are first .. last - 1
     const int qn = (n_heads + APPEND_HEADS - 1) / APPEND_HEADS, kn = (c.n_kv + APPEND_HEADS - 1) / APPEND_HEADS;
-    const int first = int(int64_t(qn + 2 * kn) * blockIdx.y / gridDim.y);
-    const int last = int(int64_t(qn + 2 * kn) * (blockIdx.y + 1) / gridDim.y);
+    // (into a Q8_0 cache the last ones, which take longest, begin first: 38 against 40 us for 4,096 rows; with a bf16 cache
+    // that order is 1 to 2 us slower)
+    const unsigned part = CA == AS_Q8 ? gridDim.y - 1 - blockIdx.y : blockIdx.y;
+    const int first = int(int64_t(qn + 2 * kn) * part / gridDim.y);
+    const int last = int(int64_t(qn + 2 * kn) * (part + 1) / gridDim.y);
     const E *qr = q + r * q_stride, *kr = k + r * kv_stride, *vr = v + r * kv_stride;
     constexpr int LINES = APPEND_HEADS * HD * int(sizeof(E)) / 128;        // 128-byte lines of a batch
     for (int i = lane + LINES * first; i < LINES * last; i += 32) {
@@ -306,6 +310,8 @@ cudaError_t launch_kv_append(const PagedKV &c, q3cu_dtype cache_dt, const PagedS
 // The rows' keys and values as they are in the cache (Q8_0: code times scale), dense.  Bound by memory: a warp takes one
 // row, or with few rows a part of its heads, READ_HEADS heads of k or of v at a time; a lane stores 16 bytes of a head, so
 // that 32 lanes hold one head of an f32 result or two of a bf16 one.
+// 8 sequences of up to 8,192 positions (8 kv heads), Q8_0 to bf16: 36 us, 4.5 TB/s (issue slots 68 % busy); a warp for k and one
+// for v 37, four heads at a time the same; 300 positions to f32: 4 us.
 constexpr int READ_HEADS = 8;
 template <AppendAs CA, AppendAs AS>
 __device__ __forceinline__ void read_heads(const void *pool, const float *scales, int64_t at, int64_t scale_at, int64_t step, int n,
