@@ -89,9 +89,10 @@ paged_q8_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
         dead = 0;
     }
     __syncthreads();
-    // Tails do not wait for the launch before, whose results they do not need: it began behind the plan's, and what is older.
-    // The first CTA waits for it at its end, since the launch behind waits for this grid alone.
-    if constexpr (!Seqs::TAILS) griddep_wait();
+    // Tails do not wait for the launch before, whose results they do not need: when it let this one begin, the plan and all that
+    // is older were complete.  The first CTA waits for it at its end, since the launch behind waits for this grid alone.
+    if constexpr (Seqs::TAILS) __threadfence();              // nothing here is read from an older copy of a line
+    else griddep_wait();
     griddep_launch_dependents();
 
     PagedCut cut(0, 1);

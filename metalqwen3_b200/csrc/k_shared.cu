@@ -30,7 +30,7 @@ shared_join_kernel(const SharedOut sh, const PagedKV c, const TailSeqs b, const 
                    int shared_runs, int tail_runs, const float *part, const float *tails, uint16_t *out) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int s = int(blockIdx.x / unsigned(c.n_kv)), kv = int(blockIdx.x % unsigned(c.n_kv));
-    // before the wait: the plan is older than the launch before this one, which has begun
+    __threadfence();                                         // before the wait: the plan was complete when the launch before began
     const PagedSpan mine = b.span(c, s, nullptr);
     const int64_t tails_before = b.before[s], tails_all = b.before[b.n_seqs], shared_all = sh.plan.all->units;
     const SharedEntry of = sh.plan.of[s];
