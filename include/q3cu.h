@@ -328,13 +328,15 @@ typedef struct {
 /* q3cu_attention_paged for a batch whose sequences share prefixes: the shared
  * positions are attended to once for the whole group, on the tensor cores.  The
  * result is that of q3cu_attention_paged over tables that list the first
- * sequence's pages for all of the group, but for the probabilities of shared positions, which
- * are rounded to bf16 (sums binary32); over a Q8_0 cache their keys and values
- * are, too.  A sequence with fewer positions than are shared, or alone in its
- * group, attends to its own pages as if it were in none; a len beyond the table sets
- * Q3CU_DEV_BAD_INDEX and is cut.  q and out are bf16, the cache bf16 or Q8_0;
- * work: 32-byte aligned, q3cu_attention_shared_workspace bytes for the batch's n_seqs (or more).  All else as
- * above. */
+ * sequence's pages for all of the group, but for the roundings of the shared
+ * positions, which are q3cu_attention_prompt's (sums binary32).  A sequence
+ * with fewer positions than are shared, or alone in its group, attends to its
+ * own pages as if it were in none; a len beyond the table sets
+ * Q3CU_DEV_BAD_INDEX and is cut.  A NaN or infinity at a shared position, where
+ * the formula makes an infinity of it, may make a NaN.  q and out are bf16, the
+ * cache bf16 or Q8_0; work: 32-byte aligned, q3cu_attention_shared_workspace
+ * bytes for the batch's n_seqs (or more), used by one call at a time.  All else
+ * as above. */
 q3cu_status q3cu_attention_shared(q3cu_ctx *ctx, const q3cu_kv_cache *cache, const q3cu_kv_batch *batch,
                                   const q3cu_kv_prefix *prefix, const void *q, q3cu_dtype dtype, int64_t q_stride,
                                   int n_heads, void *work, size_t work_bytes, void *out, q3cu_stream stream);
@@ -345,9 +347,13 @@ q3cu_status q3cu_attention_shared_workspace(q3cu_ctx *ctx, int n_seqs, int n_hea
  * keys and values already (q3cu_kv_append): a row at position p over positions
  * 0..p.  A whole prompt has kv_len equal to its rows; a chunk behind a cached
  * prefix has more.  q: [rows][n_heads][128] with q_stride elements between
- * rows; out: [rows][n_heads][128], other memory than q.  Both of the cache's type, or bf16 over a Q8_0 cache: bf16 runs on
- * the tensor cores with probabilities rounded to bf16, and a Q8_0 cache's keys and values (the sums binary32), f32 with binary32's
- * accuracy (elements below 2^-109 keep fewer bits).  Grouped heads, scale, softmax, empty rows, unused page space, bad
+ * rows; out: [rows][n_heads][128], other memory than q.  Both of the cache's
+ * type, or bf16 over a Q8_0 cache: bf16 runs on the tensor cores with
+ * probabilities rounded to bf16 (the sums binary32); over a Q8_0 cache they are
+ * rounded to f16 instead, by 2^-11 of themselves or 2^-32, and so are keys and
+ * values, by 2^-10 of themselves or 2^-39 of the largest of 128 positions; f32
+ * runs with binary32's accuracy (elements below 2^-109 keep fewer bits).
+ * Grouped heads, scale, softmax, empty rows, unused page space, bad
  * pages and alignment as above.  A NaN or infinity at a position changes no row
  * before it; where one would, the row is computed again by itself, at some 0.2 us
  * a key (a bf16 prompt does so for a second at most in one tile of rows; what is

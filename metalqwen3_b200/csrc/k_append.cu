@@ -33,8 +33,8 @@
 // access, and the two angles of a lane, found once, serve all its heads.  The
 // row is on its way to L2 while the warp finds its sequence, position and page.
 // 4,096 rows (32/8 heads): f32 to bf16 28.2 us, 5.4 TB/s, bf16 to bf16 23.6 us, 4.3
-// TB/s, f32 to f32 35.6 us, 5.7 TB/s, f32 to f32 queries and Q8_0 38 us, 4.4 TB/s (the
-// codes' instructions); one row: 3.0 us, into Q8_0 6.4 us.
+// TB/s, f32 to f32 35.6 us, 5.7 TB/s, f32 to Q8_0 (bf16 queries) 29 us, 5.0 TB/s; one
+// row: 3.0 us, into Q8_0 3.8 us.
 #include "q3cu_paged.cuh"
 
 #include <type_traits>
@@ -194,7 +194,7 @@ kv_append_kernel(const PagedKV c, const PagedSeqs b, int rows, const typename El
     if (r >= rows) return;
     // the row's batches: of query heads, of key heads, of value heads; this warp's are first .. last - 1
     const int qn = (n_heads + APPEND_HEADS - 1) / APPEND_HEADS, kn = (c.n_kv + APPEND_HEADS - 1) / APPEND_HEADS;
-    // (into a Q8_0 cache the last ones, which take longest, begin first: 38 against 40 us for 4,096 rows; with a bf16 cache
+    // (into a Q8_0 cache the last ones, which take longest, begin first: 29 against 31 us for 4,096 rows; with a bf16 cache
     // that order is 1 to 2 us slower)
     const unsigned part = CA == AS_Q8 ? gridDim.y - 1 - blockIdx.y : blockIdx.y;
     const int first = int(int64_t(qn + 2 * kn) * part / gridDim.y);

@@ -3,7 +3,8 @@
 // The operation, the split into equal runs of tiles and the join are those of
 // k_paged.cu; a key is k_i = c_i s_(i / 64) with int8 codes c and one f32 scale to
 // 64 elements, a value likewise.  Bound by memory: 136 bytes a position, kv head
-// and side, where bf16 takes 256.
+// and side, where bf16 takes 256.  64 sequences of up to 16,384 positions (32/8 heads,
+// bf16 queries): 179 us, 6.1 TB/s; one of 512 (16/8, f32 queries): 9 us, all latency.
 //
 // A CTA is one fetching warp and four computing warps around a ring of three 34 KB
 // stages, filled page by page by TMA: 128 positions' codes of K and of V (128-byte

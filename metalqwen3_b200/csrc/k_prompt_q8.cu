@@ -6,7 +6,7 @@
 // tiles are in flight where a bf16 cache has five; the codes ahead of them make up for it.
 //
 // The operands are f16: a code times its scale has more than bf16's 8 bits, and rounding keys and values to bf16 doubled the
-// error of the result (0.0039 of it against 0.0017 now, which is the result's own rounding).  f16 has 11 bits but little
+// error of the result (0.0039 of it against 0.0019 now, of which the result's own rounding is 0.0017).  f16 has 11 bits but little
 // range, so everything is lifted by powers of two:
 //   keys, values  by tile: the largest scale to [2^14, 2^15), codes as code / 128.  An element is rounded by 2^-10 of itself
 //                 (its scale and the product, 2^-11 each) and by no less than 2^-39 of the tile's largest.
@@ -18,8 +18,14 @@
 // rows that see only a part of the tile are computed again from the formula, so that a later position takes no bits from
 // an earlier row (SecondLook).
 //
-// Bound as k_prompt.cu is, and by the conversion's 1.75 instructions an element, which take an eighth of the issue slots of
-// a step.
+// Bound as k_prompt.cu is, by the chain from scores to probabilities to products, with the conversion beside it: a key tile
+// takes some 4,700 cycles (3,000 over a bf16 cache) for 2,048 of products and as many of exponentials; the conversion's 1.75
+// instructions an element are a tenth of the issue slots, a tile's conversion 1,420 cycles.  2,043 rows in four chunks
+// behind up to 8,192 positions (32/8 heads) 247 us, 714 TFLOP/s; 4,096 rows in six prompts 98 us.
+// Measured and left out (us for the chunks, against 247 or what it was at the time): a quarter of the exponentials by
+// polynomial (329 for 288; fewer of them less so), eight warps converting (410 for 240: registers), items of 32 rows less with a ring of four
+// (320 for 252), lifts by a warp of their own (267 for 247), codes read before the wait for their place (253), the lifts
+// waited for before the scores (247).
 #include "q3cu_prompt.cuh"
 
 namespace q3 {
