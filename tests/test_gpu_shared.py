@@ -1,7 +1,7 @@
 """Attention of one new token per sequence where groups of sequences share their first positions, against the formula in
 binary64.  Tolerances as in test_gpu_paged.py for bf16 prompts (a probability is rounded to bf16, 2^-8 relative, at shared
 positions; elsewhere to less) and, over a Q8_0 cache, as in test_gpu_paged_q8.py, with the shared positions' elements
-rounded to bf16 as prompts round them.  The join of the parts is one product and one sum in binary32 for each: up to 450
+rounded as prompts round them.  The join of the parts is one product and one sum in binary32 for each: up to 450
 of them, which the (n + 64) u of n positions covers, as every part has one at least."""
 import math
 
@@ -257,6 +257,94 @@ def test_far_positions_pass_32_bits(q3):
     kk, vv = (t[table[0, at // page].long(), :, at % page].double() for t in (k, v))
     for s in range(3):
         check_attention(got[s:s + 1], q[s:s + 1], kk[:lens[s]], vv[:lens[s]], [lens[s]], BF16, H)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_more_groups_than_threads(q3, q8):
+    """1,300 groups (the plan's CTA has 1,024 threads) of 2,700 sequences, many of which share nothing or hold nothing."""
+    from metalqwen3_b200.q3cu import KVPrefix
+    n = 2700
+    p = (Quantised([20] * n, 1, 16, seed=40) if q8 else Paged([20] * n, 1, 16, BF16, seed=40)).fill(41)
+    gen = torch.Generator().manual_seed(42)
+    lens = torch.randint(0, 21, (n,), generator=gen).int()
+    first = torch.arange(1301).int() * 2 + 50                 # pairs, from sequence 50 on
+    shared = torch.randint(0, 21, (1300,), generator=gen).int()
+    lead, other = first[:-1].long(), first[:-1].long() + 1
+    for t in [p.k, p.v] + ([p.ks, p.vs] if q8 else []):       # the second holds the same positions on its own pages
+        for i in range(2):
+            t[p.table[other.cuda(), i].long()] = t[p.table[lead.cuda(), i].long()]
+    p.kv_len.copy_(lens)
+    q = queries(n, 2, BF16, 43)
+    cache, batch = p.handles()
+    got = q3.attention_shared(cache, batch, KVPrefix(first.cuda(), shared.cuda()), q).double()
+    assert q3.device_status() == 0
+    want = q3.attention_paged(cache, batch, q).double()
+    empty = (lens == 0).cuda()
+    assert empty.any() and (got[empty] == 0).all() and torch.isfinite(got).all()
+    p.lens = lens.tolist()
+    group = {int(x): i // 2 for i, x in enumerate(torch.stack([lead, other], 1).flatten())}
+    active = [s for s in range(n) if s in group and 0 < shared[group[s]] <= min(lens[s], lens[lead[group[s]]])]
+    assert len(active) > 500
+    for s in active[::7]:
+        m, k, v = int(shared[group[s]]), *p.rows(s)
+        if q8:
+            k, v = (torch.cat([a[:m], b[m:]]) for a, b in zip(rounded(p, int(lead[group[s]])), (k, v)))
+        check_attention(got[s:s + 1], q[s:s + 1], k, v, [p.lens[s]], BF16, H)
+    # In no group, or in one that shares nothing: attention_paged's result, cut into other runs, so that a weight is rounded
+    # elsewhere (2^-11 in each) and the result with it (2^-8 in each).
+    alone = torch.tensor([s not in group or not shared[group[s]] for s in range(n)]).cuda()
+    top = max(float(p.rows(s)[1].abs().max()) for s in range(n) if p.lens[s])
+    assert ((got - want)[alone].abs() <= 1.01 * (2 * 2.0 ** -8 * want[alone].abs() + 4 * 2.0 ** -11 * top)).all()
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_calls_one_after_the_other(q3, q8):
+    """Calls on one workspace and one result, queries, lengths and groups changed between them by kernels of the same
+    stream, nothing waited for: each gives what it gives by itself."""
+    from metalqwen3_b200.q3cu import KVPrefix
+    sh = Shared([(6, 700), (5, 300)], [20 * i for i in range(11)], 4, 16, q8, seed=44)
+    p = sh.p
+    cache, batch = p.handles()
+    i32 = dict(dtype=torch.int32, device="cuda")
+    off, length = torch.tensor([0, 6, 11], **i32), torch.tensor([700, 300], **i32)
+    prefix = KVPrefix(off, length)
+    work = q3.attention_shared_workspace(cache, 11, 16)
+    out, q = (torch.empty((11, 16, 128), dtype=BF16, device="cuda") for _ in range(2))
+    ways = []
+    for i, (offs, lens, cut) in enumerate([([0, 6, 11], [700, 300], 0), ([0, 3, 6], [512, 700], 15), ([2, 6, 11], [1, 256], 40),
+                                           ([0, 0, 0], [5, 5], 3)]):
+        ways.append((torch.tensor(offs, **i32), torch.tensor(lens, **i32), p.kv_len - cut, queries(11, 16, BF16, 45 + i)))
+
+    def call(way):
+        for to, x in zip((off, length, p.kv_len, q), way):
+            to.copy_(x)
+        q3.attention_shared(cache, batch, prefix, q, out=out, work=work)
+        return out.clone()
+    alone = []
+    for way in ways:
+        torch.cuda.synchronize()
+        alone.append(call(way))
+    torch.cuda.synchronize()
+    got = [(i, call(ways[i])) for _ in range(30) for i in (0, 1, 2, 3, 1, 0, 2)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, alone[i]) for i, x in got)
+    assert q3.device_status() == 0
+
+
+def test_wild_groups(q3):
+    """Thousands of groups whose offsets jump about: what they share is anyone's guess, but nothing faults, and the next
+    call is right."""
+    from metalqwen3_b200.q3cu import KVPrefix
+    sh = Shared([(40, 60), (60, 33)], [3] * 100, 2, 16, False, seed=46)
+    cache, batch = sh.p.handles()
+    q = queries(100, 4, BF16, 47)
+    gen = torch.Generator().manual_seed(48)
+    for high in (101, 3, 1 << 30):
+        off = torch.randint(-2, high, (3001,), generator=gen).int().cuda()
+        length = torch.randint(-5, 64, (3000,), generator=gen).int().cuda()
+        q3.attention_shared(cache, batch, KVPrefix(off, length), q)
+    assert q3.device_status() == 0
+    sh.check(q3.attention_shared(cache, batch, sh.prefix(), q), q)
 
 
 def test_nan_and_peaked(q3):
