@@ -191,23 +191,28 @@ struct TileLift {
 // two that brings the largest finite one to [2^14, 2^15).
 __device__ __forceinline__ TileLift q8_lift(const uint8_t *raw, int rows) {
     const int lane = threadIdx.x & 31;
-    const float *scales = reinterpret_cast<const float *>(raw + PT_KEYS * HD);
-    uint32_t top = 0, low = 0x7f7fffffu;                     // of the scales that count, as bits
+    uint32_t w[8];
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-        const uint4 v = *reinterpret_cast<const uint4 *>(scales + 8 * lane + 4 * x);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        const uint4 v = *reinterpret_cast<const uint4 *>(raw + PT_KEYS * HD + 32 * lane + 16 * x);
+        w[4 * x] = v.x, w[4 * x + 1] = v.y, w[4 * x + 2] = v.z, w[4 * x + 3] = v.w;
+    }
+    if (rows < PT_KEYS)
 #pragma unroll
-        for (int y = 0; y < 4; ++y) {
-            const uint32_t m = w[y] & 0x7fffffffu;
-            const bool counts = 4 * lane + 2 * x + y / 2 < rows && m < 0x7f800000u;
-            top = counts ? max(top, m) : top;
-            low = counts && m ? min(low, m) : low;
-        }
+        for (int y = 0; y < 8; ++y)
+            if (4 * lane + y / 2 >= rows) w[y] = 0;
+    // Without its sign a binary32's bits order it, the exponent on top.  2^24 more, and no numbers wrap around to below all
+    // others; one less, and zero does to above (where no numbers are already).
+    uint32_t top = 0, low = 0xffffffffu;
+#pragma unroll
+    for (int y = 0; y < 8; ++y) {
+        top = max(top, 2 * w[y] + (1u << 24));
+        low = min(low, 2 * w[y] - 1);
     }
     top = __reduce_max_sync(FULL, top);
     low = __reduce_min_sync(FULL, low);
-    return {min(141 - int(top >> 23), 126), top && (top >> 23) - (low >> 23) > 24};
+    const int top_e = max(int(top >> 24) - 1, 0), low_e = int((low + 1) >> 24);          // (low_e: 0 without any, as is top_e)
+    return {min(141 - top_e, 126), low < 0xfeffffffu && top_e - low_e > 24};
 }
 // 128 rows' codes (128-byte swizzle) and scales at `raw` become the 32 KB f16 operand tile at `to`, by four warps: a lane
 // takes 16 codes of eight rows.  Rows from `rows` on are zeros.  The lifted scales are rounded to f16 (2^-11), code / 128 is
@@ -560,6 +565,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                                     if (ok) values(t, v.st, half, j > 0 || half > 0);
                                 }
                                 if (!ok) break;
+                                if (t == int(j < it.nt[1])) tc_commit(&empty[v.st]);         // the last to use it
                                 ++steps[t];
                                 if (j + 1 == it.nt[t]) {
                                     tc_commit(&o_full[t]);
@@ -573,7 +579,6 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                             }
                         }
                         if (!ok) break;
-                        tc_commit(&empty[v.st]);
                         if (j + 1 < nkv) {
                             tc_commit(&empty[at.st]);
                             if (j + 2 == nkv) tc_commit(&q_empty);            // the item's last scores
@@ -720,6 +725,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                 [[maybe_unused]] int shift = 0;              // of the probabilities' exponents
                 bool sink = false;
                 if constexpr (Q8) {
+                    // (after the scores' wait: before it the barrier may be phases behind, where its parity means another tile)
                     const uint32_t n = tiles + j;
                     ok = __all_sync(FULL, mbar_wait(&lifts[n & 1], n >> 1 & 1u, lane == 0 ? status : nullptr));
                     if (!ok) break;
