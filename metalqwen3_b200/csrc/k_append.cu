@@ -44,6 +44,10 @@ namespace q3 {
 __device__ __forceinline__ void prefetch_l2(const void *p) { asm volatile("prefetch.global.L2 [%0];" :: "l"(p)); }
 
 constexpr int APPEND_HEADS = 4, APPEND_WARPS = 8;
+// Where part i of `parts` (at most 65,535) begins among `all` batches; a 64-bit division takes some hundred instructions.
+__device__ __forceinline__ int part_of(int all, unsigned i, unsigned parts) {
+    return all < 65536 ? int(unsigned(all) * i / parts) : int(uint64_t(all) * i / parts);
+}
 
 // Coherent loads: q_out may be q itself (a lane reads its elements before it stores them).
 __device__ __forceinline__ float2 load_pair(const float *p) { return *reinterpret_cast<const float2 *>(p); }
@@ -197,8 +201,7 @@ kv_append_kernel(const PagedKV c, const PagedSeqs b, int rows, const typename El
     // (into a Q8_0 cache the last ones, which take longest, begin first: 29 against 31 us for 4,096 rows; with a bf16 cache
     // that order is 1 to 2 us slower)
     const unsigned part = CA == AS_Q8 ? gridDim.y - 1 - blockIdx.y : blockIdx.y;
-    const int first = int(int64_t(qn + 2 * kn) * part / gridDim.y);
-    const int last = int(int64_t(qn + 2 * kn) * (part + 1) / gridDim.y);
+    const int first = part_of(qn + 2 * kn, part, gridDim.y), last = part_of(qn + 2 * kn, part + 1, gridDim.y);
     const E *qr = q + r * q_stride, *kr = k + r * kv_stride, *vr = v + r * kv_stride;
     constexpr int LINES = APPEND_HEADS * HD * int(sizeof(E)) / 128;        // 128-byte lines of a batch
     for (int i = lane + LINES * first; i < LINES * last; i += 32) {
@@ -377,7 +380,7 @@ kv_read_kernel(const PagedKV c, const PagedSeqs b, int rows, void *k, void *v, i
     const int64_t step = HD << c.page_shift, at = page < 0 ? 0 : paged_at(c, page, 0, pos);
     const int64_t sc = page < 0 || CA != AS_Q8 ? 0 : paged_scale_at(c, page, 0, pos);
     const int n = (c.n_kv + READ_HEADS - 1) / READ_HEADS;    // batches of k, and of v
-    const int first = int(int64_t(2 * n) * blockIdx.y / gridDim.y), last = int(int64_t(2 * n) * (blockIdx.y + 1) / gridDim.y);
+    const int first = part_of(2 * n, blockIdx.y, gridDim.y), last = part_of(2 * n, blockIdx.y + 1, gridDim.y);
     constexpr int BYTES = AS == AS_BF16 ? 2 : 4;
     for (int x = first; x < last; ++x) {
         const bool side = x >= n;
