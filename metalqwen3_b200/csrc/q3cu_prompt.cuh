@@ -188,8 +188,8 @@ struct TileLift {
     bool uneven;
 };
 // The lift of 128 rows by their scales, of which those before `rows` count (one warp; every lane returns it): by the power of
-// two that brings the largest finite one to [2^14, 2^15).
-__device__ __forceinline__ TileLift q8_lift(const uint8_t *raw, int rows) {
+// two that brings the largest finite one to [2^14, 2^15).  Whether they are uneven is found if COMPARE.
+template <bool COMPARE> __device__ __forceinline__ TileLift q8_lift(const uint8_t *raw, int rows) {
     const int lane = threadIdx.x & 31;
     uint32_t w[8];
 #pragma unroll
@@ -207,10 +207,10 @@ __device__ __forceinline__ TileLift q8_lift(const uint8_t *raw, int rows) {
 #pragma unroll
     for (int y = 0; y < 8; ++y) {
         top = max(top, 2 * w[y] + (1u << 24));
-        low = min(low, 2 * w[y] - 1);
+        if (COMPARE) low = min(low, 2 * w[y] - 1);
     }
     top = __reduce_max_sync(FULL, top);
-    low = __reduce_min_sync(FULL, low);
+    if (COMPARE) low = __reduce_min_sync(FULL, low);
     const int top_e = max(int(top >> 24) - 1, 0), low_e = int((low + 1) >> 24);          // (low_e: 0 without any, as is top_e)
     return {min(141 - top_e, 126), low < 0xfeffffffu && top_e - low_e > 24};
 }
@@ -626,8 +626,9 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                              mbar_wait(&raw_full[values.st], values.ph, lane == 0 ? status : nullptr);
                         ok = __all_sync(FULL, ok);
                         if (!ok) break;
-                        lift[0] = q8_lift(raw + from.st * PT_RAW, rows);
-                        lift[1] = q8_lift(raw + values.st * PT_RAW, rows);
+                        // (shared positions: every row sees the whole tile, so that uneven scales are of no account)
+                        lift[0] = q8_lift<!SHARED>(raw + from.st * PT_RAW, rows);
+                        lift[1] = q8_lift<!SHARED>(raw + values.st * PT_RAW, rows);
                         if (entries >= PT_NS) ok = mbar_wait(&empty[to.st], to.ph ^ 1u, lane == 0 ? status : nullptr);
                         if (threadIdx.x == 12 * 32) {        // every warp finds the same
                             k_back[n & 1] = __uint_as_float(uint32_t(134 - lift[0].e) << 23);
