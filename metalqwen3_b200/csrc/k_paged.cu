@@ -98,7 +98,8 @@ paged_split_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constan
     if (warp == PD_WARPS) {
         // ---- fetch: lane = box (K or V, column block, rows of one page) ------------------
         constexpr int TS = CF32 ? 5 : 6, CS = CF32 ? 2 : 1, CB = 1 << CS;     // log2 of TILE; column blocks of 128 B
-        const int bs = min(c.page_shift, TS), br = 1 << bs, ns = TS - bs;     // rows of a box; log2 of boxes of a tile
+        static_assert(TAIL_ALIGN == 32, "5 below");
+        const int bs = min(c.page_shift, Seqs::TAILS ? 5 : TS), br = 1 << bs, ns = TS - bs;     // rows of a box; log2 of boxes of a tile
         const int box = lane & ((1 << ns) - 1), col = (lane >> ns) & (CB - 1), side = lane >> (ns + CS);
         auto page_of = [&]() -> int {                        // n_pages reads as zeros
             const int t = w.template pos<TILE, Seqs>(w.tile) + box * br;
@@ -521,7 +522,8 @@ static cudaError_t launch_split(const PagedKV &c, const Seqs &b, const void *q, 
     typedef typename Elem<T>::type E;
     CUtensorMap mk, mv;
     const q3cu_dtype dt = Elem<TC>::BYTES == 4 ? Q3CU_F32 : Q3CU_BF16;
-    if (!encode_pages_map(&mk, c.k, c, dt, pd_tile<TC>()) || !encode_pages_map(&mv, c.v, c, dt, pd_tile<TC>())) return cudaErrorInvalidValue;
+    const int box = Seqs::TAILS ? TAIL_ALIGN : pd_tile<TC>();
+    if (!encode_pages_map(&mk, c.k, c, dt, box) || !encode_pages_map(&mv, c.v, c, dt, box)) return cudaErrorInvalidValue;
     const int group = n_heads / c.n_kv;
     auto *kernel = group > 8 ? paged_split_kernel<T, TC, true, Seqs> : paged_split_kernel<T, TC, false, Seqs>;
     cudaError_t e = ensure_smem_attr(reinterpret_cast<const void *>(kernel), PD_SMEM, slot + (group > 8));

@@ -112,7 +112,8 @@ paged_q8_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
 
     if (warp == PQ_WARPS) {
         // ---- fetch: lane = box (codes of K or V, or their scales; rows of one page) --------
-        const int bs = min(c.page_shift, 7), br = 1 << bs, ns = 7 - bs;      // rows of a box; log2 of boxes of a tile
+        static_assert(TAIL_ALIGN == 32, "5 below");
+        const int bs = min(c.page_shift, Seqs::TAILS ? 5 : 7), br = 1 << bs, ns = 7 - bs;       // rows of a box; log2 of boxes of a tile
         const int box = lane & ((1 << ns) - 1), kind = lane >> ns;           // kind: K, V, scales of K, of V
         auto page_of = [&]() -> int {                        // n_pages reads as zeros
             const int t = w.template pos<PQ_TILE, Seqs>(w.tile) + box * br;
@@ -454,8 +455,9 @@ static cudaError_t launch_q8(const PagedKV &c, const Seqs &b, const void *q, int
                              float *tails, void *out, uint32_t *status, cudaStream_t stream, int runs, int slot) {
     typedef typename Elem<T>::type E;
     CUtensorMap mk, mv, mks, mvs;
-    if (!encode_pages_map(&mk, c.k, c, Q3CU_Q8_0, PQ_TILE) || !encode_pages_map(&mv, c.v, c, Q3CU_Q8_0, PQ_TILE) ||
-        !encode_scales_map(&mks, c.k_scale, c, PQ_TILE) || !encode_scales_map(&mvs, c.v_scale, c, PQ_TILE))
+    const int box = Seqs::TAILS ? TAIL_ALIGN : PQ_TILE;
+    if (!encode_pages_map(&mk, c.k, c, Q3CU_Q8_0, box) || !encode_pages_map(&mv, c.v, c, Q3CU_Q8_0, box) ||
+        !encode_scales_map(&mks, c.k_scale, c, box) || !encode_scales_map(&mvs, c.v_scale, c, box))
         return cudaErrorInvalidValue;
     const int group = n_heads / c.n_kv;
     auto *kernel = group > 8 ? paged_q8_kernel<T, true, Seqs> : paged_q8_kernel<T, false, Seqs>;

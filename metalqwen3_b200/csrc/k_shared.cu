@@ -20,7 +20,7 @@
 // (over Q8_0 to f16, k_prompt_q8.cu).
 //
 // Measured: 64 sequences behind 16,384 bf16 positions, 512 of their own (32/8 heads) 56 to 60 us, 150 in three groups behind
-// 12,001 Q8_0 ones, up to 1,024 of their own (40/8) 140 to 143 us, five behind 700 (16/8) 17 us.  Bound by the steps of the
+// 12,001 Q8_0 ones, up to 1,024 of their own (40/8) 138 to 141 us, five behind 700 (16/8) 16 us.  Bound by the steps of the
 // tensor-core kernel (some 3,600 cycles a key tile for 2,048 of products, over Q8_0 4,400, or 3,950 where a group is one row
 // tile), then by the bytes of the own positions (74 and 223 MB in 20 and 52 us), then by latency: set-up some 10 us, the join
 // 8.  With the plan made beside the products of the second launch, each CTA searching the groups for itself and the tails
@@ -198,7 +198,7 @@ shared_plan_kernel(const PagedGroups groups, const SharedPlan plan, const PagedK
                 }
             }
             plan.spans[s] = make_int2(from, len);
-            if (len > from) x = TAIL_LEAD + (len + tail_tile - 1) / tail_tile - from / tail_tile;
+            if (len > from) x = TAIL_LEAD + PagedSpan{from, len}.tiles(tail_tile);
         }
         const int64_t mine = x;
         block_prefix(x, y, all_x, all_y);

@@ -27,13 +27,15 @@ struct PagedCut {
     }
 };
 
-// Positions from .. len - 1 of a sequence that one-token attention goes through, one tile after the other.  The tiles
-// begin at multiples of their size: the first may hold positions before `from`.
+// Positions from .. len - 1 of a sequence that one-token attention goes through, one tile after the other.  The first tile
+// begins at a multiple of TAIL_ALIGN, and may hold positions before `from`.  (At a multiple of its size, with boxes as large:
+// 143 against 141 us for 150 sequences behind 12,001 Q8_0 positions; boxes of 16 rows cost more than they save.)
+constexpr int TAIL_ALIGN = 32;                               // rows of a box, at most, where `from` is not 0
 struct PagedSpan {
     int from, len;
-    template <int TILE> __device__ __forceinline__ int tiles() const {
-        return len > from ? (len + TILE - 1) / TILE - from / TILE : 0;
-    }
+    __device__ __forceinline__ int base() const { return from & -TAIL_ALIGN; }
+    __device__ __forceinline__ int tiles(int tile) const { return len > from ? (len - base() + tile - 1) / tile : 0; }
+    template <int TILE> __device__ __forceinline__ int tiles() const { return tiles(TILE); }
 };
 // The batch's whole sequences.
 struct WholeSeqs : PagedSeqs {
@@ -91,7 +93,7 @@ struct PagedWalk {
     int s, head, tile, from, len, tiles;
     int lead;                // tails: units before the tile
     template <int TILE, typename Seqs> __device__ __forceinline__ int pos(int at) const {    // of tile `at`'s first row
-        return (Seqs::TAILS ? from / TILE + at : at) * TILE;
+        return (Seqs::TAILS ? from & -TAIL_ALIGN : 0) + at * TILE;
     }
 };
 
