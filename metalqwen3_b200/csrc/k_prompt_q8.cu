@@ -19,12 +19,13 @@
 // an earlier row (SecondLook).
 //
 // Bound as k_prompt.cu is, by the chain from scores to probabilities to products, with the conversion beside it: a key tile
-// takes some 4,400 cycles (3,000 over a bf16 cache) for 2,048 of products and as many of exponentials.  Conversion and softmax
-// share each quarter's queue for shared memory and special functions, so that a tile's conversion (2 x 1,400 cycles) makes the
-// softmax beside it slower (1,950 cycles of exponentials for 1,290); the conversion's 1.75 instructions an element are not the
-// cost (none of them: the same time).  2,043 rows in four chunks behind up to 8,192 positions (32/8 heads) 241 us, 730 TFLOP/s;
-// 4,096 rows in six prompts 96 us.
-// Measured and left out (us for the chunks, against 241 or what it was at the time): a quarter of the exponentials by
+// takes some 4,200 cycles (3,000 over a bf16 cache) for 2,048 of products and as many of exponentials.  The conversion beside it
+// makes the softmax slower, though its 1.75 instructions an element are not the cost (none of them: the same time): the two
+// share each quarter's queue for shared memory and special functions, and its store of instructions, for which a smaller
+// loop is quicker than one that is unrolled (q8_tile).  2,043 rows in four chunks behind up to 8,192 positions (32/8 heads)
+// 230 us, 770 TFLOP/s; 4,096 rows in six prompts 96 us.
+// Measured and left out (us for the chunks, against 241 or what it was at the time): scores read twice in two halves, for
+// smaller code and fewer registers (244 for 229), a quarter of the exponentials by
 // polynomial (275, an eighth 258), eight warps converting (410 for 240: registers), items of 32 rows less with a ring of four
 // (320 for 252), lifts by a warp of their own (267 for 247; with the scales in a ring of theirs, far ahead, 281), lifts without
 // the comparison where it can be told beforehand (253: what runs earlier is in the softmax's way), codes read before the wait
