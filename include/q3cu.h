@@ -350,7 +350,8 @@ q3cu_status q3cu_attention_shared_workspace(q3cu_ctx *ctx, int n_seqs, int n_hea
  * rows; out: [rows][n_heads][128], other memory than q.  Both of the cache's
  * type, or bf16 over a Q8_0 cache: bf16 runs on the tensor cores with
  * probabilities rounded to bf16 (the sums binary32); over a Q8_0 cache they are
- * rounded to f16 instead, by 2^-11 of themselves or 2^-32, and so are keys and
+ * rounded to f16 instead, by 2^-11 of themselves or 2^-32 (2^-24 where a value
+ * is smaller than those at positions before), and so are keys and
  * values, by 2^-10 of themselves or 2^-39 of the largest of 128 positions; f32
  * runs with binary32's accuracy (elements below 2^-109 keep fewer bits).
  * Grouped heads, scale, softmax, empty rows, unused page space, bad

@@ -11,10 +11,13 @@
 //   keys, values  by tile: the largest scale to [2^14, 2^15), codes as code / 128.  An element is rounded by 2^-10 of itself
 //                 (its scale and the product, 2^-11 each) and by no less than 2^-39 of the tile's largest.
 //   queries       by row, by the same warps when an item begins; exact, but for 2^-39 of the row's largest.
-//   probabilities times 2^7, by 2^-11 of themselves and no less than 2^-32.
-// The inverse lifts of query and keys go into the factor that makes scores exponents.  O is kept times the smallest lift of
-// the value tiles so far: a tile of larger values takes O down with it (in binary32, on the path that rescales O for a larger
-// maximum), a tile of smaller ones has its probabilities lowered.  Where the scales of one tile differ by more than 2^24,
+//   probabilities times 2^7, by 2^-11 of themselves and no less than 2^-32; up to 2^8 lower, so 2^-24, as the next lines say.
+// The inverse lifts of query and keys go into the factor that makes scores exponents.  O is kept, row by row, times the lift
+// of the tiles that it sees: a tile of larger values takes O down with it (in binary32, on the path that rescales O for a larger
+// maximum), a tile of values up to 2^8 smaller has its probabilities lowered, and one of still smaller ones takes O up, as far
+// as binary32 goes: what does not fit then is 2^-100 of the row's result.  (Kept times the smallest lift so far, a row lost
+// values 2^33 smaller than any before them, though those had no weight.)  A tile that the row does not see leaves O as it is.
+// Where the scales of one tile differ by more than 2^24,
 // rows that see only a part of the tile are computed again from the formula, so that a later position takes no bits from
 // an earlier row (SecondLook).
 //

@@ -28,6 +28,7 @@ constexpr uint32_t PT_IDESC = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(128
 constexpr uint32_t PT_IDESC_V = PT_IDESC | (1u << 16);
 constexpr uint32_t PT_F16 = (1u << 7) | (1u << 10);          // the bits that say bf16 where f16 has none
 constexpr int PT_BIAS = 7;                                   // Q8_0: probabilities are times 2^7 in f16, at most 2^15
+constexpr int PT_SLACK = 8;                                  // Q8_0: the most by which values' probabilities are lowered (2^-8)
 constexpr float PT_LOG2 = ATT_SCALE * 1.44269504088896341f;  // scores to base-2 exponents
 constexpr float PT_LAZY = 8.0f / PT_LOG2;                    // growth of the maximum (as a raw score) that rescales O
 
@@ -722,9 +723,8 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                     for (int y = 0; y < 4; ++y)
                         mx[y] = fmaxf(fmaxf(mx[y], __uint_as_float(u[x + y])), __uint_as_float(u[x + y + 4]));
                 float tile_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                float unit = PT_LOG2, lower = 1.0f;          // of S to exponents; what O is to be multiplied by besides
-                [[maybe_unused]] int shift = 0;              // of the probabilities' exponents
-                bool sink = false;
+                float unit = PT_LOG2;                        // of S to exponents
+                [[maybe_unused]] int e = 0, change = 0;      // the tile's lift; of the exponent of O's
                 if constexpr (Q8) {
                     // (after the scores' wait: before it the barrier may be phases behind, where its parity means another tile)
                     const uint32_t n = tiles + j;
@@ -733,25 +733,38 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                     // (the queries were converted before this tile; q_ready may be a phase ahead by now)
                     if (j == 0) row_back = q_back[qs & 1][t * PT_ROWS + r];
                     const float back = fmaxf(row_back * k_back[n & 1], 0x1p-120f);
-                    const int e = v_lift[n & 1];
+                    e = v_lift[n & 1];
                     redo |= !SHARED && rough[n & 1] && limit < min(it.len, (it.from() + j + 1) * PT_KEYS);
                     tile_max *= back;
                     unit *= back;
                     if (j == 0) lifted = e;
-                    sink = e < lifted;                       // larger values than before: O goes down
-                    if (sink) {
-                        lower = e - lifted < -126 ? 0.0f : __uint_as_float(uint32_t(127 + e - lifted) << 23);
-                        lifted = e;
-                    }
-                    shift = max(lifted - e, -64);            // smaller ones: their probabilities go down
+                    // larger values than before: O goes down; much smaller ones: up again; a tile that the row does not see
+                    // changes nothing
+                    if ((e < lifted || e > lifted + PT_SLACK) && (SHARED || limit > (it.from() + j) * PT_KEYS)) change = e - lifted;
                 }
                 const bool grow = tile_max > m + PT_LAZY || (m == -INFINITY && tile_max > m);
-                if (__any_sync(FULL, grow) || sink) {
+                if (__any_sync(FULL, grow || change != 0)) {
                     const float nm = grow ? tile_max : m;
                     float f = grow ? (m == -INFINITY ? 0.0f : ex2_approx_ftz((m - nm) * PT_LOG2)) : 1.0f;
                     m = nm;
                     sum *= f;
-                    if constexpr (Q8) f *= lower;
+                    if constexpr (Q8) {
+                        if (__any_sync(FULL, change > 0)) {      // (j > 0) no higher than binary32 allows
+                            float top = 0.0f;
+#pragma unroll 1
+                            for (int x = 0; x < 8; ++x) {
+                                uint32_t o[16];
+                                tc_ld16(to + 16 * x, o);
+                                tc_wait_ld16(o);
+#pragma unroll
+                                for (int y = 0; y < 16; ++y) top = fmaxf(top, fabsf(__uint_as_float(o[y])));
+                            }
+                            top *= f;
+                            if (top > 0.0f && change > 0) change = max(min(change, min(227 - int(__float_as_uint(top) >> 23), 126)), 0);
+                        }
+                        lifted += change;
+                        f *= change < -126 ? 0.0f : __uint_as_float(uint32_t(127 + min(change, 126)) << 23);
+                    }
                     if (j > 0) {                                 // O of the tiles before (their product has completed)
 #pragma unroll 1
                         for (int x = 0; x < 8; ++x) {
@@ -765,6 +778,8 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                     }
                 }
                 float off = m == -INFINITY ? 0.0f : -m * PT_LOG2;
+                // smaller values than O is kept for: their probabilities go down
+                [[maybe_unused]] const int shift = Q8 ? max(min(lifted - e, 0), -64) : 0;
                 if constexpr (Q8) off += float(shift + PT_BIAS);
                 const f2 off2 = pk2(off, off), scale2 = pk2(unit, unit);
                 f2 part[2] = {pk2(0.0f, 0.0f), pk2(0.0f, 0.0f)};
