@@ -358,7 +358,10 @@ q3cu_status q3cu_attention_shared_workspace(q3cu_ctx *ctx, int n_seqs, int n_hea
  * pages and alignment as above.  A NaN or infinity at a position changes no row
  * before it; where one would, the row is computed again by itself, at some 0.2 us
  * a key (a bf16 prompt does so for a second at most in one tile of rows; what is
- * left then stays NaN and Q3CU_DEV_TIMEOUT is set).  Sequences with one row are
+ * left then stays NaN and Q3CU_DEV_TIMEOUT is set).  Over a Q8_0 cache that is
+ * also done for a row behind which, among the 128 positions from a multiple of
+ * 128 on where its last one lies, a scale is more than 2^24 times the largest
+ * that it sees of them; what is left there keeps a result of fewer bits.  Sequences with one row are
  * allowed, but q3cu_attention_paged is made for them. */
 q3cu_status q3cu_attention_prompt(q3cu_ctx *ctx, const q3cu_kv_cache *cache, const q3cu_kv_batch *batch,
                                   int64_t rows, const void *q, q3cu_dtype dtype, int64_t q_stride, int n_heads,

@@ -315,8 +315,7 @@ template <typename TC> struct SecondLook {
         return top;
     }
 };
-// Over a Q8_0 cache only a scale can be no finite number, or large; scales that differ by more than 2^24 count as large too
-// (a tile that holds them has too few bits for the smaller ones, so that a row that does not see the larger is done again).
+// Over a Q8_0 cache only a scale can be no finite number, or large.
 template <> struct SecondLook<q8raw> {
     int tile = -1, last;
     bool huge;
@@ -326,7 +325,6 @@ template <> struct SecondLook<q8raw> {
         last = -1;
         huge = false;
         const int lane = threadIdx.x & 31;
-        float top[2] = {0.0f, 0.0f}, least[2] = {INFINITY, INFINITY};        // finite ones that are not 0, of K and V
         // 16 positions, which one page holds: a lane looks at one scale of K and of V
         for (int t = 0; t < hi; t += 16) {
             const int page = paged_page(b, c, s, t, nullptr), at = t + (lane >> 1);
@@ -338,19 +336,8 @@ template <> struct SecondLook<q8raw> {
                 v = fabsf(c.v_scale[i]);
             }
             huge |= __any_sync(FULL, k >= 0x1p93f || v >= 0x1p93f);          // times 127: 2^100
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const float a = x ? v : k;
-                if (a > 0.0f && a < INFINITY) top[x] = fmaxf(top[x], a), least[x] = fminf(least[x], a);
-            }
             const unsigned odd = __ballot_sync(FULL, at >= lo && !(v < INFINITY));
             if (odd) last = t + ((31 - __clz(odd)) >> 1);
-        }
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {                        // magnitudes compare as their bits do; exponents by 2^23
-            const uint32_t hi_bits = __reduce_max_sync(FULL, __float_as_uint(top[x]));
-            const uint32_t lo_bits = __reduce_min_sync(FULL, __float_as_uint(least[x]));
-            huge |= hi_bits && (hi_bits >> 23) - (lo_bits >> 23) > 24;
         }
     }
     __device__ __forceinline__ bool wanted(int limit, float4 q) const {

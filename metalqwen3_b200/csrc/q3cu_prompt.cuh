@@ -215,6 +215,36 @@ template <bool COMPARE> __device__ __forceinline__ TileLift q8_lift(const uint8_
     const int top_e = max(int(top >> 24) - 1, 0), low_e = int((low + 1) >> 24);          // (low_e: 0 without any, as is top_e)
     return {min(141 - top_e, 126), low < 0xfeffffffu && top_e - low_e > 24};
 }
+// Whether a row that sees the first n keys of a sequence lost bits to others: behind them in the same tile lies a scale that
+// is more than 2^24 times the largest it sees there, of keys or of values (one warp; every lane returns it).
+__device__ __forceinline__ bool larger_behind(const PagedKV &c, const PagedSeqs &b, int s, int head, int n, int len) {
+    const int tile = n / PT_KEYS * PT_KEYS, t = tile + 4 * (threadIdx.x & 31), end = min(len, tile + PT_KEYS);
+    uint32_t seen[2] = {0, 0}, hidden[2] = {0, 0};           // of K and V; magnitudes compare as their bits do
+    const int page = t < end ? paged_page(b, c, s, t, nullptr) : -1;
+    if (page >= 0) {
+        const int64_t at = paged_scale_at(c, page, head, t); // four positions, which one page holds
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const uint4 *p = reinterpret_cast<const uint4 *>((x ? c.v_scale : c.k_scale) + at);
+            const uint4 lo = p[0], hi = p[1];
+            const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+            for (int y = 0; y < 8; ++y) {
+                const uint32_t bits = w[y] & 0x7fffffffu;
+                if (t + y / 2 >= end || bits >= 0x7f800000u) continue;
+                if (t + y / 2 < n) seen[x] = max(seen[x], bits);
+                else hidden[x] = max(hidden[x], bits);
+            }
+        }
+    }
+    bool larger = false;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        const uint32_t a = __reduce_max_sync(FULL, seen[x]), z = __reduce_max_sync(FULL, hidden[x]);
+        larger |= a && (z >> 23) > (a >> 23) + 24;
+    }
+    return larger;
+}
 // 128 rows' codes (128-byte swizzle) and scales at `raw` become the 32 KB f16 operand tile at `to`, by four warps: a lane
 // takes 16 codes of eight rows.  Rows from `rows` on are zeros.  The lifted scales are rounded to f16 (2^-11), code / 128 is
 // exact, the product is rounded once more: 1.75 instructions an element.  A word's codes become the pairs (0, 2) and (1, 3), one
@@ -352,7 +382,8 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
 
     const int qt = PT_ROWS / group;                          // queries of a tile
     float2 stat = make_float2(-INFINITY, -1.0f);             // SPLIT: maximum and sum of this thread's row, -1: given up
-    [[maybe_unused]] float part_back = 1.0f;                 // and what its O is to be multiplied by (Q8_0)
+    [[maybe_unused]] float part_back = 1.0f;                 // and what its O is to be multiplied by (Q8_0),
+    [[maybe_unused]] bool part_redo = false;                 // and whether a tile of the part is uneven
     // the item of a round, copied from its announcement; false after the last, or if a wait gave up
     auto next_item = [&](int round, Round &it, bool whole_warp) -> bool {
         bool ok = mbar_wait(&item_full[round & 1], uint32_t(round >> 1) & 1u, !whole_warp || lane == 0 ? status : nullptr);
@@ -701,7 +732,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
             // Q8_0: S is q . k times 1 / (row's and tile's inverse lifts), O is times 2^lift
             [[maybe_unused]] float row_back = 0.0f;
             [[maybe_unused]] int lifted = 0;
-            [[maybe_unused]] bool redo = false;              // a tile that the row sees in part is uneven
+            [[maybe_unused]] bool redo = false;              // the tile that the row sees in part is uneven
             const int nkv = max(it.nt[0], it.nt[1]);
             for (int j = 0; j < nt; ++j, ++steps) {
                 ok = __all_sync(FULL, mbar_wait(&s_full[t], steps & 1u, lane == 0 ? status : nullptr));
@@ -734,13 +765,14 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                     if (j == 0) row_back = q_back[qs & 1][t * PT_ROWS + r];
                     const float back = fmaxf(row_back * k_back[n & 1], 0x1p-120f);
                     e = v_lift[n & 1];
-                    redo |= !SHARED && rough[n & 1] && limit < min(it.len, (it.from() + j + 1) * PT_KEYS);
+                    const int tile = (it.from() + j) * PT_KEYS;
+                    redo |= !SHARED && rough[n & 1] && limit > tile && limit < min(it.len, tile + PT_KEYS);
                     tile_max *= back;
                     unit *= back;
                     if (j == 0) lifted = e;
                     // larger values than before: O goes down; much smaller ones: up again; a tile that the row does not see
                     // changes nothing
-                    if ((e < lifted || e > lifted + PT_SLACK) && (SHARED || limit > (it.from() + j) * PT_KEYS)) change = e - lifted;
+                    if ((e < lifted || e > lifted + PT_SLACK) && (SHARED || limit > tile)) change = e - lifted;
                 }
                 const bool grow = tile_max > m + PT_LAZY || (m == -INFINITY && tile_max > m);
                 if (__any_sync(FULL, grow || change != 0)) {
@@ -822,12 +854,12 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                 if constexpr (Q8) sum = fmaf(s0 + s1, __uint_as_float(uint32_t(127 - PT_BIAS - shift) << 23), sum);
                 else sum += s0 + s1;
             }
-            // what O is to be multiplied by (values are 2^7 below their lift, probabilities 2^7 above; NaN: to be done again)
+            // what O is to be multiplied by (values are 2^7 below their lift, probabilities 2^7 above)
             [[maybe_unused]] float o_back = 1.0f;
             if constexpr (Q8) {
                 tiles += nkv;
                 qs += nkv > 0;
-                o_back = redo ? __uint_as_float(0x7fffffffu) : ldexpf(1.0f, -lifted);
+                o_back = ldexpf(1.0f, -lifted);
             }
             // ---- the result ----------------------------------------------------------------
             if (nt > 0 && ok) {
@@ -836,7 +868,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
             }
             if constexpr (SPLIT) {
                 if (ok) stat = make_float2(m, sum);
-                if constexpr (Q8) part_back = o_back;
+                if constexpr (Q8) part_back = o_back, part_redo = redo;
                 if (it.parts > 1) continue;                  // joined below
             }
             if constexpr (SHARED) {
@@ -916,8 +948,9 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&o_empty[t]);
                 }
-                // rows that came out as no numbers, once more from the formula
-                unsigned again = __ballot_sync(FULL, live && limit > 0 && nan);
+                // rows that came out as no numbers, and such as lost bits to positions that they do not see, once more from
+                // the formula (over what is stored, which stays where time is up)
+                unsigned again = __ballot_sync(FULL, live && limit > 0 && (nan || (Q8 && redo)));
                 SecondLook<Cached> second;
                 const uint64_t began = again ? global_ns() : 0;
                 while (again) {
@@ -928,11 +961,17 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                     const int l = __ffs(again) - 1;
                     again &= again - 1;
                     __syncwarp();
-                    second.look(t, c, b, it.s, it.head, it.seen(it.first + t * qt), min(it.len, it.nt[t] * PT_KEYS));
                     const int il = __shfl_sync(FULL, i, l), n = __shfl_sync(FULL, limit, l);
                     const int h = it.head * group + __shfl_sync(FULL, r_head, l);
                     float4 x = load_quad(q + int64_t(it.base + il) * q_stride + int64_t(h) * HD + 4 * lane);
-                    if (!second.wanted(n, x)) continue;
+                    bool want = false;
+                    if (__shfl_sync(FULL, int(nan), l)) {
+                        second.look(t, c, b, it.s, it.head, it.seen(it.first + t * qt), min(it.len, it.nt[t] * PT_KEYS));
+                        want = second.wanted(n, x);
+                    }
+                    if constexpr (Q8)
+                        if (!want && __shfl_sync(FULL, int(redo), l)) want = larger_behind(c, b, it.s, it.head, n, it.len);
+                    if (!want) continue;
                     x = make_float4(x.x * ATT_SCALE, x.y * ATT_SCALE, x.z * ATT_SCALE, x.w * ATT_SCALE);
                     store_quad(out + (int64_t(it.base + il) * n_heads + h) * HD + 4 * lane,
                                attend_row<Cached, 4>(c, b, it.s, it.head, n, x, status));
@@ -948,8 +987,10 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
         const int rank = int(blockIdx.x % unsigned(ctas));
         if (it.parts > 1 && rank < it.parts) {               // the same for all of the CTA
             float2 *stats = reinterpret_cast<float2 *>(smem);
+            [[maybe_unused]] uint32_t *marks = reinterpret_cast<uint32_t *>(stats + 2 * PT_ROWS);
             if (warp < 8) {                                  // the rows' results, 128 KB in the ring's place
                 stats[threadIdx.x] = stat;
+                if constexpr (Q8) marks[threadIdx.x] = part_redo;
                 const int t = warp >> 2;
                 uint8_t *row = ring + threadIdx.x * (HD * 4);
 #pragma unroll 1
@@ -984,11 +1025,25 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                 float4 v = join_parts(smem_addr(ring) + r * (HD * 4), smem_addr(stats + r), r, it.parts, PT_LOG2, ok);
                 if (!ok) continue;
                 if (limit <= 0) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (limit > 0 && __any_sync(FULL, !all_finite(v))) {
-                    const int first = it.first + (r >> 7) * qt, seen = it.seen(min(first + qt, it.rows) - 1);
-                    second.look(r >> 7, c, b, it.s, it.head, it.seen(first), min(it.len, (seen + PT_KEYS - 1) / PT_KEYS * PT_KEYS));
+                const bool nan = __any_sync(FULL, !all_finite(v));
+                bool uneven = false;
+                if constexpr (Q8) {
+                    uint32_t mark = 0;
+                    if (lane < it.parts)
+                        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(mark) : "r"(peer_smem(smem_addr(marks + r), lane)) : "memory");
+                    uneven = __any_sync(FULL, mark != 0);
+                }
+                if (limit > 0 && (nan || uneven)) {
                     const float4 x = load_quad(q + int64_t(it.base + i) * q_stride + int64_t(head) * HD + 4 * lane);
-                    if (second.wanted(limit, x))
+                    bool want = false;
+                    if (nan) {
+                        const int first = it.first + (r >> 7) * qt, seen = it.seen(min(first + qt, it.rows) - 1);
+                        second.look(r >> 7, c, b, it.s, it.head, it.seen(first), min(it.len, (seen + PT_KEYS - 1) / PT_KEYS * PT_KEYS));
+                        want = second.wanted(limit, x);
+                    }
+                    if constexpr (Q8)
+                        if (!want && uneven) want = larger_behind(c, b, it.s, it.head, limit, it.len);
+                    if (want)
                         v = attend_row<Cached, 4>(c, b, it.s, it.head, limit,
                                                 make_float4(x.x * ATT_SCALE, x.y * ATT_SCALE, x.z * ATT_SCALE, x.w * ATT_SCALE),
                                                 status);

@@ -116,3 +116,35 @@ def test_larger_values_behind_change_nothing(q3, rows, n):
     early = rows - (4 if rows == 9 else 16)
     assert early > 0 and torch.equal(got[0][:early], got[1][:early]) and (got[0][:early] != 0).any()
     assert torch.isfinite(got[1].float()).all() and q3.device_status() == 0
+
+
+@pytest.mark.parametrize("rows,n", [(300, 300), (100, 700), (7, 3000)])
+def test_small_scales_cost_no_second_computation(q3, rows, n):
+    """A value group and a key group 2^-60 as large as the others, in the tile that the last rows see in part: what the
+    products give of them is 0 (f16 has no less than 2^-24, the largest are lifted to 2^15), so the results are, bit for bit,
+    those of scales that are 0, which no row is computed again for."""
+    got = []
+    for size in (0.0, 2.0 ** -60):
+        p = Quantised([n], 2, 16, seed=80).fill(81)
+        page, slot = p.where(0, [n - rows // 2 - 1, n - rows])
+        p.vs[page, 0, slot, 1] *= size
+        p.ks[page, 1, slot, 0] *= size
+        got.append(q3.attention_prompt(*p.handles([0, rows]), queries(rows, 8, BF16, 82)))
+    assert torch.equal(got[0], got[1]) and q3.device_status() == 0
+
+
+def test_time_for_second_computations_runs_out(q3):
+    """The last position's values 2^40 times larger, behind 300,000: the rows before it are computed again for a second, and
+    what is left keeps the tensor cores' result."""
+    from metalqwen3_b200.q3cu import DEV_TIMEOUT
+    n, rows = 300_000, 1280
+    p = Quantised([n], 8, 256, seed=83).fill(84)
+    page, slot = p.where(0, [n - 1])
+    p.vs[page, 0, slot] *= 2.0 ** 40
+    got = q3.attention_prompt(*p.handles([0, rows]), queries(rows, 32, BF16, 85))
+    try:
+        timed_out = q3.device_status() == DEV_TIMEOUT
+    except Exception:
+        timed_out = True
+    assert timed_out and torch.isfinite(got.float()).all()
+    assert q3.device_status() == 0
