@@ -318,7 +318,9 @@ q3cu_status q3cu_attention_paged_workspace(q3cu_ctx *ctx, int n_heads, int n_kv,
 /* Sequences that begin alike: sequences seq_off[g] .. seq_off[g+1]-1 of the
  * batch have their first len[g] positions in common, which are read from the
  * pages of the group's first sequence (the other sequences' entries for pages
- * that lie wholly before len[g] are not read).  Device arrays, read when the kernels run. */
+ * that lie wholly before len[g] are not read).  Where that first sequence holds
+ * fewer than len[g] positions, its kv_len being less, the group shares nothing,
+ * and each sequence attends to the pages of its own table.  Device arrays, read when the kernels run. */
 typedef struct {
     const int32_t *seq_off;  /* [n_groups + 1], rising within 0 .. n_seqs; sequences outside all groups share nothing */
     const int32_t *len;      /* [n_groups] */

@@ -55,13 +55,15 @@ struct PagedGroups {
         const int a = off[g], z = off[g + 1];
         return a >= 0 && z <= n_seqs && a < z ? z - a : 0;
     }
-    // Positions that the group's first sequence has pages for and all have in common; one sequence alone shares nothing.
+    // Positions that the group's first sequence holds and all have in common; one sequence alone shares nothing, and neither
+    // do those whose first holds fewer (its slot may have been freed, and its page ids be another's).
     __host__ __device__ __forceinline__ int shared(int g, const PagedSeqs &b, const PagedKV &c, uint32_t *status) const {
         const int64_t cap = int64_t(b.max_pages) << c.page_shift;
         const int n = len[g];
         if (n <= 0 || count(g, b.n_seqs) < 2) return 0;
         if (n > cap) flag_bad_index(status);
-        return int(n > cap ? cap : n);
+        const int cut = int(n > cap ? cap : n);
+        return paged_len(b, c, off[g], nullptr) < cut ? 0 : cut;
     }
     // The group of sequence s, or -1.
     __host__ __device__ __forceinline__ int of(int s, int n_seqs) const {

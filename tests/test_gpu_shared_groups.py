@@ -1,0 +1,32 @@
+"""Which sequences of a group share what, where lengths and offsets are not as they mostly are.  Tolerances as in
+test_gpu_shared.py."""
+import pytest
+import torch
+
+from test_gpu_paged import BF16, H, queries
+from test_gpu_paged_q8 import check_attention
+from test_gpu_shared import Shared
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("held", [0, 150, -4])
+def test_a_first_sequence_that_holds_less_than_is_shared(q3, q8, held):
+    """Its slot was freed, say, and its page ids are another sequence's by now: the group shares nothing then, and each
+    sequence attends to its own pages.  A group beside it shares as before."""
+    sh = Shared([(4, 200), (3, 90)], [10, 20, 30, 40, 5, 6, 7], 2, 16, q8, seed=51)
+    p = sh.p
+    p.table[0, :13] = p.table[3, :13].flip(0)           # stale, and of other positions
+    p.kv_len[0] = held
+    q = queries(7, 8, BF16, 52)
+    got = q3.attention_shared(*p.handles(), sh.prefix(), q)
+    assert q3.device_status() == 0
+    for s in (1, 2, 3):
+        check_attention(got[s:s + 1], q[s:s + 1], *p.rows(s), [sh.lens[s]], BF16, H)
+    sh.check(got, q, (4, 5, 6))
+    if held > 0:
+        p.lens[0] = held
+        check_attention(got[:1], q[:1], *p.rows(0), [held], BF16, H)
+    else:
+        assert (got[0] == 0).all()
