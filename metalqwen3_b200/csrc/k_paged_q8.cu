@@ -102,7 +102,7 @@ paged_q8_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
     PagedWalk w = walk_run<PQ_TILE>(b, c, int(blockIdx.x), int(gridDim.x), cut, u0, u1,
                                     blockIdx.x == 0 && warp == 0 ? status : nullptr);
     for (int s = int(blockIdx.x); s < b.n_seqs; s += int(gridDim.x))       // sequences without positions: zeros
-        if (b.kv_len[s] <= 0 || b.max_pages == 0)
+        if (b.span(c, s, nullptr).len == 0)
             for (int i = threadIdx.x; i < n_heads * (HD / 4); i += PQ_THREADS)
                 store_quad(out + int64_t(s) * n_heads * HD + 4 * i, make_float4(0.0f, 0.0f, 0.0f, 0.0f));
     if (u0 == u1) {

@@ -5,7 +5,7 @@
 // which lie on the pages of the group's first sequence.  Four launches, joined by the softmax's maxima and sums:
 //
 //   plan              one CTA: which groups share something, and how the work of the others is cut.  Lengths and groups are
-//                     read here and by no launch behind, so that a captured step can be replayed while they change.
+//                     read here and by no launch behind, so that all go by the same ones, whatever the arrays hold.
 //   shared positions  the tensor-core kernel of k_prompt.cu (q3cu_prompt.cuh, PT_SHARED) with sequences in the place of
 //                     prompt rows: row r of a tile is sequence r / g, head r % g of the g query heads of a kv head, and
 //                     all rows see the same keys.  The units are key tiles (128 positions) of (group, kv head, block of

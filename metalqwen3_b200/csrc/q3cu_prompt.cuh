@@ -724,8 +724,16 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
         Round it;
         for (int round = 0; ok && next_item(round, it, true); ++round) {
             const int nt = it.nt[t], i = it.first + r_query; // i: the sequence's row
-            // (PT_SHARED: a sequence that holds fewer positions attends by itself)
-            const bool live = r_used && i < it.rows && (!SHARED || b.kv_len[it.base + i] >= it.len);
+            // (PT_SHARED: a sequence that holds fewer positions attends by itself, and one that another group claims too, where
+            // offsets do not rise, behind the one that the plan found it in)
+            bool live = r_used && i < it.rows;
+            if constexpr (SHARED)
+                if (live && sh.plan.spans[it.base + i].x > 0) {
+                    const SharedEntry of = sh.plan.of[it.base + i];
+                    live = of.first == it.base && of.count == it.rows && of.len == it.len;
+                } else {
+                    live = false;
+                }
             const int limit = SHARED ? it.len : live ? it.seen(i) : 0;
             const int sure = SHARED ? it.len : it.seen(it.first + t * qt);   // keys that every row of the tile sees
             float m = -INFINITY, sum = 0.0f;

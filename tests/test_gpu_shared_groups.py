@@ -30,3 +30,25 @@ def test_a_first_sequence_that_holds_less_than_is_shared(q3, q8, held):
         check_attention(got[:1], q[:1], *p.rows(0), [held], BF16, H)
     else:
         assert (got[0] == 0).all()
+
+
+def test_groups_that_overlap(q3):
+    """Offsets that fall make two groups claim the same sequences: each sequence attends behind one first sequence, the one
+    whose group the plan finds it in, and no other group writes its results.  The long third group makes runs of several
+    items, so that the second group's results are written behind the first's."""
+    from metalqwen3_b200.q3cu import KVPrefix
+    i32 = dict(dtype=torch.int32, device="cuda")
+    sh = Shared([(4, 96), (2, 96), (2, 50_000)], [10 + i for i in range(8)], 2, 16, False, seed=53)
+    p = sh.p
+    q = queries(8, 32, BF16, 54)
+    # sequences 0 .. 3, again 2 .. 5 (of which 2 and 3 are the first group's), and 6, 7
+    prefix = KVPrefix(torch.tensor([0, 0, 4, 2, 6, 8], **i32), torch.tensor([0, 96, 0, 96, 50_000], **i32))
+    p.table[2, :6] = p.table[4, :6].flip(0)           # what sequence 2 has there is its own
+    got = q3.attention_shared(*p.handles(), prefix, q)
+    assert q3.device_status() == 0
+    for s in range(8):
+        first = 0 if s < 4 else 2 if s < 6 else 6
+        n = 96 if s < 6 else 50_000
+        own, lead = p.rows(s), p.rows(first)
+        k, v = (torch.cat([a[:n], b[n:]]) for a, b in zip(lead, own))
+        check_attention(got[s:s + 1], q[s:s + 1], k, v, [sh.lens[s]], BF16, H)
