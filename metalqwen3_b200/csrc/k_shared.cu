@@ -43,22 +43,20 @@ shared_join_kernel(const SharedOut sh, const PagedKV c, const TailSeqs b, const 
     const int64_t tails_before = b.before[s], tails_all = b.before[b.n_seqs], shared_all = sh.plan.all->units;
     const SharedEntry of = sh.plan.of[s];
     const int tiles = mine.tiles<TILE>();
-    int tail_first = 0, tail_n = 0, shared_first = 0, shared_n = 0, slot = 0;
-    bool tail_late = false, shared_late = false;             // part 0 is the second of its run
+    int tail_n = 0, shared_n = 0, slot = 0;
+    PartsOf tail_parts(PagedCut(1, 1), 0, 0, 1), shared_parts = tail_parts;
     if (tiles > 0) {
         const PagedCut cut(tails_all * c.n_kv, tail_runs);
         const int64_t a = tails_before * c.n_kv + int64_t(kv) * (TAIL_LEAD + tiles);
-        tail_first = cut.run_of(a + TAIL_LEAD);
-        tail_n = cut.run_of(a + TAIL_LEAD + tiles - 1) - tail_first + 1;
-        tail_late = a > cut.begin(tail_first);
+        tail_parts = PartsOf(cut, a, a + TAIL_LEAD, a + TAIL_LEAD + tiles);
+        tail_n = tail_parts.n;
     }
     if (mine.from > 0) {
         const PagedCut cut(shared_all * c.n_kv, shared_runs);
         const int keys = (mine.from + PT_KEYS - 1) / PT_KEYS, at = s - of.first, block = per_block(at);
         const int64_t a = of.units * c.n_kv + (int64_t(kv) * (per_block(of.count - 1) + 1) + block) * keys;
-        shared_first = cut.run_of(a);
-        shared_n = cut.run_of(a + keys - 1) - shared_first + 1;
-        shared_late = a > cut.begin(shared_first);
+        shared_parts = PartsOf(cut, a, a, a + keys);
+        shared_n = shared_parts.n;
         slot = (at - block * per_block.d) * group;
     }
     griddep_wait();
@@ -69,11 +67,10 @@ shared_join_kernel(const SharedOut sh, const PagedKV c, const TailSeqs b, const 
         auto at = [&](int i) -> const float * {              // part i: 128 elements, maximum, sum
             if (i < shared_n)
                 return sh.rows + SHARED_ROW * (shared_n == 1 ? row
-                                                             : int64_t(b.n_seqs) * n_heads +
-                                                                   (2 * int64_t(shared_first + i) + (i == 0 && shared_late)) * sh.slot_rows + slot + h);
+                                                             : int64_t(b.n_seqs) * n_heads + shared_parts.slot(i) * sh.slot_rows + slot + h);
             i -= shared_n;
             return tail_n == 1 ? tails + row * SHARED_ROW
-                               : part + ((2 * int64_t(tail_first + i) + (i == 0 && tail_late)) * group + h) * SHARED_ROW;
+                               : part + (tail_parts.slot(i) * group + h) * SHARED_ROW;
         };
         float m = -INFINITY;
         for (int i = lane; i < n; i += 32) m = fmaxf(m, at(i)[HD]);

@@ -10,7 +10,8 @@ constexpr float PD_LOG2 = ATT_SCALE * 1.44269504088896341f;  // scores to base-2
 constexpr int PD_PART = HD + 2;                              // floats of a row's partial result: 128, maximum, sum
 
 // a / b for 0 <= a, 0 < b: 32-bit division where it serves (a 64-bit one is a chain of some hundred instructions).
-__device__ __forceinline__ int64_t quot(int64_t a, int b) {
+// (This and the cut below host and device: their arithmetic is also checked on the CPU.)
+__host__ __device__ __forceinline__ int64_t quot(int64_t a, int b) {
     return a < (int64_t(1) << 32) ? int64_t(uint32_t(a) / uint32_t(b)) : a / b;
 }
 
@@ -18,13 +19,22 @@ __device__ __forceinline__ int64_t quot(int64_t a, int b) {
 struct PagedCut {
     int64_t total, each;
     int more;
-    __device__ __forceinline__ PagedCut(int64_t t, int runs) : total(t), each(quot(t, runs)), more(int(t - each * runs)) {}
-    __device__ __forceinline__ int64_t begin(int run) const { return each * run + min(run, more); }
-    __device__ __forceinline__ int run_of(int64_t u) const {                 // u < total
+    __host__ __device__ __forceinline__ PagedCut(int64_t t, int runs) : total(t), each(quot(t, runs)), more(int(t - each * runs)) {}
+    __host__ __device__ __forceinline__ int64_t begin(int run) const { return each * run + (run < more ? run : more); }
+    __host__ __device__ __forceinline__ int run_of(int64_t u) const {        // u < total
         const int64_t edge = (each + 1) * more;
         return u < edge ? int(each < INT32_MAX ? quot(u, int(each + 1)) : u / (each + 1))
                         : more + int(each < INT32_MAX ? quot(u - edge, int(each)) : (u - edge) / each);
     }
+};
+// Where the parts of an item lie that begins with unit `begin` and has its tiles in units a .. z - 1 (a < z): in the first slots
+// of runs first .. first + n - 1, but the first of them in its run's second slot if the run began with another item (`late`).
+struct PartsOf {
+    int first, n;
+    bool late;
+    __host__ __device__ __forceinline__ PartsOf(const PagedCut &cut, int64_t begin, int64_t a, int64_t z)
+        : first(cut.run_of(a)), n(cut.run_of(z - 1) - first + 1), late(begin > cut.begin(first)) {}
+    __host__ __device__ __forceinline__ int64_t slot(int i) const { return 2 * int64_t(first + i) + (i == 0 && late); }
 };
 
 // Positions from .. len - 1 of a sequence that one-token attention goes through, one tile after the other.  The first tile
@@ -33,9 +43,9 @@ struct PagedCut {
 constexpr int TAIL_ALIGN = 32;                               // rows of a box, at most, where `from` is not 0
 struct PagedSpan {
     int from, len;
-    __device__ __forceinline__ int base() const { return from & -TAIL_ALIGN; }
-    __device__ __forceinline__ int tiles(int tile) const { return len > from ? (len - base() + tile - 1) / tile : 0; }
-    template <int TILE> __device__ __forceinline__ int tiles() const { return tiles(TILE); }
+    __host__ __device__ __forceinline__ int base() const { return from & -TAIL_ALIGN; }
+    __host__ __device__ __forceinline__ int tiles(int tile) const { return len > from ? (len - base() + tile - 1) / tile : 0; }
+    template <int TILE> __host__ __device__ __forceinline__ int tiles() const { return tiles(TILE); }
 };
 // The batch's whole sequences.
 struct WholeSeqs : PagedSeqs {
@@ -90,6 +100,14 @@ struct TailSeqs : PagedSeqs {
     }
 };
 
+// Unit `at` of a sequence of `tiles` tiles: kv head, tile, and units before the tile.
+__host__ __device__ __forceinline__ void tail_place(int64_t at, int tiles, int &head, int &tile, int &lead) {
+    head = int(quot(at, TAIL_LEAD + tiles));
+    const int unit = int(at - int64_t(head) * (TAIL_LEAD + tiles));
+    tile = unit > TAIL_LEAD ? unit - TAIL_LEAD : 0;
+    lead = unit < TAIL_LEAD ? TAIL_LEAD - unit : 0;
+}
+
 // A place in the batch's tiles: sequence, kv head, tile, and the sequence's span and tiles.
 struct PagedWalk {
     int s, head, tile, from, len, tiles;
@@ -137,11 +155,7 @@ __device__ __forceinline__ PagedWalk walk_run(const Seqs &b, const PagedKV &c, i
                     w.from = mine.from;
                     w.len = mine.len;
                     w.tiles = mine.tiles<TILE>();
-                    const int64_t at = u0 - __shfl_sync(FULL, x[r], l) * c.n_kv;
-                    w.head = int(quot(at, TAIL_LEAD + w.tiles));
-                    const int unit = int(at - int64_t(w.head) * (TAIL_LEAD + w.tiles));
-                    w.tile = max(unit - TAIL_LEAD, 0);
-                    w.lead = max(TAIL_LEAD - unit, 0);
+                    tail_place(u0 - __shfl_sync(FULL, x[r], l) * c.n_kv, w.tiles, w.head, w.tile, w.lead);
                     return w;
                 }
             }
