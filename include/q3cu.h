@@ -354,7 +354,10 @@ q3cu_status q3cu_attention_shared_workspace(q3cu_ctx *ctx, int n_seqs, int n_hea
  * probabilities rounded to bf16 (the sums binary32); over a Q8_0 cache they are
  * rounded to f16 instead, by 2^-11 of themselves or 2^-32 (2^-24 where a value
  * is smaller than those at positions before), and so are keys and
- * values, by 2^-10 of themselves or 2^-39 of the largest of 128 positions; f32
+ * values, by 2^-10 of themselves or 2^-39 of the largest of 128 positions (so a
+ * score moves by up to 2^-10 sum |q_i k_i| / sqrt(128), and a weight by that share
+ * of itself: scores of several hundred give other weights than
+ * q3cu_attention_paged, which takes the codes exactly); f32
  * runs with binary32's accuracy (elements below 2^-109 keep fewer bits).
  * Grouped heads, scale, softmax, empty rows, unused page space, bad
  * pages and alignment as above.  A NaN or infinity at a position changes no row
