@@ -16,7 +16,7 @@
 // code exactly: a byte becomes 1024 + (code + 128) by a byte permutation and the
 // code by one packed subtraction, 1.25 instructions an element, where going through
 // bf16 (8 bits) or f32 takes twice that.  The scales never touch the elements:
-//     score = s_0 (q_lo . c_lo) + s_1 (q_hi . c_hi)         two chains of products
+//     score = s_0 (q_lo . c_lo) + s_1 (q_hi . c_hi)         two chains of products (s with q's inverse lift, see below)
 //     o_lo += sum_t (p_t s_0t) c_t,lo                       the weights take them
 // The other operands go to f16 as well, each times a power of two that brings the
 // largest of them to [2^14, 2^15) (of a query row, and of a warp's 32 value scales),
@@ -191,7 +191,7 @@ paged_q8_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
 #pragma unroll
                     for (int h = 0; h < 2; ++h) query(x, n, h, qf[x][n][h]);
         }
-        float back[NH][2];                                   // a score times this is q . k, of heads 8 n + 2 t4, + 1
+        float back[NH][2];                                   // products times this are those with q, of heads 8 n + 2 t4, + 1
 #pragma unroll
         for (int n = 0; n < NH; ++n) back[n][0] = row_back[8 * n + 2 * t4], back[n][1] = row_back[8 * n + 2 * t4 + 1];
         // o[j][n]: dimensions 16 j + 2 g and (+ 2) the next one by heads 8 n + 2 t4, + 1
@@ -247,12 +247,12 @@ paged_q8_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
                                 mma_f16(acc, a[y][0], a[y][1], a[y][2], a[y][3], QREG ? qf[QREG ? x : 0][QREG ? n : 0][h][2 * y] : mem[2 * y],
                                         QREG ? qf[QREG ? x : 0][QREG ? n : 0][h][2 * y + 1] : mem[2 * y + 1]);
                         }
-                        const float f0 = h ? sc0.y : sc0.x, f1 = h ? sc1.y : sc1.x;
-                        if (h == 0) {
-                            s[kb][n][0] = f0 * acc[0], s[kb][n][1] = f0 * acc[1], s[kb][n][2] = f1 * acc[2], s[kb][n][3] = f1 * acc[3];
-                        } else {
-                            s[kb][n][0] = fmaf(f0, acc[0], s[kb][n][0]), s[kb][n][1] = fmaf(f0, acc[1], s[kb][n][1]);
-                            s[kb][n][2] = fmaf(f1, acc[2], s[kb][n][2]), s[kb][n][3] = fmaf(f1, acc[3], s[kb][n][3]);
+                        // scales times the query's inverse lift, a power of two: products alone of a lifted query and keys from
+                        // 2^100 on would leave binary32, where scores do not
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            const float sc = x < 2 ? (h ? sc0.y : sc0.x) : (h ? sc1.y : sc1.x), f = sc * back[n][x & 1];
+                            s[kb][n][x] = h == 0 ? f * acc[x] : fmaf(f, acc[x], s[kb][n][x]);
                         }
                     }
                 }
@@ -275,8 +275,6 @@ paged_q8_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__
             for (int n = 0; n < NH; ++n)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    s[0][n][h] *= back[n][h], s[0][n][2 + h] *= back[n][h];
-                    s[1][n][h] *= back[n][h], s[1][n][2 + h] *= back[n][h];
                     float tm = fmaxf(fmaxf(s[0][n][h], s[0][n][2 + h]), fmaxf(s[1][n][h], s[1][n][2 + h]));
 #pragma unroll
                     for (int x = 4; x < 32; x <<= 1) tm = fmaxf(tm, __shfl_xor_sync(FULL, tm, x));

@@ -10,7 +10,8 @@ import pytest
 import torch
 
 from test_gpu_kv_forms import Quantised
-from test_gpu_paged import BF16, H, U, attend, queries
+from test_gpu_paged import BF16, F32, H, U, attend, queries
+from test_gpu_paged_q8 import check_attention
 
 pytestmark = pytest.mark.gpu
 W = 2.0 ** -11
@@ -147,4 +148,24 @@ def test_time_for_second_computations_runs_out(q3):
     except Exception:
         timed_out = True
     assert timed_out and torch.isfinite(got.float()).all()
+    assert q3.device_status() == 0
+
+
+@pytest.mark.parametrize("io", [F32, BF16])
+@pytest.mark.parametrize("size_q,size_kv", [(1e-33, 1e33), (1e-36, 1e36), (1e33, 1e-33), (1e-30, 1e30)])
+def test_one_token_far_from_1(q3, io, size_q, size_kv):
+    """Keys and values up to the end of binary32 with scores as usual, alone and behind a shared prefix."""
+    from metalqwen3_b200.q3cu import KVPrefix
+    for heads in (8, 32):
+        p = Quantised([300, 300], 2, 16, seed=86).fill(87, size_kv)
+        p.table[1, :16] = p.table[0, :16]
+        q = queries(2, heads, io, 88, size_q)
+        got = [q3.attention_paged(*p.handles(), q)]
+        if io == BF16:
+            i32 = dict(dtype=torch.int32, device="cuda")
+            got.append(q3.attention_shared(*p.handles(), KVPrefix(torch.tensor([0, 2], **i32), torch.tensor([256], **i32)), q))
+        for x, elements in zip(got, (p.rows, lambda s: tuple(torch.cat([a[:256], b[256:]]) for a, b in zip(rounded(p, s), p.rows(s))))):
+            for s in range(2):
+                k, v = elements(s)
+                check_attention(x[s:s + 1], q[s:s + 1], k, v, [300], io, W if io == BF16 else 0.0, 2.0 ** -32 if len(got) > 1 else 2.0 ** -39)
     assert q3.device_status() == 0
