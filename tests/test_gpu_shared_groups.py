@@ -52,3 +52,24 @@ def test_groups_that_overlap(q3):
         own, lead = p.rows(s), p.rows(first)
         k, v = (torch.cat([a[:n], b[n:]]) for a, b in zip(lead, own))
         check_attention(got[s:s + 1], q[s:s + 1], k, v, [sh.lens[s]], BF16, H)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("page,shared", [(16, 200), (64, 200), (256, 500)])
+def test_first_slots_of_a_page_that_is_shared_in_part(q3, q8, page, shared):
+    """The shared positions on a sequence's own page are the first sequence's to hold: NaN there (in a Q8_0 cache's scales)
+    reaches nothing."""
+    sh = Shared([(5, shared)], [1, 60, 3, 300, 2], 2, page, q8, seed=55)
+    q = queries(5, 8, BF16, 56)
+    clean = q3.attention_shared(*sh.p.handles(), sh.prefix(), q)
+    for s in range(1, 5):
+        b = int(sh.p.table[s, shared // page])
+        for t in (sh.p.ks, sh.p.vs) if q8 else (sh.p.k, sh.p.v):
+            t[b, :, :shared % page] = float("nan")
+    assert torch.equal(q3.attention_shared(*sh.p.handles(), sh.prefix(), q), clean)
+    for s in range(1, 5):                                # (the formula takes the first sequence's)
+        a, b = int(sh.p.table[0, shared // page]), int(sh.p.table[s, shared // page])
+        for t in (sh.p.ks, sh.p.vs) if q8 else (sh.p.k, sh.p.v):
+            t[b, :, :shared % page] = t[a, :, :shared % page]
+    sh.check(clean, q)
+    assert q3.device_status() == 0
