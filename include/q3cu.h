@@ -268,7 +268,8 @@ typedef struct {
     int32_t scaling;         /* q3cu_rope_scaling: none; every frequency divided by factor; or YaRN (Peng et al., 2023):
                                 pairs that turn more than beta_fast times over `original` positions keep their
                                 frequency, those that turn less than beta_slow times have it divided by factor, with a
-                                linear ramp over the pairs between (its ends rounded outwards to whole pairs) */
+                                linear ramp over the pairs between (its ends rounded outwards to whole pairs, and cut to 0 and
+                                dim - 1: where even pair 0 turns less than beta_slow times, it alone keeps its frequency) */
     float factor;            /* at least 1 (read when scaled) */
     float original;          /* positions trained on (YaRN) */
     float beta_fast, beta_slow;  /* YaRN: 32 and 1 usually */

@@ -5,7 +5,7 @@
 // 64 elements, a value likewise.  Bound by memory: 136 bytes a position, kv head
 // and side, where bf16 takes 256.  64 sequences of up to 16,384 positions (32/8 heads,
 // bf16 queries): 176 to 194 us, up to 6.2 TB/s; one of 512 (16/8, f32 queries): 9 us,
-// all latency.
+// all latency.  f32 queries for 64 such sequences: 220 us where bf16 ones take 177.
 //
 // A CTA is one fetching warp and four computing warps around a ring of three 34 KB
 // stages, filled page by page by TMA: 128 positions' codes of K and of V (128-byte

@@ -22,11 +22,11 @@
 // later position takes no bits from an earlier row (larger_behind; some 0.2 us a key, a look alone a microsecond).
 //
 // Bound as k_prompt.cu is, by the chain from scores to probabilities to products, with the conversion beside it: a key tile
-// takes some 4,200 cycles (3,000 over a bf16 cache) for 2,048 of products and as many of exponentials.  The conversion beside it
+// takes 4,200 to 4,400 cycles (3,000 over a bf16 cache) for 2,048 of products and as many of exponentials.  The conversion beside it
 // makes the softmax slower, though its 1.75 instructions an element are not the cost (none of them: the same time): the two
 // share each quarter's queue for shared memory and special functions, and its store of instructions, for which a smaller
 // loop is quicker than one that is unrolled (q8_tile).  2,043 rows in four chunks behind up to 8,192 positions (32/8 heads)
-// 230 us, 770 TFLOP/s; 4,096 rows in six prompts 96 us.
+// 229 to 245 us from one GPU to the next, 720 to 770 TFLOP/s; 4,096 rows in six prompts 96 to 98 us; 16 rows behind 8,000 34 us.
 // Measured and left out (us for the chunks, against 241 or what it was at the time): scores read twice in two halves, for
 // smaller code and fewer registers (244 for 229), a quarter of the exponentials by
 // polynomial (275, an eighth 258), eight warps converting (410 for 240: registers), items of 32 rows less with a ring of four

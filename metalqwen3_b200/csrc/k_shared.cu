@@ -20,7 +20,7 @@
 // (over Q8_0 to f16, k_prompt_q8.cu).
 //
 // Measured: 64 sequences behind 16,384 bf16 positions, 512 of their own (32/8 heads) 56 to 60 us, 150 in three groups behind
-// 12,001 Q8_0 ones, up to 1,024 of their own (40/8) 133 to 136 us, five behind 700 (16/8) 16 us.  Bound by the steps of the
+// 12,001 Q8_0 ones, up to 1,024 of their own (40/8) 133 to 136 us, five behind 700 (16/8) 16 to 17 us.  Bound by the steps of the
 // tensor-core kernel (some 3,600 cycles a key tile for 2,048 of products, over Q8_0 4,200, or 3,800 where a group is one row
 // tile), then by the bytes of the own positions (69 and 178 MB in 20 and 49 us), then by latency: set-up some 10 us, the join
 // 8.  With the plan made beside the products of the second launch, each CTA searching the groups for itself and the tails
