@@ -336,7 +336,8 @@ typedef struct {
  * with fewer positions than are shared, or alone in its group, attends to its
  * own pages as if it were in none; a len beyond the table sets
  * Q3CU_DEV_BAD_INDEX and is cut.  A NaN or infinity at a shared position, where
- * the formula makes an infinity of it, may make a NaN.  q and out are bf16, the
+ * the formula makes an infinity of it, may make a NaN; over a Q8_0 cache, values
+ * more than 2^120 times those before may take these to 0.  q and out are bf16, the
  * cache bf16 or Q8_0; work: 32-byte aligned, q3cu_attention_shared_workspace
  * bytes for the batch's n_seqs (or more), used by one call at a time.  All else
  * as above. */
@@ -367,7 +368,8 @@ q3cu_status q3cu_attention_shared_workspace(q3cu_ctx *ctx, int n_seqs, int n_hea
  * left then stays NaN and Q3CU_DEV_TIMEOUT is set).  Over a Q8_0 cache that is
  * also done for a row behind which, among the 128 positions from a multiple of
  * 128 on where its last one lies, a scale is more than 2^24 times the largest
- * that it sees of them; what is left there keeps a result of fewer bits.  Sequences with one row are
+ * that it sees of them, and for one that sees values more than 2^120 times those
+ * before; what is left there keeps a result of fewer bits.  Sequences with one row are
  * allowed, but q3cu_attention_paged is made for them. */
 q3cu_status q3cu_attention_prompt(q3cu_ctx *ctx, const q3cu_kv_cache *cache, const q3cu_kv_batch *batch,
                                   int64_t rows, const void *q, q3cu_dtype dtype, int64_t q_stride, int n_heads,

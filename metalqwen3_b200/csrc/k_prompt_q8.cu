@@ -17,6 +17,7 @@
 // maximum), a tile of values up to 2^8 smaller has its probabilities lowered, and one of still smaller ones takes O up, as far
 // as binary32 goes: what does not fit then is 2^-100 of the row's result.  (Kept times the smallest lift so far, a row lost
 // values 2^33 smaller than any before them, though those had no weight.)  A tile that the row does not see leaves O as it is.
+// (Where O would go down by more than 2^120 at once, which binary32 may not hold, the row is computed again from the formula.)
 // Where the scales of one tile differ by more than 2^24, rows that see only a part of the tile look at the scales again: one that
 // has a scale more than 2^24 times the largest it sees behind it in the tile is computed again from the formula, so that a
 // later position takes no bits from an earlier row (larger_behind; some 0.2 us a key, a look alone a microsecond).

@@ -28,6 +28,7 @@ constexpr uint32_t PT_IDESC = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(128
 constexpr uint32_t PT_IDESC_V = PT_IDESC | (1u << 16);
 constexpr uint32_t PT_F16 = (1u << 7) | (1u << 10);          // the bits that say bf16 where f16 has none
 constexpr int PT_BIAS = 7;                                   // Q8_0: probabilities are times 2^7 in f16, at most 2^15
+constexpr int PT_DEEP = 120;                                 // Q8_0: O lowered by more may leave binary32
 constexpr int PT_SLACK = 8;                                  // Q8_0: the most by which values' probabilities are lowered (2^-8)
 constexpr float PT_LOG2 = ATT_SCALE * 1.44269504088896341f;  // scores to base-2 exponents
 constexpr float PT_LAZY = 8.0f / PT_LOG2;                    // growth of the maximum (as a raw score) that rescales O
@@ -216,7 +217,8 @@ template <bool COMPARE> __device__ __forceinline__ TileLift q8_lift(const uint8_
     return {min(141 - top_e, 126), low < 0xfeffffffu && top_e - low_e > 24};
 }
 // Whether a row that sees the first n keys of a sequence lost bits to others: behind them in the same tile lies a scale that
-// is more than 2^24 times the largest it sees there, of keys or of values (one warp; every lane returns it).
+// is more than 2^24 times the largest it sees there, of keys or of values (one warp; every lane returns it).  Where it sees
+// none but zeros there, nothing of the tile can be lost.
 __device__ __forceinline__ bool larger_behind(const PagedKV &c, const PagedSeqs &b, int s, int head, int n, int len) {
     const int tile = n / PT_KEYS * PT_KEYS, t = tile + 4 * (threadIdx.x & 31), end = min(len, tile + PT_KEYS);
     uint32_t seen[2] = {0, 0}, hidden[2] = {0, 0};           // of K and V; magnitudes compare as their bits do
@@ -384,7 +386,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
     const int qt = PT_ROWS / group;                          // queries of a tile
     float2 stat = make_float2(-INFINITY, -1.0f);             // SPLIT: maximum and sum of this thread's row, -1: given up
     [[maybe_unused]] float part_back = 1.0f;                 // and what its O is to be multiplied by (Q8_0),
-    [[maybe_unused]] bool part_redo = false;                 // and whether a tile of the part is uneven
+    [[maybe_unused]] int part_redo = 0;                      // and whether the part lost bits
     // the item of a round, copied from its announcement; false after the last, or if a wait gave up
     auto next_item = [&](int round, Round &it, bool whole_warp) -> bool {
         bool ok = mbar_wait(&item_full[round & 1], uint32_t(round >> 1) & 1u, !whole_warp || lane == 0 ? status : nullptr);
@@ -741,7 +743,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
             // Q8_0: S is q . k times 1 / (row's and tile's inverse lifts), O is times 2^lift
             [[maybe_unused]] float row_back = 0.0f;
             [[maybe_unused]] int lifted = 0;
-            [[maybe_unused]] bool redo = false;              // the tile that the row sees in part is uneven
+            [[maybe_unused]] int redo = 0;                   // 1: the tile that the row sees in part is uneven, 2: O went down too far
             const int nkv = max(it.nt[0], it.nt[1]);
             for (int j = 0; j < nt; ++j, ++steps) {
                 ok = __all_sync(FULL, mbar_wait(&s_full[t], steps & 1u, lane == 0 ? status : nullptr));
@@ -775,13 +777,14 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                     const float back = fmaxf(row_back * k_back[n & 1], 0x1p-120f);
                     e = v_lift[n & 1];
                     const int tile = (it.from() + j) * PT_KEYS;
-                    redo |= !SHARED && rough[n & 1] && limit > tile && limit < min(it.len, tile + PT_KEYS);
+                    if (!SHARED && rough[n & 1] && limit > tile && limit < min(it.len, tile + PT_KEYS)) redo = max(redo, 1);
                     tile_max *= back;
                     unit *= back;
                     if (j == 0) lifted = e;
                     // larger values than before: O goes down; much smaller ones: up again; a tile that the row does not see
                     // changes nothing
                     if ((e < lifted || e > lifted + PT_SLACK) && (SHARED || limit > tile)) change = e - lifted;
+                    if (!SHARED && change < -PT_DEEP) redo = 2;
                 }
                 const bool grow = tile_max > m + PT_LAZY || (m == -INFINITY && tile_max > m);
                 if (__any_sync(FULL, grow || change != 0)) {
@@ -959,7 +962,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                 }
                 // rows that came out as no numbers, and such as lost bits to positions that they do not see, once more from
                 // the formula (over what is stored, which stays where time is up)
-                unsigned again = __ballot_sync(FULL, live && limit > 0 && (nan || (Q8 && redo)));
+                unsigned again = __ballot_sync(FULL, live && limit > 0 && (nan || (Q8 && redo > 0)));
                 SecondLook<Cached> second;
                 const uint64_t began = again ? global_ns() : 0;
                 while (again) {
@@ -973,13 +976,14 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                     const int il = __shfl_sync(FULL, i, l), n = __shfl_sync(FULL, limit, l);
                     const int h = it.head * group + __shfl_sync(FULL, r_head, l);
                     float4 x = load_quad(q + int64_t(it.base + il) * q_stride + int64_t(h) * HD + 4 * lane);
-                    bool want = false;
-                    if (__shfl_sync(FULL, int(nan), l)) {
+                    const int lost = Q8 ? __shfl_sync(FULL, redo, l) : 0;
+                    bool want = lost == 2;
+                    if (!want && __shfl_sync(FULL, int(nan), l)) {
                         second.look(t, c, b, it.s, it.head, it.seen(it.first + t * qt), min(it.len, it.nt[t] * PT_KEYS));
                         want = second.wanted(n, x);
                     }
                     if constexpr (Q8)
-                        if (!want && __shfl_sync(FULL, int(redo), l)) want = larger_behind(c, b, it.s, it.head, n, it.len);
+                        if (!want && lost) want = larger_behind(c, b, it.s, it.head, n, it.len);
                     if (!want) continue;
                     x = make_float4(x.x * ATT_SCALE, x.y * ATT_SCALE, x.z * ATT_SCALE, x.w * ATT_SCALE);
                     store_quad(out + (int64_t(it.base + il) * n_heads + h) * HD + 4 * lane,
@@ -1035,23 +1039,23 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant_
                 if (!ok) continue;
                 if (limit <= 0) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 const bool nan = __any_sync(FULL, !all_finite(v));
-                bool uneven = false;
+                uint32_t lost = 0;
                 if constexpr (Q8) {
                     uint32_t mark = 0;
                     if (lane < it.parts)
                         asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(mark) : "r"(peer_smem(smem_addr(marks + r), lane)) : "memory");
-                    uneven = __any_sync(FULL, mark != 0);
+                    lost = __reduce_max_sync(FULL, mark);
                 }
-                if (limit > 0 && (nan || uneven)) {
+                if (limit > 0 && (nan || lost)) {
                     const float4 x = load_quad(q + int64_t(it.base + i) * q_stride + int64_t(head) * HD + 4 * lane);
-                    bool want = false;
-                    if (nan) {
+                    bool want = lost == 2;
+                    if (!want && nan) {
                         const int first = it.first + (r >> 7) * qt, seen = it.seen(min(first + qt, it.rows) - 1);
                         second.look(r >> 7, c, b, it.s, it.head, it.seen(first), min(it.len, (seen + PT_KEYS - 1) / PT_KEYS * PT_KEYS));
                         want = second.wanted(limit, x);
                     }
                     if constexpr (Q8)
-                        if (!want && uneven) want = larger_behind(c, b, it.s, it.head, limit, it.len);
+                        if (!want && lost) want = larger_behind(c, b, it.s, it.head, limit, it.len);
                     if (want)
                         v = attend_row<Cached, 4>(c, b, it.s, it.head, limit,
                                                 make_float4(x.x * ATT_SCALE, x.y * ATT_SCALE, x.z * ATT_SCALE, x.w * ATT_SCALE),

@@ -169,3 +169,33 @@ def test_one_token_far_from_1(q3, io, size_q, size_kv):
                 k, v = elements(s)
                 check_attention(x[s:s + 1], q[s:s + 1], k, v, [300], io, W if io == BF16 else 0.0, 2.0 ** -32 if len(got) > 1 else 2.0 ** -39)
     assert q3.device_status() == 0
+
+
+@pytest.mark.parametrize("n,rows", [(300, 300), (300, 60), (2000, 1800), (2000, 90)])
+def test_sizes_from_end_to_end(q3, n, rows):
+    """Values 2^130 times larger, in one case behind zeros in the tile that a row sees in part, in the other seen but without
+    weight: what is lowered for them does not go under."""
+    big = n // 128 * 128
+    for light in (False, True):
+        p = Quantised([n], 2, 16, seed=95).fill(96, 2.0 ** -60)
+        page, slot = p.where(0, range(n))
+        p.k[page, :, slot, 0] = 0
+        at = list(range(big, big + 1)) if light else list(range(big + 1, n))
+        if not light:
+            p.vs[page[big], :, slot[big]] = 0
+        for _ in range(2):
+            p.vs[page[at], :, slot[at]] *= 2.0 ** 65
+        p.ks[page, :, slot] *= 2.0 ** 60
+        if light:
+            p.k[page[at], :, slot[at], :64] = 0
+            p.k[page[at], :, slot[at], 0] = -127
+            p.ks[page[at], :, slot[at], 0] = 60.0 / 127
+        q = light_queries(rows, 8, 98)
+        got = q3.attention_prompt(*p.handles([0, rows]), q)
+        k, v = rounded(p, 0)
+        pick = [i for i in range(rows) if (i >= rows - n + big) == light][:: 1 + rows // 64]
+        if not light:
+            pick.append(rows - n + big)                 # (the one that sees the zeros)
+        check(got[pick], q[pick], k[:big + 1] if not light else k, v[:big + 1] if not light else v,
+              [n - rows + i + 1 for i in pick], at if light else ())
+    assert q3.device_status() == 0
